@@ -70,11 +70,27 @@ SIGNATURES = {
     "ethos_expert_forward": (ctypes.c_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp,
                                             _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _sz, _vp, _vp,
                                             _vp]),
+    "ethos_linear_ce_state_bytes": (_sz, [_i64, _i32, _i32]),
+    "ethos_linear_ce_workspace_bytes": (_sz, [_i64, _i32, _i64, _i32]),
+    "ethos_linear_ce": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i32, _i64, _i64, _i32, _i32, _vp, _sz, _vp, _sz, _vp, _vp]),
+    "ethos_linear_ce_grad_workspace_bytes": (_sz, [_i64, _i32, _i64, _i32]),
+    "ethos_linear_ce_grad": (ctypes.c_int, [_vp, _sz, _vp, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _sz, _vp, _vp, _vp]),
+    "ethos_embedding": (ctypes.c_int, [_vp, _i32, _vp, _i64, _i32, _i64, _f32, _i32, _vp, _vp]),
+    "ethos_embedding_grad_workspace_bytes": (_sz, [_i64, _i32, _i64]),
+    "ethos_embedding_grad": (ctypes.c_int, [_vp, _i32, _vp, _i64, _i32, _i64, _f32, _i64, _i32, _vp, _sz, _vp, _vp]),
+    "ethos_balance_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "ethos_balance": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, _i32, _i64, _i32, _vp, _sz, _vp, _vp, _vp]),
+    "ethos_balance_grad": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i64, _i32, _i32, _i64, _i32, _vp, _vp]),
+    "ethos_clip_grads_workspace_bytes": (_sz, [_vp, _i32]),
+    "ethos_clip_grads": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _f64, _vp, _sz, _vp, _vp]),
     "ethos_token_proj": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp]),
     "ethos_apply_hidden_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32]),
     "ethos_apply_hidden": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32,
                                           _vp, _sz, _vp, _vp]),
 }
+
+# ethos_linear_ce's reductions (ETHOS_LOSS_* in the header)
+REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 # ethos_sort_segment_noalloc's limit (ETHOS_NOALLOC_MAX_PAIRS in the header)
 NOALLOC_MAX_PAIRS = 1 << 20

@@ -11,6 +11,7 @@
 #include "../../include/ethos_hip.h"
 #include "ethos_common.hpp"
 #include "ethos_launch.hpp"
+#include "ethos_train.hpp"
 
 namespace {
 
@@ -921,6 +922,196 @@ int ethos_layer_forward(const void* x, const void* wq, const void* wq_prepared, 
     return ethos_expert_forward(x, latents, n_experts, w1, w2, wut, xp, uniq, seg_off, n_unique, l.max_u, perm, sorted_slot,
                                 pair_slot, gates, n_tok, n_heads, top_k, d_latent, d_hidden, d_model, dtype, order, w + l.ews,
                                 l.ews_bytes, w + l.h, out, stream);
+}
+
+namespace {
+
+constexpr int64_t kMaxItems = (int64_t)1 << 30;
+
+// Sizes of the loss over the vocabulary.
+int ce_sizes(int64_t n, int32_t d, int64_t vocab, int32_t reduction, int32_t dtype, const char* what) {
+    if (!dtype_ok(dtype)) return fail(ETHOS_EDTYPE, "%s: unknown dtype %d", what, dtype);
+    if (n < 0 || n > kMaxItems || d <= 0 || vocab <= 0 || vocab > kMaxItems || reduction < 0 || reduction > 2)
+        return fail(ETHOS_ESIZE, "%s: bad sizes n_tok=%lld d=%d vocab=%lld reduction=%d", what, (long long)n, d, (long long)vocab,
+                    reduction);
+    if (d % 8 || d > 32768) return fail(ETHOS_EUNSUPPORTED, "%s: d must be a multiple of 8, at most 32768 (got %d)", what, d);
+    return 0;
+}
+
+}  // namespace
+
+size_t ethos_linear_ce_state_bytes(int64_t n_tok, int32_t d, int32_t dtype) {
+    if (n_tok <= 0 || n_tok > kMaxItems || d <= 0 || !dtype_ok(dtype)) return 256;
+    return ethos::linear_ce_state_bytes(n_tok, d, dtype);
+}
+
+size_t ethos_linear_ce_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype) {
+    if (n_tok <= 0 || n_tok > kMaxItems || d <= 0 || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
+    return ethos::linear_ce_workspace_bytes(n_tok, d, vocab, dtype);
+}
+
+int ethos_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* labels, int64_t n_tok, int32_t d, int64_t vocab,
+                    int64_t ignore_index, int32_t reduction, int32_t dtype, void* state, size_t state_bytes, void* workspace,
+                    size_t workspace_bytes, float* loss, void* stream) {
+    g_err[0] = 0;
+    if (const int rc = ce_sizes(n_tok, d, vocab, reduction, dtype, "ethos_linear_ce")) return rc;
+    const int vec = dtype == ETHOS_BF16 ? 8 : 4;
+    if (ldh < d) return fail(ETHOS_ESIZE, "ethos_linear_ce: ldh %lld below d", (long long)ldh);
+    if (ldh % vec) return fail(ETHOS_EUNSUPPORTED, "ethos_linear_ce: ldh must be a multiple of %d", vec);
+    if (n_tok == 0) return 0;
+    if (!h || !w || !labels || !state || !workspace || !loss) return fail(ETHOS_ENULL, "ethos_linear_ce: null pointer");
+    if (state_bytes < ethos::linear_ce_state_bytes(n_tok, d, dtype) ||
+        workspace_bytes < ethos::linear_ce_workspace_bytes(n_tok, d, vocab, dtype))
+        return fail(ETHOS_EWORKSPACE, "ethos_linear_ce: state of %zu or workspace of %zu bytes too small", state_bytes, workspace_bytes);
+    if (!aligned16(h) || !aligned16(w) || !aligned16(state) || !aligned16(workspace))
+        return fail(ETHOS_EALIGN, "ethos_linear_ce: h, w, state and workspace must be 16-byte aligned");
+    return hip_status(ethos::launch_linear_ce(h, ldh, w, labels, n_tok, d, vocab, ignore_index, reduction, dtype, state, workspace, loss,
+                                              num_cus(), (hipStream_t)stream),
+                      "ethos_linear_ce");
+}
+
+size_t ethos_linear_ce_grad_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype) {
+    if (n_tok <= 0 || n_tok > kMaxItems || d <= 0 || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
+    return ethos::linear_ce_grad_workspace_bytes(n_tok, d, vocab, dtype, num_cus());
+}
+
+int ethos_linear_ce_grad(const void* state, size_t state_bytes, const void* w, const float* dloss, int64_t n_tok, int32_t d,
+                         int64_t vocab, int32_t reduction, int32_t dtype, void* workspace, size_t workspace_bytes, void* dh, void* dw,
+                         void* stream) {
+    g_err[0] = 0;
+    if (const int rc = ce_sizes(n_tok, d, vocab, reduction, dtype, "ethos_linear_ce_grad")) return rc;
+    if (n_tok == 0 || (!dh && !dw)) return 0;
+    if (!state || !w || !dloss || !workspace) return fail(ETHOS_ENULL, "ethos_linear_ce_grad: null pointer");
+    if (state_bytes < ethos::linear_ce_state_bytes(n_tok, d, dtype) ||
+        workspace_bytes < ethos::linear_ce_grad_workspace_bytes(n_tok, d, vocab, dtype, num_cus()))
+        return fail(ETHOS_EWORKSPACE, "ethos_linear_ce_grad: state of %zu or workspace of %zu bytes too small", state_bytes,
+                    workspace_bytes);
+    if (!aligned16(state) || !aligned16(w) || !aligned16(workspace) || !aligned16(dh) || !aligned16(dw))
+        return fail(ETHOS_EALIGN, "ethos_linear_ce_grad: state, w, workspace, dh and dw must be 16-byte aligned");
+    return hip_status(ethos::launch_linear_ce_grad(state, w, dloss, n_tok, d, vocab, reduction, dtype, workspace, dh, dw, num_cus(),
+                                                   (hipStream_t)stream),
+                      "ethos_linear_ce_grad");
+}
+
+namespace {
+
+int embed_sizes(int64_t n, int32_t d, int64_t vocab, int32_t dtype, const char* what) {
+    if (!dtype_ok(dtype)) return fail(ETHOS_EDTYPE, "%s: unknown dtype %d", what, dtype);
+    if (n < 0 || d <= 0 || vocab <= 0 || n >= INT32_MAX || d >= INT32_MAX || vocab >= INT32_MAX)
+        return fail(ETHOS_ESIZE, "%s: bad sizes n=%lld d=%d vocab=%lld", what, (long long)n, d, (long long)vocab);
+    return 0;
+}
+bool aligned_to(const void* p, int32_t dtype) { return ((uintptr_t)p & (dtype == ETHOS_BF16 ? 1u : 3u)) == 0; }
+
+}  // namespace
+
+int ethos_embedding(const void* ids, int32_t ids_64, const void* w, int64_t n, int32_t d, int64_t vocab, float scale, int32_t dtype,
+                    void* out, void* stream) {
+    g_err[0] = 0;
+    if (const int rc = embed_sizes(n, d, vocab, dtype, "ethos_embedding")) return rc;
+    if (n == 0) return 0;
+    if (!ids || !w || !out) return fail(ETHOS_ENULL, "ethos_embedding: null pointer");
+    if (!aligned_to(w, dtype) || !aligned_to(out, dtype)) return fail(ETHOS_EALIGN, "ethos_embedding: w or out misaligned");
+    return hip_status(ethos::launch_embedding(ids, ids_64, w, n, d, vocab, scale, dtype, out, num_cus(), (hipStream_t)stream),
+                      "ethos_embedding");
+}
+
+size_t ethos_embedding_grad_workspace_bytes(int64_t n, int32_t d, int64_t vocab) {
+    if (n <= 0 || d <= 0 || vocab <= 0 || n >= INT32_MAX || vocab >= INT32_MAX) return 256;
+    return ethos::embedding_grad_workspace_bytes(n, d, vocab);
+}
+
+int ethos_embedding_grad(const void* ids, int32_t ids_64, const void* dy, int64_t n, int32_t d, int64_t vocab, float scale,
+                         int64_t padding, int32_t dtype, void* workspace, size_t workspace_bytes, void* dw, void* stream) {
+    g_err[0] = 0;
+    if (const int rc = embed_sizes(n, d, vocab, dtype, "ethos_embedding_grad")) return rc;
+    if (!dw || !workspace || (n > 0 && (!ids || !dy))) return fail(ETHOS_ENULL, "ethos_embedding_grad: null pointer");
+    if (workspace_bytes < ethos::embedding_grad_workspace_bytes(n, d, vocab))
+        return fail(ETHOS_EWORKSPACE, "ethos_embedding_grad: workspace of %zu bytes, %zu needed", workspace_bytes,
+                    ethos::embedding_grad_workspace_bytes(n, d, vocab));
+    if (!aligned16(dy) || !aligned16(dw) || !aligned16(workspace))
+        return fail(ETHOS_EALIGN, "ethos_embedding_grad: dy, dw and workspace must be 16-byte aligned");
+    return hip_status(ethos::launch_embedding_grad(ids, ids_64, dy, n, d, vocab, scale, padding, dtype, workspace, dw, num_cus(),
+                                                   (hipStream_t)stream),
+                      "ethos_embedding_grad");
+}
+
+namespace {
+
+int balance_sizes(int64_t n, int32_t heads, int32_t k, int64_t n_experts, int32_t dtype, const char* what) {
+    if (!dtype_ok(dtype)) return fail(ETHOS_EDTYPE, "%s: unknown dtype %d", what, dtype);
+    if (n < 0 || heads <= 0 || k <= 0 || n_experts <= 0 || n_experts > INT32_MAX || n > INT32_MAX || (int64_t)heads * k > INT32_MAX ||
+        n * heads > INT32_MAX || n * heads * k > INT32_MAX)
+        return fail(ETHOS_ESIZE, "%s: bad sizes n_tok=%lld n_heads=%d top_k=%d n_experts=%lld", what, (long long)n, heads, k,
+                    (long long)n_experts);
+    return 0;
+}
+double balance_scale(int64_t n, int32_t heads, int32_t k, int64_t n_experts) {
+    const double rows = (double)n * heads;
+    return n > 0 ? (double)n_experts / (rows * k * rows) : 0.0;
+}
+
+}  // namespace
+
+size_t ethos_balance_workspace_bytes(int64_t n_tok, int32_t n_heads, int32_t top_k) {
+    return ethos::balance_workspace_bytes(n_tok > 0 && n_heads > 0 && top_k > 0 ? n_tok * n_heads * top_k : 1);
+}
+
+int ethos_balance(const void* gates, const void* ids, int32_t ids_64, int64_t n_tok, int32_t n_heads, int32_t top_k, int64_t n_experts,
+                  int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* counts, float* loss, void* stream) {
+    g_err[0] = 0;
+    if (const int rc = balance_sizes(n_tok, n_heads, top_k, n_experts, dtype, "ethos_balance")) return rc;
+    const int64_t pairs = n_tok * n_heads * top_k;
+    if (!counts || !loss || !workspace || (pairs > 0 && (!gates || !ids))) return fail(ETHOS_ENULL, "ethos_balance: null pointer");
+    if (workspace_bytes < ethos::balance_workspace_bytes(pairs))
+        return fail(ETHOS_EWORKSPACE, "ethos_balance: workspace of %zu bytes, %zu needed", workspace_bytes,
+                    ethos::balance_workspace_bytes(pairs));
+    if (!aligned16(workspace) || !aligned_to(gates, dtype)) return fail(ETHOS_EALIGN, "ethos_balance: workspace or gates misaligned");
+    return hip_status(ethos::launch_balance(gates, ids, ids_64, pairs, n_experts, balance_scale(n_tok, n_heads, top_k, n_experts), dtype,
+                                            workspace, counts, loss, num_cus(), (hipStream_t)stream),
+                      "ethos_balance");
+}
+
+int ethos_balance_grad(const void* ids, int32_t ids_64, const int32_t* counts, const float* dloss, int64_t n_tok, int32_t n_heads,
+                       int32_t top_k, int64_t n_experts, int32_t dtype, void* dgates, void* stream) {
+    g_err[0] = 0;
+    if (const int rc = balance_sizes(n_tok, n_heads, top_k, n_experts, dtype, "ethos_balance_grad")) return rc;
+    const int64_t pairs = n_tok * n_heads * top_k;
+    if (pairs == 0) return 0;
+    if (!ids || !counts || !dloss || !dgates) return fail(ETHOS_ENULL, "ethos_balance_grad: null pointer");
+    if (!aligned_to(dgates, dtype)) return fail(ETHOS_EALIGN, "ethos_balance_grad: dgates misaligned");
+    return hip_status(ethos::launch_balance_grad(ids, ids_64, counts, dloss, pairs, n_experts,
+                                                 balance_scale(n_tok, n_heads, top_k, n_experts), dtype, dgates, num_cus(),
+                                                 (hipStream_t)stream),
+                      "ethos_balance_grad");
+}
+
+size_t ethos_clip_grads_workspace_bytes(const int64_t* sizes, int32_t n_tensors) {
+    if (!sizes || n_tensors <= 0) return 256;
+    return ethos::clip_workspace_bytes(sizes, n_tensors);
+}
+
+int ethos_clip_grads(const void* const* in, void* const* out, const int64_t* sizes, const int32_t* dtypes, int32_t n_tensors,
+                     int32_t inf_norm, double max_norm, void* workspace, size_t workspace_bytes, float* total, void* stream) {
+    g_err[0] = 0;
+    if (n_tensors < 0) return fail(ETHOS_ESIZE, "ethos_clip_grads: n_tensors %d", n_tensors);
+    if (!total || !workspace || (n_tensors > 0 && (!in || !out || !sizes || !dtypes)))
+        return fail(ETHOS_ENULL, "ethos_clip_grads: null pointer");
+    int64_t all = 0;
+    for (int i = 0; i < n_tensors; ++i) {
+        if (!dtype_ok(dtypes[i])) return fail(ETHOS_EDTYPE, "ethos_clip_grads: unknown dtype %d of tensor %d", dtypes[i], i);
+        if (sizes[i] < 0 || sizes[i] > ((int64_t)1 << 40) || (all += sizes[i]) > ((int64_t)1 << 44))
+            return fail(ETHOS_ESIZE, "ethos_clip_grads: size %lld of tensor %d", (long long)sizes[i], i);
+        if (sizes[i] > 0 && (!in[i] || !out[i])) return fail(ETHOS_ENULL, "ethos_clip_grads: null pointer of tensor %d", i);
+        if (!aligned_to(in[i], dtypes[i]) || !aligned_to(out[i], dtypes[i]))
+            return fail(ETHOS_EALIGN, "ethos_clip_grads: tensor %d misaligned", i);
+    }
+    const size_t need = ethos::clip_workspace_bytes(sizes, n_tensors);
+    if (workspace_bytes < need)
+        return fail(ETHOS_EWORKSPACE, "ethos_clip_grads: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (!aligned16(workspace)) return fail(ETHOS_EALIGN, "ethos_clip_grads: workspace must be 16-byte aligned");
+    return hip_status(ethos::launch_clip(in, out, sizes, dtypes, n_tensors, inf_norm, max_norm, workspace, total, (hipStream_t)stream),
+                      "ethos_clip_grads");
 }
 
 }  // extern "C"

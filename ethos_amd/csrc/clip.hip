@@ -1,0 +1,194 @@
+// Global gradient norm over many tensors, and clipping:
+//   total = (sum over every tensor's values of g^2)^(1/2), or max |g|;
+//   out = RN_T(g min(1, max_norm / (total + 1e-6))).
+// Two passes over the gradients with one workgroup per piece of kPiece values: the squares' sums
+// (float64: no gradient's square overflows or vanishes there) in a fixed order, one small kernel
+// for the norm and the factor, then the scaled copy.  The tensors' addresses travel as kernel
+// arguments, kPerLaunch tensors to a launch.
+#include "ethos_common.hpp"
+#include "ethos_rows.hpp"
+#include "ethos_train.hpp"
+
+namespace ethos {
+namespace {
+
+constexpr int64_t kPiece = 32768;
+constexpr int kPerLaunch = 128;  // 28 bytes each of the 4 KiB of a launch's arguments
+
+struct ClipList {
+    const void* in[kPerLaunch];
+    void* out[kPerLaunch];
+    int64_t size[kPerLaunch];   // values, negative (~size) for float32
+    int32_t first[kPerLaunch];  // first piece of the tensor in this launch
+    int32_t count;
+    int32_t pieces;  // of this launch
+    int32_t base;    // pieces before this launch
+};
+static_assert(sizeof(ClipList) + 64 <= 4096, "kernel arguments");
+
+// The tensor that holds piece b: the last one whose first piece is not past it.
+__device__ __forceinline__ int clip_find(const ClipList& l, int b) {
+    int lo = 0, hi = l.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (l.first[mid] <= b) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <typename T, typename F>
+__device__ __forceinline__ void clip_values(const T* p, int64_t n, F f) {
+    constexpr int N = Vec16<T>::kN;
+    if (((uintptr_t)p & 15u) == 0) {
+        const int64_t whole = n / N;
+        for (int64_t i = threadIdx.x; i < whole; i += 256) {
+            float v[N];
+            Vec16<T>::unpack(reinterpret_cast<const typename Vec16<T>::raw*>(p)[i], v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) f(v[j]);
+        }
+        for (int64_t i = whole * N + threadIdx.x; i < n; i += 256) f(Elem<T>::to_f32(p[i]));
+    } else {
+        for (int64_t i = threadIdx.x; i < n; i += 256) f(Elem<T>::to_f32(p[i]));
+    }
+}
+
+// Larger of two magnitudes, NaN if one is.
+__device__ __forceinline__ double nan_max(double a, double b) { return a != a ? a : b != b ? b : a > b ? a : b; }
+
+template <bool INF>
+__device__ __forceinline__ double clip_join(double a, double b) {
+    return INF ? nan_max(a, b) : a + b;
+}
+
+template <bool INF>
+__device__ __forceinline__ double clip_reduce(double v, double* lds) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = clip_join<INF>(v, __shfl_xor(v, o));
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = lds[0];
+    for (int i = 1; i < (int)(blockDim.x >> 6); ++i) s = clip_join<INF>(s, lds[i]);
+    return s;
+}
+
+template <bool INF>
+__global__ __launch_bounds__(256) void clip_norm_kernel(ClipList l, double* __restrict__ part) {
+    __shared__ double lds[4];
+    const int t = clip_find(l, blockIdx.x);
+    const int64_t at = (int64_t)((int)blockIdx.x - l.first[t]) * kPiece;
+    const bool f32 = l.size[t] < 0;
+    const int64_t size = f32 ? ~l.size[t] : l.size[t];
+    const int64_t n = size - at < kPiece ? size - at : kPiece;
+    double s = 0.0;
+    auto add = [&](float v) { s = INF ? nan_max(s, fabs((double)v)) : __builtin_fma((double)v, (double)v, s); };
+    if (f32) clip_values((const float*)l.in[t] + at, n, add);
+    else clip_values((const uint16_t*)l.in[t] + at, n, add);
+    s = clip_reduce<INF>(s, lds);
+    if (threadIdx.x == 0) part[l.base + blockIdx.x] = s;
+}
+
+template <bool INF>
+__global__ __launch_bounds__(1024) void clip_total_kernel(const double* __restrict__ part, int64_t n, double max_norm,
+                                                          float* __restrict__ total, float* __restrict__ factor) {
+    __shared__ double lds[16];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s = clip_join<INF>(s, part[i]);
+    s = clip_reduce<INF>(s, lds);
+    if (threadIdx.x == 0) {
+        const double norm = INF ? s : sqrt(s);
+        *total = (float)norm;
+        const double k = max_norm / (norm + 1e-6);
+        *factor = k < 1.0 ? (float)k : k != k ? (float)k : 1.0f;
+    }
+}
+
+template <typename T, typename W>
+__device__ __forceinline__ void clip_scale(const T* in, T* out, int64_t n, float k) {
+    constexpr int N = sizeof(W) / sizeof(T);
+    const int64_t whole = n / N;
+    for (int64_t i = threadIdx.x; i < whole; i += 256) {
+        union {
+            W w;
+            T t[N];
+        } v;
+        v.w = reinterpret_cast<const W*>(in)[i];
+#pragma unroll
+        for (int j = 0; j < N; ++j) v.t[j] = Elem<T>::from_f32(Elem<T>::to_f32(v.t[j]) * k);
+        reinterpret_cast<W*>(out)[i] = v.w;
+    }
+    for (int64_t i = whole * N + threadIdx.x; i < n; i += 256) out[i] = Elem<T>::from_f32(Elem<T>::to_f32(in[i]) * k);
+}
+
+template <typename T>
+__device__ __forceinline__ void clip_piece(const T* in, T* out, int64_t n, float k) {
+    const uintptr_t a = (uintptr_t)in | (uintptr_t)out;
+    if ((a & 15u) == 0) clip_scale<T, uint4>(in, out, n, k);
+    else if ((a & 3u) == 0) clip_scale<T, uint32_t>(in, out, n, k);
+    else clip_scale<T, T>(in, out, n, k);
+}
+
+__global__ __launch_bounds__(256) void clip_scale_kernel(ClipList l, const float* __restrict__ factor) {
+    const int b = l.pieces - 1 - (int)blockIdx.x;
+    const int t = clip_find(l, b);
+    const float k = *factor;
+    if (k == 1.0f && l.in[t] == l.out[t]) return;
+    const int64_t at = (int64_t)(b - l.first[t]) * kPiece;
+    const bool f32 = l.size[t] < 0;
+    const int64_t size = f32 ? ~l.size[t] : l.size[t];
+    const int64_t n = size - at < kPiece ? size - at : kPiece;
+    if (f32) clip_piece((const float*)l.in[t] + at, (float*)l.out[t] + at, n, k);
+    else clip_piece((const uint16_t*)l.in[t] + at, (uint16_t*)l.out[t] + at, n, k);
+}
+
+int64_t clip_pieces(int64_t size) { return (size + kPiece - 1) / kPiece; }
+
+}  // namespace
+
+size_t clip_workspace_bytes(const int64_t* sizes, int n_tensors) {
+    int64_t p = 0;
+    for (int i = 0; i < n_tensors; ++i) p += clip_pieces(sizes[i]);
+    return (size_t)p * sizeof(double) + 256;
+}
+
+int launch_clip(const void* const* in, void* const* out, const int64_t* sizes, const int32_t* dtypes, int n_tensors, int inf_norm,
+                double max_norm, void* ws, float* total, hipStream_t stream) {
+    float* factor = (float*)ws;
+    double* part = (double*)((char*)ws + 256);
+    int64_t base = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        base = 0;
+        ClipList l;
+        l.count = 0;
+        l.pieces = 0;
+        l.base = 0;
+        for (int i = 0; i <= n_tensors; ++i) {
+            if (l.count == kPerLaunch || (i == n_tensors && l.count > 0)) {
+                if (pass == 1) hipLaunchKernelGGL(clip_scale_kernel, dim3(l.pieces), dim3(256), 0, stream, l, factor);
+                else if (inf_norm) hipLaunchKernelGGL((clip_norm_kernel<true>), dim3(l.pieces), dim3(256), 0, stream, l, part);
+                else hipLaunchKernelGGL((clip_norm_kernel<false>), dim3(l.pieces), dim3(256), 0, stream, l, part);
+                base += l.pieces;
+                l.count = 0;
+                l.pieces = 0;
+                l.base = (int32_t)base;
+            }
+            if (i == n_tensors || sizes[i] == 0) continue;
+            l.in[l.count] = in[i];
+            l.out[l.count] = out[i];
+            l.size[l.count] = dtypes[i] == kF32 ? ~sizes[i] : sizes[i];
+            l.first[l.count] = l.pieces;
+            l.pieces += (int32_t)clip_pieces(sizes[i]);
+            ++l.count;
+        }
+        if (pass == 0) {
+            if (inf_norm)
+                hipLaunchKernelGGL((clip_total_kernel<true>), dim3(1), dim3(1024), 0, stream, part, base, max_norm, total, factor);
+            else
+                hipLaunchKernelGGL((clip_total_kernel<false>), dim3(1), dim3(1024), 0, stream, part, base, max_norm, total, factor);
+        }
+    }
+    return (int)hipGetLastError();
+}
+
+}  // namespace ethos

@@ -4,9 +4,11 @@ tensors and raises on anything else -- there is no CPU path.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
-from ._lib import check, dtype_code, load
+from ._lib import REDUCTIONS, check, dtype_code, load
 
 
 def _stream_slow() -> int:
@@ -49,8 +51,6 @@ def workspace(nbytes: int, device) -> tuple[torch.Tensor, int]:
 def stage_events(events) -> None:
     """Hand the library torch.cuda.Event objects (already recorded once, so that they exist)
     to record, in order, at the stage boundaries of this thread's next calls; [] clears."""
-    import ctypes
-
     handles = [e.cuda_event for e in events]
     if any(h == 0 for h in handles):
         raise RuntimeError("stage_events: record each event once before handing it over")
@@ -445,8 +445,6 @@ def expert_grads(x: torch.Tensor, dy: torch.Tensor, h: torch.Tensor, latents: to
 
 def _pointers(ts):
     """A host array of the tensors' device pointers (None: a null array), for the length of a call."""
-    import ctypes
-
     return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts]) if ts is not None else None
 
 
@@ -654,3 +652,115 @@ def mla_attention(q: torch.Tensor, kv: torch.Tensor, k_rot: torch.Tensor, positi
                                     out.data_ptr(), _stream())
     check(rc, "ethos_mla_attention")
     return out
+
+
+# ----------------------------------------------------------- operators of a training step
+def _need_here(t: torch.Tensor, name: str, dtypes, dim=None) -> None:
+    """_need, with one of several dtypes and on the current device."""
+    _need(t, name, dim=dim)
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+    if t.device.index != _current_device():
+        raise RuntimeError(f"{name} is on {t.device}, not on the current device")
+
+
+FLOATS = (torch.bfloat16, torch.float32)
+INTS = (torch.int32, torch.int64)
+
+
+def linear_ce(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, ignore_index: int, reduction: str):
+    """(loss float32, state): softmax cross entropy of h [n, d] (rows evenly spaced) against w [V, d];
+    the state is what linear_ce_grad takes."""
+    _need_here(w, "weight", FLOATS, 2)
+    _need_here(labels, "labels", (torch.int64,), 1)
+    n, d = h.shape
+    code, lib = dtype_code(h.dtype), load()
+    V = w.shape[0]
+    st, st_bytes = workspace(lib.ethos_linear_ce_state_bytes(n, d, code), h.device)
+    ws, ws_bytes = workspace(lib.ethos_linear_ce_workspace_bytes(n, d, V, code), h.device)
+    loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=h.device)
+    rc = lib.ethos_linear_ce(h.data_ptr(), h.stride(0) if n > 1 else d, w.data_ptr(), labels.data_ptr(), n, d, V, int(ignore_index),
+                             REDUCTIONS[reduction], code, st.data_ptr(), st_bytes, ws.data_ptr(), ws_bytes, loss.data_ptr(), _stream())
+    check(rc, "ethos_linear_ce")
+    return loss, st
+
+
+def linear_ce_grad(state: torch.Tensor, w: torch.Tensor, dloss: torch.Tensor, n: int, reduction: str, want_h: bool, want_w: bool):
+    """(dh [n, d], dw [V, d]) from dloss (float32, contiguous); None for one not wanted."""
+    V, d = w.shape
+    code, lib = dtype_code(w.dtype), load()
+    ws, ws_bytes = workspace(lib.ethos_linear_ce_grad_workspace_bytes(n, d, V, code), w.device)
+    dh = torch.empty((n, d), dtype=w.dtype, device=w.device) if want_h else None
+    dw = torch.empty((V, d), dtype=w.dtype, device=w.device) if want_w else None
+    rc = lib.ethos_linear_ce_grad(state.data_ptr(), state.numel() * 8, w.data_ptr(), dloss.data_ptr(), n, d, V, REDUCTIONS[reduction],
+                                  code, ws.data_ptr(), ws_bytes, dh.data_ptr() if want_h else None,
+                                  dw.data_ptr() if want_w else None, _stream())
+    check(rc, "ethos_linear_ce_grad")
+    return dh, dw
+
+
+def embedding(ids: torch.Tensor, w: torch.Tensor, scale: float) -> torch.Tensor:
+    """Rows scale * w[ids], [*ids.shape, d]."""
+    _need_here(ids, "ids", INTS)
+    _need_here(w, "weight", FLOATS, 2)
+    V, d = w.shape
+    out = torch.empty((*ids.shape, d), dtype=w.dtype, device=w.device)
+    rc = load().ethos_embedding(ids.data_ptr(), int(ids.dtype == torch.int64), w.data_ptr(), ids.numel(), d, V, scale,
+                                dtype_code(w.dtype), out.data_ptr(), _stream())
+    check(rc, "ethos_embedding")
+    return out
+
+
+def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, vocab: int, scale: float, padding: int) -> torch.Tensor:
+    """The table's gradient [vocab, d] from dy [*ids.shape, d]; positions of id `padding` are left out."""
+    _need_here(ids, "ids", INTS)
+    _need_here(dy, "dy", FLOATS)
+    n, d = ids.numel(), dy.shape[-1]
+    lib = load()
+    ws, ws_bytes = workspace(lib.ethos_embedding_grad_workspace_bytes(n, d, vocab), dy.device)
+    dw = torch.empty((vocab, d), dtype=dy.dtype, device=dy.device)
+    rc = lib.ethos_embedding_grad(ids.data_ptr(), int(ids.dtype == torch.int64), dy.data_ptr(), n, d, vocab, scale, padding,
+                                  dtype_code(dy.dtype), ws.data_ptr(), ws_bytes, dw.data_ptr(), _stream())
+    check(rc, "ethos_embedding_grad")
+    return dw
+
+
+def balance(gates: torch.Tensor, ids: torch.Tensor, n_experts: int):
+    """(loss float32 [], counts int32 [n_experts]) of gates and ids [..., heads, k]."""
+    _need_here(gates, "gates", FLOATS)
+    _need_here(ids, "ids", INTS)
+    H, k = gates.shape[-2:]
+    n = gates.numel() // (H * k)
+    lib = load()
+    ws, ws_bytes = workspace(lib.ethos_balance_workspace_bytes(n, H, k), gates.device)
+    counts = torch.empty((n_experts,), dtype=torch.int32, device=gates.device)
+    loss = torch.empty((), dtype=torch.float32, device=gates.device)
+    rc = lib.ethos_balance(gates.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), n, H, k, n_experts, dtype_code(gates.dtype),
+                           ws.data_ptr(), ws_bytes, counts.data_ptr(), loss.data_ptr(), _stream())
+    check(rc, "ethos_balance")
+    return loss, counts
+
+
+def balance_grad(ids: torch.Tensor, counts: torch.Tensor, dloss: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The gates' gradient, the shape of ids."""
+    H, k = ids.shape[-2:]
+    out = torch.empty(ids.shape, dtype=dtype, device=ids.device)
+    rc = load().ethos_balance_grad(ids.data_ptr(), int(ids.dtype == torch.int64), counts.data_ptr(), dloss.data_ptr(),
+                                   ids.numel() // (H * k), H, k, counts.numel(), dtype_code(dtype), out.data_ptr(), _stream())
+    check(rc, "ethos_balance_grad")
+    return out
+
+
+def clip_grads(grads, out, max_norm: float, inf_norm: bool) -> torch.Tensor:
+    """The norm (float32 []) of contiguous tensors on the current device, whose clipped values go to `out`."""
+    n, lib = len(grads), load()
+    src, dst = [t.data_ptr() for t in grads], [t.data_ptr() for t in out]
+    pointers = ctypes.c_void_p * n
+    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
+    codes = (ctypes.c_int32 * n)(*[dtype_code(t.dtype) for t in grads])
+    ws, ws_bytes = workspace(lib.ethos_clip_grads_workspace_bytes(sizes, n), grads[0].device)
+    total = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    rc = lib.ethos_clip_grads(pointers(*src), pointers(*dst), sizes, codes, n, int(inf_norm), max_norm, ws.data_ptr(), ws_bytes,
+                              total.data_ptr(), _stream())
+    check(rc, "ethos_clip_grads")
+    return total

@@ -614,16 +614,17 @@ class EthosExpertLayer(nn.Module):
         return hip.expert_forward(x_flat, latents, w1, w2, seg, gates, self.num_heads, self.top_k,
                                   hidden_space=self.hidden_space, wut=wut, xp=xp)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, routing: list | None = None) -> torch.Tensor:
         if x.dim() != 3 or x.shape[-1] != self.d_model:
             raise RuntimeError(f"expected x of shape [batch, seq, {self.d_model}], got {tuple(x.shape)}")
         b, s, d = x.shape
         x_flat = _as_input(x, 3).view(-1, d)
         if x_flat.shape[0] == 0:
             return torch.zeros_like(x)
-        return self.forward_flat(x_flat).view(b, s, d)
+        return self.forward_flat(x_flat, routing=routing).view(b, s, d)
 
-    def forward_flat(self, x_flat: torch.Tensor, mark=None, side_stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    def forward_flat(self, x_flat: torch.Tensor, mark=None, side_stream: torch.cuda.Stream | None = None,
+                     routing: list | None = None) -> torch.Tensor:
         """The layer on [n_tok, d_model] rows (model.py:288-343), in eval mode one library call;
         with `mark` or `side_stream` (and in training mode) stage by stage.  `mark(stage)`, if given, is
         called after the query projection, the routing and the sort are enqueued on the
@@ -631,16 +632,20 @@ class EthosExpertLayer(nn.Module):
         stages inside it).  `side_stream`: the token projection x W_u, which needs only x, runs
         there while the routing and the sort run on the current stream, which waits for it
         before the expert stages (worth its host cost under graph capture; see
-        ethos_amd.graphs)."""
+        ethos_amd.graphs).  `routing`, if given, gets the pass's gates (with their graph under
+        autograd) and expert ids appended as a pair, for losses on them."""
         if _wants_grad(x_flat, self):
             with torch.no_grad():
                 gates, ids = self.router.route(x_flat)
                 seg = hip.sort_segment(ids.view(-1), self.num_experts)
             g = self.router._gate_graph(x_flat, ids, gates)
+            if routing is not None:
+                routing.append((g, ids))
             return _ExpertStages.apply(x_flat, g, self.expert_latents.weight, self.generation_network.net[0].weight,
                                        self.generation_network.net[2].weight, self, gates, seg)
         router = self._modules["router"]
-        if mark is None and side_stream is None and x_flat.shape[0] > 0 and not router._bn_uses_batch_stats():
+        if (mark is None and side_stream is None and routing is None and x_flat.shape[0] > 0
+                and not router._bn_uses_batch_stats()):
             with torch.no_grad():
                 w = router._packed_weights(x_flat.dtype, x_flat.device, 0)
                 packed = w[:4] + tuple(router._bn_coefficients(x_flat.device))
@@ -659,6 +664,8 @@ class EthosExpertLayer(nn.Module):
                 with torch.cuda.stream(side_stream):
                     hip.token_proj(x_flat, w2, wut, out=xp)
             gates, ids = self.router.route(x_flat, mark)
+            if routing is not None:
+                routing.append((gates, ids))
             if xp is None and ids.numel() <= hip.SMALL_SORT_MAX and x_flat.dtype == torch.bfloat16:
                 # small batches: the token projection runs in the sort's launch, beside its
                 # single workgroup

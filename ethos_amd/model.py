@@ -27,12 +27,13 @@ from __future__ import annotations
 
 import math
 from types import SimpleNamespace
+from typing import NamedTuple
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import hip
+from . import hip, training
 from .layer import EthosExpertLayer
 
 # the reference's configs/default.yaml, with the benchmarked expert-layer shape (d_query
@@ -201,9 +202,20 @@ class TransformerBlock(nn.Module):
         self.input_layernorm = RMSNorm(config.d_model, eps=config.rms_norm_eps)
         self.post_attention_layernorm = RMSNorm(config.d_model, eps=config.rms_norm_eps)
 
-    def forward(self, x, attention_mask, position_ids):
+    def forward(self, x, attention_mask, position_ids, routing: list | None = None):
+        """`routing`, if given, gets (gates, expert ids) of an expert layer appended."""
         h = x + self.self_attn(self.input_layernorm(x), attention_mask, position_ids)
-        return h + self.mlp(self.post_attention_layernorm(h))
+        y = self.post_attention_layernorm(h)
+        return h + (self.mlp(y, routing) if routing is not None and isinstance(self.mlp, EthosExpertLayer) else self.mlp(y))
+
+
+class LossParts(NamedTuple):
+    """What CompressedMoEModel.loss returns."""
+
+    loss: torch.Tensor            # carries the graph
+    cross_entropy: torch.Tensor
+    balance: torch.Tensor | None  # mean over the expert layers
+    counts: list                  # per expert layer, how often each expert was chosen
 
 
 class CompressedMoEModel(nn.Module):
@@ -226,6 +238,25 @@ class CompressedMoEModel(nn.Module):
         for block in self.layers:
             h = block(h, None, pos)  # None: causal attention
         return self.output(self.norm(h))
+
+    def loss(self, input_ids: torch.Tensor, labels: torch.Tensor, balance_weight: float = 0.0, ignore_index: int = -100) -> LossParts:
+        """The training loss of token ids [batch, seq]: labels int64 [batch, seq], the token that each
+        position is to predict (`ignore_index`: none), which enter a mean cross entropy over the tied
+        head; and, with a balance_weight, the mean of the expert layers' balance losses times it.  The
+        logits that `forward` returns are not formed (ethos_amd.training)."""
+        if labels.shape != input_ids.shape:
+            raise RuntimeError(f"labels {tuple(labels.shape)} must have the shape of input_ids {tuple(input_ids.shape)}")
+        routing: list | None = [] if balance_weight != 0.0 else None
+        pos = torch.arange(input_ids.shape[1], device=input_ids.device)
+        h = training.embedding(input_ids, self.tok_embeddings.weight)
+        for block in self.layers:
+            h = block(h, None, pos, routing)
+        ce = training.linear_cross_entropy(self.norm(h), self.output.weight, labels, ignore_index=ignore_index)
+        if not routing:
+            return LossParts(ce, ce.detach(), None, [])
+        parts = [training.balance_loss(gates, ids, self.config.num_experts) for gates, ids in routing]
+        balance = torch.stack([p[0] for p in parts]).mean()
+        return LossParts(ce + balance_weight * balance, ce.detach(), balance.detach(), [p[1] for p in parts])
 
 
 def init_random_(model: CompressedMoEModel, seed: int = 0) -> CompressedMoEModel:

@@ -1,0 +1,231 @@
+"""Operators of a language model's training step around its blocks, as HIP kernels
+(include/ethos_hip.h):
+
+  linear_cross_entropy  softmax cross entropy of hidden rows against a head matrix, and its
+                        gradients, without the logits in memory
+  embedding             rows of a table, scaled; the table's gradient by sorted tokens
+  balance_loss          how often each expert was chosen, the load-balance loss, its gradient
+  clip_grads            the global norm of many gradients, and the clipped gradients
+
+The reference trains through torch operations (F.cross_entropy of model.py:396's logits, nn.Embedding,
+nn.utils.clip_grad_norm_) and has no balance loss.  Inputs are HIP tensors on the current device, bf16
+or float32; there is no CPU path.  All work goes to the current stream.  Results are the same on
+every run.  The gradients are those of a single backward (no create_graph)."""
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import hip
+
+__all__ = ["balance_loss", "clip_grads", "embedding", "linear_cross_entropy"]
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous at a 16-byte address (a copy where it is not)."""
+    t = t.detach().contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[n, d] rows of t [..., d] that the kernels can read: evenly spaced, 16-byte aligned."""
+    t = t.detach()
+    ld = hip.row_stride(t)
+    if ld >= t.shape[-1] and ld * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
+        n = t.numel() // t.shape[-1] if t.numel() else 0
+        return t.as_strided((n, t.shape[-1]), (ld, 1))
+    return _dense(t).view(-1, t.shape[-1])
+
+
+def _device_check(name: str, t: torch.Tensor) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{name} must be on a HIP device (got {t.device}); the ETHOS kernels have no CPU path")
+    if t.device.index != hip._current_device():
+        raise RuntimeError(f"{name} is on {t.device}, not on the current device")
+
+
+# -------------------------------------------------------------------------- cross entropy
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, weight, labels, ignore_index, reduction):
+        rows, w = _rows(h), _dense(weight)
+        loss, state = hip.linear_ce(rows, w, labels, ignore_index, reduction)
+        # the weight itself is saved, so that a change in place before the backward is noticed
+        ctx.save_for_backward(state, weight)
+        ctx.copy = w if w.data_ptr() != weight.data_ptr() else None
+        ctx.shape, ctx.reduction = h.shape, reduction
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        state, weight = ctx.saved_tensors
+        w = weight.detach() if ctx.copy is None else ctx.copy
+        n = math.prod(ctx.shape[:-1])
+        want_h, want_w = ctx.needs_input_grad[:2]
+        dh, dw = hip.linear_ce_grad(state, w, dloss.float().contiguous(), n, ctx.reduction, want_h, want_w)
+        return dh.view(ctx.shape) if want_h else None, dw, None, None, None
+
+
+def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
+                         reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of h @ weight.T against labels, without forming the logits.
+
+    h [..., d] and weight [vocab, d] of one dtype (bf16 or float32), d a multiple of 8 up to 32768;
+    labels int64 [...].  Positions whose label is `ignore_index` have no part in the loss or its
+    gradients; another label outside the vocabulary makes the loss NaN.  `reduction`: "mean" over the
+    labelled positions (NaN without one), "sum", or "none" (float32 [...], zero where ignored).  The
+    loss is float32.  Gradients go to h and weight, in their dtype; logits are formed a second time
+    for them, a piece of the vocabulary at a time."""
+    for name, t in (("h", h), ("weight", weight), ("labels", labels)):
+        _device_check(name, t)
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    if h.dtype not in hip.FLOATS or weight.dtype != h.dtype:
+        raise TypeError(f"h and weight must both be bfloat16 or both float32, got {h.dtype} and {weight.dtype}")
+    if labels.dtype != torch.int64:
+        raise TypeError(f"labels must be int64, got {labels.dtype}")
+    if h.dim() < 1 or weight.dim() != 2 or h.shape[-1] != weight.shape[1] or labels.shape != h.shape[:-1]:
+        raise RuntimeError(f"linear_cross_entropy: inconsistent shapes {tuple(h.shape)}, {tuple(weight.shape)}, {tuple(labels.shape)}")
+    d = h.shape[-1]
+    if weight.shape[0] == 0 or d == 0 or d % 8 or d > 32768:
+        raise RuntimeError(f"linear_cross_entropy: needs a vocabulary and d a multiple of 8 up to 32768, got weight {tuple(weight.shape)}")
+    if labels.numel() == 0:  # the sum over nothing, with zero gradients
+        zero = h.float().sum() + 0.0 * weight[:1].float().sum() if reduction != "none" else h.float().sum(-1)
+        return zero if reduction != "mean" else zero / 0.0
+    flat = labels.contiguous().view(-1)
+    if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
+        loss = _LinearCrossEntropy.apply(h, weight, flat, int(ignore_index), reduction)
+    else:
+        loss = hip.linear_ce(_rows(h), _dense(weight), flat, int(ignore_index), reduction)[0]
+    return loss.view(labels.shape) if reduction == "none" else loss
+
+
+# -------------------------------------------------------------------------- embedding
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding):
+        ctx.save_for_backward(ids)
+        ctx.vocab, ctx.scale, ctx.padding = weight.shape[0], scale, padding
+        return hip.embedding(ids, weight.detach().contiguous(), scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (ids,) = ctx.saved_tensors
+        return hip.embedding_grad(ids, _dense(dy), ctx.vocab, ctx.scale, ctx.padding), None, None, None
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
+    """scale * weight[ids], [*ids.shape, d], for a table weight [vocab, d] (bf16 or float32) and ids of
+    any shape (int32 or int64).  The table's gradient is dense, leaves out positions of `padding_idx`
+    (negative ones count from the end) and adds a token's positions in their order, in float32.  An
+    id outside the table gives a row of NaN."""
+    _device_check("ids", ids)
+    _device_check("weight", weight)
+    if weight.dtype not in hip.FLOATS:
+        raise TypeError(f"weight must be bfloat16 or float32, got {weight.dtype}")
+    if ids.dtype not in hip.INTS:
+        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise RuntimeError(f"embedding: weight must be [vocab, d], got {tuple(weight.shape)}")
+    padding = -1
+    if padding_idx is not None:
+        if not -weight.shape[0] <= padding_idx < weight.shape[0]:
+            raise ValueError(f"padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
+        padding = padding_idx % weight.shape[0]
+    ids = ids.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _Embedding.apply(weight, ids, float(scale), padding)
+    return hip.embedding(ids, weight.detach().contiguous(), float(scale))
+
+
+# -------------------------------------------------------------------------- balance
+class _Balance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gates, ids, n_experts):
+        loss, counts = hip.balance(gates.detach().contiguous(), ids, n_experts)
+        ctx.save_for_backward(ids, counts)
+        ctx.dtype = gates.dtype
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        return loss, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss, _):
+        if dloss is None:
+            return None, None, None
+        ids, counts = ctx.saved_tensors
+        return hip.balance_grad(ids, counts, dloss, ctx.dtype), None, None
+
+
+def balance_loss(gates: torch.Tensor, ids: torch.Tensor, n_experts: int):
+    """(loss, counts): the load-balance loss of a routing and how often each expert was chosen.
+
+    gates [..., heads, k] (bf16 or float32) and ids of the same shape (int32 or int64), as
+    ProductKeyRouter returns them.  With n tokens (the product of the leading dimensions),
+    loss = n_experts * sum_e f_e s_e (float32), f_e = counts[e] / (n heads k) held fixed and s_e the
+    sum of expert e's gates over (n heads); it is 1 when both are even over the experts.  counts is int32
+    [n_experts].  Ids outside [0, n_experts) count nowhere.  Without tokens both are zero."""
+    _device_check("gates", gates)
+    _device_check("ids", ids)
+    if gates.dtype not in hip.FLOATS:
+        raise TypeError(f"gates must be bfloat16 or float32, got {gates.dtype}")
+    if ids.dtype not in hip.INTS:
+        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
+    if gates.dim() < 2 or gates.shape != ids.shape or 0 in gates.shape[-2:]:
+        raise RuntimeError(f"balance_loss: gates and ids must both be [..., heads, k], got {tuple(gates.shape)} and {tuple(ids.shape)}")
+    if n_experts <= 0:
+        raise ValueError(f"n_experts must be positive, got {n_experts}")
+    ids = ids.contiguous()
+    if torch.is_grad_enabled() and gates.requires_grad:
+        return _Balance.apply(gates, ids, int(n_experts))
+    return hip.balance(gates.detach().contiguous(), ids, int(n_experts))
+
+
+# -------------------------------------------------------------------------- clipping
+@torch.no_grad()
+def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
+    """The global norm of `grads` (tensors, bf16 or float32, all taken as one vector), a float32 scalar
+    on the device, and the gradients times min(1, max_norm / (norm + 1e-6)) in `out` (tensors of the same
+    shapes and dtypes, for example parts of a reduction's buffer), or in place without it.
+    norm_type: 2 (squares summed in float64) or inf.  A NaN gradient makes norm and outputs NaN.  Tensors
+    may not overlap, but an output may be its own input."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    out = grads if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    if norm_type not in (2, math.inf):
+        raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative, got {max_norm}")
+    if len(out) != len(grads):
+        raise ValueError(f"{len(grads)} gradients but {len(out)} outputs")
+    device = None
+    for t in grads if out is grads else grads + out:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("clip_grads takes tensors")
+        if device is None and t.is_cuda:
+            device = hip._current_device()
+        if t.get_device() != device:
+            raise RuntimeError(f"clip_grads: tensors must be on the current HIP device, got one on {t.device}")
+        if t.dtype not in hip.FLOATS:
+            raise TypeError(f"clip_grads: tensors must be bfloat16 or float32, got {t.dtype}")
+    if out is not grads and any(g.shape != o.shape or g.dtype != o.dtype for g, o in zip(grads, out)):
+        raise RuntimeError("clip_grads: outputs must have the gradients' shapes and dtypes")
+    if not grads:
+        return torch.zeros((), dtype=torch.float32, device="cuda")
+    places = [o.data_ptr() for o in out if o.numel()]
+    if len(set(places)) != len(places):
+        raise ValueError("clip_grads: an output is given twice")
+    src = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    dst = [o if o.is_contiguous() else torch.empty_like(s) for s, o in zip(src, out)]
+    total = hip.clip_grads(src, dst, float(max_norm), norm_type == math.inf)
+    for o, t in zip(out, dst):
+        if o is not t:
+            o.copy_(t)
+    torch.autograd.graph.increment_version([o for o in out if not o.is_inference()])  # written by address
+    return total

@@ -23,6 +23,10 @@
  *   ethos_gate_grads     the routing gates' backward: x, query projections, BatchNorm, sub-keys
  *   ethos_rms_norm, ethos_swiglu, ethos_mla_attention  the language model's blocks
  *   ethos_expert_grads   the expert stages' backward whole: every gradient in one call
+ *   ethos_linear_ce, ethos_linear_ce_grad  the loss over the vocabulary and its gradients
+ *   ethos_embedding, ethos_embedding_grad  embedding rows and their table's gradient
+ *   ethos_balance, ethos_balance_grad      expert counts, the load-balance loss, its gradient
+ *   ethos_clip_grads     the global norm of many gradients, and clipping
  *
  * Conventions (every entry point):
  *   - All pointers are device pointers owned by the caller; nothing is allocated.
@@ -33,7 +37,7 @@
  *     message for the calling thread's last failure.
  *   - dtype: ETHOS_F32 or ETHOS_BF16; tensors of "dtype T" hold that type, row-major.
  *   - Every entry point is deterministic: the same inputs give bit-identical outputs on
- *     every run (no atomics; every sum has a fixed order).
+ *     every run (every sum of floating-point values has a fixed order; the only atomics count).
  */
 #ifndef ETHOS_HIP_H
 #define ETHOS_HIP_H
@@ -495,6 +499,83 @@ int ethos_layer_forward(const void* x, const void* wq, const void* wq_prepared, 
                         int32_t d_query, int32_t n_sub_keys, int32_t top_k, int32_t k_cand, int64_t n_experts, int32_t d_latent,
                         int32_t d_hidden, int32_t dtype, int32_t order, void* workspace, size_t workspace_bytes, void* out,
                         void* stream);
+
+/*
+ * Softmax cross entropy of rows h against a head matrix w, without the logits in memory (the
+ * reference's training would form model.py:396's logits and take F.cross_entropy of them):
+ *   loss_i = log sum_v exp(h_i . w_v) - h_i . w_label(i)
+ *   h       [n_tok] rows of d values of dtype T, ldh apart
+ *   w       [vocab, d] dtype T
+ *   labels  [n_tok] int64; ignore_index: no label (the row has no part in loss and gradients).  Any
+ *           other label outside [0, vocab) makes the row's loss, and the gradients it reaches, NaN.
+ *   reduction  ETHOS_LOSS_MEAN over the rows with a label (NaN without one), _SUM, _NONE
+ *   state   >= ethos_linear_ce_state_bytes(...) bytes: what ethos_linear_ce_grad reads (the rows with
+ *           a label in dense form, their log-sums)
+ *   loss    float32, one value or (NONE) [n_tok]
+ * Logits, exponentials' sums and losses are float32, a reduction's sum float64.
+ * ethos_linear_ce_grad: dh [n_tok, d] and dw [vocab, d] of dtype T (either may be NULL) from dloss
+ * (float32: one value or, NONE, [n_tok]), with the state that the forward left and the same w.  It
+ * forms a piece of the vocabulary's logits at a time again (at most 1 GiB, or 256 words); for bf16 the
+ * logits' gradients are rounded to bf16 for the products with h and w.
+ * Limits: d a multiple of 8, at most 32768; ldh a multiple of 8 (bf16) or 4; vocab <= 2^30; n_tok
+ * <= 2^30; h, w, state, workspace, dh and dw 16-byte aligned.  n_tok = 0 does nothing.
+ */
+#define ETHOS_LOSS_MEAN 0
+#define ETHOS_LOSS_SUM 1
+#define ETHOS_LOSS_NONE 2
+size_t ethos_linear_ce_state_bytes(int64_t n_tok, int32_t d, int32_t dtype);
+size_t ethos_linear_ce_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype);
+int ethos_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* labels, int64_t n_tok, int32_t d, int64_t vocab,
+                    int64_t ignore_index, int32_t reduction, int32_t dtype, void* state, size_t state_bytes, void* workspace,
+                    size_t workspace_bytes, float* loss, void* stream);
+size_t ethos_linear_ce_grad_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype);
+int ethos_linear_ce_grad(const void* state, size_t state_bytes, const void* w, const float* dloss, int64_t n_tok, int32_t d,
+                         int64_t vocab, int32_t reduction, int32_t dtype, void* workspace, size_t workspace_bytes, void* dh, void* dw,
+                         void* stream);
+
+/*
+ * Embedding rows (the lookup of model.py:390): out[i] = RN_T(scale w[ids[i]]), and the table's
+ * gradient dw[v] = RN_T(scale sum over {i: ids[i] = v} dy[i]), float32 sums in the order of i; every
+ * row of dw is written.  ids: int32, or int64 with ids_64; an id outside [0, vocab) gives a row of
+ * NaN and has no part in the gradient, nor have positions whose id is `padding` (negative: none).
+ *   w, dw [vocab, d], dy, out [n, d] dtype T, at any address a T may have; dy and dw 16-byte aligned
+ *   workspace  >= ethos_embedding_grad_workspace_bytes(...) bytes, 16-byte aligned (scratch)
+ * Limits: n, d, vocab < 2^31 - 1.
+ */
+int ethos_embedding(const void* ids, int32_t ids_64, const void* w, int64_t n, int32_t d, int64_t vocab, float scale, int32_t dtype,
+                    void* out, void* stream);
+size_t ethos_embedding_grad_workspace_bytes(int64_t n, int32_t d, int64_t vocab);
+int ethos_embedding_grad(const void* ids, int32_t ids_64, const void* dy, int64_t n, int32_t d, int64_t vocab, float scale,
+                         int64_t padding, int32_t dtype, void* workspace, size_t workspace_bytes, void* dw, void* stream);
+
+/*
+ * How often each expert was chosen, and a load-balance loss of the routing (none in the reference):
+ *   counts[e] = #{p: ids[p] = e},  loss = n_experts sum_e f_e s_e,
+ *   f_e = counts[e] / (n_tok n_heads top_k),  s_e = (sum of gates[p] over ids[p] = e) / (n_tok n_heads)
+ * and, with the counts held fixed, dgates[p] = dloss n_experts f_ids[p] / (n_tok n_heads).
+ *   gates, dgates [n_tok, n_heads, top_k] dtype T; ids the same shape, int32 or (ids_64) int64; an id
+ *   outside [0, n_experts) counts nowhere
+ *   workspace  >= ethos_balance_workspace_bytes(...) bytes, 16-byte aligned (scratch)
+ * No tokens: counts and loss are zero.  Limits: n_tok n_heads top_k < 2^31, n_experts < 2^31.
+ */
+size_t ethos_balance_workspace_bytes(int64_t n_tok, int32_t n_heads, int32_t top_k);
+int ethos_balance(const void* gates, const void* ids, int32_t ids_64, int64_t n_tok, int32_t n_heads, int32_t top_k, int64_t n_experts,
+                  int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* counts, float* loss, void* stream);
+int ethos_balance_grad(const void* ids, int32_t ids_64, const int32_t* counts, const float* dloss, int64_t n_tok, int32_t n_heads,
+                       int32_t top_k, int64_t n_experts, int32_t dtype, void* dgates, void* stream);
+
+/*
+ * Clipping by the global norm of n_tensors gradients (no counterpart in the reference):
+ *   total = sqrt(sum of every value's square), or (inf_norm) the largest magnitude;
+ *   out[t] = RN(in[t] min(1, max_norm / (total + 1e-6))).
+ * in, out, sizes (values) and dtypes: host arrays, read during the call only; out[t] may be in[t], else
+ * no tensor may overlap another.  Squares are summed in float64; a NaN value makes total and every
+ * output NaN.  total: float32 [1].
+ *   workspace  >= ethos_clip_grads_workspace_bytes(...) bytes, 16-byte aligned (scratch)
+ */
+size_t ethos_clip_grads_workspace_bytes(const int64_t* sizes, int32_t n_tensors);
+int ethos_clip_grads(const void* const* in, void* const* out, const int64_t* sizes, const int32_t* dtypes, int32_t n_tensors,
+                     int32_t inf_norm, double max_norm, void* workspace, size_t workspace_bytes, float* total, void* stream);
 
 #ifdef __cplusplus
 }
