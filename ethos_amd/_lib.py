@@ -75,10 +75,10 @@ SIGNATURES = {
     "ethos_linear_ce": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i32, _i64, _i64, _i32, _i32, _vp, _sz, _vp, _sz, _vp, _vp]),
     "ethos_linear_ce_grad_workspace_bytes": (_sz, [_i64, _i32, _i64, _i32]),
     "ethos_linear_ce_grad": (ctypes.c_int, [_vp, _sz, _vp, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _sz, _vp, _vp, _vp]),
-    "ethos_embedding": (ctypes.c_int, [_vp, _i32, _vp, _i64, _i32, _i64, _f32, _i32, _vp, _vp]),
+    "ethos_embedding": (ctypes.c_int, [_vp, _i32, _vp, _i64, _i32, _i64, _f32, _i64, _i32, _vp, _vp, _vp]),
     "ethos_embedding_grad_workspace_bytes": (_sz, [_i64, _i32, _i64]),
-    "ethos_embedding_grad": (ctypes.c_int, [_vp, _i32, _vp, _i64, _i32, _i64, _f32, _i64, _i32, _vp, _sz, _vp, _vp]),
-    "ethos_balance_workspace_bytes": (_sz, [_i64, _i32, _i32]),
+    "ethos_embedding_grad": (ctypes.c_int, [_vp, _vp, _i64, _i32, _i64, _f32, _i32, _vp, _sz, _vp, _vp]),
+    "ethos_balance_workspace_bytes": (_sz, [_i64, _i32, _i32, _i64]),
     "ethos_balance": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i32, _i32, _i64, _i32, _vp, _sz, _vp, _vp, _vp]),
     "ethos_balance_grad": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i64, _i32, _i32, _i64, _i32, _vp, _vp]),
     "ethos_clip_grads_workspace_bytes": (_sz, [_vp, _i32]),

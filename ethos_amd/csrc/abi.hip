@@ -947,7 +947,7 @@ size_t ethos_linear_ce_state_bytes(int64_t n_tok, int32_t d, int32_t dtype) {
 
 size_t ethos_linear_ce_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype) {
     if (n_tok <= 0 || n_tok > kMaxItems || d <= 0 || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
-    return ethos::linear_ce_workspace_bytes(n_tok, d, vocab, dtype);
+    return ethos::linear_ce_workspace_bytes(n_tok, d, vocab, dtype, num_cus());
 }
 
 int ethos_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* labels, int64_t n_tok, int32_t d, int64_t vocab,
@@ -961,7 +961,7 @@ int ethos_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* la
     if (n_tok == 0) return 0;
     if (!h || !w || !labels || !state || !workspace || !loss) return fail(ETHOS_ENULL, "ethos_linear_ce: null pointer");
     if (state_bytes < ethos::linear_ce_state_bytes(n_tok, d, dtype) ||
-        workspace_bytes < ethos::linear_ce_workspace_bytes(n_tok, d, vocab, dtype))
+        workspace_bytes < ethos::linear_ce_workspace_bytes(n_tok, d, vocab, dtype, num_cus()))
         return fail(ETHOS_EWORKSPACE, "ethos_linear_ce: state of %zu or workspace of %zu bytes too small", state_bytes, workspace_bytes);
     if (!aligned16(h) || !aligned16(w) || !aligned16(state) || !aligned16(workspace))
         return fail(ETHOS_EALIGN, "ethos_linear_ce: h, w, state and workspace must be 16-byte aligned");
@@ -1005,14 +1005,15 @@ bool aligned_to(const void* p, int32_t dtype) { return ((uintptr_t)p & (dtype ==
 
 }  // namespace
 
-int ethos_embedding(const void* ids, int32_t ids_64, const void* w, int64_t n, int32_t d, int64_t vocab, float scale, int32_t dtype,
-                    void* out, void* stream) {
+int ethos_embedding(const void* ids, int32_t ids_64, const void* w, int64_t n, int32_t d, int64_t vocab, float scale, int64_t padding,
+                    int32_t dtype, void* out, int32_t* keys, void* stream) {
     g_err[0] = 0;
     if (const int rc = embed_sizes(n, d, vocab, dtype, "ethos_embedding")) return rc;
     if (n == 0) return 0;
     if (!ids || !w || !out) return fail(ETHOS_ENULL, "ethos_embedding: null pointer");
     if (!aligned_to(w, dtype) || !aligned_to(out, dtype)) return fail(ETHOS_EALIGN, "ethos_embedding: w or out misaligned");
-    return hip_status(ethos::launch_embedding(ids, ids_64, w, n, d, vocab, scale, dtype, out, num_cus(), (hipStream_t)stream),
+    return hip_status(ethos::launch_embedding(ids, ids_64, w, n, d, vocab, scale, padding, dtype, out, keys, num_cus(),
+                                              (hipStream_t)stream),
                       "ethos_embedding");
 }
 
@@ -1021,18 +1022,17 @@ size_t ethos_embedding_grad_workspace_bytes(int64_t n, int32_t d, int64_t vocab)
     return ethos::embedding_grad_workspace_bytes(n, d, vocab);
 }
 
-int ethos_embedding_grad(const void* ids, int32_t ids_64, const void* dy, int64_t n, int32_t d, int64_t vocab, float scale,
-                         int64_t padding, int32_t dtype, void* workspace, size_t workspace_bytes, void* dw, void* stream) {
+int ethos_embedding_grad(const int32_t* keys, const void* dy, int64_t n, int32_t d, int64_t vocab, float scale, int32_t dtype,
+                         void* workspace, size_t workspace_bytes, void* dw, void* stream) {
     g_err[0] = 0;
     if (const int rc = embed_sizes(n, d, vocab, dtype, "ethos_embedding_grad")) return rc;
-    if (!dw || !workspace || (n > 0 && (!ids || !dy))) return fail(ETHOS_ENULL, "ethos_embedding_grad: null pointer");
+    if (!dw || !workspace || (n > 0 && (!keys || !dy))) return fail(ETHOS_ENULL, "ethos_embedding_grad: null pointer");
     if (workspace_bytes < ethos::embedding_grad_workspace_bytes(n, d, vocab))
         return fail(ETHOS_EWORKSPACE, "ethos_embedding_grad: workspace of %zu bytes, %zu needed", workspace_bytes,
                     ethos::embedding_grad_workspace_bytes(n, d, vocab));
     if (!aligned16(dy) || !aligned16(dw) || !aligned16(workspace))
         return fail(ETHOS_EALIGN, "ethos_embedding_grad: dy, dw and workspace must be 16-byte aligned");
-    return hip_status(ethos::launch_embedding_grad(ids, ids_64, dy, n, d, vocab, scale, padding, dtype, workspace, dw, num_cus(),
-                                                   (hipStream_t)stream),
+    return hip_status(ethos::launch_embedding_grad(keys, dy, n, d, vocab, scale, dtype, workspace, dw, num_cus(), (hipStream_t)stream),
                       "ethos_embedding_grad");
 }
 
@@ -1053,8 +1053,9 @@ double balance_scale(int64_t n, int32_t heads, int32_t k, int64_t n_experts) {
 
 }  // namespace
 
-size_t ethos_balance_workspace_bytes(int64_t n_tok, int32_t n_heads, int32_t top_k) {
-    return ethos::balance_workspace_bytes(n_tok > 0 && n_heads > 0 && top_k > 0 ? n_tok * n_heads * top_k : 1);
+size_t ethos_balance_workspace_bytes(int64_t n_tok, int32_t n_heads, int32_t top_k, int64_t n_experts) {
+    if (balance_sizes(n_tok, n_heads, top_k, n_experts, ETHOS_F32, "ethos_balance_workspace_bytes") != 0) return 256;
+    return ethos::balance_workspace_bytes(n_tok * n_heads * top_k, n_experts);
 }
 
 int ethos_balance(const void* gates, const void* ids, int32_t ids_64, int64_t n_tok, int32_t n_heads, int32_t top_k, int64_t n_experts,
@@ -1063,9 +1064,9 @@ int ethos_balance(const void* gates, const void* ids, int32_t ids_64, int64_t n_
     if (const int rc = balance_sizes(n_tok, n_heads, top_k, n_experts, dtype, "ethos_balance")) return rc;
     const int64_t pairs = n_tok * n_heads * top_k;
     if (!counts || !loss || !workspace || (pairs > 0 && (!gates || !ids))) return fail(ETHOS_ENULL, "ethos_balance: null pointer");
-    if (workspace_bytes < ethos::balance_workspace_bytes(pairs))
+    if (workspace_bytes < ethos::balance_workspace_bytes(pairs, n_experts))
         return fail(ETHOS_EWORKSPACE, "ethos_balance: workspace of %zu bytes, %zu needed", workspace_bytes,
-                    ethos::balance_workspace_bytes(pairs));
+                    ethos::balance_workspace_bytes(pairs, n_experts));
     if (!aligned16(workspace) || !aligned_to(gates, dtype)) return fail(ETHOS_EALIGN, "ethos_balance: workspace or gates misaligned");
     return hip_status(ethos::launch_balance(gates, ids, ids_64, pairs, n_experts, balance_scale(n_tok, n_heads, top_k, n_experts), dtype,
                                             workspace, counts, loss, num_cus(), (hipStream_t)stream),

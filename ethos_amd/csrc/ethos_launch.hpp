@@ -54,6 +54,12 @@ size_t sort_workspace_bytes(int64_t n, int64_t n_experts);
 int launch_sort_segment(const int32_t* ids, int64_t n, int64_t n_experts, void* ws, int32_t* perm, int32_t* uniq,
                         int32_t* seg_off, int32_t* pair_slot, int32_t* sorted_slot, int32_t* n_unique,
                         hipStream_t stream);
+// The same with zeros written over an array of zero_bytes (16-byte aligned), beside the sort where a
+// single workgroup takes it.
+int launch_sort_segment_zero(const int32_t* ids, int64_t n, int64_t n_experts, void* ws, int32_t* perm, int32_t* uniq,
+                             int32_t* seg_off, int32_t* pair_slot, int32_t* sorted_slot, int32_t* n_unique, void* zeros,
+                             int64_t zero_bytes, int num_cus, hipStream_t stream);
+int launch_zero(void* p, int64_t bytes, int num_cus, hipStream_t stream);
 int launch_sort_empty(int32_t* seg_off, int32_t* n_unique, hipStream_t stream);
 // The sort with the bf16 token projection xp = RN(x W_u) (W_u^T given) in the same launch,
 // for batches the single-workgroup sort takes; -1 (nothing launched) otherwise.

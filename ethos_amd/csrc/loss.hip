@@ -5,14 +5,18 @@
 //
 // Rows without a label (ignore_index) are left out before anything else: the rows with one are
 // copied into a dense block (zero-padded to whole tiles), which every product reads; their count
-// stays on the device.  bf16: the forward product keeps a maximum and a sum of exponentials per row
-// and tile of vocabulary.  The backward forms the logits of a piece of the vocabulary again,
-// turns them into dl (bf16) in its epilogue, and multiplies the piece by h and by W.
-// float32: the products of gemm.hip on a piece of float32 logits.
+// stays on the device.  The forward product keeps a maximum and a sum of exponentials per row and tile
+// of vocabulary.  The backward forms the logits of a piece of the vocabulary again, turns them into dl
+// (bf16) in its epilogue, and multiplies the piece by h and by W.
+//
+// float32 operands go through the same kernels as three bf16 planes each, x = hi + mid + lo
+// (ethos_split.hpp): a product is six bf16 products, exact in the float32 sums, the smallest first.
+#include <type_traits>
+
 #include "ethos_common.hpp"
-#include "ethos_gemm.hpp"
 #include "ethos_mfma.hpp"
 #include "ethos_rows.hpp"
+#include "ethos_split.hpp"
 #include "ethos_train.hpp"
 
 namespace ethos {
@@ -24,6 +28,8 @@ constexpr int kPadRows = 256;  // labelled rows are padded with zero rows to a m
 
 __host__ __device__ constexpr int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
+constexpr int planes_of(int dtype) { return dtype == kBF16 ? 1 : 3; }
+
 // What the forward leaves for the backward.
 struct CeState {
     int32_t* count;  // labelled rows
@@ -32,7 +38,8 @@ struct CeState {
     int32_t* lab;    // label of a labelled row (-1: outside the vocabulary)
     float* lse;      // log of the sum of exponentials
     float* ll;       // logit of the label
-    void* h;         // the labelled rows [padded n][ldh]
+    uint16_t* h;     // the labelled rows [planes][padded n][ldh]
+    int32_t* ticket; // zero between kernels
     int64_t np;      // n padded
     int ldh;
     size_t bytes;
@@ -47,13 +54,14 @@ CeState ce_state(char* p, int64_t n, int d, int dtype) {
         at += (bytes + 255) / 256 * 256;
         return r;
     };
-    s.count = (int32_t*)take(4);
+    s.count = (int32_t*)take(8);
     s.idx = (int32_t*)take(s.np * 4);
     s.inv = (int32_t*)take(s.np * 4);
     s.lab = (int32_t*)take(s.np * 4);
     s.lse = (float*)take(s.np * 4);
     s.ll = (float*)take(s.np * 4);
-    s.h = take((size_t)s.np * s.ldh * (dtype == kBF16 ? 2 : 4));
+    s.h = (uint16_t*)take((size_t)s.np * s.ldh * 2 * planes_of(dtype));
+    s.ticket = s.count + 1;
     s.bytes = at;
     return s;
 }
@@ -64,7 +72,7 @@ CeState ce_state(char* p, int64_t n, int d, int dtype) {
 __global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict__ labels, int64_t n, int64_t vocab, int64_t ignore,
                                                        int32_t* __restrict__ count, int32_t* __restrict__ idx,
                                                        int32_t* __restrict__ inv, int32_t* __restrict__ lab,
-                                                       float* __restrict__ loss_rows) {
+                                                       float* __restrict__ loss_rows, int32_t* __restrict__ ticket) {
     __shared__ int32_t sums[16];
     const int tid = threadIdx.x, wave = tid >> 6;
     int32_t base = 0;
@@ -93,42 +101,130 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict
         base += all;
         __syncthreads();
     }
-    if (tid == 0) *count = base;
+    if (tid == 0) {
+        *count = base;
+        *ticket = 0;
+    }
 }
 
-// A wave per row of the dense block: the row of h (zeros in the padding) and its label's logit.
-template <typename T>
-__global__ __launch_bounds__(256) void ce_gather_kernel(const T* __restrict__ h, int64_t ld, const T* __restrict__ w,
-                                                        const int32_t* __restrict__ count, const int32_t* __restrict__ idx,
-                                                        const int32_t* __restrict__ lab, int d, int ldh, T* __restrict__ out,
-                                                        float* __restrict__ ll) {
-    constexpr int N = Vec16<T>::kN;
-    typedef typename Vec16<T>::raw Raw;
-    const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t m = *count;
-    if (r >= round_up(m, kPadRows)) return;
-    const bool in = r < m;
-    const T* src = h + (in ? (int64_t)idx[r] : 0) * ld;
-    const int label = in ? lab[r] : -1;
-    const T* row = w + (int64_t)(label < 0 ? 0 : label) * d;
-    float s = 0.0f;
-    for (int c = lane * N; c < ldh; c += 64 * N) {
-        Raw v = {};
-        if (in && c < d) {
-            v = *reinterpret_cast<const Raw*>(src + c);
-            if (label >= 0) {
-                float a[N], b[N];
-                Vec16<T>::unpack(v, a);
-                Vec16<T>::unpack(*reinterpret_cast<const Raw*>(row + c), b);
+// Eight values of T as bf16 planes, `stride` values apart.
+__device__ __forceinline__ void put_planes(const uint16_t* src, uint16_t* out, int64_t) {
+    *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(src);
+}
+__device__ __forceinline__ void put_planes(const float* src, uint16_t* out, int64_t stride) {
+    const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+    uint4 p[3];
+    split3(a.x, a.y, p[0].x, p[1].x, p[2].x);
+    split3(a.z, a.w, p[0].y, p[1].y, p[2].y);
+    split3(b.x, b.y, p[0].z, p[1].z, p[2].z);
+    split3(b.z, b.w, p[0].w, p[1].w, p[2].w);
 #pragma unroll
-                for (int j = 0; j < N; ++j) s = __builtin_fmaf(a[j], b[j], s);
-            }
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4*>(out + i * stride) = p[i];
+}
+__device__ __forceinline__ float dot8(const uint16_t* a, const uint16_t* b, float s) {
+    float x[8], y[8];
+    Vec16<uint16_t>::unpack(*reinterpret_cast<const uint4*>(a), x);
+    Vec16<uint16_t>::unpack(*reinterpret_cast<const uint4*>(b), y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = __builtin_fmaf(x[j], y[j], s);
+    return s;
+}
+__device__ __forceinline__ float dot8(const float* a, const float* b, float s) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = __builtin_fmaf(a[j], b[j], s);
+    return s;
+}
+
+// Row r of the dense block: row `row` of h (negative: zeros), and its label's logit.
+template <typename T>
+__device__ __forceinline__ void ce_gather_row(const T* h, int64_t ld, const T* w, int64_t row, int label, int64_t r, int d, int ldh,
+                                              int64_t plane, uint16_t* out, float* ll, int lane) {
+    const T* src = h + (row < 0 ? 0 : row) * ld;
+    const T* word = w + (int64_t)(label < 0 ? 0 : label) * d;
+    float s = 0.0f;
+    for (int c = lane * 8; c < ldh; c += 64 * 8) {
+        uint16_t* o = out + r * ldh + c;
+        if (row >= 0 && c < d) {
+            put_planes(src + c, o, plane);
+            if (label >= 0) s = dot8(src + c, word + c, s);
+        } else {
+#pragma unroll
+            for (int i = 0; i < (sizeof(T) == 2 ? 1 : 3); ++i) *reinterpret_cast<uint4*>(o + i * plane) = make_uint4(0, 0, 0, 0);
         }
-        *reinterpret_cast<Raw*>(out + r * ldh + c) = v;
     }
     s = wave_sum(s);
     if (lane == 0) ll[r] = label >= 0 ? s : __builtin_nanf("");
+}
+
+// A wave per row of the dense block.
+template <typename T>
+__global__ __launch_bounds__(256) void ce_gather_kernel(const T* __restrict__ h, int64_t ld, const T* __restrict__ w,
+                                                        const int32_t* __restrict__ count, const int32_t* __restrict__ idx,
+                                                        const int32_t* __restrict__ lab, int d, int ldh, int64_t plane,
+                                                        uint16_t* __restrict__ out, float* __restrict__ ll) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t m = *count;
+    if (r >= round_up(m, kPadRows)) return;
+    ce_gather_row(h, ld, w, r < m ? (int64_t)idx[r] : -1, r < m ? lab[r] : -1, r, d, ldh, plane, out, ll, threadIdx.x & 63);
+}
+
+// Both steps for up to kFewRows rows, in one launch: every workgroup finds the labelled rows itself.
+constexpr int kFewRows = 1024;
+template <typename T>
+__global__ __launch_bounds__(256) void ce_few_rows_kernel(const int64_t* __restrict__ labels, int n, int64_t vocab, int64_t ignore,
+                                                          const T* __restrict__ h, int64_t ld, const T* __restrict__ w,
+                                                          int32_t* __restrict__ count, int32_t* __restrict__ idx,
+                                                          int32_t* __restrict__ inv, int32_t* __restrict__ lab,
+                                                          float* __restrict__ loss_rows, int32_t* __restrict__ ticket, int d, int ldh,
+                                                          int64_t plane, uint16_t* __restrict__ out, float* __restrict__ ll) {
+    __shared__ int32_t sums[4];
+    __shared__ int32_t rows[kFewRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool first = blockIdx.x == 0;
+    int64_t l[kFewRows / 256];
+#pragma unroll
+    for (int c = 0; c < kFewRows / 256; ++c) l[c] = c * 256 + tid < n ? labels[c * 256 + tid] : ignore;
+    int32_t m = 0;
+#pragma unroll
+    for (int c = 0; c < kFewRows / 256; ++c) {
+        if (c * 256 >= n) break;
+        const int i = c * 256 + tid;
+        const bool use = l[c] != ignore;
+        const uint64_t mask = ballot(use);
+        if (lane == 0) sums[wave] = __popcll(mask);
+        __syncthreads();
+        int32_t at = m + count_below(mask);
+        for (int v = 0; v < 4; ++v) {
+            if (v < wave) at += sums[v];
+            m += sums[v];
+        }
+        if (use) rows[at] = i;
+        if (first && i < n) {
+            inv[i] = use ? at : -1;
+            if (use) {
+                idx[at] = i;
+                lab[at] = l[c] >= 0 && l[c] < vocab ? (int32_t)l[c] : -1;
+            } else if (loss_rows) {
+                loss_rows[i] = 0.0f;
+            }
+        }
+        __syncthreads();
+    }
+    if (first && tid == 0) {
+        *count = m;
+        *ticket = 0;
+    }
+    const int r = blockIdx.x * 4 + wave;
+    if (r >= round_up(m, kPadRows)) return;
+    const int row = r < m ? rows[r] : -1;
+    const int64_t label = row >= 0 ? labels[row] : -1;
+    ce_gather_row(h, ld, w, row, label >= 0 && label < vocab ? (int32_t)label : -1, r, d, ldh, plane, out, ll, lane);
+}
+
+// W's planes, eight values a thread.
+__global__ __launch_bounds__(256) void ce_split_kernel(const float* __restrict__ w, int64_t n8, uint16_t* __restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (int64_t)gridDim.x * 256)
+        put_planes(w + i * 8, out + i * 8, n8 * 8);
 }
 
 // ------------------------------------------------------------------------ sums over the vocabulary
@@ -141,45 +237,58 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
     return {m, a.s * __builtin_amdgcn_exp2f((a.m - z) * kLog2e) + b.s * __builtin_amdgcn_exp2f((b.m - z) * kLog2e)};
 }
 
-// lse and loss of each labelled row from its partial (maximum, sum) pairs part[e][np], e < n_part.
-__global__ __launch_bounds__(256) void ce_lse_kernel(const float2* __restrict__ part, int n_part, int64_t np,
-                                                     const int32_t* __restrict__ count, const int32_t* __restrict__ idx,
-                                                     const float* __restrict__ ll, float* __restrict__ lse,
-                                                     float* __restrict__ loss_rows, float* __restrict__ row_loss) {
-    __shared__ MaxSum lds[4][64];
+// lse and loss of each labelled row from its partial (maximum, sum) pairs part[e][np], e < n_part; 16 rows
+// a workgroup, whose 64 groups of 16 lanes take every 64th pair.  A sum or mean over the rows: the workgroup
+// that finishes last adds up the row losses in their order.
+__global__ __launch_bounds__(1024) void ce_lse_kernel(const float2* __restrict__ part, int n_part, int64_t np,
+                                                      const int32_t* __restrict__ count, const int32_t* __restrict__ idx,
+                                                      const float* __restrict__ ll, int reduction, float* __restrict__ lse,
+                                                      float* row_loss, int32_t* ticket, float* __restrict__ loss) {
+    __shared__ MaxSum lds[16][16];
+    __shared__ double sums[16];
+    __shared__ bool last;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t r = (int64_t)blockIdx.x * 64 + lane, m = *count;
-    if ((int64_t)blockIdx.x * 64 >= m) return;
-    MaxSum a = {-__builtin_inff(), 0.0f};
-    for (int e = wave; e < n_part; e += 4) {
-        const float2 p = part[(int64_t)e * np + r];
-        a = join(a, {p.x, p.y});
+    const int64_t r = (int64_t)blockIdx.x * 16 + (lane & 15), m = *count;
+    if ((int64_t)blockIdx.x * 16 < m) {
+        MaxSum a = {-__builtin_inff(), 0.0f};
+        for (int e = wave * 4 + (lane >> 4); e < n_part; e += 64 * 8) {
+            float2 p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = part[(int64_t)(e + j * 64 < n_part ? e + j * 64 : e) * np + r];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (e + j * 64 < n_part) a = join(a, {p[j].x, p[j].y});
+        }
+        a = join(a, {__shfl_xor(a.m, 16), __shfl_xor(a.s, 16)});
+        a = join(a, {__shfl_xor(a.m, 32), __shfl_xor(a.s, 32)});
+        if (lane < 16) lds[wave][lane] = a;
+        __syncthreads();
+        if (wave == 0 && lane < 16 && r < m) {
+            for (int w = 1; w < 16; ++w) a = join(a, lds[w][lane]);
+            const float x = ll[r];
+            const float l = x == x ? a.m + __builtin_amdgcn_logf(a.s) * 0.69314718055994530942f : x;
+            lse[r] = l;
+            if (reduction == kLossNone) loss[idx[r]] = l - x;
+            else __hip_atomic_store(row_loss + r, l - x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
     }
-    lds[wave][lane] = a;
+    if (reduction == kLossNone) return;
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int32_t)gridDim.x - 1;
     __syncthreads();
-    if (wave != 0 || r >= m) return;
-    for (int w = 1; w < 4; ++w) a = join(a, lds[w][lane]);
-    const float x = ll[r];
-    const float l = x == x ? a.m + __builtin_amdgcn_logf(a.s) * 0.69314718055994530942f : x;
-    lse[r] = l;
-    if (loss_rows) loss_rows[idx[r]] = l - x;
-    else row_loss[r] = l - x;
-}
-
-__global__ __launch_bounds__(1024) void ce_total_kernel(const float* __restrict__ row_loss, const int32_t* __restrict__ count,
-                                                        int mean, float* __restrict__ loss) {
-    __shared__ double lds[16];
-    const int64_t m = *count;
+    if (!last) return;
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < m; i += 1024) s += (double)row_loss[i];
+    for (int64_t i = threadIdx.x; i < m; i += 1024) s += (double)__hip_atomic_load(row_loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    if (lane == 0) sums[wave] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
         double t = 0.0;
-        for (int i = 0; i < 16; ++i) t += lds[i];
-        *loss = (float)(mean ? t / (double)m : t);
+        for (int i = 0; i < 16; ++i) t += sums[i];
+        *loss = (float)(reduction == kLossMean ? t / (double)m : t);
+        *ticket = 0;
     }
 }
 
@@ -188,16 +297,35 @@ __device__ __forceinline__ float row_gradient(const float* dloss, const int32_t*
     return reduction == kLossNone ? dloss[idx[r]] : reduction == kLossMean ? *dloss / (float)m : *dloss;
 }
 
-// ------------------------------------------------------------------------ bf16 products
-// C[m][n] = sum_k A(m, k) B(k, n) in tiles of 256 x 256, k in steps of 64, eight waves (two along m, four
-// along n: 128 x 64 each, 128 accumulators a lane).  Operands go from memory straight into LDS, the
-// next step's while the current one is multiplied.  An operand is stored with k contiguous ("K": rows
-// of m or n) or with k as the row ("R"); R tiles are read with the transposing LDS loads.
-// LDS rows of a K tile are 64 k (8 pieces of 16 bytes), piece c at c ^ (row / 2 % 8); of an R tile
-// 256 columns (32 pieces), piece c at c ^ 4 (k % 4).
-constexpr int kTile = 256, kStep = 64, kTileThreads = 512;
-constexpr int kOperandBytes = kTile * kStep * 2;
+// ------------------------------------------------------------------------ products
+// C[m][n] = sum_k A(m, k) B(k, n) in tiles of B x B (256: eight waves, two along m and four along n, 128 x 64 each;
+// 128: four waves of 64 x 64), k in steps of kK.  Operands go from memory
+// straight into LDS, the next step's while the current one is multiplied.  An operand is stored with k
+// contiguous ("K": rows of m or n) or with k as the row ("R"); R tiles are read with the transposing LDS
+// loads.  LDS rows of a K tile are kK k (kK / 8 pieces of 16 bytes, their places by k_piece); of an R
+// tile B columns (B / 8 pieces), piece c at c ^ 4 (k % 4): 16 lanes' reads touch all banks.
+constexpr int kTileMax = 256;
+// dl is stored in panels of 256 words, [panel][np][256], so that a tile of it is one stretch of memory (with the rows of
+// the whole piece, 200 KB apart, a tile is spread over as many pages: 920 us for 4,096 rows against 905)
+constexpr int kPanel = 256;
 constexpr uint32_t kOutside = 0x80000000u;  // an offset past every buffer's end: reads zeros
+
+// float32: the pairs of planes, (2, 0), (1, 1), (0, 2), (1, 0), (0, 1), (0, 0).  The three left out, mid x lo, lo x mid
+// and lo x lo, are at most 2^-22 of a product and 2^-26 on the root mean square, below the rounding of a float32 sum
+// of 16 such products; a third of the products' time.
+constexpr int kPairs = 6;
+constexpr uint32_t kPairsA = 0x001012, kPairsB = 0x010210;
+
+template <int B> struct Tile {
+    static constexpr int kWaves = B == 256 ? 8 : 4, kThreads = kWaves * 64;
+    static constexpr int kWN = kWaves / 2;                           // waves along n (two along m)
+    static constexpr int kMI = B / 64, kNI = B / kWN / 32;           // MFMA tiles of a wave
+    static constexpr int kK = 64;                                    // step of the reduction
+    static constexpr int kStages = 2;                                // steps in LDS
+    static constexpr int kBytes = B * kK * 2;                        // one operand's step
+    static constexpr int kCopies = kBytes / 1024 / kWaves;           // copies of a wave per operand and step
+    static constexpr int kLds = kStages * 2 * kBytes;
+};
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(3))) bf16x8_t* lds_frag_ptr;
@@ -205,138 +333,251 @@ typedef __attribute__((address_space(3))) s16x4_t* lds_tr_ptr;
 
 // One operand: where its tiles are in memory.
 struct Feed {
-    uint64_t base;   // address of the tile's first step
-    int64_t left;    // bytes from there to the operand's end
-    int64_t step;    // bytes from a step to the next
-    int k_left;      // K: k from this step's first to the end
-    uint32_t off[4];  // this lane's offsets
+    uint64_t base;  // address of the next step
+    int64_t left;   // bytes from there to the operand's end
+    int64_t step;   // bytes from a step to the next
+    int k_left;     // K: k from the next step's first to the end
+    uint32_t off[4];  // this lane's offsets (kCopies of them)
+    uint64_t base0;  // the first plane's first step
+    int64_t left0, plane;
+    int k0;
+    int64_t jump;   // dl by rows: bytes to the next panel, taken after the panel's last step
+    int at, at0;    // steps taken in the panel
 };
 
-template <bool KC>
-__device__ __forceinline__ void feed_init(Feed& f, const uint16_t* p, int64_t bytes, int64_t ld, int k, int cols, int wave, int lane) {
-    f.base = (uint64_t)p;
-    f.left = bytes;
-    f.step = KC ? kStep * 2 : kStep * ld * 2;
-    f.k_left = k;
+// The piece of a K tile's row at place c, and the other way round.
+template <int K>
+__device__ __forceinline__ int k_piece(int row, int c) {
+    return K == 64 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3);
+}
+
+template <int B, bool KC>
+__device__ __forceinline__ void feed_init(Feed& f, const uint16_t* p, int64_t bytes, int64_t ld, int k, int cols, int64_t plane,
+                                          int wave, int lane) {
+    f.base = f.base0 = (uint64_t)p;
+    f.left = f.left0 = bytes;
+    typedef Tile<B> Ti;
+    f.step = KC ? Ti::kK * 2 : Ti::kK * ld * 2;
+    f.k_left = f.k0 = k;
+    f.plane = plane * 2;
+    f.jump = 0;
+    f.at = f.at0 = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int slot = (j * 8 + wave) * 64 + lane;
+    for (int j = 0; j < Ti::kCopies; ++j) {
+        const int slot = (j * Ti::kWaves + wave) * 64 + lane;
         if (KC) {
-            const int row = slot >> 3, c = (slot & 7) ^ ((row >> 1) & 7);
+            const int row = slot / (Ti::kK / 8), c = k_piece<Ti::kK>(row, slot % (Ti::kK / 8));
             f.off[j] = (uint32_t)(row * ld * 2 + c * 16);
         } else {
-            const int kk = slot >> 5, c = (slot & 31) ^ ((kk & 3) << 2);
+            const int kk = slot / (B / 8), c = (slot % (B / 8)) ^ ((kk & 3) << 2);
             f.off[j] = c * 8 < cols ? (uint32_t)(kk * ld * 2 + c * 16) : kOutside;
         }
     }
 }
 
-// This step's tile into LDS at `lds`, and on to the next step.
-template <bool KC>
-__device__ __forceinline__ void feed_issue(Feed& f, uint32_t lds, int wave, int lane) {
+__device__ __forceinline__ void feed_plane(Feed& f, int p) {
+    f.base = f.base0 + (uint64_t)(p * f.plane);
+    f.left = f.left0;
+    f.k_left = f.k0;
+    f.at = f.at0;
+}
+
+// The next step's tile into LDS at `lds`: one of the wave's copies, or all of them and on to the step after.
+template <int B, bool KC>
+__device__ __forceinline__ void feed_copy(const Feed& f, int j, uint32_t lds, int wave, int lane) {
+    typedef Tile<B> Ti;
     const int64_t left = f.left < 0 ? 0 : f.left > 0x7fffffff ? 0x7fffffff : f.left;
-    const i32x4_t rs = buffer_rsrc((const void*)f.base, (uint32_t)left);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t off = f.off[j];
-        if (KC && f.k_left < kStep) {
-            const int slot = (j * 8 + wave) * 64 + lane, c = (slot & 7) ^ ((slot >> 4) & 7);
-            off = c * 8 < f.k_left ? off : kOutside;
-        }
-        lds_dma16(rs, (int)off, 0, lds + (j * 8 + wave) * 1024);
+    uint32_t off = f.off[j];
+    if (KC && f.k_left < Ti::kK) {
+        const int slot = (j * Ti::kWaves + wave) * 64 + lane;
+        off = k_piece<Ti::kK>(slot / (Ti::kK / 8), slot % (Ti::kK / 8)) * 8 < f.k_left ? off : kOutside;
     }
+    lds_dma16(buffer_rsrc((const void*)f.base, (uint32_t)left), (int)off, 0, lds + (j * Ti::kWaves + wave) * 1024);
+}
+template <int B>
+__device__ __forceinline__ void feed_advance(Feed& f) {
     f.base += f.step;
     f.left -= f.step;
-    f.k_left -= kStep;
+    f.k_left -= Tile<B>::kK;
+    if (++f.at == kPanel / Tile<B>::kK) {
+        f.at = 0;
+        f.base += f.jump;
+        f.left -= f.jump;
+    }
 }
 
 // Fragments of 32 rows (or columns) i at row0 + 32 i, reduction step s of 16.
-template <bool KC, int N> struct Reader {
-    uint32_t at[KC ? 4 : N];
+template <int B, bool KC, int N> struct Reader {
+    static constexpr int K = Tile<B>::kK;
+    uint32_t at[KC ? K / 16 : N];
     __device__ __forceinline__ void init(int row0, int lane) {
         if constexpr (KC) {
             const int row = row0 + (lane & 31);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) at[s] = row * 128 + (((2 * s + (lane >> 5)) ^ ((row >> 1) & 7)) << 4);
+            for (int s = 0; s < K / 16; ++s) at[s] = row * (K * 2) + (k_piece<K>(row, 2 * s + (lane >> 5)) << 4);
         } else {
             const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int c = (row0 + 32 * i) / 8 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-                at[i] = k * 512 + ((c ^ ((k & 3) << 2)) << 4) + (lane & 1) * 8;
+                at[i] = k * (B * 2) + ((c ^ ((k & 3) << 2)) << 4) + (lane & 1) * 8;
             }
         }
     }
     __device__ __forceinline__ bf16x8_t get(uint32_t lds, int i, int s) const {
         if constexpr (KC) {
-            return *(lds_frag_ptr)(size_t)(lds + at[s] + i * 4096);
+            return *(lds_frag_ptr)(size_t)(lds + at[s] + i * (K * 64));
         } else {
             union {
                 s16x4_t h[2];
                 bf16x8_t f;
             } u;
-            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(lds + at[i] + s * 8192));
-            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(lds + at[i] + s * 8192 + 2048));
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(lds + at[i] + s * (B * 32)));
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(lds + at[i] + s * (B * 32) + B * 8));
             return u.f;
         }
     }
 };
 
+// All of this wave's copies but the newest `N` have landed, its LDS reads are done, and so with every wave.
+template <int N>
 __device__ __forceinline__ void step_barrier() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// The tile's products over `steps` steps; this wave's 128 x 64 part in acc[4][2].
-template <bool AK, bool BK>
-__device__ __forceinline__ void tile_product(Feed& fa, Feed& fb, int64_t steps, uint32_t lds, f32x16_t (&acc)[4][2], int wave, int lane) {
-    Reader<AK, 4> ra;
-    Reader<BK, 2> rb;
-    ra.init((wave >> 2) * 128, lane);
-    rb.init((wave & 3) * 64, lane);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = f32x16_zero();
-    if (steps <= 0) return;
-    feed_issue<AK>(fa, lds, wave, lane);
-    feed_issue<BK>(fb, lds + kOperandBytes, wave, lane);
-    step_barrier();
-    for (int64_t t = 0; t < steps; ++t) {
-        const uint32_t cur = lds + (uint32_t)(t & 1) * 2 * kOperandBytes;
-        if (t + 1 < steps) {
-            const uint32_t nxt = lds + (uint32_t)((t + 1) & 1) * 2 * kOperandBytes;
-            feed_issue<AK>(fa, nxt, wave, lane);
-            feed_issue<BK>(fb, nxt + kOperandBytes, wave, lane);
-        }
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            bf16x8_t a[4], b[2];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = ra.get(cur, i, s);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) b[j] = rb.get(cur + kOperandBytes, j, s);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
-        }
-        step_barrier();
+// This wave's LDS accesses are done, and so with every wave.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// The copies of a tile's first step, into the first place in LDS.
+template <int B, int PL, bool AK, bool BK>
+__device__ __forceinline__ void tile_begin(Feed& fa, Feed& fb, uint32_t lds, int wave, int lane) {
+    typedef Tile<B> Ti;
+    if (PL > 1) {
+        feed_plane(fa, kPairsA & 3);
+        feed_plane(fb, kPairsB & 3);
     }
+#pragma unroll
+    for (int c = 0; c < Ti::kCopies; ++c) feed_copy<B, AK>(fa, c, lds, wave, lane);
+#pragma unroll
+    for (int c = 0; c < Ti::kCopies; ++c) feed_copy<B, BK>(fb, c, lds + Ti::kBytes, wave, lane);
 }
 
-// A tile of C transposed through LDS: rows n of 256 bf16 values m, the pieces of 16 bytes at
-// c ^ (n % 32), then whole rows to memory.
-__device__ __forceinline__ void put4(uint32_t lds, int n, int m, float a, float b, float c, float d) {
-    typedef __attribute__((address_space(3))) u32x2_t* ptr;
-    *(ptr)(size_t)(lds + n * 512 + (((m >> 3) ^ (n & 31)) << 4) + (m & 4) * 2) = u32x2_t{pack_bf16x2(a, b), pack_bf16x2(c, d)};
+// The tile's products over `steps` steps, after tile_begin (whose copies every wave has waited for).  float32: of
+// each pair of planes, from the two lowest up.  Between the
+// products of 16 k stand the LDS reads of the next 16, one at a time; the step's barrier stands before its last
+// products, which cover the first reads of the next step and the copies into the step just freed.
+template <int B, int PL, bool AK, bool BK>
+__device__ __forceinline__ void tile_run(Feed& fa, Feed& fb, int64_t steps, uint32_t lds, f32x16_t (&acc)[Tile<B>::kMI][Tile<B>::kNI],
+                                             int wave, int lane) {
+    typedef Tile<B> Ti;
+    constexpr int MI = Ti::kMI, NI = Ti::kNI, S = Ti::kStages, C = Ti::kCopies, Q = MI * NI, kLast = Ti::kK / 16 - 1;
+    Reader<B, AK, MI> ra;
+    Reader<B, BK, NI> rb;
+    ra.init(wave / Ti::kWN * (B / 2), lane);
+    rb.init(wave % Ti::kWN * (32 * NI), lane);
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = f32x16_zero();
+    if (steps <= 0) return;
+    int64_t in = 0;
+    int pair = 0;
+    auto copy = [&](uint32_t to, int c) {
+        if (c < C) feed_copy<B, AK>(fa, c, to, wave, lane);
+        else feed_copy<B, BK>(fb, c - C, to + Ti::kBytes, wave, lane);
+    };
+    auto advance = [&]() {
+        feed_advance<B>(fa);
+        feed_advance<B>(fb);
+        if (PL > 1 && ++in == steps) {
+            in = 0;
+            ++pair;
+            feed_plane(fa, (int)(kPairsA >> (4 * pair)) & 3);
+            feed_plane(fb, (int)(kPairsB >> (4 * pair)) & 3);
+        }
+    };
+    bf16x8_t a[2][MI], b[2][NI];
+    // read r of 16 k: in the order in which the products take them
+    auto read = [&](uint32_t from, int s, int r) {
+        if (r == 0) a[s & 1][0] = ra.get(from, 0, s);
+        else if (r <= NI) b[s & 1][r - 1] = rb.get(from + Ti::kBytes, r - 1, s);
+        else if (r < NI + MI) a[s & 1][r - NI] = ra.get(from, r - NI, s);
+    };
+    // the products of 16 k, after each of which `between(q)` is issued
+    auto multiply = [&](int s, auto between) {
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            const int i = q / NI, j = q % NI;
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[s & 1][i], b[s & 1][j], acc[i][j], 0, 0, 0);
+            between(q);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    constexpr int R = (MI + NI + Q - 1) / Q;  // reads after a product
+    const int64_t total = PL > 1 ? steps * kPairs : steps;
+    advance();
+    for (int t = 1; t < S && t < total; ++t) {
+#pragma unroll
+        for (int c = 0; c < 2 * C; ++c) copy(lds + t * 2 * Ti::kBytes, c);
+        advance();
+    }
+#pragma unroll
+    for (int r = 0; r < MI + NI; ++r) read(lds, 0, r);
+    uint32_t cur = 0, from = lds, next = lds;
+    auto head = [&]() {  // all but the step's last products
+        from = lds + cur * 2 * Ti::kBytes;
+        cur = cur + 1 == S ? 0 : cur + 1;
+        next = lds + cur * 2 * Ti::kBytes;
+#pragma unroll
+        for (int s = 0; s < kLast; ++s)
+            multiply(s, [&](int q) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) read(from, s + 1, q * R + r);
+            });
+    };
+    for (int64_t t = S; t < total; ++t) {
+        head();
+        step_barrier<2 * C * (S - 2)>();
+        multiply(kLast, [&](int q) {
+            constexpr int P = (2 * C + Q - 1) / Q;  // copies after a product
+#pragma unroll
+            for (int r = 0; r < R; ++r) read(next, 0, q * R + r);
+#pragma unroll
+            for (int c = 0; c < P; ++c)
+                if (q * P + c < 2 * C) copy(from, q * P + c);
+        });
+        advance();
+    }
+    // the steps that are in LDS or on their way (the last one's reads of a next step go unused)
+    for (int t = total < S ? (int)total : S; t > 0; --t) {
+        head();
+        step_barrier<0>();
+        multiply(kLast, [&](int q) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) read(next, 0, q * R + r);
+        });
+    }
+    step_barrier<0>();
 }
+
+// A tile of C transposed through LDS: rows n of B bf16 values m, the pieces of 16 bytes at
+// c ^ (n % (B / 8)), then whole rows to memory.
+template <int B>
+__device__ __forceinline__ uint32_t row_slot(int n, int m) {
+    return n * (B * 2) + (((m >> 3) ^ (n & (B / 8 - 1))) << 4) + (m & 7) * 2;
+}
+template <int B>
+__device__ __forceinline__ void put4(uint32_t lds, int n, int m, uint32_t lo, uint32_t hi) {
+    typedef __attribute__((address_space(3))) u32x2_t* ptr;
+    *(ptr)(size_t)(lds + row_slot<B>(n, m)) = u32x2_t{lo, hi};
+}
+template <int B, int ROWS>
 __device__ __forceinline__ void tile_to_rows(uint32_t lds, uint16_t* out, int64_t ld, int rows, int cols, int tid) {
     typedef const __attribute__((address_space(3))) u32x4_t* ptr;
 #pragma unroll 4
-    for (int q = tid; q < kTile * 32; q += kTileThreads) {
-        const int n = q >> 5, c = q & 31;
-        if (n < rows && c * 8 < cols)
-            *reinterpret_cast<u32x4_t*>(out + (int64_t)n * ld + c * 8) = *(ptr)(size_t)(lds + n * 512 + ((c ^ (n & 31)) << 4));
+    for (int q = tid; q < ROWS * (B / 8); q += Tile<B>::kThreads) {
+        const int n = q / (B / 8), c = q % (B / 8);
+        if (n < rows && c * 8 < cols) *reinterpret_cast<u32x4_t*>(out + (int64_t)n * ld + c * 8) = *(ptr)(size_t)(lds + row_slot<B>(n, c * 8));
     }
 }
 
@@ -345,199 +586,281 @@ struct Place {
     int64_t group;
     int within;
 };
-__device__ __forceinline__ Place tile_place(int each) {
-    const int64_t i = blockIdx.x / 8;
-    return {i / each * 8 + blockIdx.x % 8, (int)(i % each)};
+__device__ __forceinline__ Place tile_place(int64_t block, int each) {
+    const int64_t i = block / 8;
+    return {i / each * 8 + block % 8, (int)(i % each)};
 }
 
 // Logits of a piece of the vocabulary, transposed (a lane holds values of two rows of h): GRAD 0: the
-// maximum and sum of exponentials over each wave's 128 words; 1: dl rows [np][ldp].
+// maximum and sum of exponentials over each wave's B / 2 words; 1: dl [planes][ldp / 256][np][256].
 struct LogitArgs {
-    const uint16_t* w;  // the piece's first row
+    const uint16_t* w;   // the piece's first row, [planes][vocab][d]
+    const float* w32;    // float32: the piece's first row itself
     const uint16_t* h;
     const int32_t *count, *idx, *lab;
     const float *lse, *ll, *dloss;
-    int64_t v0, v1, np, ldp;  // the piece
+    int64_t v0, v1, np, ldp, w_plane;  // the piece [v0, v1)
     float2* part;
     uint16_t* p;
-    int d, ldh, n_tiles, reduction;
+    int d, ldh, reduction;
 };
 
-template <int GRAD>
-__global__ __launch_bounds__(kTileThreads, 2) void ce_logits_kernel(LogitArgs g) {
-    __shared__ __align__(16) char smem[4 * kOperandBytes];
+// A logit as a float32 chain: what an infinity needs, which against the other operand's lower planes gives
+// NaN (times zero).
+__device__ __forceinline__ float logit_chain(const LogitArgs& g, int64_t v, int64_t r) {
+    float s = 0.0f;
+    const uint16_t* h = g.h + r * g.ldh;
+    const int64_t plane = g.np * g.ldh;
+    for (int k = 0; k < g.d && s == s; ++k) {
+        const float x = bf16_bits_to_f32(h[k]) + (bf16_bits_to_f32(h[k + plane]) + bf16_bits_to_f32(h[k + 2 * plane]));
+        s = __builtin_fmaf(x, g.w32[v * g.d + k], s);
+    }
+    return s;
+}
+
+template <int B, int PL, int GRAD>
+__global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitArgs g) {
+    typedef Tile<B> Ti;
+    constexpr int MI = Ti::kMI, NI = Ti::kNI;
+    __shared__ __align__(16) char smem[Ti::kLds];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Place at = tile_place(g.n_tiles);
-    const int64_t m0 = at.group * kTile, words = g.v1 - g.v0, m = *g.count;
-    const int64_t n0 = (int64_t)at.within * kTile;
-    if (m0 >= words || n0 >= m) return;
-    const uint32_t lds = lds_addr(smem);
-    f32x16_t acc[4][2];
-    {
-        Feed fa, fb;
-        feed_init<true>(fa, g.w + m0 * g.d, (words - m0) * g.d * 2, g.d, g.d, 0, wave, lane);
-        feed_init<true>(fb, g.h + n0 * g.ldh, (g.np - n0) * g.ldh * 2, g.ldh, g.d, 0, wave, lane);
-        tile_product<true, true>(fa, fb, (g.d + kStep - 1) / kStep, lds, acc, wave, lane);
-    }
-    const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
-    // words past the vocabulary
-    if (m0 + wm + 128 > words) {
+    const uint32_t lds = lds_addr(smem), rows_lds = lds + 2 * Ti::kBytes;
+    const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
+    const int64_t words = g.v1 - g.v0, m = *g.count;
+    // this workgroup's tiles: those of the vocabulary tiles of its XCD, one after the other, every gridDim / 8th
+    const int n_tiles = (int)((m + B - 1) / B), xcd = blockIdx.x % 8;
+    const int64_t m_tiles = (words + B - 1) / B, tiles = (m_tiles - xcd + 7) / 8 * n_tiles;
+    int64_t tile = blockIdx.x / 8;
+    if (tile >= tiles) return;
+    Feed fa, fb;
+    int64_t m0, n0;
+    auto begin = [&]() {
+        m0 = (tile / n_tiles * 8 + xcd) * B;
+        n0 = tile % n_tiles * B;
+        feed_init<B, true>(fa, g.w + m0 * g.d, (words - m0) * g.d * 2, g.d, g.d, 0, g.w_plane, wave, lane);
+        feed_init<B, true>(fb, g.h + n0 * g.ldh, (g.np - n0) * g.ldh * 2, g.ldh, g.d, 0, g.np * g.ldh, wave, lane);
+        tile_begin<B, PL, true, true>(fa, fb, lds, wave, lane);
+    };
+    begin();
+    step_barrier<0>();
+    for (;;) {
+        const int64_t tm0 = m0, tn0 = n0;
+        // what the epilogue needs of this lane's rows (and, a thread per row, of their labels)
+        float lse[NI], k[NI], label_value = 0.0f;
+        int label_at = -1;
+        if constexpr (GRAD == 1) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (m0 + wm + i * 32 + mfma32_row(e, lane) >= words) acc[i][0][e] = acc[i][1][e] = -__builtin_inff();
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int nl = wn + j * 32 + (lane & 31);
-        const int64_t r = n0 + nl;
-        if constexpr (GRAD == 0) {
-            float x = -__builtin_inff();
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x = fmaxf(x, acc[i][j][e]);
-            x = fmaxf(x, __shfl_xor(x, 32));
-            float s = 0.0f;
-            if (ballot(!(fabsf(x) < kScaled)) == 0) {
-                const float z = x * kLog2e;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -z));
-            } else {
-                const float z = x == -__builtin_inff() ? 0.0f : x;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - z) * kLog2e);
+            for (int j = 0; j < NI; ++j) {
+                const int64_t r = tn0 + wn + j * 32 + (lane & 31);
+                lse[j] = r < m ? g.lse[r] : 0.0f;
+                k[j] = r < m ? row_gradient(g.dloss, g.idx, r, m, g.reduction) : 0.0f;
             }
-            s += __shfl_xor(s, 32);
-            if (lane < 32) g.part[((g.v0 + m0) / 128 + (wave >> 2)) * g.np + r] = make_float2(x, s);
-        } else {
-            const bool in = r < m;
-            const float y = in ? g.lse[r] : 0.0f;
-            if (ballot(!(fabsf(y) < kScaled)) != 0) {  // beyond scaling: from here on relative to lse
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) acc[i][j][e] -= y;
-            }
-            const float z = ballot(!(fabsf(y) < kScaled)) != 0 ? 0.0f : y * kLog2e;
-            const float k = in ? row_gradient(g.dloss, g.idx, r, m, g.reduction) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    float v[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) v[q] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e + q], kLog2e, -z)) * k;
-                    put4(lds, nl, wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5), in ? v[0] : 0.0f, in ? v[1] : 0.0f, in ? v[2] : 0.0f,
-                         in ? v[3] : 0.0f);
+            if (tid < B && tn0 + tid < m) {
+                const int64_t r = tn0 + tid, v = (int64_t)g.lab[r] - g.v0 - tm0;
+                if (v >= 0 && v < B) {
+                    label_at = (int)v;
+                    // exp(l - lse) - 1 without the cancellation
+                    label_value = expm1f(g.ll[r] - g.lse[r]) * row_gradient(g.dloss, g.idx, r, m, g.reduction);
                 }
-        }
-    }
-    if constexpr (GRAD == 1) {
-        __syncthreads();
-        // the label's value: exp(l - lse) - 1 without the cancellation
-        if (tid < kTile && n0 + tid < m) {
-            const int64_t r = n0 + tid, v = (int64_t)g.lab[r] - g.v0 - m0;
-            if (v >= 0 && v < kTile) {
-                const float x = expm1f(g.ll[r] - g.lse[r]) * row_gradient(g.dloss, g.idx, r, m, g.reduction);
-                typedef __attribute__((address_space(3))) uint16_t* ptr;
-                *(ptr)(size_t)(lds + tid * 512 + ((((int)v >> 3) ^ (tid & 31)) << 4) + ((int)v & 7) * 2) = f32_to_bf16_bits(x);
             }
         }
-        __syncthreads();
-        tile_to_rows(lds, g.p + n0 * g.ldp + m0, g.ldp, kTile, kTile, tid);
+        f32x16_t acc[MI][NI];
+        tile_run<B, PL, true, true>(fa, fb, (g.d + Ti::kK - 1) / Ti::kK, lds, acc, wave, lane);
+        // the next tile's first step is on its way during the epilogue
+        tile += gridDim.x / 8;
+        const bool more = tile < tiles;
+        if (more) begin();
+        // (hidden from the compiler, which would keep the epilogue's addresses in registers through the products)
+        int el = lane, et = tid;
+        asm volatile("" : "+v"(el), "+v"(et));
+        if constexpr (PL > 1) {
+            uint64_t again[NI] = {};
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (acc[i][j][e] != acc[i][j][e]) again[j] |= 1ull << (i * 16 + e);
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                if (ballot(again[j] != 0) == 0) continue;
+                const int64_t r = tn0 + wn + j * 32 + (el & 31);
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int64_t v = tm0 + wm + i * 32 + mfma32_row(e, el);
+                        if ((again[j] >> (i * 16 + e) & 1) && v < words && r < m) acc[i][j][e] = logit_chain(g, v, r);
+                    }
+            }
+        }
+        // words past the vocabulary
+        if (tm0 + wm + B / 2 > words) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (tm0 + wm + i * 32 + mfma32_row(e, el) >= words)
+#pragma unroll
+                        for (int j = 0; j < NI; ++j) acc[i][j][e] = -__builtin_inff();
+        }
+        if constexpr (GRAD == 0) {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const int64_t r = tn0 + wn + j * 32 + (el & 31);
+                float x = -__builtin_inff();
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x = fmaxf(x, acc[i][j][e]);
+                x = fmaxf(x, __shfl_xor(x, 32));
+                float s = 0.0f;
+                if (ballot(!(fabsf(x) < kScaled)) == 0) {
+                    const float z = x * kLog2e;
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -z));
+                } else {
+                    const float z = x == -__builtin_inff() ? 0.0f : x;
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - z) * kLog2e);
+                }
+                s += __shfl_xor(s, 32);
+                if (el < 32) g.part[((g.v0 + tm0) / (B / 2) + wave / Ti::kWN) * g.np + r] = make_float2(x, s);
+            }
+            if (!more) break;
+            step_barrier<0>();
+        } else {
+            // dl, in place
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const bool in = tn0 + wn + j * 32 + (el & 31) < m;
+                const bool far = ballot(!(fabsf(lse[j]) < kScaled)) != 0;  // beyond scaling: relative to lse first
+                const float z = far ? 0.0f : lse[j] * kLog2e;
+                if (far) {
+#pragma unroll
+                    for (int i = 0; i < MI; ++i)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[i][j][e] -= lse[j];
+                }
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -z)) * k[j];
+                        acc[i][j][e] = in ? v : 0.0f;
+                    }
+            }
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl) {
+                // this plane of the tile, half of its rows at a time; what is left of the values stays in acc
+                uint16_t* out = g.p + pl * g.np * g.ldp + (tm0 / kPanel * g.np + tn0) * kPanel + tm0 % kPanel;
+                float rest = label_value;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (wn / (B / 2) == half) {
+#pragma unroll
+                        for (int j = 0; j < NI; ++j)
+#pragma unroll
+                            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                                for (int e = 0; e < 16; e += 4) {
+                                    uint32_t q[2];
+#pragma unroll
+                                    for (int u = 0; u < 2; ++u) {
+                                        q[u] = pack_bf16x2(acc[i][j][e + 2 * u], acc[i][j][e + 2 * u + 1]);
+                                        if (pl + 1 < PL) {
+                                            acc[i][j][e + 2 * u] -= __uint_as_float(q[u] << 16);
+                                            acc[i][j][e + 2 * u + 1] -= __uint_as_float(q[u] & 0xffff0000u);
+                                        }
+                                    }
+                                    put4<B>(rows_lds, (wn & (B / 2 - 1)) + j * 32 + (el & 31), wm + i * 32 + 8 * (e >> 2) + 4 * (el >> 5), q[0], q[1]);
+                                }
+                    }
+                    // (the first wait covers the next tile's copies too; the stores come after it)
+                    if (pl == 0 && half == 0) step_barrier<0>();
+                    else lds_barrier();
+                    if (label_at >= 0 && et / (B / 2) == half) {
+                        typedef __attribute__((address_space(3))) uint16_t* ptr;
+                        const uint16_t x = f32_to_bf16_bits(rest);
+                        label_value = rest - bf16_bits_to_f32(x);
+                        *(ptr)(size_t)(rows_lds + row_slot<B>(et & (B / 2 - 1), label_at)) = x;
+                    }
+                    lds_barrier();
+                    tile_to_rows<B, B / 2>(rows_lds, out + half * (B / 2) * kPanel, kPanel, B / 2, B, et);
+                    lds_barrier();
+                }
+            }
+            if (!more) break;
+        }
     }
 }
 
-// dW of a piece: the tiles [v][d] of dl^T h, as C[m = d][n = v].
-struct HeadGradArgs {
-    const uint16_t *h, *p;
-    const int32_t* count;
-    int64_t words, np, ldp;
-    uint16_t* dw;  // the piece's first row
-    int d, ldh, m_tiles;
-};
-__global__ __launch_bounds__(kTileThreads, 2) void ce_head_grad_kernel(HeadGradArgs g) {
-    __shared__ __align__(16) char smem[4 * kOperandBytes];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Place at = tile_place(g.m_tiles);
-    const int64_t n0 = at.group * kTile;
-    const int m0 = at.within * kTile;
-    if (n0 >= g.words) return;
-    const uint32_t lds = lds_addr(smem);
-    f32x16_t acc[4][2];
-    {
-        const int64_t rows = round_up(*g.count, kPadRows);  // of h and dl
-        Feed fa, fb;
-        feed_init<false>(fa, g.h + m0, rows * g.ldh * 2 - m0 * 2, g.ldh, 0, g.d - m0, wave, lane);
-        feed_init<false>(fb, g.p + n0, rows * g.ldp * 2 - n0 * 2, g.ldp, 0, kTile, wave, lane);
-        tile_product<false, false>(fa, fb, (*g.count + kStep - 1) / kStep, lds, acc, wave, lane);
-    }
-    const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                put4(lds, wn + j * 32 + (lane & 31), wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5), acc[i][j][e], acc[i][j][e + 1],
-                     acc[i][j][e + 2], acc[i][j][e + 3]);
-    __syncthreads();
-    const int64_t rows = g.words - n0;
-    tile_to_rows(lds, g.dw + n0 * g.d + m0, g.d, rows < kTile ? (int)rows : kTile, g.d - m0, tid);
+// Parts of dh's reduction over a piece of ldp words: a tile for each CU, given the labelled rows' tiles, of at least
+// kPartWords words (a part writes and reads a float32 tile: with one step of 64 each, adding up the 128 parts of a
+// 500 x 256 dh took 38 us, longer than the products).
+constexpr int kPartWords = 256;
+__host__ __device__ inline int dh_parts(int64_t m, int tile, int n_tiles, int64_t ldp, int num_cus) {
+    const int64_t tiles = (m + tile - 1) / tile * n_tiles;
+    const int64_t s = tiles > 0 ? num_cus / tiles : 1, most = ldp / kPartWords;
+    return (int)(s < 1 ? 1 : s < most ? s : most);
 }
 
-// Parts of dh's reduction over a piece: as many as fill the chip, given the labelled rows' tiles.
-__host__ __device__ inline int dh_parts(int64_t m, int n_tiles, int num_cus) {
-    const int64_t tiles = (m + kTile - 1) / kTile * n_tiles;
-    const int64_t s = tiles > 0 ? num_cus / tiles : 1;
-    return (int)(s < 1 ? 1 : s);
-}
-
-// dh of a piece as float32 partial sums [part][m][d], added to when `add`.
-struct RowGradArgs {
-    const uint16_t *p, *w;
+// The gradients of a piece: first the workgroups of dh, float32 partial sums [part][m][d] (added to when `add`), then
+// those of dW, the tiles [v][d] of dl^T h as C[m = d][n = v].  In one launch, the short tiles of dW fill the CUs
+// that the long parts of dh leave, and the other way round.
+struct GradArgs {
+    const uint16_t *p, *h, *w;
     const int32_t* count;
-    int64_t words, ldp;
+    int64_t words, np, ldp, w_plane;
     float* part;
-    int d, n_tiles, num_cus, add;
+    void* dw;  // the piece's first row
+    int d, ldh, cols, num_cus, add;
+    int64_t row_blocks;
 };
-__global__ __launch_bounds__(kTileThreads, 2) void ce_row_grad_kernel(RowGradArgs g) {
-    __shared__ __align__(16) char smem[4 * kOperandBytes];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+template <int B, int PL>
+__device__ __forceinline__ void ce_row_grad(const GradArgs& g, int64_t block, uint32_t lds, int tid) {
+    typedef Tile<B> Ti;
+    constexpr int MI = Ti::kMI, NI = Ti::kNI;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t m = *g.count;
-    const int parts = dh_parts(m, g.n_tiles, g.num_cus);
-    const Place at = tile_place(g.n_tiles);
+    const int parts = dh_parts(m, B, g.cols, g.ldp, g.num_cus);
+    const Place at = tile_place(block, g.cols);
     const int part = (int)(at.group % parts);
-    const int64_t m0 = at.group / parts * kTile;
-    const int n0 = at.within * kTile;
+    const int64_t m0 = at.group / parts * B;
+    const int n0 = at.within * B;
     if (m0 >= m) return;
     const int64_t rows = round_up(m, kPadRows);
-    const int64_t steps = (g.words + kStep - 1) / kStep, per = (steps + parts - 1) / parts;
-    const int64_t s0 = per * part, s1 = s0 + per < steps ? s0 + per : steps;
-    f32x16_t acc[4][2];
+    const int64_t steps = (g.words + Ti::kK - 1) / Ti::kK, per = (steps + parts - 1) / parts;
+    const int64_t s0 = per * part < steps ? per * part : steps, s1 = s0 + per < steps ? s0 + per : steps;
+    f32x16_t acc[MI][NI];
     {
         Feed fa, fb;
-        feed_init<true>(fa, g.p + m0 * g.ldp + s0 * kStep, ((rows - m0) * g.ldp - s0 * kStep) * 2, g.ldp, INT32_MAX, 0, wave, lane);
-        feed_init<false>(fb, g.w + s0 * kStep * g.d + n0, ((g.words - s0 * kStep) * g.d - n0) * 2, g.d, 0, g.d - n0, wave, lane);
-        tile_product<true, false>(fa, fb, s1 - s0, lds_addr(smem), acc, wave, lane);
+        constexpr int64_t kSteps = kPanel / Ti::kK;
+        const int64_t first = (s0 / kSteps * g.np + m0) * kPanel + s0 % kSteps * Ti::kK;
+        feed_init<B, true>(fa, g.p + first, (g.np * g.ldp - first) * 2, kPanel, INT32_MAX, 0, g.np * g.ldp, wave, lane);
+        fa.jump = (g.np - 1) * kPanel * 2;
+        fa.at = fa.at0 = (int)(s0 % kSteps);
+        feed_init<B, false>(fb, g.w + s0 * Ti::kK * g.d + n0, ((g.words - s0 * Ti::kK) * g.d - n0) * 2, g.d, 0, g.d - n0, g.w_plane, wave,
+                            lane);
+        if (s0 < s1) tile_begin<B, PL, true, false>(fa, fb, lds, wave, lane);
+        step_barrier<0>();
+        tile_run<B, PL, true, false>(fa, fb, s1 - s0, lds, acc, wave, lane);
     }
-    const int wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
+    const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
     float* out = g.part + (int64_t)part * rows * g.d;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NI; ++j) {
         const int n = n0 + wn + j * 32 + (lane & 31);
         if (n >= g.d) continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 float* o = out + (m0 + wm + i * 32 + mfma32_row(e, lane)) * g.d + n;
@@ -546,14 +869,61 @@ __global__ __launch_bounds__(kTileThreads, 2) void ce_row_grad_kernel(RowGradArg
     }
 }
 
-// dh in h's rows and type: the sum of the parts, zeros for rows without a label.  A row of `part` has
-// d values; 4 columns a thread.
+template <int B, int PL>
+__device__ __forceinline__ void ce_head_grad(const GradArgs& g, int64_t block, uint32_t lds, int tid) {
+    typedef Tile<B> Ti;
+    constexpr int MI = Ti::kMI, NI = Ti::kNI;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Place at = tile_place(block, g.cols);
+    const int64_t n0 = at.group * B;
+    const int m0 = at.within * B;
+    if (n0 >= g.words) return;
+    f32x16_t acc[MI][NI];
+    {
+        const int64_t rows = round_up(*g.count, kPadRows), steps = (*g.count + Ti::kK - 1) / Ti::kK;
+        Feed fa, fb;
+        feed_init<B, false>(fa, g.h + m0, (rows * g.ldh - m0) * 2, g.ldh, 0, g.d - m0, g.np * g.ldh, wave, lane);
+        feed_init<B, false>(fb, g.p + n0 / kPanel * g.np * kPanel + n0 % kPanel, (rows * kPanel - n0 % kPanel) * 2, kPanel, 0, B,
+                            g.np * g.ldp, wave, lane);
+        if (steps > 0) tile_begin<B, PL, false, false>(fa, fb, lds, wave, lane);
+        step_barrier<0>();
+        tile_run<B, PL, false, false>(fa, fb, steps, lds, acc, wave, lane);
+    }
+    const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
+    const int rows = g.words - n0 < B ? (int)(g.words - n0) : B;
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int n = wn + j * 32 + (lane & 31), mm = wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5);
+                const f32x16_t& a = acc[i][j];
+                if constexpr (PL == 1)
+                    put4<B>(lds, n, mm, pack_bf16x2(a[e], a[e + 1]), pack_bf16x2(a[e + 2], a[e + 3]));
+                else if (n < rows && m0 + mm < g.d)
+                    *reinterpret_cast<float4*>((float*)g.dw + (n0 + n) * g.d + m0 + mm) = make_float4(a[e], a[e + 1], a[e + 2], a[e + 3]);
+            }
+    if constexpr (PL == 1) {
+        lds_barrier();
+        tile_to_rows<B, B>(lds, (uint16_t*)g.dw + n0 * g.d + m0, g.d, rows, g.d - m0, tid);
+    }
+}
+
+template <int B, int PL>
+__global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_grads_kernel(GradArgs g) {
+    __shared__ __align__(16) char smem[Tile<B>::kLds];
+    if (blockIdx.x < g.row_blocks) ce_row_grad<B, PL>(g, blockIdx.x, lds_addr(smem), threadIdx.x);
+    else ce_head_grad<B, PL>(g, blockIdx.x - g.row_blocks, lds_addr(smem), threadIdx.x);
+}
+
+// dh in h's rows and type: the sum of the parts, zeros for rows without a label; 4 columns a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void ce_row_grad_out_kernel(const float* __restrict__ part, const int32_t* __restrict__ count,
-                                                              const int32_t* __restrict__ inv, int64_t n, int d, int n_tiles,
-                                                              int num_cus, int pad, T* __restrict__ dh) {
-    const int64_t m = *count, size = (pad ? round_up(m, kPadRows) : m) * d;
-    const int parts = n_tiles > 0 ? dh_parts(m, n_tiles, num_cus) : 1;
+                                                              const int32_t* __restrict__ inv, int64_t n, int d, int tile, int n_tiles,
+                                                              int64_t ldp, int num_cus, T* __restrict__ dh) {
+    const int64_t m = *count, size = round_up(m, kPadRows) * d;
+    const int parts = dh_parts(m, tile, n_tiles, ldp, num_cus);
     const int64_t total = n * (d / 4);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / (d / 4);
@@ -561,71 +931,39 @@ __global__ __launch_bounds__(256) void ce_row_grad_out_kernel(const float* __res
         const int64_t at = inv[r];
         float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (at >= 0)
-            for (int p = 0; p < parts; ++p) {
-                const float4 v = *reinterpret_cast<const float4*>(part + p * size + at * d + c);
-                s.x += v.x;
-                s.y += v.y;
-                s.z += v.z;
-                s.w += v.w;
+            for (int p0 = 0; p0 < parts; p0 += 4) {
+                float4 v[4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) v[p] = *reinterpret_cast<const float4*>(part + (p0 + p < parts ? p0 + p : p0) * size + at * d + c);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    if (p0 + p >= parts) break;
+                    s.x += v[p].x;
+                    s.y += v[p].y;
+                    s.z += v[p].z;
+                    s.w += v[p].w;
+                }
             }
         if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dh + r * d + c) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
         else *reinterpret_cast<float4*>(dh + r * d + c) = s;
     }
 }
 
-// ------------------------------------------------------------------------ float32: pieces of logits
-// Maximum and sum of a row of a piece's logits [m][ld]; one workgroup per row.
-__global__ __launch_bounds__(256) void ce_piece_stats_kernel(const float* __restrict__ logits, int64_t ld, int64_t words,
-                                                             const int32_t* __restrict__ count, float2* __restrict__ part) {
-    __shared__ MaxSum lds[4];
-    const int64_t r = blockIdx.x;
-    if (r >= *count) return;
-    float x = -__builtin_inff();
-    for (int64_t c = threadIdx.x; c < words; c += 256) x = fmaxf(x, logits[r * ld + c]);
-    const float z = x == -__builtin_inff() ? 0.0f : x;
-    MaxSum a = {x, 0.0f};
-    for (int64_t c = threadIdx.x; c < words; c += 256) a.s += expf(logits[r * ld + c] - z);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = join(a, {__shfl_xor(a.m, o), __shfl_xor(a.s, o)});
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 4; ++w) a = join(a, lds[w]);
-        part[r] = make_float2(a.m, a.s);
-    }
-}
-
-// A piece's logits into dl, in place; the columns up to ld get zeros.
-__global__ __launch_bounds__(256) void ce_piece_grad_kernel(float* __restrict__ logits, int64_t ld, int64_t v0, int64_t words,
-                                                            const int32_t* __restrict__ count, const int32_t* __restrict__ idx,
-                                                            const int32_t* __restrict__ lab, const float* __restrict__ lse,
-                                                            const float* __restrict__ ll, const float* __restrict__ dloss, int reduction) {
-    const int64_t r = blockIdx.x, m = *count;
-    if (r >= m) return;
-    const float g = row_gradient(dloss, idx, r, m, reduction), z = lse[r];
-    const int64_t label = lab[r] - v0;
-    for (int64_t c = threadIdx.x; c < ld; c += 256) {
-        float* p = logits + r * ld + c;
-        *p = c >= words ? 0.0f : g * (c == label ? expm1f(ll[r] - z) : expf(*p - z));
-    }
-}
-
-__global__ __launch_bounds__(256) void ce_add_kernel(float* __restrict__ a, const float* __restrict__ b, const int32_t* __restrict__ count,
-                                                     int d) {
-    const int64_t n = (int64_t)*count * d;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) a[i] += b[i];
-}
-
 // ------------------------------------------------------------------------ sizes
-constexpr size_t kPieceBytes = (size_t)1 << 30;  // of dl or of float32 logits at a time
+constexpr size_t kPieceBytes = (size_t)1 << 30;  // of dl at a time
+
+// Tiles of 256 where they give every CU one, else of 128.
+int tile_for(int64_t rows, int64_t cols, int num_cus) {
+    return cols > 128 && (rows + 255) / 256 * ((cols + 255) / 256) >= num_cus ? 256 : 128;
+}
 
 // Words of the vocabulary in a piece: whole tiles, at most kPieceBytes for all rows.
-int64_t piece_words(int64_t np, int64_t vocab, int elem) {
-    int64_t v = (int64_t)(kPieceBytes / ((size_t)np * elem)) / kTile * kTile;
-    v = v < kTile ? kTile : v;
-    const int64_t all = round_up(vocab, kTile);
+int64_t piece_words(int64_t np, int64_t vocab, int planes) {
+    int64_t v = (int64_t)(kPieceBytes / ((size_t)np * 2 * planes)) / kTileMax * kTileMax;
+    v = v < kTileMax ? kTileMax : v;
+    const int64_t all = round_up(vocab, kTileMax);
     const int64_t pieces = (all + v - 1) / v;
-    return round_up((all + pieces - 1) / pieces, kTile);
+    return round_up((all + pieces - 1) / pieces, kTileMax);
 }
 
 struct Take {
@@ -641,63 +979,77 @@ struct Take {
 struct FwdWs {
     float2* part;
     float* row_loss;
-    float* logits;
-    int n_part;
-    int64_t piece;
+    uint16_t* w;  // float32: W's planes
+    int tile, n_part;
     size_t bytes;
 };
-FwdWs fwd_ws(char* p, int64_t n, int64_t vocab, int dtype) {
+FwdWs fwd_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
     FwdWs w;
     Take take{p};
     const int64_t np = round_up(n, kPadRows);
-    w.piece = dtype == kBF16 ? 0 : piece_words(np, vocab, 4);
-    w.n_part = dtype == kBF16 ? (int)(round_up(vocab, kTile) / 128) : (int)((vocab + w.piece - 1) / w.piece);
+    w.tile = tile_for(vocab, n, num_cus);
+    w.n_part = (int)(round_up(vocab, w.tile) / (w.tile / 2));
     w.part = (float2*)take((size_t)w.n_part * np * 8);
     w.row_loss = (float*)take((size_t)np * 4);
-    w.logits = dtype == kBF16 ? nullptr : (float*)take((size_t)np * w.piece * 4);
+    w.w = dtype == kBF16 ? nullptr : (uint16_t*)take((size_t)vocab * d * 6);
     w.bytes = take.at;
     return w;
 }
 
 struct GradWs {
-    void* p;      // dl of a piece
-    float* part;  // dh: parts, or (float32) the sum and a piece's product
-    float* split;
-    int64_t piece, part_rows;
-    int splits;
+    uint16_t* p;  // dl of a piece
+    float* part;  // dh's parts
+    uint16_t* w;  // float32: W's planes
+    int64_t piece, part_tiles;
+    int logit_tile, grad_tile;
     size_t bytes;
 };
 GradWs grad_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
     GradWs w;
     Take take{p};
     const int64_t np = round_up(n, kPadRows);
-    const int elem = dtype == kBF16 ? 2 : 4;
-    w.piece = piece_words(np, vocab, elem);
-    w.p = take((size_t)np * w.piece * elem);
-    w.split = nullptr;
-    w.splits = 1;
-    if (dtype == kBF16) {
-        // parts x rows for any count of labelled rows: at most a tile per CU, or one part
-        const int64_t cols = round_up(d, kTile) / kTile;
-        const int64_t most = num_cus / cols > np / kTile ? num_cus / cols : np / kTile;
-        w.part_rows = most * kTile;
-        w.part = (float*)take((size_t)w.part_rows * d * 4);
-    } else {
-        w.part_rows = np;
-        w.part = (float*)take((size_t)np * d * 4 * 2);
-        w.splits = gemm_split(np, d, w.piece, num_cus);
-        w.split = (float*)take((size_t)w.splits * np * d * 4);
-    }
+    const int planes = planes_of(dtype);
+    w.piece = piece_words(np, vocab, planes);
+    const int64_t words = vocab < w.piece ? vocab : w.piece;
+    w.logit_tile = tile_for(words, n, num_cus);
+    // tiles of 256 for the gradients where dW's and dh's parts give every CU one
+    const int64_t cols256 = (d + 255) / 256, m256 = (n + 255) / 256 * cols256;
+    const int64_t row256 = m256 * (num_cus / m256 < 1 ? 1 : num_cus / m256 < w.piece / kPartWords ? num_cus / m256 : w.piece / kPartWords);
+    w.grad_tile = d > 128 && (words + 255) / 256 * cols256 + row256 >= num_cus ? 256 : 128;
+    w.p = (uint16_t*)take((size_t)np * w.piece * 2 * planes);
+    // parts x tiles of rows for any count of labelled rows: as many as fill the chip, or one part
+    const int64_t cols = (d + w.grad_tile - 1) / w.grad_tile, slots = num_cus / cols;
+    w.part_tiles = slots > np / w.grad_tile ? slots : np / w.grad_tile;
+    // a part has the padded rows, up to two tiles of 128 for one
+    w.part = (float*)take((size_t)w.part_tiles * kTileMax * d * 4);
+    w.w = dtype == kBF16 ? nullptr : (uint16_t*)take((size_t)vocab * d * 6);
     w.bytes = take.at;
     return w;
 }
 
 unsigned xcd_grid(int64_t groups, int each) { return (unsigned)((groups + 7) / 8 * 8 * each); }
 
-LogitArgs logit_args(const CeState& s, const void* w, int64_t v0, int64_t v1, int d, int64_t n) {
+// f(tile, planes) with both as constants.
+template <int V> struct Int {
+    static constexpr int v = V;
+};
+template <typename F>
+void with_tile(int tile, int dtype, F f) {
+    if (dtype == kBF16) {
+        if (tile == 256) f(Int<256>{}, Int<1>{});
+        else f(Int<128>{}, Int<1>{});
+    } else {
+        if (tile == 256) f(Int<256>{}, Int<3>{});
+        else f(Int<128>{}, Int<3>{});
+    }
+}
+
+LogitArgs logit_args(const CeState& s, const void* w, const uint16_t* planes, int64_t v0, int64_t v1, int64_t vocab, int d, int dtype) {
     LogitArgs g{};
-    g.w = (const uint16_t*)w + v0 * d;
-    g.h = (const uint16_t*)s.h;
+    g.w = (dtype == kBF16 ? (const uint16_t*)w : planes) + v0 * d;
+    g.w32 = dtype == kBF16 ? nullptr : (const float*)w + v0 * d;
+    g.w_plane = vocab * d;
+    g.h = s.h;
     g.count = s.count;
     g.idx = s.idx;
     g.lab = s.lab;
@@ -708,29 +1060,32 @@ LogitArgs logit_args(const CeState& s, const void* w, int64_t v0, int64_t v1, in
     g.np = s.np;
     g.d = d;
     g.ldh = s.ldh;
-    g.n_tiles = (int)((n + kTile - 1) / kTile);
     return g;
 }
 
-Gemm logits_gemm(const CeState& s, const float* w, int64_t n, int d, int64_t words, float* out, int64_t ld) {
-    Gemm g;
-    g.a = s.h;
-    g.lda = s.ldh;
-    g.b = w;
-    g.ldb = d;
-    g.c = out;
-    g.ldc = ld;
-    g.m = n;
-    g.n = (int)words;
-    g.k = d;
-    g.dyn = s.count;
-    return g;
+template <int GRAD>
+void run_logits(const LogitArgs& g, int tile, int dtype, int64_t n, int num_cus, hipStream_t stream) {
+    // as many workgroups as run at once (one to a CU, or two of tiles of 128)
+    const int64_t tiles = xcd_grid((g.v1 - g.v0 + tile - 1) / tile, (int)((n + tile - 1) / tile));
+    const int64_t most = round_up(num_cus, 8) * (tile == 256 ? 1 : 2);
+    const dim3 grid((unsigned)(tiles < most ? tiles : most));
+    with_tile(tile, dtype, [&](auto b, auto pl) {
+        constexpr int B = decltype(b)::v, PL = decltype(pl)::v;
+        hipLaunchKernelGGL((ce_logits_kernel<B, PL, GRAD>), grid, dim3(Tile<B>::kThreads), 0, stream, g);
+    });
+}
+
+void split_weights(const void* w, int64_t vocab, int d, uint16_t* out, int num_cus, hipStream_t stream) {
+    const int64_t n8 = vocab * d / 8, b = (n8 + 255) / 256;
+    hipLaunchKernelGGL(ce_split_kernel, dim3((unsigned)(b < num_cus * 16 ? b : num_cus * 16)), dim3(256), 0, stream, (const float*)w, n8, out);
 }
 
 }  // namespace
 
 size_t linear_ce_state_bytes(int64_t n, int d, int dtype) { return ce_state(nullptr, n, d, dtype).bytes; }
-size_t linear_ce_workspace_bytes(int64_t n, int, int64_t vocab, int dtype) { return fwd_ws(nullptr, n, vocab, dtype).bytes; }
+size_t linear_ce_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
+    return fwd_ws(nullptr, n, d, vocab, dtype, num_cus).bytes;
+}
 size_t linear_ce_grad_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
     return grad_ws(nullptr, n, d, vocab, dtype, num_cus).bytes;
 }
@@ -738,32 +1093,32 @@ size_t linear_ce_grad_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype
 int launch_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* labels, int64_t n, int d, int64_t vocab,
                      int64_t ignore, int reduction, int dtype, void* state, void* ws, float* loss, int num_cus, hipStream_t stream) {
     const CeState s = ce_state((char*)state, n, d, dtype);
-    const FwdWs f = fwd_ws((char*)ws, n, vocab, dtype);
-    float* rows = reduction == kLossNone ? loss : nullptr;
-    hipLaunchKernelGGL(ce_rows_kernel, dim3(1), dim3(1024), 0, stream, labels, n, vocab, ignore, s.count, s.idx, s.inv, s.lab, rows);
+    const FwdWs f = fwd_ws((char*)ws, n, d, vocab, dtype, num_cus);
+    float* loss_rows = reduction == kLossNone ? loss : nullptr;
     const dim3 gg((unsigned)(s.np / 4));
-    if (dtype == kBF16) {
-        hipLaunchKernelGGL((ce_gather_kernel<uint16_t>), gg, dim3(256), 0, stream, (const uint16_t*)h, ldh, (const uint16_t*)w, s.count,
-                           s.idx, s.lab, d, s.ldh, (uint16_t*)s.h, s.ll);
-        LogitArgs g = logit_args(s, w, 0, vocab, d, n);
-        g.part = f.part;
-        hipLaunchKernelGGL((ce_logits_kernel<0>), dim3(xcd_grid((vocab + kTile - 1) / kTile, g.n_tiles)), dim3(kTileThreads), 0, stream,
-                           g);
-    } else {
-        hipLaunchKernelGGL((ce_gather_kernel<float>), gg, dim3(256), 0, stream, (const float*)h, ldh, (const float*)w, s.count, s.idx,
-                           s.lab, d, s.ldh, (float*)s.h, s.ll);
-        for (int e = 0; e < f.n_part; ++e) {
-            const int64_t v0 = e * f.piece, words = vocab - v0 < f.piece ? vocab - v0 : f.piece;
-            const int rc = launch_gemm(kGemmFK_FK, logits_gemm(s, (const float*)w + v0 * d, n, d, words, f.logits, f.piece), num_cus, stream);
-            if (rc != 0) return rc;
-            hipLaunchKernelGGL(ce_piece_stats_kernel, dim3((unsigned)n), dim3(256), 0, stream, f.logits, f.piece, words, s.count,
-                               f.part + e * s.np);
+    auto gather = [&](const auto* hh, const auto* ww) {
+        typedef typename std::decay<decltype(*hh)>::type T;
+        if (n <= kFewRows) {
+            hipLaunchKernelGGL((ce_few_rows_kernel<T>), gg, dim3(256), 0, stream, labels, (int)n, vocab, ignore, hh, ldh, ww, s.count, s.idx,
+                               s.inv, s.lab, loss_rows, s.ticket, d, s.ldh, s.np * s.ldh, s.h, s.ll);
+            return;
         }
+        hipLaunchKernelGGL(ce_rows_kernel, dim3(1), dim3(1024), 0, stream, labels, n, vocab, ignore, s.count, s.idx, s.inv, s.lab, loss_rows,
+                           s.ticket);
+        hipLaunchKernelGGL((ce_gather_kernel<T>), gg, dim3(256), 0, stream, hh, ldh, ww, s.count, s.idx, s.lab, d, s.ldh, s.np * s.ldh, s.h,
+                           s.ll);
+    };
+    if (dtype == kBF16) {
+        gather((const uint16_t*)h, (const uint16_t*)w);
+    } else {
+        gather((const float*)h, (const float*)w);
+        split_weights(w, vocab, d, f.w, num_cus, stream);
     }
-    hipLaunchKernelGGL(ce_lse_kernel, dim3((unsigned)(s.np / 64)), dim3(256), 0, stream, f.part, f.n_part, s.np, s.count, s.idx, s.ll,
-                       s.lse, rows, f.row_loss);
-    if (!rows)
-        hipLaunchKernelGGL(ce_total_kernel, dim3(1), dim3(1024), 0, stream, f.row_loss, s.count, reduction == kLossMean ? 1 : 0, loss);
+    LogitArgs g = logit_args(s, w, f.w, 0, vocab, vocab, d, dtype);
+    g.part = f.part;
+    run_logits<0>(g, f.tile, dtype, n, num_cus, stream);
+    hipLaunchKernelGGL(ce_lse_kernel, dim3((unsigned)(s.np / 16)), dim3(1024), 0, stream, f.part, f.n_part, s.np, s.count, s.idx, s.ll,
+                       reduction, s.lse, f.row_loss, s.ticket, loss);
     return (int)hipGetLastError();
 }
 
@@ -771,81 +1126,34 @@ int launch_linear_ce_grad(const void* state, const void* w, const float* dloss, 
                           int dtype, void* ws, void* dh, void* dw, int num_cus, hipStream_t stream) {
     const CeState s = ce_state((char*)state, n, d, dtype);
     const GradWs b = grad_ws((char*)ws, n, d, vocab, dtype, num_cus);
-    const int cols = (d + kTile - 1) / kTile;
-    const int64_t m_tiles = (n + kTile - 1) / kTile;
+    const int cols = (d + b.grad_tile - 1) / b.grad_tile;
+    if (dtype != kBF16) split_weights(w, vocab, d, b.w, num_cus, stream);
     for (int64_t v0 = 0; v0 < vocab; v0 += b.piece) {
         const int64_t words = vocab - v0 < b.piece ? vocab - v0 : b.piece;
-        if (dtype == kBF16) {
-            LogitArgs g = logit_args(s, w, v0, v0 + words, d, n);
-            g.p = (uint16_t*)b.p;
-            g.ldp = b.piece;
-            g.dloss = dloss;
-            g.reduction = reduction;
-            hipLaunchKernelGGL((ce_logits_kernel<1>), dim3(xcd_grid((words + kTile - 1) / kTile, g.n_tiles)), dim3(kTileThreads), 0, stream,
-                               g);
-            if (dw) {
-                const HeadGradArgs a{(const uint16_t*)s.h, (const uint16_t*)b.p, s.count, words, s.np, b.piece, (uint16_t*)dw + v0 * d,
-                                     d, s.ldh, cols};
-                hipLaunchKernelGGL(ce_head_grad_kernel, dim3(xcd_grid((words + kTile - 1) / kTile, cols)), dim3(kTileThreads), 0, stream, a);
-            }
-            if (dh) {
-                const RowGradArgs a{(const uint16_t*)b.p, (const uint16_t*)w + v0 * d, s.count, words, b.piece, b.part, d, cols, num_cus,
-                                    v0 > 0 ? 1 : 0};
-                hipLaunchKernelGGL(ce_row_grad_kernel, dim3(xcd_grid(b.part_rows / kTile, cols)), dim3(kTileThreads), 0, stream, a);
-            }
-        } else {
-            const float* wp = (const float*)w + v0 * d;
-            float* p = (float*)b.p;
-            int rc = launch_gemm(kGemmFK_FK, logits_gemm(s, wp, n, d, words, p, b.piece), num_cus, stream);
-            if (rc != 0) return rc;
-            hipLaunchKernelGGL(ce_piece_grad_kernel, dim3((unsigned)n), dim3(256), 0, stream, p, b.piece, v0, words, s.count, s.idx, s.lab,
-                               s.lse, s.ll, dloss, reduction);
-            if (dw) {
-                Gemm g;
-                g.a = p;
-                g.lda = b.piece;
-                g.b = s.h;
-                g.ldb = s.ldh;
-                g.c = (float*)dw + v0 * d;
-                g.ldc = d;
-                g.m = words;
-                g.n = d;
-                g.k = n;
-                g.dyn = s.count;
-                g.dyn_k = true;
-                rc = launch_gemm(kGemmFR_FR, g, num_cus, stream);
-                if (rc != 0) return rc;
-            }
-            if (dh) {
-                Gemm g;
-                g.a = p;
-                g.lda = b.piece;
-                g.b = wp;
-                g.ldb = d;
-                g.c = b.part + (v0 > 0 ? s.np * d : 0);
-                g.ldc = d;
-                g.m = n;
-                g.n = d;
-                g.k = words;
-                g.split = b.splits;
-                g.part = b.split;
-                g.dyn = s.count;
-                rc = launch_gemm(kGemmFK_FR, g, num_cus, stream);
-                if (rc != 0) return rc;
-                if (v0 > 0)
-                    hipLaunchKernelGGL(ce_add_kernel, dim3((unsigned)(num_cus * 8)), dim3(256), 0, stream, b.part, b.part + s.np * d, s.count, d);
-            }
-        }
+        LogitArgs g = logit_args(s, w, b.w, v0, v0 + words, vocab, d, dtype);
+        g.p = b.p;
+        g.ldp = b.piece;
+        g.dloss = dloss;
+        g.reduction = reduction;
+        run_logits<1>(g, b.logit_tile, dtype, n, num_cus, stream);
+        const int64_t row_blocks = dh ? xcd_grid(b.part_tiles, cols) : 0;
+        const int64_t head_blocks = dw ? xcd_grid((words + b.grad_tile - 1) / b.grad_tile, cols) : 0;
+        const GradArgs a{b.p, s.h, g.w, s.count, words, s.np, b.piece, g.w_plane, b.part, (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4), d,
+                         s.ldh, cols, num_cus, v0 > 0 ? 1 : 0, row_blocks};
+        with_tile(b.grad_tile, dtype, [&](auto t, auto pl) {
+            constexpr int B = decltype(t)::v, PL = decltype(pl)::v;
+            hipLaunchKernelGGL((ce_grads_kernel<B, PL>), dim3((unsigned)(row_blocks + head_blocks)), dim3(Tile<B>::kThreads), 0, stream, a);
+        });
     }
     if (dh) {
         int64_t blocks = (n * (d / 4) + 255) / 256;
         blocks = blocks < num_cus * 16 ? blocks : num_cus * 16;
         if (dtype == kBF16)
             hipLaunchKernelGGL((ce_row_grad_out_kernel<uint16_t>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, n,
-                               d, cols, num_cus, 1, (uint16_t*)dh);
+                               d, b.grad_tile, cols, b.piece, num_cus, (uint16_t*)dh);
         else
             hipLaunchKernelGGL((ce_row_grad_out_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, n, d,
-                               0, num_cus, 0, (float*)dh);
+                               b.grad_tile, cols, b.piece, num_cus, (float*)dh);
     }
     return (int)hipGetLastError();
 }

@@ -1038,6 +1038,13 @@ __global__ __launch_bounds__(kSmallWaves * 64) void sort_small_kernel(const int3
                     max_unique);
 }
 
+// Part `b` of `parts` of a fill with zeros; 16-byte stores, the last bytes one at a time.
+__device__ __forceinline__ void zero_fill(unsigned char* p, int64_t bytes, int b, int parts) {
+    const int64_t n16 = bytes / 16, step = (int64_t)parts * 1024;
+    for (int64_t i = (int64_t)b * 1024 + threadIdx.x; i < n16; i += step) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+    if (b == 0 && threadIdx.x < bytes % 16) p[n16 * 16 + threadIdx.x] = 0;
+}
+
 // The small sort in workgroup 0 and the bf16 token projection xp = RN(x W_u) in the
 // others (tile b - 1: column tile (b - 1) % nct, token tile (b - 1) / nct), which needs
 // only x: the tiles run on CUs the single sorting workgroup leaves idle.
@@ -1057,6 +1064,49 @@ __global__ __launch_bounds__(kSmallWaves * 64) void sort_small_tp_kernel(
         const int b = (int)blockIdx.x - 1;
         token_proj_bf16_tile(lds, x, wut, n_tok, d, dh, xp, (b % nct) * kTpCols, (b / nct) * kTpRows);
     }
+}
+
+// The small sort in workgroup 0 and zeros over a 16-byte-aligned array in the others.
+__global__ __launch_bounds__(kSmallWaves * 64) void sort_small_zero_kernel(
+    const int32_t* __restrict__ ids, int n, int key_bits_, int vb, int passes, int32_t* __restrict__ perm,
+    int32_t* __restrict__ uniq, int32_t* __restrict__ seg_off, int32_t* __restrict__ pair_slot,
+    int32_t* __restrict__ sorted_slot, int32_t* __restrict__ n_unique, int32_t max_unique, unsigned char* __restrict__ zeros,
+    int64_t zero_bytes) {
+    __shared__ __align__(16) unsigned char lds[kSmallLds];
+    if (blockIdx.x == 0)
+        sort_small_body(lds, ids, n, key_bits_, vb, passes, perm, uniq, seg_off, pair_slot, sorted_slot, n_unique, max_unique);
+    else
+        zero_fill(zeros, zero_bytes, (int)blockIdx.x - 1, (int)gridDim.x - 1);
+}
+
+__global__ __launch_bounds__(1024) void zero_kernel(unsigned char* __restrict__ zeros, int64_t zero_bytes) {
+    zero_fill(zeros, zero_bytes, blockIdx.x, gridDim.x);
+}
+
+int launch_zero(void* p, int64_t bytes, int num_cus, hipStream_t stream) {
+    const int64_t b = (bytes + 65535) / 65536;
+    if (bytes > 0)
+        hipLaunchKernelGGL(zero_kernel, dim3((unsigned)(b < num_cus * 2 ? b : num_cus * 2)), dim3(1024), 0, stream, (unsigned char*)p, bytes);
+    return (int)hipGetLastError();
+}
+
+int launch_sort_segment_zero(const int32_t* ids, int64_t n, int64_t n_experts, void* ws, int32_t* perm, int32_t* uniq,
+                             int32_t* seg_off, int32_t* pair_slot, int32_t* sorted_slot, int32_t* n_unique, void* zeros,
+                             int64_t zero_bytes, int num_cus, hipStream_t stream) {
+    const int bits = sort_key_bits(n_experts);
+    int vb = 0;
+    while (vb < 31 && ((int64_t)1 << vb) < n) ++vb;
+    if (n <= kSmallMax && bits + vb <= 32) {
+        // one workgroup of zeros per CU that the sort leaves idle (each holds the sort's LDS)
+        const int64_t b = (zero_bytes + 65535) / 65536, most = num_cus > 1 ? num_cus - 1 : 1;
+        hipLaunchKernelGGL(sort_small_zero_kernel, dim3((unsigned)(1 + (b < most ? b : most))), dim3(kSmallWaves * 64), 0, stream, ids,
+                           (int)n, bits, vb, sort_passes(n_experts), perm, uniq, seg_off, pair_slot, sorted_slot, n_unique,
+                           (int32_t)(n < n_experts ? n : n_experts), (unsigned char*)zeros, zero_bytes);
+        return (int)hipGetLastError();
+    }
+    const int rc = launch_zero(zeros, zero_bytes, num_cus, stream);
+    return rc != 0 ? rc
+                   : launch_sort_segment(ids, n, n_experts, ws, perm, uniq, seg_off, pair_slot, sorted_slot, n_unique, stream);
 }
 
 int launch_sort_segment_tp(const int32_t* ids, int64_t n, int64_t n_experts, int32_t* perm, int32_t* uniq,

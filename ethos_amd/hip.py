@@ -699,28 +699,29 @@ def linear_ce_grad(state: torch.Tensor, w: torch.Tensor, dloss: torch.Tensor, n:
     return dh, dw
 
 
-def embedding(ids: torch.Tensor, w: torch.Tensor, scale: float) -> torch.Tensor:
-    """Rows scale * w[ids], [*ids.shape, d]."""
+def embedding(ids: torch.Tensor, w: torch.Tensor, scale: float, padding: int = -1, want_keys: bool = False):
+    """(rows scale * w[ids] [*ids.shape, d], keys): the keys (int32, or None) are what embedding_grad
+    takes; positions of id `padding` have none."""
     _need_here(ids, "ids", INTS)
     _need_here(w, "weight", FLOATS, 2)
     V, d = w.shape
     out = torch.empty((*ids.shape, d), dtype=w.dtype, device=w.device)
-    rc = load().ethos_embedding(ids.data_ptr(), int(ids.dtype == torch.int64), w.data_ptr(), ids.numel(), d, V, scale,
-                                dtype_code(w.dtype), out.data_ptr(), _stream())
+    keys = torch.empty(ids.shape, dtype=torch.int32, device=w.device) if want_keys else None
+    rc = load().ethos_embedding(ids.data_ptr(), ids.dtype == torch.int64, w.data_ptr(), ids.numel(), d, V, scale, padding,
+                                dtype_code(w.dtype), out.data_ptr(), keys.data_ptr() if want_keys else None, _stream())
     check(rc, "ethos_embedding")
-    return out
+    return out, keys
 
 
-def embedding_grad(ids: torch.Tensor, dy: torch.Tensor, vocab: int, scale: float, padding: int) -> torch.Tensor:
-    """The table's gradient [vocab, d] from dy [*ids.shape, d]; positions of id `padding` are left out."""
-    _need_here(ids, "ids", INTS)
+def embedding_grad(keys: torch.Tensor, dy: torch.Tensor, vocab: int, scale: float) -> torch.Tensor:
+    """The table's gradient [vocab, d] from dy [*keys.shape, d] and the lookup's keys."""
     _need_here(dy, "dy", FLOATS)
-    n, d = ids.numel(), dy.shape[-1]
+    n, d = keys.numel(), dy.shape[-1]
     lib = load()
     ws, ws_bytes = workspace(lib.ethos_embedding_grad_workspace_bytes(n, d, vocab), dy.device)
     dw = torch.empty((vocab, d), dtype=dy.dtype, device=dy.device)
-    rc = lib.ethos_embedding_grad(ids.data_ptr(), int(ids.dtype == torch.int64), dy.data_ptr(), n, d, vocab, scale, padding,
-                                  dtype_code(dy.dtype), ws.data_ptr(), ws_bytes, dw.data_ptr(), _stream())
+    rc = lib.ethos_embedding_grad(keys.data_ptr(), dy.data_ptr(), n, d, vocab, scale, dtype_code(dy.dtype), ws.data_ptr(), ws_bytes,
+                                  dw.data_ptr(), _stream())
     check(rc, "ethos_embedding_grad")
     return dw
 
@@ -732,7 +733,7 @@ def balance(gates: torch.Tensor, ids: torch.Tensor, n_experts: int):
     H, k = gates.shape[-2:]
     n = gates.numel() // (H * k)
     lib = load()
-    ws, ws_bytes = workspace(lib.ethos_balance_workspace_bytes(n, H, k), gates.device)
+    ws, ws_bytes = workspace(lib.ethos_balance_workspace_bytes(n, H, k, n_experts), gates.device)
     counts = torch.empty((n_experts,), dtype=torch.int32, device=gates.device)
     loss = torch.empty((), dtype=torch.float32, device=gates.device)
     rc = lib.ethos_balance(gates.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), n, H, k, n_experts, dtype_code(gates.dtype),

@@ -109,15 +109,14 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, ids, scale, padding):
-        ctx.save_for_backward(ids)
-        ctx.vocab, ctx.scale, ctx.padding = weight.shape[0], scale, padding
-        return hip.embedding(ids, weight.detach().contiguous(), scale)
+        out, keys = hip.embedding(ids, weight.detach().contiguous(), scale, padding, True)
+        ctx.keys, ctx.vocab, ctx.scale = keys, weight.shape[0], scale  # keys: this node's own tensor
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        (ids,) = ctx.saved_tensors
-        return hip.embedding_grad(ids, _dense(dy), ctx.vocab, ctx.scale, ctx.padding), None, None, None
+        return hip.embedding_grad(ctx.keys, _dense(dy), ctx.vocab, ctx.scale), None, None, None
 
 
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
@@ -141,7 +140,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     ids = ids.contiguous()
     if torch.is_grad_enabled() and weight.requires_grad:
         return _Embedding.apply(weight, ids, float(scale), padding)
-    return hip.embedding(ids, weight.detach().contiguous(), float(scale))
+    return hip.embedding(ids, weight.detach().contiguous(), float(scale))[0]
 
 
 # -------------------------------------------------------------------------- balance

@@ -535,18 +535,20 @@ int ethos_linear_ce_grad(const void* state, size_t state_bytes, const void* w, c
 
 /*
  * Embedding rows (the lookup of model.py:390): out[i] = RN_T(scale w[ids[i]]), and the table's
- * gradient dw[v] = RN_T(scale sum over {i: ids[i] = v} dy[i]), float32 sums in the order of i; every
+ * gradient dw[v] = RN_T(scale sum over {i: ids[i] = v} dy[i]), float32 sums in a fixed order; every
  * row of dw is written.  ids: int32, or int64 with ids_64; an id outside [0, vocab) gives a row of
  * NaN and has no part in the gradient, nor have positions whose id is `padding` (negative: none).
- *   w, dw [vocab, d], dy, out [n, d] dtype T, at any address a T may have; dy and dw 16-byte aligned
+ *   w, out [vocab, d], [n, d] dtype T, at any address a T may have; dy [n, d], dw [vocab, d] 16-byte aligned
+ *   keys   [n] int32, written by ethos_embedding unless NULL, read by ethos_embedding_grad: the id, or
+ *          vocab where a position has no part in the gradient
  *   workspace  >= ethos_embedding_grad_workspace_bytes(...) bytes, 16-byte aligned (scratch)
  * Limits: n, d, vocab < 2^31 - 1.
  */
-int ethos_embedding(const void* ids, int32_t ids_64, const void* w, int64_t n, int32_t d, int64_t vocab, float scale, int32_t dtype,
-                    void* out, void* stream);
+int ethos_embedding(const void* ids, int32_t ids_64, const void* w, int64_t n, int32_t d, int64_t vocab, float scale, int64_t padding,
+                    int32_t dtype, void* out, int32_t* keys, void* stream);
 size_t ethos_embedding_grad_workspace_bytes(int64_t n, int32_t d, int64_t vocab);
-int ethos_embedding_grad(const void* ids, int32_t ids_64, const void* dy, int64_t n, int32_t d, int64_t vocab, float scale,
-                         int64_t padding, int32_t dtype, void* workspace, size_t workspace_bytes, void* dw, void* stream);
+int ethos_embedding_grad(const int32_t* keys, const void* dy, int64_t n, int32_t d, int64_t vocab, float scale, int32_t dtype,
+                         void* workspace, size_t workspace_bytes, void* dw, void* stream);
 
 /*
  * How often each expert was chosen, and a load-balance loss of the routing (none in the reference):
@@ -558,7 +560,7 @@ int ethos_embedding_grad(const void* ids, int32_t ids_64, const void* dy, int64_
  *   workspace  >= ethos_balance_workspace_bytes(...) bytes, 16-byte aligned (scratch)
  * No tokens: counts and loss are zero.  Limits: n_tok n_heads top_k < 2^31, n_experts < 2^31.
  */
-size_t ethos_balance_workspace_bytes(int64_t n_tok, int32_t n_heads, int32_t top_k);
+size_t ethos_balance_workspace_bytes(int64_t n_tok, int32_t n_heads, int32_t top_k, int64_t n_experts);
 int ethos_balance(const void* gates, const void* ids, int32_t ids_64, int64_t n_tok, int32_t n_heads, int32_t top_k, int64_t n_experts,
                   int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* counts, float* loss, void* stream);
 int ethos_balance_grad(const void* ids, int32_t ids_64, const int32_t* counts, const float* dloss, int64_t n_tok, int32_t n_heads,

@@ -44,13 +44,13 @@ def test_linear_ce_argument_errors_are_codes():
 def test_embedding_balance_and_clip_argument_errors_are_codes():
     L = _lib.load()
     big, top = 1 << 40, 2 ** 31 - 1
-    emb = lambda ids=16, w=16, n=4, d=8, V=9, dt=1, out=16: L.ethos_embedding(ids, 1, w, n, d, V, 1.0, dt, out, None)  # noqa: E731
+    emb = lambda ids=16, w=16, n=4, d=8, V=9, dt=1, out=16: L.ethos_embedding(ids, 1, w, n, d, V, 1.0, -1, dt, out, None, None)  # noqa: E731
     assert emb(dt=3) == -1 and emb(n=-1) == -2 and emb(d=0) == -2 and emb(V=0) == -2 and emb(V=top) == -2 and emb(n=top) == -2
     assert emb(ids=None) == -3 and emb(w=None) == -3 and emb(out=None) == -3 and emb(w=17) == -4 and emb(out=18, dt=0) == -4
     assert emb(n=0, ids=None) == 0
 
     def egrad(ids=16, dy=16, n=4, d=8, V=9, dt=1, ws=16, ws_bytes=big, dw=16):
-        return L.ethos_embedding_grad(ids, 1, dy, n, d, V, 1.0, -1, dt, ws, ws_bytes, dw, None)
+        return L.ethos_embedding_grad(ids, dy, n, d, V, 1.0, dt, ws, ws_bytes, dw, None)
 
     assert egrad(dt=3) == -1 and egrad(V=0) == -2 and egrad(ids=None) == -3 and egrad(dy=None) == -3 and egrad(dw=None) == -3
     assert egrad(dy=24) == -4 and egrad(dw=24) == -4 and egrad(ws=8) == -4
@@ -63,7 +63,7 @@ def test_embedding_balance_and_clip_argument_errors_are_codes():
     assert bal(n=1 << 20, H=1 << 10, k=4) == -2 and bal(n=top, H=top, k=top) == -2
     for name in ("g", "ids", "ws", "c", "loss"):
         assert bal(**{name: None}) == -3, name
-    assert bal(ws=8) == -4 and bal(g=17) == -4 and bal(ws_bytes=L.ethos_balance_workspace_bytes(4, 2, 3) - 1) == -5
+    assert bal(ws=8) == -4 and bal(g=17) == -4 and bal(ws_bytes=L.ethos_balance_workspace_bytes(4, 2, 3, 5) - 1) == -5
     bgrad = lambda ids=16, c=16, dl=16, n=4, dt=1, out=16: L.ethos_balance_grad(ids, 1, c, dl, n, 2, 3, 5, dt, out, None)  # noqa: E731
     assert bgrad(dt=9) == -1 and bgrad(n=-1) == -2 and bgrad(out=17) == -4 and bgrad(n=0, ids=None) == 0
     for name in ("ids", "c", "dl", "out"):
