@@ -41,14 +41,28 @@ template <typename T, typename F>
 __device__ __forceinline__ void clip_values(const T* p, int64_t n, F f) {
     constexpr int N = Vec16<T>::kN;
     if (((uintptr_t)p & 15u) == 0) {
+        typedef typename Vec16<T>::raw Raw;
         const int64_t whole = n / N;
-        for (int64_t i = threadIdx.x; i < whole; i += 256) {
+        int64_t i = threadIdx.x;
+        for (; i + 3 * 256 < whole; i += 4 * 256) {  // four loads on their way
+            Raw r[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) r[c] = reinterpret_cast<const Raw*>(p)[i + c * 256];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float v[N];
+                Vec16<T>::unpack(r[c], v);
+#pragma unroll
+                for (int j = 0; j < N; ++j) f(v[j]);
+            }
+        }
+        for (; i < whole; i += 256) {
             float v[N];
-            Vec16<T>::unpack(reinterpret_cast<const typename Vec16<T>::raw*>(p)[i], v);
+            Vec16<T>::unpack(reinterpret_cast<const Raw*>(p)[i], v);
 #pragma unroll
             for (int j = 0; j < N; ++j) f(v[j]);
         }
-        for (int64_t i = whole * N + threadIdx.x; i < n; i += 256) f(Elem<T>::to_f32(p[i]));
+        for (i = whole * N + threadIdx.x; i < n; i += 256) f(Elem<T>::to_f32(p[i]));
     } else {
         for (int64_t i = threadIdx.x; i < n; i += 256) f(Elem<T>::to_f32(p[i]));
     }

@@ -4,7 +4,9 @@ tensors and raises on anything else -- there is no CPU path.
 """
 from __future__ import annotations
 
+import array
 import ctypes
+import functools
 
 import torch
 
@@ -657,11 +659,23 @@ def mla_attention(q: torch.Tensor, kv: torch.Tensor, k_rot: torch.Tensor, positi
 # ----------------------------------------------------------- operators of a training step
 def _need_here(t: torch.Tensor, name: str, dtypes, dim=None) -> None:
     """_need, with one of several dtypes and on the current device."""
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.is_contiguous() and (dim is None or t.dim() == dim)
+            and t.get_device() == _current_device()):
+        return
     _need(t, name, dim=dim)
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if t.device.index != _current_device():
-        raise RuntimeError(f"{name} is on {t.device}, not on the current device")
+    raise RuntimeError(f"{name} is on {t.device}, not on the current device")
+
+
+@functools.lru_cache(maxsize=1024)
+def _size(name: str, device: int, *args: int) -> int:
+    """A workspace size function's answer (`device`: some depend on the GPU's CUs)."""
+    return getattr(load(), name)(*args)
+
+
+def _scratch(name: str, device: torch.device, *args: int):
+    return workspace(_size(name, device.index, *args), device)
 
 
 FLOATS = (torch.bfloat16, torch.float32)
@@ -676,8 +690,8 @@ def linear_ce(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, ignore_ind
     n, d = h.shape
     code, lib = dtype_code(h.dtype), load()
     V = w.shape[0]
-    st, st_bytes = workspace(lib.ethos_linear_ce_state_bytes(n, d, code), h.device)
-    ws, ws_bytes = workspace(lib.ethos_linear_ce_workspace_bytes(n, d, V, code), h.device)
+    st, st_bytes = _scratch("ethos_linear_ce_state_bytes", h.device, n, d, code)
+    ws, ws_bytes = _scratch("ethos_linear_ce_workspace_bytes", h.device, n, d, V, code)
     loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=h.device)
     rc = lib.ethos_linear_ce(h.data_ptr(), h.stride(0) if n > 1 else d, w.data_ptr(), labels.data_ptr(), n, d, V, int(ignore_index),
                              REDUCTIONS[reduction], code, st.data_ptr(), st_bytes, ws.data_ptr(), ws_bytes, loss.data_ptr(), _stream())
@@ -689,7 +703,7 @@ def linear_ce_grad(state: torch.Tensor, w: torch.Tensor, dloss: torch.Tensor, n:
     """(dh [n, d], dw [V, d]) from dloss (float32, contiguous); None for one not wanted."""
     V, d = w.shape
     code, lib = dtype_code(w.dtype), load()
-    ws, ws_bytes = workspace(lib.ethos_linear_ce_grad_workspace_bytes(n, d, V, code), w.device)
+    ws, ws_bytes = _scratch("ethos_linear_ce_grad_workspace_bytes", w.device, n, d, V, code)
     dh = torch.empty((n, d), dtype=w.dtype, device=w.device) if want_h else None
     dw = torch.empty((V, d), dtype=w.dtype, device=w.device) if want_w else None
     rc = lib.ethos_linear_ce_grad(state.data_ptr(), state.numel() * 8, w.data_ptr(), dloss.data_ptr(), n, d, V, REDUCTIONS[reduction],
@@ -718,7 +732,7 @@ def embedding_grad(keys: torch.Tensor, dy: torch.Tensor, vocab: int, scale: floa
     _need_here(dy, "dy", FLOATS)
     n, d = keys.numel(), dy.shape[-1]
     lib = load()
-    ws, ws_bytes = workspace(lib.ethos_embedding_grad_workspace_bytes(n, d, vocab), dy.device)
+    ws, ws_bytes = _scratch("ethos_embedding_grad_workspace_bytes", dy.device, n, d, vocab)
     dw = torch.empty((vocab, d), dtype=dy.dtype, device=dy.device)
     rc = lib.ethos_embedding_grad(keys.data_ptr(), dy.data_ptr(), n, d, vocab, scale, dtype_code(dy.dtype), ws.data_ptr(), ws_bytes,
                                   dw.data_ptr(), _stream())
@@ -733,7 +747,7 @@ def balance(gates: torch.Tensor, ids: torch.Tensor, n_experts: int):
     H, k = gates.shape[-2:]
     n = gates.numel() // (H * k)
     lib = load()
-    ws, ws_bytes = workspace(lib.ethos_balance_workspace_bytes(n, H, k, n_experts), gates.device)
+    ws, ws_bytes = _scratch("ethos_balance_workspace_bytes", gates.device, n, H, k, n_experts)
     counts = torch.empty((n_experts,), dtype=torch.int32, device=gates.device)
     loss = torch.empty((), dtype=torch.float32, device=gates.device)
     rc = lib.ethos_balance(gates.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), n, H, k, n_experts, dtype_code(gates.dtype),
@@ -752,16 +766,15 @@ def balance_grad(ids: torch.Tensor, counts: torch.Tensor, dloss: torch.Tensor, d
     return out
 
 
-def clip_grads(grads, out, max_norm: float, inf_norm: bool) -> torch.Tensor:
-    """The norm (float32 []) of contiguous tensors on the current device, whose clipped values go to `out`."""
-    n, lib = len(grads), load()
-    src, dst = [t.data_ptr() for t in grads], [t.data_ptr() for t in out]
-    pointers = ctypes.c_void_p * n
-    sizes = (ctypes.c_int64 * n)(*[t.numel() for t in grads])
-    codes = (ctypes.c_int32 * n)(*[dtype_code(t.dtype) for t in grads])
-    ws, ws_bytes = workspace(lib.ethos_clip_grads_workspace_bytes(sizes, n), grads[0].device)
-    total = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    rc = lib.ethos_clip_grads(pointers(*src), pointers(*dst), sizes, codes, n, int(inf_norm), max_norm, ws.data_ptr(), ws_bytes,
-                              total.data_ptr(), _stream())
+def clip_grads(src: list, dst: list, sizes: list, codes: list, device: torch.device, max_norm: float, inf_norm: bool) -> torch.Tensor:
+    """The norm (float32 []) of contiguous tensors on the current device, given by their addresses, sizes
+    (values) and dtype codes, whose clipped values go to the addresses `dst`."""
+    n, lib = len(src), load()
+    a, b, c, t = array.array("Q", src), array.array("Q", dst), array.array("q", sizes), array.array("i", codes)
+    at = c.buffer_info()[0]
+    ws, ws_bytes = workspace(lib.ethos_clip_grads_workspace_bytes(at, n), device)
+    total = torch.empty((), dtype=torch.float32, device=device)
+    rc = lib.ethos_clip_grads(a.buffer_info()[0], b.buffer_info()[0], at, t.buffer_info()[0], n, int(inf_norm), max_norm,
+                              ws.data_ptr(), ws_bytes, total.data_ptr(), _stream())
     check(rc, "ethos_clip_grads")
     return total

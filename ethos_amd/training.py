@@ -23,6 +23,9 @@ from . import hip
 __all__ = ["balance_loss", "clip_grads", "embedding", "linear_cross_entropy"]
 
 
+_FLOATS = set(hip.FLOATS)
+
+
 def _dense(t: torch.Tensor) -> torch.Tensor:
     """t contiguous at a 16-byte address (a copy where it is not)."""
     t = t.detach().contiguous()
@@ -40,12 +43,13 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _device_check(name: str, t: torch.Tensor) -> None:
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == hip._current_device():
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{name} must be on a HIP device (got {t.device}); the ETHOS kernels have no CPU path")
-    if t.device.index != hip._current_device():
-        raise RuntimeError(f"{name} is on {t.device}, not on the current device")
+    raise RuntimeError(f"{name} is on {t.device}, not on the current device")
 
 
 # -------------------------------------------------------------------------- cross entropy
@@ -203,28 +207,34 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torc
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if len(out) != len(grads):
         raise ValueError(f"{len(grads)} gradients but {len(out)} outputs")
-    device = None
-    for t in grads if out is grads else grads + out:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError("clip_grads takes tensors")
-        if device is None and t.is_cuda:
-            device = hip._current_device()
-        if t.get_device() != device:
-            raise RuntimeError(f"clip_grads: tensors must be on the current HIP device, got one on {t.device}")
-        if t.dtype not in hip.FLOATS:
-            raise TypeError(f"clip_grads: tensors must be bfloat16 or float32, got {t.dtype}")
-    if out is not grads and any(g.shape != o.shape or g.dtype != o.dtype for g, o in zip(grads, out)):
-        raise RuntimeError("clip_grads: outputs must have the gradients' shapes and dtypes")
-    if not grads:
+    ts = grads if out is grads else grads + out
+    if not all([isinstance(t, torch.Tensor) for t in ts]):
+        raise TypeError("clip_grads takes tensors")
+    if not ts:
         return torch.zeros((), dtype=torch.float32, device="cuda")
-    places = [o.data_ptr() for o in out if o.numel()]
-    if len(set(places)) != len(places):
+    devices = {t.get_device() for t in ts}
+    if -1 in devices or devices != {hip._current_device()}:
+        raise RuntimeError(f"clip_grads: tensors must be on the current HIP device, got some on {sorted({str(t.device) for t in ts})}")
+    dtypes = [t.dtype for t in grads]
+    kinds = set(dtypes)
+    if not kinds <= _FLOATS:
+        raise TypeError(f"clip_grads: tensors must be bfloat16 or float32, got {kinds - _FLOATS}")
+    if out is not grads and ([t.dtype for t in out] != dtypes or [t.shape for t in out] != [t.shape for t in grads]):
+        raise RuntimeError("clip_grads: outputs must have the gradients' shapes and dtypes")
+    src = grads if all([t.is_contiguous() for t in grads]) else [g if g.is_contiguous() else g.contiguous() for g in grads]
+    dst = src if out is grads and src is grads else [o if o.is_contiguous() else torch.empty_like(s) for s, o in zip(src, out)]
+    sizes = [t.numel() for t in src]
+    to = [t.data_ptr() for t in dst]
+    if len(set(to)) != len(to) and len({p for p, n in zip(to, sizes) if n}) != sum(n > 0 for n in sizes):
         raise ValueError("clip_grads: an output is given twice")
-    src = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    dst = [o if o.is_contiguous() else torch.empty_like(s) for s, o in zip(src, out)]
-    total = hip.clip_grads(src, dst, float(max_norm), norm_type == math.inf)
-    for o, t in zip(out, dst):
+    codes = [int(dt == torch.bfloat16) for dt in dtypes] if len(kinds) > 1 else [int(torch.bfloat16 in kinds)] * len(dtypes)
+    total = hip.clip_grads(to if dst is src else [t.data_ptr() for t in src], to, sizes, codes, grads[0].device, float(max_norm),
+                           norm_type == math.inf)
+    for o, t in zip(out, dst) if dst is not out else ():
         if o is not t:
             o.copy_(t)
-    torch.autograd.graph.increment_version([o for o in out if not o.is_inference()])  # written by address
+    try:
+        torch.autograd.graph.increment_version(out)  # written by address
+    except RuntimeError:  # some are inference tensors, which have none
+        torch.autograd.graph.increment_version([o for o in out if not o.is_inference()])
     return total
