@@ -73,32 +73,39 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict
                                                        int32_t* __restrict__ count, int32_t* __restrict__ idx,
                                                        int32_t* __restrict__ inv, int32_t* __restrict__ lab,
                                                        float* __restrict__ loss_rows, int32_t* __restrict__ ticket) {
-    __shared__ int32_t sums[16];
+    __shared__ int32_t sums[2][16];
     const int tid = threadIdx.x, wave = tid >> 6;
+    constexpr int C = 8;  // labels a thread asks for at once
     int32_t base = 0;
-    for (int64_t i0 = 0; i0 < n; i0 += 1024) {
-        const int64_t i = i0 + tid;
-        const int64_t l = i < n ? labels[i] : ignore;
-        const bool use = i < n && l != ignore;
-        const uint64_t m = ballot(use);
-        if ((tid & 63) == 0) sums[wave] = __popcll(m);
-        __syncthreads();
-        int32_t before = base, all = 0;
-        for (int w = 0; w < 16; ++w) {
-            if (w < wave) before += sums[w];
-            all += sums[w];
-        }
-        if (i < n) {
-            const int32_t at = before + count_below(m);
-            inv[i] = use ? at : -1;
-            if (use) {
-                idx[at] = (int32_t)i;
-                lab[at] = l >= 0 && l < vocab ? (int32_t)l : -1;
-            } else if (loss_rows) {
-                loss_rows[i] = 0.0f;
+    for (int64_t i0 = 0; i0 < n; i0 += C * 1024) {
+        int64_t l[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) l[c] = i0 + c * 1024 + tid < n ? labels[i0 + c * 1024 + tid] : ignore;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int64_t i = i0 + c * 1024 + tid;
+            if (i0 + c * 1024 >= n) break;
+            const bool use = l[c] != ignore;
+            const uint64_t m = ballot(use);
+            if ((tid & 63) == 0) sums[c & 1][wave] = __popcll(m);
+            __syncthreads();
+            int32_t before = base, all = 0;
+            for (int w = 0; w < 16; ++w) {
+                if (w < wave) before += sums[c & 1][w];
+                all += sums[c & 1][w];
             }
+            if (i < n) {
+                const int32_t at = before + count_below(m);
+                inv[i] = use ? at : -1;
+                if (use) {
+                    idx[at] = (int32_t)i;
+                    lab[at] = l[c] >= 0 && l[c] < vocab ? (int32_t)l[c] : -1;
+                } else if (loss_rows) {
+                    loss_rows[i] = 0.0f;
+                }
+            }
+            base += all;
         }
-        base += all;
         __syncthreads();
     }
     if (tid == 0) {
@@ -321,10 +328,10 @@ template <int B> struct Tile {
     static constexpr int kWN = kWaves / 2;                           // waves along n (two along m)
     static constexpr int kMI = B / 64, kNI = B / kWN / 32;           // MFMA tiles of a wave
     static constexpr int kK = 64;                                    // step of the reduction
-    static constexpr int kStages = 2;                                // steps in LDS
     static constexpr int kBytes = B * kK * 2;                        // one operand's step
     static constexpr int kCopies = kBytes / 1024 / kWaves;           // copies of a wave per operand and step
-    static constexpr int kLds = kStages * 2 * kBytes;
+    static constexpr int kLds = 2 * 2 * kBytes;                      // two steps
+    static constexpr int kRowsLds = kWaves * 4096;                   // the logits' epilogue: 4 KB a wave
 };
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -392,7 +399,8 @@ __device__ __forceinline__ void feed_copy(const Feed& f, int j, uint32_t lds, in
         const int slot = (j * Ti::kWaves + wave) * 64 + lane;
         off = k_piece<Ti::kK>(slot / (Ti::kK / 8), slot % (Ti::kK / 8)) * 8 < f.k_left ? off : kOutside;
     }
-    lds_dma16(buffer_rsrc((const void*)f.base, (uint32_t)left), (int)off, 0, lds + (j * Ti::kWaves + wave) * 1024);
+    lds_dma16(buffer_rsrc((const void*)f.base, (uint32_t)left), (int)off, 0,
+              __builtin_amdgcn_readfirstlane(lds + (j * Ti::kWaves + wave) * 1024));
 }
 template <int B>
 __device__ __forceinline__ void feed_advance(Feed& f) {
@@ -439,38 +447,65 @@ template <int B, bool KC, int N> struct Reader {
     }
 };
 
-// All of this wave's copies but the newest `N` have landed, its LDS reads are done, and so with every wave.
-template <int N>
-__device__ __forceinline__ void step_barrier() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
+// This wave's copies have landed and its LDS reads are done, and so with every wave.
+__device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// This wave's LDS accesses are done, and so with every wave.
+// The same of LDS accesses alone.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// The copies of a tile's first step, into the first place in LDS.
-template <int B, int PL, bool AK, bool BK>
-__device__ __forceinline__ void tile_begin(Feed& fa, Feed& fb, uint32_t lds, int wave, int lane) {
-    typedef Tile<B> Ti;
-    if (PL > 1) {
-        feed_plane(fa, kPairsA & 3);
-        feed_plane(fb, kPairsB & 3);
-    }
-#pragma unroll
-    for (int c = 0; c < Ti::kCopies; ++c) feed_copy<B, AK>(fa, c, lds, wave, lane);
-#pragma unroll
-    for (int c = 0; c < Ti::kCopies; ++c) feed_copy<B, BK>(fb, c, lds + Ti::kBytes, wave, lane);
+// A tile's operands and how far its copies are.
+struct Pair {
+    Feed a, b;
+    int64_t steps, in;  // steps of a pair of planes; taken of the present one
+    int pair;
+};
+
+template <int B, bool AK, bool BK>
+__device__ __forceinline__ void tile_copy(const Pair& p, uint32_t to, int c, int wave, int lane) {
+    constexpr int C = Tile<B>::kCopies;
+    if (c < C) feed_copy<B, AK>(p.a, c, to, wave, lane);
+    else feed_copy<B, BK>(p.b, c - C, to + Tile<B>::kBytes, wave, lane);
 }
 
-// The tile's products over `steps` steps, after tile_begin (whose copies every wave has waited for).  float32: of
-// each pair of planes, from the two lowest up.  Between the
-// products of 16 k stand the LDS reads of the next 16, one at a time; the step's barrier stands before its last
-// products, which cover the first reads of the next step and the copies into the step just freed.
+template <int B, int PL>
+__device__ __forceinline__ void tile_advance(Pair& p) {
+    feed_advance<B>(p.a);
+    feed_advance<B>(p.b);
+    if (PL > 1 && ++p.in == p.steps) {
+        p.in = 0;
+        ++p.pair;
+        feed_plane(p.a, (int)(kPairsA >> (4 * p.pair)) & 3);
+        feed_plane(p.b, (int)(kPairsB >> (4 * p.pair)) & 3);
+    }
+}
+
+// The copies of a tile's first two steps (or the one it has).
 template <int B, int PL, bool AK, bool BK>
-__device__ __forceinline__ void tile_run(Feed& fa, Feed& fb, int64_t steps, uint32_t lds, f32x16_t (&acc)[Tile<B>::kMI][Tile<B>::kNI],
-                                             int wave, int lane) {
+__device__ __forceinline__ void tile_begin(Pair& p, int64_t steps, uint32_t lds, int wave, int lane) {
+    p.steps = steps;
+    p.in = 0;
+    p.pair = 0;
+    if (PL > 1) {
+        feed_plane(p.a, kPairsA & 3);
+        feed_plane(p.b, kPairsB & 3);
+    }
+    const int n = steps <= 0 ? 0 : PL > 1 || steps > 1 ? 2 : 1;
+    for (int t = 0; t < n; ++t) {
+#pragma unroll
+        for (int c = 0; c < 2 * Tile<B>::kCopies; ++c) tile_copy<B, AK, BK>(p, lds + t * 2 * Tile<B>::kBytes, c, wave, lane);
+        tile_advance<B, PL>(p);
+    }
+}
+
+// The tile's products, after tile_begin, whose copies every wave has waited for.  float32: of each pair of planes,
+// from the lowest up.  Between the products of 16 k stand the LDS reads of the next 16, one at a time; the step's
+// barrier stands before its last products, which cover the first reads of the next step and the copies into the step
+// just freed.  (Reads and copies in a row before the products: 54% of the matrix pipes' cycles used at 2.0 GHz; so:
+// 72% at 1.78 GHz, which the power allows; with no copies at all 81% at 1.82 GHz.)
+template <int B, int PL, bool AK, bool BK>
+__device__ __forceinline__ void tile_run(Pair& p, uint32_t lds, f32x16_t (&acc)[Tile<B>::kMI][Tile<B>::kNI], int wave, int lane) {
     typedef Tile<B> Ti;
-    constexpr int MI = Ti::kMI, NI = Ti::kNI, S = Ti::kStages, C = Ti::kCopies, Q = MI * NI, kLast = Ti::kK / 16 - 1;
+    constexpr int MI = Ti::kMI, NI = Ti::kNI, C = Ti::kCopies, Q = MI * NI, kLast = Ti::kK / 16 - 1;
     Reader<B, AK, MI> ra;
     Reader<B, BK, NI> rb;
     ra.init(wave / Ti::kWN * (B / 2), lane);
@@ -479,23 +514,7 @@ __device__ __forceinline__ void tile_run(Feed& fa, Feed& fb, int64_t steps, uint
     for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j) acc[i][j] = f32x16_zero();
-    if (steps <= 0) return;
-    int64_t in = 0;
-    int pair = 0;
-    auto copy = [&](uint32_t to, int c) {
-        if (c < C) feed_copy<B, AK>(fa, c, to, wave, lane);
-        else feed_copy<B, BK>(fb, c - C, to + Ti::kBytes, wave, lane);
-    };
-    auto advance = [&]() {
-        feed_advance<B>(fa);
-        feed_advance<B>(fb);
-        if (PL > 1 && ++in == steps) {
-            in = 0;
-            ++pair;
-            feed_plane(fa, (int)(kPairsA >> (4 * pair)) & 3);
-            feed_plane(fb, (int)(kPairsB >> (4 * pair)) & 3);
-        }
-    };
+    if (p.steps <= 0) return;
     bf16x8_t a[2][MI], b[2][NI];
     // read r of 16 k: in the order in which the products take them
     auto read = [&](uint32_t from, int s, int r) {
@@ -514,20 +533,16 @@ __device__ __forceinline__ void tile_run(Feed& fa, Feed& fb, int64_t steps, uint
         }
     };
     constexpr int R = (MI + NI + Q - 1) / Q;  // reads after a product
-    const int64_t total = PL > 1 ? steps * kPairs : steps;
-    advance();
-    for (int t = 1; t < S && t < total; ++t) {
-#pragma unroll
-        for (int c = 0; c < 2 * C; ++c) copy(lds + t * 2 * Ti::kBytes, c);
-        advance();
-    }
+    const int64_t total = PL > 1 ? p.steps * kPairs : p.steps;
 #pragma unroll
     for (int r = 0; r < MI + NI; ++r) read(lds, 0, r);
-    uint32_t cur = 0, from = lds, next = lds;
-    auto head = [&]() {  // all but the step's last products
+    uint32_t cur = 0, from = lds, next = lds + 2 * Ti::kBytes;
+    auto flip = [&]() {
+        cur ^= 1;
         from = lds + cur * 2 * Ti::kBytes;
-        cur = cur + 1 == S ? 0 : cur + 1;
-        next = lds + cur * 2 * Ti::kBytes;
+        next = lds + (cur ^ 1) * 2 * Ti::kBytes;
+    };
+    auto head = [&]() {  // all but the step's last products
 #pragma unroll
         for (int s = 0; s < kLast; ++s)
             multiply(s, [&](int q) {
@@ -535,29 +550,32 @@ __device__ __forceinline__ void tile_run(Feed& fa, Feed& fb, int64_t steps, uint
                 for (int r = 0; r < R; ++r) read(from, s + 1, q * R + r);
             });
     };
-    for (int64_t t = S; t < total; ++t) {
+    for (int64_t t = 2; t < total; ++t) {
         head();
-        step_barrier<2 * C * (S - 2)>();
+        if (t == 2) lds_barrier();  // (the second step is there; stores before it may still be on their way)
+        else step_barrier();
         multiply(kLast, [&](int q) {
             constexpr int P = (2 * C + Q - 1) / Q;  // copies after a product
 #pragma unroll
             for (int r = 0; r < R; ++r) read(next, 0, q * R + r);
 #pragma unroll
             for (int c = 0; c < P; ++c)
-                if (q * P + c < 2 * C) copy(from, q * P + c);
+                if (q * P + c < 2 * C) tile_copy<B, AK, BK>(p, from, q * P + c, wave, lane);
         });
-        advance();
+        tile_advance<B, PL>(p);
+        flip();
     }
     // the steps that are in LDS or on their way (the last one's reads of a next step go unused)
-    for (int t = total < S ? (int)total : S; t > 0; --t) {
+    for (int t = total < 2 ? (int)total : 2; t > 0; --t) {
         head();
-        step_barrier<0>();
+        step_barrier();
         multiply(kLast, [&](int q) {
 #pragma unroll
             for (int r = 0; r < R; ++r) read(next, 0, q * R + r);
         });
+        flip();
     }
-    step_barrier<0>();
+    lds_barrier();
 }
 
 // A tile of C transposed through LDS: rows n of B bf16 values m, the pieces of 16 bytes at
@@ -571,11 +589,11 @@ __device__ __forceinline__ void put4(uint32_t lds, int n, int m, uint32_t lo, ui
     typedef __attribute__((address_space(3))) u32x2_t* ptr;
     *(ptr)(size_t)(lds + row_slot<B>(n, m)) = u32x2_t{lo, hi};
 }
-template <int B, int ROWS>
+template <int B>
 __device__ __forceinline__ void tile_to_rows(uint32_t lds, uint16_t* out, int64_t ld, int rows, int cols, int tid) {
     typedef const __attribute__((address_space(3))) u32x4_t* ptr;
 #pragma unroll 4
-    for (int q = tid; q < ROWS * (B / 8); q += Tile<B>::kThreads) {
+    for (int q = tid; q < B * (B / 8); q += Tile<B>::kThreads) {
         const int n = q / (B / 8), c = q % (B / 8);
         if (n < rows && c * 8 < cols) *reinterpret_cast<u32x4_t*>(out + (int64_t)n * ld + c * 8) = *(ptr)(size_t)(lds + row_slot<B>(n, c * 8));
     }
@@ -622,10 +640,10 @@ template <int B, int PL, int GRAD>
 __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitArgs g) {
     typedef Tile<B> Ti;
     constexpr int MI = Ti::kMI, NI = Ti::kNI;
-    __shared__ __align__(16) char smem[Ti::kLds];
+    __shared__ __align__(16) char smem[Ti::kLds + (GRAD ? Ti::kRowsLds : 0)];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t lds = lds_addr(smem), rows_lds = lds + 2 * Ti::kBytes;
+    const uint32_t lds = lds_addr(smem), mine = lds + Ti::kLds + wave * 4096;
     const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
     const int64_t words = g.v1 - g.v0, m = *g.count;
     // this workgroup's tiles: those of the vocabulary tiles of its XCD, one after the other, every gridDim / 8th
@@ -633,47 +651,42 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
     const int64_t m_tiles = (words + B - 1) / B, tiles = (m_tiles - xcd + 7) / 8 * n_tiles;
     int64_t tile = blockIdx.x / 8;
     if (tile >= tiles) return;
-    Feed fa, fb;
+    Pair p;
     int64_t m0, n0;
     auto begin = [&]() {
         m0 = (tile / n_tiles * 8 + xcd) * B;
         n0 = tile % n_tiles * B;
-        feed_init<B, true>(fa, g.w + m0 * g.d, (words - m0) * g.d * 2, g.d, g.d, 0, g.w_plane, wave, lane);
-        feed_init<B, true>(fb, g.h + n0 * g.ldh, (g.np - n0) * g.ldh * 2, g.ldh, g.d, 0, g.np * g.ldh, wave, lane);
-        tile_begin<B, PL, true, true>(fa, fb, lds, wave, lane);
+        feed_init<B, true>(p.a, g.w + m0 * g.d, (words - m0) * g.d * 2, g.d, g.d, 0, g.w_plane, wave, lane);
+        feed_init<B, true>(p.b, g.h + n0 * g.ldh, (g.np - n0) * g.ldh * 2, g.ldh, g.d, 0, g.np * g.ldh, wave, lane);
+        tile_begin<B, PL, true, true>(p, (g.d + Ti::kK - 1) / Ti::kK, lds, wave, lane);
     };
     begin();
-    step_barrier<0>();
+    step_barrier();
     for (;;) {
         const int64_t tm0 = m0, tn0 = n0;
-        // what the epilogue needs of this lane's rows (and, a thread per row, of their labels)
-        float lse[NI], k[NI], label_value = 0.0f;
-        int label_at = -1;
+        // what the epilogue needs of this lane's rows
+        float lse[NI], k[NI], label_value[NI];
+        int label_at[NI];  // the label's word in the wave's B / 2 words
         if constexpr (GRAD == 1) {
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
-                const int64_t r = tn0 + wn + j * 32 + (lane & 31);
-                lse[j] = r < m ? g.lse[r] : 0.0f;
-                k[j] = r < m ? row_gradient(g.dloss, g.idx, r, m, g.reduction) : 0.0f;
-            }
-            if (tid < B && tn0 + tid < m) {
-                const int64_t r = tn0 + tid, v = (int64_t)g.lab[r] - g.v0 - tm0;
-                if (v >= 0 && v < B) {
-                    label_at = (int)v;
-                    // exp(l - lse) - 1 without the cancellation
-                    label_value = expm1f(g.ll[r] - g.lse[r]) * row_gradient(g.dloss, g.idx, r, m, g.reduction);
-                }
+                const int64_t r = tn0 + wn + j * 32 + (lane & 31), rc = r < m ? r : m - 1;
+                lse[j] = g.lse[rc];
+                k[j] = row_gradient(g.dloss, g.idx, rc, m, g.reduction);
+                const int64_t v = (int64_t)g.lab[rc] - g.v0 - tm0 - wm;
+                label_at[j] = v >= 0 && v < B / 2 && r < m && lane < 32 ? (int)v : -1;
+                label_value[j] = expm1f(g.ll[rc] - lse[j]) * k[j];  // exp(l - lse) - 1 without the cancellation
             }
         }
         f32x16_t acc[MI][NI];
-        tile_run<B, PL, true, true>(fa, fb, (g.d + Ti::kK - 1) / Ti::kK, lds, acc, wave, lane);
-        // the next tile's first step is on its way during the epilogue
+        tile_run<B, PL, true, true>(p, lds, acc, wave, lane);
+        // the next tile's first steps are on their way during the epilogue
         tile += gridDim.x / 8;
         const bool more = tile < tiles;
         if (more) begin();
         // (hidden from the compiler, which would keep the epilogue's addresses in registers through the products)
-        int el = lane, et = tid;
-        asm volatile("" : "+v"(el), "+v"(et));
+        int el = lane;
+        asm volatile("" : "+v"(el));
         if constexpr (PL > 1) {
             uint64_t again[NI] = {};
 #pragma unroll
@@ -734,7 +747,7 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                 if (el < 32) g.part[((g.v0 + tm0) / (B / 2) + wave / Ti::kWN) * g.np + r] = make_float2(x, s);
             }
             if (!more) break;
-            step_barrier<0>();
+            step_barrier();
         } else {
             // dl, in place
 #pragma unroll
@@ -756,59 +769,69 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                         acc[i][j][e] = in ? v : 0.0f;
                     }
             }
+            // the next tile's copies, before the stores, which no one waits for
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            // 32 rows by 64 words at a time through the wave's own LDS; what a plane leaves stays in acc
 #pragma unroll
-            for (int pl = 0; pl < PL; ++pl) {
-                // this plane of the tile, half of its rows at a time; what is left of the values stays in acc
-                uint16_t* out = g.p + pl * g.np * g.ldp + (tm0 / kPanel * g.np + tn0) * kPanel + tm0 % kPanel;
-                float rest = label_value;
+            for (int j = 0; j < NI; ++j)
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (wn / (B / 2) == half) {
+                for (int c = 0; c < MI / 2; ++c)
 #pragma unroll
-                        for (int j = 0; j < NI; ++j)
+                    for (int pl = 0; pl < PL; ++pl) {
+                        const int n = el & 31;
 #pragma unroll
-                            for (int i = 0; i < MI; ++i)
+                        for (int i = 0; i < 2; ++i)
 #pragma unroll
-                                for (int e = 0; e < 16; e += 4) {
-                                    uint32_t q[2];
+                            for (int e = 0; e < 16; e += 4) {
+                                f32x16_t& v = acc[2 * c + i][j];
+                                uint32_t q[2];
 #pragma unroll
-                                    for (int u = 0; u < 2; ++u) {
-                                        q[u] = pack_bf16x2(acc[i][j][e + 2 * u], acc[i][j][e + 2 * u + 1]);
-                                        if (pl + 1 < PL) {
-                                            acc[i][j][e + 2 * u] -= __uint_as_float(q[u] << 16);
-                                            acc[i][j][e + 2 * u + 1] -= __uint_as_float(q[u] & 0xffff0000u);
-                                        }
+                                for (int u = 0; u < 2; ++u) {
+                                    q[u] = pack_bf16x2(v[e + 2 * u], v[e + 2 * u + 1]);
+                                    if (pl + 1 < PL) {
+                                        v[e + 2 * u] -= __uint_as_float(q[u] << 16);
+                                        v[e + 2 * u + 1] -= __uint_as_float(q[u] & 0xffff0000u);
                                     }
-                                    put4<B>(rows_lds, (wn & (B / 2 - 1)) + j * 32 + (el & 31), wm + i * 32 + 8 * (e >> 2) + 4 * (el >> 5), q[0], q[1]);
                                 }
+                                typedef __attribute__((address_space(3))) u32x2_t* ptr;
+                                *(ptr)(size_t)(mine + n * 128 + (k_piece<64>(n, i * 4 + (e >> 2)) << 4) + 8 * (el >> 5)) = u32x2_t{q[0], q[1]};
+                            }
+                        if (label_at[j] >= 0 && label_at[j] / 64 == c) {
+                            typedef __attribute__((address_space(3))) uint16_t* ptr;
+                            const int w = label_at[j] % 64;
+                            const uint16_t x = f32_to_bf16_bits(label_value[j]);
+                            label_value[j] -= bf16_bits_to_f32(x);
+                            *(ptr)(size_t)(mine + n * 128 + (k_piece<64>(n, w >> 3) << 4) + (w & 7) * 2) = x;
+                        }
+                        __builtin_amdgcn_wave_barrier();
+                        uint16_t* out = g.p + pl * g.np * g.ldp + (tm0 / kPanel * g.np + tn0 + wn + j * 32) * kPanel + tm0 % kPanel + wm + c * 64;
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            typedef const __attribute__((address_space(3))) u32x4_t* ptr;
+                            const int r = t * 8 + (el >> 3);
+                            __builtin_nontemporal_store(*(ptr)(size_t)(mine + r * 128 + (k_piece<64>(r, el & 7) << 4)),
+                                                        reinterpret_cast<u32x4_t*>(out + r * kPanel + (el & 7) * 8));
+                        }
+                        __builtin_amdgcn_wave_barrier();
                     }
-                    // (the first wait covers the next tile's copies too; the stores come after it)
-                    if (pl == 0 && half == 0) step_barrier<0>();
-                    else lds_barrier();
-                    if (label_at >= 0 && et / (B / 2) == half) {
-                        typedef __attribute__((address_space(3))) uint16_t* ptr;
-                        const uint16_t x = f32_to_bf16_bits(rest);
-                        label_value = rest - bf16_bits_to_f32(x);
-                        *(ptr)(size_t)(rows_lds + row_slot<B>(et & (B / 2 - 1), label_at)) = x;
-                    }
-                    lds_barrier();
-                    tile_to_rows<B, B / 2>(rows_lds, out + half * (B / 2) * kPanel, kPanel, B / 2, B, et);
-                    lds_barrier();
-                }
-            }
             if (!more) break;
+            lds_barrier();
         }
     }
 }
 
-// Parts of dh's reduction over a piece of ldp words: a tile for each CU, given the labelled rows' tiles, of at least
-// kPartWords words (a part writes and reads a float32 tile: with one step of 64 each, adding up the 128 parts of a
-// 500 x 256 dh took 38 us, longer than the products).
+// Parts of dh's reduction over a piece of ldp words, given the labelled rows: none longer than a CU's share of the
+// launch's steps, of at least kPartWords words (a part writes and reads a float32 tile: 128 parts of 64 words for a
+// 500 x 256 dh took 38 us to add up, longer than the products).
 constexpr int kPartWords = 256;
-__host__ __device__ inline int dh_parts(int64_t m, int tile, int n_tiles, int64_t ldp, int num_cus) {
-    const int64_t tiles = (m + tile - 1) / tile * n_tiles;
-    const int64_t s = tiles > 0 ? num_cus / tiles : 1, most = ldp / kPartWords;
-    return (int)(s < 1 ? 1 : s < most ? s : most);
+__host__ __device__ inline int dh_parts(int64_t m, int tile, int cols, int64_t ldp, int num_cus, int with_dw) {
+    const int64_t rows = (m + tile - 1) / tile * cols, steps = ldp / 64;
+    const int64_t all = rows * steps + (with_dw ? (ldp + tile - 1) / tile * cols * ((m + 63) / 64) : 0);
+    const int64_t share = all / num_cus > 1 ? all / num_cus : 1, slots = rows > 0 ? num_cus / rows : 1, most = ldp / kPartWords;
+    int64_t s = (steps + share - 1) / share;
+    s = s < slots ? s : slots;
+    s = s < most ? s : most;
+    return (int)(s < 1 ? 1 : s);
 }
 
 // The gradients of a piece: first the workgroups of dh, float32 partial sums [part][m][d] (added to when `add`), then
@@ -820,7 +843,7 @@ struct GradArgs {
     int64_t words, np, ldp, w_plane;
     float* part;
     void* dw;  // the piece's first row
-    int d, ldh, cols, num_cus, add;
+    int d, ldh, cols, num_cus, add, with_dw;
     int64_t row_blocks;
 };
 
@@ -830,7 +853,7 @@ __device__ __forceinline__ void ce_row_grad(const GradArgs& g, int64_t block, ui
     constexpr int MI = Ti::kMI, NI = Ti::kNI;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t m = *g.count;
-    const int parts = dh_parts(m, B, g.cols, g.ldp, g.num_cus);
+    const int parts = dh_parts(m, B, g.cols, g.ldp, g.num_cus, g.with_dw);
     const Place at = tile_place(block, g.cols);
     const int part = (int)(at.group % parts);
     const int64_t m0 = at.group / parts * B;
@@ -841,17 +864,17 @@ __device__ __forceinline__ void ce_row_grad(const GradArgs& g, int64_t block, ui
     const int64_t s0 = per * part < steps ? per * part : steps, s1 = s0 + per < steps ? s0 + per : steps;
     f32x16_t acc[MI][NI];
     {
-        Feed fa, fb;
+        Pair p;
         constexpr int64_t kSteps = kPanel / Ti::kK;
         const int64_t first = (s0 / kSteps * g.np + m0) * kPanel + s0 % kSteps * Ti::kK;
-        feed_init<B, true>(fa, g.p + first, (g.np * g.ldp - first) * 2, kPanel, INT32_MAX, 0, g.np * g.ldp, wave, lane);
-        fa.jump = (g.np - 1) * kPanel * 2;
-        fa.at = fa.at0 = (int)(s0 % kSteps);
-        feed_init<B, false>(fb, g.w + s0 * Ti::kK * g.d + n0, ((g.words - s0 * Ti::kK) * g.d - n0) * 2, g.d, 0, g.d - n0, g.w_plane, wave,
+        feed_init<B, true>(p.a, g.p + first, (g.np * g.ldp - first) * 2, kPanel, INT32_MAX, 0, g.np * g.ldp, wave, lane);
+        p.a.jump = (g.np - 1) * kPanel * 2;
+        p.a.at = p.a.at0 = (int)(s0 % kSteps);
+        feed_init<B, false>(p.b, g.w + s0 * Ti::kK * g.d + n0, ((g.words - s0 * Ti::kK) * g.d - n0) * 2, g.d, 0, g.d - n0, g.w_plane, wave,
                             lane);
-        if (s0 < s1) tile_begin<B, PL, true, false>(fa, fb, lds, wave, lane);
-        step_barrier<0>();
-        tile_run<B, PL, true, false>(fa, fb, s1 - s0, lds, acc, wave, lane);
+        tile_begin<B, PL, true, false>(p, s1 - s0, lds, wave, lane);
+        step_barrier();
+        tile_run<B, PL, true, false>(p, lds, acc, wave, lane);
     }
     const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
     float* out = g.part + (int64_t)part * rows * g.d;
@@ -881,13 +904,13 @@ __device__ __forceinline__ void ce_head_grad(const GradArgs& g, int64_t block, u
     f32x16_t acc[MI][NI];
     {
         const int64_t rows = round_up(*g.count, kPadRows), steps = (*g.count + Ti::kK - 1) / Ti::kK;
-        Feed fa, fb;
-        feed_init<B, false>(fa, g.h + m0, (rows * g.ldh - m0) * 2, g.ldh, 0, g.d - m0, g.np * g.ldh, wave, lane);
-        feed_init<B, false>(fb, g.p + n0 / kPanel * g.np * kPanel + n0 % kPanel, (rows * kPanel - n0 % kPanel) * 2, kPanel, 0, B,
+        Pair p;
+        feed_init<B, false>(p.a, g.h + m0, (rows * g.ldh - m0) * 2, g.ldh, 0, g.d - m0, g.np * g.ldh, wave, lane);
+        feed_init<B, false>(p.b, g.p + n0 / kPanel * g.np * kPanel + n0 % kPanel, (rows * kPanel - n0 % kPanel) * 2, kPanel, 0, B,
                             g.np * g.ldp, wave, lane);
-        if (steps > 0) tile_begin<B, PL, false, false>(fa, fb, lds, wave, lane);
-        step_barrier<0>();
-        tile_run<B, PL, false, false>(fa, fb, steps, lds, acc, wave, lane);
+        tile_begin<B, PL, false, false>(p, steps, lds, wave, lane);
+        step_barrier();
+        tile_run<B, PL, false, false>(p, lds, acc, wave, lane);
     }
     const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
     const int rows = g.words - n0 < B ? (int)(g.words - n0) : B;
@@ -906,7 +929,7 @@ __device__ __forceinline__ void ce_head_grad(const GradArgs& g, int64_t block, u
             }
     if constexpr (PL == 1) {
         lds_barrier();
-        tile_to_rows<B, B>(lds, (uint16_t*)g.dw + n0 * g.d + m0, g.d, rows, g.d - m0, tid);
+        tile_to_rows<B>(lds, (uint16_t*)g.dw + n0 * g.d + m0, g.d, rows, g.d - m0, tid);
     }
 }
 
@@ -920,10 +943,10 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_grads_kernel(GradArgs
 // dh in h's rows and type: the sum of the parts, zeros for rows without a label; 4 columns a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void ce_row_grad_out_kernel(const float* __restrict__ part, const int32_t* __restrict__ count,
-                                                              const int32_t* __restrict__ inv, int64_t n, int d, int tile, int n_tiles,
-                                                              int64_t ldp, int num_cus, T* __restrict__ dh) {
+                                                              const int32_t* __restrict__ inv, int64_t n, int d, int tile, int cols,
+                                                              int64_t ldp, int num_cus, int with_dw, T* __restrict__ dh) {
     const int64_t m = *count, size = round_up(m, kPadRows) * d;
-    const int parts = dh_parts(m, tile, n_tiles, ldp, num_cus);
+    const int parts = dh_parts(m, tile, cols, ldp, num_cus, with_dw);
     const int64_t total = n * (d / 4);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / (d / 4);
@@ -1117,7 +1140,7 @@ int launch_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* l
     LogitArgs g = logit_args(s, w, f.w, 0, vocab, vocab, d, dtype);
     g.part = f.part;
     run_logits<0>(g, f.tile, dtype, n, num_cus, stream);
-    hipLaunchKernelGGL(ce_lse_kernel, dim3((unsigned)(s.np / 16)), dim3(1024), 0, stream, f.part, f.n_part, s.np, s.count, s.idx, s.ll,
+    hipLaunchKernelGGL(ce_lse_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, stream, f.part, f.n_part, s.np, s.count, s.idx, s.ll,
                        reduction, s.lse, f.row_loss, s.ticket, loss);
     return (int)hipGetLastError();
 }
@@ -1139,7 +1162,7 @@ int launch_linear_ce_grad(const void* state, const void* w, const float* dloss, 
         const int64_t row_blocks = dh ? xcd_grid(b.part_tiles, cols) : 0;
         const int64_t head_blocks = dw ? xcd_grid((words + b.grad_tile - 1) / b.grad_tile, cols) : 0;
         const GradArgs a{b.p, s.h, g.w, s.count, words, s.np, b.piece, g.w_plane, b.part, (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4), d,
-                         s.ldh, cols, num_cus, v0 > 0 ? 1 : 0, row_blocks};
+                         s.ldh, cols, num_cus, v0 > 0 ? 1 : 0, dw ? 1 : 0, row_blocks};
         with_tile(b.grad_tile, dtype, [&](auto t, auto pl) {
             constexpr int B = decltype(t)::v, PL = decltype(pl)::v;
             hipLaunchKernelGGL((ce_grads_kernel<B, PL>), dim3((unsigned)(row_blocks + head_blocks)), dim3(Tile<B>::kThreads), 0, stream, a);
@@ -1150,10 +1173,10 @@ int launch_linear_ce_grad(const void* state, const void* w, const float* dloss, 
         blocks = blocks < num_cus * 16 ? blocks : num_cus * 16;
         if (dtype == kBF16)
             hipLaunchKernelGGL((ce_row_grad_out_kernel<uint16_t>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, n,
-                               d, b.grad_tile, cols, b.piece, num_cus, (uint16_t*)dh);
+                               d, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, (uint16_t*)dh);
         else
             hipLaunchKernelGGL((ce_row_grad_out_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, n, d,
-                               b.grad_tile, cols, b.piece, num_cus, (float*)dh);
+                               b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, (float*)dh);
     }
     return (int)hipGetLastError();
 }

@@ -120,6 +120,19 @@ def test_cross_entropy_several_pieces_of_vocabulary(dt, n, d, V):
         _within(got, x, e, what)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,ignored", [(700, 0.0), (1300, 0.5)])
+def test_cross_entropy_in_the_largest_tiles(dt, n, ignored):
+    d, V = 264, 30011
+    h, w, labels = _ce_inputs(n, d, V, DT[dt], seed=n, ignored=ignored)
+    gy = torch.rand(n, generator=_gen(2), device="cuda")
+    want, bound = _ce_oracle(h, w, labels, "none", gy)
+    a, b = h.requires_grad_(), w.requires_grad_()
+    loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="none")
+    for got, x, e, what in zip((loss.detach(), *torch.autograd.grad(loss, (a, b), gy)), want, bound, ("loss", "dh", "dw")):
+        _within(got, x, e, what)
+
+
 def test_cross_entropy_gradient_against_differences():
     h, w, labels = _ce_inputs(9, 16, 37, torch.float32, seed=2, ignored=0.3)
     labels[0] = 5
