@@ -3,8 +3,9 @@
 //   out = RN_T(g min(1, max_norm / (total + 1e-6))).
 // Two passes over the gradients with one workgroup per piece of kPiece values: the squares' sums
 // (float64: no gradient's square overflows or vanishes there) in a fixed order, one small kernel
-// for the norm and the factor, then the scaled copy.  The tensors' addresses travel as kernel
-// arguments, kPerLaunch tensors to a launch.
+// for the norm and the factor, then the scaled copy, last pieces first (what the norm read last may still be
+// in the caches).  The tensors' addresses travel as kernel arguments, as many as fit their 4 KiB: a launch
+// and pass for up to 180 tensors.
 #include "ethos_common.hpp"
 #include "ethos_rows.hpp"
 #include "ethos_train.hpp"
@@ -12,19 +13,22 @@
 namespace ethos {
 namespace {
 
-constexpr int64_t kPiece = 32768;
-constexpr int kPerLaunch = 128;  // 28 bytes each of the 4 KiB of a launch's arguments
+constexpr int kPiece = 32768;
+constexpr int kPerLaunch = 180;
+constexpr uint16_t kFloatBit = 0x8000;
 
+// A launch's tensors; `out` is what the scaled copies go to.
 struct ClipList {
     const void* in[kPerLaunch];
     void* out[kPerLaunch];
-    int64_t size[kPerLaunch];   // values, negative (~size) for float32
     int32_t first[kPerLaunch];  // first piece of the tensor in this launch
+    uint16_t tail[kPerLaunch];  // values of its last piece, less one; kFloatBit: float32
     int32_t count;
     int32_t pieces;  // of this launch
     int32_t base;    // pieces before this launch
 };
-static_assert(sizeof(ClipList) + 64 <= 4096, "kernel arguments");
+static_assert(sizeof(ClipList) + 32 <= 4096, "kernel arguments");
+static_assert(kPiece <= kFloatBit, "a tail's bits");
 
 // The tensor that holds piece b: the last one whose first piece is not past it.
 __device__ __forceinline__ int clip_find(const ClipList& l, int b) {
@@ -36,14 +40,19 @@ __device__ __forceinline__ int clip_find(const ClipList& l, int b) {
     }
     return lo;
 }
+// Values of piece b of tensor t.
+__device__ __forceinline__ int clip_size(const ClipList& l, int t, int b) {
+    const int end = t + 1 < l.count ? l.first[t + 1] : l.pieces;
+    return b + 1 < end ? kPiece : (l.tail[t] & (kFloatBit - 1)) + 1;
+}
 
 template <typename T, typename F>
-__device__ __forceinline__ void clip_values(const T* p, int64_t n, F f) {
+__device__ __forceinline__ void clip_values(const T* p, int n, F f) {
     constexpr int N = Vec16<T>::kN;
     if (((uintptr_t)p & 15u) == 0) {
         typedef typename Vec16<T>::raw Raw;
-        const int64_t whole = n / N;
-        int64_t i = threadIdx.x;
+        const int whole = n / N;
+        int i = threadIdx.x;
         for (; i + 3 * 256 < whole; i += 4 * 256) {  // four loads on their way
             Raw r[4];
 #pragma unroll
@@ -64,7 +73,7 @@ __device__ __forceinline__ void clip_values(const T* p, int64_t n, F f) {
         }
         for (i = whole * N + threadIdx.x; i < n; i += 256) f(Elem<T>::to_f32(p[i]));
     } else {
-        for (int64_t i = threadIdx.x; i < n; i += 256) f(Elem<T>::to_f32(p[i]));
+        for (int i = threadIdx.x; i < n; i += 256) f(Elem<T>::to_f32(p[i]));
     }
 }
 
@@ -92,9 +101,8 @@ __global__ __launch_bounds__(256) void clip_norm_kernel(ClipList l, double* __re
     __shared__ double lds[4];
     const int t = clip_find(l, blockIdx.x);
     const int64_t at = (int64_t)((int)blockIdx.x - l.first[t]) * kPiece;
-    const bool f32 = l.size[t] < 0;
-    const int64_t size = f32 ? ~l.size[t] : l.size[t];
-    const int64_t n = size - at < kPiece ? size - at : kPiece;
+    const bool f32 = (l.tail[t] & kFloatBit) != 0;
+    const int n = clip_size(l, t, blockIdx.x);
     double s = 0.0;
     auto add = [&](float v) { s = INF ? nan_max(s, fabs((double)v)) : __builtin_fma((double)v, (double)v, s); };
     if (f32) clip_values((const float*)l.in[t] + at, n, add);
@@ -119,10 +127,10 @@ __global__ __launch_bounds__(1024) void clip_total_kernel(const double* __restri
 }
 
 template <typename T, typename W>
-__device__ __forceinline__ void clip_scale(const T* in, T* out, int64_t n, float k) {
+__device__ __forceinline__ void clip_scale(const T* in, T* out, int n, float k) {
     constexpr int N = sizeof(W) / sizeof(T);
-    const int64_t whole = n / N;
-    for (int64_t i = threadIdx.x; i < whole; i += 256) {
+    const int whole = n / N;
+    for (int i = threadIdx.x; i < whole; i += 256) {
         union {
             W w;
             T t[N];
@@ -132,11 +140,11 @@ __device__ __forceinline__ void clip_scale(const T* in, T* out, int64_t n, float
         for (int j = 0; j < N; ++j) v.t[j] = Elem<T>::from_f32(Elem<T>::to_f32(v.t[j]) * k);
         reinterpret_cast<W*>(out)[i] = v.w;
     }
-    for (int64_t i = whole * N + threadIdx.x; i < n; i += 256) out[i] = Elem<T>::from_f32(Elem<T>::to_f32(in[i]) * k);
+    for (int i = whole * N + threadIdx.x; i < n; i += 256) out[i] = Elem<T>::from_f32(Elem<T>::to_f32(in[i]) * k);
 }
 
 template <typename T>
-__device__ __forceinline__ void clip_piece(const T* in, T* out, int64_t n, float k) {
+__device__ __forceinline__ void clip_piece(const T* in, T* out, int n, float k) {
     const uintptr_t a = (uintptr_t)in | (uintptr_t)out;
     if ((a & 15u) == 0) clip_scale<T, uint4>(in, out, n, k);
     else if ((a & 3u) == 0) clip_scale<T, uint32_t>(in, out, n, k);
@@ -149,9 +157,8 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(ClipList l, const float
     const float k = *factor;
     if (k == 1.0f && l.in[t] == l.out[t]) return;
     const int64_t at = (int64_t)(b - l.first[t]) * kPiece;
-    const bool f32 = l.size[t] < 0;
-    const int64_t size = f32 ? ~l.size[t] : l.size[t];
-    const int64_t n = size - at < kPiece ? size - at : kPiece;
+    const bool f32 = (l.tail[t] & kFloatBit) != 0;
+    const int n = clip_size(l, t, b);
     if (f32) clip_piece((const float*)l.in[t] + at, (float*)l.out[t] + at, n, k);
     else clip_piece((const uint16_t*)l.in[t] + at, (uint16_t*)l.out[t] + at, n, k);
 }
@@ -190,7 +197,7 @@ int launch_clip(const void* const* in, void* const* out, const int64_t* sizes, c
             if (i == n_tensors || sizes[i] == 0) continue;
             l.in[l.count] = in[i];
             l.out[l.count] = out[i];
-            l.size[l.count] = dtypes[i] == kF32 ? ~sizes[i] : sizes[i];
+            l.tail[l.count] = (uint16_t)((sizes[i] - 1) % kPiece | (dtypes[i] == kF32 ? kFloatBit : 0));
             l.first[l.count] = l.pieces;
             l.pieces += (int32_t)clip_pieces(sizes[i]);
             ++l.count;

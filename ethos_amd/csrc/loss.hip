@@ -254,38 +254,64 @@ __global__ __launch_bounds__(1024) void ce_lse_kernel(const float2* __restrict__
     __shared__ MaxSum lds[16][16];
     __shared__ double sums[16];
     __shared__ bool last;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t r = (int64_t)blockIdx.x * 16 + (lane & 15), m = *count;
-    if ((int64_t)blockIdx.x * 16 < m) {
-        MaxSum a = {-__builtin_inff(), 0.0f};
-        for (int e = wave * 4 + (lane >> 4); e < n_part; e += 64 * 8) {
-            float2 p[8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = wave * 4 + (lane >> 4);
+    const int64_t r = (int64_t)blockIdx.x * 16 + (lane & 15);
+    constexpr int C = 8;  // pairs asked for at once, before the count is known (rows past it are memory of the same array)
+    float2 p[C];
+    auto ask = [&](int e) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = part[(int64_t)(e + j * 64 < n_part ? e + j * 64 : e) * np + r];
+        for (int j = 0; j < C; ++j) p[j] = part[(int64_t)(e + j * 64 < n_part ? e + j * 64 : n_part - 1) * np + r];
+    };
+    ask(first);
+    const float x = ll[r];
+    const int64_t m = *count;
+    const int64_t row = reduction == kLossNone && r < m ? idx[r] : 0;
+    MaxSum a = {-__builtin_inff(), 0.0f};
+    for (int e = first; e < n_part; e += 64 * C) {
+        if (e != first) ask(e);
+        MaxSum b = {p[0].x, 0.0f};
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (e + j * 64 < n_part) a = join(a, {p[j].x, p[j].y});
-        }
+        for (int j = 1; j < C; ++j) b.m = fmaxf(b.m, p[j].x);
+        const float z = b.m == -__builtin_inff() ? 0.0f : b.m;
+#pragma unroll
+        for (int j = 0; j < C; ++j)
+            if (e + j * 64 < n_part) b.s += p[j].y * __builtin_amdgcn_exp2f((p[j].x - z) * kLog2e);
+        a = join(a, b);
+    }
+    a = join(a, {__shfl_xor(a.m, 16), __shfl_xor(a.s, 16)});
+    a = join(a, {__shfl_xor(a.m, 32), __shfl_xor(a.s, 32)});
+    if (lane < 16) lds[wave][lane] = a;
+    __syncthreads();
+    float out = 0.0f;
+    if (wave == 0) {
+        // the 16 waves' pairs of a row over four lanes each, then over those
+        a = lds[lane >> 4][lane & 15];
+        for (int w = 4; w < 16; w += 4) a = join(a, lds[w + (lane >> 4)][lane & 15]);
         a = join(a, {__shfl_xor(a.m, 16), __shfl_xor(a.s, 16)});
         a = join(a, {__shfl_xor(a.m, 32), __shfl_xor(a.s, 32)});
-        if (lane < 16) lds[wave][lane] = a;
-        __syncthreads();
-        if (wave == 0 && lane < 16 && r < m) {
-            for (int w = 1; w < 16; ++w) a = join(a, lds[w][lane]);
-            const float x = ll[r];
-            const float l = x == x ? a.m + __builtin_amdgcn_logf(a.s) * 0.69314718055994530942f : x;
+        const float l = x == x ? a.m + __builtin_amdgcn_logf(a.s) * 0.69314718055994530942f : x;
+        out = l - x;
+        if (lane < 16 && r < m) {
             lse[r] = l;
-            if (reduction == kLossNone) loss[idx[r]] = l - x;
-            else __hip_atomic_store(row_loss + r, l - x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (reduction == kLossNone) loss[row] = out;
+            else if (gridDim.x > 1) __hip_atomic_store(row_loss + r, out, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        __syncthreads();
     }
     if (reduction == kLossNone) return;
+    double s = 0.0;
+    if (gridDim.x == 1) {
+        if (wave != 0) return;
+        s = lane < 16 && r < m ? (double)out : 0.0;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+        if (lane == 0) *loss = (float)(reduction == kLossMean ? s / (double)m : s);
+        return;
+    }
+    __syncthreads();
     if (threadIdx.x == 0)
         last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int32_t)gridDim.x - 1;
     __syncthreads();
     if (!last) return;
-    double s = 0.0;
     for (int64_t i = threadIdx.x; i < m; i += 1024) s += (double)__hip_atomic_load(row_loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
@@ -295,7 +321,6 @@ __global__ __launch_bounds__(1024) void ce_lse_kernel(const float2* __restrict__
         double t = 0.0;
         for (int i = 0; i < 16; ++i) t += sums[i];
         *loss = (float)(reduction == kLossMean ? t / (double)m : t);
-        *ticket = 0;
     }
 }
 

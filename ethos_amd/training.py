@@ -14,6 +14,7 @@ every run.  The gradients are those of a single backward (no create_graph)."""
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -24,6 +25,8 @@ __all__ = ["balance_loss", "clip_grads", "embedding", "linear_cross_entropy"]
 
 
 _FLOATS = set(hip.FLOATS)
+_TENSORS = {torch.Tensor, torch.nn.Parameter}
+_dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
@@ -207,28 +210,28 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torc
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     if len(out) != len(grads):
         raise ValueError(f"{len(grads)} gradients but {len(out)} outputs")
+    # (a training step has hundreds of tensors: each check is one pass of a C function over them)
     ts = grads if out is grads else grads + out
-    if not all([isinstance(t, torch.Tensor) for t in ts]):
+    if not set(map(type, ts)) <= _TENSORS and not all([isinstance(t, torch.Tensor) for t in ts]):
         raise TypeError("clip_grads takes tensors")
     if not ts:
         return torch.zeros((), dtype=torch.float32, device="cuda")
-    devices = {t.get_device() for t in ts}
+    devices = set(map(torch.Tensor.get_device, ts))
     if -1 in devices or devices != {hip._current_device()}:
         raise RuntimeError(f"clip_grads: tensors must be on the current HIP device, got some on {sorted({str(t.device) for t in ts})}")
-    dtypes = [t.dtype for t in grads]
+    dtypes = list(map(_dtype, grads))
     kinds = set(dtypes)
     if not kinds <= _FLOATS:
         raise TypeError(f"clip_grads: tensors must be bfloat16 or float32, got {kinds - _FLOATS}")
-    if out is not grads and ([t.dtype for t in out] != dtypes or [t.shape for t in out] != [t.shape for t in grads]):
+    if out is not grads and (list(map(_dtype, out)) != dtypes or list(map(_shape, out)) != list(map(_shape, grads))):
         raise RuntimeError("clip_grads: outputs must have the gradients' shapes and dtypes")
-    src = grads if all([t.is_contiguous() for t in grads]) else [g if g.is_contiguous() else g.contiguous() for g in grads]
-    dst = src if out is grads and src is grads else [o if o.is_contiguous() else torch.empty_like(s) for s, o in zip(src, out)]
-    sizes = [t.numel() for t in src]
-    to = [t.data_ptr() for t in dst]
+    src = grads if all(map(torch.Tensor.is_contiguous, grads)) else [g.contiguous() for g in grads]
+    dst = out if all(map(torch.Tensor.is_contiguous, out)) else [o if o.is_contiguous() else torch.empty_like(s) for s, o in zip(src, out)]
+    sizes, to = list(map(torch.Tensor.numel, src)), list(map(torch.Tensor.data_ptr, dst))
     if len(set(to)) != len(to) and len({p for p, n in zip(to, sizes) if n}) != sum(n > 0 for n in sizes):
         raise ValueError("clip_grads: an output is given twice")
     codes = [int(dt == torch.bfloat16) for dt in dtypes] if len(kinds) > 1 else [int(torch.bfloat16 in kinds)] * len(dtypes)
-    total = hip.clip_grads(to if dst is src else [t.data_ptr() for t in src], to, sizes, codes, grads[0].device, float(max_norm),
+    total = hip.clip_grads(to if dst is src else list(map(torch.Tensor.data_ptr, src)), to, sizes, codes, grads[0].device, float(max_norm),
                            norm_type == math.inf)
     for o, t in zip(out, dst) if dst is not out else ():
         if o is not t:
