@@ -72,9 +72,10 @@ SIGNATURES = {
                                             _vp]),
     "ethos_linear_ce_state_bytes": (_sz, [_i64, _i32, _i32]),
     "ethos_linear_ce_workspace_bytes": (_sz, [_i64, _i32, _i64, _i32]),
-    "ethos_linear_ce": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i32, _i64, _i64, _i32, _i32, _vp, _sz, _vp, _sz, _vp, _vp]),
-    "ethos_linear_ce_grad_workspace_bytes": (_sz, [_i64, _i32, _i64, _i32]),
-    "ethos_linear_ce_grad": (ctypes.c_int, [_vp, _sz, _vp, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _sz, _vp, _vp, _vp]),
+    "ethos_linear_ce": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i32, _i64, _i64, _i32, _i32] + [_vp, _sz] * 3 + [_vp, _vp]),
+    "ethos_linear_ce_exps_bytes": (_sz, [_i64, _i64, _i32]),
+    "ethos_linear_ce_grad_workspace_bytes": (_sz, [_i64, _i32, _i64, _i32, _i32]),
+    "ethos_linear_ce_grad": (ctypes.c_int, [_vp, _sz, _vp, _sz, _vp, _vp, _i64, _i32, _i64, _i32, _i32, _vp, _sz, _vp, _vp, _vp]),
     "ethos_embedding": (ctypes.c_int, [_vp, _i32, _vp, _i64, _i32, _i64, _f32, _i64, _i32, _vp, _vp, _vp]),
     "ethos_embedding_grad_workspace_bytes": (_sz, [_i64, _i32, _i64]),
     "ethos_embedding_grad": (ctypes.c_int, [_vp, _vp, _i64, _i32, _i64, _f32, _i32, _vp, _sz, _vp, _vp]),

@@ -951,8 +951,8 @@ size_t ethos_linear_ce_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, 
 }
 
 int ethos_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* labels, int64_t n_tok, int32_t d, int64_t vocab,
-                    int64_t ignore_index, int32_t reduction, int32_t dtype, void* state, size_t state_bytes, void* workspace,
-                    size_t workspace_bytes, float* loss, void* stream) {
+                    int64_t ignore_index, int32_t reduction, int32_t dtype, void* state, size_t state_bytes, void* exps, size_t exps_bytes,
+                    void* workspace, size_t workspace_bytes, float* loss, void* stream) {
     g_err[0] = 0;
     if (const int rc = ce_sizes(n_tok, d, vocab, reduction, dtype, "ethos_linear_ce")) return rc;
     const int vec = dtype == ETHOS_BF16 ? 8 : 4;
@@ -963,19 +963,27 @@ int ethos_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* la
     if (state_bytes < ethos::linear_ce_state_bytes(n_tok, d, dtype) ||
         workspace_bytes < ethos::linear_ce_workspace_bytes(n_tok, d, vocab, dtype, num_cus()))
         return fail(ETHOS_EWORKSPACE, "ethos_linear_ce: state of %zu or workspace of %zu bytes too small", state_bytes, workspace_bytes);
-    if (!aligned16(h) || !aligned16(w) || !aligned16(state) || !aligned16(workspace))
-        return fail(ETHOS_EALIGN, "ethos_linear_ce: h, w, state and workspace must be 16-byte aligned");
-    return hip_status(ethos::launch_linear_ce(h, ldh, w, labels, n_tok, d, vocab, ignore_index, reduction, dtype, state, workspace, loss,
+    if (exps && exps_bytes < ethos::linear_ce_exps_bytes(n_tok, vocab, dtype))
+        return fail(ETHOS_EWORKSPACE, "ethos_linear_ce: exps of %zu bytes, %zu needed", exps_bytes,
+                    ethos::linear_ce_exps_bytes(n_tok, vocab, dtype));
+    if (!aligned16(h) || !aligned16(w) || !aligned16(state) || !aligned16(exps) || !aligned16(workspace))
+        return fail(ETHOS_EALIGN, "ethos_linear_ce: h, w, state, exps and workspace must be 16-byte aligned");
+    return hip_status(ethos::launch_linear_ce(h, ldh, w, labels, n_tok, d, vocab, ignore_index, reduction, dtype, state, exps, workspace, loss,
                                               num_cus(), (hipStream_t)stream),
                       "ethos_linear_ce");
 }
 
-size_t ethos_linear_ce_grad_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype) {
-    if (n_tok <= 0 || n_tok > kMaxItems || d <= 0 || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
-    return ethos::linear_ce_grad_workspace_bytes(n_tok, d, vocab, dtype, num_cus());
+size_t ethos_linear_ce_exps_bytes(int64_t n_tok, int64_t vocab, int32_t dtype) {
+    if (n_tok <= 0 || n_tok > kMaxItems || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
+    return ethos::linear_ce_exps_bytes(n_tok, vocab, dtype);
 }
 
-int ethos_linear_ce_grad(const void* state, size_t state_bytes, const void* w, const float* dloss, int64_t n_tok, int32_t d,
+size_t ethos_linear_ce_grad_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype, int32_t kept) {
+    if (n_tok <= 0 || n_tok > kMaxItems || d <= 0 || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
+    return ethos::linear_ce_grad_workspace_bytes(n_tok, d, vocab, dtype, num_cus(), kept != 0);
+}
+
+int ethos_linear_ce_grad(const void* state, size_t state_bytes, void* exps, size_t exps_bytes, const void* w, const float* dloss, int64_t n_tok, int32_t d,
                          int64_t vocab, int32_t reduction, int32_t dtype, void* workspace, size_t workspace_bytes, void* dh, void* dw,
                          void* stream) {
     g_err[0] = 0;
@@ -983,12 +991,15 @@ int ethos_linear_ce_grad(const void* state, size_t state_bytes, const void* w, c
     if (n_tok == 0 || (!dh && !dw)) return 0;
     if (!state || !w || !dloss || !workspace) return fail(ETHOS_ENULL, "ethos_linear_ce_grad: null pointer");
     if (state_bytes < ethos::linear_ce_state_bytes(n_tok, d, dtype) ||
-        workspace_bytes < ethos::linear_ce_grad_workspace_bytes(n_tok, d, vocab, dtype, num_cus()))
+        workspace_bytes < ethos::linear_ce_grad_workspace_bytes(n_tok, d, vocab, dtype, num_cus(), exps != nullptr))
         return fail(ETHOS_EWORKSPACE, "ethos_linear_ce_grad: state of %zu or workspace of %zu bytes too small", state_bytes,
                     workspace_bytes);
-    if (!aligned16(state) || !aligned16(w) || !aligned16(workspace) || !aligned16(dh) || !aligned16(dw))
-        return fail(ETHOS_EALIGN, "ethos_linear_ce_grad: state, w, workspace, dh and dw must be 16-byte aligned");
-    return hip_status(ethos::launch_linear_ce_grad(state, w, dloss, n_tok, d, vocab, reduction, dtype, workspace, dh, dw, num_cus(),
+    if (exps && exps_bytes < ethos::linear_ce_exps_bytes(n_tok, vocab, dtype))
+        return fail(ETHOS_EWORKSPACE, "ethos_linear_ce_grad: exps of %zu bytes, %zu needed", exps_bytes,
+                    ethos::linear_ce_exps_bytes(n_tok, vocab, dtype));
+    if (!aligned16(state) || !aligned16(exps) || !aligned16(w) || !aligned16(workspace) || !aligned16(dh) || !aligned16(dw))
+        return fail(ETHOS_EALIGN, "ethos_linear_ce_grad: state, exps, w, workspace, dh and dw must be 16-byte aligned");
+    return hip_status(ethos::launch_linear_ce_grad(state, exps, w, dloss, n_tok, d, vocab, reduction, dtype, workspace, dh, dw, num_cus(),
                                                    (hipStream_t)stream),
                       "ethos_linear_ce_grad");
 }

@@ -9,6 +9,13 @@
 // of vocabulary.  The backward forms the logits of a piece of the vocabulary again, turns them into dl
 // (bf16) in its epilogue, and multiplies the piece by h and by W.
 //
+// Where dl of the whole vocabulary is at most what a piece may take, the forward under gradients leaves the
+// exponentials behind, E_iv = exp(l_iv - l_i,label) in bf16, in the memory that dl would take in the backward anyway: relative
+// to the label's own logit, which is known before the products, so that one factor per row, f_i = g_i exp(l_i,label -
+// lse_i), turns them into dl.  It is applied to h for dW and to the sums for dh, and the label's own value is put in
+// as 1 - exp(lse_i - l_i,label); the logits are then formed once.  Where a label lies more than e^60 below its row's
+// sum (or is infinite, or missing) the backward forms all logits again.
+//
 // float32 operands go through the same kernels as three bf16 planes each, x = hi + mid + lo
 // (ethos_split.hpp): a product is six bf16 products, exact in the float32 sums, the smallest first.
 #include <type_traits>
@@ -24,6 +31,7 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kScaled = 1e38f;  // logits below this in size can be scaled by log2(e)
+constexpr float kFar = 60.0f;     // kept exponentials reach e^60 relative to their label's (bf16 holds e^88)
 constexpr int kPadRows = 256;  // labelled rows are padded with zero rows to a multiple of this
 
 __host__ __device__ constexpr int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -39,7 +47,8 @@ struct CeState {
     float* lse;      // log of the sum of exponentials
     float* ll;       // logit of the label
     uint16_t* h;     // the labelled rows [planes][padded n][ldh]
-    int32_t* ticket; // zero between kernels
+    int32_t* ticket; // of the workgroups that finish the loss
+    int32_t* far;    // a label's logit is more than kFar below its row's log-sum
     int64_t np;      // n padded
     int ldh;
     size_t bytes;
@@ -54,7 +63,7 @@ CeState ce_state(char* p, int64_t n, int d, int dtype) {
         at += (bytes + 255) / 256 * 256;
         return r;
     };
-    s.count = (int32_t*)take(8);
+    s.count = (int32_t*)take(12);
     s.idx = (int32_t*)take(s.np * 4);
     s.inv = (int32_t*)take(s.np * 4);
     s.lab = (int32_t*)take(s.np * 4);
@@ -62,6 +71,7 @@ CeState ce_state(char* p, int64_t n, int d, int dtype) {
     s.ll = (float*)take(s.np * 4);
     s.h = (uint16_t*)take((size_t)s.np * s.ldh * 2 * planes_of(dtype));
     s.ticket = s.count + 1;
+    s.far = s.count + 2;
     s.bytes = at;
     return s;
 }
@@ -110,7 +120,7 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict
     }
     if (tid == 0) {
         *count = base;
-        *ticket = 0;
+        ticket[0] = ticket[1] = 0;  // (and CeState::far)
     }
 }
 
@@ -219,7 +229,7 @@ __global__ __launch_bounds__(256) void ce_few_rows_kernel(const int64_t* __restr
     }
     if (first && tid == 0) {
         *count = m;
-        *ticket = 0;
+        ticket[0] = ticket[1] = 0;  // (and CeState::far)
     }
     const int r = blockIdx.x * 4 + wave;
     if (r >= round_up(m, kPadRows)) return;
@@ -293,6 +303,7 @@ __global__ __launch_bounds__(1024) void ce_lse_kernel(const float2* __restrict__
         out = l - x;
         if (lane < 16 && r < m) {
             lse[r] = l;
+            if (!(fabsf(x) < kScaled && l - x <= kFar)) __hip_atomic_store(ticket + 1, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (reduction == kLossNone) loss[row] = out;
             else if (gridDim.x > 1) __hip_atomic_store(row_loss + r, out, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -635,7 +646,8 @@ __device__ __forceinline__ Place tile_place(int64_t block, int each) {
 }
 
 // Logits of a piece of the vocabulary, transposed (a lane holds values of two rows of h): GRAD 0: the
-// maximum and sum of exponentials over each wave's B / 2 words; 1: dl [planes][ldp / 256][np][256].
+// sum of exponentials over each wave's B / 2 words and what it is relative to; 1: dl [planes][ldp / 256][np][256]; 2: as
+// 0, and the exponentials in dl's place.
 struct LogitArgs {
     const uint16_t* w;   // the piece's first row, [planes][vocab][d]
     const float* w32;    // float32: the piece's first row itself
@@ -646,6 +658,7 @@ struct LogitArgs {
     float2* part;
     uint16_t* p;
     int d, ldh, reduction;
+    const int32_t* when;  // run only if it is not zero (null: run)
 };
 
 // A logit as a float32 chain: what an infinity needs, which against the other operand's lower planes gives
@@ -670,6 +683,7 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lds = lds_addr(smem), mine = lds + Ti::kLds + wave * 4096;
     const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
+    if (g.when && *g.when == 0) return;
     const int64_t words = g.v1 - g.v0, m = *g.count;
     // this workgroup's tiles: those of the vocabulary tiles of its XCD, one after the other, every gridDim / 8th
     const int n_tiles = (int)((m + B - 1) / B), xcd = blockIdx.x % 8;
@@ -701,6 +715,13 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                 const int64_t v = (int64_t)g.lab[rc] - g.v0 - tm0 - wm;
                 label_at[j] = v >= 0 && v < B / 2 && r < m && lane < 32 ? (int)v : -1;
                 label_value[j] = expm1f(g.ll[rc] - lse[j]) * k[j];  // exp(l - lse) - 1 without the cancellation
+            }
+        }
+        if constexpr (GRAD != 1) {
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const int64_t r = tn0 + wn + j * 32 + (lane & 31);
+                lse[j] = r < m ? g.ll[r] : 0.0f;  // what the row's exponentials are relative to
             }
         }
         f32x16_t acc[MI][NI];
@@ -744,35 +765,43 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
 #pragma unroll
                         for (int j = 0; j < NI; ++j) acc[i][j][e] = -__builtin_inff();
         }
-        if constexpr (GRAD == 0) {
+        if constexpr (GRAD != 1) {
+            // the sum of exponentials relative to the label's logit, or, beyond its reach, to the maximum
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 const int64_t r = tn0 + wn + j * 32 + (el & 31);
+                const bool in = r < m;
                 float x = -__builtin_inff();
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x = fmaxf(x, acc[i][j][e]);
                 x = fmaxf(x, __shfl_xor(x, 32));
-                float s = 0.0f;
-                if (ballot(!(fabsf(x) < kScaled)) == 0) {
-                    const float z = x * kLog2e;
+                float s = 0.0f, top = lse[j];
+                if (ballot(in && !(fabsf(top) < kScaled && x - top <= kFar)) == 0) {
+                    const float z = top * kLog2e;
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -z));
+                        for (int e = 0; e < 16; ++e) {
+                            const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -z));
+                            s += v;
+                            if (GRAD == 2) acc[i][j][e] = in ? v : 0.0f;
+                        }
                 } else {
+                    top = x;
                     const float z = x == -__builtin_inff() ? 0.0f : x;
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f((acc[i][j][e] - z) * kLog2e);
+                        for (int e = 0; e < 16; ++e) {
+                            s += __builtin_amdgcn_exp2f((acc[i][j][e] - z) * kLog2e);
+                            if (GRAD == 2) acc[i][j][e] = 0.0f;  // (kept exponentials of such a row are not used)
+                        }
                 }
                 s += __shfl_xor(s, 32);
-                if (el < 32) g.part[((g.v0 + tm0) / (B / 2) + wave / Ti::kWN) * g.np + r] = make_float2(x, s);
+                if (el < 32) g.part[((g.v0 + tm0) / (B / 2) + wave / Ti::kWN) * g.np + r] = make_float2(top, s);
             }
-            if (!more) break;
-            step_barrier();
         } else {
             // dl, in place
 #pragma unroll
@@ -794,6 +823,11 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                         acc[i][j][e] = in ? v : 0.0f;
                     }
             }
+        }
+        if constexpr (GRAD == 0) {
+            if (!more) break;
+            step_barrier();
+        } else {
             // the next tile's copies, before the stores, which no one waits for
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             // 32 rows by 64 words at a time through the wave's own LDS; what a plane leaves stays in acc
@@ -821,14 +855,15 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                                 typedef __attribute__((address_space(3))) u32x2_t* ptr;
                                 *(ptr)(size_t)(mine + n * 128 + (k_piece<64>(n, i * 4 + (e >> 2)) << 4) + 8 * (el >> 5)) = u32x2_t{q[0], q[1]};
                             }
-                        if (label_at[j] >= 0 && label_at[j] / 64 == c) {
+                        asm volatile("" ::: "memory");
+                        if (GRAD == 1 && label_at[j] >= 0 && label_at[j] / 64 == c) {
                             typedef __attribute__((address_space(3))) uint16_t* ptr;
                             const int w = label_at[j] % 64;
                             const uint16_t x = f32_to_bf16_bits(label_value[j]);
                             label_value[j] -= bf16_bits_to_f32(x);
                             *(ptr)(size_t)(mine + n * 128 + (k_piece<64>(n, w >> 3) << 4) + (w & 7) * 2) = x;
                         }
-                        __builtin_amdgcn_wave_barrier();
+                        asm volatile("" ::: "memory");
                         uint16_t* out = g.p + pl * g.np * g.ldp + (tm0 / kPanel * g.np + tn0 + wn + j * 32) * kPanel + tm0 % kPanel + wm + c * 64;
 #pragma unroll
                         for (int t = 0; t < 4; ++t) {
@@ -837,7 +872,7 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                             __builtin_nontemporal_store(*(ptr)(size_t)(mine + r * 128 + (k_piece<64>(r, el & 7) << 4)),
                                                         reinterpret_cast<u32x4_t*>(out + r * kPanel + (el & 7) * 8));
                         }
-                        __builtin_amdgcn_wave_barrier();
+                        asm volatile("" ::: "memory");
                     }
             if (!more) break;
             lds_barrier();
@@ -969,7 +1004,8 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_grads_kernel(GradArgs
 template <typename T>
 __global__ __launch_bounds__(256) void ce_row_grad_out_kernel(const float* __restrict__ part, const int32_t* __restrict__ count,
                                                               const int32_t* __restrict__ inv, int64_t n, int d, int tile, int cols,
-                                                              int64_t ldp, int num_cus, int with_dw, T* __restrict__ dh) {
+                                                              int64_t ldp, int num_cus, int with_dw, const float* __restrict__ factor,
+                                                              T* __restrict__ dh) {
     const int64_t m = *count, size = round_up(m, kPadRows) * d;
     const int parts = dh_parts(m, tile, cols, ldp, num_cus, with_dw);
     const int64_t total = n * (d / 4);
@@ -992,8 +1028,69 @@ __global__ __launch_bounds__(256) void ce_row_grad_out_kernel(const float* __res
                     s.w += v[p].w;
                 }
             }
+        if (factor && at >= 0) {
+            const float f = factor[at];
+            s.x *= f;
+            s.y *= f;
+            s.z *= f;
+            s.w *= f;
+        }
         if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dh + r * d + c) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
         else *reinterpret_cast<float4*>(dh + r * d + c) = s;
+    }
+}
+
+// What turns kept exponentials into dl, a wave per row of the dense block: the row's factor, its row of h times it, the
+// label's value.  (Where the logits are formed again, dl is whole: the factor is one.)
+struct FactorArgs {
+    const int32_t *count, *idx, *lab, *far;
+    const float *lse, *ll, *dloss;
+    const uint16_t* h;
+    uint16_t *scaled, *e;
+    float* factor;
+    int64_t np, ldp;
+    int ldh, reduction;
+};
+template <int PL>
+__global__ __launch_bounds__(256) void ce_factor_kernel(FactorArgs g) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t m = *g.count;
+    if (r >= round_up(m, kPadRows)) return;
+    const bool far = *g.far != 0;
+    float f = 1.0f;
+    if (r < m && !far) {
+        const float below = g.lse[r] - g.ll[r];
+        f = row_gradient(g.dloss, g.idx, r, m, g.reduction) * expf(-below);
+        if (lane == 0) {
+            const int64_t v = g.lab[r];
+            float x = -expm1f(below);
+#pragma unroll
+            for (int i = 0; i < PL; ++i) {
+                const uint16_t q = f32_to_bf16_bits(x);
+                x -= bf16_bits_to_f32(q);
+                g.e[i * g.np * g.ldp + (v / kPanel * g.np + r) * kPanel + v % kPanel] = q;
+            }
+        }
+    }
+    if (lane == 0) g.factor[r] = f;
+    const int64_t plane = g.np * g.ldh;
+    for (int c = lane * 8; c < g.ldh; c += 64 * 8) {
+        const int64_t at = r * g.ldh + c;
+        float x[8], y[8];
+        Vec16<uint16_t>::unpack(*reinterpret_cast<const uint4*>(g.h + at), x);
+        if constexpr (PL > 1) {
+#pragma unroll
+            for (int i = PL - 1; i > 0; --i) {
+                Vec16<uint16_t>::unpack(*reinterpret_cast<const uint4*>(g.h + at + i * plane), y);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] += y[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= f;
+        if constexpr (PL > 1) put_planes(x, g.scaled + at, plane);
+        else *reinterpret_cast<uint4*>(g.scaled + at) = Vec16<uint16_t>::pack(x);
     }
 }
 
@@ -1045,26 +1142,30 @@ FwdWs fwd_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
 }
 
 struct GradWs {
-    uint16_t* p;  // dl of a piece
+    uint16_t* p;  // dl of a piece (not kept exponentials, which have their own memory)
+    uint16_t* h;  // kept exponentials: h times the rows' factors
+    float* factor;
     float* part;  // dh's parts
     uint16_t* w;  // float32: W's planes
     int64_t piece, part_tiles;
     int logit_tile, grad_tile;
     size_t bytes;
 };
-GradWs grad_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
+GradWs grad_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus, bool kept) {
     GradWs w;
     Take take{p};
     const int64_t np = round_up(n, kPadRows);
     const int planes = planes_of(dtype);
-    w.piece = piece_words(np, vocab, planes);
+    w.piece = kept ? round_up(vocab, kTileMax) : piece_words(np, vocab, planes);
     const int64_t words = vocab < w.piece ? vocab : w.piece;
     w.logit_tile = tile_for(words, n, num_cus);
     // tiles of 256 for the gradients where dW's and dh's parts give every CU one
     const int64_t cols256 = (d + 255) / 256, m256 = (n + 255) / 256 * cols256;
     const int64_t row256 = m256 * (num_cus / m256 < 1 ? 1 : num_cus / m256 < w.piece / kPartWords ? num_cus / m256 : w.piece / kPartWords);
     w.grad_tile = d > 128 && (words + 255) / 256 * cols256 + row256 >= num_cus ? 256 : 128;
-    w.p = (uint16_t*)take((size_t)np * w.piece * 2 * planes);
+    w.p = kept ? nullptr : (uint16_t*)take((size_t)np * w.piece * 2 * planes);
+    w.h = kept ? (uint16_t*)take((size_t)np * round_up(d, 64) * 2 * planes) : nullptr;
+    w.factor = kept ? (float*)take((size_t)np * 4) : nullptr;
     // parts x tiles of rows for any count of labelled rows: as many as fill the chip, or one part
     const int64_t cols = (d + w.grad_tile - 1) / w.grad_tile, slots = num_cus / cols;
     w.part_tiles = slots > np / w.grad_tile ? slots : np / w.grad_tile;
@@ -1134,12 +1235,16 @@ size_t linear_ce_state_bytes(int64_t n, int d, int dtype) { return ce_state(null
 size_t linear_ce_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
     return fwd_ws(nullptr, n, d, vocab, dtype, num_cus).bytes;
 }
-size_t linear_ce_grad_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
-    return grad_ws(nullptr, n, d, vocab, dtype, num_cus).bytes;
+size_t linear_ce_exps_bytes(int64_t n, int64_t vocab, int dtype) {
+    return (size_t)round_up(n, kPadRows) * round_up(vocab, kTileMax) * 2 * planes_of(dtype);
+}
+size_t linear_ce_grad_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus, bool kept) {
+    return grad_ws(nullptr, n, d, vocab, dtype, num_cus, kept).bytes;
 }
 
 int launch_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* labels, int64_t n, int d, int64_t vocab,
-                     int64_t ignore, int reduction, int dtype, void* state, void* ws, float* loss, int num_cus, hipStream_t stream) {
+                     int64_t ignore, int reduction, int dtype, void* state, void* exps, void* ws, float* loss, int num_cus,
+                     hipStream_t stream) {
     const CeState s = ce_state((char*)state, n, d, dtype);
     const FwdWs f = fwd_ws((char*)ws, n, d, vocab, dtype, num_cus);
     float* loss_rows = reduction == kLossNone ? loss : nullptr;
@@ -1164,29 +1269,42 @@ int launch_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* l
     }
     LogitArgs g = logit_args(s, w, f.w, 0, vocab, vocab, d, dtype);
     g.part = f.part;
-    run_logits<0>(g, f.tile, dtype, n, num_cus, stream);
+    if (exps) {
+        g.p = (uint16_t*)exps;
+        g.ldp = round_up(vocab, kTileMax);
+        run_logits<2>(g, f.tile, dtype, n, num_cus, stream);
+    } else {
+        run_logits<0>(g, f.tile, dtype, n, num_cus, stream);
+    }
     hipLaunchKernelGGL(ce_lse_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, stream, f.part, f.n_part, s.np, s.count, s.idx, s.ll,
                        reduction, s.lse, f.row_loss, s.ticket, loss);
     return (int)hipGetLastError();
 }
 
-int launch_linear_ce_grad(const void* state, const void* w, const float* dloss, int64_t n, int d, int64_t vocab, int reduction,
+int launch_linear_ce_grad(const void* state, void* exps, const void* w, const float* dloss, int64_t n, int d, int64_t vocab, int reduction,
                           int dtype, void* ws, void* dh, void* dw, int num_cus, hipStream_t stream) {
     const CeState s = ce_state((char*)state, n, d, dtype);
-    const GradWs b = grad_ws((char*)ws, n, d, vocab, dtype, num_cus);
+    const GradWs b = grad_ws((char*)ws, n, d, vocab, dtype, num_cus, exps != nullptr);
     const int cols = (d + b.grad_tile - 1) / b.grad_tile;
     if (dtype != kBF16) split_weights(w, vocab, d, b.w, num_cus, stream);
     for (int64_t v0 = 0; v0 < vocab; v0 += b.piece) {
         const int64_t words = vocab - v0 < b.piece ? vocab - v0 : b.piece;
         LogitArgs g = logit_args(s, w, b.w, v0, v0 + words, vocab, d, dtype);
-        g.p = b.p;
+        g.p = exps ? (uint16_t*)exps : b.p;
         g.ldp = b.piece;
         g.dloss = dloss;
         g.reduction = reduction;
+        g.when = exps ? s.far : nullptr;
         run_logits<1>(g, b.logit_tile, dtype, n, num_cus, stream);
+        if (exps) {
+            const FactorArgs a{s.count, s.idx, s.lab, s.far, s.lse, s.ll, dloss, s.h, b.h, g.p, b.factor, s.np, b.piece, s.ldh, reduction};
+            const dim3 grid((unsigned)(s.np / 4));
+            if (dtype == kBF16) hipLaunchKernelGGL((ce_factor_kernel<1>), grid, dim3(256), 0, stream, a);
+            else hipLaunchKernelGGL((ce_factor_kernel<3>), grid, dim3(256), 0, stream, a);
+        }
         const int64_t row_blocks = dh ? xcd_grid(b.part_tiles, cols) : 0;
         const int64_t head_blocks = dw ? xcd_grid((words + b.grad_tile - 1) / b.grad_tile, cols) : 0;
-        const GradArgs a{b.p, s.h, g.w, s.count, words, s.np, b.piece, g.w_plane, b.part, (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4), d,
+        const GradArgs a{g.p, exps ? b.h : s.h, g.w, s.count, words, s.np, b.piece, g.w_plane, b.part, (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4), d,
                          s.ldh, cols, num_cus, v0 > 0 ? 1 : 0, dw ? 1 : 0, row_blocks};
         with_tile(b.grad_tile, dtype, [&](auto t, auto pl) {
             constexpr int B = decltype(t)::v, PL = decltype(pl)::v;
@@ -1198,10 +1316,10 @@ int launch_linear_ce_grad(const void* state, const void* w, const float* dloss, 
         blocks = blocks < num_cus * 16 ? blocks : num_cus * 16;
         if (dtype == kBF16)
             hipLaunchKernelGGL((ce_row_grad_out_kernel<uint16_t>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, n,
-                               d, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, (uint16_t*)dh);
+                               d, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, b.factor, (uint16_t*)dh);
         else
             hipLaunchKernelGGL((ce_row_grad_out_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, n, d,
-                               b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, (float*)dh);
+                               b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, b.factor, (float*)dh);
     }
     return (int)hipGetLastError();
 }

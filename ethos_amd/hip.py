@@ -682,33 +682,38 @@ FLOATS = (torch.bfloat16, torch.float32)
 INTS = (torch.int32, torch.int64)
 
 
-def linear_ce(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, ignore_index: int, reduction: str):
-    """(loss float32, state): softmax cross entropy of h [n, d] (rows evenly spaced) against w [V, d];
-    the state is what linear_ce_grad takes."""
+def linear_ce(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, ignore_index: int, reduction: str, keep: int = 0):
+    """(loss float32, state, exps): softmax cross entropy of h [n, d] (rows evenly spaced) against w [V, d];
+    the state and exps (None where they would take more than `keep` bytes) are what linear_ce_grad takes."""
     _need_here(w, "weight", FLOATS, 2)
     _need_here(labels, "labels", (torch.int64,), 1)
     n, d = h.shape
-    code, lib = dtype_code(h.dtype), load()
+    code, lib, device = dtype_code(h.dtype), load(), h.device
     V = w.shape[0]
-    st, st_bytes = _scratch("ethos_linear_ce_state_bytes", h.device, n, d, code)
-    ws, ws_bytes = _scratch("ethos_linear_ce_workspace_bytes", h.device, n, d, V, code)
-    loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=h.device)
+    st, st_bytes = _scratch("ethos_linear_ce_state_bytes", device, n, d, code)
+    ws, ws_bytes = _scratch("ethos_linear_ce_workspace_bytes", device, n, d, V, code)
+    exps, exps_bytes = None, _size("ethos_linear_ce_exps_bytes", device.index, n, V, code) if keep else 0
+    if keep and exps_bytes <= keep:
+        exps, exps_bytes = workspace(exps_bytes, device)
+    loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=device)
     rc = lib.ethos_linear_ce(h.data_ptr(), h.stride(0) if n > 1 else d, w.data_ptr(), labels.data_ptr(), n, d, V, int(ignore_index),
-                             REDUCTIONS[reduction], code, st.data_ptr(), st_bytes, ws.data_ptr(), ws_bytes, loss.data_ptr(), _stream())
+                             REDUCTIONS[reduction], code, st.data_ptr(), st_bytes, exps.data_ptr() if exps is not None else None,
+                             exps_bytes, ws.data_ptr(), ws_bytes, loss.data_ptr(), _stream())
     check(rc, "ethos_linear_ce")
-    return loss, st
+    return loss, st, exps
 
 
-def linear_ce_grad(state: torch.Tensor, w: torch.Tensor, dloss: torch.Tensor, n: int, reduction: str, want_h: bool, want_w: bool):
+def linear_ce_grad(state: torch.Tensor, exps: torch.Tensor | None, w: torch.Tensor, dloss: torch.Tensor, n: int, reduction: str,
+                   want_h: bool, want_w: bool):
     """(dh [n, d], dw [V, d]) from dloss (float32, contiguous); None for one not wanted."""
     V, d = w.shape
-    code, lib = dtype_code(w.dtype), load()
-    ws, ws_bytes = _scratch("ethos_linear_ce_grad_workspace_bytes", w.device, n, d, V, code)
+    code, lib, kept = dtype_code(w.dtype), load(), exps is not None
+    ws, ws_bytes = _scratch("ethos_linear_ce_grad_workspace_bytes", w.device, n, d, V, code, int(kept))
     dh = torch.empty((n, d), dtype=w.dtype, device=w.device) if want_h else None
     dw = torch.empty((V, d), dtype=w.dtype, device=w.device) if want_w else None
-    rc = lib.ethos_linear_ce_grad(state.data_ptr(), state.numel() * 8, w.data_ptr(), dloss.data_ptr(), n, d, V, REDUCTIONS[reduction],
-                                  code, ws.data_ptr(), ws_bytes, dh.data_ptr() if want_h else None,
-                                  dw.data_ptr() if want_w else None, _stream())
+    rc = lib.ethos_linear_ce_grad(state.data_ptr(), state.numel() * 8, exps.data_ptr() if kept else None, exps.numel() * 8 if kept else 0,
+                                  w.data_ptr(), dloss.data_ptr(), n, d, V, REDUCTIONS[reduction], code, ws.data_ptr(), ws_bytes,
+                                  dh.data_ptr() if want_h else None, dw.data_ptr() if want_w else None, _stream())
     check(rc, "ethos_linear_ce_grad")
     return dh, dw
 

@@ -58,11 +58,11 @@ def _device_check(name: str, t: torch.Tensor) -> None:
 # -------------------------------------------------------------------------- cross entropy
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h, weight, labels, ignore_index, reduction):
+    def forward(ctx, h, weight, labels, ignore_index, reduction, keep_bytes):
         rows, w = _rows(h), _dense(weight)
-        loss, state = hip.linear_ce(rows, w, labels, ignore_index, reduction)
         # the weight itself is saved, so that a change in place before the backward is noticed
-        ctx.save_for_backward(state, weight)
+        loss, state, exps = hip.linear_ce(rows, w, labels, ignore_index, reduction, keep_bytes)
+        ctx.save_for_backward(weight, state, exps)
         ctx.copy = w if w.data_ptr() != weight.data_ptr() else None
         ctx.shape, ctx.reduction = h.shape, reduction
         return loss
@@ -70,24 +70,26 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        state, weight = ctx.saved_tensors
+        weight, state, exps = ctx.saved_tensors
         w = weight.detach() if ctx.copy is None else ctx.copy
         n = math.prod(ctx.shape[:-1])
         want_h, want_w = ctx.needs_input_grad[:2]
-        dh, dw = hip.linear_ce_grad(state, w, dloss.float().contiguous(), n, ctx.reduction, want_h, want_w)
-        return dh.view(ctx.shape) if want_h else None, dw, None, None, None
+        dh, dw = hip.linear_ce_grad(state, exps, w, dloss.float().contiguous(), n, ctx.reduction, want_h, want_w)
+        return dh.view(ctx.shape) if want_h else None, dw, None, None, None, None
 
 
 def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
-                         reduction: str = "mean") -> torch.Tensor:
+                         reduction: str = "mean", keep_bytes: int = 1 << 30) -> torch.Tensor:
     """Softmax cross entropy of h @ weight.T against labels, without forming the logits.
 
     h [..., d] and weight [vocab, d] of one dtype (bf16 or float32), d a multiple of 8 up to 32768;
     labels int64 [...].  Positions whose label is `ignore_index` have no part in the loss or its
     gradients; another label outside the vocabulary makes the loss NaN.  `reduction`: "mean" over the
     labelled positions (NaN without one), "sum", or "none" (float32 [...], zero where ignored).  The
-    loss is float32.  Gradients go to h and weight, in their dtype; logits are formed a second time
-    for them, a piece of the vocabulary at a time."""
+    loss is float32.  Gradients go to h and weight, in their dtype.  For them the forward leaves the
+    exponentials behind in 16 bits (float32: 48) where these take at most `keep_bytes`, in the memory that
+    the backward would take anyway; else, and with 0, the backward forms the logits again, a piece of the
+    vocabulary at a time."""
     for name, t in (("h", h), ("weight", weight), ("labels", labels)):
         _device_check(name, t)
     if reduction not in ("mean", "sum", "none"):
@@ -106,7 +108,7 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
         return zero if reduction != "mean" else zero / 0.0
     flat = labels.contiguous().view(-1)
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
-        loss = _LinearCrossEntropy.apply(h, weight, flat, int(ignore_index), reduction)
+        loss = _LinearCrossEntropy.apply(h, weight, flat, int(ignore_index), reduction, int(keep_bytes))
     else:
         loss = hip.linear_ce(_rows(h), _dense(weight), flat, int(ignore_index), reduction)[0]
     return loss.view(labels.shape) if reduction == "none" else loss

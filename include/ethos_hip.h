@@ -512,13 +512,17 @@ int ethos_layer_forward(const void* x, const void* wq, const void* wq_prepared, 
  *   state   >= ethos_linear_ce_state_bytes(...) bytes: what ethos_linear_ce_grad reads (the rows with
  *           a label in dense form, their log-sums)
  *   loss    float32, one value or (NONE) [n_tok]
+ *   exps    NULL, or >= ethos_linear_ce_exps_bytes(...) bytes: the forward leaves the exponentials in bf16
+ *           (float32: three bf16 planes) there for ethos_linear_ce_grad, which then does not form the logits
+ *           again (unless a label lies more than e^60 below its row's sum).  Both calls, or neither, get it.
  * Logits, exponentials' sums and losses are float32, a reduction's sum float64.
  * ethos_linear_ce_grad: dh [n_tok, d] and dw [vocab, d] of dtype T (either may be NULL) from dloss
- * (float32: one value or, NONE, [n_tok]), with the state that the forward left and the same w.  It
- * forms a piece of the vocabulary's logits at a time again (at most 1 GiB, or 256 words); for bf16 the
- * logits' gradients are rounded to bf16 for the products with h and w.
+ * (float32: one value or, NONE, [n_tok]), with the state that the forward left and the same w.  Without exps it
+ * forms a piece of the vocabulary's logits at a time again (their gradients take at most 1 GiB, or 256 words); for
+ * bf16 the logits' gradients are rounded to bf16 for the products with h and w (with exps the exponentials are, and
+ * h times a factor per row).
  * Limits: d a multiple of 8, at most 32768; ldh a multiple of 8 (bf16) or 4; vocab <= 2^30; n_tok
- * <= 2^30; h, w, state, workspace, dh and dw 16-byte aligned.  n_tok = 0 does nothing.
+ * <= 2^30; h, w, state, exps, workspace, dh and dw 16-byte aligned.  n_tok = 0 does nothing.
  */
 #define ETHOS_LOSS_MEAN 0
 #define ETHOS_LOSS_SUM 1
@@ -526,10 +530,11 @@ int ethos_layer_forward(const void* x, const void* wq, const void* wq_prepared, 
 size_t ethos_linear_ce_state_bytes(int64_t n_tok, int32_t d, int32_t dtype);
 size_t ethos_linear_ce_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype);
 int ethos_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* labels, int64_t n_tok, int32_t d, int64_t vocab,
-                    int64_t ignore_index, int32_t reduction, int32_t dtype, void* state, size_t state_bytes, void* workspace,
-                    size_t workspace_bytes, float* loss, void* stream);
-size_t ethos_linear_ce_grad_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype);
-int ethos_linear_ce_grad(const void* state, size_t state_bytes, const void* w, const float* dloss, int64_t n_tok, int32_t d,
+                    int64_t ignore_index, int32_t reduction, int32_t dtype, void* state, size_t state_bytes, void* exps, size_t exps_bytes,
+                    void* workspace, size_t workspace_bytes, float* loss, void* stream);
+size_t ethos_linear_ce_exps_bytes(int64_t n_tok, int64_t vocab, int32_t dtype);
+size_t ethos_linear_ce_grad_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype, int32_t kept);
+int ethos_linear_ce_grad(const void* state, size_t state_bytes, void* exps, size_t exps_bytes, const void* w, const float* dloss, int64_t n_tok, int32_t d,
                          int64_t vocab, int32_t reduction, int32_t dtype, void* workspace, size_t workspace_bytes, void* dh, void* dw,
                          void* stream);
 

@@ -32,11 +32,12 @@ def _ce_inputs(n, d, V, dt, seed=0, ignored=0.0):
     return h.to(dt), w.to(dt), labels
 
 
-def _ce_oracle(h, w, labels, reduction, gy):
+def _ce_oracle(h, w, labels, reduction, gy, kept=True):
     """(loss, dh, dw) in float64 and bounds of their errors: a logit's sum of d products is off by at
     most (d + 2) U times the sum of the products' sizes, the log-sum by that of its largest logit and a
     few roundings of its own; dl is off by its factor's error and (bf16) its rounding, the products
-    with it by their sums of float32 additions, the results by their rounding."""
+    with it by their sums of float32 additions, the results by their rounding.  `kept`: dW's products take
+    exponentials and h times a factor per row, each rounded once."""
     x, m = h.double(), w.double()
     n, V, d = len(x), len(m), x.shape[1]
     keep = labels != -100
@@ -67,7 +68,7 @@ def _ce_oracle(h, w, labels, reduction, gy):
     e_dl = e_dl * g.abs()[:, None] + dl.abs() * (8 * U + (t if h.dtype == torch.bfloat16 else 0.0))
     dh, dw = dl @ m, dl.T @ x
     e_dh = e_dl @ m.abs() + (V + 64) * U * (dl.abs() @ m.abs()) + t * dh.abs() * 1.01
-    e_dw = e_dl.T @ x.abs() + (n + 64) * U * (dl.abs().T @ x.abs()) + t * dw.abs() * 1.01
+    e_dw = e_dl.T @ x.abs() + ((n + 64) * U + (t if kept and h.dtype == torch.bfloat16 else 0.0)) * (dl.abs().T @ x.abs()) + t * dw.abs() * 1.01
     return (loss, dh, dw), (e_loss, e_dh, e_dw)
 
 
@@ -85,12 +86,12 @@ CE_SIZES = [(1, 64, 500), (2, 8, 1), (7, 1024, 1000), (255, 72, 511), (256, 64, 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
 @pytest.mark.parametrize("n,d,V", CE_SIZES)
 def test_cross_entropy_against_float64(n, d, V, dt, reduction):
-    for ignored in (0.0, 0.6, 1.0):
+    for ignored, keep in ((0.0, 1 << 30), (0.6, 1 << 30), (0.6, 0), (1.0, 1 << 30), (1.0, 0)):
         h, w, labels = _ce_inputs(n, d, V, DT[dt], seed=n + V, ignored=ignored)
         gy = torch.randn(n if reduction == "none" else (), generator=_gen(5), device="cuda")
-        want, bound = _ce_oracle(h, w, labels, reduction, gy)
+        want, bound = _ce_oracle(h, w, labels, reduction, gy, kept=keep > 0)
         a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
-        loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction=reduction)
+        loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction=reduction, keep_bytes=keep)
         assert loss.dtype == torch.float32
         dh, dw = torch.autograd.grad(loss, (a, b), gy)
         assert dh.dtype == h.dtype and dw.dtype == w.dtype and dh.shape == h.shape and dw.shape == w.shape
@@ -105,7 +106,9 @@ def test_cross_entropy_against_float64(n, d, V, dt, reduction):
         for got, x, e, what in zip((loss.detach(), dh, dw), want, bound, ("loss", "dh", "dw")):
             _within(got, x, e, f"{what} ignored={ignored}")
         assert bool((dh[labels == -100] == 0).all())
-        again = torch.autograd.grad(ethos_amd.linear_cross_entropy(a, b, labels, reduction=reduction), (a, b), gy)
+        loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction=reduction, keep_bytes=keep)
+        torch.autograd.grad(loss, (a, b), gy * 3.0, retain_graph=True)
+        again = torch.autograd.grad(loss, (a, b), gy)
         assert torch.equal(again[0], dh) and torch.equal(again[1], dw)
 
 
@@ -113,7 +116,7 @@ def test_cross_entropy_against_float64(n, d, V, dt, reduction):
 def test_cross_entropy_several_pieces_of_vocabulary(dt, n, d, V):
     h, w, labels = _ce_inputs(n, d, V, DT[dt], seed=3, ignored=0.1)
     gy = torch.ones((), device="cuda")
-    want, bound = _ce_oracle(h, w, labels, "mean", gy)
+    want, bound = _ce_oracle(h, w, labels, "mean", gy, kept=False)  # 1.15 GB and 1.7 GB are not kept
     a, b = h.requires_grad_(), w.requires_grad_()
     loss = ethos_amd.linear_cross_entropy(a, b, labels)
     for got, x, e, what in zip((loss.detach(), *torch.autograd.grad(loss, (a, b), gy)), want, bound, ("loss", "dh", "dw")):
@@ -121,14 +124,14 @@ def test_cross_entropy_several_pieces_of_vocabulary(dt, n, d, V):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
-@pytest.mark.parametrize("n,ignored", [(700, 0.0), (1300, 0.5)])
-def test_cross_entropy_in_the_largest_tiles(dt, n, ignored):
+@pytest.mark.parametrize("n,ignored,keep", [(700, 0.0, 1 << 30), (1300, 0.5, 0), (1300, 0.5, 1 << 30)])
+def test_cross_entropy_in_the_largest_tiles(dt, n, ignored, keep):
     d, V = 264, 30011
     h, w, labels = _ce_inputs(n, d, V, DT[dt], seed=n, ignored=ignored)
     gy = torch.rand(n, generator=_gen(2), device="cuda")
-    want, bound = _ce_oracle(h, w, labels, "none", gy)
+    want, bound = _ce_oracle(h, w, labels, "none", gy, kept=keep > 0)
     a, b = h.requires_grad_(), w.requires_grad_()
-    loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="none")
+    loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="none", keep_bytes=keep)
     for got, x, e, what in zip((loss.detach(), *torch.autograd.grad(loss, (a, b), gy)), want, bound, ("loss", "dh", "dw")):
         _within(got, x, e, what)
 
@@ -202,6 +205,27 @@ def test_cross_entropy_masked_words_large_logits_and_wrong_labels(dt):
     assert ethos_amd.linear_cross_entropy(h, w.detach(), labels, reduction="none").isnan().nonzero()[:, 0].tolist() == [9]
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_cross_entropy_with_a_few_labels_out_of_reach(dt):
+    """Kept exponentials are not used where a label's logit is far below its row's sum: one row of 300
+    at 61 below, one at 59 (used), one at 400."""
+    h, w, labels = _ce_inputs(300, 64, 900, DT[dt], seed=12)
+    g = _gen(4)
+    for rows in ((5,), (5, 6, 7)):
+        x = h.clone()
+        for row, below in zip(rows, (59.0, 61.0, 400.0)):
+            # a row against its label's: h = -c w, with c so that its logit is `below` under the others' sum
+            v = w[labels[row]].double()
+            c = below / float(v @ v)
+            x[row] = (-c * v).to(x.dtype)
+        a, b = x.requires_grad_(), w.clone().requires_grad_()
+        gy = torch.rand(300, generator=g, device="cuda")
+        want, bound = _ce_oracle(a.detach(), b.detach(), labels, "none", gy)
+        loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="none")
+        for got, y, e, what in zip((loss.detach(), *torch.autograd.grad(loss, (a, b), gy)), want, bound, ("loss", "dh", "dw")):
+            _within(got, y, e, f"{what} {rows}")
+
+
 def test_cross_entropy_table_past_32_bits():
     n, d, V = 5, 16384, 140000  # 4.6 GB
     w = torch.empty(V, d, dtype=torch.bfloat16, device="cuda")
@@ -225,7 +249,7 @@ def test_cross_entropy_table_past_32_bits():
     u = half_step(torch.bfloat16)
     for v in (0, 1, 65535, 65536, 131071, 131072, 131073, V - 2, V - 1):
         x = dl[:, v] @ h.detach()[keep].double()
-        _within(dw[v], x, (u + 3 * e + 2.0 ** -19) * (dl[:, v].abs() @ h.detach()[keep].double().abs()) + u * x.abs(), f"dw[{v}]")
+        _within(dw[v], x, (2 * u + 3 * e + 2.0 ** -19) * (dl[:, v].abs() @ h.detach()[keep].double().abs()) + u * x.abs(), f"dw[{v}]")
     x = sum(dl[:, i:i + 10000] @ p.double() for i, p in zip(range(0, V, 10000), w.detach().split(10000)))
     m = sum(dl[:, i:i + 10000].abs() @ p.double().abs() for i, p in zip(range(0, V, 10000), w.detach().split(10000)))
     _within(dh[keep], x, (u + 3 * e + 2.0 ** -19 + V * U) * m + u * x.abs(), "dh")
@@ -455,15 +479,24 @@ def test_on_another_stream_and_in_a_graph(dt):
         assert all(torch.equal(a, b) for a, b in zip(held, want)), seed
 
 
-def test_no_copy_of_the_logits():
-    """The loss's memory beside its inputs and outputs stays a small part of the logits'."""
+@pytest.mark.parametrize("train", [False, True])
+def test_no_copy_of_the_logits(train):
+    """Without gradients, or with none of the exponentials kept, the loss's memory beside its inputs and
+    outputs stays a small part of the logits'; what is kept for a backward is gone after it."""
     h, w, labels = _ce_inputs(4096, 64, 100000, torch.bfloat16)
+    h.requires_grad_(train)
     torch.cuda.synchronize()
     torch.cuda.reset_peak_memory_stats()
     before = torch.cuda.memory_allocated()
-    ethos_amd.linear_cross_entropy(h, w, labels)
+    loss = ethos_amd.linear_cross_entropy(h, w, labels, keep_bytes=0 if train else 1 << 30)
     torch.cuda.synchronize()
     assert torch.cuda.max_memory_allocated() - before < 4096 * 100000 * 4 / 20
+    if train:
+        del loss
+        loss = ethos_amd.linear_cross_entropy(h, w, labels)
+        assert torch.cuda.memory_allocated() - before > 4096 * 100000 * 2
+        dh = torch.autograd.grad(loss, h)[0]
+        assert torch.cuda.memory_allocated() - before < 4096 * 100000 * 2 / 20 and dh.shape == h.shape
 
 
 def test_wrappers_refuse_other_devices(monkeypatch):

@@ -13,8 +13,9 @@ def test_linear_ce_argument_errors_are_codes():
     L = _lib.load()
     big = 1 << 40
 
-    def ce(h=16, ldh=64, w=16, labels=16, n=4, d=64, V=9, ignore=-100, red=0, dt=1, st=16, st_bytes=big, ws=16, ws_bytes=big, loss=16):
-        return L.ethos_linear_ce(h, ldh, w, labels, n, d, V, ignore, red, dt, st, st_bytes, ws, ws_bytes, loss, None)
+    def ce(h=16, ldh=64, w=16, labels=16, n=4, d=64, V=9, ignore=-100, red=0, dt=1, st=16, st_bytes=big, ex=None, ex_bytes=0,
+           ws=16, ws_bytes=big, loss=16):
+        return L.ethos_linear_ce(h, ldh, w, labels, n, d, V, ignore, red, dt, st, st_bytes, ex, ex_bytes, ws, ws_bytes, loss, None)
 
     assert ce(dt=2) == -1 and b"dtype" in L.ethos_last_error()
     for bad in (dict(n=-1), dict(n=(1 << 30) + 1), dict(d=0), dict(V=0), dict(V=(1 << 30) + 1), dict(red=3), dict(red=-1), dict(ldh=56)):
@@ -27,17 +28,19 @@ def test_linear_ce_argument_errors_are_codes():
             assert ce(**{name: 24}) == -4, name
     assert ce(st_bytes=L.ethos_linear_ce_state_bytes(4, 64, 1) - 1) == -5
     assert ce(ws_bytes=L.ethos_linear_ce_workspace_bytes(4, 64, 9, 1) - 1) == -5
+    assert ce(ex=16, ex_bytes=L.ethos_linear_ce_exps_bytes(4, 9, 1) - 1) == -5 and ce(ex=24, ex_bytes=big) == -4
     assert ce(n=0, h=None) == 0 and L.ethos_last_error() == b""
 
-    def grad(st=16, st_bytes=big, w=16, dl=16, n=4, d=64, V=9, red=0, dt=1, ws=16, ws_bytes=big, dh=16, dw=16):
-        return L.ethos_linear_ce_grad(st, st_bytes, w, dl, n, d, V, red, dt, ws, ws_bytes, dh, dw, None)
+    def grad(st=16, st_bytes=big, ex=None, ex_bytes=0, w=16, dl=16, n=4, d=64, V=9, red=0, dt=1, ws=16, ws_bytes=big, dh=16, dw=16):
+        return L.ethos_linear_ce_grad(st, st_bytes, ex, ex_bytes, w, dl, n, d, V, red, dt, ws, ws_bytes, dh, dw, None)
 
     assert grad(dt=7) == -1 and grad(V=0) == -2 and grad(red=5) == -2 and grad(d=4) == -6
     for name in ("st", "w", "dl", "ws"):
         assert grad(**{name: None}) == -3, name
     for name in ("st", "w", "ws", "dh", "dw"):
         assert grad(**{name: 8}) == -4, name
-    assert grad(ws_bytes=L.ethos_linear_ce_grad_workspace_bytes(4, 64, 9, 1) - 1) == -5 and grad(st_bytes=8) == -5
+    assert grad(ws_bytes=L.ethos_linear_ce_grad_workspace_bytes(4, 64, 9, 1, 0) - 1) == -5 and grad(st_bytes=8) == -5
+    assert grad(ex=16, ex_bytes=8) == -5 and grad(ex=24, ex_bytes=big) == -4
     assert grad(n=0, w=None) == 0 and grad(dh=None, dw=None) == 0
 
 
