@@ -963,9 +963,10 @@ int ethos_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* la
     if (state_bytes < ethos::linear_ce_state_bytes(n_tok, d, dtype) ||
         workspace_bytes < ethos::linear_ce_workspace_bytes(n_tok, d, vocab, dtype, num_cus()))
         return fail(ETHOS_EWORKSPACE, "ethos_linear_ce: state of %zu or workspace of %zu bytes too small", state_bytes, workspace_bytes);
-    if (exps && exps_bytes < ethos::linear_ce_exps_bytes(n_tok, vocab, dtype))
+    if (exps && dtype != ETHOS_BF16) return fail(ETHOS_EUNSUPPORTED, "ethos_linear_ce: exps are for bf16");
+    if (exps && exps_bytes < ethos::linear_ce_exps_bytes(n_tok, vocab, dtype, num_cus()))
         return fail(ETHOS_EWORKSPACE, "ethos_linear_ce: exps of %zu bytes, %zu needed", exps_bytes,
-                    ethos::linear_ce_exps_bytes(n_tok, vocab, dtype));
+                    ethos::linear_ce_exps_bytes(n_tok, vocab, dtype, num_cus()));
     if (!aligned16(h) || !aligned16(w) || !aligned16(state) || !aligned16(exps) || !aligned16(workspace))
         return fail(ETHOS_EALIGN, "ethos_linear_ce: h, w, state, exps and workspace must be 16-byte aligned");
     return hip_status(ethos::launch_linear_ce(h, ldh, w, labels, n_tok, d, vocab, ignore_index, reduction, dtype, state, exps, workspace, loss,
@@ -974,8 +975,8 @@ int ethos_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* la
 }
 
 size_t ethos_linear_ce_exps_bytes(int64_t n_tok, int64_t vocab, int32_t dtype) {
-    if (n_tok <= 0 || n_tok > kMaxItems || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
-    return ethos::linear_ce_exps_bytes(n_tok, vocab, dtype);
+    if (n_tok <= 0 || n_tok > kMaxItems || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 0;
+    return ethos::linear_ce_exps_bytes(n_tok, vocab, dtype, num_cus());
 }
 
 size_t ethos_linear_ce_grad_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype, int32_t kept) {
@@ -994,9 +995,10 @@ int ethos_linear_ce_grad(const void* state, size_t state_bytes, void* exps, size
         workspace_bytes < ethos::linear_ce_grad_workspace_bytes(n_tok, d, vocab, dtype, num_cus(), exps != nullptr))
         return fail(ETHOS_EWORKSPACE, "ethos_linear_ce_grad: state of %zu or workspace of %zu bytes too small", state_bytes,
                     workspace_bytes);
-    if (exps && exps_bytes < ethos::linear_ce_exps_bytes(n_tok, vocab, dtype))
+    if (exps && dtype != ETHOS_BF16) return fail(ETHOS_EUNSUPPORTED, "ethos_linear_ce_grad: exps are for bf16");
+    if (exps && exps_bytes < ethos::linear_ce_exps_bytes(n_tok, vocab, dtype, num_cus()))
         return fail(ETHOS_EWORKSPACE, "ethos_linear_ce_grad: exps of %zu bytes, %zu needed", exps_bytes,
-                    ethos::linear_ce_exps_bytes(n_tok, vocab, dtype));
+                    ethos::linear_ce_exps_bytes(n_tok, vocab, dtype, num_cus()));
     if (!aligned16(state) || !aligned16(exps) || !aligned16(w) || !aligned16(workspace) || !aligned16(dh) || !aligned16(dw))
         return fail(ETHOS_EALIGN, "ethos_linear_ce_grad: state, exps, w, workspace, dh and dw must be 16-byte aligned");
     return hip_status(ethos::launch_linear_ce_grad(state, exps, w, dloss, n_tok, d, vocab, reduction, dtype, workspace, dh, dw, num_cus(),

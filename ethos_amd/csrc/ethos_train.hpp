@@ -13,7 +13,7 @@ enum Reduction : int { kLossMean = 0, kLossSum = 1, kLossNone = 2 };
 // Softmax cross entropy of rows h against a head matrix w [vocab, d].
 size_t linear_ce_state_bytes(int64_t n, int d, int dtype);
 size_t linear_ce_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus);
-size_t linear_ce_exps_bytes(int64_t n, int64_t vocab, int dtype);
+size_t linear_ce_exps_bytes(int64_t n, int64_t vocab, int dtype, int num_cus);
 size_t linear_ce_grad_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus, bool kept);
 int launch_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* labels, int64_t n, int d, int64_t vocab,
                      int64_t ignore, int reduction, int dtype, void* state, void* exps, void* ws, float* loss, int num_cus,

@@ -9,12 +9,11 @@
 // of vocabulary.  The backward forms the logits of a piece of the vocabulary again, turns them into dl
 // (bf16) in its epilogue, and multiplies the piece by h and by W.
 //
-// Where dl of the whole vocabulary is at most what a piece may take, the forward under gradients leaves the
-// exponentials behind, E_iv = exp(l_iv - l_i,label) in bf16, in the memory that dl would take in the backward anyway: relative
-// to the label's own logit, which is known before the products, so that one factor per row, f_i = g_i exp(l_i,label -
-// lse_i), turns them into dl.  It is applied to h for dW and to the sums for dh, and the label's own value is put in
-// as 1 - exp(lse_i - l_i,label); the logits are then formed once.  Where a label lies more than e^60 below its row's
-// sum (or is infinite, or missing) the backward forms all logits again.
+// bf16, where dl of the whole vocabulary is at most what a piece may take: the forward under gradients leaves the
+// exponentials behind, in the memory that dl would take in the backward anyway, and the backward turns them into dl in
+// place instead of forming the logits again (4,096 rows of 1,024 over 100,277 words: 292 us against 783).  They are
+// fp16 values relative to the maximum of their row's B / 2 words: off by 2^-11 of their size, or by 2^-25 of the
+// maximum's, against the 2^-8 of dl's own rounding to bf16.
 //
 // float32 operands go through the same kernels as three bf16 planes each, x = hi + mid + lo
 // (ethos_split.hpp): a product is six bf16 products, exact in the float32 sums, the smallest first.
@@ -31,7 +30,6 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kScaled = 1e38f;  // logits below this in size can be scaled by log2(e)
-constexpr float kFar = 60.0f;     // kept exponentials reach e^60 relative to their label's (bf16 holds e^88)
 constexpr int kPadRows = 256;  // labelled rows are padded with zero rows to a multiple of this
 
 __host__ __device__ constexpr int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -48,7 +46,6 @@ struct CeState {
     float* ll;       // logit of the label
     uint16_t* h;     // the labelled rows [planes][padded n][ldh]
     int32_t* ticket; // of the workgroups that finish the loss
-    int32_t* far;    // a label's logit is more than kFar below its row's log-sum
     int64_t np;      // n padded
     int ldh;
     size_t bytes;
@@ -63,7 +60,7 @@ CeState ce_state(char* p, int64_t n, int d, int dtype) {
         at += (bytes + 255) / 256 * 256;
         return r;
     };
-    s.count = (int32_t*)take(12);
+    s.count = (int32_t*)take(8);
     s.idx = (int32_t*)take(s.np * 4);
     s.inv = (int32_t*)take(s.np * 4);
     s.lab = (int32_t*)take(s.np * 4);
@@ -71,7 +68,6 @@ CeState ce_state(char* p, int64_t n, int d, int dtype) {
     s.ll = (float*)take(s.np * 4);
     s.h = (uint16_t*)take((size_t)s.np * s.ldh * 2 * planes_of(dtype));
     s.ticket = s.count + 1;
-    s.far = s.count + 2;
     s.bytes = at;
     return s;
 }
@@ -120,7 +116,7 @@ __global__ __launch_bounds__(1024) void ce_rows_kernel(const int64_t* __restrict
     }
     if (tid == 0) {
         *count = base;
-        ticket[0] = ticket[1] = 0;  // (and CeState::far)
+        *ticket = 0;
     }
 }
 
@@ -229,7 +225,7 @@ __global__ __launch_bounds__(256) void ce_few_rows_kernel(const int64_t* __restr
     }
     if (first && tid == 0) {
         *count = m;
-        ticket[0] = ticket[1] = 0;  // (and CeState::far)
+        *ticket = 0;
     }
     const int r = blockIdx.x * 4 + wave;
     if (r >= round_up(m, kPadRows)) return;
@@ -303,7 +299,6 @@ __global__ __launch_bounds__(1024) void ce_lse_kernel(const float2* __restrict__
         out = l - x;
         if (lane < 16 && r < m) {
             lse[r] = l;
-            if (!(fabsf(x) < kScaled && l - x <= kFar)) __hip_atomic_store(ticket + 1, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (reduction == kLossNone) loss[row] = out;
             else if (gridDim.x > 1) __hip_atomic_store(row_loss + r, out, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -646,8 +641,8 @@ __device__ __forceinline__ Place tile_place(int64_t block, int each) {
 }
 
 // Logits of a piece of the vocabulary, transposed (a lane holds values of two rows of h): GRAD 0: the
-// sum of exponentials over each wave's B / 2 words and what it is relative to; 1: dl [planes][ldp / 256][np][256]; 2: as
-// 0, and the exponentials in dl's place.
+// maximum and sum of exponentials over each wave's B / 2 words; 1: dl [planes][ldp / 256][np][256]; 2: as 0, and the
+// exponentials (fp16, relative to that maximum) in dl's place.
 struct LogitArgs {
     const uint16_t* w;   // the piece's first row, [planes][vocab][d]
     const float* w32;    // float32: the piece's first row itself
@@ -658,8 +653,19 @@ struct LogitArgs {
     float2* part;
     uint16_t* p;
     int d, ldh, reduction;
-    const int32_t* when;  // run only if it is not zero (null: run)
 };
+
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+    typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+    const f32x2_t f = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2_t));
+}
+__device__ __forceinline__ void unpack_f16x2(uint32_t v, float& a, float& b) {
+    typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+    const f16x2_t h = __builtin_bit_cast(f16x2_t, v);
+    a = (float)h[0];
+    b = (float)h[1];
+}
 
 // A logit as a float32 chain: what an infinity needs, which against the other operand's lower planes gives
 // NaN (times zero).
@@ -683,7 +689,6 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lds = lds_addr(smem), mine = lds + Ti::kLds + wave * 4096;
     const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
-    if (g.when && *g.when == 0) return;
     const int64_t words = g.v1 - g.v0, m = *g.count;
     // this workgroup's tiles: those of the vocabulary tiles of its XCD, one after the other, every gridDim / 8th
     const int n_tiles = (int)((m + B - 1) / B), xcd = blockIdx.x % 8;
@@ -715,13 +720,6 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                 const int64_t v = (int64_t)g.lab[rc] - g.v0 - tm0 - wm;
                 label_at[j] = v >= 0 && v < B / 2 && r < m && lane < 32 ? (int)v : -1;
                 label_value[j] = expm1f(g.ll[rc] - lse[j]) * k[j];  // exp(l - lse) - 1 without the cancellation
-            }
-        }
-        if constexpr (GRAD != 1) {
-#pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                const int64_t r = tn0 + wn + j * 32 + (lane & 31);
-                lse[j] = r < m ? g.ll[r] : 0.0f;  // what the row's exponentials are relative to
             }
         }
         f32x16_t acc[MI][NI];
@@ -766,41 +764,39 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                         for (int j = 0; j < NI; ++j) acc[i][j][e] = -__builtin_inff();
         }
         if constexpr (GRAD != 1) {
-            // the sum of exponentials relative to the label's logit, or, beyond its reach, to the maximum
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 const int64_t r = tn0 + wn + j * 32 + (el & 31);
-                const bool in = r < m;
                 float x = -__builtin_inff();
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x = fmaxf(x, acc[i][j][e]);
                 x = fmaxf(x, __shfl_xor(x, 32));
-                float s = 0.0f, top = lse[j];
-                if (ballot(in && !(fabsf(top) < kScaled && x - top <= kFar)) == 0) {
-                    const float z = top * kLog2e;
+                float s = 0.0f;
+                if (ballot(!(fabsf(x) < kScaled)) == 0) {
+                    const float z = x * kLog2e;
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -z));
                             s += v;
-                            if (GRAD == 2) acc[i][j][e] = in ? v : 0.0f;
+                            if (GRAD == 2) acc[i][j][e] = v;
                         }
                 } else {
-                    top = x;
                     const float z = x == -__builtin_inff() ? 0.0f : x;
 #pragma unroll
                     for (int i = 0; i < MI; ++i)
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            s += __builtin_amdgcn_exp2f((acc[i][j][e] - z) * kLog2e);
-                            if (GRAD == 2) acc[i][j][e] = 0.0f;  // (kept exponentials of such a row are not used)
+                            const float v = __builtin_amdgcn_exp2f((acc[i][j][e] - z) * kLog2e);
+                            s += v;
+                            if (GRAD == 2) acc[i][j][e] = v;
                         }
                 }
                 s += __shfl_xor(s, 32);
-                if (el < 32) g.part[((g.v0 + tm0) / (B / 2) + wave / Ti::kWN) * g.np + r] = make_float2(top, s);
+                if (el < 32) g.part[((g.v0 + tm0) / (B / 2) + wave / Ti::kWN) * g.np + r] = make_float2(x, s);
             }
         } else {
             // dl, in place
@@ -846,7 +842,7 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                                 uint32_t q[2];
 #pragma unroll
                                 for (int u = 0; u < 2; ++u) {
-                                    q[u] = pack_bf16x2(v[e + 2 * u], v[e + 2 * u + 1]);
+                                    q[u] = GRAD == 2 ? pack_f16x2(v[e + 2 * u], v[e + 2 * u + 1]) : pack_bf16x2(v[e + 2 * u], v[e + 2 * u + 1]);
                                     if (pl + 1 < PL) {
                                         v[e + 2 * u] -= __uint_as_float(q[u] << 16);
                                         v[e + 2 * u + 1] -= __uint_as_float(q[u] & 0xffff0000u);
@@ -1004,8 +1000,7 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_grads_kernel(GradArgs
 template <typename T>
 __global__ __launch_bounds__(256) void ce_row_grad_out_kernel(const float* __restrict__ part, const int32_t* __restrict__ count,
                                                               const int32_t* __restrict__ inv, int64_t n, int d, int tile, int cols,
-                                                              int64_t ldp, int num_cus, int with_dw, const float* __restrict__ factor,
-                                                              T* __restrict__ dh) {
+                                                              int64_t ldp, int num_cus, int with_dw, T* __restrict__ dh) {
     const int64_t m = *count, size = round_up(m, kPadRows) * d;
     const int parts = dh_parts(m, tile, cols, ldp, num_cus, with_dw);
     const int64_t total = n * (d / 4);
@@ -1028,69 +1023,53 @@ __global__ __launch_bounds__(256) void ce_row_grad_out_kernel(const float* __res
                     s.w += v[p].w;
                 }
             }
-        if (factor && at >= 0) {
-            const float f = factor[at];
-            s.x *= f;
-            s.y *= f;
-            s.z *= f;
-            s.w *= f;
-        }
         if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dh + r * d + c) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
         else *reinterpret_cast<float4*>(dh + r * d + c) = s;
     }
 }
 
-// What turns kept exponentials into dl, a wave per row of the dense block: the row's factor, its row of h times it, the
-// label's value.  (Where the logits are formed again, dl is whole: the factor is one.)
-struct FactorArgs {
-    const int32_t *count, *idx, *lab, *far;
+// Kept exponentials into dl, in place: times the row's gradient and exp(their maximum - lse), and the label's value.  A
+// workgroup takes 64 rows of a panel (32 KB), 8 words a thread at a time; zeros for the padding's rows.
+struct KeptArgs {
+    const int32_t *count, *idx, *lab;
     const float *lse, *ll, *dloss;
-    const uint16_t* h;
-    uint16_t *scaled, *e;
-    float* factor;
-    int64_t np, ldp;
-    int ldh, reduction;
+    const float2* part;  // [ldp / words of a maximum][np]
+    uint16_t* p;
+    int64_t np;
+    int each, reduction;  // words of a maximum
 };
-template <int PL>
-__global__ __launch_bounds__(256) void ce_factor_kernel(FactorArgs g) {
-    const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t m = *g.count;
-    if (r >= round_up(m, kPadRows)) return;
-    const bool far = *g.far != 0;
-    float f = 1.0f;
-    if (r < m && !far) {
-        const float below = g.lse[r] - g.ll[r];
-        f = row_gradient(g.dloss, g.idx, r, m, g.reduction) * expf(-below);
-        if (lane == 0) {
-            const int64_t v = g.lab[r];
-            float x = -expm1f(below);
+__global__ __launch_bounds__(256) void ce_kept_kernel(KeptArgs g) {
+    const int64_t m = *g.count, r0 = (int64_t)blockIdx.y * 64;
+    if (r0 >= round_up(m, kPadRows)) return;
+    const int64_t panel = blockIdx.x;
+    const int word = (threadIdx.x & 31) * 8;
+    uint16_t* p = g.p + (panel * g.np + r0 + (threadIdx.x >> 5)) * kPanel + word;
+    const float2* part = g.part + (panel * kPanel + word) / g.each * g.np;
 #pragma unroll
-            for (int i = 0; i < PL; ++i) {
-                const uint16_t q = f32_to_bf16_bits(x);
-                x -= bf16_bits_to_f32(q);
-                g.e[i * g.np * g.ldp + (v / kPanel * g.np + r) * kPanel + v % kPanel] = q;
+    for (int t = 0; t < 8; t += 4) {
+        u32x4_t v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + (t + u) * 8 * kPanel));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t r = r0 + (threadIdx.x >> 5) + (t + u) * 8, rc = r < m ? r : m > 0 ? m - 1 : 0;
+            const float lse = g.lse[rc], x = part[rc].x, k = m > 0 ? row_gradient(g.dloss, g.idx, rc, m, g.reduction) : 0.0f;
+            const float f = x == -__builtin_inff() ? k * 0.0f : k * expf(x - lse);  // (no word of the row's: zeros, or NaN)
+            const int64_t label = (int64_t)g.lab[rc] - panel * kPanel - word;
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) unpack_f16x2(v[u][j], y[2 * j], y[2 * j + 1]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] *= f;
+            if (label >= 0 && label < 8) {
+                const float one = expm1f(g.ll[rc] - lse) * k;  // exp(l - lse) - 1 without the cancellation
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = j == label ? one : y[j];
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[u][j] = r < m ? pack_bf16x2(y[2 * j], y[2 * j + 1]) : 0u;
+            __builtin_nontemporal_store(v[u], reinterpret_cast<u32x4_t*>(p + (t + u) * 8 * kPanel));
         }
-    }
-    if (lane == 0) g.factor[r] = f;
-    const int64_t plane = g.np * g.ldh;
-    for (int c = lane * 8; c < g.ldh; c += 64 * 8) {
-        const int64_t at = r * g.ldh + c;
-        float x[8], y[8];
-        Vec16<uint16_t>::unpack(*reinterpret_cast<const uint4*>(g.h + at), x);
-        if constexpr (PL > 1) {
-#pragma unroll
-            for (int i = PL - 1; i > 0; --i) {
-                Vec16<uint16_t>::unpack(*reinterpret_cast<const uint4*>(g.h + at + i * plane), y);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] += y[j];
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= f;
-        if constexpr (PL > 1) put_planes(x, g.scaled + at, plane);
-        else *reinterpret_cast<uint4*>(g.scaled + at) = Vec16<uint16_t>::pack(x);
     }
 }
 
@@ -1143,8 +1122,6 @@ FwdWs fwd_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
 
 struct GradWs {
     uint16_t* p;  // dl of a piece (not kept exponentials, which have their own memory)
-    uint16_t* h;  // kept exponentials: h times the rows' factors
-    float* factor;
     float* part;  // dh's parts
     uint16_t* w;  // float32: W's planes
     int64_t piece, part_tiles;
@@ -1164,8 +1141,6 @@ GradWs grad_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus,
     const int64_t row256 = m256 * (num_cus / m256 < 1 ? 1 : num_cus / m256 < w.piece / kPartWords ? num_cus / m256 : w.piece / kPartWords);
     w.grad_tile = d > 128 && (words + 255) / 256 * cols256 + row256 >= num_cus ? 256 : 128;
     w.p = kept ? nullptr : (uint16_t*)take((size_t)np * w.piece * 2 * planes);
-    w.h = kept ? (uint16_t*)take((size_t)np * round_up(d, 64) * 2 * planes) : nullptr;
-    w.factor = kept ? (float*)take((size_t)np * 4) : nullptr;
     // parts x tiles of rows for any count of labelled rows: as many as fill the chip, or one part
     const int64_t cols = (d + w.grad_tile - 1) / w.grad_tile, slots = num_cus / cols;
     w.part_tiles = slots > np / w.grad_tile ? slots : np / w.grad_tile;
@@ -1218,8 +1193,8 @@ void run_logits(const LogitArgs& g, int tile, int dtype, int64_t n, int num_cus,
     const int64_t tiles = xcd_grid((g.v1 - g.v0 + tile - 1) / tile, (int)((n + tile - 1) / tile));
     const int64_t most = round_up(num_cus, 8) * (tile == 256 ? 1 : 2);
     const dim3 grid((unsigned)(tiles < most ? tiles : most));
-    with_tile(tile, dtype, [&](auto b, auto pl) {
-        constexpr int B = decltype(b)::v, PL = decltype(pl)::v;
+    with_tile(tile, GRAD == 2 ? (int)kBF16 : dtype, [&](auto b, auto pl) {
+        constexpr int B = decltype(b)::v, PL = GRAD == 2 ? 1 : decltype(pl)::v;
         hipLaunchKernelGGL((ce_logits_kernel<B, PL, GRAD>), grid, dim3(Tile<B>::kThreads), 0, stream, g);
     });
 }
@@ -1235,8 +1210,10 @@ size_t linear_ce_state_bytes(int64_t n, int d, int dtype) { return ce_state(null
 size_t linear_ce_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
     return fwd_ws(nullptr, n, d, vocab, dtype, num_cus).bytes;
 }
-size_t linear_ce_exps_bytes(int64_t n, int64_t vocab, int dtype) {
-    return (size_t)round_up(n, kPadRows) * round_up(vocab, kTileMax) * 2 * planes_of(dtype);
+// The kept exponentials, and behind them the maxima that they are relative to (with the sums).
+size_t exps_values(int64_t n, int64_t vocab) { return (size_t)round_up(n, kPadRows) * round_up(vocab, kTileMax) * 2; }
+size_t linear_ce_exps_bytes(int64_t n, int64_t vocab, int dtype, int num_cus) {
+    return dtype == kBF16 ? exps_values(n, vocab) + (size_t)round_up(n, kPadRows) * (round_up(vocab, kTileMax) / (tile_for(vocab, n, num_cus) / 2)) * 8 : 0;
 }
 size_t linear_ce_grad_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus, bool kept) {
     return grad_ws(nullptr, n, d, vocab, dtype, num_cus, kept).bytes;
@@ -1272,11 +1249,12 @@ int launch_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* l
     if (exps) {
         g.p = (uint16_t*)exps;
         g.ldp = round_up(vocab, kTileMax);
+        g.part = (float2*)((char*)exps + exps_values(n, vocab));
         run_logits<2>(g, f.tile, dtype, n, num_cus, stream);
     } else {
         run_logits<0>(g, f.tile, dtype, n, num_cus, stream);
     }
-    hipLaunchKernelGGL(ce_lse_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, stream, f.part, f.n_part, s.np, s.count, s.idx, s.ll,
+    hipLaunchKernelGGL(ce_lse_kernel, dim3((unsigned)((n + 15) / 16)), dim3(1024), 0, stream, g.part, f.n_part, s.np, s.count, s.idx, s.ll,
                        reduction, s.lse, f.row_loss, s.ticket, loss);
     return (int)hipGetLastError();
 }
@@ -1294,17 +1272,16 @@ int launch_linear_ce_grad(const void* state, void* exps, const void* w, const fl
         g.ldp = b.piece;
         g.dloss = dloss;
         g.reduction = reduction;
-        g.when = exps ? s.far : nullptr;
-        run_logits<1>(g, b.logit_tile, dtype, n, num_cus, stream);
         if (exps) {
-            const FactorArgs a{s.count, s.idx, s.lab, s.far, s.lse, s.ll, dloss, s.h, b.h, g.p, b.factor, s.np, b.piece, s.ldh, reduction};
-            const dim3 grid((unsigned)(s.np / 4));
-            if (dtype == kBF16) hipLaunchKernelGGL((ce_factor_kernel<1>), grid, dim3(256), 0, stream, a);
-            else hipLaunchKernelGGL((ce_factor_kernel<3>), grid, dim3(256), 0, stream, a);
+            const KeptArgs a{s.count, s.idx, s.lab, s.lse, s.ll, dloss, (const float2*)((char*)exps + exps_values(n, vocab)), g.p, s.np,
+                             tile_for(vocab, n, num_cus) / 2, reduction};
+            hipLaunchKernelGGL(ce_kept_kernel, dim3((unsigned)(b.piece / kPanel), (unsigned)(s.np / 64)), dim3(256), 0, stream, a);
+        } else {
+            run_logits<1>(g, b.logit_tile, dtype, n, num_cus, stream);
         }
         const int64_t row_blocks = dh ? xcd_grid(b.part_tiles, cols) : 0;
         const int64_t head_blocks = dw ? xcd_grid((words + b.grad_tile - 1) / b.grad_tile, cols) : 0;
-        const GradArgs a{g.p, exps ? b.h : s.h, g.w, s.count, words, s.np, b.piece, g.w_plane, b.part, (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4), d,
+        const GradArgs a{g.p, s.h, g.w, s.count, words, s.np, b.piece, g.w_plane, b.part, (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4), d,
                          s.ldh, cols, num_cus, v0 > 0 ? 1 : 0, dw ? 1 : 0, row_blocks};
         with_tile(b.grad_tile, dtype, [&](auto t, auto pl) {
             constexpr int B = decltype(t)::v, PL = decltype(pl)::v;
@@ -1316,10 +1293,10 @@ int launch_linear_ce_grad(const void* state, void* exps, const void* w, const fl
         blocks = blocks < num_cus * 16 ? blocks : num_cus * 16;
         if (dtype == kBF16)
             hipLaunchKernelGGL((ce_row_grad_out_kernel<uint16_t>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, n,
-                               d, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, b.factor, (uint16_t*)dh);
+                               d, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, (uint16_t*)dh);
         else
             hipLaunchKernelGGL((ce_row_grad_out_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, n, d,
-                               b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, b.factor, (float*)dh);
+                               b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, (float*)dh);
     }
     return (int)hipGetLastError();
 }

@@ -684,7 +684,8 @@ INTS = (torch.int32, torch.int64)
 
 def linear_ce(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, ignore_index: int, reduction: str, keep: int = 0):
     """(loss float32, state, exps): softmax cross entropy of h [n, d] (rows evenly spaced) against w [V, d];
-    the state and exps (None where they would take more than `keep` bytes) are what linear_ce_grad takes."""
+    the state and exps (None where they would take more than `keep` bytes) are what linear_ce_grad takes,
+    which overwrites exps."""
     _need_here(w, "weight", FLOATS, 2)
     _need_here(labels, "labels", (torch.int64,), 1)
     n, d = h.shape
@@ -693,7 +694,7 @@ def linear_ce(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, ignore_ind
     st, st_bytes = _scratch("ethos_linear_ce_state_bytes", device, n, d, code)
     ws, ws_bytes = _scratch("ethos_linear_ce_workspace_bytes", device, n, d, V, code)
     exps, exps_bytes = None, _size("ethos_linear_ce_exps_bytes", device.index, n, V, code) if keep else 0
-    if keep and exps_bytes <= keep:
+    if 0 < exps_bytes <= keep:
         exps, exps_bytes = workspace(exps_bytes, device)
     loss = torch.empty((n,) if reduction == "none" else (), dtype=torch.float32, device=device)
     rc = lib.ethos_linear_ce(h.data_ptr(), h.stride(0) if n > 1 else d, w.data_ptr(), labels.data_ptr(), n, d, V, int(ignore_index),

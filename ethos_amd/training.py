@@ -64,13 +64,16 @@ class _LinearCrossEntropy(torch.autograd.Function):
         loss, state, exps = hip.linear_ce(rows, w, labels, ignore_index, reduction, keep_bytes)
         ctx.save_for_backward(weight, state, exps)
         ctx.copy = w if w.data_ptr() != weight.data_ptr() else None
-        ctx.shape, ctx.reduction = h.shape, reduction
+        ctx.shape, ctx.reduction, ctx.first = h.shape, reduction, True
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
         weight, state, exps = ctx.saved_tensors
+        if not ctx.first:  # a second backward of a retained graph: the first has used the exponentials up
+            exps = None
+        ctx.first = False
         w = weight.detach() if ctx.copy is None else ctx.copy
         n = math.prod(ctx.shape[:-1])
         want_h, want_w = ctx.needs_input_grad[:2]
@@ -86,10 +89,9 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     labels int64 [...].  Positions whose label is `ignore_index` have no part in the loss or its
     gradients; another label outside the vocabulary makes the loss NaN.  `reduction`: "mean" over the
     labelled positions (NaN without one), "sum", or "none" (float32 [...], zero where ignored).  The
-    loss is float32.  Gradients go to h and weight, in their dtype.  For them the forward leaves the
-    exponentials behind in 16 bits (float32: 48) where these take at most `keep_bytes`, in the memory that
-    the backward would take anyway; else, and with 0, the backward forms the logits again, a piece of the
-    vocabulary at a time."""
+    loss is float32.  Gradients go to h and weight, in their dtype.  For them the backward forms the logits
+    again, a piece of the vocabulary at a time; in bf16 the forward leaves the exponentials behind instead (in
+    16 bits, in the memory that the backward would take anyway) where these take at most `keep_bytes`."""
     for name, t in (("h", h), ("weight", weight), ("labels", labels)):
         _device_check(name, t)
     if reduction not in ("mean", "sum", "none"):

@@ -512,15 +512,14 @@ int ethos_layer_forward(const void* x, const void* wq, const void* wq_prepared, 
  *   state   >= ethos_linear_ce_state_bytes(...) bytes: what ethos_linear_ce_grad reads (the rows with
  *           a label in dense form, their log-sums)
  *   loss    float32, one value or (NONE) [n_tok]
- *   exps    NULL, or >= ethos_linear_ce_exps_bytes(...) bytes: the forward leaves the exponentials in bf16
- *           (float32: three bf16 planes) there for ethos_linear_ce_grad, which then does not form the logits
- *           again (unless a label lies more than e^60 below its row's sum).  Both calls, or neither, get it.
+ *   exps    NULL, or (bf16) >= ethos_linear_ce_exps_bytes(...) bytes, which is 0 for float32: the forward leaves the
+ *           exponentials there, in 16 bits, for one ethos_linear_ce_grad, which then does not form the logits
+ *           again (and overwrites exps)
  * Logits, exponentials' sums and losses are float32, a reduction's sum float64.
  * ethos_linear_ce_grad: dh [n_tok, d] and dw [vocab, d] of dtype T (either may be NULL) from dloss
  * (float32: one value or, NONE, [n_tok]), with the state that the forward left and the same w.  Without exps it
  * forms a piece of the vocabulary's logits at a time again (their gradients take at most 1 GiB, or 256 words); for
- * bf16 the logits' gradients are rounded to bf16 for the products with h and w (with exps the exponentials are, and
- * h times a factor per row).
+ * bf16 the logits' gradients are rounded to bf16 for the products with h and w.
  * Limits: d a multiple of 8, at most 32768; ldh a multiple of 8 (bf16) or 4; vocab <= 2^30; n_tok
  * <= 2^30; h, w, state, exps, workspace, dh and dw 16-byte aligned.  n_tok = 0 does nothing.
  */

@@ -29,6 +29,7 @@ def test_linear_ce_argument_errors_are_codes():
     assert ce(st_bytes=L.ethos_linear_ce_state_bytes(4, 64, 1) - 1) == -5
     assert ce(ws_bytes=L.ethos_linear_ce_workspace_bytes(4, 64, 9, 1) - 1) == -5
     assert ce(ex=16, ex_bytes=L.ethos_linear_ce_exps_bytes(4, 9, 1) - 1) == -5 and ce(ex=24, ex_bytes=big) == -4
+    assert ce(ex=16, ex_bytes=big, dt=0) == -6 and L.ethos_linear_ce_exps_bytes(4, 9, 0) == 0
     assert ce(n=0, h=None) == 0 and L.ethos_last_error() == b""
 
     def grad(st=16, st_bytes=big, ex=None, ex_bytes=0, w=16, dl=16, n=4, d=64, V=9, red=0, dt=1, ws=16, ws_bytes=big, dh=16, dw=16):
@@ -40,7 +41,7 @@ def test_linear_ce_argument_errors_are_codes():
     for name in ("st", "w", "ws", "dh", "dw"):
         assert grad(**{name: 8}) == -4, name
     assert grad(ws_bytes=L.ethos_linear_ce_grad_workspace_bytes(4, 64, 9, 1, 0) - 1) == -5 and grad(st_bytes=8) == -5
-    assert grad(ex=16, ex_bytes=8) == -5 and grad(ex=24, ex_bytes=big) == -4
+    assert grad(ex=16, ex_bytes=8) == -5 and grad(ex=24, ex_bytes=big) == -4 and grad(ex=16, ex_bytes=big, dt=0) == -6
     assert grad(n=0, w=None) == 0 and grad(dh=None, dw=None) == 0
 
 
