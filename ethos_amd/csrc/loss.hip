@@ -340,7 +340,7 @@ __device__ __forceinline__ float row_gradient(const float* dloss, const int32_t*
 // 128: four waves of 64 x 64), k in steps of kK.  Operands go from memory
 // straight into LDS, the next step's while the current one is multiplied.  An operand is stored with k
 // contiguous ("K": rows of m or n) or with k as the row ("R"); R tiles are read with the transposing LDS
-// loads.  LDS rows of a K tile are kK k (kK / 8 pieces of 16 bytes, their places by k_piece); of an R
+// loads.  LDS rows of a K tile are 64 k (8 pieces of 16 bytes, their places by k_piece); of an R
 // tile B columns (B / 8 pieces), piece c at c ^ 4 (k % 4): 16 lanes' reads touch all banks.
 constexpr int kTileMax = 256;
 // dl is stored in panels of 256 words, [panel][np][256], so that a tile of it is one stretch of memory (with the rows of
@@ -358,7 +358,7 @@ template <int B> struct Tile {
     static constexpr int kWaves = B == 256 ? 8 : 4, kThreads = kWaves * 64;
     static constexpr int kWN = kWaves / 2;                           // waves along n (two along m)
     static constexpr int kMI = B / 64, kNI = B / kWN / 32;           // MFMA tiles of a wave
-    static constexpr int kK = 64;                                    // step of the reduction
+    static constexpr int kK = 64;                                    // step of the reduction (8 pieces of 16 bytes)
     static constexpr int kBytes = B * kK * 2;                        // one operand's step
     static constexpr int kCopies = kBytes / 1024 / kWaves;           // copies of a wave per operand and step
     static constexpr int kLds = 2 * 2 * kBytes;                      // two steps
@@ -384,10 +384,7 @@ struct Feed {
 };
 
 // The piece of a K tile's row at place c, and the other way round.
-template <int K>
-__device__ __forceinline__ int k_piece(int row, int c) {
-    return K == 64 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3);
-}
+__device__ __forceinline__ int k_piece(int row, int c) { return c ^ ((row >> 1) & 7); }
 
 template <int B, bool KC>
 __device__ __forceinline__ void feed_init(Feed& f, const uint16_t* p, int64_t bytes, int64_t ld, int k, int cols, int64_t plane,
@@ -404,7 +401,7 @@ __device__ __forceinline__ void feed_init(Feed& f, const uint16_t* p, int64_t by
     for (int j = 0; j < Ti::kCopies; ++j) {
         const int slot = (j * Ti::kWaves + wave) * 64 + lane;
         if (KC) {
-            const int row = slot / (Ti::kK / 8), c = k_piece<Ti::kK>(row, slot % (Ti::kK / 8));
+            const int row = slot / (Ti::kK / 8), c = k_piece(row, slot % (Ti::kK / 8));
             f.off[j] = (uint32_t)(row * ld * 2 + c * 16);
         } else {
             const int kk = slot / (B / 8), c = (slot % (B / 8)) ^ ((kk & 3) << 2);
@@ -428,7 +425,7 @@ __device__ __forceinline__ void feed_copy(const Feed& f, int j, uint32_t lds, in
     uint32_t off = f.off[j];
     if (KC && f.k_left < Ti::kK) {
         const int slot = (j * Ti::kWaves + wave) * 64 + lane;
-        off = k_piece<Ti::kK>(slot / (Ti::kK / 8), slot % (Ti::kK / 8)) * 8 < f.k_left ? off : kOutside;
+        off = k_piece(slot / (Ti::kK / 8), slot % (Ti::kK / 8)) * 8 < f.k_left ? off : kOutside;
     }
     lds_dma16(buffer_rsrc((const void*)f.base, (uint32_t)left), (int)off, 0,
               __builtin_amdgcn_readfirstlane(lds + (j * Ti::kWaves + wave) * 1024));
@@ -453,7 +450,7 @@ template <int B, bool KC, int N> struct Reader {
         if constexpr (KC) {
             const int row = row0 + (lane & 31);
 #pragma unroll
-            for (int s = 0; s < K / 16; ++s) at[s] = row * (K * 2) + (k_piece<K>(row, 2 * s + (lane >> 5)) << 4);
+            for (int s = 0; s < K / 16; ++s) at[s] = row * (K * 2) + (k_piece(row, 2 * s + (lane >> 5)) << 4);
         } else {
             const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
 #pragma unroll
@@ -849,7 +846,7 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                                     }
                                 }
                                 typedef __attribute__((address_space(3))) u32x2_t* ptr;
-                                *(ptr)(size_t)(mine + n * 128 + (k_piece<64>(n, i * 4 + (e >> 2)) << 4) + 8 * (el >> 5)) = u32x2_t{q[0], q[1]};
+                                *(ptr)(size_t)(mine + n * 128 + (k_piece(n, i * 4 + (e >> 2)) << 4) + 8 * (el >> 5)) = u32x2_t{q[0], q[1]};
                             }
                         asm volatile("" ::: "memory");
                         if (GRAD == 1 && label_at[j] >= 0 && label_at[j] / 64 == c) {
@@ -857,7 +854,7 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                             const int w = label_at[j] % 64;
                             const uint16_t x = f32_to_bf16_bits(label_value[j]);
                             label_value[j] -= bf16_bits_to_f32(x);
-                            *(ptr)(size_t)(mine + n * 128 + (k_piece<64>(n, w >> 3) << 4) + (w & 7) * 2) = x;
+                            *(ptr)(size_t)(mine + n * 128 + (k_piece(n, w >> 3) << 4) + (w & 7) * 2) = x;
                         }
                         asm volatile("" ::: "memory");
                         uint16_t* out = g.p + pl * g.np * g.ldp + (tm0 / kPanel * g.np + tn0 + wn + j * 32) * kPanel + tm0 % kPanel + wm + c * 64;
@@ -865,7 +862,7 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
                         for (int t = 0; t < 4; ++t) {
                             typedef const __attribute__((address_space(3))) u32x4_t* ptr;
                             const int r = t * 8 + (el >> 3);
-                            __builtin_nontemporal_store(*(ptr)(size_t)(mine + r * 128 + (k_piece<64>(r, el & 7) << 4)),
+                            __builtin_nontemporal_store(*(ptr)(size_t)(mine + r * 128 + (k_piece(r, el & 7) << 4)),
                                                         reinterpret_cast<u32x4_t*>(out + r * kPanel + (el & 7) * 8));
                         }
                         asm volatile("" ::: "memory");

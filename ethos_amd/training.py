@@ -29,6 +29,10 @@ _TENSORS = {torch.Tensor, torch.nn.Parameter}
 _dtype, _shape = operator.attrgetter("dtype"), operator.attrgetter("shape")
 
 
+def _contiguous(t):
+    return t.contiguous() if isinstance(t, torch.Tensor) and not t.is_contiguous() else t
+
+
 def _dense(t: torch.Tensor) -> torch.Tensor:
     """t contiguous at a 16-byte address (a copy where it is not)."""
     t = t.detach().contiguous()
@@ -64,16 +68,20 @@ class _LinearCrossEntropy(torch.autograd.Function):
         loss, state, exps = hip.linear_ce(rows, w, labels, ignore_index, reduction, keep_bytes)
         ctx.save_for_backward(weight, state, exps)
         ctx.copy = w if w.data_ptr() != weight.data_ptr() else None
-        ctx.shape, ctx.reduction, ctx.first = h.shape, reduction, True
+        ctx.shape, ctx.reduction = h.shape, reduction
+        ctx.fresh, ctx.captured = True, torch.cuda.is_current_stream_capturing()
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
         weight, state, exps = ctx.saved_tensors
-        if not ctx.first:  # a second backward of a retained graph: the first has used the exponentials up
+        # the first backward uses the exponentials up: a second one of a retained graph has none, nor has one that
+        # is captured alone, to be replayed
+        if not ctx.fresh or (exps is not None and not ctx.captured and torch.cuda.is_current_stream_capturing()):
             exps = None
-        ctx.first = False
+        else:
+            ctx.fresh = False
         w = weight.detach() if ctx.copy is None else ctx.copy
         n = math.prod(ctx.shape[:-1])
         want_h, want_w = ctx.needs_input_grad[:2]
@@ -120,7 +128,7 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, ids, scale, padding):
-        out, keys = hip.embedding(ids, weight.detach().contiguous(), scale, padding, True)
+        out, keys = hip.embedding(ids, weight, scale, padding, True)
         ctx.keys, ctx.vocab, ctx.scale = keys, weight.shape[0], scale  # keys: this node's own tensor
         return out
 
@@ -133,32 +141,26 @@ class _Embedding(torch.autograd.Function):
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
     """scale * weight[ids], [*ids.shape, d], for a table weight [vocab, d] (bf16 or float32) and ids of
     any shape (int32 or int64).  The table's gradient is dense, leaves out positions of `padding_idx`
-    (negative ones count from the end) and adds a token's positions in their order, in float32.  An
+    (negative ones count from the end) and adds a token's positions in a fixed order, in float32.  An
     id outside the table gives a row of NaN."""
-    _device_check("ids", ids)
-    _device_check("weight", weight)
-    if weight.dtype not in hip.FLOATS:
-        raise TypeError(f"weight must be bfloat16 or float32, got {weight.dtype}")
-    if ids.dtype not in hip.INTS:
-        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
-    if weight.dim() != 2 or weight.numel() == 0:
-        raise RuntimeError(f"embedding: weight must be [vocab, d], got {tuple(weight.shape)}")
+    ids, w = _contiguous(ids), _contiguous(weight)  # (types and devices: hip.embedding)
+    if isinstance(w, torch.Tensor) and (w.dim() != 2 or w.numel() == 0):
+        raise RuntimeError(f"embedding: weight must be [vocab, d], got {tuple(w.shape)}")
     padding = -1
     if padding_idx is not None:
         if not -weight.shape[0] <= padding_idx < weight.shape[0]:
             raise ValueError(f"padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
         padding = padding_idx % weight.shape[0]
-    ids = ids.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return _Embedding.apply(weight, ids, float(scale), padding)
-    return hip.embedding(ids, weight.detach().contiguous(), float(scale))[0]
+    if torch.is_grad_enabled() and isinstance(w, torch.Tensor) and w.requires_grad:
+        return _Embedding.apply(w, ids, float(scale), padding)  # (a copied weight's gradient goes through the copy)
+    return hip.embedding(ids, w, float(scale))[0]
 
 
 # -------------------------------------------------------------------------- balance
 class _Balance(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gates, ids, n_experts):
-        loss, counts = hip.balance(gates.detach().contiguous(), ids, n_experts)
+        loss, counts = hip.balance(gates, ids, n_experts)
         ctx.save_for_backward(ids, counts)
         ctx.dtype = gates.dtype
         ctx.mark_non_differentiable(counts)
@@ -184,18 +186,14 @@ def balance_loss(gates: torch.Tensor, ids: torch.Tensor, n_experts: int):
     [n_experts].  Ids outside [0, n_experts) count nowhere.  Without tokens both are zero."""
     _device_check("gates", gates)
     _device_check("ids", ids)
-    if gates.dtype not in hip.FLOATS:
-        raise TypeError(f"gates must be bfloat16 or float32, got {gates.dtype}")
-    if ids.dtype not in hip.INTS:
-        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
+    gates, ids = _contiguous(gates), _contiguous(ids)  # (dtypes: hip.balance)
     if gates.dim() < 2 or gates.shape != ids.shape or 0 in gates.shape[-2:]:
         raise RuntimeError(f"balance_loss: gates and ids must both be [..., heads, k], got {tuple(gates.shape)} and {tuple(ids.shape)}")
     if n_experts <= 0:
         raise ValueError(f"n_experts must be positive, got {n_experts}")
-    ids = ids.contiguous()
     if torch.is_grad_enabled() and gates.requires_grad:
         return _Balance.apply(gates, ids, int(n_experts))
-    return hip.balance(gates.detach().contiguous(), ids, int(n_experts))
+    return hip.balance(gates, ids, int(n_experts))
 
 
 # -------------------------------------------------------------------------- clipping

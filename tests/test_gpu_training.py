@@ -303,7 +303,8 @@ def test_embedding_ids_outside_the_table_and_views():
 # ------------------------------------------------------------------------------- balance
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
 @pytest.mark.parametrize("itype", [torch.int32, torch.int64])
-@pytest.mark.parametrize("n,H,k,E", [(1, 1, 1, 1), (1, 2, 4, 256), (37, 3, 5, 1000), (500, 4, 8, 4096), (1000, 8, 16, 262144)])
+@pytest.mark.parametrize("n,H,k,E", [(1, 1, 1, 1), (1, 2, 4, 256), (37, 3, 5, 1000), (500, 4, 8, 4096), (1000, 8, 16, 262144),
+                                     (300, 4, 8, 600000)])
 def test_balance_against_float64(n, H, k, E, dt, itype):
     g = _gen(n + E)
     gates = torch.softmax(torch.randn(n, H, k, generator=g, device="cuda"), -1).to(DT[dt]).requires_grad_()
@@ -480,6 +481,28 @@ def test_on_another_stream_and_in_a_graph(dt):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, want)), seed
+
+
+def test_a_backward_captured_alone_can_be_replayed():
+    h, w, labels = _ce_inputs(130, 64, 700, torch.bfloat16, seed=3)
+    a, b, gy = h.requires_grad_(), w.requires_grad_(), torch.ones((), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = ethos_amd.linear_cross_entropy(a, b, labels)
+        want = torch.autograd.grad(ethos_amd.linear_cross_entropy(a, b, labels, keep_bytes=0), (a, b), gy)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = torch.autograd.grad(loss, (a, b), gy, retain_graph=True)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        # the eager graph's own backward still has what the forward left
+        eager = torch.autograd.grad(loss, (a, b), gy)
+        again = torch.autograd.grad(ethos_amd.linear_cross_entropy(a, b, labels), (a, b), gy)
+        assert torch.equal(eager[0], again[0]) and torch.equal(eager[1], again[1])
 
 
 @pytest.mark.parametrize("train", [False, True])
