@@ -377,6 +377,24 @@ def test_clip_against_float64(norm, share, in_place):
         assert all(torch.equal(t, k) for t, k in zip(grads, keep))
 
 
+@pytest.mark.parametrize("norm", [2.0, math.inf])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_clip_of_many_pieces(norm, dt):
+    # one tensor of 2^27 + 10001 values and 1,200 of a few
+    g = _gen(19)
+    big = torch.randn(2 ** 27 + 10001, generator=g, device="cuda", dtype=DT[dt])
+    big[-1] = 100.0
+    grads = [big] + [t.clone() for t in torch.randn(1200, 3, generator=g, device="cuda").to(DT[dt])]
+    size = float(_norm(grads, norm))
+    keep = [t.clone() for t in grads]
+    total = ethos_amd.clip_grads(grads, 0.5 * size, norm_type=norm)
+    assert abs(float(total) - size) <= 2 * U * size
+    factor = 0.5 * size / (size + 1e-6)
+    for i, (o, k) in enumerate(zip(grads, keep)):
+        x = k.double() * factor
+        _within(o, x, (half_step(o.dtype) + 3 * U) * 1.01 * x.abs(), f"tensor {i}")
+
+
 def test_clip_extreme_values():
     big = torch.full((100000,), 3e38, device="cuda")
     total = ethos_amd.clip_grads([big], 1.0)
