@@ -337,8 +337,8 @@ __device__ __forceinline__ float row_gradient(const float* dloss, const int32_t*
 
 // ------------------------------------------------------------------------ products
 // C[m][n] = sum_k A(m, k) B(k, n) in tiles of B x B (256: eight waves, two along m and four along n, 128 x 64 each;
-// 128: four waves of 64 x 64), k in steps of kK.  Operands go from memory
-// straight into LDS, the next step's while the current one is multiplied.  An operand is stored with k
+// 128: four waves of 64 x 64, or eight of 64 x 32), k in steps of kK.  Operands go from memory
+// straight into LDS, which holds S steps: the one that is multiplied and those on their way.  An operand is stored with k
 // contiguous ("K": rows of m or n) or with k as the row ("R"); R tiles are read with the transposing LDS
 // loads.  LDS rows of a K tile are 64 k (8 pieces of 16 bytes, their places by k_piece); of an R
 // tile B columns (B / 8 pieces), piece c at c ^ 4 (k % 4): 16 lanes' reads touch all banks.
@@ -354,14 +354,15 @@ constexpr uint32_t kOutside = 0x80000000u;  // an offset past every buffer's end
 constexpr int kPairs = 6;
 constexpr uint32_t kPairsA = 0x001012, kPairsB = 0x010210;
 
-template <int B> struct Tile {
-    static constexpr int kWaves = B == 256 ? 8 : 4, kThreads = kWaves * 64;
+template <int TB, int TS> struct Tile {
+    static constexpr int B = TB, S = TS;
+    static constexpr int kWaves = B == 256 || S == 4 ? 8 : 4, kThreads = kWaves * 64;
     static constexpr int kWN = kWaves / 2;                           // waves along n (two along m)
     static constexpr int kMI = B / 64, kNI = B / kWN / 32;           // MFMA tiles of a wave
     static constexpr int kK = 64;                                    // step of the reduction (8 pieces of 16 bytes)
     static constexpr int kBytes = B * kK * 2;                        // one operand's step
     static constexpr int kCopies = kBytes / 1024 / kWaves;           // copies of a wave per operand and step
-    static constexpr int kLds = 2 * 2 * kBytes;                      // two steps
+    static constexpr int kLds = S * 2 * kBytes;
     static constexpr int kRowsLds = kWaves * 4096;                   // the logits' epilogue: 4 KB a wave
 };
 
@@ -386,12 +387,11 @@ struct Feed {
 // The piece of a K tile's row at place c, and the other way round.
 __device__ __forceinline__ int k_piece(int row, int c) { return c ^ ((row >> 1) & 7); }
 
-template <int B, bool KC>
+template <typename Ti, bool KC>
 __device__ __forceinline__ void feed_init(Feed& f, const uint16_t* p, int64_t bytes, int64_t ld, int k, int cols, int64_t plane,
                                           int wave, int lane) {
     f.base = f.base0 = (uint64_t)p;
     f.left = f.left0 = bytes;
-    typedef Tile<B> Ti;
     f.step = KC ? Ti::kK * 2 : Ti::kK * ld * 2;
     f.k_left = f.k0 = k;
     f.plane = plane * 2;
@@ -404,7 +404,7 @@ __device__ __forceinline__ void feed_init(Feed& f, const uint16_t* p, int64_t by
             const int row = slot / (Ti::kK / 8), c = k_piece(row, slot % (Ti::kK / 8));
             f.off[j] = (uint32_t)(row * ld * 2 + c * 16);
         } else {
-            const int kk = slot / (B / 8), c = (slot % (B / 8)) ^ ((kk & 3) << 2);
+            const int kk = slot / (Ti::B / 8), c = (slot % (Ti::B / 8)) ^ ((kk & 3) << 2);
             f.off[j] = c * 8 < cols ? (uint32_t)(kk * ld * 2 + c * 16) : kOutside;
         }
     }
@@ -418,9 +418,8 @@ __device__ __forceinline__ void feed_plane(Feed& f, int p) {
 }
 
 // The next step's tile into LDS at `lds`: one of the wave's copies, or all of them and on to the step after.
-template <int B, bool KC>
+template <typename Ti, bool KC>
 __device__ __forceinline__ void feed_copy(const Feed& f, int j, uint32_t lds, int wave, int lane) {
-    typedef Tile<B> Ti;
     const int64_t left = f.left < 0 ? 0 : f.left > 0x7fffffff ? 0x7fffffff : f.left;
     uint32_t off = f.off[j];
     if (KC && f.k_left < Ti::kK) {
@@ -430,12 +429,12 @@ __device__ __forceinline__ void feed_copy(const Feed& f, int j, uint32_t lds, in
     lds_dma16(buffer_rsrc((const void*)f.base, (uint32_t)left), (int)off, 0,
               __builtin_amdgcn_readfirstlane(lds + (j * Ti::kWaves + wave) * 1024));
 }
-template <int B>
+template <typename Ti>
 __device__ __forceinline__ void feed_advance(Feed& f) {
     f.base += f.step;
     f.left -= f.step;
-    f.k_left -= Tile<B>::kK;
-    if (++f.at == kPanel / Tile<B>::kK) {
+    f.k_left -= Ti::kK;
+    if (++f.at == kPanel / Ti::kK) {
         f.at = 0;
         f.base += f.jump;
         f.left -= f.jump;
@@ -443,8 +442,8 @@ __device__ __forceinline__ void feed_advance(Feed& f) {
 }
 
 // Fragments of 32 rows (or columns) i at row0 + 32 i, reduction step s of 16.
-template <int B, bool KC, int N> struct Reader {
-    static constexpr int K = Tile<B>::kK;
+template <typename Ti, bool KC, int N> struct Reader {
+    static constexpr int K = Ti::kK, B = Ti::B;
     uint32_t at[KC ? K / 16 : N];
     __device__ __forceinline__ void init(int row0, int lane) {
         if constexpr (KC) {
@@ -475,8 +474,9 @@ template <int B, bool KC, int N> struct Reader {
     }
 };
 
-// This wave's copies have landed and its LDS reads are done, and so with every wave.
-__device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// This wave's copies but the last N have landed and its LDS reads are done, and so with every wave.
+template <int N = 0>
+__device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
 // The same of LDS accesses alone.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -488,17 +488,17 @@ struct Pair {
     int pair;
 };
 
-template <int B, bool AK, bool BK>
+template <typename Ti, bool AK, bool BK>
 __device__ __forceinline__ void tile_copy(const Pair& p, uint32_t to, int c, int wave, int lane) {
-    constexpr int C = Tile<B>::kCopies;
-    if (c < C) feed_copy<B, AK>(p.a, c, to, wave, lane);
-    else feed_copy<B, BK>(p.b, c - C, to + Tile<B>::kBytes, wave, lane);
+    constexpr int C = Ti::kCopies;
+    if (c < C) feed_copy<Ti, AK>(p.a, c, to, wave, lane);
+    else feed_copy<Ti, BK>(p.b, c - C, to + Ti::kBytes, wave, lane);
 }
 
-template <int B, int PL>
+template <typename Ti, int PL>
 __device__ __forceinline__ void tile_advance(Pair& p) {
-    feed_advance<B>(p.a);
-    feed_advance<B>(p.b);
+    feed_advance<Ti>(p.a);
+    feed_advance<Ti>(p.b);
     if (PL > 1 && ++p.in == p.steps) {
         p.in = 0;
         ++p.pair;
@@ -507,8 +507,8 @@ __device__ __forceinline__ void tile_advance(Pair& p) {
     }
 }
 
-// The copies of a tile's first two steps (or the one it has).
-template <int B, int PL, bool AK, bool BK>
+// The copies of a tile's first S steps (or those it has).
+template <typename Ti, int PL, bool AK, bool BK>
 __device__ __forceinline__ void tile_begin(Pair& p, int64_t steps, uint32_t lds, int wave, int lane) {
     p.steps = steps;
     p.in = 0;
@@ -517,11 +517,12 @@ __device__ __forceinline__ void tile_begin(Pair& p, int64_t steps, uint32_t lds,
         feed_plane(p.a, kPairsA & 3);
         feed_plane(p.b, kPairsB & 3);
     }
-    const int n = steps <= 0 ? 0 : PL > 1 || steps > 1 ? 2 : 1;
+    const int64_t total = PL > 1 ? steps * kPairs : steps;
+    const int n = total < Ti::S ? (int)total : Ti::S;
     for (int t = 0; t < n; ++t) {
 #pragma unroll
-        for (int c = 0; c < 2 * Tile<B>::kCopies; ++c) tile_copy<B, AK, BK>(p, lds + t * 2 * Tile<B>::kBytes, c, wave, lane);
-        tile_advance<B, PL>(p);
+        for (int c = 0; c < 2 * Ti::kCopies; ++c) tile_copy<Ti, AK, BK>(p, lds + t * 2 * Ti::kBytes, c, wave, lane);
+        tile_advance<Ti, PL>(p);
     }
 }
 
@@ -530,12 +531,11 @@ __device__ __forceinline__ void tile_begin(Pair& p, int64_t steps, uint32_t lds,
 // barrier stands before its last products, which cover the first reads of the next step and the copies into the step
 // just freed.  (Reads and copies in a row before the products: 54% of the matrix pipes' cycles used at 2.0 GHz; so:
 // 72% at 1.78 GHz, which the power allows; with no copies at all 81% at 1.82 GHz.)
-template <int B, int PL, bool AK, bool BK>
-__device__ __forceinline__ void tile_run(Pair& p, uint32_t lds, f32x16_t (&acc)[Tile<B>::kMI][Tile<B>::kNI], int wave, int lane) {
-    typedef Tile<B> Ti;
-    constexpr int MI = Ti::kMI, NI = Ti::kNI, C = Ti::kCopies, Q = MI * NI, kLast = Ti::kK / 16 - 1;
-    Reader<B, AK, MI> ra;
-    Reader<B, BK, NI> rb;
+template <typename Ti, int PL, bool AK, bool BK>
+__device__ __forceinline__ void tile_run(Pair& p, uint32_t lds, f32x16_t (&acc)[Ti::kMI][Ti::kNI], int wave, int lane) {
+    constexpr int B = Ti::B, S = Ti::S, MI = Ti::kMI, NI = Ti::kNI, C = Ti::kCopies, Q = MI * NI, kLast = Ti::kK / 16 - 1;
+    Reader<Ti, AK, MI> ra;
+    Reader<Ti, BK, NI> rb;
     ra.init(wave / Ti::kWN * (B / 2), lane);
     rb.init(wave % Ti::kWN * (32 * NI), lane);
 #pragma unroll
@@ -566,9 +566,9 @@ __device__ __forceinline__ void tile_run(Pair& p, uint32_t lds, f32x16_t (&acc)[
     for (int r = 0; r < MI + NI; ++r) read(lds, 0, r);
     uint32_t cur = 0, from = lds, next = lds + 2 * Ti::kBytes;
     auto flip = [&]() {
-        cur ^= 1;
+        cur = (cur + 1) % S;
         from = lds + cur * 2 * Ti::kBytes;
-        next = lds + (cur ^ 1) * 2 * Ti::kBytes;
+        next = lds + (cur + 1) % S * 2 * Ti::kBytes;
     };
     auto head = [&]() {  // all but the step's last products
 #pragma unroll
@@ -578,25 +578,27 @@ __device__ __forceinline__ void tile_run(Pair& p, uint32_t lds, f32x16_t (&acc)[
                 for (int r = 0; r < R; ++r) read(from, s + 1, q * R + r);
             });
     };
-    for (int64_t t = 2; t < total; ++t) {
+    for (int64_t t = S; t < total; ++t) {
         head();
-        if (t == 2) lds_barrier();  // (the second step is there; stores before it may still be on their way)
-        else step_barrier();
+        if (t < 2 * S - 1) lds_barrier();  // (the first S steps are there; stores before them may still be on their way)
+        else step_barrier<2 * C * (S - 2)>();
         multiply(kLast, [&](int q) {
             constexpr int P = (2 * C + Q - 1) / Q;  // copies after a product
 #pragma unroll
             for (int r = 0; r < R; ++r) read(next, 0, q * R + r);
 #pragma unroll
             for (int c = 0; c < P; ++c)
-                if (q * P + c < 2 * C) tile_copy<B, AK, BK>(p, from, q * P + c, wave, lane);
+                if (q * P + c < 2 * C) tile_copy<Ti, AK, BK>(p, from, q * P + c, wave, lane);
         });
-        tile_advance<B, PL>(p);
+        tile_advance<Ti, PL>(p);
         flip();
     }
     // the steps that are in LDS or on their way (the last one's reads of a next step go unused)
-    for (int t = total < 2 ? (int)total : 2; t > 0; --t) {
+    for (int t = total < Ti::S ? (int)total : S; t > 0; --t) {
         head();
-        step_barrier();
+        if (S == 4 && t == 4) step_barrier<4 * C>();
+        else if (S == 4 && t == 3) step_barrier<2 * C>();
+        else step_barrier();
         multiply(kLast, [&](int q) {
 #pragma unroll
             for (int r = 0; r < R; ++r) read(next, 0, q * R + r);
@@ -617,11 +619,12 @@ __device__ __forceinline__ void put4(uint32_t lds, int n, int m, uint32_t lo, ui
     typedef __attribute__((address_space(3))) u32x2_t* ptr;
     *(ptr)(size_t)(lds + row_slot<B>(n, m)) = u32x2_t{lo, hi};
 }
-template <int B>
+template <typename Ti>
 __device__ __forceinline__ void tile_to_rows(uint32_t lds, uint16_t* out, int64_t ld, int rows, int cols, int tid) {
+    constexpr int B = Ti::B;
     typedef const __attribute__((address_space(3))) u32x4_t* ptr;
 #pragma unroll 4
-    for (int q = tid; q < B * (B / 8); q += Tile<B>::kThreads) {
+    for (int q = tid; q < B * (B / 8); q += Ti::kThreads) {
         const int n = q / (B / 8), c = q % (B / 8);
         if (n < rows && c * 8 < cols) *reinterpret_cast<u32x4_t*>(out + (int64_t)n * ld + c * 8) = *(ptr)(size_t)(lds + row_slot<B>(n, c * 8));
     }
@@ -677,10 +680,9 @@ __device__ __forceinline__ float logit_chain(const LogitArgs& g, int64_t v, int6
     return s;
 }
 
-template <int B, int PL, int GRAD>
-__global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitArgs g) {
-    typedef Tile<B> Ti;
-    constexpr int MI = Ti::kMI, NI = Ti::kNI;
+template <typename Ti, int PL, int GRAD>
+__global__ __launch_bounds__(Ti::kThreads, 2) void ce_logits_kernel(LogitArgs g) {
+    constexpr int B = Ti::B, MI = Ti::kMI, NI = Ti::kNI;
     __shared__ __align__(16) char smem[Ti::kLds + (GRAD ? Ti::kRowsLds : 0)];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -697,9 +699,9 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
     auto begin = [&]() {
         m0 = (tile / n_tiles * 8 + xcd) * B;
         n0 = tile % n_tiles * B;
-        feed_init<B, true>(p.a, g.w + m0 * g.d, (words - m0) * g.d * 2, g.d, g.d, 0, g.w_plane, wave, lane);
-        feed_init<B, true>(p.b, g.h + n0 * g.ldh, (g.np - n0) * g.ldh * 2, g.ldh, g.d, 0, g.np * g.ldh, wave, lane);
-        tile_begin<B, PL, true, true>(p, (g.d + Ti::kK - 1) / Ti::kK, lds, wave, lane);
+        feed_init<Ti, true>(p.a, g.w + m0 * g.d, (words - m0) * g.d * 2, g.d, g.d, 0, g.w_plane, wave, lane);
+        feed_init<Ti, true>(p.b, g.h + n0 * g.ldh, (g.np - n0) * g.ldh * 2, g.ldh, g.d, 0, g.np * g.ldh, wave, lane);
+        tile_begin<Ti, PL, true, true>(p, (g.d + Ti::kK - 1) / Ti::kK, lds, wave, lane);
     };
     begin();
     step_barrier();
@@ -720,7 +722,7 @@ __global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_logits_kernel(LogitAr
             }
         }
         f32x16_t acc[MI][NI];
-        tile_run<B, PL, true, true>(p, lds, acc, wave, lane);
+        tile_run<Ti, PL, true, true>(p, lds, acc, wave, lane);
         // the next tile's first steps are on their way during the epilogue
         tile += gridDim.x / 8;
         const bool more = tile < tiles;
@@ -880,7 +882,7 @@ constexpr int kPartWords = 256;
 __host__ __device__ inline int dh_parts(int64_t m, int tile, int cols, int64_t ldp, int num_cus, int with_dw) {
     const int64_t rows = (m + tile - 1) / tile * cols, steps = ldp / 64;
     const int64_t all = rows * steps + (with_dw ? (ldp + tile - 1) / tile * cols * ((m + 63) / 64) : 0);
-    const int64_t share = all / num_cus > 1 ? all / num_cus : 1, slots = rows > 0 ? num_cus / rows : 1, most = ldp / kPartWords;
+    const int64_t share = all > num_cus ? (all + num_cus - 1) / num_cus : 1, slots = rows > 0 ? num_cus / rows : 1, most = ldp / kPartWords;
     int64_t s = (steps + share - 1) / share;
     s = s < slots ? s : slots;
     s = s < most ? s : most;
@@ -900,10 +902,9 @@ struct GradArgs {
     int64_t row_blocks;
 };
 
-template <int B, int PL>
+template <typename Ti, int PL>
 __device__ __forceinline__ void ce_row_grad(const GradArgs& g, int64_t block, uint32_t lds, int tid) {
-    typedef Tile<B> Ti;
-    constexpr int MI = Ti::kMI, NI = Ti::kNI;
+    constexpr int B = Ti::B, MI = Ti::kMI, NI = Ti::kNI;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t m = *g.count;
     const int parts = dh_parts(m, B, g.cols, g.ldp, g.num_cus, g.with_dw);
@@ -920,14 +921,14 @@ __device__ __forceinline__ void ce_row_grad(const GradArgs& g, int64_t block, ui
         Pair p;
         constexpr int64_t kSteps = kPanel / Ti::kK;
         const int64_t first = (s0 / kSteps * g.np + m0) * kPanel + s0 % kSteps * Ti::kK;
-        feed_init<B, true>(p.a, g.p + first, (g.np * g.ldp - first) * 2, kPanel, INT32_MAX, 0, g.np * g.ldp, wave, lane);
+        feed_init<Ti, true>(p.a, g.p + first, (g.np * g.ldp - first) * 2, kPanel, INT32_MAX, 0, g.np * g.ldp, wave, lane);
         p.a.jump = (g.np - 1) * kPanel * 2;
         p.a.at = p.a.at0 = (int)(s0 % kSteps);
-        feed_init<B, false>(p.b, g.w + s0 * Ti::kK * g.d + n0, ((g.words - s0 * Ti::kK) * g.d - n0) * 2, g.d, 0, g.d - n0, g.w_plane, wave,
+        feed_init<Ti, false>(p.b, g.w + s0 * Ti::kK * g.d + n0, ((g.words - s0 * Ti::kK) * g.d - n0) * 2, g.d, 0, g.d - n0, g.w_plane, wave,
                             lane);
-        tile_begin<B, PL, true, false>(p, s1 - s0, lds, wave, lane);
+        tile_begin<Ti, PL, true, false>(p, s1 - s0, lds, wave, lane);
         step_barrier();
-        tile_run<B, PL, true, false>(p, lds, acc, wave, lane);
+        tile_run<Ti, PL, true, false>(p, lds, acc, wave, lane);
     }
     const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
     float* out = g.part + (int64_t)part * rows * g.d;
@@ -945,10 +946,9 @@ __device__ __forceinline__ void ce_row_grad(const GradArgs& g, int64_t block, ui
     }
 }
 
-template <int B, int PL>
+template <typename Ti, int PL>
 __device__ __forceinline__ void ce_head_grad(const GradArgs& g, int64_t block, uint32_t lds, int tid) {
-    typedef Tile<B> Ti;
-    constexpr int MI = Ti::kMI, NI = Ti::kNI;
+    constexpr int B = Ti::B, MI = Ti::kMI, NI = Ti::kNI;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Place at = tile_place(block, g.cols);
     const int64_t n0 = at.group * B;
@@ -958,12 +958,12 @@ __device__ __forceinline__ void ce_head_grad(const GradArgs& g, int64_t block, u
     {
         const int64_t rows = round_up(*g.count, kPadRows), steps = (*g.count + Ti::kK - 1) / Ti::kK;
         Pair p;
-        feed_init<B, false>(p.a, g.h + m0, (rows * g.ldh - m0) * 2, g.ldh, 0, g.d - m0, g.np * g.ldh, wave, lane);
-        feed_init<B, false>(p.b, g.p + n0 / kPanel * g.np * kPanel + n0 % kPanel, (rows * kPanel - n0 % kPanel) * 2, kPanel, 0, B,
+        feed_init<Ti, false>(p.a, g.h + m0, (rows * g.ldh - m0) * 2, g.ldh, 0, g.d - m0, g.np * g.ldh, wave, lane);
+        feed_init<Ti, false>(p.b, g.p + n0 / kPanel * g.np * kPanel + n0 % kPanel, (rows * kPanel - n0 % kPanel) * 2, kPanel, 0, B,
                             g.np * g.ldp, wave, lane);
-        tile_begin<B, PL, false, false>(p, steps, lds, wave, lane);
+        tile_begin<Ti, PL, false, false>(p, steps, lds, wave, lane);
         step_barrier();
-        tile_run<B, PL, false, false>(p, lds, acc, wave, lane);
+        tile_run<Ti, PL, false, false>(p, lds, acc, wave, lane);
     }
     const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
     const int rows = g.words - n0 < B ? (int)(g.words - n0) : B;
@@ -982,15 +982,15 @@ __device__ __forceinline__ void ce_head_grad(const GradArgs& g, int64_t block, u
             }
     if constexpr (PL == 1) {
         lds_barrier();
-        tile_to_rows<B>(lds, (uint16_t*)g.dw + n0 * g.d + m0, g.d, rows, g.d - m0, tid);
+        tile_to_rows<Ti>(lds, (uint16_t*)g.dw + n0 * g.d + m0, g.d, rows, g.d - m0, tid);
     }
 }
 
-template <int B, int PL>
-__global__ __launch_bounds__(Tile<B>::kThreads, 2) void ce_grads_kernel(GradArgs g) {
-    __shared__ __align__(16) char smem[Tile<B>::kLds];
-    if (blockIdx.x < g.row_blocks) ce_row_grad<B, PL>(g, blockIdx.x, lds_addr(smem), threadIdx.x);
-    else ce_head_grad<B, PL>(g, blockIdx.x - g.row_blocks, lds_addr(smem), threadIdx.x);
+template <typename Ti, int PL>
+__global__ __launch_bounds__(Ti::kThreads, 2) void ce_grads_kernel(GradArgs g) {
+    __shared__ __align__(16) char smem[Ti::kLds];
+    if (blockIdx.x < g.row_blocks) ce_row_grad<Ti, PL>(g, blockIdx.x, lds_addr(smem), threadIdx.x);
+    else ce_head_grad<Ti, PL>(g, blockIdx.x - g.row_blocks, lds_addr(smem), threadIdx.x);
 }
 
 // dh in h's rows and type: the sum of the parts, zeros for rows without a label; 4 columns a thread.
@@ -1150,19 +1150,21 @@ GradWs grad_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus,
 
 unsigned xcd_grid(int64_t groups, int each) { return (unsigned)((groups + 7) / 8 * 8 * each); }
 
-// f(tile, planes) with both as constants.
+// f(tile, planes) as constants.  Tiles of 128 that have a CU each (`alone`) get four steps in LDS and eight waves,
+// otherwise two of four waves, with two steps each, share a CU.  100 rows of 4,096 against 16,000 words (125 tiles): 48 us with four
+// steps, 62 with two; gradients of 1,500 float32 rows of 256 against 8,009 words (over 500 tiles): 304 and 260 us.
 template <int V> struct Int {
     static constexpr int v = V;
 };
 template <typename F>
-void with_tile(int tile, int dtype, F f) {
-    if (dtype == kBF16) {
-        if (tile == 256) f(Int<256>{}, Int<1>{});
-        else f(Int<128>{}, Int<1>{});
-    } else {
-        if (tile == 256) f(Int<256>{}, Int<3>{});
-        else f(Int<128>{}, Int<3>{});
-    }
+void with_tile(int tile, bool alone, int dtype, F f) {
+    auto planes = [&](auto t) {
+        if (dtype == kBF16) f(t, Int<1>{});
+        else f(t, Int<3>{});
+    };
+    if (tile == 256) planes(Tile<256, 2>{});
+    else if (alone) planes(Tile<128, 4>{});
+    else planes(Tile<128, 2>{});
 }
 
 LogitArgs logit_args(const CeState& s, const void* w, const uint16_t* planes, int64_t v0, int64_t v1, int64_t vocab, int d, int dtype) {
@@ -1187,12 +1189,14 @@ LogitArgs logit_args(const CeState& s, const void* w, const uint16_t* planes, in
 template <int GRAD>
 void run_logits(const LogitArgs& g, int tile, int dtype, int64_t n, int num_cus, hipStream_t stream) {
     // as many workgroups as run at once (one to a CU, or two of tiles of 128)
-    const int64_t tiles = xcd_grid((g.v1 - g.v0 + tile - 1) / tile, (int)((n + tile - 1) / tile));
+    const int64_t m_tiles = (g.v1 - g.v0 + tile - 1) / tile, n_tiles = (n + tile - 1) / tile;
+    const int64_t tiles = xcd_grid(m_tiles, (int)n_tiles);
     const int64_t most = round_up(num_cus, 8) * (tile == 256 ? 1 : 2);
     const dim3 grid((unsigned)(tiles < most ? tiles : most));
-    with_tile(tile, GRAD == 2 ? (int)kBF16 : dtype, [&](auto b, auto pl) {
-        constexpr int B = decltype(b)::v, PL = GRAD == 2 ? 1 : decltype(pl)::v;
-        hipLaunchKernelGGL((ce_logits_kernel<B, PL, GRAD>), grid, dim3(Tile<B>::kThreads), 0, stream, g);
+    with_tile(tile, m_tiles * n_tiles <= num_cus, GRAD == 2 ? (int)kBF16 : dtype, [&](auto t, auto pl) {
+        typedef decltype(t) Ti;
+        constexpr int PL = GRAD == 2 ? 1 : decltype(pl)::v;
+        hipLaunchKernelGGL((ce_logits_kernel<Ti, PL, GRAD>), grid, dim3(Ti::kThreads), 0, stream, g);
     });
 }
 
@@ -1280,9 +1284,11 @@ int launch_linear_ce_grad(const void* state, void* exps, const void* w, const fl
         const int64_t head_blocks = dw ? xcd_grid((words + b.grad_tile - 1) / b.grad_tile, cols) : 0;
         const GradArgs a{g.p, s.h, g.w, s.count, words, s.np, b.piece, g.w_plane, b.part, (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4), d,
                          s.ldh, cols, num_cus, v0 > 0 ? 1 : 0, dw ? 1 : 0, row_blocks};
-        with_tile(b.grad_tile, dtype, [&](auto t, auto pl) {
-            constexpr int B = decltype(t)::v, PL = decltype(pl)::v;
-            hipLaunchKernelGGL((ce_grads_kernel<B, PL>), dim3((unsigned)(row_blocks + head_blocks)), dim3(Tile<B>::kThreads), 0, stream, a);
+        const int64_t head = dw ? (words + b.grad_tile - 1) / b.grad_tile * cols : 0;
+        const int64_t row = dh ? (n + b.grad_tile - 1) / b.grad_tile * cols * dh_parts(n, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0) : 0;
+        with_tile(b.grad_tile, head + row <= num_cus, dtype, [&](auto t, auto pl) {
+            typedef decltype(t) Ti;
+            hipLaunchKernelGGL((ce_grads_kernel<Ti, decltype(pl)::v>), dim3((unsigned)(row_blocks + head_blocks)), dim3(Ti::kThreads), 0, stream, a);
         });
     }
     if (dh) {

@@ -140,6 +140,20 @@ def test_cross_entropy_in_the_largest_tiles(dt, n, ignored, keep):
         _within(got, x, e, what)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,d,V", [(40, 136, 300), (130, 320, 260), (200, 384, 700), (330, 448, 129)])
+def test_cross_entropy_of_a_few_steps(n, d, V, dt):
+    # 3, 5, 6 and 7 steps of d; 1 to 6 of rows; 1 to 11 of words
+    h, w, labels = _ce_inputs(n, d, V, DT[dt], seed=d)
+    gy = torch.ones((), device="cuda")
+    want, bound = _ce_oracle(h, w, labels, "sum", gy)
+    a, b = h.requires_grad_(), w.requires_grad_()
+    for keep in (0, 1 << 30):
+        loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="sum", keep_bytes=keep)
+        for got, x, e, what in zip((loss.detach(), *torch.autograd.grad(loss, (a, b), gy)), want, bound, ("loss", "dh", "dw")):
+            _within(got, x, e, what)
+
+
 def test_cross_entropy_gradient_against_differences():
     h, w, labels = _ce_inputs(9, 16, 37, torch.float32, seed=2, ignored=0.3)
     labels[0] = 5
