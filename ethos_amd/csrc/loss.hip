@@ -337,7 +337,10 @@ __device__ __forceinline__ float row_gradient(const float* dloss, const int32_t*
 
 // ------------------------------------------------------------------------ products
 // C[m][n] = sum_k A(m, k) B(k, n) in tiles of B x B (256: eight waves, two along m and four along n, 128 x 64 each;
-// 128: four waves of 64 x 64, or eight of 64 x 32), k in steps of kK.  Operands go from memory
+// 128: four waves of 64 x 64, or eight of 64 x 32), k in steps of kK.  float32 operands are
+// PL = 3 bf16 planes each: a step of tiles of 128 has all of them (P = 3) and takes every pair's products from it; tiles of
+// 256, for which LDS has no room, go over the operands once for each pair (500 x 256 x 8,009: gradients 29 us against 38 with
+// passes, logits 17.5 and 20).  Operands go from memory
 // straight into LDS, which holds S steps: the one that is multiplied and those on their way.  An operand is stored with k
 // contiguous ("K": rows of m or n) or with k as the row ("R"); R tiles are read with the transposing LDS
 // loads.  LDS rows of a K tile are 64 k (8 pieces of 16 bytes, their places by k_piece); of an R
@@ -348,19 +351,20 @@ constexpr int kTileMax = 256;
 constexpr int kPanel = 256;
 constexpr uint32_t kOutside = 0x80000000u;  // an offset past every buffer's end: reads zeros
 
-// float32: the pairs of planes, (2, 0), (1, 1), (0, 2), (1, 0), (0, 1), (0, 0).  The three left out, mid x lo, lo x mid
-// and lo x lo, are at most 2^-22 of a product and 2^-26 on the root mean square, below the rounding of a float32 sum
-// of 16 such products; a third of the products' time.
+// float32: the pairs of planes, (0, 0) into one sum and (0, 1), (1, 0), (1, 1), (0, 2), (2, 0), whose products are 2^-8 of
+// that and less, into another.  The three left out, mid x lo, lo x mid and lo x lo, are at most 2^-22 of a product and
+// 2^-26 on the root mean square, below the rounding of a float32 sum of 16 such products; a third of the products' time.
 constexpr int kPairs = 6;
-constexpr uint32_t kPairsA = 0x001012, kPairsB = 0x010210;
+constexpr uint32_t kPairsA = 0x201100, kPairsB = 0x021010;
 
-template <int TB, int TS> struct Tile {
-    static constexpr int B = TB, S = TS;
-    static constexpr int kWaves = B == 256 || S == 4 ? 8 : 4, kThreads = kWaves * 64;
+template <int TB, int TS, int TP> struct Tile {
+    static constexpr int B = TB, S = TS, P = TP;
+    static constexpr int kWaves = B == 256 || S == 4 || P > 1 ? 8 : 4, kThreads = kWaves * 64;
     static constexpr int kWN = kWaves / 2;                           // waves along n (two along m)
     static constexpr int kMI = B / 64, kNI = B / kWN / 32;           // MFMA tiles of a wave
-    static constexpr int kK = 64;                                    // step of the reduction (8 pieces of 16 bytes)
-    static constexpr int kBytes = B * kK * 2;                        // one operand's step
+    static constexpr int kK = P == 1 ? 64 : 32;                      // step of the reduction
+    static constexpr int kPlane = B * kK * 2;                        // a plane of one operand's step
+    static constexpr int kBytes = P * kPlane;                        // one operand's step
     static constexpr int kCopies = kBytes / 1024 / kWaves;           // copies of a wave per operand and step
     static constexpr int kLds = S * 2 * kBytes;
     static constexpr int kRowsLds = kWaves * 4096;                   // the logits' epilogue: 4 KB a wave
@@ -376,16 +380,20 @@ struct Feed {
     int64_t left;   // bytes from there to the operand's end
     int64_t step;   // bytes from a step to the next
     int k_left;     // K: k from the next step's first to the end
-    uint32_t off[4];  // this lane's offsets (kCopies of them)
-    uint64_t base0;  // the first plane's first step
-    int64_t left0, plane;
-    int k0;
+    uint32_t off[4];  // this lane's offsets in a plane (kCopies / P of them)
+    int64_t plane;  // bytes from a plane to the next
     int64_t jump;   // dl by rows: bytes to the next panel, taken after the panel's last step
-    int at, at0;    // steps taken in the panel
+    int at;         // steps taken in the panel
+    uint64_t base0;  // passes over the planes: the first plane's first step
+    int64_t left0;
+    int k0, at0;
 };
 
-// The piece of a K tile's row at place c, and the other way round.
-__device__ __forceinline__ int k_piece(int row, int c) { return c ^ ((row >> 1) & 7); }
+// The piece of a K tile's row (of K k) at place c, and the other way round.
+template <int K = 64>
+__device__ __forceinline__ int k_piece(int row, int c) {
+    return K == 64 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3);
+}
 
 template <typename Ti, bool KC>
 __device__ __forceinline__ void feed_init(Feed& f, const uint16_t* p, int64_t bytes, int64_t ld, int k, int cols, int64_t plane,
@@ -398,10 +406,10 @@ __device__ __forceinline__ void feed_init(Feed& f, const uint16_t* p, int64_t by
     f.jump = 0;
     f.at = f.at0 = 0;
 #pragma unroll
-    for (int j = 0; j < Ti::kCopies; ++j) {
+    for (int j = 0; j < Ti::kCopies / Ti::P; ++j) {
         const int slot = (j * Ti::kWaves + wave) * 64 + lane;
         if (KC) {
-            const int row = slot / (Ti::kK / 8), c = k_piece(row, slot % (Ti::kK / 8));
+            const int row = slot / (Ti::kK / 8), c = k_piece<Ti::kK>(row, slot % (Ti::kK / 8));
             f.off[j] = (uint32_t)(row * ld * 2 + c * 16);
         } else {
             const int kk = slot / (Ti::B / 8), c = (slot % (Ti::B / 8)) ^ ((kk & 3) << 2);
@@ -410,6 +418,7 @@ __device__ __forceinline__ void feed_init(Feed& f, const uint16_t* p, int64_t by
     }
 }
 
+// Back to the first step, of plane p.
 __device__ __forceinline__ void feed_plane(Feed& f, int p) {
     f.base = f.base0 + (uint64_t)(p * f.plane);
     f.left = f.left0;
@@ -420,13 +429,14 @@ __device__ __forceinline__ void feed_plane(Feed& f, int p) {
 // The next step's tile into LDS at `lds`: one of the wave's copies, or all of them and on to the step after.
 template <typename Ti, bool KC>
 __device__ __forceinline__ void feed_copy(const Feed& f, int j, uint32_t lds, int wave, int lane) {
+    constexpr int kEach = Ti::kCopies / Ti::P;  // copies of a plane
     const int64_t left = f.left < 0 ? 0 : f.left > 0x7fffffff ? 0x7fffffff : f.left;
-    uint32_t off = f.off[j];
+    uint32_t off = f.off[j % kEach];
     if (KC && f.k_left < Ti::kK) {
-        const int slot = (j * Ti::kWaves + wave) * 64 + lane;
-        off = k_piece(slot / (Ti::kK / 8), slot % (Ti::kK / 8)) * 8 < f.k_left ? off : kOutside;
+        const int slot = (j % kEach * Ti::kWaves + wave) * 64 + lane;
+        off = k_piece<Ti::kK>(slot / (Ti::kK / 8), slot % (Ti::kK / 8)) * 8 < f.k_left ? off : kOutside;
     }
-    lds_dma16(buffer_rsrc((const void*)f.base, (uint32_t)left), (int)off, 0,
+    lds_dma16(buffer_rsrc((const void*)(f.base + j / kEach * f.plane), (uint32_t)left), (int)off, 0,
               __builtin_amdgcn_readfirstlane(lds + (j * Ti::kWaves + wave) * 1024));
 }
 template <typename Ti>
@@ -449,7 +459,7 @@ template <typename Ti, bool KC, int N> struct Reader {
         if constexpr (KC) {
             const int row = row0 + (lane & 31);
 #pragma unroll
-            for (int s = 0; s < K / 16; ++s) at[s] = row * (K * 2) + (k_piece(row, 2 * s + (lane >> 5)) << 4);
+            for (int s = 0; s < K / 16; ++s) at[s] = row * (K * 2) + (k_piece<K>(row, 2 * s + (lane >> 5)) << 4);
         } else {
             const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
 #pragma unroll
@@ -481,11 +491,11 @@ __device__ __forceinline__ void step_barrier() { asm volatile("s_waitcnt vmcnt(%
 // The same of LDS accesses alone.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// A tile's operands and how far its copies are.
+// A tile's operands, and with passes over their planes the present one.
 struct Pair {
     Feed a, b;
-    int64_t steps, in;  // steps of a pair of planes; taken of the present one
-    int pair;
+    int64_t steps, in;  // steps of a pass; taken of the present one
+    int pass;
 };
 
 template <typename Ti, bool AK, bool BK>
@@ -495,29 +505,27 @@ __device__ __forceinline__ void tile_copy(const Pair& p, uint32_t to, int c, int
     else feed_copy<Ti, BK>(p.b, c - C, to + Ti::kBytes, wave, lane);
 }
 
+// Pass i: the pairs from the lowest up.
+__device__ __forceinline__ void tile_pass(Pair& p, int i) {
+    p.in = 0;
+    p.pass = i;
+    feed_plane(p.a, (int)(kPairsA >> (4 * (kPairs - 1 - i))) & 3);
+    feed_plane(p.b, (int)(kPairsB >> (4 * (kPairs - 1 - i))) & 3);
+}
+
 template <typename Ti, int PL>
 __device__ __forceinline__ void tile_advance(Pair& p) {
     feed_advance<Ti>(p.a);
     feed_advance<Ti>(p.b);
-    if (PL > 1 && ++p.in == p.steps) {
-        p.in = 0;
-        ++p.pair;
-        feed_plane(p.a, (int)(kPairsA >> (4 * p.pair)) & 3);
-        feed_plane(p.b, (int)(kPairsB >> (4 * p.pair)) & 3);
-    }
+    if (PL > Ti::P && ++p.in == p.steps && p.pass + 1 < kPairs) tile_pass(p, p.pass + 1);
 }
 
 // The copies of a tile's first S steps (or those it has).
 template <typename Ti, int PL, bool AK, bool BK>
 __device__ __forceinline__ void tile_begin(Pair& p, int64_t steps, uint32_t lds, int wave, int lane) {
     p.steps = steps;
-    p.in = 0;
-    p.pair = 0;
-    if (PL > 1) {
-        feed_plane(p.a, kPairsA & 3);
-        feed_plane(p.b, kPairsB & 3);
-    }
-    const int64_t total = PL > 1 ? steps * kPairs : steps;
+    if (PL > Ti::P) tile_pass(p, 0);
+    const int64_t total = PL > Ti::P ? steps * kPairs : steps;
     const int n = total < Ti::S ? (int)total : Ti::S;
     for (int t = 0; t < n; ++t) {
 #pragma unroll
@@ -526,44 +534,50 @@ __device__ __forceinline__ void tile_begin(Pair& p, int64_t steps, uint32_t lds,
     }
 }
 
-// The tile's products, after tile_begin, whose copies every wave has waited for.  float32: of each pair of planes,
-// from the lowest up.  Between the products of 16 k stand the LDS reads of the next 16, one at a time; the step's
-// barrier stands before its last products, which cover the first reads of the next step and the copies into the step
-// just freed.  (Reads and copies in a row before the products: 54% of the matrix pipes' cycles used at 2.0 GHz; so:
-// 72% at 1.78 GHz, which the power allows; with no copies at all 81% at 1.82 GHz.)
+// The tile's products, after tile_begin, whose copies every wave has waited for.  Between the products of 16 k stand
+// the LDS reads of the next 16, one at a time; the step's barrier stands before its last products, which cover the first
+// reads of the next step and the copies into the step just freed.  (Reads and copies in a row before the products: 54% of
+// the matrix pipes' cycles used at 2.0 GHz; so: 72% at 1.78 GHz, which the power allows; with no copies at all 81% at
+// 1.82 GHz.)
 template <typename Ti, int PL, bool AK, bool BK>
 __device__ __forceinline__ void tile_run(Pair& p, uint32_t lds, f32x16_t (&acc)[Ti::kMI][Ti::kNI], int wave, int lane) {
-    constexpr int B = Ti::B, S = Ti::S, MI = Ti::kMI, NI = Ti::kNI, C = Ti::kCopies, Q = MI * NI, kLast = Ti::kK / 16 - 1;
+    constexpr int B = Ti::B, S = Ti::S, P = Ti::P, MI = Ti::kMI, NI = Ti::kNI, C = Ti::kCopies, Q = (P == 1 ? 1 : kPairs) * MI * NI;
+    constexpr int kReads = P * (MI + NI), kLast = Ti::kK / 16 - 1;
     Reader<Ti, AK, MI> ra;
     Reader<Ti, BK, NI> rb;
     ra.init(wave / Ti::kWN * (B / 2), lane);
     rb.init(wave % Ti::kWN * (32 * NI), lane);
+    f32x16_t low[MI][NI];  // float32: the sum of the lower pairs
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = f32x16_zero();
+        for (int j = 0; j < NI; ++j) acc[i][j] = low[i][j] = f32x16_zero();
     if (p.steps <= 0) return;
-    bf16x8_t a[2][MI], b[2][NI];
+    bf16x8_t a[2][P][MI], b[2][P][NI];
     // read r of 16 k: in the order in which the products take them
     auto read = [&](uint32_t from, int s, int r) {
-        if (r == 0) a[s & 1][0] = ra.get(from, 0, s);
-        else if (r <= NI) b[s & 1][r - 1] = rb.get(from + Ti::kBytes, r - 1, s);
-        else if (r < NI + MI) a[s & 1][r - NI] = ra.get(from, r - NI, s);
+        if (r >= kReads) return;
+        const int l = r / (MI + NI), w = r % (MI + NI);
+        if (w == 0) a[s & 1][l][0] = ra.get(from + l * Ti::kPlane, 0, s);
+        else if (w <= NI) b[s & 1][l][w - 1] = rb.get(from + Ti::kBytes + l * Ti::kPlane, w - 1, s);
+        else a[s & 1][l][w - NI] = ra.get(from + l * Ti::kPlane, w - NI, s);
     };
     // the products of 16 k, after each of which `between(q)` is issued
     auto multiply = [&](int s, auto between) {
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
-            const int i = q / NI, j = q % NI;
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[s & 1][i], b[s & 1][j], acc[i][j], 0, 0, 0);
+            const int pair = q / (MI * NI), i = q / NI % MI, j = q % NI;
+            const int la = kPairsA >> (4 * pair) & 3, lb = kPairsB >> (4 * pair) & 3;
+            f32x16_t& c = pair == 0 ? acc[i][j] : low[i][j];
+            c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[s & 1][la][i], b[s & 1][lb][j], c, 0, 0, 0);
             between(q);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    constexpr int R = (MI + NI + Q - 1) / Q;  // reads after a product
-    const int64_t total = PL > 1 ? p.steps * kPairs : p.steps;
+    constexpr int R = (kReads + Q - 1) / Q;  // reads after a product
+    const int64_t total = PL > Ti::P ? p.steps * kPairs : p.steps;
 #pragma unroll
-    for (int r = 0; r < MI + NI; ++r) read(lds, 0, r);
+    for (int r = 0; r < kReads; ++r) read(lds, 0, r);
     uint32_t cur = 0, from = lds, next = lds + 2 * Ti::kBytes;
     auto flip = [&]() {
         cur = (cur + 1) % S;
@@ -583,12 +597,12 @@ __device__ __forceinline__ void tile_run(Pair& p, uint32_t lds, f32x16_t (&acc)[
         if (t < 2 * S - 1) lds_barrier();  // (the first S steps are there; stores before them may still be on their way)
         else step_barrier<2 * C * (S - 2)>();
         multiply(kLast, [&](int q) {
-            constexpr int P = (2 * C + Q - 1) / Q;  // copies after a product
+            constexpr int N = (2 * C + Q - 1) / Q;  // copies after a product
 #pragma unroll
             for (int r = 0; r < R; ++r) read(next, 0, q * R + r);
 #pragma unroll
-            for (int c = 0; c < P; ++c)
-                if (q * P + c < 2 * C) tile_copy<Ti, AK, BK>(p, from, q * P + c, wave, lane);
+            for (int c = 0; c < N; ++c)
+                if (q * N + c < 2 * C) tile_copy<Ti, AK, BK>(p, from, q * N + c, wave, lane);
         });
         tile_advance<Ti, PL>(p);
         flip();
@@ -604,6 +618,15 @@ __device__ __forceinline__ void tile_run(Pair& p, uint32_t lds, f32x16_t (&acc)[
             for (int r = 0; r < R; ++r) read(next, 0, q * R + r);
         });
         flip();
+    }
+    if constexpr (P > 1) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                acc[i][j] += low[i][j];
+                asm volatile("" : "+v"(acc[i][j]));  // (one value from here on: the compiler would keep both sums for the epilogue)
+            }
     }
     lds_barrier();
 }
@@ -1073,9 +1096,11 @@ __global__ __launch_bounds__(256) void ce_kept_kernel(KeptArgs g) {
 // ------------------------------------------------------------------------ sizes
 constexpr size_t kPieceBytes = (size_t)1 << 30;  // of dl at a time
 
-// Tiles of 256 where they give every CU one, else of 128.
-int tile_for(int64_t rows, int64_t cols, int num_cus) {
-    return cols > 128 && (rows + 255) / 256 * ((cols + 255) / 256) >= num_cus ? 256 : 128;
+// The logits' tiles: of 256 where they give every CU one, or three in float32, where tiles of 128 take all planes at
+// once (1,000 x 512 x 20,000, 316 tiles of 256: 139 us with tiles of 128, 171 with 256; 2,048 x 512 x 32,000, 1,000
+// tiles: 400 and 361 us), else of 128.
+int tile_for(int64_t rows, int64_t cols, int dtype, int num_cus) {
+    return cols > 128 && (rows + 255) / 256 * ((cols + 255) / 256) >= num_cus * (dtype == kBF16 ? 1 : 3) ? 256 : 128;
 }
 
 // Words of the vocabulary in a piece: whole tiles, at most kPieceBytes for all rows.
@@ -1108,7 +1133,7 @@ FwdWs fwd_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus) {
     FwdWs w;
     Take take{p};
     const int64_t np = round_up(n, kPadRows);
-    w.tile = tile_for(vocab, n, num_cus);
+    w.tile = tile_for(vocab, n, dtype, num_cus);
     w.n_part = (int)(round_up(vocab, w.tile) / (w.tile / 2));
     w.part = (float2*)take((size_t)w.n_part * np * 8);
     w.row_loss = (float*)take((size_t)np * 4);
@@ -1132,11 +1157,12 @@ GradWs grad_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus,
     const int planes = planes_of(dtype);
     w.piece = kept ? round_up(vocab, kTileMax) : piece_words(np, vocab, planes);
     const int64_t words = vocab < w.piece ? vocab : w.piece;
-    w.logit_tile = tile_for(words, n, num_cus);
-    // tiles of 256 for the gradients where dW's and dh's parts give every CU one
+    w.logit_tile = tile_for(words, n, dtype, num_cus);
+    // tiles of 256 for bf16 gradients where dW's and dh's parts give every CU one (a float32 pass of 4,096 x 1,024 x 50,000: 9.4 ms
+    // with 256, 8.9 with 128)
     const int64_t cols256 = (d + 255) / 256, m256 = (n + 255) / 256 * cols256;
     const int64_t row256 = m256 * (num_cus / m256 < 1 ? 1 : num_cus / m256 < w.piece / kPartWords ? num_cus / m256 : w.piece / kPartWords);
-    w.grad_tile = d > 128 && (words + 255) / 256 * cols256 + row256 >= num_cus ? 256 : 128;
+    w.grad_tile = dtype == kBF16 && d > 128 && (words + 255) / 256 * cols256 + row256 >= num_cus ? 256 : 128;
     w.p = kept ? nullptr : (uint16_t*)take((size_t)np * w.piece * 2 * planes);
     // parts x tiles of rows for any count of labelled rows: as many as fill the chip, or one part
     const int64_t cols = (d + w.grad_tile - 1) / w.grad_tile, slots = num_cus / cols;
@@ -1150,21 +1176,22 @@ GradWs grad_ws(char* p, int64_t n, int d, int64_t vocab, int dtype, int num_cus,
 
 unsigned xcd_grid(int64_t groups, int each) { return (unsigned)((groups + 7) / 8 * 8 * each); }
 
-// f(tile, planes) as constants.  Tiles of 128 that have a CU each (`alone`) get four steps in LDS and eight waves,
+// f(tile, planes) as constants.  bf16 tiles of 128 that have a CU each (`alone`) get four steps in LDS and eight waves,
 // otherwise two of four waves, with two steps each, share a CU.  100 rows of 4,096 against 16,000 words (125 tiles): 48 us with four
-// steps, 62 with two; gradients of 1,500 float32 rows of 256 against 8,009 words (over 500 tiles): 304 and 260 us.
+// steps, 62 with two.
 template <int V> struct Int {
     static constexpr int v = V;
 };
 template <typename F>
 void with_tile(int tile, bool alone, int dtype, F f) {
-    auto planes = [&](auto t) {
-        if (dtype == kBF16) f(t, Int<1>{});
-        else f(t, Int<3>{});
-    };
-    if (tile == 256) planes(Tile<256, 2>{});
-    else if (alone) planes(Tile<128, 4>{});
-    else planes(Tile<128, 2>{});
+    if (dtype == kBF16) {
+        if (tile == 256) f(Tile<256, 2, 1>{}, Int<1>{});
+        else if (alone) f(Tile<128, 4, 1>{}, Int<1>{});
+        else f(Tile<128, 2, 1>{}, Int<1>{});
+    } else {
+        if (tile == 256) f(Tile<256, 2, 1>{}, Int<3>{});
+        else f(Tile<128, 2, 3>{}, Int<3>{});
+    }
 }
 
 LogitArgs logit_args(const CeState& s, const void* w, const uint16_t* planes, int64_t v0, int64_t v1, int64_t vocab, int d, int dtype) {
@@ -1188,15 +1215,16 @@ LogitArgs logit_args(const CeState& s, const void* w, const uint16_t* planes, in
 
 template <int GRAD>
 void run_logits(const LogitArgs& g, int tile, int dtype, int64_t n, int num_cus, hipStream_t stream) {
-    // as many workgroups as run at once (one to a CU, or two of tiles of 128)
+    // as many workgroups as run at once (one to a CU, or two of bf16 tiles of 128)
     const int64_t m_tiles = (g.v1 - g.v0 + tile - 1) / tile, n_tiles = (n + tile - 1) / tile;
     const int64_t tiles = xcd_grid(m_tiles, (int)n_tiles);
-    const int64_t most = round_up(num_cus, 8) * (tile == 256 ? 1 : 2);
+    const int64_t most = round_up(num_cus, 8) * (tile == 256 || dtype != kBF16 ? 1 : 2);
     const dim3 grid((unsigned)(tiles < most ? tiles : most));
-    with_tile(tile, m_tiles * n_tiles <= num_cus, GRAD == 2 ? (int)kBF16 : dtype, [&](auto t, auto pl) {
+    with_tile(tile, m_tiles * n_tiles <= num_cus, dtype, [&](auto t, auto pl) {
         typedef decltype(t) Ti;
-        constexpr int PL = GRAD == 2 ? 1 : decltype(pl)::v;
-        hipLaunchKernelGGL((ce_logits_kernel<Ti, PL, GRAD>), grid, dim3(Ti::kThreads), 0, stream, g);
+        constexpr int PL = decltype(pl)::v;
+        if constexpr (GRAD != 2 || PL == 1)  // (float32 exponentials are not kept)
+            hipLaunchKernelGGL((ce_logits_kernel<Ti, PL, GRAD>), grid, dim3(Ti::kThreads), 0, stream, g);
     });
 }
 
@@ -1214,7 +1242,7 @@ size_t linear_ce_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int
 // The kept exponentials, and behind them the maxima that they are relative to (with the sums).
 size_t exps_values(int64_t n, int64_t vocab) { return (size_t)round_up(n, kPadRows) * round_up(vocab, kTileMax) * 2; }
 size_t linear_ce_exps_bytes(int64_t n, int64_t vocab, int dtype, int num_cus) {
-    return dtype == kBF16 ? exps_values(n, vocab) + (size_t)round_up(n, kPadRows) * (round_up(vocab, kTileMax) / (tile_for(vocab, n, num_cus) / 2)) * 8 : 0;
+    return dtype == kBF16 ? exps_values(n, vocab) + (size_t)round_up(n, kPadRows) * (round_up(vocab, kTileMax) / (tile_for(vocab, n, dtype, num_cus) / 2)) * 8 : 0;
 }
 size_t linear_ce_grad_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus, bool kept) {
     return grad_ws(nullptr, n, d, vocab, dtype, num_cus, kept).bytes;
@@ -1275,7 +1303,7 @@ int launch_linear_ce_grad(const void* state, void* exps, const void* w, const fl
         g.reduction = reduction;
         if (exps) {
             const KeptArgs a{s.count, s.idx, s.lab, s.lse, s.ll, dloss, (const float2*)((char*)exps + exps_values(n, vocab)), g.p, s.np,
-                             tile_for(vocab, n, num_cus) / 2, reduction};
+                             tile_for(vocab, n, dtype, num_cus) / 2, reduction};
             hipLaunchKernelGGL(ce_kept_kernel, dim3((unsigned)(b.piece / kPanel), (unsigned)(s.np / 64)), dim3(256), 0, stream, a);
         } else {
             run_logits<1>(g, b.logit_tile, dtype, n, num_cus, stream);
@@ -1288,7 +1316,9 @@ int launch_linear_ce_grad(const void* state, void* exps, const void* w, const fl
         const int64_t row = dh ? (n + b.grad_tile - 1) / b.grad_tile * cols * dh_parts(n, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0) : 0;
         with_tile(b.grad_tile, head + row <= num_cus, dtype, [&](auto t, auto pl) {
             typedef decltype(t) Ti;
-            hipLaunchKernelGGL((ce_grads_kernel<Ti, decltype(pl)::v>), dim3((unsigned)(row_blocks + head_blocks)), dim3(Ti::kThreads), 0, stream, a);
+            constexpr int PL = decltype(pl)::v;
+            if constexpr (PL == 1 || Ti::P == PL)  // (float32 gradients: tiles of 128 alone)
+                hipLaunchKernelGGL((ce_grads_kernel<Ti, PL>), dim3((unsigned)(row_blocks + head_blocks)), dim3(Ti::kThreads), 0, stream, a);
         });
     }
     if (dh) {
