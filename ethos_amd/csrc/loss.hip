@@ -335,6 +335,16 @@ __device__ __forceinline__ float row_gradient(const float* dloss, const int32_t*
     return reduction == kLossNone ? dloss[idx[r]] : reduction == kLossMean ? *dloss / (float)m : *dloss;
 }
 
+// The first labelled row's g without its power of two.  dl is held in units of it, and the gradients are multiplied by it
+// last, in float32: where all rows have one g (a mean, or equal weights), a label's dl of nearly -g would otherwise be
+// rounded alike in every row, and whole gradients be off by up to the half step of bf16 (2^-8; error against float64
+// 3.0e-3 for a mean over a third of 1,777 rows, with it 1.8e-3).
+__device__ __forceinline__ float gradient_unit(const float* dloss, const int32_t* idx, int64_t m, int reduction) {
+    if (m == 0) return 1.0f;
+    const uint32_t b = __float_as_uint(row_gradient(dloss, idx, 0, m, reduction)), e = b & 0x7f800000u;
+    return e == 0 || e == 0x7f800000u ? 1.0f : __uint_as_float((b & 0x007fffffu) | 0x3f800000u);
+}
+
 // ------------------------------------------------------------------------ products
 // C[m][n] = sum_k A(m, k) B(k, n) in tiles of B x B (256: eight waves, two along m and four along n, 128 x 64 each;
 // 128: four waves of 64 x 64, or eight of 64 x 32), k in steps of kK.  float32 operands are
@@ -734,11 +744,12 @@ __global__ __launch_bounds__(Ti::kThreads, 2) void ce_logits_kernel(LogitArgs g)
         float lse[NI], k[NI], label_value[NI];
         int label_at[NI];  // the label's word in the wave's B / 2 words
         if constexpr (GRAD == 1) {
+            const float unit = gradient_unit(g.dloss, g.idx, m, g.reduction);
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
                 const int64_t r = tn0 + wn + j * 32 + (lane & 31), rc = r < m ? r : m - 1;
                 lse[j] = g.lse[rc];
-                k[j] = row_gradient(g.dloss, g.idx, rc, m, g.reduction);
+                k[j] = row_gradient(g.dloss, g.idx, rc, m, g.reduction) / unit;
                 const int64_t v = (int64_t)g.lab[rc] - g.v0 - tm0 - wm;
                 label_at[j] = v >= 0 && v < B / 2 && r < m && lane < 32 ? (int)v : -1;
                 label_value[j] = expm1f(g.ll[rc] - lse[j]) * k[j];  // exp(l - lse) - 1 without the cancellation
@@ -917,11 +928,12 @@ __host__ __device__ inline int dh_parts(int64_t m, int tile, int cols, int64_t l
 // that the long parts of dh leave, and the other way round.
 struct GradArgs {
     const uint16_t *p, *h, *w;
-    const int32_t* count;
+    const int32_t *count, *idx;
+    const float* dloss;
     int64_t words, np, ldp, w_plane;
     float* part;
     void* dw;  // the piece's first row
-    int d, ldh, cols, num_cus, add, with_dw;
+    int d, ldh, cols, num_cus, add, with_dw, reduction;
     int64_t row_blocks;
 };
 
@@ -990,6 +1002,7 @@ __device__ __forceinline__ void ce_head_grad(const GradArgs& g, int64_t block, u
     }
     const int wm = wave / Ti::kWN * (B / 2), wn = wave % Ti::kWN * (32 * NI);
     const int rows = g.words - n0 < B ? (int)(g.words - n0) : B;
+    const float unit = gradient_unit(g.dloss, g.idx, *g.count, g.reduction);
 #pragma unroll
     for (int j = 0; j < NI; ++j)
 #pragma unroll
@@ -997,7 +1010,7 @@ __device__ __forceinline__ void ce_head_grad(const GradArgs& g, int64_t block, u
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int n = wn + j * 32 + (lane & 31), mm = wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5);
-                const f32x16_t& a = acc[i][j];
+                const f32x16_t a = acc[i][j] * unit;
                 if constexpr (PL == 1)
                     put4<B>(lds, n, mm, pack_bf16x2(a[e], a[e + 1]), pack_bf16x2(a[e + 2], a[e + 3]));
                 else if (n < rows && m0 + mm < g.d)
@@ -1019,10 +1032,12 @@ __global__ __launch_bounds__(Ti::kThreads, 2) void ce_grads_kernel(GradArgs g) {
 // dh in h's rows and type: the sum of the parts, zeros for rows without a label; 4 columns a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void ce_row_grad_out_kernel(const float* __restrict__ part, const int32_t* __restrict__ count,
-                                                              const int32_t* __restrict__ inv, int64_t n, int d, int tile, int cols,
-                                                              int64_t ldp, int num_cus, int with_dw, T* __restrict__ dh) {
+                                                              const int32_t* __restrict__ inv, const int32_t* __restrict__ idx,
+                                                              const float* __restrict__ dloss, int reduction, int64_t n, int d, int tile,
+                                                              int cols, int64_t ldp, int num_cus, int with_dw, T* __restrict__ dh) {
     const int64_t m = *count, size = round_up(m, kPadRows) * d;
     const int parts = dh_parts(m, tile, cols, ldp, num_cus, with_dw);
+    const float unit = gradient_unit(dloss, idx, m, reduction);
     const int64_t total = n * (d / 4);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t r = i / (d / 4);
@@ -1043,6 +1058,7 @@ __global__ __launch_bounds__(256) void ce_row_grad_out_kernel(const float* __res
                     s.w += v[p].w;
                 }
             }
+        s = make_float4(s.x * unit, s.y * unit, s.z * unit, s.w * unit);
         if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dh + r * d + c) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
         else *reinterpret_cast<float4*>(dh + r * d + c) = s;
     }
@@ -1063,6 +1079,7 @@ __global__ __launch_bounds__(256) void ce_kept_kernel(KeptArgs g) {
     if (r0 >= round_up(m, kPadRows)) return;
     const int64_t panel = blockIdx.x;
     const int word = (threadIdx.x & 31) * 8;
+    const float unit = gradient_unit(g.dloss, g.idx, m, g.reduction);
     uint16_t* p = g.p + (panel * g.np + r0 + (threadIdx.x >> 5)) * kPanel + word;
     const float2* part = g.part + (panel * kPanel + word) / g.each * g.np;
 #pragma unroll
@@ -1073,7 +1090,7 @@ __global__ __launch_bounds__(256) void ce_kept_kernel(KeptArgs g) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int64_t r = r0 + (threadIdx.x >> 5) + (t + u) * 8, rc = r < m ? r : m > 0 ? m - 1 : 0;
-            const float lse = g.lse[rc], x = part[rc].x, k = m > 0 ? row_gradient(g.dloss, g.idx, rc, m, g.reduction) : 0.0f;
+            const float lse = g.lse[rc], x = part[rc].x, k = m > 0 ? row_gradient(g.dloss, g.idx, rc, m, g.reduction) / unit : 0.0f;
             const float f = x == -__builtin_inff() ? k * 0.0f : k * expf(x - lse);  // (no word of the row's: zeros, or NaN)
             const int64_t label = (int64_t)g.lab[rc] - panel * kPanel - word;
             float y[8];
@@ -1310,8 +1327,8 @@ int launch_linear_ce_grad(const void* state, void* exps, const void* w, const fl
         }
         const int64_t row_blocks = dh ? xcd_grid(b.part_tiles, cols) : 0;
         const int64_t head_blocks = dw ? xcd_grid((words + b.grad_tile - 1) / b.grad_tile, cols) : 0;
-        const GradArgs a{g.p, s.h, g.w, s.count, words, s.np, b.piece, g.w_plane, b.part, (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4), d,
-                         s.ldh, cols, num_cus, v0 > 0 ? 1 : 0, dw ? 1 : 0, row_blocks};
+        const GradArgs a{g.p, s.h, g.w, s.count, s.idx, dloss, words, s.np, b.piece, g.w_plane, b.part, (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4), d,
+                         s.ldh, cols, num_cus, v0 > 0 ? 1 : 0, dw ? 1 : 0, reduction, row_blocks};
         const int64_t head = dw ? (words + b.grad_tile - 1) / b.grad_tile * cols : 0;
         const int64_t row = dh ? (n + b.grad_tile - 1) / b.grad_tile * cols * dh_parts(n, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0) : 0;
         with_tile(b.grad_tile, head + row <= num_cus, dtype, [&](auto t, auto pl) {
@@ -1325,11 +1342,11 @@ int launch_linear_ce_grad(const void* state, void* exps, const void* w, const fl
         int64_t blocks = (n * (d / 4) + 255) / 256;
         blocks = blocks < num_cus * 16 ? blocks : num_cus * 16;
         if (dtype == kBF16)
-            hipLaunchKernelGGL((ce_row_grad_out_kernel<uint16_t>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, n,
-                               d, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, (uint16_t*)dh);
+            hipLaunchKernelGGL((ce_row_grad_out_kernel<uint16_t>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv,
+                               s.idx, dloss, reduction, n, d, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, (uint16_t*)dh);
         else
-            hipLaunchKernelGGL((ce_row_grad_out_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, n, d,
-                               b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, (float*)dh);
+            hipLaunchKernelGGL((ce_row_grad_out_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, stream, b.part, s.count, s.inv, s.idx,
+                               dloss, reduction, n, d, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0, (float*)dh);
     }
     return (int)hipGetLastError();
 }

@@ -154,6 +154,25 @@ def test_cross_entropy_of_a_few_steps(n, d, V, dt):
             _within(got, x, e, what)
 
 
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("keep", [0, 1 << 30])
+def test_cross_entropy_of_equal_weights_rounds_rows_apart(reduction, keep):
+    # every row's g lies in the middle of two bf16 values, and every label's probability is near 0: a rounding of g
+    # itself would move both gradients by 2^-8.  Left: the results' rounding, at most 2^-8 / sqrt(3) on the root mean
+    # square, and dl's, of 1 - p to 1, at most 2^-9.
+    n, d, V = 512, 128, 3000
+    g = _gen(23)
+    h, w = torch.randn(n, d, generator=g, device="cuda").bfloat16() * 0.01, torch.randn(V, d, generator=g, device="cuda").bfloat16()
+    labels = torch.randint(0, V, (n,), generator=g, device="cuda")
+    gy = torch.full((n,) if reduction == "none" else (), 1.0 + 2.0 ** -8, device="cuda")
+    (_, *want), _ = _ce_oracle(h, w, labels, reduction, gy)
+    a, b = h.requires_grad_(), w.requires_grad_()
+    loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction=reduction, keep_bytes=keep)
+    for got, x, what in zip(torch.autograd.grad(loss, (a, b), gy), want, ("dh", "dw")):
+        err = float((got.double() - x).norm() / x.norm())
+        assert err <= math.hypot(2.0 ** -8 / math.sqrt(3.0), 2.0 ** -9), f"{what} {err}"
+
+
 def test_cross_entropy_gradient_against_differences():
     h, w, labels = _ce_inputs(9, 16, 37, torch.float32, seed=2, ignored=0.3)
     labels[0] = 5
