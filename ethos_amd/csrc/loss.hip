@@ -16,7 +16,8 @@
 // maximum's, against the 2^-8 of dl's own rounding to bf16.
 //
 // float32 operands go through the same kernels as three bf16 planes each, x = hi + mid + lo
-// (ethos_split.hpp): a product is six bf16 products, exact in the float32 sums, the smallest first.
+// (ethos_split.hpp): a product is six bf16 products, each exact in float32, the lower five in a sum of their own or (in
+// tiles of 256) the smallest first.
 #include <type_traits>
 
 #include "ethos_common.hpp"
