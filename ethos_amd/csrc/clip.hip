@@ -6,9 +6,9 @@
 // for the norm and the factor, then the scaled copy, last pieces first (what the norm read last may still be
 // in the caches).  Bound by memory: the gradients are read twice, as the norm comes before the first scaled value.
 // 535 MB in 186 tensors take 267 us (norm 92, copy 175), 6.0 TB/s of 1.6 GB.  What was measured there: pieces of 8192,
-// 16384, 24576 and 32768 values 325, 267, 279 and 289 us; copies that go into the caches 317 us (they push out what the
-// next norm reads, and leave it their own writing back); one load on its way in the copy 3% more.  The tensors' addresses travel as kernel arguments, as many as fit their 4 KiB: a launch
-// and pass for up to 180 tensors.
+// 16384, 24576 and 32768 values 325, 267, 279 and 289 us; with the last, copies that go into the caches 318 us (they push
+// out what the next norm reads, and leave it their own writing back), and one load on its way in the copy 331.  The
+// tensors' addresses travel as kernel arguments, as many as fit their 4 KiB: a launch and pass for up to 180 tensors.
 #include "ethos_common.hpp"
 #include "ethos_rows.hpp"
 #include "ethos_train.hpp"

@@ -1260,7 +1260,9 @@ size_t linear_ce_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int
 // The kept exponentials, and behind them the maxima that they are relative to (with the sums).
 size_t exps_values(int64_t n, int64_t vocab) { return (size_t)round_up(n, kPadRows) * round_up(vocab, kTileMax) * 2; }
 size_t linear_ce_exps_bytes(int64_t n, int64_t vocab, int dtype, int num_cus) {
-    return dtype == kBF16 ? exps_values(n, vocab) + (size_t)round_up(n, kPadRows) * (round_up(vocab, kTileMax) / (tile_for(vocab, n, dtype, num_cus) / 2)) * 8 : 0;
+    if (dtype != kBF16) return 0;
+    const int64_t maxima = round_up(vocab, kTileMax) / (tile_for(vocab, n, dtype, num_cus) / 2);
+    return exps_values(n, vocab) + (size_t)round_up(n, kPadRows) * maxima * 8;
 }
 size_t linear_ce_grad_workspace_bytes(int64_t n, int d, int64_t vocab, int dtype, int num_cus, bool kept) {
     return grad_ws(nullptr, n, d, vocab, dtype, num_cus, kept).bytes;
@@ -1328,8 +1330,9 @@ int launch_linear_ce_grad(const void* state, void* exps, const void* w, const fl
         }
         const int64_t row_blocks = dh ? xcd_grid(b.part_tiles, cols) : 0;
         const int64_t head_blocks = dw ? xcd_grid((words + b.grad_tile - 1) / b.grad_tile, cols) : 0;
-        const GradArgs a{g.p, s.h, g.w, s.count, s.idx, dloss, words, s.np, b.piece, g.w_plane, b.part, (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4), d,
-                         s.ldh, cols, num_cus, v0 > 0 ? 1 : 0, dw ? 1 : 0, reduction, row_blocks};
+        void* const dw_piece = dw ? (char*)dw + v0 * d * (dtype == kBF16 ? 2 : 4) : nullptr;
+        const GradArgs a{g.p, s.h, g.w, s.count, s.idx, dloss, words, s.np, b.piece, g.w_plane, b.part, dw_piece, d, s.ldh, cols, num_cus,
+                         v0 > 0 ? 1 : 0, dw ? 1 : 0, reduction, row_blocks};
         const int64_t head = dw ? (words + b.grad_tile - 1) / b.grad_tile * cols : 0;
         const int64_t row = dh ? (n + b.grad_tile - 1) / b.grad_tile * cols * dh_parts(n, b.grad_tile, cols, b.piece, num_cus, dw ? 1 : 0) : 0;
         with_tile(b.grad_tile, head + row <= num_cus, dtype, [&](auto t, auto pl) {
