@@ -30,7 +30,10 @@ namespace ethos {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kScaled = 1e38f;  // logits below this in size can be scaled by log2(e)
+// exp(l - x) is taken as exp2(l log2(e) - RN(x log2(e))) where |x| is below this: at l = x that is not 1 but 2^r, with r
+// the rounding of x log2(e), here within 2^-14 (a factor of 4e-5 and less, as much as float32 rounds a logit of that size
+// by; at 1e10 r is in the hundreds).  Beyond it x is subtracted first, which is exact near l = x and below it never positive.
+constexpr float kScaled = 1024.0f;
 constexpr int kPadRows = 256;  // labelled rows are padded with zero rows to a multiple of this
 
 __host__ __device__ constexpr int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }

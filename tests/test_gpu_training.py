@@ -262,6 +262,62 @@ def test_cross_entropy_with_labels_far_below(dt):
             _within(got, y, e, f"{what} {rows}")
 
 
+@pytest.mark.parametrize("mask", [-1e4, -1e6, -1e9, -1e10, -1e20, -1e30, -1e37])
+@pytest.mark.parametrize("dt,n,V", [("bf16", 50, 700), ("fp32", 50, 700), ("bf16", 700, 30011), ("fp32", 2048, 30011)])
+def test_cross_entropy_blocks_of_masked_words(dt, n, V, mask):
+    """Words masked by a finite low logit, blocks of 64 and 128 of them in a row (in tiles of 128 and of 256): they
+    have no part in the loss and no gradient, whichever way the backward goes."""
+    h, w, labels = _ce_inputs(n, 64, V, DT[dt], seed=V)
+    lo, hi = V // 3, 2 * V // 3
+    h[:, 0] = 1.0
+    w[lo:hi, 0] = mask
+    labels %= lo
+    gy = torch.rand(n, generator=_gen(7), device="cuda")
+    want, bound = _ce_oracle(h, torch.cat([w[:lo], w[hi:]]), labels, "none", gy)
+    for keep in (0, 1 << 30):
+        a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="none", keep_bytes=keep)
+        dh, dw = torch.autograd.grad(loss, (a, b), gy)
+        assert bool((dw[lo:hi] == 0).all()), f"masked words keep={keep}"
+        for got, x, e, what in zip((loss.detach(), dh, torch.cat([dw[:lo], dw[hi:]])), want, bound, ("loss", "dh", "dw")):
+            _within(got, x, e, f"{what} keep={keep}")
+
+
+@pytest.mark.parametrize("size", [2 ** 9, -2 ** 9, 2 ** 12, -2 ** 12, 2 ** 20, 7 * 2 ** 31, -7 * 2 ** 31, 9 * 2 ** 31, -9 * 2 ** 31])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_cross_entropy_of_large_logits(dt, size):
+    """Logits `size` plus small whole numbers (none above 2^20), exact in every partial sum.  Left are the roundings of
+    the log-sum and of values scaled by log2(e), U |lse| each: they move the loss, and a probability by their exponential."""
+    n, d, V = 40, 64, 700
+    g = _gen(17)
+    h = torch.randint(-1, 2, (n, d), generator=g, device="cuda").double()
+    w = torch.randint(-1, 2, (V, d), generator=g, device="cuda").double()
+    if abs(size) > 2 ** 20:
+        w.zero_()
+    h[:, 0], w[:, 0] = 1.0, float(size)
+    labels = torch.randint(0, V, (n,), generator=g, device="cuda")
+    x = h @ w.T
+    lse = torch.logsumexp(x, 1)
+    at = torch.arange(n, device="cuda"), labels
+    rows = lse - x[at]
+    e_loss = 2 * U * lse.abs() + 2.0 ** -18 + 2 * U * rows
+    dl = (x - lse[:, None]).exp()
+    e_dl = dl * torch.expm1(3 * U * lse.abs() + 2.0 ** -17).clamp(max=1e30)[:, None] + dl * 2.0 ** -11 + 2.0 ** -25
+    dl[at] -= 1.0
+    t = half_step(DT[dt])
+    e_dl += dl.abs() * (8 * U + (t if dt == "bf16" else 0.0))
+    dh, dw = (dl @ w)[:, 1:], dl.T @ h
+    e_dh = (e_dl @ w.abs() + (V + 64) * U * (dl.abs() @ w.abs()))[:, 1:] + t * dh.abs() * 1.01
+    e_dw = e_dl.T @ h.abs() + (n + 64) * U * (dl.abs().T @ h.abs()) + t * dw.abs() * 1.01
+    for keep in (0, 1 << 30):
+        a, b = h.to(DT[dt]).requires_grad_(), w.to(DT[dt]).requires_grad_()
+        loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="none", keep_bytes=keep)
+        got = torch.autograd.grad(loss, (a, b), torch.ones(n, device="cuda"))
+        _within(loss.detach(), rows, e_loss, f"loss keep={keep}")
+        _within(got[0][:, 1:], dh, e_dh, f"dh keep={keep}")
+        _within(got[1], dw, e_dw, f"dw keep={keep}")
+
+
 def test_cross_entropy_table_past_32_bits():
     n, d, V = 5, 16384, 140000  # 4.6 GB
     w = torch.empty(V, d, dtype=torch.bfloat16, device="cuda")
