@@ -70,6 +70,7 @@ SIGNATURES = {
     "ethos_expert_forward": (ctypes.c_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp,
                                             _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _sz, _vp, _vp,
                                             _vp]),
+    "ethos_capture_id": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_uint64)]),
     "ethos_linear_ce_state_bytes": (_sz, [_i64, _i32, _i32]),
     "ethos_linear_ce_workspace_bytes": (_sz, [_i64, _i32, _i64, _i32]),
     "ethos_linear_ce": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i32, _i64, _i64, _i32, _i32] + [_vp, _sz] * 3 + [_vp, _vp]),

@@ -109,6 +109,18 @@ int ethos_stage_events(void* const* events, int32_t n_events) {
     return 0;
 }
 
+int ethos_capture_id(void* stream, uint64_t* id) {
+    g_err[0] = 0;
+    if (!id) return fail(ETHOS_ENULL, "ethos_capture_id: null pointer");
+    *id = 0;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long n = 0;
+    const hipError_t rc = hipStreamGetCaptureInfo((hipStream_t)stream, &status, &n);
+    if (rc != hipSuccess) return hip_status((int)rc, "ethos_capture_id");
+    if (status == hipStreamCaptureStatusActive) *id = (uint64_t)n + 1;
+    return 0;
+}
+
 const char* ethos_last_error(void) { return g_err; }
 
 int ethos_abi_version(void) { return ETHOS_ABI_VERSION; }

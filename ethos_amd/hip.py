@@ -60,6 +60,15 @@ def stage_events(events) -> None:
     check(load().ethos_stage_events(arr, len(handles)), "ethos_stage_events")
 
 
+def capture_id() -> int:
+    """A number of the capture that records the current stream, 0 without one."""
+    if not torch.cuda.is_current_stream_capturing():
+        return 0
+    n = ctypes.c_uint64()
+    check(load().ethos_capture_id(_stream(), ctypes.byref(n)), "ethos_capture_id")
+    return n.value
+
+
 def key_norm_bounds(sub_keys_1: torch.Tensor, sub_keys_2: torch.Tensor) -> torch.Tensor:
     """fp32 [2, K] upper bounds of the sub-key row norms, on the tables' device: fp64 norms of
     the stored values, inflated by 2^-20 and rounded (once per parameter version)."""

@@ -69,7 +69,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         ctx.save_for_backward(weight, state, exps)
         ctx.copy = w if w.data_ptr() != weight.data_ptr() else None
         ctx.shape, ctx.reduction = h.shape, reduction
-        ctx.fresh, ctx.captured = True, torch.cuda.is_current_stream_capturing()
+        ctx.fresh, ctx.capture = True, hip.capture_id()
         return loss
 
     @staticmethod
@@ -77,8 +77,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def backward(ctx, dloss):
         weight, state, exps = ctx.saved_tensors
         # the first backward uses the exponentials up: a second one of a retained graph has none, nor has one that
-        # is captured alone, to be replayed
-        if not ctx.fresh or (exps is not None and not ctx.captured and torch.cuda.is_current_stream_capturing()):
+        # is captured apart from its forward, to be replayed more often than that
+        if not ctx.fresh or (exps is not None and hip.capture_id() not in (0, ctx.capture)):
             exps = None
         else:
             ctx.fresh = False

@@ -73,6 +73,12 @@ extern "C" {
  */
 int ethos_stage_events(void* const* events, int32_t n_events);
 
+/*
+ * The capture that `stream` is recorded by (hipStreamBeginCapture), no counterpart in the reference: *id (host
+ * memory) is a number of that capture's own, 0 without one.  Two calls with one number are replayed together.
+ */
+int ethos_capture_id(void* stream, uint64_t* id);
+
 /* Message for the calling thread's last failed call ("" after a success). */
 const char* ethos_last_error(void);
 

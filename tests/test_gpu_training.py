@@ -612,6 +612,38 @@ def test_a_backward_captured_alone_can_be_replayed():
         assert torch.equal(eager[0], again[0]) and torch.equal(eager[1], again[1])
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_a_backward_captured_apart_from_its_forward_can_be_replayed(dt):
+    """Forward and backward in graphs of their own, as wrappers of callables capture them: the backward's replays after
+    one replay of the forward, each of another gradient, against eager results."""
+    h, w, labels = _ce_inputs(130, 64, 700, DT[dt], seed=3)
+    a, b, gy = h.requires_grad_(), w.requires_grad_(), torch.ones(130, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def eager():
+        return torch.autograd.grad(ethos_amd.linear_cross_entropy(a, b, labels, reduction="none", keep_bytes=0), (a, b), gy)
+
+    with torch.cuda.stream(side):
+        eager()
+        torch.cuda.synchronize()
+        forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(forward, stream=side):
+            loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="none")
+        with torch.cuda.graph(backward, stream=side):
+            got = torch.autograd.grad(loss, (a, b), gy, retain_graph=True)
+        for seed in (1, 2):
+            labels.copy_(torch.randint(0, 700, (130,), generator=_gen(seed), device="cuda"))
+            forward.replay()
+            for scale in (1.0, -3.0, 0.5):
+                gy.copy_(torch.rand(130, generator=_gen(seed), device="cuda") * scale)
+                backward.replay()
+                torch.cuda.synchronize()
+                want = eager()
+                torch.cuda.synchronize()
+                assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (seed, scale)
+
+
 @pytest.mark.parametrize("train", [False, True])
 def test_no_copy_of_the_logits(train):
     """Without gradients, or with none of the exponentials kept, the loss's memory beside its inputs and

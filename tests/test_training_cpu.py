@@ -45,6 +45,11 @@ def test_linear_ce_argument_errors_are_codes():
     assert grad(n=0, w=None) == 0 and grad(dh=None, dw=None) == 0
 
 
+def test_capture_id_needs_a_place_for_it():
+    L = _lib.load()
+    assert L.ethos_capture_id(None, None) == -3 and b"null" in L.ethos_last_error()
+
+
 def test_embedding_balance_and_clip_argument_errors_are_codes():
     L = _lib.load()
     big, top = 1 << 40, 2 ** 31 - 1
