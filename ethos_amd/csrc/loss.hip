@@ -1095,7 +1095,8 @@ __global__ __launch_bounds__(256) void ce_kept_kernel(KeptArgs g) {
         for (int u = 0; u < 4; ++u) {
             const int64_t r = r0 + (threadIdx.x >> 5) + (t + u) * 8, rc = r < m ? r : m > 0 ? m - 1 : 0;
             const float lse = g.lse[rc], x = part[rc].x, k = m > 0 ? row_gradient(g.dloss, g.idx, rc, m, g.reduction) / unit : 0.0f;
-            const float f = x == -__builtin_inff() ? k * 0.0f : k * expf(x - lse);  // (no word of the row's: zeros, or NaN)
+            // (no word of the row's there: zeros, or NaN; no word of it at all, a log-sum of -inf: NaN)
+            const float f = x == -__builtin_inff() && lse > x ? k * 0.0f : k * expf(x - lse);
             const int64_t label = (int64_t)g.lab[rc] - panel * kPanel - word;
             float y[8];
 #pragma unroll

@@ -318,6 +318,21 @@ def test_cross_entropy_of_large_logits(dt, size):
         _within(got[1], dw, e_dw, f"dw keep={keep}")
 
 
+@pytest.mark.parametrize("keep", [0, 1 << 30])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_cross_entropy_of_a_row_without_any_word(dt, keep):
+    # every logit of row 3 is -inf, so none of its probabilities is a number
+    h, w, labels = _ce_inputs(20, 64, 700, DT[dt], seed=9)
+    h[:, 0], w[:, 0] = 1.0, 0.25
+    h[3, 0] = -math.inf
+    a, b = h.requires_grad_(), w.requires_grad_()
+    loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="none", keep_bytes=keep)
+    assert loss.isnan().nonzero()[:, 0].tolist() == [3]
+    dh, dw = torch.autograd.grad(loss, (a, b), torch.ones(20, device="cuda"))
+    assert dh.isnan().all(1).nonzero()[:, 0].tolist() == [3] and not bool(dh[:3].isnan().any() | dh[4:].isnan().any())
+    assert bool(dw.isnan().all())
+
+
 def test_cross_entropy_table_past_32_bits():
     n, d, V = 5, 16384, 140000  # 4.6 GB
     w = torch.empty(V, d, dtype=torch.bfloat16, device="cuda")
