@@ -299,7 +299,10 @@ __global__ __launch_bounds__(1024) void ce_lse_kernel(const float2* __restrict__
         for (int w = 4; w < 16; w += 4) a = join(a, lds[w + (lane >> 4)][lane & 15]);
         a = join(a, {__shfl_xor(a.m, 16), __shfl_xor(a.s, 16)});
         a = join(a, {__shfl_xor(a.m, 32), __shfl_xor(a.s, 32)});
-        const float l = x == x ? a.m + __builtin_amdgcn_logf(a.s) * 0.69314718055994530942f : x;
+        const float sum = a.m + __builtin_amdgcn_logf(a.s) * 0.69314718055994530942f;
+        // The label's logit x is summed in another order than the products: where it is all of the sum, it may come out
+        // above it, which it never is.  (A NaN of either stays.)
+        const float l = x != x || sum < x ? x : sum;
         out = l - x;
         if (lane < 16 && r < m) {
             lse[r] = l;

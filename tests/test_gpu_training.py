@@ -333,6 +333,25 @@ def test_cross_entropy_of_a_row_without_any_word(dt, keep):
     assert bool(dw.isnan().all())
 
 
+@pytest.mark.parametrize("keep", [0, 1 << 30])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_cross_entropy_is_never_negative(dt, keep):
+    """Rows along their labels' rows: the labels' logits (some 5,000) are all of their log-sums but e^-4000, so a loss is the
+    difference of two roundings of one sum of d products.  It is not negative, and its gradient moves no logit of a label down."""
+    n, d, V = 256, 1024, 512
+    g = _gen(31)
+    w = torch.randn(V, d, generator=g, device="cuda").to(DT[dt])
+    labels = torch.randint(0, V, (n,), generator=g, device="cuda")
+    h = w[labels] * 5.0
+    a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="none", keep_bytes=keep)
+    dh, _ = torch.autograd.grad(loss, (a, b), torch.ones(n, device="cuda"))
+    assert bool((loss >= 0).all()), float(loss.min())
+    _within(loss.detach(), torch.zeros(n, device="cuda").double(), 2 * (d + 2) * U * (h.double().abs() * w[labels].double().abs()).sum(1), "loss")
+    assert float((dh.double() * w[labels].double()).sum(1).max()) <= 0.0
+    assert float(ethos_amd.linear_cross_entropy(h, w, labels)) >= 0.0
+
+
 def test_cross_entropy_table_past_32_bits():
     n, d, V = 5, 16384, 140000  # 4.6 GB
     w = torch.empty(V, d, dtype=torch.bfloat16, device="cuda")
