@@ -10,13 +10,15 @@
 The reference trains through torch operations (F.cross_entropy of model.py:396's logits, nn.Embedding,
 nn.utils.clip_grad_norm_) and has no balance loss.  Inputs are HIP tensors on the current device, bf16
 or float32; there is no CPU path.  All work goes to the current stream.  Results are the same on
-every run.  The gradients are those of a single backward (no create_graph)."""
+every run.  The gradients are those of a single backward (no create_graph); forward-mode derivatives and
+torch.jit.trace, which would not see the kernels' results, are refused."""
 from __future__ import annotations
 
 import math
 import operator
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import hip
@@ -47,6 +49,15 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
         n = t.numel() // t.shape[-1] if t.numel() else 0
         return t.as_strided((n, t.shape[-1]), (ld, 1))
     return _dense(t).view(-1, t.shape[-1])
+
+
+def _refuse_followed(what: str, *ts) -> None:
+    """Raise where something follows the operations on the tensors that the kernels, which take addresses, hide
+    from it: forward-mode derivatives would be lost, a trace would record results that nothing writes."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} cannot be traced by torch.jit.trace")
+    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 def _device_check(name: str, t: torch.Tensor) -> None:
@@ -100,6 +111,7 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     loss is float32.  Gradients go to h and weight, in their dtype.  For them the backward forms the logits
     again, a piece of the vocabulary at a time; in bf16 the forward leaves the exponentials behind instead (in
     16 bits, in the memory that the backward would take anyway) where these take at most `keep_bytes`."""
+    _refuse_followed("linear_cross_entropy", h, weight)
     for name, t in (("h", h), ("weight", weight), ("labels", labels)):
         _device_check(name, t)
     if reduction not in ("mean", "sum", "none"):
@@ -143,6 +155,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     any shape (int32 or int64).  The table's gradient is dense, leaves out positions of `padding_idx`
     (negative ones count from the end) and adds a token's positions in a fixed order, in float32.  An
     id outside the table gives a row of NaN."""
+    _refuse_followed("embedding", weight)
     ids, w = _contiguous(ids), _contiguous(weight)  # (types and devices: hip.embedding)
     if isinstance(w, torch.Tensor) and (w.dim() != 2 or w.numel() == 0):
         raise RuntimeError(f"embedding: weight must be [vocab, d], got {tuple(w.shape)}")
@@ -184,6 +197,7 @@ def balance_loss(gates: torch.Tensor, ids: torch.Tensor, n_experts: int):
     loss = n_experts * sum_e f_e s_e (float32), f_e = counts[e] / (n heads k) held fixed and s_e the
     sum of expert e's gates over (n heads); it is 1 when both are even over the experts.  counts is int32
     [n_experts].  Ids outside [0, n_experts) count nowhere.  Without tokens both are zero."""
+    _refuse_followed("balance_loss", gates)
     _device_check("gates", gates)
     _device_check("ids", ids)
     gates, ids = _contiguous(gates), _contiguous(ids)  # (dtypes: hip.balance)
@@ -214,6 +228,7 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torc
         raise ValueError(f"{len(grads)} gradients but {len(out)} outputs")
     # (a training step has hundreds of tensors: each check is one pass of a C function over them)
     ts = grads if out is grads else grads + out
+    _refuse_followed("clip_grads", *ts)
     if not set(map(type, ts)) <= _TENSORS and not all([isinstance(t, torch.Tensor) for t in ts]):
         raise TypeError("clip_grads takes tensors")
     if not ts:

@@ -96,3 +96,33 @@ def test_entry_points_refuse_host_tensors():
             call()
     with pytest.raises(TypeError):
         ethos_amd.linear_cross_entropy(None, h, l)
+
+
+def _calls(f, i):
+    """The four entry points with a float tensor f [4, 8] in each differentiable place, and whole numbers i [4, 8]."""
+    ids = i.view(-1)[:4]
+    return (lambda: ethos_amd.linear_cross_entropy(f, f.detach(), ids), lambda: ethos_amd.linear_cross_entropy(f.detach(), f, ids),
+            lambda: ethos_amd.embedding(ids, f), lambda: ethos_amd.balance_loss(f, i, 4), lambda: ethos_amd.clip_grads([f], 1.0),
+            lambda: ethos_amd.clip_grads([f.detach()], 1.0, out=[f]))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_entry_points_refuse_forward_mode_derivatives(grad):
+    i = torch.zeros(4, 8, dtype=torch.int64)
+    with torch.autograd.forward_ad.dual_level():
+        f = torch.autograd.forward_ad.make_dual(torch.ones(4, 8, requires_grad=grad), torch.ones(4, 8))
+        # (torch's detach keeps the tangent: both operands of the loss have one)
+        for call in _calls(f, i):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        # without a tangent it goes on, here to the refusal of host tensors
+        for call in _calls(torch.ones(4, 8), i):
+            with pytest.raises(RuntimeError, match="HIP device"):
+                call()
+
+
+def test_entry_points_refuse_tracing():
+    i = torch.zeros(4, 8, dtype=torch.int64)
+    for k in range(len(_calls(torch.ones(4, 8), i))):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(lambda f: _calls(f, i)[k](), (torch.ones(4, 8),))
