@@ -100,6 +100,21 @@ class _LinearCrossEntropy(torch.autograd.Function):
         return dh.view(ctx.shape) if want_h else None, dw, None, None, None, None
 
 
+class _NoRows(torch.autograd.Function):
+    """The loss of no rows (`value`), with zero gradients."""
+
+    @staticmethod
+    def forward(ctx, h, weight, value):
+        ctx.like = h.shape, weight.shape, weight.dtype, weight.device
+        return value
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _):
+        rows, table, dtype, device = ctx.like
+        return torch.zeros(rows, dtype=dtype, device=device), torch.zeros(table, dtype=dtype, device=device), None
+
+
 def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100,
                          reduction: str = "mean", keep_bytes: int = 1 << 30) -> torch.Tensor:
     """Softmax cross entropy of h @ weight.T against labels, without forming the logits.
@@ -125,9 +140,10 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     d = h.shape[-1]
     if weight.shape[0] == 0 or d == 0 or d % 8 or d > 32768:
         raise RuntimeError(f"linear_cross_entropy: needs a vocabulary and d a multiple of 8 up to 32768, got weight {tuple(weight.shape)}")
-    if labels.numel() == 0:  # the sum over nothing, with zero gradients
-        zero = h.float().sum() + 0.0 * weight[:1].float().sum() if reduction != "none" else h.float().sum(-1)
-        return zero if reduction != "mean" else zero / 0.0
+    if labels.numel() == 0:
+        shape = labels.shape if reduction == "none" else ()
+        value = torch.full(shape, math.nan if reduction == "mean" else 0.0, dtype=torch.float32, device=h.device)
+        return _NoRows.apply(h, weight, value)
     flat = labels.contiguous().view(-1)
     if torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad):
         loss = _LinearCrossEntropy.apply(h, weight, flat, int(ignore_index), reduction, int(keep_bytes))

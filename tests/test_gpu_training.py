@@ -352,6 +352,25 @@ def test_cross_entropy_is_never_negative(dt, keep):
     assert float(ethos_amd.linear_cross_entropy(h, w, labels)) >= 0.0
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_cross_entropy_of_no_rows(dt, reduction):
+    h, w = torch.zeros(2, 0, 16, device="cuda", dtype=DT[dt]), torch.randn(9, 16, device="cuda", generator=_gen(0)).to(DT[dt])
+    w[0, 0], w[1, 1] = math.inf, math.nan
+    labels = torch.zeros(2, 0, dtype=torch.int64, device="cuda")
+    a, b = h.requires_grad_(), w.requires_grad_()
+    loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction=reduction)
+    assert loss.dtype == torch.float32 and loss.shape == ((2, 0) if reduction == "none" else ()) and loss.requires_grad
+    value = loss.detach()
+    assert reduction == "none" or (float(value) == 0.0 if reduction == "sum" else math.isnan(float(value)))
+    # as for a batch of ignored positions
+    dh, dw = torch.autograd.grad(loss, (a, b), torch.ones_like(loss))
+    assert dh.shape == h.shape and dh.dtype == h.dtype and dw.dtype == w.dtype and bool((dw == 0).all()) and dw.shape == w.shape
+    with torch.no_grad():
+        same = ethos_amd.linear_cross_entropy(a, b, labels, reduction=reduction)
+    assert not same.requires_grad and torch.equal(same.nan_to_num(7.0), loss.detach().nan_to_num(7.0))
+
+
 def test_cross_entropy_table_past_32_bits():
     n, d, V = 5, 16384, 140000  # 4.6 GB
     w = torch.empty(V, d, dtype=torch.bfloat16, device="cuda")
