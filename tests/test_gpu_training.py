@@ -723,6 +723,34 @@ def test_wrappers_refuse_other_devices(monkeypatch):
         ethos_amd.embedding(torch.zeros(3, dtype=torch.int64, device="cuda"), torch.zeros(4, 8, device="cuda"))
 
 
+def test_wrappers_refuse_what_the_kernels_cannot_read():
+    """Each wrapper with one argument wrong: on the host, of another type, of too few values."""
+    z = lambda *s, dt=torch.float32: torch.zeros(s, dtype=dt, device="cuda")  # noqa: E731
+    i32, i64 = torch.int32, torch.int64
+
+    def refused(call, good, **bad):
+        call(**good)
+        for name, values in bad.items():
+            for v in values:
+                with pytest.raises((RuntimeError, TypeError)):
+                    call(**{**good, name: v})
+
+    ce = dict(h=z(4, 16), w=z(9, 16), labels=z(4, dt=i64), ignore_index=-100, reduction="none")
+    refused(hip.linear_ce, ce, h=(z(4, 16).cpu(), z(4, 16, dt=torch.bfloat16), z(3, 16), z(4, 8), z(16, 4).t(), z(2, 2, 16), None),
+            w=(z(9, 16).cpu(), z(9, 8), z(16, 9).t()), labels=(z(4).long().cpu(), z(4, dt=i32), z(5, dt=i64)))
+    _, state, _ = hip.linear_ce(**ce)
+    grad = dict(state=state, exps=None, w=ce["w"], dloss=z(4), n=4, reduction="none", want_h=True, want_w=True)
+    refused(hip.linear_ce_grad, grad, state=(state.cpu(), state[:1], state.int()), w=(ce["w"].cpu(), z(16, 9).t()),
+            dloss=(z(4).cpu(), z(3), z(1), z(4).double(), z(8)[::2]), exps=(state.cpu(), state))
+    keys = dict(keys=z(4, dt=i32), dy=z(4, 16), vocab=9, scale=1.0)
+    refused(hip.embedding_grad, keys, keys=(z(4, dt=i64), z(4, dt=i32).cpu(), z(5, dt=i32)), dy=(z(4, 16).cpu(), z(3, 16), z(16, 4).t()))
+    bal = dict(gates=z(4, 2, 3), ids=z(4, 2, 3, dt=i32), n_experts=5)
+    refused(hip.balance, bal, gates=(z(3, 2, 3), z(4, 2, 3).cpu(), z(6)), ids=(z(4, 2, 2, dt=i32), z(4, 2, 3, dt=i32).cpu()))
+    back = dict(ids=bal["ids"], counts=z(5, dt=i32), dloss=z(), dtype=torch.float32)
+    refused(hip.balance_grad, back, ids=(bal["ids"].cpu(), z(4, dt=i32)), counts=(z(5, dt=i32).cpu(), z(5, dt=i64)),
+            dloss=(z().cpu(), z().double(), z(2)))
+
+
 # ------------------------------------------------------------------------------- the model's loss
 def _tiny_model(seed=0):
     from ethos_amd.model import CompressedMoEModel
