@@ -442,6 +442,22 @@ def test_embedding_ids_outside_the_table_and_views():
     assert torch.equal(ethos_amd.embedding(ids.view(-1)[::3], odd), w[[3, 49]])
 
 
+def test_embedding_gradient_of_more_runs_than_a_launch_takes_at_once():
+    # 2^24 + 2 runs of eight positions; whole numbers, whose sums stay below 2^24 and so are exact in float32
+    n, V, d = 2 ** 27 + 13, 1000, 2
+    g = _gen(29)
+    ids = torch.randint(0, V, (n,), generator=g, device="cuda", dtype=torch.int32)
+    ids[-9:] = V - 1
+    p = torch.zeros(V, d, device="cuda", requires_grad=True)
+    y = ethos_amd.embedding(ids, p)
+    dy = torch.randint(-8, 9, (n, d), generator=g, device="cuda", dtype=torch.int8).float()
+    dw = torch.autograd.grad(y, p, dy)[0]
+    want = torch.zeros(V, d, dtype=torch.float64, device="cuda")
+    for i, x in zip(ids.split(2 ** 24), dy.split(2 ** 24)):
+        want.index_add_(0, i, x.double())
+    assert float(want.abs().max()) < 2 ** 24 and torch.equal(dw.double(), want)
+
+
 # ------------------------------------------------------------------------------- balance
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
 @pytest.mark.parametrize("itype", [torch.int32, torch.int64])
