@@ -939,11 +939,13 @@ int ethos_layer_forward(const void* x, const void* wq, const void* wq_prepared, 
 namespace {
 
 constexpr int64_t kMaxItems = (int64_t)1 << 30;
+// Rows of the loss: its launches have up to 64 threads for each of them (rounded up to 256), which have to stay below 2^32.
+constexpr int64_t kMaxRows = ((int64_t)1 << 26) - 256;
 
 // Sizes of the loss over the vocabulary.
 int ce_sizes(int64_t n, int32_t d, int64_t vocab, int32_t reduction, int32_t dtype, const char* what) {
     if (!dtype_ok(dtype)) return fail(ETHOS_EDTYPE, "%s: unknown dtype %d", what, dtype);
-    if (n < 0 || n > kMaxItems || d <= 0 || vocab <= 0 || vocab > kMaxItems || reduction < 0 || reduction > 2)
+    if (n < 0 || n > kMaxRows || d <= 0 || vocab <= 0 || vocab > kMaxItems || reduction < 0 || reduction > 2)
         return fail(ETHOS_ESIZE, "%s: bad sizes n_tok=%lld d=%d vocab=%lld reduction=%d", what, (long long)n, d, (long long)vocab,
                     reduction);
     if (d % 8 || d > 32768) return fail(ETHOS_EUNSUPPORTED, "%s: d must be a multiple of 8, at most 32768 (got %d)", what, d);
@@ -953,12 +955,12 @@ int ce_sizes(int64_t n, int32_t d, int64_t vocab, int32_t reduction, int32_t dty
 }  // namespace
 
 size_t ethos_linear_ce_state_bytes(int64_t n_tok, int32_t d, int32_t dtype) {
-    if (n_tok <= 0 || n_tok > kMaxItems || d <= 0 || !dtype_ok(dtype)) return 256;
+    if (n_tok <= 0 || n_tok > kMaxRows || d <= 0 || !dtype_ok(dtype)) return 256;
     return ethos::linear_ce_state_bytes(n_tok, d, dtype);
 }
 
 size_t ethos_linear_ce_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype) {
-    if (n_tok <= 0 || n_tok > kMaxItems || d <= 0 || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
+    if (n_tok <= 0 || n_tok > kMaxRows || d <= 0 || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
     return ethos::linear_ce_workspace_bytes(n_tok, d, vocab, dtype, num_cus());
 }
 
@@ -987,12 +989,12 @@ int ethos_linear_ce(const void* h, int64_t ldh, const void* w, const int64_t* la
 }
 
 size_t ethos_linear_ce_exps_bytes(int64_t n_tok, int64_t vocab, int32_t dtype) {
-    if (n_tok <= 0 || n_tok > kMaxItems || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 0;
+    if (n_tok <= 0 || n_tok > kMaxRows || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 0;
     return ethos::linear_ce_exps_bytes(n_tok, vocab, dtype, num_cus());
 }
 
 size_t ethos_linear_ce_grad_workspace_bytes(int64_t n_tok, int32_t d, int64_t vocab, int32_t dtype, int32_t kept) {
-    if (n_tok <= 0 || n_tok > kMaxItems || d <= 0 || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
+    if (n_tok <= 0 || n_tok > kMaxRows || d <= 0 || vocab <= 0 || vocab > kMaxItems || !dtype_ok(dtype)) return 256;
     return ethos::linear_ce_grad_workspace_bytes(n_tok, d, vocab, dtype, num_cus(), kept != 0);
 }
 

@@ -1242,7 +1242,7 @@ template <int GRAD>
 void run_logits(const LogitArgs& g, int tile, int dtype, int64_t n, int num_cus, hipStream_t stream) {
     // as many workgroups as run at once (one to a CU, or two of bf16 tiles of 128)
     const int64_t m_tiles = (g.v1 - g.v0 + tile - 1) / tile, n_tiles = (n + tile - 1) / tile;
-    const int64_t tiles = xcd_grid(m_tiles, (int)n_tiles);
+    const int64_t tiles = (m_tiles + 7) / 8 * 8 * n_tiles;
     const int64_t most = round_up(num_cus, 8) * (tile == 256 || dtype != kBF16 ? 1 : 2);
     const dim3 grid((unsigned)(tiles < most ? tiles : most));
     with_tile(tile, m_tiles * n_tiles <= num_cus, dtype, [&](auto t, auto pl) {

@@ -527,7 +527,7 @@ int ethos_layer_forward(const void* x, const void* wq, const void* wq_prepared, 
  * forms a piece of the vocabulary's logits at a time again (their gradients take at most 1 GiB, or 256 words); for
  * bf16 the logits' gradients are rounded to bf16 for the products with h and w.
  * Limits: d a multiple of 8, at most 32768; ldh a multiple of 8 (bf16) or 4; vocab <= 2^30; n_tok
- * <= 2^30; h, w, state, exps, workspace, dh and dw 16-byte aligned.  n_tok = 0 does nothing.
+ * <= 2^26 - 256; h, w, state, exps, workspace, dh and dw 16-byte aligned.  n_tok = 0 does nothing.
  */
 #define ETHOS_LOSS_MEAN 0
 #define ETHOS_LOSS_SUM 1

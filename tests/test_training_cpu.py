@@ -45,6 +45,15 @@ def test_linear_ce_argument_errors_are_codes():
     assert grad(n=0, w=None) == 0 and grad(dh=None, dw=None) == 0
 
 
+def test_linear_ce_refuses_more_rows_than_its_launches_have_threads_for():
+    L = _lib.load()
+    big, most = 1 << 60, (1 << 26) - 256
+    for n, code in ((most, -3), (most + 1, -2), (1 << 26, -2), (1 << 30, -2)):
+        assert L.ethos_linear_ce(None, 8, 16, 16, n, 8, 9, -100, 0, 1, 16, big, None, 0, 16, big, 16, None) == code, n
+        assert L.ethos_linear_ce_grad(None, big, None, 0, 16, 16, n, 8, 9, 0, 1, 16, big, 16, 16, None) == code, n
+    assert L.ethos_linear_ce_state_bytes(most, 8, 1) > most and L.ethos_linear_ce_state_bytes(most + 1, 8, 1) == 256
+
+
 def test_capture_id_needs_a_place_for_it():
     L = _lib.load()
     assert L.ethos_capture_id(None, None) == -3 and b"null" in L.ethos_last_error()
