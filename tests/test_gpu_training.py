@@ -140,6 +140,18 @@ def test_cross_entropy_in_the_largest_tiles(dt, n, ignored, keep):
         _within(got, x, e, what)
 
 
+@pytest.mark.parametrize("n,d,ignored", [(2048, 264, 0.0), (2048, 40, 0.0), (2300, 320, 0.2)])
+def test_cross_entropy_float32_passes_over_planes_in_the_largest_tiles(n, d, ignored):
+    # 118 x 8 and x 9 tiles of 256, above three a CU: the planes' pairs in passes over one, five and (partly) five steps of 64
+    h, w, labels = _ce_inputs(n, d, 30011, torch.float32, seed=d, ignored=ignored)
+    gy = torch.rand(n, generator=_gen(2), device="cuda")
+    want, bound = _ce_oracle(h, w, labels, "none", gy)
+    a, b = h.requires_grad_(), w.requires_grad_()
+    loss = ethos_amd.linear_cross_entropy(a, b, labels, reduction="none")
+    for got, x, e, what in zip((loss.detach(), *torch.autograd.grad(loss, (a, b), gy)), want, bound, ("loss", "dh", "dw")):
+        _within(got, x, e, what)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
 @pytest.mark.parametrize("n,d,V", [(40, 136, 300), (130, 320, 260), (200, 384, 700), (330, 448, 129)])
 def test_cross_entropy_of_a_few_steps(n, d, V, dt):
