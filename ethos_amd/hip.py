@@ -677,6 +677,11 @@ def _need_here(t: torch.Tensor, name: str, dtypes, dim=None) -> None:
     raise RuntimeError(f"{name} is on {t.device}, not on the current device")
 
 
+def _dense_at(device: int, t, dtype=None) -> bool:
+    """Whether t is a contiguous tensor on that device (of that type): the backwards' check, in few calls."""
+    return isinstance(t, torch.Tensor) and t.get_device() == device and t.is_contiguous() and (dtype is None or t.dtype == dtype)
+
+
 @functools.lru_cache(maxsize=1024)
 def _size(name: str, device: int, *args: int) -> int:
     """A workspace size function's answer (`device`: some depend on the GPU's CUs)."""
@@ -697,9 +702,9 @@ def linear_ce(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, ignore_ind
     which overwrites exps."""
     _need_here(w, "weight", FLOATS, 2)
     _need_here(labels, "labels", (torch.int64,), 1)
-    if not isinstance(h, torch.Tensor) or h.device != w.device or h.dtype != w.dtype:
+    if not isinstance(h, torch.Tensor) or h.get_device() != w.get_device() or h.dtype != w.dtype:
         raise RuntimeError(f"h must be a tensor of {w.dtype} on {w.device}")
-    if h.dim() != 2 or h.shape != (labels.numel(), w.shape[1]) or h.stride(1) != 1:
+    if h.dim() != 2 or h.shape[0] != labels.numel() or h.shape[1] != w.shape[1] or h.stride(1) != 1:
         raise RuntimeError(f"h must be [{labels.numel()}, {w.shape[1]}] with contiguous rows, got {tuple(h.shape)} of strides {h.stride()}")
     n, d = h.shape
     code, lib, device = dtype_code(h.dtype), load(), h.device
@@ -720,11 +725,14 @@ def linear_ce(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, ignore_ind
 def linear_ce_grad(state: torch.Tensor, exps: torch.Tensor | None, w: torch.Tensor, dloss: torch.Tensor, n: int, reduction: str,
                    want_h: bool, want_w: bool):
     """(dh [n, d], dw [V, d]) from dloss (float32, contiguous); None for one not wanted."""
-    _need_here(w, "weight", FLOATS, 2)
-    _need_here(state, "state", (torch.int64,), 1)
-    _need_here(dloss, "dloss", (torch.float32,))
-    if exps is not None:
-        _need_here(exps, "exps", (torch.int64,), 1)
+    device = _current_device()
+    if not (_dense_at(device, state, torch.int64) and _dense_at(device, dloss, torch.float32) and _dense_at(device, w) and w.dim() == 2
+            and (exps is None or _dense_at(device, exps, torch.int64))):
+        _need_here(w, "weight", FLOATS, 2)
+        _need_here(state, "state", (torch.int64,))
+        _need_here(dloss, "dloss", (torch.float32,))
+        if exps is not None:
+            _need_here(exps, "exps", (torch.int64,))
     if dloss.numel() != (n if reduction == "none" else 1):
         raise RuntimeError(f"dloss must have {n if reduction == 'none' else 1} values, got {dloss.numel()}")
     V, d = w.shape
@@ -755,9 +763,10 @@ def embedding(ids: torch.Tensor, w: torch.Tensor, scale: float, padding: int = -
 
 def embedding_grad(keys: torch.Tensor, dy: torch.Tensor, vocab: int, scale: float) -> torch.Tensor:
     """The table's gradient [vocab, d] from dy [*keys.shape, d] and the lookup's keys."""
-    _need_here(keys, "keys", (torch.int32,))
+    if not _dense_at(_current_device(), keys, torch.int32):
+        _need_here(keys, "keys", (torch.int32,))
     _need_here(dy, "dy", FLOATS)
-    if dy.dim() == 0 or dy.shape[:-1] != keys.shape:
+    if dy.dim() == 0 or keys.numel() * dy.shape[-1] != dy.numel():
         raise RuntimeError(f"dy must be [*keys.shape, d], got {tuple(dy.shape)} for keys {tuple(keys.shape)}")
     n, d = keys.numel(), dy.shape[-1]
     lib = load()
@@ -773,9 +782,9 @@ def balance(gates: torch.Tensor, ids: torch.Tensor, n_experts: int):
     """(loss float32 [], counts int32 [n_experts]) of gates and ids [..., heads, k]."""
     _need_here(gates, "gates", FLOATS)
     _need_here(ids, "ids", INTS)
-    if gates.dim() < 2 or gates.shape != ids.shape or 0 in gates.shape[-2:]:
-        raise RuntimeError(f"gates and ids must both be [..., heads, k], got {tuple(gates.shape)} and {tuple(ids.shape)}")
-    H, k = gates.shape[-2:]
+    H, k = gates.shape[-2:] if gates.dim() > 1 else (0, 0)
+    if H == 0 or k == 0 or gates.shape != ids.shape:
+        raise RuntimeError(f"balance: gates and ids must both be [..., heads, k], got {tuple(gates.shape)} and {tuple(ids.shape)}")
     n = gates.numel() // (H * k)
     lib = load()
     ws, ws_bytes = _scratch("ethos_balance_workspace_bytes", gates.device, n, H, k, n_experts)
@@ -789,12 +798,15 @@ def balance(gates: torch.Tensor, ids: torch.Tensor, n_experts: int):
 
 def balance_grad(ids: torch.Tensor, counts: torch.Tensor, dloss: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """The gates' gradient, the shape of ids."""
-    _need_here(ids, "ids", INTS)
-    _need_here(counts, "counts", (torch.int32,), 1)
-    _need_here(dloss, "dloss", (torch.float32,))
-    if ids.dim() < 2 or 0 in ids.shape[-2:] or dloss.numel() != 1:
+    device = _current_device()
+    if not (_dense_at(device, ids) and _dense_at(device, counts, torch.int32) and _dense_at(device, dloss, torch.float32)
+            and ids.dtype in INTS):
+        _need_here(ids, "ids", INTS)
+        _need_here(counts, "counts", (torch.int32,))
+        _need_here(dloss, "dloss", (torch.float32,))
+    H, k = ids.shape[-2:] if ids.dim() > 1 else (0, 0)
+    if H == 0 or k == 0 or dloss.numel() != 1:
         raise RuntimeError(f"ids must be [..., heads, k] and dloss one value, got {tuple(ids.shape)} and {tuple(dloss.shape)}")
-    H, k = ids.shape[-2:]
     out = torch.empty(ids.shape, dtype=dtype, device=ids.device)
     rc = load().ethos_balance_grad(ids.data_ptr(), int(ids.dtype == torch.int64), counts.data_ptr(), dloss.data_ptr(),
                                    ids.numel() // (H * k), H, k, counts.numel(), dtype_code(dtype), out.data_ptr(), _stream())

@@ -35,15 +35,15 @@ def _contiguous(t):
     return t.contiguous() if isinstance(t, torch.Tensor) and not t.is_contiguous() else t
 
 
+# (both without gradients: within autograd functions, or on tensors that need none)
 def _dense(t: torch.Tensor) -> torch.Tensor:
     """t contiguous at a 16-byte address (a copy where it is not)."""
-    t = t.detach().contiguous()
+    t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """[n, d] rows of t [..., d] that the kernels can read: evenly spaced, 16-byte aligned."""
-    t = t.detach()
     ld = hip.row_stride(t)
     if ld >= t.shape[-1] and ld * t.element_size() % 16 == 0 and t.data_ptr() % 16 == 0:
         n = t.numel() // t.shape[-1] if t.numel() else 0
@@ -51,12 +51,16 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return _dense(t).view(-1, t.shape[-1])
 
 
+def _is_followed() -> bool:
+    return torch._C._is_tracing() or forward_ad._current_level >= 0
+
+
 def _refuse_followed(what: str, *ts) -> None:
     """Raise where something follows the operations on the tensors that the kernels, which take addresses, hide
     from it: forward-mode derivatives would be lost, a trace would record results that nothing writes."""
     if torch.jit.is_tracing():
         raise RuntimeError(f"{what} cannot be traced by torch.jit.trace")
-    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in ts):
         raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
@@ -93,7 +97,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
             exps = None
         else:
             ctx.fresh = False
-        w = weight.detach() if ctx.copy is None else ctx.copy
+        w = weight if ctx.copy is None else ctx.copy
         n = math.prod(ctx.shape[:-1])
         want_h, want_w = ctx.needs_input_grad[:2]
         dh, dw = hip.linear_ce_grad(state, exps, w, dloss.float().contiguous(), n, ctx.reduction, want_h, want_w)
@@ -126,7 +130,8 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     loss is float32.  Gradients go to h and weight, in their dtype.  For them the backward forms the logits
     again, a piece of the vocabulary at a time; in bf16 the forward leaves the exponentials behind instead (in
     16 bits, in the memory that the backward would take anyway) where these take at most `keep_bytes`."""
-    _refuse_followed("linear_cross_entropy", h, weight)
+    if _is_followed():
+        _refuse_followed("linear_cross_entropy", h, weight)
     for name, t in (("h", h), ("weight", weight), ("labels", labels)):
         _device_check(name, t)
     if reduction not in ("mean", "sum", "none"):
@@ -171,7 +176,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, paddi
     any shape (int32 or int64).  The table's gradient is dense, leaves out positions of `padding_idx`
     (negative ones count from the end) and adds a token's positions in a fixed order, in float32.  An
     id outside the table gives a row of NaN."""
-    _refuse_followed("embedding", weight)
+    if _is_followed():
+        _refuse_followed("embedding", weight)
     ids, w = _contiguous(ids), _contiguous(weight)  # (types and devices: hip.embedding)
     if isinstance(w, torch.Tensor) and (w.dim() != 2 or w.numel() == 0):
         raise RuntimeError(f"embedding: weight must be [vocab, d], got {tuple(w.shape)}")
@@ -213,15 +219,12 @@ def balance_loss(gates: torch.Tensor, ids: torch.Tensor, n_experts: int):
     loss = n_experts * sum_e f_e s_e (float32), f_e = counts[e] / (n heads k) held fixed and s_e the
     sum of expert e's gates over (n heads); it is 1 when both are even over the experts.  counts is int32
     [n_experts].  Ids outside [0, n_experts) count nowhere.  Without tokens both are zero."""
-    _refuse_followed("balance_loss", gates)
-    _device_check("gates", gates)
-    _device_check("ids", ids)
-    gates, ids = _contiguous(gates), _contiguous(ids)  # (dtypes: hip.balance)
-    if gates.dim() < 2 or gates.shape != ids.shape or 0 in gates.shape[-2:]:
-        raise RuntimeError(f"balance_loss: gates and ids must both be [..., heads, k], got {tuple(gates.shape)} and {tuple(ids.shape)}")
+    if _is_followed():
+        _refuse_followed("balance_loss", gates)
+    gates, ids = _contiguous(gates), _contiguous(ids)  # (types, shapes and devices: hip.balance)
     if n_experts <= 0:
         raise ValueError(f"n_experts must be positive, got {n_experts}")
-    if torch.is_grad_enabled() and gates.requires_grad:
+    if torch.is_grad_enabled() and isinstance(gates, torch.Tensor) and gates.requires_grad:
         return _Balance.apply(gates, ids, int(n_experts))
     return hip.balance(gates, ids, int(n_experts))
 
@@ -244,7 +247,8 @@ def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torc
         raise ValueError(f"{len(grads)} gradients but {len(out)} outputs")
     # (a training step has hundreds of tensors: each check is one pass of a C function over them)
     ts = grads if out is grads else grads + out
-    _refuse_followed("clip_grads", *ts)
+    if _is_followed():
+        _refuse_followed("clip_grads", *ts)
     if not set(map(type, ts)) <= _TENSORS and not all([isinstance(t, torch.Tensor) for t in ts]):
         raise TypeError("clip_grads takes tensors")
     if not ts:
