@@ -2,7 +2,7 @@
 (include/ethos_hip.h):
 
   linear_cross_entropy  softmax cross entropy of hidden rows against a head matrix, and its
-                        gradients, without the logits in memory
+                        gradients, without the logits in memory (their exponentials may be)
   embedding             rows of a table, scaled; the table's gradient by sorted tokens
   balance_loss          how often each expert was chosen, the load-balance loss, its gradient
   clip_grads            the global norm of many gradients, and the clipped gradients
@@ -128,8 +128,9 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     gradients; another label outside the vocabulary makes the loss NaN.  `reduction`: "mean" over the
     labelled positions (NaN without one), "sum", or "none" (float32 [...], zero where ignored).  The
     loss is float32.  Gradients go to h and weight, in their dtype.  For them the backward forms the logits
-    again, a piece of the vocabulary at a time; in bf16 the forward leaves the exponentials behind instead (in
-    16 bits, in the memory that the backward would take anyway) where these take at most `keep_bytes`."""
+    again, a piece of the vocabulary at a time; in bf16 the forward leaves the exponentials behind instead, in
+    16 bits, where these take at most `keep_bytes`.  They take what the backward would take anyway, but from the
+    forward on, once for every loss that waits for its backward."""
     if _is_followed():
         _refuse_followed("linear_cross_entropy", h, weight)
     for name, t in (("h", h), ("weight", weight), ("labels", labels)):

@@ -27,6 +27,7 @@
  *   ethos_embedding, ethos_embedding_grad  embedding rows and their table's gradient
  *   ethos_balance, ethos_balance_grad      expert counts, the load-balance loss, its gradient
  *   ethos_clip_grads     the global norm of many gradients, and clipping
+ *   ethos_capture_id     which capture records a stream
  *
  * Conventions (every entry point):
  *   - All pointers are device pointers owned by the caller; nothing is allocated.
@@ -520,7 +521,7 @@ int ethos_layer_forward(const void* x, const void* wq, const void* wq_prepared, 
  *   loss    float32, one value or (NONE) [n_tok]
  *   exps    NULL, or (bf16) >= ethos_linear_ce_exps_bytes(...) bytes, which is 0 for float32: the forward leaves the
  *           exponentials there, in 16 bits, for one ethos_linear_ce_grad, which then does not form the logits
- *           again (and overwrites exps)
+ *           again (and overwrites exps: in captured graphs, each replay of that call needs one of the forward)
  * Logits, exponentials' sums and losses are float32, a reduction's sum float64.
  * ethos_linear_ce_grad: dh [n_tok, d] and dw [vocab, d] of dtype T (either may be NULL) from dloss
  * (float32: one value or, NONE, [n_tok]), with the state that the forward left and the same w.  Without exps it
