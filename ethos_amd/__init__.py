@@ -4,7 +4,8 @@ as gfx950 HIP kernels behind a C-ABI (include/ethos_hip.h).
 
 The layer classes are drop-ins for the reference's (wrmedford/ETHOS model.py and
 kernels.py); see ethos_amd.layer.  Around them stand the operators of a training step: the loss over the
-vocabulary, the embedding, the experts' balance and gradient clipping; see ethos_amd.training.
+vocabulary, the embedding, the experts' balance and gradient clipping; see ethos_amd.training.  The model is
+served from a cache of latents in pages; see ethos_amd.serving.
 """
 from .layer import (  # noqa: F401
     EthosExpertLayer,
@@ -13,6 +14,7 @@ from .layer import (  # noqa: F401
     ProductKeyRouter,
     SimplifiedHypernetMoE,
 )
+from .serving import copy_pages, latent_append, paged_attention, verify_drafts  # noqa: F401
 from .training import balance_loss, clip_grads, embedding, linear_cross_entropy  # noqa: F401
 
 __all__ = [
@@ -23,6 +25,10 @@ __all__ = [
     "SimplifiedHypernetMoE",
     "balance_loss",
     "clip_grads",
+    "copy_pages",
     "embedding",
+    "latent_append",
     "linear_cross_entropy",
+    "paged_attention",
+    "verify_drafts",
 ]

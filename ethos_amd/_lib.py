@@ -85,6 +85,14 @@ SIGNATURES = {
     "ethos_balance_grad": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i64, _i32, _i32, _i64, _i32, _vp, _vp]),
     "ethos_clip_grads_workspace_bytes": (_sz, [_vp, _i32]),
     "ethos_clip_grads": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _f64, _vp, _sz, _vp, _vp]),
+    "ethos_latent_append": (ctypes.c_int, [_vp, _i64] + [_vp] * 3 + [_i64, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i64, _i32, _f32, _i32, _vp,
+                                           _vp]),
+    "ethos_copy_pages": (ctypes.c_int, [_vp] + [_i64] * 4 + [_vp, _vp, _i32, _vp]),
+    "ethos_paged_attention_workspace_bytes": (_sz, [_i64] + [_i32] * 7),
+    "ethos_paged_attention": (ctypes.c_int, [_vp] * 4 + [_i64, _i32] + [_vp] * 3 + [_i64] + [_i32] * 6 + [_i64, _i32, _i32, _f32, _vp, _sz, _vp,
+                                             _vp]),
+    "ethos_verify_workspace_bytes": (_sz, [_i64, _i32, _i64]),
+    "ethos_verify": (ctypes.c_int, [_vp] * 3 + [_i32] + [_vp] * 3 + [_i64, _i32, _i64, _f64, _i32, _vp, _sz, _vp, _vp, _vp]),
     "ethos_token_proj": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp]),
     "ethos_apply_hidden_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32]),
     "ethos_apply_hidden": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32,

@@ -11,6 +11,7 @@
 #include "../../include/ethos_hip.h"
 #include "ethos_common.hpp"
 #include "ethos_launch.hpp"
+#include "ethos_serve.hpp"
 #include "ethos_train.hpp"
 
 namespace {
@@ -1140,6 +1141,148 @@ int ethos_clip_grads(const void* const* in, void* const* out, const int64_t* siz
     if (!aligned16(workspace)) return fail(ETHOS_EALIGN, "ethos_clip_grads: workspace must be 16-byte aligned");
     return hip_status(ethos::launch_clip(in, out, sizes, dtypes, n_tensors, inf_norm, max_norm, workspace, total, (hipStream_t)stream),
                       "ethos_clip_grads");
+}
+
+namespace {
+
+// The parts of a batch over a cache that the host can see (what the tables hold is checked on the device).
+int batch_sizes(int64_t n_rows, int32_t n_seq, int64_t table_ld, int32_t table_width, int64_t n_pages, int32_t page, int32_t rank, int32_t rope,
+                int32_t dtype, const char* what) {
+    if (!dtype_ok(dtype)) return fail(ETHOS_EDTYPE, "%s: unknown dtype %d", what, dtype);
+    if (n_rows < 0 || n_rows > INT32_MAX / 4 || n_seq < 0 || n_seq > (1 << 20) || table_width < 0 || table_ld < table_width || n_pages <= 0 ||
+        n_pages > INT32_MAX || page <= 0 || rank <= 0 || rope < 0)
+        return fail(ETHOS_ESIZE, "%s: bad sizes n_rows=%lld n_seq=%d table_width=%d n_pages=%lld page=%d rank=%d rope=%d", what,
+                    (long long)n_rows, n_seq, table_width, (long long)n_pages, page, rank, rope);
+    const int vec = dtype == ETHOS_BF16 ? 8 : 4;
+    if ((page & (page - 1)) || page > 65536)
+        return fail(ETHOS_EUNSUPPORTED, "%s: page must be a power of two up to 65536, got %d", what, page);
+    if (rank % vec || rope % vec || rank > 512 || rope > 128)
+        return fail(ETHOS_EUNSUPPORTED, "%s: rank and rope must be multiples of %d, at most 512 and 128 (got %d, %d)", what, vec, rank, rope);
+    return 0;
+}
+ethos::Batch batch_of(const int32_t* table, int64_t table_ld, int32_t table_width, const int32_t* lens, const int32_t* starts, int32_t n_seq,
+                      int64_t n_rows, int64_t n_pages, int32_t page) {
+    int log = 0;
+    while ((1 << log) < page) ++log;
+    return ethos::Batch{table, table_ld, table_width, lens, starts, n_seq, n_rows, n_pages, log};
+}
+
+}  // namespace
+
+int ethos_latent_append(const void* rows, int64_t ld, const void* gain, const float* rates, const int32_t* table, int64_t table_ld,
+                        int32_t table_width, const int32_t* lens, const int32_t* starts, int32_t n_seq, int64_t n_rows, int32_t rank,
+                        int32_t rope, int64_t n_pages, int32_t page, float eps, int32_t dtype, void* pool, void* stream) {
+    g_err[0] = 0;
+    if (const int rc = batch_sizes(n_rows, n_seq, table_ld, table_width, n_pages, page, rank, rope, dtype, "ethos_latent_append")) return rc;
+    if (ld < (int64_t)rank + rope || ld % (dtype == ETHOS_BF16 ? 8 : 4))
+        return fail(ETHOS_ESIZE, "ethos_latent_append: ld %lld must be at least rank + rope and keep rows 16-byte aligned", (long long)ld);
+    if (n_rows == 0 || n_seq == 0) return 0;
+    if (!rows || !gain || (rope > 0 && !rates) || (table_width > 0 && !table) || !lens || !starts || !pool)
+        return fail(ETHOS_ENULL, "ethos_latent_append: null pointer");
+    if (!aligned16(rows) || !aligned16(gain) || !aligned16(pool))
+        return fail(ETHOS_EALIGN, "ethos_latent_append: rows, gain and pool must be 16-byte aligned");
+    return hip_status(ethos::launch_latent_append(rows, ld, gain, rates,
+                                                  batch_of(table, table_ld, table_width, lens, starts, n_seq, n_rows, n_pages, page), rank, rope,
+                                                  eps, dtype, pool, (hipStream_t)stream),
+                      "ethos_latent_append");
+}
+
+int ethos_copy_pages(void* pool, int64_t n_blocks, int64_t block_bytes, int64_t n_pages, int64_t page_bytes, const int32_t* src,
+                     const int32_t* dst, int32_t n_pairs, void* stream) {
+    g_err[0] = 0;
+    if (n_blocks < 0 || n_blocks > 65535 || n_pages < 0 || n_pages > INT32_MAX || page_bytes <= 0 || page_bytes % 2 || n_pairs < 0 ||
+        page_bytes > ((int64_t)1 << 40) || (n_pages > 0 && block_bytes / page_bytes < n_pages))
+        return fail(ETHOS_ESIZE, "ethos_copy_pages: bad sizes n_blocks=%lld block_bytes=%lld n_pages=%lld page_bytes=%lld n_pairs=%d",
+                    (long long)n_blocks, (long long)block_bytes, (long long)n_pages, (long long)page_bytes, n_pairs);
+    if (n_blocks == 0 || n_pairs == 0) return 0;
+    if (!pool || !src || !dst) return fail(ETHOS_ENULL, "ethos_copy_pages: null pointer");
+    if (((uintptr_t)pool & 1u) || block_bytes % 2) return fail(ETHOS_EALIGN, "ethos_copy_pages: pool or block_bytes misaligned");
+    for (int32_t i = 0; i < n_pairs; ++i)
+        if (src[i] < 0 || src[i] >= n_pages || dst[i] < 0 || dst[i] >= n_pages)
+            return fail(ETHOS_ESIZE, "ethos_copy_pages: pair %d (%d to %d) is outside the %lld pages", i, src[i], dst[i], (long long)n_pages);
+    return hip_status(ethos::launch_copy_pages(pool, n_blocks, block_bytes, page_bytes, src, dst, n_pairs, num_cus(), (hipStream_t)stream),
+                      "ethos_copy_pages");
+}
+
+namespace {
+
+int paged_sizes(int64_t n_rows, int32_t n_heads, int32_t nope, int32_t v_dim, const char* what) {
+    if (n_heads <= 0 || n_heads > 1024 || nope < 0 || v_dim <= 0 || nope > 4096 || v_dim > 4096)
+        return fail(ETHOS_ESIZE, "%s: bad sizes n_heads=%d nope=%d v_dim=%d", what, n_heads, nope, v_dim);
+    if (n_rows * n_heads > INT32_MAX / 4) return fail(ETHOS_ESIZE, "%s: too many rows", what);
+    return 0;
+}
+
+}  // namespace
+
+size_t ethos_paged_attention_workspace_bytes(int64_t n_rows, int32_t n_seq, int32_t n_heads, int32_t rank, int32_t rope, int32_t nope,
+                                             int32_t v_dim, int32_t dtype) {
+    if (n_rows <= 0 || n_seq <= 0 || batch_sizes(n_rows, n_seq, 0, 0, 1, 1, rank, rope, dtype, "ethos_paged_attention_workspace_bytes") != 0 ||
+        paged_sizes(n_rows, n_heads, nope, v_dim, "ethos_paged_attention_workspace_bytes") != 0)
+        return 256;
+    return ethos::paged_attention_workspace_bytes(n_rows, n_seq, n_heads, rank, rope, nope, v_dim, dtype, num_cus());
+}
+
+int ethos_paged_attention(const void* q, const void* w, const void* pool, const int32_t* table, int64_t table_ld, int32_t table_width,
+                          const int32_t* lens, const int32_t* starts, const float* rates, int64_t n_rows, int32_t n_seq, int32_t n_heads,
+                          int32_t rank, int32_t rope, int32_t nope, int32_t v_dim, int64_t n_pages, int32_t page, int32_t dtype, float scale,
+                          void* workspace, size_t workspace_bytes, void* out, void* stream) {
+    g_err[0] = 0;
+    if (const int rc = batch_sizes(n_rows, n_seq, table_ld, table_width, n_pages, page, rank, rope, dtype, "ethos_paged_attention")) return rc;
+    if (const int rc = paged_sizes(n_rows, n_heads, nope, v_dim, "ethos_paged_attention")) return rc;
+    if (!(scale > 0.0f && scale <= 3.0e38f)) return fail(ETHOS_ESIZE, "ethos_paged_attention: scale must be positive, got %g", (double)scale);
+    if (n_rows == 0 || n_seq == 0) return 0;
+    if (!q || !w || !pool || (table_width > 0 && !table) || !lens || !starts || (rope > 0 && !rates) || !workspace || !out)
+        return fail(ETHOS_ENULL, "ethos_paged_attention: null pointer");
+    const size_t need = ethos::paged_attention_workspace_bytes(n_rows, n_seq, n_heads, rank, rope, nope, v_dim, dtype, num_cus());
+    if (workspace_bytes < need)
+        return fail(ETHOS_EWORKSPACE, "ethos_paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (!aligned16(q) || !aligned16(w) || !aligned16(pool) || !aligned16(workspace) || !aligned16(out))
+        return fail(ETHOS_EALIGN, "ethos_paged_attention: q, w, pool, workspace and out must be 16-byte aligned");
+    return hip_status(ethos::launch_paged_attention(q, w, pool,
+                                                    batch_of(table, table_ld, table_width, lens, starts, n_seq, n_rows, n_pages, page), rates,
+                                                    n_heads, rank, rope, nope, v_dim, dtype, scale, workspace, out, num_cus(),
+                                                    (hipStream_t)stream),
+                      "ethos_paged_attention");
+}
+
+namespace {
+
+int verify_sizes(int64_t n_seq, int32_t n_drafts, int64_t vocab, const char* what) {
+    if (n_seq < 0 || n_drafts < 0 || vocab <= 0 || n_seq > INT32_MAX)
+        return fail(ETHOS_ESIZE, "%s: bad sizes n_seq=%lld n_drafts=%d vocab=%lld", what, (long long)n_seq, n_drafts, (long long)vocab);
+    if (n_drafts > 255 || vocab > ((int64_t)1 << 24))
+        return fail(ETHOS_EUNSUPPORTED, "%s: at most 255 drafts and 2^24 words, got %d and %lld", what, n_drafts, (long long)vocab);
+    if (n_seq * (n_drafts + 1) * ((vocab + 2047) / 2048) > INT32_MAX / 2) return fail(ETHOS_ESIZE, "%s: too many rows", what);
+    return 0;
+}
+
+}  // namespace
+
+size_t ethos_verify_workspace_bytes(int64_t n_seq, int32_t n_drafts, int64_t vocab) {
+    if (n_seq == 0 || verify_sizes(n_seq, n_drafts, vocab, "ethos_verify_workspace_bytes") != 0) return 256;
+    return ethos::verify_workspace_bytes(n_seq, n_drafts, vocab);
+}
+
+int ethos_verify(const void* logits, const int64_t* drafts, const void* probs, int32_t probs_dtype, const int32_t* counts,
+                 const float* u_accept, const float* u_sample, int64_t n_seq, int32_t n_drafts, int64_t vocab, double temperature,
+                 int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* accepted, int64_t* tokens, void* stream) {
+    g_err[0] = 0;
+    if (!dtype_ok(dtype) || (probs && !dtype_ok(probs_dtype)))
+        return fail(ETHOS_EDTYPE, "ethos_verify: unknown dtype %d or %d", dtype, probs_dtype);
+    if (const int rc = verify_sizes(n_seq, n_drafts, vocab, "ethos_verify")) return rc;
+    if (!(temperature == 0.0 || (temperature >= 1e-6 && temperature <= 1e6)))
+        return fail(ETHOS_ESIZE, "ethos_verify: temperature must be 0 or from 1e-6 to 1e6, got %g", temperature);
+    if (n_seq == 0) return 0;
+    if (!logits || (n_drafts > 0 && (!drafts || !u_accept)) || !u_sample || !workspace || !accepted || !tokens)
+        return fail(ETHOS_ENULL, "ethos_verify: null pointer");
+    const size_t need = ethos::verify_workspace_bytes(n_seq, n_drafts, vocab);
+    if (workspace_bytes < need) return fail(ETHOS_EWORKSPACE, "ethos_verify: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    if (!aligned16(workspace) || !aligned_to(logits, dtype) || !aligned_to(probs, probs_dtype))
+        return fail(ETHOS_EALIGN, "ethos_verify: logits, probs or workspace misaligned");
+    return hip_status(ethos::launch_verify(logits, drafts, probs, probs_dtype, counts, u_accept, u_sample, n_seq, n_drafts, vocab, temperature,
+                                           dtype, workspace, accepted, tokens, (hipStream_t)stream),
+                      "ethos_verify");
 }
 
 }  // extern "C"

@@ -826,3 +826,111 @@ def clip_grads(src: list, dst: list, sizes: list, codes: list, device: torch.dev
                               ws.data_ptr(), ws_bytes, total.data_ptr(), _stream())
     check(rc, "ethos_clip_grads")
     return total
+
+
+# ----------------------------------------------------------- operators of serving from a cache
+def _batch(pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor, rates: torch.Tensor, rope: int):
+    """Checks a batch over a cache: (table's row distance, its width, sequences)."""
+    _need_here(pool, "pool", FLOATS, 3)
+    _need_here(lens, "lens", (torch.int32,), 1)
+    _need_here(starts, "starts", (torch.int32,), 1)
+    _need_here(rates, "rates", (torch.float32,), 1)
+    if not isinstance(table, torch.Tensor) or table.get_device() != pool.get_device() or table.dtype != torch.int32 or table.dim() != 2:
+        raise RuntimeError(f"table must be an int32 tensor [sequences, pages] on {pool.device}")
+    n, width = table.shape
+    if width > 1 and table.stride(1) != 1 or n > 1 and table.stride(0) < width:
+        raise RuntimeError(f"table must have contiguous rows, got strides {table.stride()}")
+    if lens.numel() != n or starts.numel() != n + 1:
+        raise RuntimeError(f"{n} rows of table need as many lens and one more of starts, got {lens.numel()} and {starts.numel()}")
+    if rope % 2 or rates.numel() != rope // 2:
+        raise RuntimeError(f"rates must have {rope // 2} values for a rotary width of {rope}, got {rates.numel()}")
+    return (table.stride(0) if n > 1 else width), width, n
+
+
+def latent_append(rows: torch.Tensor, gain: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                  starts: torch.Tensor, rates: torch.Tensor, eps: float) -> None:
+    """Writes the cache's rows of the new tokens' rows [n, rank + rope] (evenly spaced) into the pool."""
+    rank = gain.numel()
+    _need_here(gain, "gain", FLOATS, 1)
+    ld, width, n_seq = _batch(pool, table, lens, starts, rates, pool.shape[-1] - rank)
+    if not isinstance(rows, torch.Tensor) or rows.get_device() != pool.get_device() or rows.dtype != pool.dtype or gain.dtype != pool.dtype:
+        raise RuntimeError(f"rows and gain must be {pool.dtype} on {pool.device}")
+    if rows.dim() != 2 or rows.shape[1] != pool.shape[2] or rows.stride(1) != 1:
+        raise RuntimeError(f"rows must be [n, {pool.shape[2]}] with contiguous rows, got {tuple(rows.shape)} of strides {rows.stride()}")
+    rc = load().ethos_latent_append(rows.data_ptr(), rows.stride(0) if rows.shape[0] > 1 else rows.shape[1], gain.data_ptr(), rates.data_ptr(),
+                                    table.data_ptr(), ld, width, lens.data_ptr(), starts.data_ptr(), n_seq, rows.shape[0], rank,
+                                    pool.shape[2] - rank, pool.shape[0], pool.shape[1], float(eps), dtype_code(pool.dtype), pool.data_ptr(),
+                                    _stream())
+    check(rc, "ethos_latent_append")
+
+
+def paged_attention(q: torch.Tensor, w: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor,
+                    rates: torch.Tensor, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of q [n, heads, nope + rope] over the cache -> [n, heads v_dim]."""
+    _need_here(q, "q", FLOATS, 3)
+    _need_here(w, "weight", FLOATS, 2)
+    n, H, qw = q.shape
+    rank = w.shape[1]
+    rope = pool.shape[-1] - rank
+    ld, width, n_seq = _batch(pool, table, lens, starts, rates, rope)
+    nope = qw - rope
+    v_dim = w.shape[0] // max(1, H) - nope
+    if q.dtype != pool.dtype or w.dtype != pool.dtype:
+        raise TypeError(f"q, weight and pool must have one dtype, got {q.dtype}, {w.dtype} and {pool.dtype}")
+    if H == 0 or w.shape[0] % H or nope < 0 or v_dim <= 0:
+        raise RuntimeError(f"paged_attention: inconsistent shapes q {tuple(q.shape)}, weight {tuple(w.shape)}, pool {tuple(pool.shape)}")
+    if out is None:
+        out = torch.empty((n, H * v_dim), dtype=q.dtype, device=q.device)
+    else:
+        _need_here(out, "out", (q.dtype,), 2)
+        if out.shape != (n, H * v_dim):
+            raise RuntimeError(f"out must be {(n, H * v_dim)}, got {tuple(out.shape)}")
+    lib, code = load(), dtype_code(q.dtype)
+    ws, ws_bytes = _scratch("ethos_paged_attention_workspace_bytes", q.device, n, n_seq, H, rank, rope, nope, v_dim, code)
+    rc = lib.ethos_paged_attention(q.data_ptr(), w.data_ptr(), pool.data_ptr(), table.data_ptr(), ld, width, lens.data_ptr(), starts.data_ptr(),
+                                   rates.data_ptr(), n, n_seq, H, rank, rope, nope, v_dim, pool.shape[0], pool.shape[1], code, float(scale),
+                                   ws.data_ptr(), ws_bytes, out.data_ptr(), _stream())
+    check(rc, "ethos_paged_attention")
+    return out
+
+
+def copy_pages(pool: torch.Tensor, src: list, dst: list) -> None:
+    """Copies pages src[i] to dst[i] in every block of pool [blocks, pages, ...]."""
+    a, b = array.array("i", src), array.array("i", dst)
+    size = pool.element_size()
+    pages, page_bytes = pool.shape[1], pool[0, 0].numel() * size if pool.numel() else 0
+    if page_bytes == 0 or not src:
+        return
+    rc = load().ethos_copy_pages(pool.data_ptr(), pool.shape[0], pages * page_bytes, pages, page_bytes, a.buffer_info()[0], b.buffer_info()[0],
+                                 len(a), _stream())
+    check(rc, "ethos_copy_pages")
+
+
+def verify(logits: torch.Tensor, drafts: torch.Tensor, probs: torch.Tensor | None, counts: torch.Tensor | None, u_accept: torch.Tensor,
+           u_sample: torch.Tensor, temperature: float):
+    """(accepted int32 [b], tokens int64 [b]) of logits [b, m + 1, V]."""
+    _need_here(logits, "logits", FLOATS, 3)
+    _need_here(drafts, "drafts", (torch.int64,), 2)
+    _need_here(u_accept, "u_accept", (torch.float32,), 2)
+    _need_here(u_sample, "u_sample", (torch.float32,), 1)
+    b, rows, V = logits.shape
+    m = rows - 1
+    if probs is not None:
+        _need_here(probs, "draft_probs", FLOATS, 3)
+    if counts is not None:
+        _need_here(counts, "counts", (torch.int32,), 1)
+    if (rows == 0 or drafts.shape != (b, m) or u_accept.shape != (b, m) or u_sample.shape != (b,)
+            or probs is not None and probs.shape != (b, m, V) or counts is not None and counts.shape != (b,)):
+        raise RuntimeError(f"verify_drafts: inconsistent shapes logits {tuple(logits.shape)}, drafts {tuple(drafts.shape)}, draft_probs "
+                           f"{None if probs is None else tuple(probs.shape)}, counts {None if counts is None else tuple(counts.shape)}, "
+                           f"u_accept {tuple(u_accept.shape)}, u_sample {tuple(u_sample.shape)}")
+    accepted = torch.empty((b,), dtype=torch.int32, device=logits.device)
+    tokens = torch.empty((b,), dtype=torch.int64, device=logits.device)
+    lib = load()
+    ws, ws_bytes = _scratch("ethos_verify_workspace_bytes", logits.device, b, m, V)
+    rc = lib.ethos_verify(logits.data_ptr(), drafts.data_ptr(), probs.data_ptr() if probs is not None else None,
+                          dtype_code(probs.dtype) if probs is not None else 0, counts.data_ptr() if counts is not None else None,
+                          u_accept.data_ptr(), u_sample.data_ptr(), b, m, V, float(temperature), dtype_code(logits.dtype), ws.data_ptr(),
+                          ws_bytes, accepted.data_ptr(), tokens.data_ptr(), _stream())
+    check(rc, "ethos_verify")
+    return accepted, tokens

@@ -1,0 +1,133 @@
+"""Operators of serving the language model from a cache, as HIP kernels (include/ethos_hip.h):
+
+  latent_append    the new tokens' rows of a cache of latents: normalised latent, rotated key
+  paged_attention  latent attention of the new tokens over the cache
+  copy_pages       pages of the cache copied, in every block's part at once
+  verify_drafts    drafted tokens accepted or not by the model's probabilities, the token after them
+
+The reference has no cache and decodes nothing; its attention forms every token's keys and values anew
+(model.py:104-160).  Inputs are HIP tensors on the current device, bf16 or float32; there is no CPU path.
+All work goes to the current stream.  Results are the same on every run.  The operators have no gradients:
+tensors that ask for one, forward-mode derivatives and torch.jit.trace are refused."""
+from __future__ import annotations
+
+import operator
+
+import torch
+
+from . import hip, training
+
+__all__ = ["copy_pages", "latent_append", "paged_attention", "verify_drafts"]
+
+
+def _check(what: str, *ts) -> None:
+    """Refuses what the kernels would hide from autograd, and other devices than the current one."""
+    if training._is_followed():
+        training._refuse_followed(what, *ts)
+    grad = torch.is_grad_enabled()
+    for t in ts:
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == hip._current_device()):
+            training._device_check(f"{what}: an input", t)
+        if grad and t.requires_grad:
+            raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+
+
+def _written(t: torch.Tensor) -> None:
+    """t was written by address."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
+def latent_append(rows: torch.Tensor, gain: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                  starts: torch.Tensor, rates: torch.Tensor, eps: float = 1e-6) -> None:
+    """Writes the new tokens of a batch into a cache of latents.
+
+    rows [n, rank + rope]: each token's latent and rotary key as they leave the projection (rows evenly spaced, for
+    example a part of a wider one); gain [rank]: the latent's RMSNorm; pool [pages, page, rank + rope], contiguous, the
+    page a power of two.  Sequence i has the pages table[i] (int32 [sequences, width]) and lens[i] tokens (int32), the new
+    ones included, which are rows starts[i] .. starts[i + 1] - 1 (int32 [sequences + 1], ascending).  Their place in the cache
+    gets the normalised latent (gain x / sqrt(mean(x^2) + eps)) and the key rotated by position times rates
+    (float32 [rope / 2], Rotary.rates), computed in float32 and rounded once.  Rows of no sequence, positions
+    without a page and pages outside the pool are left out.  The sequences' new tokens may not share places."""
+    _check("latent_append", rows, gain, pool, table, lens, starts, rates)
+    if rows.dim() != 2 or gain.dim() != 1 or pool.dim() != 3:
+        raise RuntimeError(f"latent_append: rows, gain and pool must have 2, 1 and 3 dims, got {tuple(rows.shape)}, {tuple(gain.shape)} and "
+                           f"{tuple(pool.shape)}")
+    if rows.shape[1] != pool.shape[2] or gain.numel() > rows.shape[1]:
+        raise RuntimeError(f"latent_append: inconsistent shapes {tuple(rows.shape)}, {tuple(gain.shape)} and {tuple(pool.shape)}")
+    if rows.dtype not in hip.FLOATS or rows.dtype != pool.dtype or gain.dtype != pool.dtype:
+        raise TypeError(f"rows, gain and pool must all be bfloat16 or all float32, got {rows.dtype}, {gain.dtype} and {pool.dtype}")
+    hip.latent_append(training._rows(rows), training._dense(gain), pool, table, lens, starts, rates, eps)
+    _written(pool)
+
+
+def paged_attention(q: torch.Tensor, weight: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                    starts: torch.Tensor, rates: torch.Tensor, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Latent attention of a batch's new tokens over the cache that latent_append filled: [n, heads v_dim].
+
+    q [n, heads, nope + rope], the rotary part not yet rotated; weight [heads (nope + v_dim), rank], kv_b_proj's;
+    pool, table, lens, starts and rates as latent_append takes them.  A token sees its sequence's positions up to its own:
+    softmax(scale q k) v over them, with k = [weight's nope rows of the head times the latent | the cached key] and v its
+    v_dim rows times the latent.  One token a sequence, a few or thousands: any mixture.  Rows of no sequence are left as
+    they are (`out`, or uninitialised); a token that sees nothing has zeros; one that sees a position without a page,
+    or a latent that is not finite, NaN.  In bf16 the products with the weight and the exponentials are rounded to
+    bf16, scores and sums are float32.  `out`: a contiguous tensor for the result, apart from the inputs."""
+    _check("paged_attention", q, weight, pool, table, lens, starts, rates, *(() if out is None else (out,)))
+    if q.dim() != 3 or weight.dim() != 2 or pool.dim() != 3:
+        raise RuntimeError(f"paged_attention: q, weight and pool must have 3, 2 and 3 dims, got {tuple(q.shape)}, {tuple(weight.shape)} and "
+                           f"{tuple(pool.shape)}")
+    o = hip.paged_attention(training._dense(q), training._dense(weight), pool, table, lens, starts, rates, scale, out)
+    if out is not None:
+        _written(out)
+    return o
+
+
+def _page_list(name: str, v, n_pages: int) -> list:
+    if isinstance(v, torch.Tensor):
+        if v.is_cuda:
+            raise TypeError(f"copy_pages: {name} must be on the host (a list, or a CPU tensor)")
+        v = v.tolist()
+    v = [operator.index(x) for x in v]
+    if v and not (0 <= min(v) and max(v) < n_pages):
+        raise IndexError(f"copy_pages: {name} holds pages outside the pool's {n_pages}")
+    return v
+
+
+def copy_pages(pool: torch.Tensor, src, dst) -> None:
+    """Copies page src[i] to page dst[i], for every i, in all blocks of pool [blocks, pages, ...] (contiguous, any dtype of
+    two or four bytes).  src and dst: sequences of whole numbers on the host, read during the call; no page may be written
+    twice or both read and written."""
+    _check("copy_pages", pool)
+    if pool.dim() < 3 or not pool.is_contiguous() or pool.element_size() not in (2, 4):
+        raise RuntimeError(f"copy_pages: pool must be contiguous [blocks, pages, ...] of 2 or 4 bytes a value, got {tuple(pool.shape)} "
+                           f"{pool.dtype}")
+    src, dst = _page_list("src", src, pool.shape[1]), _page_list("dst", dst, pool.shape[1])
+    if len(src) != len(dst):
+        raise ValueError(f"copy_pages: {len(src)} pages to copy but {len(dst)} places")
+    to = set(dst)
+    if len(to) != len(dst) or not to.isdisjoint(src):
+        raise ValueError("copy_pages: a page is written twice, or both read and written")
+    hip.copy_pages(pool, src, dst)
+    _written(pool)
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u_accept: torch.Tensor, u_sample: torch.Tensor,
+                  draft_probs: torch.Tensor | None = None, counts: torch.Tensor | None = None, temperature: float = 1.0):
+    """(accepted int32 [b], tokens int64 [b]): how many drafted tokens of each sequence stand, and the token after them.
+
+    logits [b, m + 1, vocab] (bf16 or float32): row j follows draft j - 1, row 0 the last token before the drafts;
+    drafts int64 [b, m], of which a sequence has counts[i] (int32 [b]; all m without it); draft_probs [b, m, vocab]
+    (bf16 or float32): what each was drawn from, None where it had probability 1; u_accept [b, m] and u_sample [b]: float32,
+    uniform in [0, 1).  With p_j = softmax(logits_j / temperature) (0: 1 at the first largest logit), draft j stands if all
+    before it do and u_accept q_j(x_j) < p_j(x_j).  The token is drawn from max(p_a - q_a, 0) behind the a-th (from p_a if all
+    stand, or that is 0 everywhere): the lowest index whose weights up to it exceed u_sample of their sum.  Tokens and drafts
+    together are then distributed as p's.  Without drafts (m = 0) it samples.  Words may be masked by logits of -inf.  A
+    token is -1 where its row has a NaN, no finite logit, or one that is +inf (with a temperature).  All in float64."""
+    _check("verify_drafts", *(t for t in (logits, drafts, u_accept, u_sample, draft_probs, counts) if t is not None))
+    for name, t, kinds in (("logits", logits, hip.FLOATS), ("draft_probs", draft_probs, hip.FLOATS), ("drafts", drafts, (torch.int64,)),
+                           ("counts", counts, (torch.int32,)), ("u_accept", u_accept, (torch.float32,)),
+                           ("u_sample", u_sample, (torch.float32,))):
+        if t is not None and t.dtype not in kinds:
+            raise TypeError(f"{name} must be {' or '.join(str(k) for k in kinds)}, got {t.dtype}")
+    dense = [None if t is None else t.contiguous() for t in (logits, drafts, draft_probs, counts, u_accept, u_sample)]
+    return hip.verify(*dense, temperature)

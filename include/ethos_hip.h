@@ -28,6 +28,9 @@
  *   ethos_balance, ethos_balance_grad      expert counts, the load-balance loss, its gradient
  *   ethos_clip_grads     the global norm of many gradients, and clipping
  *   ethos_capture_id     which capture records a stream
+ *   ethos_latent_append, ethos_copy_pages  a cache of latents in pages: its rows, copies of pages
+ *   ethos_paged_attention  attention of new tokens over that cache
+ *   ethos_verify         drafted tokens against the model's probabilities
  *
  * Conventions (every entry point):
  *   - All pointers are device pointers owned by the caller; nothing is allocated.
@@ -589,6 +592,80 @@ int ethos_balance_grad(const void* ids, int32_t ids_64, const int32_t* counts, c
 size_t ethos_clip_grads_workspace_bytes(const int64_t* sizes, int32_t n_tensors);
 int ethos_clip_grads(const void* const* in, void* const* out, const int64_t* sizes, const int32_t* dtypes, int32_t n_tensors,
                      int32_t inf_norm, double max_norm, void* workspace, size_t workspace_bytes, float* total, void* stream);
+
+/*
+ * A cache of latents in pages (the reference keeps none) and a batch of new tokens over it, as the next
+ * two calls take them; everything here is device data:
+ *   pool    [n_pages, page, rank + rope] dtype T: a token's row is its normalised latent, then its rotated key
+ *   table   [n_seq] rows of table_width page numbers, table_ld apart, int32: position p of sequence i is row
+ *           p % page of page table[i][p / page]
+ *   lens    [n_seq] int32: tokens of each sequence, the new ones included
+ *   starts  [n_seq + 1] int32, ascending: rows starts[i] .. starts[i + 1] - 1 of the batch's n_rows are sequence i's new
+ *           tokens, the last ones of its lens[i]; rows of no sequence (behind the last one) are left as they are
+ * What table, lens and starts hold cannot make a kernel leave the arrays: a page outside [0, n_pages), or a position
+ * without one, is neither written nor read.
+ * Limits: page a power of two up to 65536; rank <= 512 and rope <= 128, multiples of 8 (bf16) or 4; n_seq <= 2^20.
+ *
+ * ethos_latent_append writes the new tokens' rows (model.py:104-125 before the heads' projections): of the
+ * batch's rows [latent | key] (ld apart), y = RN_T(gain x / sqrt(mean(x^2) + eps)) of the latent and, of the key's halves
+ * [a, b], RN_T([a c - b s, b c + a s]) with c, s the cosine and sine of position times rates [rope / 2] (float32), the
+ * angles in float64 and the rest in float32.  Two sequences may share pages, but not the rows that the call writes.
+ * rows, gain and pool 16-byte aligned, ld a multiple of 8 (bf16) or 4.
+ */
+int ethos_latent_append(const void* rows, int64_t ld, const void* gain, const float* rates, const int32_t* table, int64_t table_ld,
+                        int32_t table_width, const int32_t* lens, const int32_t* starts, int32_t n_seq, int64_t n_rows, int32_t rank,
+                        int32_t rope, int64_t n_pages, int32_t page, float eps, int32_t dtype, void* pool, void* stream);
+
+/*
+ * Latent attention (model.py:104-160) of the batch's new tokens, each over its sequence's positions up to its own:
+ *   q    [n_rows, n_heads, nope + rope] dtype T, the rotary part not yet rotated
+ *   w    [n_heads (nope + v_dim), rank] dtype T (kv_b_proj's weight): head h's keys are its first nope rows times the
+ *        cached latent, then the cached key; its values the next v_dim rows times the latent
+ *   out  [n_rows, n_heads, v_dim] dtype T: softmax(scale q k) v
+ * The weight enters with the queries and behind the sums over latents: in bf16 these products, and the exponentials,
+ * are rounded to bf16; scores, maxima and sums are float32.  A token that sees no position has a row of zeros; one that sees
+ * a position without a page, or a row with a value that is not finite, has NaN, as have all tokens of a sequence whose
+ * length is negative or beyond its table, or whose rows are not in the batch.
+ *   workspace  >= ethos_paged_attention_workspace_bytes(...) bytes (scratch)
+ * q, w, pool, workspace and out 16-byte aligned; scale positive.
+ */
+size_t ethos_paged_attention_workspace_bytes(int64_t n_rows, int32_t n_seq, int32_t n_heads, int32_t rank, int32_t rope, int32_t nope,
+                                             int32_t v_dim, int32_t dtype);
+int ethos_paged_attention(const void* q, const void* w, const void* pool, const int32_t* table, int64_t table_ld, int32_t table_width,
+                          const int32_t* lens, const int32_t* starts, const float* rates, int64_t n_rows, int32_t n_seq, int32_t n_heads,
+                          int32_t rank, int32_t rope, int32_t nope, int32_t v_dim, int64_t n_pages, int32_t page, int32_t dtype, float scale,
+                          void* workspace, size_t workspace_bytes, void* out, void* stream);
+
+/*
+ * Copies pages: of each of n_blocks arrays of n_pages pages, block_bytes apart, page src[i] to page dst[i].
+ * src and dst: host arrays, read during the call only; every page inside the pool, no page twice in dst, none of dst
+ * in src.  pool, page_bytes and block_bytes even; fastest as multiples of 16.
+ */
+int ethos_copy_pages(void* pool, int64_t n_blocks, int64_t block_bytes, int64_t n_pages, int64_t page_bytes, const int32_t* src,
+                     const int32_t* dst, int32_t n_pairs, void* stream);
+
+/*
+ * Drafted tokens against the model's probabilities (nothing in the reference decodes):
+ *   logits    [n_seq, n_drafts + 1, vocab] dtype T: row j follows draft j - 1 (row 0 the last token before them)
+ *   drafts    [n_seq, n_drafts] int64
+ *   probs     [n_seq, n_drafts, vocab] of probs_dtype: what each draft was drawn from; NULL: each had probability 1
+ *   counts    [n_seq] int32: how many of them a sequence has (NULL: n_drafts of them)
+ *   u_accept  [n_seq, n_drafts], u_sample [n_seq] float32, uniform in [0, 1)
+ * With p_j = softmax(logits_j / temperature) (temperature 0: 1 at the largest logit, the first of equal ones), draft j
+ * is accepted if all before it are and u_accept probs_j[x_j] < p_j[x_j] (a draft outside the vocabulary is not).
+ *   accepted  [n_seq] int32: a, the number of accepted drafts
+ *   tokens    [n_seq] int64: the token behind them, the lowest index whose sum of weights up to it exceeds
+ *             u_sample times their sum; the weights are p_a where all were accepted, else max(p_a - probs_a, 0)
+ *             (where that is 0 everywhere, p_a).  -1 where p_a is no distribution: a NaN, no finite logit, or
+ *             (not greedy) one that is +inf.
+ * Exponentials and sums are float64.
+ *   workspace  >= ethos_verify_workspace_bytes(...) bytes, 16-byte aligned (scratch)
+ * Limits: n_drafts <= 255, vocab <= 2^24; temperature 0, or from 1e-6 to 1e6.
+ */
+size_t ethos_verify_workspace_bytes(int64_t n_seq, int32_t n_drafts, int64_t vocab);
+int ethos_verify(const void* logits, const int64_t* drafts, const void* probs, int32_t probs_dtype, const int32_t* counts,
+                 const float* u_accept, const float* u_sample, int64_t n_seq, int32_t n_drafts, int64_t vocab, double temperature,
+                 int32_t dtype, void* workspace, size_t workspace_bytes, int32_t* accepted, int64_t* tokens, void* stream);
 
 #ifdef __cplusplus
 }
