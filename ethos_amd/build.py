@@ -35,8 +35,9 @@ HIPCC_FLAGS = [
 # Per-source extra flags: MFMA results go to VGPRs (the VGPR form of v_mfma).  In
 # generate.hip that leaves the AGPRs to the register-resident hidden activations; in
 # qproj.hip every accumulator is read by VALU code, which would otherwise copy it out of
-# the AGPRs first.
+# the AGPRs first, and so are paged.hip's weighted sums, rescaled in every step.
 EXTRA_FLAGS = {
+    "paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "generate.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "qproj.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }

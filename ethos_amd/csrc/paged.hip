@@ -24,6 +24,7 @@ namespace {
 constexpr int kKeys = 64;          // keys of a tile of work
 constexpr float kLog2E = 1.44269504f;
 constexpr float kLowest = -0x1p126f;  // a running maximum's start: finite, so that masked scores weigh nothing
+constexpr int32_t kLongest = 1 << 30;  // a sequence's length, at most
 
 // A tile of rows: `rows` of sequence seq from its row `row0` (token row0 / H, head row0 % H) on; the first new
 // token of the sequence is row tok0 of the batch, at position pos0.
@@ -75,7 +76,8 @@ Layout layout(int64_t n_rows, int n_seq, int H, int width, int tile_rows, int gr
 }
 
 // ------------------------------------------------------------------------- the plan
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int tid, int64_t& total) {  // inclusive, 1,024 threads
+template <int NT>
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int tid, int64_t& total) {  // inclusive, NT threads
     const int lane = tid & 63, wave = tid >> 6;
     for (int d = 1; d < 64; d <<= 1) {
         const int64_t o = __shfl_up(v, d, 64);
@@ -86,7 +88,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* lds, int tid, 
     __syncthreads();
     int64_t before = 0;
     total = 0;
-    for (int w = 0; w < 16; ++w) {
+    for (int w = 0; w < NT / 64; ++w) {
         if (w < wave) before += lds[w];
         total += lds[w];
     }
@@ -99,17 +101,18 @@ __device__ __forceinline__ int64_t new_tokens(const Batch& b, int i) {
     return first < 0 || last > b.n_rows || last < first ? 0 : last - first;
 }
 __device__ __forceinline__ bool fits(const Batch& b, int i) {
-    return b.lens[i] >= 0 && (int64_t)b.lens[i] <= (int64_t)b.width << b.page_log;
+    return b.lens[i] >= 0 && b.lens[i] <= kLongest && (int64_t)b.lens[i] <= (int64_t)b.width << b.page_log;
 }
 
-// One workgroup of 1,024 threads.
+// One workgroup of NT threads.
+template <int NT>
 __device__ void make_plan(const Batch& b, const Shape& s, int64_t max_items, Plan* plan, Item* items, int32_t* seq_item, int tid) {
-    __shared__ int64_t lds[16];
+    __shared__ int64_t lds[NT / 64];
     int64_t base = 0, total;
-    for (int at = 0; at < b.n_seq; at += 1024) {
+    for (int at = 0; at < b.n_seq; at += NT) {
         const int i = at + tid;
         const int64_t n = i < b.n_seq ? (new_tokens(b, i) * s.H + s.rows - 1) / s.rows : 0;
-        const int64_t end = base + block_scan(n, lds, tid, total);
+        const int64_t end = base + block_scan<NT>(n, lds, tid, total);
         // (starts that overlap could ask for more than there is room for: those sequences get none)
         const int64_t first = end - n;
         if (i < b.n_seq) seq_item[i] = end <= max_items ? (int32_t)first : -1;
@@ -130,7 +133,7 @@ __device__ void make_plan(const Batch& b, const Shape& s, int64_t max_items, Pla
     const int64_t n_items = base < max_items ? base : max_items;
     __syncthreads();
     int64_t tiles = 0;
-    for (int64_t at = 0; at < n_items; at += 1024) {
+    for (int64_t at = 0; at < n_items; at += NT) {
         const int64_t k = at + tid;
         int64_t n = 0;
         if (k < n_items) {
@@ -139,7 +142,7 @@ __device__ void make_plan(const Batch& b, const Shape& s, int64_t max_items, Pla
             const int64_t keys = (int64_t)it.pos0 + (it.row0 + it.rows - 1) / s.H + 1;
             n = fits(b, it.seq) && keys > 0 ? (keys + kKeys - 1) / kKeys : 0;
         }
-        const int64_t end = tiles + block_scan(n, lds, tid, total);
+        const int64_t end = tiles + block_scan<NT>(n, lds, tid, total);
         if (k < n_items) items[k].end = end;
         tiles += total;
     }
@@ -173,7 +176,7 @@ __global__ __launch_bounds__(1024) void any_prepare_kernel(const T* __restrict__
                                                            Batch b, Shape s, int64_t max_items, Plan* plan, Item* items, int32_t* seq_item,
                                                            int32_t* tok_seq, float* __restrict__ queries) {
     if (blockIdx.x == 0) {
-        make_plan(b, s, max_items, plan, items, seq_item, threadIdx.x);
+        make_plan<1024>(b, s, max_items, plan, items, seq_item, threadIdx.x);
         return;
     }
     const int64_t t = blockIdx.x - 1;
@@ -370,16 +373,504 @@ int launch_any(const T* q, const T* w, const T* pool, const Batch& b, const floa
     return (int)hipGetLastError();
 }
 
+// ------------------------------------------------------------------------- bf16, rank 256 and rope 64
+// Tiles of rows are multiples of 32, the columns of S^T = K Q^T: a lane holds scores of one row, so that its
+// maximum, sum and rescaling stay in the lane (one exchange between the wave's halves), and the exponentials
+// lie as the B operand of O^T = C^T P^T takes them.  C is the latent part of the same rows of K, read from LDS once
+// more with the transposing loads, keys in the order in which the scores lie.
+//
+// A tile of 64 cached rows is 40 KB of LDS in five planes of 64 columns: a copy of 1 KB is then 8 rows of a plane, and a
+// lane's rows are the same ones in every plane.  In a plane's row of 128 bytes piece c lies at c ^ swizzle(row): 16
+// rows' reads of one piece, and the transposing reads' 4 rows by 4 pieces, touch every bank once.  Rows go from
+// memory straight into LDS at 64-bit addresses, page by page; rows behind the last key come from a row of zeros, rows without a page from
+// one of NaN, so that the loop has no bounds to check.  Page numbers come the same way, two tiles ahead of their rows.
+constexpr int kRank = 256, kRope = 64, kWidth = kRank + kRope;
+constexpr int kPlane = kKeys * 128, kStage = kWidth / 64 * kPlane;
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef const __attribute__((address_space(3))) bf16x8_t* lds_frag_ptr;
+typedef __attribute__((address_space(3))) s16x4_t* lds_tr_ptr;
+typedef __attribute__((address_space(3))) u32x4_t* lds_u4_ptr;
+typedef __attribute__((address_space(3))) float* lds_f_ptr;
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+union Frag {
+    u32x4_t u;
+    uint32_t w[4];
+    bf16x8_t f;
+    s16x4_t h[2];
+};
+
+__device__ __forceinline__ int swizzle(int row) { return ((row >> 1) & 1) << 2 | ((row >> 2) & 3); }
+
+// 16 or 4 bytes a lane from any address into LDS at lds + 16 or 4 times the lane (lds: wave-uniform).  The caller waits (vmcnt).
+__device__ __forceinline__ void copy16(const void* p, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
+}
+__device__ __forceinline__ void copy4(const void* p, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p) : "memory");
+}
+// This wave's copies but the last N have landed and its LDS accesses are done, and so with every wave.
+template <int N>
+__device__ __forceinline__ void copies_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Block 0: the plan and the two special rows.  The others: 32 tokens of a head; [c][token] = W_k,h^T q^T, the weight
+// (k as the row) through LDS in the layout of the loss's R tiles.
+__global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ w,
+                                                      const float* __restrict__ rates, Batch b, Shape s, int64_t max_items, Plan* plan,
+                                                      Item* items, int32_t* seq_item, int32_t* tok_seq, uint16_t* __restrict__ specials,
+                                                      uint16_t* __restrict__ queries) {
+    __shared__ __align__(16) uint16_t ws[64 * kRank];
+    __shared__ int64_t pos[32];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (blockIdx.x == 0) {
+        for (int e = tid; e < 2 * kWidth; e += 256) specials[e] = e < kWidth ? 0 : 0x7fc0;
+        make_plan<256>(b, s, max_items, plan, items, seq_item, tid);
+        return;
+    }
+    const int h = (blockIdx.x - 1) % s.H, qw = s.nope + kRope;
+    const int64_t t0 = (int64_t)((blockIdx.x - 1) / s.H) * 32;
+    if (tid < 32) {
+        const int64_t t = t0 + tid;
+        const int i = t < b.n_rows ? batch_seq(b, t) : -1;
+        if (h == 0 && t < b.n_rows) tok_seq[t] = i;
+        pos[tid] = i >= 0 ? (int64_t)b.lens[i] - b.starts[i + 1] + t : 0;
+    }
+    const int64_t my_t = t0 + (lane & 31) < b.n_rows ? t0 + (lane & 31) : b.n_rows - 1;
+    const uint16_t* qp = q + (my_t * s.H + h) * qw;
+    f32x16_t acc[2] = {f32x16_zero(), f32x16_zero()};
+    for (int j0 = 0; j0 < s.nope; j0 += 64) {
+        const int rows = s.nope - j0 < 64 ? s.nope - j0 : 64;
+        const uint16_t* wh = w + ((int64_t)h * (s.nope + s.v_dim) + j0) * kRank;
+        if (j0 > 0) __syncthreads();
+        for (int e = tid; e < rows * 32; e += 256) {
+            const int r = e >> 5, c = e & 31;
+            *reinterpret_cast<u32x4_t*>(ws + r * kRank + ((c ^ ((r & 3) << 2)) * 8)) =
+                *reinterpret_cast<const u32x4_t*>(wh + (int64_t)r * kRank + c * 8);
+        }
+        __syncthreads();
+        const uint32_t lds = lds_addr(ws);
+        const int k = 8 * half + ((lane & 15) >> 2);
+        for (int st = 0; st < rows / 16; ++st) {
+            Frag x;
+            x.u = *reinterpret_cast<const u32x4_t*>(qp + j0 + 16 * st + 8 * half);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int c = wave * 8 + i * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+                const uint32_t at = lds + (16 * st + k) * (kRank * 2) + ((c ^ ((k & 3) << 2)) << 4) + (lane & 1) * 8;
+                Frag a;
+                a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)at);
+                a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(at + 4 * kRank * 2));
+                acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f, x.f, acc[i], 0, 0, 0);
+            }
+        }
+    }
+    if (s.nope == 0) __syncthreads();
+    if (t0 + (lane & 31) < b.n_rows) {
+        uint16_t* to = queries + (my_t * s.H + h) * kWidth + wave * 64 + 4 * half;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<uint2*>(to + 32 * i + 2 * e) =
+                    make_uint2(pack_bf16x2(acc[i][e], acc[i][e + 1]), pack_bf16x2(acc[i][e + 2], acc[i][e + 3]));
+    }
+    for (int e = tid; e < 32 * (kRope / 2); e += 256) {
+        const int64_t t = t0 + (e >> 5);
+        const int p = e & 31;
+        if (t >= b.n_rows) break;
+        float c, sn;
+        rotary_angle(pos[e >> 5], rates[p], c, sn);
+        const uint16_t* r = q + (t * s.H + h) * qw + s.nope;
+        const float u = bf16_bits_to_f32(r[p]), v = bf16_bits_to_f32(r[32 + p]);
+        uint16_t* to = queries + (t * s.H + h) * kWidth + kRank;
+        to[p] = f32_to_bf16_bits(u * c - v * sn);
+        to[32 + p] = f32_to_bf16_bits(v * c + u * sn);
+    }
+}
+
+// WR KW waves: WR share a tile of 32 WR rows, 32 each, KW the 64 keys of a step.  S stages of LDS.
+template <int WR, int KW, int S>
+__global__ __launch_bounds__(WR * KW * 64) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
+                                                              const Item* __restrict__ items, const uint16_t* __restrict__ queries,
+                                                              const uint16_t* __restrict__ specials, float* __restrict__ sums,
+                                                              float2* __restrict__ stats) {
+    constexpr int W = WR * KW, KB = 2 / KW, NB = 8 / W, NC = NB * (kWidth / 64), RT = 32 * WR;
+    __shared__ __align__(16) unsigned char ring[S * kStage];
+    __shared__ __align__(16) int32_t numbers[W][4][64];
+    __shared__ uint32_t wild[2];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave / KW, wk = wave % KW;
+    const uint32_t lds = lds_addr(ring), list = lds_addr(&numbers[0][0][0]) + wave * 1024;
+    const int64_t quota = plan->quota, last = plan->tiles;
+    int64_t t = blockIdx.x * quota;
+    const int64_t stop = t + quota < last ? t + quota : last;
+    if (t >= stop) return;
+
+    // LDS places of the fragments: K's four steps of a plane, and C's two rows by two blocks of 32 columns
+    uint32_t k_at[4], c_at[2][2];
+    {
+        const int key = 32 * (KW == 2 ? wk : 0) + (lane & 31);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k_at[i] = key * 128 + (((2 * i + half) ^ swizzle(key)) << 4);
+        const int row = 32 * (KW == 2 ? wk : 0) + 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                const int r = row + 8 * i, c = 4 * d + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+                c_at[i][d] = r * 128 + ((c ^ swizzle(r)) << 4) + (lane & 1) * 8;
+            }
+    }
+
+    int item = find_item(items, plan->n_items, t, lane);
+    for (; t < stop; ++item) {
+        const Item it = items[item];
+        const int64_t begin = item > 0 ? items[item - 1].end : 0;
+        const int64_t to = it.end < stop ? it.end : stop;
+        if (to <= t) continue;
+        const int k_begin = (int)(t - begin), k_end = (int)(to - begin);
+        const int row_last = it.rows - 1;
+        const int end = it.pos0 + (it.row0 + row_last) / s.H + 1;  // keys that some row sees
+        const int first_pos = it.pos0 + it.row0 / s.H;
+        const int my = wr * 32 + (lane & 31), my_row = my < row_last ? my : row_last;
+        const int my_pos = it.pos0 + (it.row0 + my_row) / s.H;
+        const int wave_row = wr * 32 < row_last ? wr * 32 : row_last;
+        const int wave_pos = it.pos0 + (it.row0 + wave_row) / s.H;  // its first row's
+        const int32_t* table = b.table + it.seq * b.table_ld;
+
+        auto copy_numbers = [&](int k) {
+            int at = (k * kKeys + lane) >> b.page_log;
+            at = at < b.width ? at : b.width - 1;
+            copy4(table + at, __builtin_amdgcn_readfirstlane(list + (k & 3) * 256));
+        };
+        auto copy_rows = [&](int k, int stage) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const int blk = wave * NB + i, row = blk * 8 + (lane >> 3), p = k * kKeys + row;
+                const int32_t page = numbers[wave][k & 3][row];
+                const bool ok = page >= 0 && page < b.n_pages;
+                const int64_t at = ((int64_t)page << b.page_log) + (p & ((1 << b.page_log) - 1));
+                const uint16_t* from = p >= end ? specials : ok ? pool + at * kWidth : specials + kWidth;
+                from += ((lane & 7) ^ swizzle(row)) * 8;
+#pragma unroll
+                for (int pl = 0; pl < kWidth / 64; ++pl)
+                    copy16(from + pl * 64, __builtin_amdgcn_readfirstlane(lds + stage * kStage + pl * kPlane + blk * 1024));
+            }
+        };
+
+#pragma unroll
+        for (int i = 0; i <= S; ++i) copy_numbers(k_begin + i);
+        Frag fq[kWidth / 16];
+        {
+            const uint16_t* qp = queries + ((int64_t)it.tok0 * s.H + it.row0 + my_row) * kWidth + 8 * half;
+#pragma unroll
+            for (int i = 0; i < kWidth / 16; ++i) fq[i].u = *reinterpret_cast<const u32x4_t*>(qp + 16 * i);
+            // (here, not in the loop, is where they are waited for)
+#pragma unroll
+            for (int i = 0; i < kWidth / 16; ++i) asm volatile("" : "+v"(fq[i].u));
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i)
+            if (k_begin + i < k_end) copy_rows(k_begin + i, i);
+
+        f32x16_t o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = f32x16_zero();
+        float shift = kLowest, l = 0.0f;  // the running maximum of the scores times scale2, and the sum
+        int stage = 0;
+        for (int k = k_begin; k < k_end; ++k) {
+            if (S == 3 && k + 1 < k_end) copies_barrier<(S - 2) * NC>();
+            else copies_barrier<0>();
+            if (k + S - 1 < k_end) {
+                copy_numbers(k + S + 1);
+                copy_rows(k + S - 1, stage == 0 ? S - 1 : stage - 1);
+            }
+            const uint32_t at = lds + stage * kStage;
+            const int key0 = k * kKeys;
+            stage = stage == S - 1 ? 0 : stage + 1;
+            // rows that some of the tile's rows do not see may hold anything: those whose latents are not finite
+            uint64_t odd = 0;
+            if (first_pos < end - 1 && key0 + kKeys - 1 > first_pos) {
+                if (tid < 2) wild[tid] = 0;
+                lds_barrier();
+                for (int e = tid; e < kKeys * 32; e += W * 64) {
+                    const int r = e & 63, c = e >> 6;  // pieces of a row in any order
+                    const u32x4_t v = *(lds_u4_ptr)(size_t)(at + (c >> 3) * kPlane + r * 128 + (c & 7) * 16);
+                    bool bad = false;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+                    if (bad) atomicOr(&wild[r >> 5], 1u << (r & 31));
+                }
+                lds_barrier();
+                odd = (uint64_t)__builtin_amdgcn_readfirstlane(wild[1]) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane(wild[0]);
+            }
+            f32x16_t x[KB];
+#pragma unroll
+            for (int i = 0; i < KB; ++i) x[i] = f32x16_zero();
+#pragma unroll
+            for (int st = 0; st < kWidth / 16; ++st)
+#pragma unroll
+                for (int i = 0; i < KB; ++i) {
+                    const bf16x8_t a = *(lds_frag_ptr)(size_t)(at + k_at[st & 3] + (st >> 2) * kPlane + i * 32 * 128);
+                    x[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, fq[st].f, x[i], 0, 0, 0);
+                }
+            const int my_key0 = key0 + 32 * (KW == 2 ? wk : 0);
+            if (my_key0 + 32 * KB - 1 > wave_pos) {
+#pragma unroll
+                for (int i = 0; i < KB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        x[i][e] = my_key0 + 32 * i + mfma32_row(e, lane) > my_pos ? -INFINITY : x[i][e];
+            }
+            if (odd != 0) {
+                // a row that sees one of them has no result; for the others they are zeros
+#pragma unroll
+                for (int i = 0; i < KB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = 32 * (KW == 2 ? wk : 0) + 32 * i + mfma32_row(e, lane);
+                        if ((odd >> key & 1) && key0 + key <= my_pos) l = NAN;
+                    }
+                lds_barrier();
+                for (int e = tid; e < kKeys * 32; e += W * 64) {
+                    const int r = e & 63, c = e >> 6;
+                    if (odd >> r & 1) *(lds_u4_ptr)(size_t)(at + (c >> 3) * kPlane + r * 128 + (c & 7) * 16) = u32x4_t{0, 0, 0, 0};
+                }
+                lds_barrier();
+            }
+            float top = x[0][0];
+#pragma unroll
+            for (int i = 0; i < KB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[i][e]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float before = shift;
+            shift = fmaxf(shift, top * s.scale2);
+            const float r = __builtin_amdgcn_exp2f(before - shift);
+            l *= r;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] *= r;
+            Frag p[2 * KB];
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], s.scale2, -shift));
+                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e + 1], s.scale2, -shift));
+                    sum += e0 + e1;
+                    p[2 * i + e / 8].w[e % 8 / 2] = pack_bf16x2(e0, e1);
+                }
+            l += sum;
+#pragma unroll
+            for (int i = 0; i < 2 * KB; ++i)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    const uint32_t c = at + (d >> 1) * kPlane + i * 16 * 128;
+                    Frag a;
+                    a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(c + c_at[0][d & 1]));
+                    a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(c + c_at[1][d & 1]));
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f, p[i].f, o[d], 0, 0, 0);
+                }
+        }
+        l += __shfl_xor(l, 32, 64);
+        lds_barrier();
+        if constexpr (KW == 2) {
+            // the second wave's sums join the first's through LDS
+            static_assert(WR * 33 * 1024 <= S * kStage, "both waves' sums fit the ring");
+            const uint32_t mine = lds + wr * 33 * 1024 + lane * 4;
+            if (wk == 1) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) *(lds_f_ptr)(size_t)(mine + (i * 16 + e) * 256) = o[i][e];
+                *(lds_f_ptr)(size_t)(mine + 128 * 256) = shift;
+                *(lds_f_ptr)(size_t)(mine + 129 * 256) = l;
+            }
+            lds_barrier();
+            if (wk == 0) {
+                const float other = *(lds_f_ptr)(size_t)(mine + 128 * 256), l2 = *(lds_f_ptr)(size_t)(mine + 129 * 256);
+                const float both = fmaxf(shift, other);
+                const float f = __builtin_amdgcn_exp2f(shift - both), g = __builtin_amdgcn_exp2f(other - both);
+                shift = both;
+                l = l * f + l2 * g;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        o[i][e] = o[i][e] * f + *(lds_f_ptr)(size_t)(mine + (i * 16 + e) * 256) * g;
+            }
+            lds_barrier();
+        }
+        if (wk == 0 && my < it.rows) {
+            const int64_t slot = ((int64_t)blockIdx.x + item) * RT + my;
+            float* y = sums + slot * kRank + 4 * half;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<f32x4_t*>(y + 32 * i + 2 * e) = f32x4_t{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+            if (half == 0) stats[slot] = make_float2(shift, l);
+        }
+        t = to;
+    }
+}
+
+// TOK tokens of a head: 256 / TOK threads a token join its parts, 16 columns a thread and 16 / TOK parts side by side,
+// then [v][token] = W_v,h o^T by 16 x 16 x 32 MFMAs, a wave for every 16 of v_dim.
+template <int TOK>
+__global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict__ w, Batch b, Shape s, const Plan* plan,
+                                                     const Item* __restrict__ items, const int32_t* __restrict__ seq_item,
+                                                     const int32_t* __restrict__ tok_seq, const float* __restrict__ sums,
+                                                     const float2* __restrict__ stats, uint16_t* __restrict__ out) {
+    constexpr int G = 16 / TOK;  // groups of 16 threads that share a token
+    __shared__ __align__(16) uint16_t os[TOK][kRank + 8];
+    __shared__ __align__(16) float part[G > 1 ? 16 : 1][kRank];
+    __shared__ float tops[16], ls[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = blockIdx.x % s.H;
+    const int64_t t0 = (int64_t)(blockIdx.x / s.H) * TOK;
+    const int grp = tid >> 4, tok = grp / G, sub = grp % G, col = (tid & 15) * 4;
+    const int64_t t = t0 + tok;
+    const int i = t < b.n_rows ? tok_seq[t] : -1;
+    Parts p = {0, 0, false};
+    int in = 0;
+    if (i >= 0) p = row_parts(b, s, plan, items, seq_item, i, (t - b.starts[i]) * s.H + h, in);
+    float top = kLowest;
+    for (int k = sub; k < p.n; k += G) top = fmaxf(top, stats[(p.slot + k) * s.rows + in].x);
+    float l = 0.0f, v[16] = {};
+#pragma unroll 2
+    for (int k = sub; k < p.n; k += G) {
+        const int64_t at = (p.slot + k) * s.rows + in;
+        const float2 ml = stats[at];
+        const float f = __builtin_amdgcn_exp2f(ml.x - top);
+        l += ml.y * f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(sums + at * kRank + c * 64 + col);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * c + e] += x[e] * f;
+        }
+    }
+    if constexpr (G > 1) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) *reinterpret_cast<f32x4_t*>(&part[grp][c * 64 + col]) = f32x4_t{v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]};
+        if ((tid & 15) == 0) tops[grp] = top, ls[grp] = l;
+        __syncthreads();
+        // thread by thread again: token tid / (256 / TOK), columns of 16 G threads
+        const int mine = tok * G;
+        float all = tops[mine], sum = 0.0f, f[G];
+#pragma unroll
+        for (int g = 1; g < G; ++g) all = fmaxf(all, tops[mine + g]);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            f[g] = __builtin_amdgcn_exp2f(tops[mine + g] - all);
+            sum += ls[mine + g] * f[g];
+        }
+        const float inv = p.bad ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int c = 0; c < TOK; ++c) {
+            const int at = c * 16 * G + (sub * 16 + (tid & 15));
+            float x = 0.0f;
+#pragma unroll
+            for (int g = 0; g < G; ++g) x += part[mine + g][at] * f[g];
+            os[tok][at] = f32_to_bf16_bits(x * inv);
+        }
+    } else {
+        const float inv = p.bad ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            *reinterpret_cast<uint2*>(&os[tok][c * 64 + col]) =
+                make_uint2(pack_bf16x2(v[4 * c] * inv, v[4 * c + 1] * inv), pack_bf16x2(v[4 * c + 2] * inv, v[4 * c + 3] * inv));
+    }
+    __syncthreads();
+    const int tc = (lane & 15) < TOK ? lane & 15 : TOK - 1;
+    const int64_t to = t0 + (lane & 15);
+    const bool live = (lane & 15) < TOK && to < b.n_rows && tok_seq[to] >= 0;
+    for (int vb = wave; vb < s.v_dim / 16; vb += 4) {
+        const uint16_t* wv = w + ((int64_t)h * (s.nope + s.v_dim) + s.nope + vb * 16 + (lane & 15)) * kRank + 8 * (lane >> 4);
+        f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int st = 0; st < kRank / 32; ++st) {
+            const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(wv + 32 * st);
+            const bf16x8_t x = *reinterpret_cast<const bf16x8_t*>(&os[tc][32 * st + 8 * (lane >> 4)]);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, x, acc, 0, 0, 0);
+        }
+        if (live)
+            *reinterpret_cast<uint2*>(out + (to * s.H + h) * s.v_dim + vb * 16 + 4 * (lane >> 4)) =
+                make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
+    }
+}
+
+bool is_fast(int rank, int rope, int nope, int v_dim, int dtype) {
+    return dtype == kBF16 && rank == kRank && rope == kRope && nope % 16 == 0 && v_dim % 16 == 0;
+}
+
+// Rows of a tile: as many as a sequence's new tokens have on the average, 32, 64 or 128.  A workgroup of 32 leaves room for a
+// second one on its CU.
+int fast_rows(int64_t n_rows, int n_seq, int H) {
+    const int64_t each = n_rows * H / n_seq;
+    return each <= 32 ? 32 : each <= 64 ? 64 : 128;
+}
+int fast_groups(int rows, int num_cus) { return rows == 32 ? 2 * num_cus : num_cus; }
+
+int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, const Batch& b, const float* rates, Shape s, unsigned char* ws,
+                uint16_t* out, int num_cus, hipStream_t stream) {
+    s.rows = fast_rows(b.n_rows, b.n_seq, s.H);
+    s.groups = fast_groups(s.rows, num_cus);
+    const Layout l = layout(b.n_rows, b.n_seq, s.H, kWidth, s.rows, s.groups, 2, kRank);
+    Plan* plan = (Plan*)(ws + l.plan);
+    Item* items = (Item*)(ws + l.items);
+    int32_t *seq_item = (int32_t*)(ws + l.seq_item), *tok_seq = (int32_t*)(ws + l.tok_seq);
+    uint16_t *specials = (uint16_t*)(ws + l.specials), *queries = (uint16_t*)(ws + l.queries);
+    float* sums = (float*)(ws + l.sums);
+    float2* stats = (float2*)(ws + l.stats);
+    const unsigned tiles = (unsigned)((b.n_rows + 31) / 32);
+    hipLaunchKernelGGL(prepare_kernel, dim3(tiles * s.H + 1), dim3(256), 0, stream, q, w, rates, b, s, l.max_items, plan, items, seq_item,
+                       tok_seq, specials, queries);
+    const dim3 grid((unsigned)s.groups);
+    if (s.rows == 32)
+        hipLaunchKernelGGL((attend_kernel<1, 2, 2>), grid, dim3(128), 0, stream, pool, b, s, plan, items, queries, specials, sums, stats);
+    else if (s.rows == 64)
+        hipLaunchKernelGGL((attend_kernel<2, 2, 3>), grid, dim3(256), 0, stream, pool, b, s, plan, items, queries, specials, sums, stats);
+    else
+        hipLaunchKernelGGL((attend_kernel<4, 1, 3>), grid, dim3(256), 0, stream, pool, b, s, plan, items, queries, specials, sums, stats);
+    // (few tokens have many parts each: more threads a token)
+    if (b.n_rows <= 8)
+        hipLaunchKernelGGL((finish_kernel<1>), dim3((unsigned)(b.n_rows * s.H)), dim3(256), 0, stream, w, b, s, plan, items, seq_item, tok_seq, sums,
+                           stats, out);
+    else if (b.n_rows <= 256)
+        hipLaunchKernelGGL((finish_kernel<4>), dim3((unsigned)((b.n_rows + 3) / 4 * s.H)), dim3(256), 0, stream, w, b, s, plan, items, seq_item,
+                           tok_seq, sums, stats, out);
+    else
+        hipLaunchKernelGGL((finish_kernel<16>), dim3((unsigned)((b.n_rows + 15) / 16 * s.H)), dim3(256), 0, stream, w, b, s, plan, items, seq_item,
+                           tok_seq, sums, stats, out);
+    return (int)hipGetLastError();
+}
+
 }  // namespace
 
 size_t paged_attention_workspace_bytes(int64_t n_rows, int n_seq, int H, int rank, int rope, int nope, int v_dim, int dtype,
                                        int num_cus) {
+    if (is_fast(rank, rope, nope, v_dim, dtype)) {
+        const int rows = fast_rows(n_rows, n_seq, H);
+        return layout(n_rows, n_seq, H, kWidth, rows, fast_groups(rows, num_cus), 2, kRank).bytes;
+    }
     return layout(n_rows, n_seq, H, rank + rope, kAnyRows, any_groups(num_cus), 4, rank).bytes;
 }
 
 int launch_paged_attention(const void* q, const void* w, const void* pool, const Batch& b, const float* rates, int H, int rank, int rope,
                            int nope, int v_dim, int dtype, float scale, void* ws, void* out, int num_cus, hipStream_t stream) {
     const Shape s = {H, rank, rope, nope, v_dim, 0, 0, scale * kLog2E};
+    if (is_fast(rank, rope, nope, v_dim, dtype))
+        return launch_fast((const uint16_t*)q, (const uint16_t*)w, (const uint16_t*)pool, b, rates, s, (unsigned char*)ws, (uint16_t*)out,
+                           num_cus, stream);
     if (dtype == kBF16)
         return launch_any((const uint16_t*)q, (const uint16_t*)w, (const uint16_t*)pool, b, rates, s, (unsigned char*)ws, (uint16_t*)out,
                           num_cus, stream);

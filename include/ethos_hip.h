@@ -625,7 +625,7 @@ int ethos_latent_append(const void* rows, int64_t ld, const void* gain, const fl
  * The weight enters with the queries and behind the sums over latents: in bf16 these products, and the exponentials,
  * are rounded to bf16; scores, maxima and sums are float32.  A token that sees no position has a row of zeros; one that sees
  * a position without a page, or a row with a value that is not finite, has NaN, as have all tokens of a sequence whose
- * length is negative or beyond its table, or whose rows are not in the batch.
+ * length is negative, over 2^30 or beyond its table, or whose rows are not in the batch.
  *   workspace  >= ethos_paged_attention_workspace_bytes(...) bytes (scratch)
  * q, w, pool, workspace and out 16-byte aligned; scale positive.
  */
