@@ -66,7 +66,7 @@ Layout layout(int64_t n_rows, int n_seq, int H, int width, int tile_rows, int gr
     l.items = take((size_t)l.max_items * sizeof(Item));
     l.seq_item = take((size_t)n_seq * 4);
     l.tok_seq = take((size_t)n_rows * 4);
-    l.specials = take((size_t)2 * width * 4);
+    l.specials = take((size_t)16 * width * 2);
     l.queries = take((size_t)n_rows * H * width * query_bytes);
     const size_t slots = (size_t)(l.max_items + groups);
     l.sums = take(slots * tile_rows * rank * 4);
@@ -104,52 +104,54 @@ __device__ __forceinline__ bool fits(const Batch& b, int i) {
     return b.lens[i] >= 0 && b.lens[i] <= kLongest && (int64_t)b.lens[i] <= (int64_t)b.width << b.page_log;
 }
 
-// One workgroup of NT threads.
+// One workgroup of NT threads: NT sequences at a time, then their items, NT at a time.
 template <int NT>
 __device__ void make_plan(const Batch& b, const Shape& s, int64_t max_items, Plan* plan, Item* items, int32_t* seq_item, int tid) {
     __shared__ int64_t lds[NT / 64];
-    int64_t base = 0, total;
+    __shared__ int32_t ends[NT], counts[NT], tok0[NT], lens[NT];
+    int64_t base = 0, tiles = 0, total;
     for (int at = 0; at < b.n_seq; at += NT) {
         const int i = at + tid;
-        const int64_t n = i < b.n_seq ? (new_tokens(b, i) * s.H + s.rows - 1) / s.rows : 0;
-        const int64_t end = base + block_scan<NT>(n, lds, tid, total);
+        const int64_t count = i < b.n_seq ? new_tokens(b, i) : 0, n = (count * s.H + s.rows - 1) / s.rows;
+        const int64_t end = block_scan<NT>(n, lds, tid, total);
         // (starts that overlap could ask for more than there is room for: those sequences get none)
-        const int64_t first = end - n;
-        if (i < b.n_seq) seq_item[i] = end <= max_items ? (int32_t)first : -1;
-        for (int64_t k = first; k < end && end <= max_items; ++k) {
-            Item it;
-            it.seq = i;
-            it.row0 = (int32_t)((k - first) * s.rows);
-            const int64_t left = new_tokens(b, i) * s.H - it.row0;
-            it.rows = (int32_t)(left < s.rows ? left : s.rows);
-            it.tok0 = b.starts[i];
-            it.pos0 = (int32_t)(b.lens[i] - new_tokens(b, i));
-            it.pad = 0;
-            it.end = 0;
-            items[k] = it;
+        if (i < b.n_seq) seq_item[i] = base + end <= max_items ? (int32_t)(base + end - n) : -1;
+        const int64_t here = total < max_items - base ? total : max_items - base;
+        ends[tid] = (int32_t)(end < here ? end : here);
+        counts[tid] = (int32_t)count;
+        if (i < b.n_seq) tok0[tid] = b.starts[i], lens[tid] = fits(b, i) ? b.lens[i] : -1;
+        __syncthreads();
+        for (int64_t k0 = 0; k0 < here; k0 += NT) {
+            const int k = (int)k0 + tid;
+            Item it = {};
+            int64_t work = 0;
+            if (k < here) {
+                int lo = 0;  // the first sequence whose items end behind k
+                for (int step = NT / 2; step > 0; step >>= 1)
+                    if (ends[lo + step - 1] <= k) lo += step;
+                it.seq = at + lo;
+                it.row0 = (k - (lo > 0 ? ends[lo - 1] : 0)) * s.rows;
+                const int left = counts[lo] * s.H - it.row0;
+                it.rows = left < s.rows ? left : s.rows;
+                it.tok0 = tok0[lo];
+                it.pos0 = lens[lo] - counts[lo];
+                // keys up to the last row's own
+                const int64_t keys = (int64_t)it.pos0 + (it.row0 + it.rows - 1) / s.H + 1;
+                work = lens[lo] >= 0 && keys > 0 ? (keys + kKeys - 1) / kKeys : 0;
+            }
+            it.end = tiles + block_scan<NT>(work, lds, tid, total);
+            if (k < here) items[base + k] = it;
+            tiles += total;
         }
-        base += total;
-    }
-    const int64_t n_items = base < max_items ? base : max_items;
-    __syncthreads();
-    int64_t tiles = 0;
-    for (int64_t at = 0; at < n_items; at += NT) {
-        const int64_t k = at + tid;
-        int64_t n = 0;
-        if (k < n_items) {
-            const Item it = items[k];
-            // keys up to the last row's own
-            const int64_t keys = (int64_t)it.pos0 + (it.row0 + it.rows - 1) / s.H + 1;
-            n = fits(b, it.seq) && keys > 0 ? (keys + kKeys - 1) / kKeys : 0;
-        }
-        const int64_t end = tiles + block_scan<NT>(n, lds, tid, total);
-        if (k < n_items) items[k].end = end;
-        tiles += total;
+        base += here;
+        __syncthreads();
     }
     if (tid == 0) {
+        // (few tiles a workgroup, two workgroups a CU: one on each, whose parts are then half as many to join)
+        const int64_t groups = s.rows <= 32 && tiles < 4 * (int64_t)s.groups ? (s.groups + 1) / 2 : s.groups;
         plan->tiles = tiles;
-        plan->quota = tiles > s.groups ? (tiles + s.groups - 1) / s.groups : 1;
-        plan->n_items = (int32_t)n_items;
+        plan->quota = tiles > groups ? (tiles + groups - 1) / groups : 1;
+        plan->n_items = (int32_t)base;
     }
 }
 
@@ -374,17 +376,18 @@ int launch_any(const T* q, const T* w, const T* pool, const Batch& b, const floa
 }
 
 // ------------------------------------------------------------------------- bf16, rank 256 and rope 64
-// Tiles of rows are multiples of 32, the columns of S^T = K Q^T: a lane holds scores of one row, so that its
-// maximum, sum and rescaling stay in the lane (one exchange between the wave's halves), and the exponentials
+// Tiles of rows are multiples of 16, the columns of S^T = K Q^T: a lane holds scores of one row, so that its
+// maximum, sum and rescaling stay in the lane (and the three others of the row), and the exponentials
 // lie as the B operand of O^T = C^T P^T takes them.  C is the latent part of the same rows of K, read from LDS once
 // more with the transposing loads, keys in the order in which the scores lie.
 //
 // A tile of 64 cached rows is 40 KB of LDS in five planes of 64 columns: a copy of 1 KB is then 8 rows of a plane, and a
 // lane's rows are the same ones in every plane.  In a plane's row of 128 bytes piece c lies at c ^ swizzle(row): 16
 // rows' reads of one piece, and the transposing reads' 4 rows by 4 pieces, touch every bank once.  Rows go from
-// memory straight into LDS at 64-bit addresses, page by page; rows behind the last key come from a row of zeros, rows without a page from
-// one of NaN, so that the loop has no bounds to check.  Page numbers come the same way, two tiles ahead of their rows.
+// memory straight into LDS, eight rows of a page (which has at least eight) and a plane at a time; rows behind the last key
+// come from rows of zeros, rows without a page from rows of NaN, so that the loop has no bounds to check.
 constexpr int kRank = 256, kRope = 64, kWidth = kRank + kRope;
+constexpr int kBlockLog = 3, kBlock = 1 << kBlockLog;  // rows of a copy
 constexpr int kPlane = kKeys * 128, kStage = kWidth / 64 * kPlane;
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -401,14 +404,15 @@ union Frag {
     s16x4_t h[2];
 };
 
-__device__ __forceinline__ int swizzle(int row) { return ((row >> 1) & 1) << 2 | ((row >> 2) & 3); }
+__device__ __forceinline__ int swizzle(int row) { return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1); }
 
-// 16 or 4 bytes a lane from any address into LDS at lds + 16 or 4 times the lane (lds: wave-uniform).  The caller waits (vmcnt).
+// 16 bytes a lane into LDS at lds + 16 times the lane (lds: wave-uniform), from an address or from base + off.
+// The caller waits (vmcnt).
 __device__ __forceinline__ void copy16(const void* p, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(p) : "memory");
 }
-__device__ __forceinline__ void copy4(const void* p, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(p) : "memory");
+__device__ __forceinline__ void copy16(const void* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 // This wave's copies but the last N have landed and its LDS accesses are done, and so with every wave.
 template <int N>
@@ -426,7 +430,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (blockIdx.x == 0) {
-        for (int e = tid; e < 2 * kWidth; e += 256) specials[e] = e < kWidth ? 0 : 0x7fc0;
+        for (int e = tid; e < 2 * kBlock * kWidth; e += 256) specials[e] = e < kBlock * kWidth ? 0 : 0x7fc0;
         make_plan<256>(b, s, max_items, plan, items, seq_item, tid);
         return;
     }
@@ -491,38 +495,31 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
     }
 }
 
-// WR KW waves: WR share a tile of 32 WR rows, 32 each, KW the 64 keys of a step.  S stages of LDS.
+// WR KW waves: WR share a tile of 16 WR rows, 16 each, KW the 64 keys of a step.  S stages of LDS.
 template <int WR, int KW, int S>
-__global__ __launch_bounds__(WR * KW * 64) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
-                                                              const Item* __restrict__ items, const uint16_t* __restrict__ queries,
-                                                              const uint16_t* __restrict__ specials, float* __restrict__ sums,
-                                                              float2* __restrict__ stats) {
-    constexpr int W = WR * KW, KB = 2 / KW, NB = 8 / W, NC = NB * (kWidth / 64), RT = 32 * WR;
+__global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
+                                                                 const Item* __restrict__ items, const uint16_t* __restrict__ queries,
+                                                                 const uint16_t* __restrict__ specials, float* __restrict__ sums,
+                                                                 float2* __restrict__ stats) {
+    constexpr int W = WR * KW, KB = 4 / KW, NB = 8 / W, NC = NB * (kWidth / 64), RT = 16 * WR;
     __shared__ __align__(16) unsigned char ring[S * kStage];
-    __shared__ __align__(16) int32_t numbers[W][4][64];
-    __shared__ uint32_t wild[2];
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave / KW, wk = wave % KW;
-    const uint32_t lds = lds_addr(ring), list = lds_addr(&numbers[0][0][0]) + wave * 1024;
+    const uint32_t lds = lds_addr(ring);
     const int64_t quota = plan->quota, last = plan->tiles;
     int64_t t = blockIdx.x * quota;
     const int64_t stop = t + quota < last ? t + quota : last;
     if (t >= stop) return;
 
-    // LDS places of the fragments: K's four steps of a plane, and C's two rows by two blocks of 32 columns
-    uint32_t k_at[4], c_at[2][2];
+    // LDS places of the fragments: K's two steps of a plane, and C's four blocks of 16 columns of one
+    uint32_t k_at[2], c_at[4];
+    const int wave_key = 16 * KB * wk;
     {
-        const int key = 32 * (KW == 2 ? wk : 0) + (lane & 31);
+        const int key = wave_key + (lane & 15), row = wave_key + 4 * g + ((lane & 15) >> 2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k_at[i] = key * 128 + (((2 * i + half) ^ swizzle(key)) << 4);
-        const int row = 32 * (KW == 2 ? wk : 0) + 4 * half + ((lane & 15) >> 2);
+        for (int i = 0; i < 2; ++i) k_at[i] = key * 128 + (((4 * i + g) ^ swizzle(key)) << 4);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                const int r = row + 8 * i, c = 4 * d + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-                c_at[i][d] = r * 128 + ((c ^ swizzle(r)) << 4) + (lane & 1) * 8;
-            }
+        for (int d = 0; d < 4; ++d) c_at[d] = row * 128 + (((2 * d + ((lane & 3) >> 1)) ^ swizzle(row)) << 4) + (lane & 1) * 8;
     }
 
     int item = find_item(items, plan->n_items, t, lane);
@@ -535,105 +532,114 @@ __global__ __launch_bounds__(WR * KW * 64) void attend_kernel(const uint16_t* __
         const int row_last = it.rows - 1;
         const int end = it.pos0 + (it.row0 + row_last) / s.H + 1;  // keys that some row sees
         const int first_pos = it.pos0 + it.row0 / s.H;
-        const int my = wr * 32 + (lane & 31), my_row = my < row_last ? my : row_last;
+        const int my = wr * 16 + (lane & 15), my_row = my < row_last ? my : row_last;
         const int my_pos = it.pos0 + (it.row0 + my_row) / s.H;
-        const int wave_row = wr * 32 < row_last ? wr * 32 : row_last;
+        const int wave_row = wr * 16 < row_last ? wr * 16 : row_last;
         const int wave_pos = it.pos0 + (it.row0 + wave_row) / s.H;  // its first row's
-        const int32_t* table = b.table + it.seq * b.table_ld;
+        // (as constant memory: loads by the scalar unit, which do not queue behind the copies)
+        const auto table = (const __attribute__((address_space(4))) int32_t*)(uintptr_t)(b.table + it.seq * b.table_ld);
 
-        auto copy_numbers = [&](int k) {
-            int at = (k * kKeys + lane) >> b.page_log;
-            at = at < b.width ? at : b.width - 1;
-            copy4(table + at, __builtin_amdgcn_readfirstlane(list + (k & 3) * 256));
+        // page numbers of the rows that this wave copies of a step, and the copies
+        int32_t pages[NB];
+        auto load_pages = [&](int k) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                const int at = (int)((uint32_t)(k * kKeys + (wave * NB + i) * kBlock) >> b.page_log);
+                pages[i] = table[at < b.width ? at : b.width - 1];
+            }
         };
         auto copy_rows = [&](int k, int stage) {
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
-                const int blk = wave * NB + i, row = blk * 8 + (lane >> 3), p = k * kKeys + row;
-                const int32_t page = numbers[wave][k & 3][row];
-                const bool ok = page >= 0 && page < b.n_pages;
-                const int64_t at = ((int64_t)page << b.page_log) + (p & ((1 << b.page_log) - 1));
-                const uint16_t* from = p >= end ? specials : ok ? pool + at * kWidth : specials + kWidth;
-                from += ((lane & 7) ^ swizzle(row)) * 8;
+                const int blk = wave * NB + i, p0 = k * kKeys + blk * kBlock;
+                const int32_t page = pages[i];
+                const uint16_t* from = page >= 0 && page < b.n_pages
+                                           ? pool + (((int64_t)page << b.page_log) + (p0 & ((1 << b.page_log) - 1))) * kWidth
+                                           : specials + kBlock * kWidth;
+                if (p0 >= end) from = specials;
+                const int row = lane >> 3;
+                const uint32_t off = row * (kWidth * 2) + (((lane & 7) ^ swizzle(blk * kBlock + row)) << 4);
+                const uint32_t to_lds = lds + stage * kStage + blk * 1024;
+                if (p0 < end && p0 + kBlock > end) {  // the sequence ends in this block
+                    const unsigned char* mine = (const unsigned char*)(p0 + row < end ? from : specials) + off;
 #pragma unroll
-                for (int pl = 0; pl < kWidth / 64; ++pl)
-                    copy16(from + pl * 64, __builtin_amdgcn_readfirstlane(lds + stage * kStage + pl * kPlane + blk * 1024));
+                    for (int pl = 0; pl < kWidth / 64; ++pl) copy16(mine + pl * 128, __builtin_amdgcn_readfirstlane(to_lds + pl * kPlane));
+                } else {
+#pragma unroll
+                    for (int pl = 0; pl < kWidth / 64; ++pl) copy16(from + pl * 64, off, __builtin_amdgcn_readfirstlane(to_lds + pl * kPlane));
+                }
             }
         };
 
-#pragma unroll
-        for (int i = 0; i <= S; ++i) copy_numbers(k_begin + i);
-        Frag fq[kWidth / 16];
+        load_pages(k_begin);
+        Frag fq[kWidth / 32];
         {
-            const uint16_t* qp = queries + ((int64_t)it.tok0 * s.H + it.row0 + my_row) * kWidth + 8 * half;
+            const uint16_t* qp = queries + ((int64_t)it.tok0 * s.H + it.row0 + my_row) * kWidth + 8 * g;
 #pragma unroll
-            for (int i = 0; i < kWidth / 16; ++i) fq[i].u = *reinterpret_cast<const u32x4_t*>(qp + 16 * i);
+            for (int i = 0; i < kWidth / 32; ++i) fq[i].u = *reinterpret_cast<const u32x4_t*>(qp + 32 * i);
             // (here, not in the loop, is where they are waited for)
 #pragma unroll
-            for (int i = 0; i < kWidth / 16; ++i) asm volatile("" : "+v"(fq[i].u));
+            for (int i = 0; i < kWidth / 32; ++i) asm volatile("" : "+v"(fq[i].u));
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
         for (int i = 0; i < S - 1; ++i)
-            if (k_begin + i < k_end) copy_rows(k_begin + i, i);
+            if (k_begin + i < k_end) {
+                copy_rows(k_begin + i, i);
+                load_pages(k_begin + i + 1);
+            }
 
-        f32x16_t o[8];
+        f32x4_t o[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = f32x16_zero();
-        float shift = kLowest, l = 0.0f;  // the running maximum of the scores times scale2, and the sum
+        for (int i = 0; i < 16; ++i) o[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        float shift = kLowest, l = 0.0f;  // the running maximum of the scores times scale2, and the lane's part of the sum
         int stage = 0;
         for (int k = k_begin; k < k_end; ++k) {
             if (S == 3 && k + 1 < k_end) copies_barrier<(S - 2) * NC>();
             else copies_barrier<0>();
             if (k + S - 1 < k_end) {
-                copy_numbers(k + S + 1);
                 copy_rows(k + S - 1, stage == 0 ? S - 1 : stage - 1);
+                load_pages(k + S);
             }
             const uint32_t at = lds + stage * kStage;
-            const int key0 = k * kKeys;
+            const int key0 = k * kKeys + wave_key;  // the wave's first key
             stage = stage == S - 1 ? 0 : stage + 1;
             // rows that some of the tile's rows do not see may hold anything: those whose latents are not finite
             uint64_t odd = 0;
-            if (first_pos < end - 1 && key0 + kKeys - 1 > first_pos) {
-                if (tid < 2) wild[tid] = 0;
-                lds_barrier();
-                for (int e = tid; e < kKeys * 32; e += W * 64) {
-                    const int r = e & 63, c = e >> 6;  // pieces of a row in any order
-                    const u32x4_t v = *(lds_u4_ptr)(size_t)(at + (c >> 3) * kPlane + r * 128 + (c & 7) * 16);
-                    bool bad = false;
+            if (first_pos < end - 1 && k * kKeys + kKeys - 1 > first_pos) {
+                // (each wave by itself: a lane a row, its pieces in an order that spreads over the banks)
+                bool bad = false;
+                for (int c = 0; c < kRank / 8; ++c) {
+                    const u32x4_t v = *(lds_u4_ptr)(size_t)(at + (c >> 3) * kPlane + lane * 128 + (((c + (lane >> 1)) & 7) << 4));
 #pragma unroll
                     for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
-                    if (bad) atomicOr(&wild[r >> 5], 1u << (r & 31));
                 }
-                lds_barrier();
-                odd = (uint64_t)__builtin_amdgcn_readfirstlane(wild[1]) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane(wild[0]);
+                odd = ballot(bad);
             }
-            f32x16_t x[KB];
+            f32x4_t x[KB];
 #pragma unroll
-            for (int i = 0; i < KB; ++i) x[i] = f32x16_zero();
+            for (int i = 0; i < KB; ++i) x[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int st = 0; st < kWidth / 16; ++st)
+            for (int st = 0; st < kWidth / 32; ++st)
 #pragma unroll
                 for (int i = 0; i < KB; ++i) {
-                    const bf16x8_t a = *(lds_frag_ptr)(size_t)(at + k_at[st & 3] + (st >> 2) * kPlane + i * 32 * 128);
-                    x[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, fq[st].f, x[i], 0, 0, 0);
+                    const bf16x8_t a = *(lds_frag_ptr)(size_t)(at + k_at[st & 1] + (st >> 1) * kPlane + i * 16 * 128);
+                    x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, fq[st].f, x[i], 0, 0, 0);
                 }
-            const int my_key0 = key0 + 32 * (KW == 2 ? wk : 0);
-            if (my_key0 + 32 * KB - 1 > wave_pos) {
+            if (key0 + 16 * KB - 1 > wave_pos) {
 #pragma unroll
                 for (int i = 0; i < KB; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        x[i][e] = my_key0 + 32 * i + mfma32_row(e, lane) > my_pos ? -INFINITY : x[i][e];
+                    for (int e = 0; e < 4; ++e) x[i][e] = key0 + 16 * i + 4 * g + e > my_pos ? -INFINITY : x[i][e];
             }
             if (odd != 0) {
                 // a row that sees one of them has no result; for the others they are zeros
 #pragma unroll
                 for (int i = 0; i < KB; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int key = 32 * (KW == 2 ? wk : 0) + 32 * i + mfma32_row(e, lane);
-                        if ((odd >> key & 1) && key0 + key <= my_pos) l = NAN;
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = 16 * i + 4 * g + e;
+                        if ((odd >> (wave_key + key) & 1) && key0 + key <= my_pos) l = NAN;
                     }
                 lds_barrier();
                 for (int e = tid; e < kKeys * 32; e += W * 64) {
@@ -646,77 +652,73 @@ __global__ __launch_bounds__(WR * KW * 64) void attend_kernel(const uint16_t* __
 #pragma unroll
             for (int i = 0; i < KB; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[i][e]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float before = shift;
-            shift = fmaxf(shift, top * s.scale2);
-            const float r = __builtin_amdgcn_exp2f(before - shift);
-            l *= r;
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, x[i][e]);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64)) * s.scale2;
+            if (ballot(top > shift) != 0) {  // some row has a new maximum
+                const float before = shift;
+                shift = fmaxf(shift, top);
+                const float r = __builtin_amdgcn_exp2f(before - shift);
+                l *= r;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < 16; ++i) o[i] *= r;
+            }
+            Frag p[KB / 2];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[i][e] *= r;
-            Frag p[2 * KB];
-            float sum = 0.0f;
+            for (int i = 0; i < KB; ++i) {
+                float e[4];
 #pragma unroll
-            for (int i = 0; i < KB; ++i)
+                for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], s.scale2, -shift));
+                l += (e[0] + e[1]) + (e[2] + e[3]);
+                p[i / 2].w[(i & 1) * 2] = pack_bf16x2(e[0], e[1]);
+                p[i / 2].w[(i & 1) * 2 + 1] = pack_bf16x2(e[2], e[3]);
+            }
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], s.scale2, -shift));
-                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e + 1], s.scale2, -shift));
-                    sum += e0 + e1;
-                    p[2 * i + e / 8].w[e % 8 / 2] = pack_bf16x2(e0, e1);
-                }
-            l += sum;
+            for (int i = 0; i < KB / 2; ++i)
 #pragma unroll
-            for (int i = 0; i < 2 * KB; ++i)
-#pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    const uint32_t c = at + (d >> 1) * kPlane + i * 16 * 128;
+                for (int d = 0; d < 16; ++d) {
+                    const uint32_t c = at + (d >> 2) * kPlane + i * 32 * 128 + c_at[d & 3];
                     Frag a;
-                    a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(c + c_at[0][d & 1]));
-                    a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(c + c_at[1][d & 1]));
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f, p[i].f, o[d], 0, 0, 0);
+                    a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)c);
+                    a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(c + 16 * 128));
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.f, p[i].f, o[d], 0, 0, 0);
                 }
         }
+        l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
         lds_barrier();
         if constexpr (KW == 2) {
             // the second wave's sums join the first's through LDS
-            static_assert(WR * 33 * 1024 <= S * kStage, "both waves' sums fit the ring");
-            const uint32_t mine = lds + wr * 33 * 1024 + lane * 4;
+            static_assert(WR * 66 * 256 <= S * kStage, "both waves' sums fit the ring");
+            const uint32_t mine = lds + wr * 66 * 256 + lane * 4;
             if (wk == 1) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < 16; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) *(lds_f_ptr)(size_t)(mine + (i * 16 + e) * 256) = o[i][e];
-                *(lds_f_ptr)(size_t)(mine + 128 * 256) = shift;
-                *(lds_f_ptr)(size_t)(mine + 129 * 256) = l;
+                    for (int e = 0; e < 4; ++e) *(lds_f_ptr)(size_t)(mine + (i * 4 + e) * 256) = o[i][e];
+                *(lds_f_ptr)(size_t)(mine + 64 * 256) = shift;
+                *(lds_f_ptr)(size_t)(mine + 65 * 256) = l;
             }
             lds_barrier();
             if (wk == 0) {
-                const float other = *(lds_f_ptr)(size_t)(mine + 128 * 256), l2 = *(lds_f_ptr)(size_t)(mine + 129 * 256);
+                const float other = *(lds_f_ptr)(size_t)(mine + 64 * 256), l2 = *(lds_f_ptr)(size_t)(mine + 65 * 256);
                 const float both = fmaxf(shift, other);
-                const float f = __builtin_amdgcn_exp2f(shift - both), g = __builtin_amdgcn_exp2f(other - both);
+                const float f = __builtin_amdgcn_exp2f(shift - both), f2 = __builtin_amdgcn_exp2f(other - both);
                 shift = both;
-                l = l * f + l2 * g;
+                l = l * f + l2 * f2;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int i = 0; i < 16; ++i)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        o[i][e] = o[i][e] * f + *(lds_f_ptr)(size_t)(mine + (i * 16 + e) * 256) * g;
+                    for (int e = 0; e < 4; ++e) o[i][e] = o[i][e] * f + *(lds_f_ptr)(size_t)(mine + (i * 4 + e) * 256) * f2;
             }
             lds_barrier();
         }
         if (wk == 0 && my < it.rows) {
             const int64_t slot = ((int64_t)blockIdx.x + item) * RT + my;
-            float* y = sums + slot * kRank + 4 * half;
+            float* y = sums + slot * kRank + 4 * g;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    *reinterpret_cast<f32x4_t*>(y + 32 * i + 2 * e) = f32x4_t{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
-            if (half == 0) stats[slot] = make_float2(shift, l);
+            for (int i = 0; i < 16; ++i) *reinterpret_cast<f32x4_t*>(y + 16 * i) = o[i];
+            if (g == 0) stats[slot] = make_float2(shift, l);
         }
         t = to;
     }
@@ -742,20 +744,32 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
     Parts p = {0, 0, false};
     int in = 0;
     if (i >= 0) p = row_parts(b, s, plan, items, seq_item, i, (t - b.starts[i]) * s.H + h, in);
-    float top = kLowest;
-    for (int k = sub; k < p.n; k += G) top = fmaxf(top, stats[(p.slot + k) * s.rows + in].x);
-    float l = 0.0f, v[16] = {};
-#pragma unroll 2
-    for (int k = sub; k < p.n; k += G) {
-        const int64_t at = (p.slot + k) * s.rows + in;
-        const float2 ml = stats[at];
-        const float f = __builtin_amdgcn_exp2f(ml.x - top);
-        l += ml.y * f;
+    float top = kLowest, l = 0.0f, v[16] = {};
+    for (int k = sub; k < p.n; k += 4 * G) {  // four parts' loads on their way at a time
+        float2 ml[4];
+        f32x4_t x[4][4];
+        float next = top;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(sums + at * kRank + c * 64 + col);
+        for (int j = 0; j < 4; ++j) {
+            const int64_t at = (p.slot + (k + j * G < p.n ? k + j * G : k)) * s.rows + in;
+            ml[j] = stats[at];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * c + e] += x[e] * f;
+            for (int c = 0; c < 4; ++c) x[j][c] = *reinterpret_cast<const f32x4_t*>(sums + at * kRank + c * 64 + col);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) next = fmaxf(next, ml[j].x);
+        const float r = __builtin_amdgcn_exp2f(top - next);
+        top = next;
+        l *= r;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] *= r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (k + j * G >= p.n) break;
+            const float f = __builtin_amdgcn_exp2f(ml[j].x - top);
+            l = __builtin_fmaf(ml[j].y, f, l);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = __builtin_fmaf(x[j][e >> 2][e & 3], f, v[e]);
         }
     }
     if constexpr (G > 1) {
@@ -808,17 +822,17 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
     }
 }
 
-bool is_fast(int rank, int rope, int nope, int v_dim, int dtype) {
-    return dtype == kBF16 && rank == kRank && rope == kRope && nope % 16 == 0 && v_dim % 16 == 0;
+bool is_fast(int rank, int rope, int nope, int v_dim, int page_log, int dtype) {
+    return dtype == kBF16 && rank == kRank && rope == kRope && nope % 16 == 0 && v_dim % 16 == 0 && page_log >= kBlockLog;
 }
 
-// Rows of a tile: as many as a sequence's new tokens have on the average, 32, 64 or 128.  A workgroup of 32 leaves room for a
-// second one on its CU.
+// Rows of a tile: as many as a sequence's new tokens have on the average, 16 to 128.  Workgroups of up to 32 leave room for
+// a second one on their CU.
 int fast_rows(int64_t n_rows, int n_seq, int H) {
     const int64_t each = n_rows * H / n_seq;
-    return each <= 32 ? 32 : each <= 64 ? 64 : 128;
+    return each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
 }
-int fast_groups(int rows, int num_cus) { return rows == 32 ? 2 * num_cus : num_cus; }
+int fast_groups(int rows, int num_cus) { return rows <= 32 ? 2 * num_cus : num_cus; }
 
 int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, const Batch& b, const float* rates, Shape s, unsigned char* ws,
                 uint16_t* out, int num_cus, hipStream_t stream) {
@@ -834,13 +848,13 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
     const unsigned tiles = (unsigned)((b.n_rows + 31) / 32);
     hipLaunchKernelGGL(prepare_kernel, dim3(tiles * s.H + 1), dim3(256), 0, stream, q, w, rates, b, s, l.max_items, plan, items, seq_item,
                        tok_seq, specials, queries);
-    const dim3 grid((unsigned)s.groups);
-    if (s.rows == 32)
-        hipLaunchKernelGGL((attend_kernel<1, 2, 2>), grid, dim3(128), 0, stream, pool, b, s, plan, items, queries, specials, sums, stats);
-    else if (s.rows == 64)
-        hipLaunchKernelGGL((attend_kernel<2, 2, 3>), grid, dim3(256), 0, stream, pool, b, s, plan, items, queries, specials, sums, stats);
-    else
-        hipLaunchKernelGGL((attend_kernel<4, 1, 3>), grid, dim3(256), 0, stream, pool, b, s, plan, items, queries, specials, sums, stats);
+    auto attend = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)s.groups), dim3(threads), 0, stream, pool, b, s, plan, items, queries, specials, sums, stats);
+    };
+    if (s.rows == 16) attend(attend_kernel<1, 2, 2>, 128);
+    else if (s.rows == 32) attend(attend_kernel<2, 2, 2>, 256);
+    else if (s.rows == 64) attend(attend_kernel<4, 2, 3>, 512);
+    else attend(attend_kernel<8, 1, 3>, 512);
     // (few tokens have many parts each: more threads a token)
     if (b.n_rows <= 8)
         hipLaunchKernelGGL((finish_kernel<1>), dim3((unsigned)(b.n_rows * s.H)), dim3(256), 0, stream, w, b, s, plan, items, seq_item, tok_seq, sums,
@@ -856,19 +870,17 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(int64_t n_rows, int n_seq, int H, int rank, int rope, int nope, int v_dim, int dtype,
-                                       int num_cus) {
-    if (is_fast(rank, rope, nope, v_dim, dtype)) {
-        const int rows = fast_rows(n_rows, n_seq, H);
-        return layout(n_rows, n_seq, H, kWidth, rows, fast_groups(rows, num_cus), 2, kRank).bytes;
-    }
+size_t paged_attention_workspace_bytes(int64_t n_rows, int n_seq, int H, int rank, int rope, int nope, int v_dim, int page_log,
+                                       int dtype, int num_cus) {
+    const int rows = fast_rows(n_rows, n_seq, H);
+    if (is_fast(rank, rope, nope, v_dim, page_log, dtype)) return layout(n_rows, n_seq, H, kWidth, rows, fast_groups(rows, num_cus), 2, kRank).bytes;
     return layout(n_rows, n_seq, H, rank + rope, kAnyRows, any_groups(num_cus), 4, rank).bytes;
 }
 
 int launch_paged_attention(const void* q, const void* w, const void* pool, const Batch& b, const float* rates, int H, int rank, int rope,
                            int nope, int v_dim, int dtype, float scale, void* ws, void* out, int num_cus, hipStream_t stream) {
     const Shape s = {H, rank, rope, nope, v_dim, 0, 0, scale * kLog2E};
-    if (is_fast(rank, rope, nope, v_dim, dtype))
+    if (is_fast(rank, rope, nope, v_dim, b.page_log, dtype))
         return launch_fast((const uint16_t*)q, (const uint16_t*)w, (const uint16_t*)pool, b, rates, s, (unsigned char*)ws, (uint16_t*)out,
                            num_cus, stream);
     if (dtype == kBF16)
