@@ -88,7 +88,7 @@ SIGNATURES = {
     "ethos_latent_append": (ctypes.c_int, [_vp, _i64] + [_vp] * 3 + [_i64, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i64, _i32, _f32, _i32, _vp,
                                            _vp]),
     "ethos_copy_pages": (ctypes.c_int, [_vp] + [_i64] * 4 + [_vp, _vp, _i32, _vp]),
-    "ethos_paged_attention_workspace_bytes": (_sz, [_i64] + [_i32] * 8),
+    "ethos_paged_attention_workspace_bytes": (_sz, [_i64] + [_i32] * 9),
     "ethos_paged_attention": (ctypes.c_int, [_vp] * 4 + [_i64, _i32] + [_vp] * 3 + [_i64] + [_i32] * 6 + [_i64, _i32, _i32, _f32, _vp, _sz, _vp,
                                              _vp]),
     "ethos_verify_workspace_bytes": (_sz, [_i64, _i32, _i64]),

@@ -1219,11 +1219,11 @@ int paged_sizes(int64_t n_rows, int32_t n_heads, int32_t nope, int32_t v_dim, co
 }  // namespace
 
 size_t ethos_paged_attention_workspace_bytes(int64_t n_rows, int32_t n_seq, int32_t n_heads, int32_t rank, int32_t rope, int32_t nope,
-                                             int32_t v_dim, int32_t page, int32_t dtype) {
-    if (n_rows <= 0 || n_seq <= 0 || batch_sizes(n_rows, n_seq, 0, 0, 1, page, rank, rope, dtype, "ethos_paged_attention_workspace_bytes") != 0 ||
+                                             int32_t v_dim, int32_t table_width, int32_t page, int32_t dtype) {
+    if (n_rows <= 0 || n_seq <= 0 || batch_sizes(n_rows, n_seq, table_width, table_width, 1, page, rank, rope, dtype, "ethos_paged_attention_workspace_bytes") != 0 ||
         paged_sizes(n_rows, n_heads, nope, v_dim, "ethos_paged_attention_workspace_bytes") != 0)
         return 256;
-    return ethos::paged_attention_workspace_bytes(n_rows, n_seq, n_heads, rank, rope, nope, v_dim, log_of(page), dtype, num_cus());
+    return ethos::paged_attention_workspace_bytes(n_rows, n_seq, n_heads, rank, rope, nope, v_dim, table_width, log_of(page), dtype, num_cus());
 }
 
 int ethos_paged_attention(const void* q, const void* w, const void* pool, const int32_t* table, int64_t table_ld, int32_t table_width,
@@ -1237,7 +1237,7 @@ int ethos_paged_attention(const void* q, const void* w, const void* pool, const 
     if (n_rows == 0 || n_seq == 0) return 0;
     if (!q || !w || !pool || (table_width > 0 && !table) || !lens || !starts || (rope > 0 && !rates) || !workspace || !out)
         return fail(ETHOS_ENULL, "ethos_paged_attention: null pointer");
-    const size_t need = ethos::paged_attention_workspace_bytes(n_rows, n_seq, n_heads, rank, rope, nope, v_dim, log_of(page), dtype, num_cus());
+    const size_t need = ethos::paged_attention_workspace_bytes(n_rows, n_seq, n_heads, rank, rope, nope, v_dim, table_width, log_of(page), dtype, num_cus());
     if (workspace_bytes < need)
         return fail(ETHOS_EWORKSPACE, "ethos_paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (!aligned16(q) || !aligned16(w) || !aligned16(pool) || !aligned16(workspace) || !aligned16(out))

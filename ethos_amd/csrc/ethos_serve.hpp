@@ -60,8 +60,8 @@ int launch_latent_append(const void* rows, int64_t ld, const void* gain, const f
 int launch_copy_pages(void* pool, int64_t n_blocks, int64_t block_bytes, int64_t page_bytes, const int32_t* src, const int32_t* dst,
                       int n_pairs, int num_cus, hipStream_t stream);
 
-size_t paged_attention_workspace_bytes(int64_t n_rows, int n_seq, int H, int rank, int rope, int nope, int v_dim, int page_log,
-                                       int dtype, int num_cus);
+size_t paged_attention_workspace_bytes(int64_t n_rows, int n_seq, int H, int rank, int rope, int nope, int v_dim, int width,
+                                       int page_log, int dtype, int num_cus);
 int launch_paged_attention(const void* q, const void* w, const void* pool, const Batch& b, const float* rates, int H, int rank, int rope,
                            int nope, int v_dim, int dtype, float scale, void* ws, void* out, int num_cus, hipStream_t stream);
 

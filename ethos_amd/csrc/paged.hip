@@ -48,6 +48,7 @@ struct Shape {
     int H, rank, rope, nope, v_dim;
     int rows;    // of a tile
     int groups;  // workgroups that share the work
+    int planes;  // how often the work is there: once for all heads, or once for each
     float scale2;
 };
 
@@ -106,12 +107,19 @@ __device__ __forceinline__ bool fits(const Batch& b, int i) {
 
 // One workgroup of NT threads: NT sequences at a time, then their items, NT at a time.
 template <int NT>
-__device__ void make_plan(const Batch& b, const Shape& s, int64_t max_items, Plan* plan, Item* items, int32_t* seq_item, int tid) {
+__device__ void make_plan(const Batch& b, const Shape& s, int64_t max_items, Plan* plan, Item* items, int32_t* seq_item, int32_t* seq_keys,
+                          int tid) {
     __shared__ int64_t lds[NT / 64];
     __shared__ int32_t ends[NT], counts[NT], tok0[NT], lens[NT];
-    int64_t base = 0, tiles = 0, total;
+    int64_t base = 0, tiles = 0, key_tiles = 0, total;
     for (int at = 0; at < b.n_seq; at += NT) {
         const int i = at + tid;
+        if (seq_keys) {  // where each sequence's keys begin, if all are laid out one after the other
+            const int64_t n = i < b.n_seq && new_tokens(b, i) > 0 && fits(b, i) ? (b.lens[i] + kKeys - 1) / kKeys : 0;
+            const int64_t end = key_tiles + block_scan<NT>(n, lds, tid, total);
+            if (i < b.n_seq) seq_keys[i] = (int32_t)(end - n);
+            key_tiles += total;
+        }
         const int64_t count = i < b.n_seq ? new_tokens(b, i) : 0, n = (count * s.H + s.rows - 1) / s.rows;
         const int64_t end = block_scan<NT>(n, lds, tid, total);
         // (starts that overlap could ask for more than there is room for: those sequences get none)
@@ -147,7 +155,9 @@ __device__ void make_plan(const Batch& b, const Shape& s, int64_t max_items, Pla
         __syncthreads();
     }
     if (tid == 0) {
+        if (seq_keys) seq_keys[b.n_seq] = (int32_t)key_tiles;
         // (few tiles a workgroup, two workgroups a CU: one on each, whose parts are then half as many to join)
+        tiles *= s.planes;
         const int64_t groups = s.rows <= 32 && tiles < 4 * (int64_t)s.groups ? (s.groups + 1) / 2 : s.groups;
         plan->tiles = tiles;
         plan->quota = tiles > groups ? (tiles + groups - 1) / groups : 1;
@@ -178,7 +188,7 @@ __global__ __launch_bounds__(1024) void any_prepare_kernel(const T* __restrict__
                                                            Batch b, Shape s, int64_t max_items, Plan* plan, Item* items, int32_t* seq_item,
                                                            int32_t* tok_seq, float* __restrict__ queries) {
     if (blockIdx.x == 0) {
-        make_plan<1024>(b, s, max_items, plan, items, seq_item, threadIdx.x);
+        make_plan<1024>(b, s, max_items, plan, items, seq_item, nullptr, threadIdx.x);
         return;
     }
     const int64_t t = blockIdx.x - 1;
@@ -299,17 +309,19 @@ struct Parts {
     bool bad;  // the sequence's length does not fit its table, or there was no room for it
 };
 __device__ __forceinline__ Parts row_parts(const Batch& b, const Shape& s, const Plan* plan, const Item* items, const int32_t* seq_item, int i,
-                                           int64_t row, int& in) {
+                                           int64_t row, int plane, int& in) {
     Parts p = {0, 0, true};
     const int32_t first = seq_item[i];
     if (first < 0 || new_tokens(b, i) == 0 || !fits(b, i)) return p;
     p.bad = false;
     const int64_t item = first + row / s.rows;
     in = (int)(row % s.rows);
-    const int64_t begin = item > 0 ? items[item - 1].end : 0, end = items[item].end;
+    int64_t begin = item > 0 ? items[item - 1].end : 0, end = items[item].end;
     if (end > begin) {
+        const int64_t before = plane * (plan->tiles / s.planes);  // the work of the planes before
+        begin += before, end += before;
         const int64_t a = begin / plan->quota, z = (end - 1) / plan->quota;
-        p.slot = a + item;
+        p.slot = a + (int64_t)plane * plan->n_items + item;
         p.n = (int)(z - a + 1);
     }
     return p;
@@ -327,7 +339,7 @@ __global__ __launch_bounds__(256) void any_finish_kernel(const T* __restrict__ w
     if (i < 0) return;  // behind the last sequence
     for (int h = 0; h < s.H; ++h) {
         int in = 0;
-        const Parts p = row_parts(b, s, plan, items, seq_item, i, (t - b.starts[i]) * s.H + h, in);
+        const Parts p = row_parts(b, s, plan, items, seq_item, i, (t - b.starts[i]) * s.H + h, 0, in);
         float top = kLowest, l = 0.0f;
         for (int k = 0; k < p.n; ++k) top = fmaxf(top, stats[(p.slot + k) * s.rows + in].x);
         for (int k = 0; k < p.n; ++k) {
@@ -431,7 +443,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (blockIdx.x == 0) {
         for (int e = tid; e < 2 * kBlock * kWidth; e += 256) specials[e] = e < kBlock * kWidth ? 0 : 0x7fc0;
-        make_plan<256>(b, s, max_items, plan, items, seq_item, tid);
+        make_plan<256>(b, s, max_items, plan, items, seq_item, nullptr, tid);
         return;
     }
     const int h = (blockIdx.x - 1) % s.H, qw = s.nope + kRope;
@@ -743,7 +755,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
     const int i = t < b.n_rows ? tok_seq[t] : -1;
     Parts p = {0, 0, false};
     int in = 0;
-    if (i >= 0) p = row_parts(b, s, plan, items, seq_item, i, (t - b.starts[i]) * s.H + h, in);
+    if (i >= 0) p = row_parts(b, s, plan, items, seq_item, i, (t - b.starts[i]) * s.H + h, 0, in);
     float top = kLowest, l = 0.0f, v[16] = {};
     for (int k = sub; k < p.n; k += 4 * G) {  // four parts' loads on their way at a time
         float2 ml[4];
@@ -868,18 +880,408 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
     return (int)hipGetLastError();
 }
 
+// ------------------------------------------------------------------------- many new tokens a sequence
+// The same weight may go to the keys and values instead, once for each cached row and head: 65 K operations a
+// row and head, after which a (token, head, key) takes 384 instead of 1,152.  That is the shorter way from some
+// kChunkRows new tokens a sequence on.  Keys and values of a head lie one sequence behind the other, 64 | 64 columns a row,
+// each sequence's rows filled up with zeros to a multiple of 64; the keys' rotated parts, which the heads share, likewise.
+// The attention is then that of any causal head: 128 tokens of a head a workgroup, 32 a wave, keys in steps of 64,
+// and heads as the outer dimension of the even shares, so that an XCD's workgroups read the same two heads' keys from its L2.
+constexpr int kHead = 64;         // columns of a head's keys (before the rotated ones) and of its values
+constexpr int kChunkTok = 128;    // tokens of a tile
+constexpr int kChunkRows = 128;   // new tokens a sequence, on the average, from which this is the shorter way
+constexpr size_t kChunkBytes = (size_t)1 << 30;  // of keys and values, at most
+
+struct ChunkLayout {
+    size_t plan, items, seq_item, tok_seq, seq_keys, turns, keys, shared, sums, stats, bytes;
+    int64_t max_items, key_rows;
+};
+
+ChunkLayout chunk_layout(int64_t n_rows, int n_seq, int H, int64_t capacity, int groups) {
+    ChunkLayout l;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t p = at;
+        at += round256(bytes);
+        return p;
+    };
+    l.max_items = n_rows / kChunkTok + n_seq;
+    l.key_rows = n_seq * ((capacity + kKeys - 1) / kKeys * kKeys);
+    l.plan = take(sizeof(Plan));
+    l.items = take((size_t)l.max_items * sizeof(Item));
+    l.seq_item = take((size_t)n_seq * 4);
+    l.tok_seq = take((size_t)n_rows * 4);
+    l.seq_keys = take((size_t)(n_seq + 1) * 4);
+    l.turns = take((size_t)n_rows * kRope / 2 * 8);
+    l.keys = take((size_t)l.key_rows * H * 2 * kHead * 2);
+    l.shared = take((size_t)l.key_rows * kRope * 2);
+    const size_t slots = (size_t)(l.max_items * H + groups);
+    l.sums = take(slots * kChunkTok * kHead * 4);
+    l.stats = take(slots * kChunkTok * 8);
+    l.bytes = at;
+    return l;
+}
+
+// Block 0: the plan.  The others: eight tokens' sequences, cosines and sines.
+__global__ __launch_bounds__(256) void chunk_prepare_kernel(const float* __restrict__ rates, Batch b, Shape s, int64_t max_items, Plan* plan,
+                                                            Item* items, int32_t* seq_item, int32_t* seq_keys, int32_t* tok_seq,
+                                                            float2* __restrict__ turns) {
+    if (blockIdx.x == 0) {
+        Shape one = s;
+        one.H = 1;
+        make_plan<256>(b, one, max_items, plan, items, seq_item, seq_keys, threadIdx.x);
+        return;
+    }
+    const int64_t t = (int64_t)(blockIdx.x - 1) * 8 + (threadIdx.x >> 5);
+    const int p = threadIdx.x & 31;
+    if (t >= b.n_rows) return;
+    const int i = batch_seq(b, t);
+    if (p == 0) tok_seq[t] = i;
+    if (i < 0) return;
+    float2 c;
+    rotary_angle((int64_t)b.lens[i] - b.starts[i + 1] + t, rates[p], c.x, c.y);
+    turns[t * 32 + p] = c;
+}
+
+// Keys and values of 64 cached rows for four heads: [column][row] = W_h c^T, a wave 32 of a head's 128 columns; the
+// weight's fragments from memory, the rows from LDS in the planes of above.  Workgroups go round (64 rows, heads).
+__global__ __launch_bounds__(256) void expand_kernel(const uint16_t* __restrict__ w, const uint16_t* __restrict__ pool, Batch b, Shape s,
+                                                     const int32_t* __restrict__ seq_keys, int64_t key_rows, uint16_t* __restrict__ keys,
+                                                     uint16_t* __restrict__ shared) {
+    __shared__ __align__(16) unsigned char rows[kRank / 64 * kPlane];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t lds = lds_addr(rows);
+    const int parts = (s.H + 3) / 4;
+    const int64_t work = (int64_t)seq_keys[b.n_seq] * parts;
+    for (int64_t u = blockIdx.x; u < work; u += gridDim.x) {
+        const int tile = (int)(u / parts), h0 = (int)(u % parts) * 4;
+        int lo = 0, hi = b.n_seq;  // the last sequence whose tiles begin at or before this one
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (seq_keys[mid] <= tile) lo = mid;
+            else hi = mid;
+        }
+        const int key0 = (tile - seq_keys[lo]) * kKeys, len = b.lens[lo];
+        // a thread's pieces: 10 of 64 rows of 40
+        for (int e = tid; e < kKeys * (kWidth / 8); e += 256) {
+            const int r = e / (kWidth / 8), c = e - r * (kWidth / 8), p = key0 + r;
+            u32x4_t v = {0, 0, 0, 0};
+            if (p < len) {
+                const int32_t page = batch_page(b, lo, p);
+                if (page >= 0)
+                    v = *reinterpret_cast<const u32x4_t*>(pool + (((int64_t)page << b.page_log) + (p & ((1 << b.page_log) - 1))) * kWidth + c * 8);
+                else
+                    v = u32x4_t{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+            }
+            if (c < kRank / 8) *(lds_u4_ptr)(size_t)(lds + (c >> 3) * kPlane + r * 128 + (((c & 7) ^ swizzle(r)) << 4)) = v;
+            else if (h0 == 0) *reinterpret_cast<u32x4_t*>(shared + ((int64_t)tile * kKeys + r) * kRope + (c - kRank / 8) * 8) = v;
+        }
+        __syncthreads();
+        for (int h = h0; h < h0 + 4 && h < s.H; ++h) {
+            const uint16_t* wh = w + ((int64_t)h * 2 * kHead + wave * 32 + (lane & 31)) * kRank + 8 * half;
+            f32x16_t acc[2] = {f32x16_zero(), f32x16_zero()};
+            bf16x8_t a[kRank / 16];
+#pragma unroll
+            for (int st = 0; st < kRank / 16; ++st) a[st] = *reinterpret_cast<const bf16x8_t*>(wh + 16 * st);
+#pragma unroll
+            for (int st = 0; st < kRank / 16; ++st)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 32 * i + (lane & 31);
+                    const bf16x8_t x = *(lds_frag_ptr)(size_t)(lds + (st >> 2) * kPlane + r * 128 + (((2 * (st & 3) + half) ^ swizzle(r)) << 4));
+                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[st], x, acc[i], 0, 0, 0);
+                }
+            uint16_t* to = keys + ((int64_t)h * key_rows + (int64_t)tile * kKeys + (lane & 31)) * (2 * kHead) + wave * 32 + 4 * half;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<uint2*>(to + i * 32 * 2 * kHead + 2 * e) =
+                        make_uint2(pack_bf16x2(acc[i][e], acc[i][e + 1]), pack_bf16x2(acc[i][e + 2], acc[i][e + 3]));
+        }
+        __syncthreads();
+    }
+}
+
+// A step's LDS: three planes of 64 rows, keys, rotated keys, values.
+constexpr int kChunkStage = 3 * kPlane;
+template <int S, int WGS>
+__global__ __launch_bounds__(256, WGS) void chunk_attend_kernel(const uint16_t* __restrict__ q, const float2* __restrict__ turns,
+                                                              const uint16_t* __restrict__ keys, const uint16_t* __restrict__ shared, Shape s,
+                                                              const Plan* plan, const Item* __restrict__ items,
+                                                              const int32_t* __restrict__ seq_keys, int64_t key_rows, float* __restrict__ sums,
+                                                              float2* __restrict__ stats, uint16_t* __restrict__ out) {
+    __shared__ __align__(16) unsigned char ring[S * kChunkStage];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t lds = lds_addr(ring);
+    // neighbours in the work on one XCD (workgroups go round the eight)
+    const int group = gridDim.x % 8 == 0 ? (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8) : (int)blockIdx.x;
+    const int64_t quota = plan->quota, all = plan->tiles, each = all / s.planes;
+    const int n_items = plan->n_items;
+    int64_t t = group * quota;
+    const int64_t stop = t + quota < all ? t + quota : all;
+    if (t >= stop) return;
+    uint32_t k_at[4], v_at[2][2];
+    {
+        const int key = lane & 31, row = 4 * half + ((lane & 15) >> 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k_at[i] = key * 128 + (((2 * i + half) ^ swizzle(key)) << 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                const int r = row + 8 * i, c = 4 * d + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+                v_at[i][d] = 2 * kPlane + r * 128 + ((c ^ swizzle(r)) << 4) + (lane & 1) * 8;
+            }
+    }
+    // a lane's places in a copy of 8 rows, of blocks with an even and an odd number
+    uint32_t key_off[2], shared_off[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = lane >> 3, piece = (lane & 7) ^ swizzle(8 * i + row);
+        key_off[i] = row * (4 * kHead) + piece * 16;
+        shared_off[i] = row * (2 * kRope) + piece * 16;
+    }
+
+    int h = (int)(t / each);
+    int item = find_item(items, n_items, t - h * each, lane);
+    for (; t < stop; ++item) {
+        if (item == n_items) item = 0, ++h;
+        const Item it = items[item];
+        const int64_t before = h * each, begin = before + (item > 0 ? items[item - 1].end : 0), finish = before + it.end;
+        const int64_t to = finish < stop ? finish : stop;
+        if (to <= t) continue;
+        const int k_begin = (int)(t - begin), k_end = (int)(to - begin);
+        const int my = wave * 32 + (lane & 31), my_row = my < it.rows ? my : it.rows - 1;
+        const int first_pos = it.pos0 + it.row0, my_pos = first_pos + my_row;
+        const int wave_pos = first_pos + (wave * 32 < it.rows ? wave * 32 : it.rows - 1);
+        const int64_t row = (int64_t)it.tok0 + it.row0 + my_row;
+        const int64_t key_row = (int64_t)seq_keys[it.seq] * kKeys;
+        const unsigned char* kv = (const unsigned char*)(keys + ((int64_t)h * key_rows + key_row) * (2 * kHead));
+        const unsigned char* kr = (const unsigned char*)(shared + key_row * kRope);
+
+        auto copy_step = [&](int k, int stage) {
+#pragma unroll
+            for (int i = 0; i < 6; ++i) {
+                const int pl = i >> 1, blk = 2 * wave + (i & 1);
+                const int64_t at = (int64_t)k * kKeys + blk * 8;
+                const uint32_t to_lds = __builtin_amdgcn_readfirstlane(lds + stage * kChunkStage + pl * kPlane + blk * 1024);
+                if (pl == 1) copy16(kr + at * (2 * kRope), shared_off[i & 1], to_lds);
+                else copy16(kv + at * (4 * kHead) + (pl == 2 ? 2 * kHead : 0), key_off[i & 1], to_lds);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i)
+            if (k_begin + i < k_end) copy_step(k_begin + i, i);
+        Frag fq[8];
+        {
+            const uint16_t* qp = q + (row * s.H + h) * (kHead + kRope) + 8 * half;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) fq[i].u = *reinterpret_cast<const u32x4_t*>(qp + 16 * i);
+            const float4* cs = reinterpret_cast<const float4*>(turns + row * 32 + 8 * half);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 c = cs[8 * i + j];  // cos, sin of two angles
+                    const uint32_t u = fq[4 + i].w[j], v = fq[6 + i].w[j];
+                    const float u0 = __uint_as_float(u << 16), u1 = __uint_as_float(u & 0xffff0000u);
+                    const float v0 = __uint_as_float(v << 16), v1 = __uint_as_float(v & 0xffff0000u);
+                    fq[4 + i].w[j] = pack_bf16x2(u0 * c.x - v0 * c.y, u1 * c.z - v1 * c.w);
+                    fq[6 + i].w[j] = pack_bf16x2(v0 * c.x + u0 * c.y, v1 * c.z + u1 * c.w);
+                }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(fq[i].u));
+        }
+        f32x16_t o[2] = {f32x16_zero(), f32x16_zero()};
+        float shift = kLowest, l = 0.0f;
+        int stage = 0;
+        for (int k = k_begin; k < k_end; ++k) {
+            if (S == 3 && k + 1 < k_end) copies_barrier<6 * (S - 2)>();
+            else copies_barrier<0>();
+            if (k + S - 1 < k_end) copy_step(k + S - 1, stage == 0 ? S - 1 : stage - 1);
+            const uint32_t at = lds + stage * kChunkStage;
+            const int key0 = k * kKeys;
+            stage = stage == S - 1 ? 0 : stage + 1;
+            uint64_t odd = 0;  // rows that some tokens do not see, and whose values are not finite
+            if (key0 + kKeys - 1 > first_pos) {
+                bool bad = false;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const u32x4_t v = *(lds_u4_ptr)(size_t)(at + 2 * kPlane + lane * 128 + (((c + (lane >> 1)) & 7) << 4));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+                }
+                odd = ballot(bad);
+            }
+            f32x16_t x[2] = {f32x16_zero(), f32x16_zero()};
+#pragma unroll
+            for (int st = 0; st < 8; ++st)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const bf16x8_t a = *(lds_frag_ptr)(size_t)(at + k_at[st & 3] + (st >> 2) * kPlane + i * 32 * 128);
+                    x[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, fq[st].f, x[i], 0, 0, 0);
+                }
+            if (key0 + kKeys - 1 > wave_pos) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[i][e] = key0 + 32 * i + mfma32_row(e, lane) > my_pos ? -INFINITY : x[i][e];
+            }
+            if (odd != 0) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int key = 32 * i + mfma32_row(e, lane);
+                        if ((odd >> key & 1) && key0 + key <= my_pos) l = NAN;
+                    }
+                lds_barrier();
+                for (int e = tid; e < kKeys * 8; e += 256)
+                    if (odd >> (e >> 3) & 1) *(lds_u4_ptr)(size_t)(at + 2 * kPlane + e * 16) = u32x4_t{0, 0, 0, 0};
+                lds_barrier();
+            }
+            float top = x[0][0];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[i][e]);
+            top = fmaxf(top, __shfl_xor(top, 32, 64)) * s.scale2;
+            if (ballot(top > shift) != 0) {
+                const float was = shift;
+                shift = fmaxf(shift, top);
+                const float r = __builtin_amdgcn_exp2f(was - shift);
+                l *= r;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[i][e] *= r;
+            }
+            Frag p[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], s.scale2, -shift));
+                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e + 1], s.scale2, -shift));
+                    l += e0 + e1;
+                    p[2 * i + e / 8].w[e % 8 / 2] = pack_bf16x2(e0, e1);
+                }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    Frag a;
+                    a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(at + v_at[0][d] + i * 16 * 128));
+                    a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(at + v_at[1][d] + i * 16 * 128));
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f, p[i].f, o[d], 0, 0, 0);
+                }
+        }
+        l += __shfl_xor(l, 32, 64);
+        lds_barrier();
+        if (my < it.rows) {
+            if (t == begin && to == finish) {  // the tile's whole work
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                uint16_t* y = out + (row * s.H + h) * kHead + 4 * half;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<uint2*>(y + 32 * i + 2 * e) = make_uint2(pack_bf16x2(o[i][e] * inv, o[i][e + 1] * inv),
+                                                                                   pack_bf16x2(o[i][e + 2] * inv, o[i][e + 3] * inv));
+            } else {
+                const int64_t slot = ((int64_t)group + (int64_t)h * n_items + item) * kChunkTok + my;
+                float* y = sums + slot * kHead + 4 * half;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<f32x4_t*>(y + 32 * i + 2 * e) = f32x4_t{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+                if (half == 0) stats[slot] = make_float2(shift, l);
+            }
+        }
+        t = to;
+    }
+}
+
+// 16 (token, head) rows a workgroup, 16 threads each: joins the parts of those that have several.
+__global__ __launch_bounds__(256) void chunk_finish_kernel(Batch b, Shape s, const Plan* plan, const Item* __restrict__ items,
+                                                           const int32_t* __restrict__ seq_item, const int32_t* __restrict__ tok_seq,
+                                                           const float* __restrict__ sums, const float2* __restrict__ stats,
+                                                           uint16_t* __restrict__ out) {
+    const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), t = r / s.H;
+    const int h = (int)(r - t * s.H), col = (threadIdx.x & 15) * 4;
+    if (t >= b.n_rows) return;
+    const int i = tok_seq[t];
+    if (i < 0) return;
+    int in = 0;
+    const Parts p = row_parts(b, s, plan, items, seq_item, i, t - b.starts[i], h, in);
+    if (p.n == 1) return;  // written as a whole
+    float top = kLowest, l = 0.0f;
+    f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < p.n; ++k) {
+        const int64_t at = (p.slot + k) * kChunkTok + in;
+        const float2 ml = stats[at];
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(sums + at * kHead + col);
+        const float next = fmaxf(top, ml.x), f = __builtin_amdgcn_exp2f(top - next), f2 = __builtin_amdgcn_exp2f(ml.x - next);
+        top = next;
+        l = l * f + ml.y * f2;
+        v = v * f + x * f2;
+    }
+    const float inv = p.bad ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint2*>(out + r * kHead + col) = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+}
+
+bool is_chunk(int64_t n_rows, int n_seq, int H, int nope, int v_dim, int64_t capacity) {
+    return nope == kHead && v_dim == kHead && n_rows >= (int64_t)kChunkRows * n_seq &&
+           (size_t)n_seq * (size_t)(capacity + kKeys) <= kChunkBytes / (size_t)(H * 4 * kHead);
+}
+constexpr int kChunkGroups = 2;  // workgroups a CU
+int chunk_groups(int num_cus) { return kChunkGroups * num_cus; }
+
+int launch_chunk(const uint16_t* q, const uint16_t* w, const uint16_t* pool, const Batch& b, const float* rates, Shape s, unsigned char* ws,
+                 uint16_t* out, int num_cus, hipStream_t stream) {
+    s.rows = kChunkTok;
+    s.groups = chunk_groups(num_cus);
+    s.planes = s.H;
+    const ChunkLayout l = chunk_layout(b.n_rows, b.n_seq, s.H, (int64_t)b.width << b.page_log, s.groups);
+    Plan* plan = (Plan*)(ws + l.plan);
+    Item* items = (Item*)(ws + l.items);
+    int32_t *seq_item = (int32_t*)(ws + l.seq_item), *tok_seq = (int32_t*)(ws + l.tok_seq), *seq_keys = (int32_t*)(ws + l.seq_keys);
+    float2 *turns = (float2*)(ws + l.turns), *stats = (float2*)(ws + l.stats);
+    uint16_t *keys = (uint16_t*)(ws + l.keys), *shared = (uint16_t*)(ws + l.shared);
+    float* sums = (float*)(ws + l.sums);
+    hipLaunchKernelGGL(chunk_prepare_kernel, dim3((unsigned)((b.n_rows + 7) / 8 + 1)), dim3(256), 0, stream, rates, b, s, l.max_items, plan, items,
+                       seq_item, seq_keys, tok_seq, turns);
+    hipLaunchKernelGGL(expand_kernel, dim3((unsigned)(4 * num_cus)), dim3(256), 0, stream, w, pool, b, s, seq_keys, l.key_rows, keys, shared);
+    hipLaunchKernelGGL((chunk_attend_kernel<3, kChunkGroups>), dim3((unsigned)s.groups), dim3(256), 0, stream, q, turns, keys, shared, s, plan, items, seq_keys,
+                       l.key_rows, sums, stats, out);
+    hipLaunchKernelGGL(chunk_finish_kernel, dim3((unsigned)((b.n_rows * s.H + 15) / 16)), dim3(256), 0, stream, b, s, plan, items, seq_item,
+                       tok_seq, sums, stats, out);
+    return (int)hipGetLastError();
+}
+
 }  // namespace
 
-size_t paged_attention_workspace_bytes(int64_t n_rows, int n_seq, int H, int rank, int rope, int nope, int v_dim, int page_log,
-                                       int dtype, int num_cus) {
+size_t paged_attention_workspace_bytes(int64_t n_rows, int n_seq, int H, int rank, int rope, int nope, int v_dim, int width,
+                                       int page_log, int dtype, int num_cus) {
     const int rows = fast_rows(n_rows, n_seq, H);
+    const int64_t capacity = (int64_t)width << page_log;
+    if (is_fast(rank, rope, nope, v_dim, page_log, dtype) && is_chunk(n_rows, n_seq, H, nope, v_dim, capacity))
+        return chunk_layout(n_rows, n_seq, H, capacity, chunk_groups(num_cus)).bytes;
     if (is_fast(rank, rope, nope, v_dim, page_log, dtype)) return layout(n_rows, n_seq, H, kWidth, rows, fast_groups(rows, num_cus), 2, kRank).bytes;
     return layout(n_rows, n_seq, H, rank + rope, kAnyRows, any_groups(num_cus), 4, rank).bytes;
 }
 
 int launch_paged_attention(const void* q, const void* w, const void* pool, const Batch& b, const float* rates, int H, int rank, int rope,
                            int nope, int v_dim, int dtype, float scale, void* ws, void* out, int num_cus, hipStream_t stream) {
-    const Shape s = {H, rank, rope, nope, v_dim, 0, 0, scale * kLog2E};
+    const Shape s = {H, rank, rope, nope, v_dim, 0, 0, 1, scale * kLog2E};
+    if (is_fast(rank, rope, nope, v_dim, b.page_log, dtype) &&
+        is_chunk(b.n_rows, b.n_seq, H, nope, v_dim, (int64_t)b.width << b.page_log))
+        return launch_chunk((const uint16_t*)q, (const uint16_t*)w, (const uint16_t*)pool, b, rates, s, (unsigned char*)ws, (uint16_t*)out,
+                            num_cus, stream);
     if (is_fast(rank, rope, nope, v_dim, b.page_log, dtype))
         return launch_fast((const uint16_t*)q, (const uint16_t*)w, (const uint16_t*)pool, b, rates, s, (unsigned char*)ws, (uint16_t*)out,
                            num_cus, stream);

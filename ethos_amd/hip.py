@@ -886,7 +886,8 @@ def paged_attention(q: torch.Tensor, w: torch.Tensor, pool: torch.Tensor, table:
         if out.shape != (n, H * v_dim):
             raise RuntimeError(f"out must be {(n, H * v_dim)}, got {tuple(out.shape)}")
     lib, code = load(), dtype_code(q.dtype)
-    ws, ws_bytes = _scratch("ethos_paged_attention_workspace_bytes", q.device, n, n_seq, H, rank, rope, nope, v_dim, pool.shape[1], code)
+    ws, ws_bytes = _scratch("ethos_paged_attention_workspace_bytes", q.device, n, n_seq, H, rank, rope, nope, v_dim, width, pool.shape[1],
+                           code)
     rc = lib.ethos_paged_attention(q.data_ptr(), w.data_ptr(), pool.data_ptr(), table.data_ptr(), ld, width, lens.data_ptr(), starts.data_ptr(),
                                    rates.data_ptr(), n, n_seq, H, rank, rope, nope, v_dim, pool.shape[0], pool.shape[1], code, float(scale),
                                    ws.data_ptr(), ws_bytes, out.data_ptr(), _stream())

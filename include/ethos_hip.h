@@ -630,7 +630,7 @@ int ethos_latent_append(const void* rows, int64_t ld, const void* gain, const fl
  * q, w, pool, workspace and out 16-byte aligned; scale positive.
  */
 size_t ethos_paged_attention_workspace_bytes(int64_t n_rows, int32_t n_seq, int32_t n_heads, int32_t rank, int32_t rope, int32_t nope,
-                                             int32_t v_dim, int32_t page, int32_t dtype);
+                                             int32_t v_dim, int32_t table_width, int32_t page, int32_t dtype);
 int ethos_paged_attention(const void* q, const void* w, const void* pool, const int32_t* table, int64_t table_ld, int32_t table_width,
                           const int32_t* lens, const int32_t* starts, const float* rates, int64_t n_rows, int32_t n_seq, int32_t n_heads,
                           int32_t rank, int32_t rope, int32_t nope, int32_t v_dim, int64_t n_pages, int32_t page, int32_t dtype, float scale,

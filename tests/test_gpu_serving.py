@@ -256,6 +256,71 @@ def test_attention_sees_nothing_behind_a_token(dt, rank):
             assert bool(got[hit].isnan().all()), (cut, value, i)
 
 
+def test_many_new_tokens_see_nothing_behind_them():
+    """The same where keys and values are formed first."""
+    lens, new = [450, 200, 1000], [300, 200, 131]
+    c = _case(lens, new, 3, 256, 64, 64, 64, 32, "bf16", seed=13)
+    want = _attend(c)
+    _near(want, c)
+    flat = c["pool"].view(-1, 320)
+    starts = c["starts"].tolist()
+    for cut, value in ((5, math.nan), (1, math.inf), (100, -math.inf)):
+        for i in range(3):
+            spoiled = _slots(c["table"], i, torch.arange(lens[i] - cut, lens[i], device="cuda"), 32)
+            keep = flat[spoiled].clone()
+            flat[spoiled] = value
+            got = _attend(c)
+            flat[spoiled] = keep
+            hit = torch.zeros(len(got), dtype=torch.bool, device="cuda")
+            hit[starts[i + 1] - cut:starts[i + 1]] = True
+            assert torch.equal(got[~hit], want[~hit]), (cut, value, i)
+            assert bool(got[hit].isnan().all()), (cut, value, i)
+
+
+def test_many_new_tokens_of_batches_that_do_not_fit():
+    c = _case([400, 333, 150], [200, 150, 140], 4, 256, 64, 64, 64, 16, "bf16", seed=14)
+    good = _attend(c)
+    out = torch.full((500, 256), 5.0, dtype=torch.bfloat16, device="cuda")
+    c["q"] = torch.cat((c["q"], c["q"][:10] * math.nan))
+    got = _attend(c, out=out)
+    assert torch.equal(got[:490], good) and bool((got[490:] == 5.0).all())
+    table = c["table"].clone()
+    c["table"] = table.clone()
+    c["table"][1, 15] = 10 ** 8  # positions 240 to 255, the first of them seen by all but 57 of the new tokens
+    got = _attend(c)
+    assert bool(got[200 + 57:350].isnan().all()) and torch.equal(got[:257], good[:257]) and torch.equal(got[350:490], good[350:])
+    c["table"] = table
+    for length in (16 * table.shape[1] + 1, 2 ** 31 - 1, 2 ** 30 + 1, -1, -2 ** 31):
+        c["lens"] = i32([400, length, 150])
+        got = _attend(c)
+        assert bool(got[200:350].isnan().all()) and torch.equal(got[:200], good[:200]) and torch.equal(got[350:490], good[350:]), length
+    c["lens"] = i32([400, 3, 150])  # three positions: the first 147 tokens see none
+    got = _attend(c)
+    assert float(got[200:347].float().abs().sum()) == 0.0 and not bool(got[347:350].isnan().any()) and bool((got[347:350] != 0).any())
+    assert torch.equal(got[350:490], good[350:])
+    c["lens"] = i32([400, 333, 150])
+    c["starts"] = i32([0, 200, 350, 4000])
+    got = _attend(c)
+    assert torch.equal(got[:350], good[:350]) and bool(got[350:].isnan().all())
+    c["starts"] = i32([0, 490, 0, 490])  # sequences that overlap
+    _attend(c)
+    c["starts"] = i32([0, 0, 0, 140])
+    c["q"], c["lens"] = c["q"][350:], i32([400, 333, 150])
+    out = torch.full((150, 256), 5.0, dtype=torch.bfloat16, device="cuda")
+    got = _attend(c, out=out)
+    assert bool((got[140:] == 5.0).all())
+    _near(got, c, "50 tokens a sequence on the average")  # (fewer than the form of `good` is for)
+
+
+@pytest.mark.parametrize("lens,new,H,page", [([128], [128], 1, 8), ([129], [129], 5, 64), ([5000], [128], 2, 64), ([300, 300, 300], [129, 254, 1], 16, 16),
+                                             ([2000, 700], [1100, 511], 8, 512), ([600, 1, 90], [600, 1, 0], 7, 8)])
+def test_many_new_tokens_against_float64(lens, new, H, page):
+    c = _case(lens, new, H, 256, 64, 64, 64, page, "bf16", seed=sum(new))
+    got = _attend(c)
+    _near(got, c, f"{lens} {new}")
+    assert torch.equal(_attend(c), got)
+
+
 @pytest.mark.parametrize("dt,rank", [("bf16", 256), ("bf16", 64), ("fp32", 64)])
 def test_attention_of_batches_that_do_not_fit(dt, rank):
     c = _case([70, 33, 100, 20], [3, 2, 4, 2], 4, rank, 64, 64, 64, 16, dt, seed=4)
@@ -348,10 +413,11 @@ def test_attention_under_large_scores(dt):
     assert not bool(((got.double() - want).abs() > bound)[sure].any())
 
 
-@pytest.mark.parametrize("new", [1, 6, 70])
-def test_attention_in_streams_and_graphs(new):
-    a = _case([900, 333, 64], [new, 1, new], 16, 256, 64, 64, 64, 64, "bf16", seed=8)
-    b = _case([64, 2000, 90], [new, 1, new], 16, 256, 64, 64, 64, 64, "bf16", seed=9)
+@pytest.mark.parametrize("new", [1, 6, 64])
+@pytest.mark.parametrize("middle", [1, 333])
+def test_attention_in_streams_and_graphs(new, middle):
+    a = _case([900, 333, 64], [new, middle, new], 16, 256, 64, 64, 64, 64, "bf16", seed=8)
+    b = _case([64, 2000, 90], [new, middle, new], 16, 256, 64, 64, 64, 64, "bf16", seed=9)
     want = [_attend(a), _attend(b)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]

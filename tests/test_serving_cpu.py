@@ -50,11 +50,11 @@ def test_paged_attention_argument_errors_are_codes():
         assert attend(**{name: None}) == -3, name
     for name in ("q", "w", "pool", "ws", "out"):
         assert attend(**{name: 8}) == -4, name
-    need = L.ethos_paged_attention_workspace_bytes(3, 2, 16, 256, 64, 64, 64, 64, 1)
+    need = L.ethos_paged_attention_workspace_bytes(3, 2, 16, 256, 64, 64, 64, 4, 64, 1)
     assert need > 0 and attend(ws_bytes=need - 1) == -5
     assert attend(n=0, q=None) == 0 and attend(n_seq=0, ws=None) == 0
-    assert L.ethos_paged_attention_workspace_bytes(3, 2, 16, 256, 64, 64, 64, 64, 9) == 256
-    assert L.ethos_paged_attention_workspace_bytes(-3, 2, 16, 256, 64, 64, 64, 64, 1) == 256
+    assert L.ethos_paged_attention_workspace_bytes(3, 2, 16, 256, 64, 64, 64, 4, 64, 9) == 256
+    assert L.ethos_paged_attention_workspace_bytes(-3, 2, 16, 256, 64, 64, 64, 4, 64, 1) == 256
 
 
 def test_copy_pages_argument_errors_are_codes():
