@@ -13,6 +13,8 @@
 //
 // Without bounds of the host on lengths, tables or starts: what they hold is checked where it is used.  A page
 // outside the cache reads as a row of NaN, a length beyond the table makes its sequence's outputs NaN.
+#include <type_traits>
+
 #include "ethos_launch.hpp"
 #include "ethos_mfma.hpp"
 #include "ethos_rows.hpp"
@@ -431,6 +433,19 @@ template <int N>
 __device__ __forceinline__ void copies_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// The order of a stretch of code between branches: N LDS reads, then M times a matrix product and R reads, then the
+// last products (left to itself the compiler reads one fragment ahead, and every product waits for LDS).
+template <int N, int M, int R, int L>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, N, 0);
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, L, 0);
+}
+
 // Block 0: the plan and the two special rows.  The others: 32 tokens of a head; [c][token] = W_k,h^T q^T, the weight
 // (k as the row) through LDS in the layout of the loss's R tiles.
 __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ w,
@@ -638,6 +653,7 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
                     const bf16x8_t a = *(lds_frag_ptr)(size_t)(at + k_at[st & 1] + (st >> 1) * kPlane + i * 16 * 128);
                     x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, fq[st].f, x[i], 0, 0, 0);
                 }
+            reads_ahead<8, KB * kWidth / 32 - 8, 1, 8>();
             if (key0 + 16 * KB - 1 > wave_pos) {
 #pragma unroll
                 for (int i = 0; i < KB; ++i)
@@ -695,6 +711,7 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
                     a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(c + 16 * 128));
                     o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.f, p[i].f, o[d], 0, 0, 0);
                 }
+            reads_ahead<12, 16 * KB / 2 - 6, 2, 6>();
         }
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
@@ -893,7 +910,7 @@ constexpr int kChunkRows = 128;   // new tokens a sequence, on the average, from
 constexpr size_t kChunkBytes = (size_t)1 << 30;  // of keys and values, at most
 
 struct ChunkLayout {
-    size_t plan, items, seq_item, tok_seq, seq_keys, turns, keys, shared, sums, stats, bytes;
+    size_t plan, items, seq_item, tok_seq, seq_keys, specials, turns, keys, shared, sums, stats, bytes;
     int64_t max_items, key_rows;
 };
 
@@ -912,6 +929,7 @@ ChunkLayout chunk_layout(int64_t n_rows, int n_seq, int H, int64_t capacity, int
     l.seq_item = take((size_t)n_seq * 4);
     l.tok_seq = take((size_t)n_rows * 4);
     l.seq_keys = take((size_t)(n_seq + 1) * 4);
+    l.specials = take((size_t)16 * kWidth * 2);
     l.turns = take((size_t)n_rows * kRope / 2 * 8);
     l.keys = take((size_t)l.key_rows * H * 2 * kHead * 2);
     l.shared = take((size_t)l.key_rows * kRope * 2);
@@ -925,8 +943,9 @@ ChunkLayout chunk_layout(int64_t n_rows, int n_seq, int H, int64_t capacity, int
 // Block 0: the plan.  The others: eight tokens' sequences, cosines and sines.
 __global__ __launch_bounds__(256) void chunk_prepare_kernel(const float* __restrict__ rates, Batch b, Shape s, int64_t max_items, Plan* plan,
                                                             Item* items, int32_t* seq_item, int32_t* seq_keys, int32_t* tok_seq,
-                                                            float2* __restrict__ turns) {
+                                                            uint16_t* __restrict__ specials, float2* __restrict__ turns) {
     if (blockIdx.x == 0) {
+        for (int e = threadIdx.x; e < 2 * kBlock * kWidth; e += 256) specials[e] = e < kBlock * kWidth ? 0 : 0x7fc0;
         Shape one = s;
         one.H = 1;
         make_plan<256>(b, one, max_items, plan, items, seq_item, seq_keys, threadIdx.x);
@@ -943,76 +962,99 @@ __global__ __launch_bounds__(256) void chunk_prepare_kernel(const float* __restr
     turns[t * 32 + p] = c;
 }
 
-// Keys and values of 64 cached rows for four heads: [column][row] = W_h c^T, a wave 32 of a head's 128 columns; the
-// weight's fragments from memory, the rows from LDS in the planes of above.  Workgroups go round (64 rows, heads).
-__global__ __launch_bounds__(256) void expand_kernel(const uint16_t* __restrict__ w, const uint16_t* __restrict__ pool, Batch b, Shape s,
-                                                     const int32_t* __restrict__ seq_keys, int64_t key_rows, uint16_t* __restrict__ keys,
-                                                     uint16_t* __restrict__ shared) {
-    __shared__ __align__(16) unsigned char rows[kRank / 64 * kPlane];
+// Keys and values of a head for some tiles of 64 cached rows: [column][row] = W_h c^T, a wave 32 of the
+// head's 128 columns, the weight's fragments in registers, the rows from LDS in the planes of above, the next tile's on
+// their way.  Workgroups go round the heads; the rotated keys, which are copied, are each tile's one head's.
+__global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restrict__ w, const uint16_t* __restrict__ pool, Batch b, Shape s,
+                                                        const int32_t* __restrict__ seq_keys, const uint16_t* __restrict__ specials,
+                                                        int64_t key_rows, uint16_t* __restrict__ keys, uint16_t* __restrict__ shared) {
+    __shared__ __align__(16) unsigned char ring[2 * kStage];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t lds = lds_addr(rows);
-    const int parts = (s.H + 3) / 4;
-    const int64_t work = (int64_t)seq_keys[b.n_seq] * parts;
-    for (int64_t u = blockIdx.x; u < work; u += gridDim.x) {
-        const int tile = (int)(u / parts), h0 = (int)(u % parts) * 4;
-        int lo = 0, hi = b.n_seq;  // the last sequence whose tiles begin at or before this one
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (seq_keys[mid] <= tile) lo = mid;
+    const uint32_t lds = lds_addr(ring);
+    const int h = blockIdx.x % s.H, step = gridDim.x / s.H;
+    typedef const __attribute__((address_space(4))) int32_t* const_ptr;
+    const const_ptr first = (const_ptr)(uintptr_t)seq_keys;
+    const int total = first[b.n_seq];
+    int tile = blockIdx.x / s.H;
+    if (tile >= total) return;
+
+    int seq = 0;
+    auto copy_tile = [&](int u, int stage) {
+        int hi = b.n_seq;  // the last sequence whose tiles begin at or before this one (not before that of the last tile)
+        while (hi - seq > 1) {
+            const int mid = (seq + hi) >> 1;
+            if (first[mid] <= u) seq = mid;
             else hi = mid;
         }
-        const int key0 = (tile - seq_keys[lo]) * kKeys, len = b.lens[lo];
-        // a thread's pieces: 10 of 64 rows of 40
-        for (int e = tid; e < kKeys * (kWidth / 8); e += 256) {
-            const int r = e / (kWidth / 8), c = e - r * (kWidth / 8), p = key0 + r;
-            u32x4_t v = {0, 0, 0, 0};
-            if (p < len) {
-                const int32_t page = batch_page(b, lo, p);
-                if (page >= 0)
-                    v = *reinterpret_cast<const u32x4_t*>(pool + (((int64_t)page << b.page_log) + (p & ((1 << b.page_log) - 1))) * kWidth + c * 8);
-                else
-                    v = u32x4_t{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+        const int key0 = (u - first[seq]) * kKeys, end = ((const_ptr)(uintptr_t)b.lens)[seq];
+        const const_ptr table = (const_ptr)(uintptr_t)(b.table + seq * b.table_ld);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int blk = 2 * wave + i, p0 = key0 + blk * kBlock, at = p0 >> b.page_log, row = lane >> 3;
+            const int32_t page = table[at < b.width ? at : b.width - 1];
+            const uint16_t* from = page >= 0 && page < b.n_pages
+                                       ? pool + (((int64_t)page << b.page_log) + (p0 & ((1 << b.page_log) - 1))) * kWidth
+                                       : specials + kBlock * kWidth;
+            const uint32_t off = row * (kWidth * 2) + (((lane & 7) ^ swizzle(blk * kBlock + row)) << 4);
+            const unsigned char* mine = (const unsigned char*)(p0 + row < end ? from : specials) + off;
+            const uint32_t to_lds = lds + stage * kStage + blk * 1024;
+#pragma unroll
+            for (int pl = 0; pl < kWidth / 64; ++pl)
+                if (pl < kRank / 64 || u % s.H == h) copy16(mine + pl * 128, __builtin_amdgcn_readfirstlane(to_lds + pl * kPlane));
+        }
+    };
+    copy_tile(tile, 0);
+    bf16x8_t a[kRank / 16];
+    {
+        const uint16_t* wh = w + ((int64_t)h * 2 * kHead + wave * 32 + (lane & 31)) * kRank + 8 * half;
+#pragma unroll
+        for (int st = 0; st < kRank / 16; ++st) a[st] = *reinterpret_cast<const bf16x8_t*>(wh + 16 * st);
+#pragma unroll
+        for (int st = 0; st < kRank / 16; ++st) asm volatile("" : "+v"(a[st]));
+    }
+    int stage = 0;
+    for (bool started = false; tile < total; tile += step, stage ^= 1, started = true) {
+        // (behind this tile's copies are only the last tile's stores, 8 or more)
+        if (started) copies_barrier<8>();
+        else copies_barrier<0>();
+        if (tile + step < total) copy_tile(tile + step, stage ^ 1);
+        const uint32_t at = lds + stage * kStage;
+        f32x16_t acc[2] = {f32x16_zero(), f32x16_zero()};
+#pragma unroll
+        for (int st = 0; st < kRank / 16; ++st)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 32 * i + (lane & 31);
+                const bf16x8_t x = *(lds_frag_ptr)(size_t)(at + (st >> 2) * kPlane + r * 128 + (((2 * (st & 3) + half) ^ swizzle(r)) << 4));
+                acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[st], x, acc[i], 0, 0, 0);
             }
-            if (c < kRank / 8) *(lds_u4_ptr)(size_t)(lds + (c >> 3) * kPlane + r * 128 + (((c & 7) ^ swizzle(r)) << 4)) = v;
-            else if (h0 == 0) *reinterpret_cast<u32x4_t*>(shared + ((int64_t)tile * kKeys + r) * kRope + (c - kRank / 8) * 8) = v;
+        uint16_t* to = keys + ((int64_t)h * key_rows + (int64_t)tile * kKeys + (lane & 31)) * (2 * kHead) + wave * 32 + 4 * half;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<uint2*>(to + i * 32 * 2 * kHead + 2 * e) =
+                    make_uint2(pack_bf16x2(acc[i][e], acc[i][e + 1]), pack_bf16x2(acc[i][e + 2], acc[i][e + 3]));
+        if (tile % s.H == h) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 32 * i + (tid >> 3), c = tid & 7;
+                *reinterpret_cast<u32x4_t*>(shared + ((int64_t)tile * kKeys + r) * kRope + c * 8) =
+                    *(lds_u4_ptr)(size_t)(at + kRank / 64 * kPlane + r * 128 + ((c ^ swizzle(r)) << 4));
+            }
         }
-        __syncthreads();
-        for (int h = h0; h < h0 + 4 && h < s.H; ++h) {
-            const uint16_t* wh = w + ((int64_t)h * 2 * kHead + wave * 32 + (lane & 31)) * kRank + 8 * half;
-            f32x16_t acc[2] = {f32x16_zero(), f32x16_zero()};
-            bf16x8_t a[kRank / 16];
-#pragma unroll
-            for (int st = 0; st < kRank / 16; ++st) a[st] = *reinterpret_cast<const bf16x8_t*>(wh + 16 * st);
-#pragma unroll
-            for (int st = 0; st < kRank / 16; ++st)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = 32 * i + (lane & 31);
-                    const bf16x8_t x = *(lds_frag_ptr)(size_t)(lds + (st >> 2) * kPlane + r * 128 + (((2 * (st & 3) + half) ^ swizzle(r)) << 4));
-                    acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[st], x, acc[i], 0, 0, 0);
-                }
-            uint16_t* to = keys + ((int64_t)h * key_rows + (int64_t)tile * kKeys + (lane & 31)) * (2 * kHead) + wave * 32 + 4 * half;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                    *reinterpret_cast<uint2*>(to + i * 32 * 2 * kHead + 2 * e) =
-                        make_uint2(pack_bf16x2(acc[i][e], acc[i][e + 1]), pack_bf16x2(acc[i][e + 2], acc[i][e + 3]));
-        }
-        __syncthreads();
     }
 }
 
 // A step's LDS: three planes of 64 rows, keys, rotated keys, values.
 constexpr int kChunkStage = 3 * kPlane;
-template <int S, int WGS>
-__global__ __launch_bounds__(256, WGS) void chunk_attend_kernel(const uint16_t* __restrict__ q, const float2* __restrict__ turns,
+__global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __restrict__ q, const float2* __restrict__ turns,
                                                               const uint16_t* __restrict__ keys, const uint16_t* __restrict__ shared, Shape s,
                                                               const Plan* plan, const Item* __restrict__ items,
                                                               const int32_t* __restrict__ seq_keys, int64_t key_rows, float* __restrict__ sums,
                                                               float2* __restrict__ stats, uint16_t* __restrict__ out) {
-    __shared__ __align__(16) unsigned char ring[S * kChunkStage];
+    __shared__ __align__(16) unsigned char ring[3 * kChunkStage];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lds = lds_addr(ring);
@@ -1072,9 +1114,8 @@ __global__ __launch_bounds__(256, WGS) void chunk_attend_kernel(const uint16_t* 
                 else copy16(kv + at * (4 * kHead) + (pl == 2 ? 2 * kHead : 0), key_off[i & 1], to_lds);
             }
         };
-#pragma unroll
-        for (int i = 0; i < S - 1; ++i)
-            if (k_begin + i < k_end) copy_step(k_begin + i, i);
+        copy_step(k_begin, 0);
+        if (k_begin + 1 < k_end) copy_step(k_begin + 1, 1);
         Frag fq[8];
         {
             const uint16_t* qp = q + (row * s.H + h) * (kHead + kRope) + 8 * half;
@@ -1095,61 +1136,52 @@ __global__ __launch_bounds__(256, WGS) void chunk_attend_kernel(const uint16_t* 
 #pragma unroll
             for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(fq[i].u));
         }
-        f32x16_t o[2] = {f32x16_zero(), f32x16_zero()};
+        f32x16_t o[2] = {f32x16_zero(), f32x16_zero()}, x[2], y[2];
         float shift = kLowest, l = 0.0f;
-        int stage = 0;
-        for (int k = k_begin; k < k_end; ++k) {
-            if (S == 3 && k + 1 < k_end) copies_barrier<6 * (S - 2)>();
-            else copies_barrier<0>();
-            if (k + S - 1 < k_end) copy_step(k + S - 1, stage == 0 ? S - 1 : stage - 1);
-            const uint32_t at = lds + stage * kChunkStage;
-            const int key0 = k * kKeys;
-            stage = stage == S - 1 ? 0 : stage + 1;
-            uint64_t odd = 0;  // rows that some tokens do not see, and whose values are not finite
-            if (key0 + kKeys - 1 > first_pos) {
-                bool bad = false;
+        auto scores = [&](f32x16_t (&z)[2], uint32_t at) {
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const u32x4_t v = *(lds_u4_ptr)(size_t)(at + 2 * kPlane + lane * 128 + (((c + (lane >> 1)) & 7) << 4));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
-                }
-                odd = ballot(bad);
-            }
-            f32x16_t x[2] = {f32x16_zero(), f32x16_zero()};
+            for (int i = 0; i < 2; ++i) z[i] = f32x16_zero();
 #pragma unroll
             for (int st = 0; st < 8; ++st)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const bf16x8_t a = *(lds_frag_ptr)(size_t)(at + k_at[st & 3] + (st >> 2) * kPlane + i * 32 * 128);
-                    x[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, fq[st].f, x[i], 0, 0, 0);
+                    z[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, fq[st].f, z[i], 0, 0, 0);
                 }
-            if (key0 + kKeys - 1 > wave_pos) {
+        };
+        // What the wave's tokens do not see of step k, in LDS at `at`: its scores; and rows whose values are not finite.
+        auto mask = [&](f32x16_t (&z)[2], int k, uint32_t at) {
+            const int sees = my_pos - k * kKeys - 4 * half;  // (a lane's keys are 4 half and a constant each)
+            bool bad = false;
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                const u32x4_t v = *(lds_u4_ptr)(size_t)(at + 2 * kPlane + lane * 128 + (((c + (lane >> 1)) & 7) << 4));
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[i][e] = key0 + 32 * i + mfma32_row(e, lane) > my_pos ? -INFINITY : x[i][e];
+                for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
             }
-            if (odd != 0) {
+            const uint64_t odd = ballot(bad);
+            if (odd != 0) {  // no result for a token that sees one of them, zeros for the others
+                const uint64_t mine = odd >> (4 * half);
+                uint64_t seen = 0;
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int key = 32 * i + mfma32_row(e, lane);
-                        if ((odd >> key & 1) && key0 + key <= my_pos) l = NAN;
-                    }
+                for (int e = 0; e < 32; ++e) {
+                    const int key = 32 * (e >> 4) + 8 * ((e & 15) >> 2) + (e & 3);
+                    seen |= key <= sees ? mine & (1ull << key) : 0;
+                }
+                if (seen != 0) l = NAN;
                 lds_barrier();
                 for (int e = tid; e < kKeys * 8; e += 256)
                     if (odd >> (e >> 3) & 1) *(lds_u4_ptr)(size_t)(at + 2 * kPlane + e * 16) = u32x4_t{0, 0, 0, 0};
                 lds_barrier();
             }
-            float top = x[0][0];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[i][e]);
+                for (int e = 0; e < 16; ++e) z[i][e] = 32 * i + 8 * (e >> 2) + (e & 3) > sees ? -INFINITY : z[i][e];
+        };
+        auto new_top = [&](float top) {
             top = fmaxf(top, __shfl_xor(top, 32, 64)) * s.scale2;
-            if (ballot(top > shift) != 0) {
+            if (ballot(top > shift) != 0) {  // some token has a new maximum
                 const float was = shift;
                 shift = fmaxf(shift, top);
                 const float r = __builtin_amdgcn_exp2f(was - shift);
@@ -1159,25 +1191,94 @@ __global__ __launch_bounds__(256, WGS) void chunk_attend_kernel(const uint16_t* 
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[i][e] *= r;
             }
-            Frag p[4];
+        };
+        // Step k on its scores x, whose maximum is known; with `more`, the scores y of step k + 1 beside it.  In this
+        // order: two products of y beside the exponentials of four of x, eight times; then the products with the values
+        // beside the maximum of y.  (The fences keep it: by itself the compiler puts the exponentials first.)
+        auto run_step = [&](auto more, f32x16_t (&x)[2], f32x16_t (&y)[2], int k, int stage) {
+            const int next = stage == 2 ? 0 : stage + 1;
+            if constexpr (more) {
+                copies_barrier<0>();
+                if (k + 2 < k_end) copy_step(k + 2, next == 2 ? 0 : next + 1);
+            }
+            const uint32_t at = lds + stage * kChunkStage, to = lds + next * kChunkStage;
+            Frag p[4], fv[4][2];
+            bf16x8_t fk[8][2];
+            auto read_keys = [&](int st) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) fk[st][i] = *(lds_frag_ptr)(size_t)(to + k_at[st & 3] + (st >> 2) * kPlane + i * 32 * 128);
+            };
+            if constexpr (more) {
+                read_keys(0);
+                read_keys(1);
+                y[0] = f32x16_zero();
+                y[1] = f32x16_zero();
+            }
+#pragma unroll
+            for (int st = 0; st < 8; ++st) {
+                if constexpr (more) {
+                    if (st + 2 < 8) read_keys(st + 2);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) y[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk[st][i], fq[st].f, y[i], 0, 0, 0);
+                }
+                if (st >= 4) {
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        fv[st - 4][d].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(at + v_at[0][d] + (st - 4) * 16 * 128));
+                        fv[st - 4][d].h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(at + v_at[1][d] + (st - 4) * 16 * 128));
+                    }
+                }
+                float e[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[st >> 2][4 * (st & 3) + j], s.scale2, -shift));
+                l += (e[0] + e[1]) + (e[2] + e[3]);
+                p[st >> 1].w[2 * (st & 1)] = pack_bf16x2(e[0], e[1]);
+                p[st >> 1].w[2 * (st & 1) + 1] = pack_bf16x2(e[2], e[3]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (more)
+                if ((k + 1) * kKeys + kKeys - 1 > first_pos) mask(y, k + 1, to);
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv[i][d].f, p[i].f, o[d], 0, 0, 0);
+                    if constexpr (more) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) top = fmaxf(top, y[i >> 1][8 * (i & 1) + 4 * d + e]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if constexpr (more) new_top(top);
+        };
+        if (k_begin + 1 < k_end) copies_barrier<6>();
+        else copies_barrier<0>();
+        {
+            scores(x, lds);
+            if (k_begin * kKeys + kKeys - 1 > first_pos) mask(x, k_begin, lds);
+            float top = x[0][0];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], s.scale2, -shift));
-                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e + 1], s.scale2, -shift));
-                    l += e0 + e1;
-                    p[2 * i + e / 8].w[e % 8 / 2] = pack_bf16x2(e0, e1);
-                }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    Frag a;
-                    a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(at + v_at[0][d] + i * 16 * 128));
-                    a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(at + v_at[1][d] + i * 16 * 128));
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f, p[i].f, o[d], 0, 0, 0);
-                }
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[i][e]);
+            new_top(top);
+        }
+        int k = k_begin, stage = 0;
+        constexpr std::integral_constant<bool, true> more{};
+        constexpr std::integral_constant<bool, false> none{};
+        for (; k + 2 < k_end; k += 2) {
+            run_step(more, x, y, k, stage);
+            stage = stage == 2 ? 0 : stage + 1;
+            run_step(more, y, x, k + 1, stage);
+            stage = stage == 2 ? 0 : stage + 1;
+        }
+        if (k + 1 < k_end) {
+            run_step(more, x, y, k, stage);
+            run_step(none, y, x, k + 1, stage == 2 ? 0 : stage + 1);
+        } else {
+            run_step(none, x, y, k, stage);
         }
         l += __shfl_xor(l, 32, 64);
         lds_barrier();
@@ -1238,8 +1339,7 @@ bool is_chunk(int64_t n_rows, int n_seq, int H, int nope, int v_dim, int64_t cap
     return nope == kHead && v_dim == kHead && n_rows >= (int64_t)kChunkRows * n_seq &&
            (size_t)n_seq * (size_t)(capacity + kKeys) <= kChunkBytes / (size_t)(H * 4 * kHead);
 }
-constexpr int kChunkGroups = 2;  // workgroups a CU
-int chunk_groups(int num_cus) { return kChunkGroups * num_cus; }
+int chunk_groups(int num_cus) { return 2 * num_cus; }  // two workgroups a CU
 
 int launch_chunk(const uint16_t* q, const uint16_t* w, const uint16_t* pool, const Batch& b, const float* rates, Shape s, unsigned char* ws,
                  uint16_t* out, int num_cus, hipStream_t stream) {
@@ -1251,12 +1351,13 @@ int launch_chunk(const uint16_t* q, const uint16_t* w, const uint16_t* pool, con
     Item* items = (Item*)(ws + l.items);
     int32_t *seq_item = (int32_t*)(ws + l.seq_item), *tok_seq = (int32_t*)(ws + l.tok_seq), *seq_keys = (int32_t*)(ws + l.seq_keys);
     float2 *turns = (float2*)(ws + l.turns), *stats = (float2*)(ws + l.stats);
-    uint16_t *keys = (uint16_t*)(ws + l.keys), *shared = (uint16_t*)(ws + l.shared);
+    uint16_t *specials = (uint16_t*)(ws + l.specials), *keys = (uint16_t*)(ws + l.keys), *shared = (uint16_t*)(ws + l.shared);
     float* sums = (float*)(ws + l.sums);
     hipLaunchKernelGGL(chunk_prepare_kernel, dim3((unsigned)((b.n_rows + 7) / 8 + 1)), dim3(256), 0, stream, rates, b, s, l.max_items, plan, items,
-                       seq_item, seq_keys, tok_seq, turns);
-    hipLaunchKernelGGL(expand_kernel, dim3((unsigned)(4 * num_cus)), dim3(256), 0, stream, w, pool, b, s, seq_keys, l.key_rows, keys, shared);
-    hipLaunchKernelGGL((chunk_attend_kernel<3, kChunkGroups>), dim3((unsigned)s.groups), dim3(256), 0, stream, q, turns, keys, shared, s, plan, items, seq_keys,
+                       seq_item, seq_keys, tok_seq, specials, turns);
+    hipLaunchKernelGGL(expand_kernel, dim3((unsigned)((2 * num_cus + s.H - 1) / s.H * s.H)), dim3(256), 0, stream, w, pool, b, s, seq_keys, specials,
+                       l.key_rows, keys, shared);
+    hipLaunchKernelGGL(chunk_attend_kernel, dim3((unsigned)s.groups), dim3(256), 0, stream, q, turns, keys, shared, s, plan, items, seq_keys,
                        l.key_rows, sums, stats, out);
     hipLaunchKernelGGL(chunk_finish_kernel, dim3((unsigned)((b.n_rows * s.H + 15) / 16)), dim3(256), 0, stream, b, s, plan, items, seq_item,
                        tok_seq, sums, stats, out);
