@@ -31,8 +31,9 @@ constexpr int32_t kLongest = 1 << 30;  // a sequence's length, at most
 // A tile of rows: `rows` of sequence seq from its row `row0` (token row0 / H, head row0 % H) on; the first new
 // token of the sequence is row tok0 of the batch, at position pos0.
 struct Item {
-    int32_t seq, row0, rows, tok0, pos0, pad;
-    int64_t end;  // tiles of work up to this one's last, all before it included
+    int32_t seq, row0, rows, tok0, pos0;
+    int32_t keys;  // tile of the sequence's first key, if all sequences' keys are laid out one after the other
+    int64_t end;   // tiles of work up to this one's last, all before it included
 };
 
 struct Plan {
@@ -112,14 +113,14 @@ template <int NT>
 __device__ void make_plan(const Batch& b, const Shape& s, int64_t max_items, Plan* plan, Item* items, int32_t* seq_item, int32_t* seq_keys,
                           int tid) {
     __shared__ int64_t lds[NT / 64];
-    __shared__ int32_t ends[NT], counts[NT], tok0[NT], lens[NT];
+    __shared__ int32_t ends[NT], counts[NT], tok0[NT], lens[NT], keys[NT];
     int64_t base = 0, tiles = 0, key_tiles = 0, total;
     for (int at = 0; at < b.n_seq; at += NT) {
         const int i = at + tid;
         if (seq_keys) {  // where each sequence's keys begin, if all are laid out one after the other
             const int64_t n = i < b.n_seq && new_tokens(b, i) > 0 && fits(b, i) ? (b.lens[i] + kKeys - 1) / kKeys : 0;
             const int64_t end = key_tiles + block_scan<NT>(n, lds, tid, total);
-            if (i < b.n_seq) seq_keys[i] = (int32_t)(end - n);
+            if (i < b.n_seq) seq_keys[i] = keys[tid] = (int32_t)(end - n);
             key_tiles += total;
         }
         const int64_t count = i < b.n_seq ? new_tokens(b, i) : 0, n = (count * s.H + s.rows - 1) / s.rows;
@@ -145,6 +146,7 @@ __device__ void make_plan(const Batch& b, const Shape& s, int64_t max_items, Pla
                 it.rows = left < s.rows ? left : s.rows;
                 it.tok0 = tok0[lo];
                 it.pos0 = lens[lo] - counts[lo];
+                it.keys = seq_keys ? keys[lo] : 0;
                 // keys up to the last row's own
                 const int64_t keys = (int64_t)it.pos0 + (it.row0 + it.rows - 1) / s.H + 1;
                 work = lens[lo] >= 0 && keys > 0 ? (keys + kKeys - 1) / kKeys : 0;
@@ -972,11 +974,12 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restri
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lds = lds_addr(ring);
-    const int h = blockIdx.x % s.H, step = gridDim.x / s.H;
+    // workgroups go round the eight XCDs: those of one take every eighth tile, each for all heads
+    const int round = blockIdx.x / 8, h = round % s.H, step = gridDim.x / s.H;
     typedef const __attribute__((address_space(4))) int32_t* const_ptr;
     const const_ptr first = (const_ptr)(uintptr_t)seq_keys;
     const int total = first[b.n_seq];
-    int tile = blockIdx.x / s.H;
+    int tile = round / s.H * 8 + blockIdx.x % 8;
     if (tile >= total) return;
 
     int seq = 0;
@@ -1047,14 +1050,32 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restri
     }
 }
 
-// A step's LDS: three planes of 64 rows, keys, rotated keys, values.
-constexpr int kChunkStage = 3 * kPlane;
+// A step's LDS: two planes of 64 rows for the keys and their rotated parts, one for the values.  A step takes the next
+// one's keys and its own values, so each have a ring of three steps of their own: both are copied two steps ahead.
+constexpr int kKeyStage = 2 * kPlane, kValueStage = kPlane, kValues = 3 * kKeyStage;  // (the values' ring behind the keys')
+// How far a row's maximum may grow before its sums are rescaled: exponentials stay below 2^8, of the same precision.
+constexpr float kSlack = 8.0f;
+
+constexpr int kAhead = 2;  // steps of a product that the keys' fragments are read ahead
+
+// The maximum of a lane and the one 32 from it, without a way through LDS.
+__device__ __forceinline__ float halves_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// 16 bytes a lane from base + off into LDS at ring + at + 16 times the lane.
+template <int AT>
+__device__ __forceinline__ void copy16_at(const void* base, uint32_t off, uint32_t ring) {
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(ring), "v"(off), "s"(base), "n"(AT) : "memory", "scc");
+}
+
 __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __restrict__ q, const float2* __restrict__ turns,
                                                               const uint16_t* __restrict__ keys, const uint16_t* __restrict__ shared, Shape s,
-                                                              const Plan* plan, const Item* __restrict__ items,
-                                                              const int32_t* __restrict__ seq_keys, int64_t key_rows, float* __restrict__ sums,
-                                                              float2* __restrict__ stats, uint16_t* __restrict__ out) {
-    __shared__ __align__(16) unsigned char ring[3 * kChunkStage];
+                                                              const Plan* plan, const Item* __restrict__ items, int64_t key_rows,
+                                                              float* __restrict__ sums, float2* __restrict__ stats,
+                                                              uint16_t* __restrict__ out) {
+    __shared__ __align__(16) unsigned char ring[3 * (kKeyStage + kValueStage)];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lds = lds_addr(ring);
@@ -1075,17 +1096,19 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
 #pragma unroll
             for (int d = 0; d < 2; ++d) {
                 const int r = row + 8 * i, c = 4 * d + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-                v_at[i][d] = 2 * kPlane + r * 128 + ((c ^ swizzle(r)) << 4) + (lane & 1) * 8;
+                v_at[i][d] = r * 128 + ((c ^ swizzle(r)) << 4) + (lane & 1) * 8;
             }
     }
-    // a lane's places in a copy of 8 rows, of blocks with an even and an odd number
-    uint32_t key_off[2], shared_off[2];
+    // a lane's places in the copies of the wave's two blocks of 8 rows
+    uint32_t key_off[2], value_off[2], shared_off[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int row = lane >> 3, piece = (lane & 7) ^ swizzle(8 * i + row);
+        const int row = 16 * wave + 8 * i + (lane >> 3), piece = (lane & 7) ^ swizzle(row);
         key_off[i] = row * (4 * kHead) + piece * 16;
+        value_off[i] = key_off[i] + 2 * kHead;
         shared_off[i] = row * (2 * kRope) + piece * 16;
     }
+    const uint32_t to_keys = lds + wave * 2048, to_values = lds + kValues + wave * 2048;
 
     int h = (int)(t / each);
     int item = find_item(items, n_items, t - h * each, lane);
@@ -1095,27 +1118,32 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
         const int64_t before = h * each, begin = before + (item > 0 ? items[item - 1].end : 0), finish = before + it.end;
         const int64_t to = finish < stop ? finish : stop;
         if (to <= t) continue;
-        const int k_begin = (int)(t - begin), k_end = (int)(to - begin);
+        const int k_begin = (int)(t - begin), n = (int)(to - t);  // the first step's number, and the steps
         const int my = wave * 32 + (lane & 31), my_row = my < it.rows ? my : it.rows - 1;
         const int first_pos = it.pos0 + it.row0, my_pos = first_pos + my_row;
-        const int wave_pos = first_pos + (wave * 32 < it.rows ? wave * 32 : it.rows - 1);
         const int64_t row = (int64_t)it.tok0 + it.row0 + my_row;
-        const int64_t key_row = (int64_t)seq_keys[it.seq] * kKeys;
+        const int64_t key_row = ((int64_t)it.keys + k_begin) * kKeys;
         const unsigned char* kv = (const unsigned char*)(keys + ((int64_t)h * key_rows + key_row) * (2 * kHead));
         const unsigned char* kr = (const unsigned char*)(shared + key_row * kRope);
 
-        auto copy_step = [&](int k, int stage) {
-#pragma unroll
-            for (int i = 0; i < 6; ++i) {
-                const int pl = i >> 1, blk = 2 * wave + (i & 1);
-                const int64_t at = (int64_t)k * kKeys + blk * 8;
-                const uint32_t to_lds = __builtin_amdgcn_readfirstlane(lds + stage * kChunkStage + pl * kPlane + blk * 1024);
-                if (pl == 1) copy16(kr + at * (2 * kRope), shared_off[i & 1], to_lds);
-                else copy16(kv + at * (4 * kHead) + (pl == 2 ? 2 * kHead : 0), key_off[i & 1], to_lds);
-            }
+        auto copy_keys = [&](int j, int stage) {
+            const unsigned char *from = kv + (int64_t)j * (kKeys * 4 * kHead), *rot = kr + (int64_t)j * (kKeys * 2 * kRope);
+            const uint32_t at = to_keys + stage * kKeyStage;
+            copy16_at<0>(from, key_off[0], at);
+            copy16_at<1024>(from, key_off[1], at);
+            copy16_at<kPlane>(rot, shared_off[0], at);
+            copy16_at<kPlane + 1024>(rot, shared_off[1], at);
         };
-        copy_step(k_begin, 0);
-        if (k_begin + 1 < k_end) copy_step(k_begin + 1, 1);
+        auto copy_values = [&](int j, int stage) {
+            const unsigned char* from = kv + (int64_t)j * (kKeys * 4 * kHead);
+            const uint32_t at = to_values + stage * kValueStage;
+            copy16_at<0>(from, value_off[0], at);
+            copy16_at<1024>(from, value_off[1], at);
+        };
+        copy_keys(0, 0);
+        copy_values(0, 0);
+        if (n > 1) copy_keys(1, 1), copy_values(1, 1);
+        if (n > 2) copy_keys(2, 2);
         Frag fq[8];
         {
             const uint16_t* qp = q + (row * s.H + h) * (kHead + kRope) + 8 * half;
@@ -1138,50 +1166,46 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
         }
         f32x16_t o[2] = {f32x16_zero(), f32x16_zero()}, x[2], y[2];
         float shift = kLowest, l = 0.0f;
-        auto scores = [&](f32x16_t (&z)[2], uint32_t at) {
+        // the keys' fragments of a step of the product, from where its stage begins
+        auto key_bases = [&](uint32_t at, uint32_t (&base)[4]) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) z[i] = f32x16_zero();
-#pragma unroll
-            for (int st = 0; st < 8; ++st)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const bf16x8_t a = *(lds_frag_ptr)(size_t)(at + k_at[st & 3] + (st >> 2) * kPlane + i * 32 * 128);
-                    z[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, fq[st].f, z[i], 0, 0, 0);
-                }
+            for (int i = 0; i < 4; ++i) {
+                base[i] = at + k_at[i];
+                asm volatile("" : "+v"(base[i]));  // (one sum each; the rest is the reads' constant offsets)
+            }
         };
-        // What the wave's tokens do not see of step k, in LDS at `at`: its scores; and rows whose values are not finite.
-        auto mask = [&](f32x16_t (&z)[2], int k, uint32_t at) {
-            const int sees = my_pos - k * kKeys - 4 * half;  // (a lane's keys are 4 half and a constant each)
-            bool bad = false;
-#pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-                const u32x4_t v = *(lds_u4_ptr)(size_t)(at + 2 * kPlane + lane * 128 + (((c + (lane >> 1)) & 7) << 4));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
-            }
-            const uint64_t odd = ballot(bad);
-            if (odd != 0) {  // no result for a token that sees one of them, zeros for the others
-                const uint64_t mine = odd >> (4 * half);
-                uint64_t seen = 0;
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const int key = 32 * (e >> 4) + 8 * ((e & 15) >> 2) + (e & 3);
-                    seen |= key <= sees ? mine & (1ull << key) : 0;
-                }
-                if (seen != 0) l = NAN;
-                lds_barrier();
-                for (int e = tid; e < kKeys * 8; e += 256)
-                    if (odd >> (e >> 3) & 1) *(lds_u4_ptr)(size_t)(at + 2 * kPlane + e * 16) = u32x4_t{0, 0, 0, 0};
-                lds_barrier();
-            }
+        auto read_keys = [&](const uint32_t (&base)[4], int st, int i) {
+            return *(lds_frag_ptr)(size_t)(base[st & 3] + (st >> 2) * kPlane + i * 32 * 128);
+        };
+        // What the wave's tokens do not see of step j.
+        auto mask = [&](f32x16_t (&z)[2], int j) {
+            const int sees = my_pos - (k_begin + j) * kKeys - 4 * half;  // (a lane's keys are 4 half and a constant each)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) z[i][e] = 32 * i + 8 * (e >> 2) + (e & 3) > sees ? -INFINITY : z[i][e];
         };
+        // Rows of step j, which not all tokens see, whose values are not finite: no result for a token that sees one of them,
+        // zeros for the others.
+        auto clean = [&](int j, uint32_t at) {
+            bool bad = false;
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                const u32x4_t v = *(lds_u4_ptr)(size_t)(at + lane * 128 + (((c + (lane >> 1)) & 7) << 4));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+            }
+            const uint64_t odd = ballot(bad);
+            if (odd == 0) return;
+            if ((k_begin + j) * kKeys + (int)__builtin_ctzll(odd) <= my_pos) l = NAN;  // (the first of them)
+            lds_barrier();
+            for (int e = tid; e < kKeys * 8; e += 256)
+                if (odd >> (e >> 3) & 1) *(lds_u4_ptr)(size_t)(at + e * 16) = u32x4_t{0, 0, 0, 0};
+            lds_barrier();
+        };
         auto new_top = [&](float top) {
-            top = fmaxf(top, __shfl_xor(top, 32, 64)) * s.scale2;
-            if (ballot(top > shift) != 0) {  // some token has a new maximum
+            top = halves_max(top) * s.scale2;
+            if (ballot(top > shift + kSlack) != 0) {  // some token's maximum has grown
                 const float was = shift;
                 shift = fmaxf(shift, top);
                 const float r = __builtin_amdgcn_exp2f(was - shift);
@@ -1192,52 +1216,68 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
                     for (int e = 0; e < 16; ++e) o[i][e] *= r;
             }
         };
-        // Step k on its scores x, whose maximum is known; with `more`, the scores y of step k + 1 beside it.  In this
+        // Step j on its scores x, whose maximum is known; with `more`, the scores y of step j + 1 beside it.  In this
         // order: two products of y beside the exponentials of four of x, eight times; then the products with the values
         // beside the maximum of y.  (The fences keep it: by itself the compiler puts the exponentials first.)
-        auto run_step = [&](auto more, f32x16_t (&x)[2], f32x16_t (&y)[2], int k, int stage) {
+        auto run_step = [&](auto more, f32x16_t (&x)[2], f32x16_t (&y)[2], int j, int stage) {
             const int next = stage == 2 ? 0 : stage + 1;
-            if constexpr (more) {
-                copies_barrier<0>();
-                if (k + 2 < k_end) copy_step(k + 2, next == 2 ? 0 : next + 1);
-            }
-            const uint32_t at = lds + stage * kChunkStage, to = lds + next * kChunkStage;
+            // behind the keys of step j + 1 and the values of step j, six copies: the keys of j + 2 and the values of j + 1
+            if (j + 2 < n) copies_barrier<6>();
+            else copies_barrier<0>();
+            if (j + 3 < n) copy_keys(j + 3, stage);
+            if (j + 2 < n) copy_values(j + 2, next == 2 ? 0 : next + 1);
+            uint32_t kb[4], vb[2][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    vb[i][d] = lds + kValues + stage * kValueStage + v_at[i][d];
+                    asm volatile("" : "+v"(vb[i][d]));
+                }
+            if ((k_begin + j) * kKeys + kKeys - 1 > first_pos) clean(j, lds + kValues + stage * kValueStage);
             Frag p[4], fv[4][2];
             bf16x8_t fk[8][2];
-            auto read_keys = [&](int st) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) fk[st][i] = *(lds_frag_ptr)(size_t)(to + k_at[st & 3] + (st >> 2) * kPlane + i * 32 * 128);
-            };
             if constexpr (more) {
-                read_keys(0);
-                read_keys(1);
+                key_bases(lds + next * kKeyStage, kb);
+#pragma unroll
+                for (int st = 0; st < kAhead; ++st)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) fk[st][i] = read_keys(kb, st, i);
                 y[0] = f32x16_zero();
                 y[1] = f32x16_zero();
             }
 #pragma unroll
             for (int st = 0; st < 8; ++st) {
                 if constexpr (more) {
-                    if (st + 2 < 8) read_keys(st + 2);
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) y[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk[st][i], fq[st].f, y[i], 0, 0, 0);
+                    for (int i = 0; i < 2; ++i) {
+                        if (st + kAhead < 8) fk[st + kAhead][i] = read_keys(kb, st + kAhead, i);
+                        y[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk[st][i], fq[st].f, y[i], 0, 0, 0);
+                    }
                 }
                 if (st >= 4) {
 #pragma unroll
-                    for (int d = 0; d < 2; ++d) {
-                        fv[st - 4][d].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(at + v_at[0][d] + (st - 4) * 16 * 128));
-                        fv[st - 4][d].h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(at + v_at[1][d] + (st - 4) * 16 * 128));
-                    }
+                    for (int d = 0; d < 2; ++d)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            fv[st - 4][d].h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(vb[i][d] + (st - 4) * 16 * 128));
                 }
+                if (st == 0) __builtin_amdgcn_s_setprio(1);  // (before a wave that is at its second part: 93.6 us against 96.5)
                 float e[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[st >> 2][4 * (st & 3) + j], s.scale2, -shift));
-                l += (e[0] + e[1]) + (e[2] + e[3]);
-                p[st >> 1].w[2 * (st & 1)] = pack_bf16x2(e[0], e[1]);
-                p[st >> 1].w[2 * (st & 1) + 1] = pack_bf16x2(e[2], e[3]);
+                for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[st >> 2][4 * (st & 3) + i], s.scale2, -shift));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t w = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+                    p[st >> 1].w[2 * (st & 1) + i] = w;
+                    // the sum of what the values are weighted with, rounded as they are
+                    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, w), __builtin_bit_cast(bf16x2_v, 0x3f803f80u), l, false);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (more)
-                if ((k + 1) * kKeys + kKeys - 1 > first_pos) mask(y, k + 1, to);
+                if ((k_begin + j + 1) * kKeys + kKeys - 1 > first_pos) mask(y, j + 1);
+            __builtin_amdgcn_s_setprio(0);
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -1253,11 +1293,19 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
             }
             if constexpr (more) new_top(top);
         };
-        if (k_begin + 1 < k_end) copies_barrier<6>();
+        // the first scores: behind their keys are up to 12 copies
+        if (n > 2) copies_barrier<12>();
         else copies_barrier<0>();
         {
-            scores(x, lds);
-            if (k_begin * kKeys + kKeys - 1 > first_pos) mask(x, k_begin, lds);
+            uint32_t kb[4];
+            key_bases(lds, kb);
+            x[0] = f32x16_zero();
+            x[1] = f32x16_zero();
+#pragma unroll
+            for (int st = 0; st < 8; ++st)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) x[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_keys(kb, st, i), fq[st].f, x[i], 0, 0, 0);
+            if (k_begin * kKeys + kKeys - 1 > first_pos) mask(x, 0);
             float top = x[0][0];
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -1265,41 +1313,41 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
                 for (int e = 0; e < 16; ++e) top = fmaxf(top, x[i][e]);
             new_top(top);
         }
-        int k = k_begin, stage = 0;
+        int j = 0, stage = 0;
         constexpr std::integral_constant<bool, true> more{};
         constexpr std::integral_constant<bool, false> none{};
-        for (; k + 2 < k_end; k += 2) {
-            run_step(more, x, y, k, stage);
+        for (; j + 2 < n; j += 2) {
+            run_step(more, x, y, j, stage);
             stage = stage == 2 ? 0 : stage + 1;
-            run_step(more, y, x, k + 1, stage);
+            run_step(more, y, x, j + 1, stage);
             stage = stage == 2 ? 0 : stage + 1;
         }
-        if (k + 1 < k_end) {
-            run_step(more, x, y, k, stage);
-            run_step(none, y, x, k + 1, stage == 2 ? 0 : stage + 1);
+        if (j + 1 < n) {
+            run_step(more, x, y, j, stage);
+            run_step(none, y, x, j + 1, stage == 2 ? 0 : stage + 1);
         } else {
-            run_step(none, x, y, k, stage);
+            run_step(none, x, y, j, stage);
         }
         l += __shfl_xor(l, 32, 64);
         lds_barrier();
         if (my < it.rows) {
             if (t == begin && to == finish) {  // the tile's whole work
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                uint16_t* y = out + (row * s.H + h) * kHead + 4 * half;
+                uint16_t* z = out + (row * s.H + h) * kHead + 4 * half;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<uint2*>(y + 32 * i + 2 * e) = make_uint2(pack_bf16x2(o[i][e] * inv, o[i][e + 1] * inv),
+                        *reinterpret_cast<uint2*>(z + 32 * i + 2 * e) = make_uint2(pack_bf16x2(o[i][e] * inv, o[i][e + 1] * inv),
                                                                                    pack_bf16x2(o[i][e + 2] * inv, o[i][e + 3] * inv));
             } else {
                 const int64_t slot = ((int64_t)group + (int64_t)h * n_items + item) * kChunkTok + my;
-                float* y = sums + slot * kHead + 4 * half;
+                float* z = sums + slot * kHead + 4 * half;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<f32x4_t*>(y + 32 * i + 2 * e) = f32x4_t{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+                        *reinterpret_cast<f32x4_t*>(z + 32 * i + 2 * e) = f32x4_t{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
                 if (half == 0) stats[slot] = make_float2(shift, l);
             }
         }
@@ -1355,9 +1403,9 @@ int launch_chunk(const uint16_t* q, const uint16_t* w, const uint16_t* pool, con
     float* sums = (float*)(ws + l.sums);
     hipLaunchKernelGGL(chunk_prepare_kernel, dim3((unsigned)((b.n_rows + 7) / 8 + 1)), dim3(256), 0, stream, rates, b, s, l.max_items, plan, items,
                        seq_item, seq_keys, tok_seq, specials, turns);
-    hipLaunchKernelGGL(expand_kernel, dim3((unsigned)((2 * num_cus + s.H - 1) / s.H * s.H)), dim3(256), 0, stream, w, pool, b, s, seq_keys, specials,
+    hipLaunchKernelGGL(expand_kernel, dim3((unsigned)(8 * s.H * ((2 * num_cus + 8 * s.H - 1) / (8 * s.H)))), dim3(256), 0, stream, w, pool, b, s, seq_keys, specials,
                        l.key_rows, keys, shared);
-    hipLaunchKernelGGL(chunk_attend_kernel, dim3((unsigned)s.groups), dim3(256), 0, stream, q, turns, keys, shared, s, plan, items, seq_keys,
+    hipLaunchKernelGGL(chunk_attend_kernel, dim3((unsigned)s.groups), dim3(256), 0, stream, q, turns, keys, shared, s, plan, items,
                        l.key_rows, sums, stats, out);
     hipLaunchKernelGGL(chunk_finish_kernel, dim3((unsigned)((b.n_rows * s.H + 15) / 16)), dim3(256), 0, stream, b, s, plan, items, seq_item,
                        tok_seq, sums, stats, out);
