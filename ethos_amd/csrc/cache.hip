@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void append_kernel(const T* __restrict__ rows,
         xr[c] = *reinterpret_cast<const Raw*>(x + (e < rank ? e : 0));
         gr[c] = *reinterpret_cast<const Raw*>(gain + (e < rank ? e : 0));
     }
-    const int i = batch_seq(b, r);
+    const int i = batch_seq_wave(b, r, lane);
     if (i < 0) return;
     const int64_t pos = (int64_t)b.lens[i] - b.starts[i + 1] + r;
     const int32_t page = batch_page(b, i, pos);

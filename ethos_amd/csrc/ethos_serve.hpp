@@ -37,6 +37,19 @@ __device__ __forceinline__ int batch_seq(const Batch& b, int64_t r) {
     return b.starts[lo] <= r && r < b.starts[lo + 1] ? lo : -1;
 }
 
+// The same by all lanes of a wave for one row of theirs: two rounds of loads for 4,096 sequences.
+__device__ __forceinline__ int batch_seq_wave(const Batch& b, int64_t r, int lane) {
+    int lo = 0, n = b.n_seq;  // the answer is in [lo, lo + n)
+    while (n > 1) {
+        const int step = (n + 63) / 64, at = lane * step;
+        const int k = __builtin_popcountll(__builtin_amdgcn_ballot_w64(at < n && b.starts[lo + (at < n ? at : 0)] <= r));
+        const int skip = k > 0 ? (k - 1) * step : 0;
+        lo += skip;
+        n = n - skip < step ? n - skip : step;
+    }
+    return b.starts[lo] <= r && r < b.starts[lo + 1] ? lo : -1;
+}
+
 // The page of position p of sequence i, -1 where there is none.
 __device__ __forceinline__ int32_t batch_page(const Batch& b, int i, int64_t p) {
     const int64_t at = p >> b.page_log;

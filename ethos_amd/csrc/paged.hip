@@ -36,6 +36,13 @@ struct Item {
     int64_t end;   // tiles of work up to this one's last, all before it included
 };
 
+// A token's sequence, kNoSeq without one, kBadSeq with one that has no result (its length does not fit its table, or its
+// rows are not in the batch); and its place among the sequence's new tokens.
+constexpr int kNoSeq = -1, kBadSeq = -2;
+struct Token {
+    int32_t seq, index;
+};
+
 struct Plan {
     int64_t tiles, quota;  // in all; of a workgroup
     int32_t n_items, pad[3];
@@ -43,7 +50,7 @@ struct Plan {
 
 // Where the workspace's parts are.
 struct Layout {
-    size_t plan, items, seq_item, tok_seq, specials, queries, sums, stats, bytes;
+    size_t plan, items, seq_item, tokens, specials, queries, sums, stats, bytes;
     int64_t max_items;
 };
 
@@ -69,7 +76,7 @@ Layout layout(int64_t n_rows, int n_seq, int H, int width, int tile_rows, int gr
     l.plan = take(sizeof(Plan));
     l.items = take((size_t)l.max_items * sizeof(Item));
     l.seq_item = take((size_t)n_seq * 4);
-    l.tok_seq = take((size_t)n_rows * 4);
+    l.tokens = take((size_t)n_rows * sizeof(Token));
     l.specials = take((size_t)16 * width * 2);
     l.queries = take((size_t)n_rows * H * width * query_bytes);
     const size_t slots = (size_t)(l.max_items + groups);
@@ -106,6 +113,11 @@ __device__ __forceinline__ int64_t new_tokens(const Batch& b, int i) {
 }
 __device__ __forceinline__ bool fits(const Batch& b, int i) {
     return b.lens[i] >= 0 && b.lens[i] <= kLongest && (int64_t)b.lens[i] <= (int64_t)b.width << b.page_log;
+}
+
+__device__ __forceinline__ Token token_of(const Batch& b, int64_t t, int i) {
+    if (i < 0) return Token{kNoSeq, 0};
+    return new_tokens(b, i) > 0 && fits(b, i) ? Token{i, (int32_t)(t - b.starts[i])} : Token{kBadSeq, 0};
 }
 
 // One workgroup of NT threads: NT sequences at a time, then their items, NT at a time.
@@ -190,14 +202,14 @@ constexpr int kAnyRows = 8, kAnyKeys = 16, kAnyRank = 512, kAnyRope = 128, kAnyW
 template <typename T>
 __global__ __launch_bounds__(1024) void any_prepare_kernel(const T* __restrict__ q, const T* __restrict__ w, const float* __restrict__ rates,
                                                            Batch b, Shape s, int64_t max_items, Plan* plan, Item* items, int32_t* seq_item,
-                                                           int32_t* tok_seq, float* __restrict__ queries) {
+                                                           Token* tokens, float* __restrict__ queries) {
     if (blockIdx.x == 0) {
         make_plan<1024>(b, s, max_items, plan, items, seq_item, nullptr, threadIdx.x);
         return;
     }
     const int64_t t = blockIdx.x - 1;
     const int i = batch_seq(b, t), width = s.rank + s.rope, qw = s.nope + s.rope;
-    if (threadIdx.x == 0) tok_seq[t] = i;
+    if (threadIdx.x == 0) tokens[t] = token_of(b, t, i);
     if (i < 0) return;
     const int64_t pos = (int64_t)b.lens[i] - b.starts[i + 1] + t;
     const T* qt = q + t * s.H * qw;
@@ -306,17 +318,19 @@ __global__ __launch_bounds__(256) void any_attend_kernel(const T* __restrict__ p
     }
 }
 
-// The parts of a row's sums: workgroups first .. first + n - 1 left them, in slots one apart.
+// The parts of a row's sums: n of them, in slots one apart.  `row` of the sequence's in a plane; in: its place in a part.
 struct Parts {
     int64_t slot;
     int n;
-    bool bad;  // the sequence's length does not fit its table, or there was no room for it
+    bool bad;  // no result
 };
-__device__ __forceinline__ Parts row_parts(const Batch& b, const Shape& s, const Plan* plan, const Item* items, const int32_t* seq_item, int i,
-                                           int64_t row, int plane, int& in) {
+__device__ __forceinline__ Parts row_parts(const Shape& s, const Plan* plan, const Item* items, const int32_t* seq_item, int seq, int64_t row,
+                                           int plane, int& in) {
     Parts p = {0, 0, true};
-    const int32_t first = seq_item[i];
-    if (first < 0 || new_tokens(b, i) == 0 || !fits(b, i)) return p;
+    in = 0;
+    if (seq < 0) return p;
+    const int32_t first = seq_item[seq];
+    if (first < 0) return p;  // there was no room for it
     p.bad = false;
     const int64_t item = first + row / s.rows;
     in = (int)(row % s.rows);
@@ -333,17 +347,18 @@ __device__ __forceinline__ Parts row_parts(const Batch& b, const Shape& s, const
 
 // One workgroup a token: joins each row's parts, in order, and multiplies with W_v,h.
 template <typename T>
-__global__ __launch_bounds__(256) void any_finish_kernel(const T* __restrict__ w, Batch b, Shape s, const Plan* plan,
+__global__ __launch_bounds__(256) void any_finish_kernel(const T* __restrict__ w, Shape s, const Plan* plan,
                                                          const Item* __restrict__ items, const int32_t* __restrict__ seq_item,
-                                                         const int32_t* __restrict__ tok_seq, const float* __restrict__ sums,
+                                                         const Token* __restrict__ tokens, const float* __restrict__ sums,
                                                          const float2* __restrict__ stats, T* __restrict__ out) {
     __shared__ float o[kAnyRank];
     const int64_t t = blockIdx.x;
-    const int i = tok_seq[t], tid = threadIdx.x;
-    if (i < 0) return;  // behind the last sequence
+    const Token token = tokens[t];
+    const int tid = threadIdx.x;
+    if (token.seq == kNoSeq) return;  // behind the last sequence
     for (int h = 0; h < s.H; ++h) {
         int in = 0;
-        const Parts p = row_parts(b, s, plan, items, seq_item, i, (t - b.starts[i]) * s.H + h, 0, in);
+        const Parts p = row_parts(s, plan, items, seq_item, token.seq, (int64_t)token.index * s.H + h, 0, in);
         float top = kLowest, l = 0.0f;
         for (int k = 0; k < p.n; ++k) top = fmaxf(top, stats[(p.slot + k) * s.rows + in].x);
         for (int k = 0; k < p.n; ++k) {
@@ -380,13 +395,14 @@ int launch_any(const T* q, const T* w, const T* pool, const Batch& b, const floa
     const Layout l = layout(b.n_rows, b.n_seq, s.H, s.rank + s.rope, s.rows, s.groups, 4, s.rank);
     Plan* plan = (Plan*)(ws + l.plan);
     Item* items = (Item*)(ws + l.items);
-    int32_t *seq_item = (int32_t*)(ws + l.seq_item), *tok_seq = (int32_t*)(ws + l.tok_seq);
+    int32_t* seq_item = (int32_t*)(ws + l.seq_item);
+    Token* tokens = (Token*)(ws + l.tokens);
     float *queries = (float*)(ws + l.queries), *sums = (float*)(ws + l.sums);
     float2* stats = (float2*)(ws + l.stats);
     hipLaunchKernelGGL((any_prepare_kernel<T>), dim3((unsigned)(b.n_rows + 1)), dim3(1024), 0, stream, q, w, rates, b, s, l.max_items, plan,
-                       items, seq_item, tok_seq, queries);
+                       items, seq_item, tokens, queries);
     hipLaunchKernelGGL((any_attend_kernel<T>), dim3((unsigned)s.groups), dim3(256), 0, stream, pool, b, s, plan, items, queries, sums, stats);
-    hipLaunchKernelGGL((any_finish_kernel<T>), dim3((unsigned)b.n_rows), dim3(256), 0, stream, w, b, s, plan, items, seq_item, tok_seq, sums,
+    hipLaunchKernelGGL((any_finish_kernel<T>), dim3((unsigned)b.n_rows), dim3(256), 0, stream, w, s, plan, items, seq_item, tokens, sums,
                        stats, out);
     return (int)hipGetLastError();
 }
@@ -410,6 +426,7 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(3))) bf16x8_t* lds_frag_ptr;
 typedef __attribute__((address_space(3))) s16x4_t* lds_tr_ptr;
 typedef __attribute__((address_space(3))) u32x4_t* lds_u4_ptr;
+typedef __attribute__((address_space(3))) u32x2_t* lds_u2_ptr;
 typedef __attribute__((address_space(3))) float* lds_f_ptr;
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
@@ -448,14 +465,17 @@ __device__ __forceinline__ void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x8, L, 0);
 }
 
+constexpr int kSeqsNear = 1024;
+
 // Block 0: the plan and the two special rows.  The others: 32 tokens of a head; [c][token] = W_k,h^T q^T, the weight
 // (k as the row) through LDS in the layout of the loss's R tiles.
 __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ w,
                                                       const float* __restrict__ rates, Batch b, Shape s, int64_t max_items, Plan* plan,
-                                                      Item* items, int32_t* seq_item, int32_t* tok_seq, uint16_t* __restrict__ specials,
+                                                      Item* items, int32_t* seq_item, Token* tokens, uint16_t* __restrict__ specials,
                                                       uint16_t* __restrict__ queries) {
     __shared__ __align__(16) uint16_t ws[64 * kRank];
     __shared__ int64_t pos[32];
+    __shared__ int32_t starts[kSeqsNear], lens[kSeqsNear];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (blockIdx.x == 0) {
@@ -465,23 +485,42 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
     }
     const int h = (blockIdx.x - 1) % s.H, qw = s.nope + kRope;
     const int64_t t0 = (int64_t)((blockIdx.x - 1) / s.H) * 32;
-    if (tid < 32) {
-        const int64_t t = t0 + tid;
-        const int i = t < b.n_rows ? batch_seq(b, t) : -1;
-        if (h == 0 && t < b.n_rows) tok_seq[t] = i;
-        pos[tid] = i >= 0 ? (int64_t)b.lens[i] - b.starts[i + 1] + t : 0;
-    }
     const int64_t my_t = t0 + (lane & 31) < b.n_rows ? t0 + (lane & 31) : b.n_rows - 1;
     const uint16_t* qp = q + (my_t * s.H + h) * qw;
     f32x16_t acc[2] = {f32x16_zero(), f32x16_zero()};
+    // the tokens' positions, by a search in LDS where there is room for the sequences
+    auto find_positions = [&]() {
+        const bool near = b.n_seq < kSeqsNear;
+        if (near) {
+            for (int i = tid; i <= b.n_seq; i += 256) starts[i] = b.starts[i];
+            for (int i = tid; i < b.n_seq; i += 256) lens[i] = b.lens[i];
+            __syncthreads();
+        }
+        if (tid < 32 && t0 + tid < b.n_rows) {
+            const int64_t t = t0 + tid;
+            Batch c = b;
+            if (near) c.starts = starts, c.lens = lens;
+            const int i = batch_seq(c, t);
+            if (h == 0) tokens[t] = token_of(c, t, i);
+            pos[tid] = i >= 0 ? (int64_t)c.lens[i] - c.starts[i + 1] + t : 0;
+        }
+    };
+    if (s.nope == 0) find_positions();
     for (int j0 = 0; j0 < s.nope; j0 += 64) {
         const int rows = s.nope - j0 < 64 ? s.nope - j0 : 64;
         const uint16_t* wh = w + ((int64_t)h * (s.nope + s.v_dim) + j0) * kRank;
-        if (j0 > 0) __syncthreads();
-        for (int e = tid; e < rows * 32; e += 256) {
-            const int r = e >> 5, c = e & 31;
-            *reinterpret_cast<u32x4_t*>(ws + r * kRank + ((c ^ ((r & 3) << 2)) * 8)) =
-                *reinterpret_cast<const u32x4_t*>(wh + (int64_t)r * kRank + c * 8);
+        u32x4_t part[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = (tid >> 5) + 8 * i;
+            part[i] = *reinterpret_cast<const u32x4_t*>(wh + (int64_t)(r < rows ? r : rows - 1) * kRank + (tid & 31) * 8);
+        }
+        if (j0 == 0) find_positions();  // (while the weight is on its way)
+        else __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = (tid >> 5) + 8 * i;
+            *reinterpret_cast<u32x4_t*>(ws + r * kRank + (((tid & 31) ^ ((r & 3) << 2)) * 8)) = part[i];
         }
         __syncthreads();
         const uint32_t lds = lds_addr(ws);
@@ -758,9 +797,9 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
 // TOK tokens of a head: 256 / TOK threads a token join its parts, 16 columns a thread and 16 / TOK parts side by side,
 // then [v][token] = W_v,h o^T by 16 x 16 x 32 MFMAs, a wave for every 16 of v_dim.
 template <int TOK>
-__global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict__ w, Batch b, Shape s, const Plan* plan,
+__global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict__ w, int64_t n_rows, Shape s, const Plan* plan,
                                                      const Item* __restrict__ items, const int32_t* __restrict__ seq_item,
-                                                     const int32_t* __restrict__ tok_seq, const float* __restrict__ sums,
+                                                     const Token* __restrict__ tokens, const float* __restrict__ sums,
                                                      const float2* __restrict__ stats, uint16_t* __restrict__ out) {
     constexpr int G = 16 / TOK;  // groups of 16 threads that share a token
     __shared__ __align__(16) uint16_t os[TOK][kRank + 8];
@@ -771,10 +810,15 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
     const int64_t t0 = (int64_t)(blockIdx.x / s.H) * TOK;
     const int grp = tid >> 4, tok = grp / G, sub = grp % G, col = (tid & 15) * 4;
     const int64_t t = t0 + tok;
-    const int i = t < b.n_rows ? tok_seq[t] : -1;
-    Parts p = {0, 0, false};
-    int in = 0;
-    if (i >= 0) p = row_parts(b, s, plan, items, seq_item, i, (t - b.starts[i]) * s.H + h, 0, in);
+    // (the weight's first fragments, on their way meanwhile)
+    bf16x8_t first[kRank / 32];
+    const uint16_t* wv = w + ((int64_t)h * (s.nope + s.v_dim) + s.nope + (lane & 15)) * kRank + 8 * (lane >> 4);
+#pragma unroll
+    for (int st = 0; st < kRank / 32; ++st)
+        first[st] = *reinterpret_cast<const bf16x8_t*>(wv + (int64_t)(wave * 16 < s.v_dim ? wave * 16 : 0) * kRank + 32 * st);
+    const Token token = t < n_rows ? tokens[t] : Token{kNoSeq, 0};
+    int in;
+    const Parts p = row_parts(s, plan, items, seq_item, token.seq, (int64_t)token.index * s.H + h, 0, in);
     float top = kLowest, l = 0.0f, v[16] = {};
     for (int k = sub; k < p.n; k += 4 * G) {  // four parts' loads on their way at a time
         float2 ml[4];
@@ -837,13 +881,12 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
     __syncthreads();
     const int tc = (lane & 15) < TOK ? lane & 15 : TOK - 1;
     const int64_t to = t0 + (lane & 15);
-    const bool live = (lane & 15) < TOK && to < b.n_rows && tok_seq[to] >= 0;
+    const bool live = (lane & 15) < TOK && to < n_rows && tokens[to].seq != kNoSeq;
     for (int vb = wave; vb < s.v_dim / 16; vb += 4) {
-        const uint16_t* wv = w + ((int64_t)h * (s.nope + s.v_dim) + s.nope + vb * 16 + (lane & 15)) * kRank + 8 * (lane >> 4);
         f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int st = 0; st < kRank / 32; ++st) {
-            const bf16x8_t a = *reinterpret_cast<const bf16x8_t*>(wv + 32 * st);
+            const bf16x8_t a = vb == wave ? first[st] : *reinterpret_cast<const bf16x8_t*>(wv + (int64_t)vb * 16 * kRank + 32 * st);
             const bf16x8_t x = *reinterpret_cast<const bf16x8_t*>(&os[tc][32 * st + 8 * (lane >> 4)]);
             acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, x, acc, 0, 0, 0);
         }
@@ -872,13 +915,14 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
     const Layout l = layout(b.n_rows, b.n_seq, s.H, kWidth, s.rows, s.groups, 2, kRank);
     Plan* plan = (Plan*)(ws + l.plan);
     Item* items = (Item*)(ws + l.items);
-    int32_t *seq_item = (int32_t*)(ws + l.seq_item), *tok_seq = (int32_t*)(ws + l.tok_seq);
+    int32_t* seq_item = (int32_t*)(ws + l.seq_item);
+    Token* tokens = (Token*)(ws + l.tokens);
     uint16_t *specials = (uint16_t*)(ws + l.specials), *queries = (uint16_t*)(ws + l.queries);
     float* sums = (float*)(ws + l.sums);
     float2* stats = (float2*)(ws + l.stats);
     const unsigned tiles = (unsigned)((b.n_rows + 31) / 32);
     hipLaunchKernelGGL(prepare_kernel, dim3(tiles * s.H + 1), dim3(256), 0, stream, q, w, rates, b, s, l.max_items, plan, items, seq_item,
-                       tok_seq, specials, queries);
+                       tokens, specials, queries);
     auto attend = [&](auto kernel, int threads) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)s.groups), dim3(threads), 0, stream, pool, b, s, plan, items, queries, specials, sums, stats);
     };
@@ -888,14 +932,14 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
     else attend(attend_kernel<8, 1, 3>, 512);
     // (few tokens have many parts each: more threads a token)
     if (b.n_rows <= 8)
-        hipLaunchKernelGGL((finish_kernel<1>), dim3((unsigned)(b.n_rows * s.H)), dim3(256), 0, stream, w, b, s, plan, items, seq_item, tok_seq, sums,
-                           stats, out);
+        hipLaunchKernelGGL((finish_kernel<1>), dim3((unsigned)(b.n_rows * s.H)), dim3(256), 0, stream, w, b.n_rows, s, plan, items, seq_item,
+                           tokens, sums, stats, out);
     else if (b.n_rows <= 256)
-        hipLaunchKernelGGL((finish_kernel<4>), dim3((unsigned)((b.n_rows + 3) / 4 * s.H)), dim3(256), 0, stream, w, b, s, plan, items, seq_item,
-                           tok_seq, sums, stats, out);
+        hipLaunchKernelGGL((finish_kernel<4>), dim3((unsigned)((b.n_rows + 3) / 4 * s.H)), dim3(256), 0, stream, w, b.n_rows, s, plan, items,
+                           seq_item, tokens, sums, stats, out);
     else
-        hipLaunchKernelGGL((finish_kernel<16>), dim3((unsigned)((b.n_rows + 15) / 16 * s.H)), dim3(256), 0, stream, w, b, s, plan, items, seq_item,
-                           tok_seq, sums, stats, out);
+        hipLaunchKernelGGL((finish_kernel<16>), dim3((unsigned)((b.n_rows + 15) / 16 * s.H)), dim3(256), 0, stream, w, b.n_rows, s, plan, items,
+                           seq_item, tokens, sums, stats, out);
     return (int)hipGetLastError();
 }
 
@@ -912,7 +956,7 @@ constexpr int kChunkRows = 128;   // new tokens a sequence, on the average, from
 constexpr size_t kChunkBytes = (size_t)1 << 30;  // of keys and values, at most
 
 struct ChunkLayout {
-    size_t plan, items, seq_item, tok_seq, seq_keys, specials, turns, keys, shared, sums, stats, bytes;
+    size_t plan, items, seq_item, tokens, seq_keys, specials, turns, keys, shared, sums, stats, bytes;
     int64_t max_items, key_rows;
 };
 
@@ -929,7 +973,7 @@ ChunkLayout chunk_layout(int64_t n_rows, int n_seq, int H, int64_t capacity, int
     l.plan = take(sizeof(Plan));
     l.items = take((size_t)l.max_items * sizeof(Item));
     l.seq_item = take((size_t)n_seq * 4);
-    l.tok_seq = take((size_t)n_rows * 4);
+    l.tokens = take((size_t)n_rows * sizeof(Token));
     l.seq_keys = take((size_t)(n_seq + 1) * 4);
     l.specials = take((size_t)16 * kWidth * 2);
     l.turns = take((size_t)n_rows * kRope / 2 * 8);
@@ -944,7 +988,7 @@ ChunkLayout chunk_layout(int64_t n_rows, int n_seq, int H, int64_t capacity, int
 
 // Block 0: the plan.  The others: eight tokens' sequences, cosines and sines.
 __global__ __launch_bounds__(256) void chunk_prepare_kernel(const float* __restrict__ rates, Batch b, Shape s, int64_t max_items, Plan* plan,
-                                                            Item* items, int32_t* seq_item, int32_t* seq_keys, int32_t* tok_seq,
+                                                            Item* items, int32_t* seq_item, int32_t* seq_keys, Token* tokens,
                                                             uint16_t* __restrict__ specials, float2* __restrict__ turns) {
     if (blockIdx.x == 0) {
         for (int e = threadIdx.x; e < 2 * kBlock * kWidth; e += 256) specials[e] = e < kBlock * kWidth ? 0 : 0x7fc0;
@@ -955,22 +999,29 @@ __global__ __launch_bounds__(256) void chunk_prepare_kernel(const float* __restr
     }
     const int64_t t = (int64_t)(blockIdx.x - 1) * 8 + (threadIdx.x >> 5);
     const int p = threadIdx.x & 31;
+    const int64_t wave_t = t - ((threadIdx.x >> 5) & 1);  // the wave's two tokens
+    int seq[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) seq[i] = wave_t + i < b.n_rows ? batch_seq_wave(b, wave_t + i, threadIdx.x & 63) : kNoSeq;
     if (t >= b.n_rows) return;
-    const int i = batch_seq(b, t);
-    if (p == 0) tok_seq[t] = i;
+    const int i = (threadIdx.x & 32) ? seq[1] : seq[0];
+    if (p == 0) tokens[t] = token_of(b, t, i);
     if (i < 0) return;
     float2 c;
     rotary_angle((int64_t)b.lens[i] - b.starts[i + 1] + t, rates[p], c.x, c.y);
     turns[t * 32 + p] = c;
 }
 
+constexpr int kRowStage = kRank / 64 * kPlane;  // the latents of 64 rows
+
 // Keys and values of a head for some tiles of 64 cached rows: [column][row] = W_h c^T, a wave 32 of the
 // head's 128 columns, the weight's fragments in registers, the rows from LDS in the planes of above, the next tile's on
-// their way.  Workgroups go round the heads; the rotated keys, which are copied, are each tile's one head's.
+// their way.  The result goes through LDS, so that its rows are stored 16 bytes a lane, one after the other (8 bytes a lane
+// at 32 rows: 21 us for 7,001 rows and 16 heads).  The rotated keys are copied by one head's workgroup of each tile.
 __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restrict__ w, const uint16_t* __restrict__ pool, Batch b, Shape s,
                                                         const int32_t* __restrict__ seq_keys, const uint16_t* __restrict__ specials,
                                                         int64_t key_rows, uint16_t* __restrict__ keys, uint16_t* __restrict__ shared) {
-    __shared__ __align__(16) unsigned char ring[2 * kStage];
+    __shared__ __align__(16) unsigned char ring[2 * kRowStage + kKeys * 4 * kHead];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t lds = lds_addr(ring);
@@ -982,32 +1033,50 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restri
     int tile = round / s.H * 8 + blockIdx.x % 8;
     if (tile >= total) return;
 
-    int seq = 0;
-    auto copy_tile = [&](int u, int stage) {
-        int hi = b.n_seq;  // the last sequence whose tiles begin at or before this one (not before that of the last tile)
-        while (hi - seq > 1) {
-            const int mid = (seq + hi) >> 1;
-            if (first[mid] <= u) seq = mid;
-            else hi = mid;
+    // Where a tile's rows are: looked up a tile before they are copied, so that no copy waits for it.
+    struct Place {
+        int seq, key0, end;
+        int32_t pages[2];
+    };
+    int seq = 0, seq_first = 0, seq_end = 0, seq_len = 0;  // the last tile's sequence; seq_end: its tiles' end
+    auto look_up = [&](int u) {
+        if (u >= seq_end) {
+            int hi = b.n_seq;  // the last sequence whose tiles begin at or before this one
+            while (hi - seq > 1) {
+                const int mid = (seq + hi) >> 1;
+                if (first[mid] <= u) seq = mid;
+                else hi = mid;
+            }
+            seq_first = first[seq];
+            seq_end = first[seq + 1];
+            seq_len = ((const_ptr)(uintptr_t)b.lens)[seq];
         }
-        const int key0 = (u - first[seq]) * kKeys, end = ((const_ptr)(uintptr_t)b.lens)[seq];
+        Place p = {seq, (u - seq_first) * kKeys, seq_len, {}};
         const const_ptr table = (const_ptr)(uintptr_t)(b.table + seq * b.table_ld);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int blk = 2 * wave + i, p0 = key0 + blk * kBlock, at = p0 >> b.page_log, row = lane >> 3;
-            const int32_t page = table[at < b.width ? at : b.width - 1];
-            const uint16_t* from = page >= 0 && page < b.n_pages
-                                       ? pool + (((int64_t)page << b.page_log) + (p0 & ((1 << b.page_log) - 1))) * kWidth
+            const int at = (p.key0 + (2 * wave + i) * kBlock) >> b.page_log;
+            p.pages[i] = table[at < b.width ? at : b.width - 1];
+        }
+        return p;
+    };
+    auto copy_tile = [&](const Place& p, int stage) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int blk = 2 * wave + i, p0 = p.key0 + blk * kBlock, row = lane >> 3;
+            const uint16_t* from = p.pages[i] >= 0 && p.pages[i] < b.n_pages
+                                       ? pool + (((int64_t)p.pages[i] << b.page_log) + (p0 & ((1 << b.page_log) - 1))) * kWidth
                                        : specials + kBlock * kWidth;
             const uint32_t off = row * (kWidth * 2) + (((lane & 7) ^ swizzle(blk * kBlock + row)) << 4);
-            const unsigned char* mine = (const unsigned char*)(p0 + row < end ? from : specials) + off;
-            const uint32_t to_lds = lds + stage * kStage + blk * 1024;
+            const unsigned char* mine = (const unsigned char*)(p0 + row < p.end ? from : specials) + off;
+            const uint32_t to_lds = lds + stage * kRowStage + blk * 1024;
 #pragma unroll
-            for (int pl = 0; pl < kWidth / 64; ++pl)
-                if (pl < kRank / 64 || u % s.H == h) copy16(mine + pl * 128, __builtin_amdgcn_readfirstlane(to_lds + pl * kPlane));
+            for (int pl = 0; pl < kRank / 64; ++pl) copy16(mine + pl * 128, __builtin_amdgcn_readfirstlane(to_lds + pl * kPlane));
         }
     };
-    copy_tile(tile, 0);
+    Place now = look_up(tile), next = now;
+    copy_tile(now, 0);
+    if (tile + step < total) next = look_up(tile + step);
     bf16x8_t a[kRank / 16];
     {
         const uint16_t* wh = w + ((int64_t)h * 2 * kHead + wave * 32 + (lane & 31)) * kRank + 8 * half;
@@ -1018,11 +1087,14 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restri
     }
     int stage = 0;
     for (bool started = false; tile < total; tile += step, stage ^= 1, started = true) {
-        // (behind this tile's copies are only the last tile's stores, 8 or more)
-        if (started) copies_barrier<8>();
+        // (behind this tile's copies are only the last tile's stores, four or more)
+        if (started) copies_barrier<4>();
         else copies_barrier<0>();
-        if (tile + step < total) copy_tile(tile + step, stage ^ 1);
-        const uint32_t at = lds + stage * kStage;
+        const Place here = now;
+        now = next;
+        if (tile + step < total) copy_tile(now, stage ^ 1);
+        if (tile + 2 * step < total) next = look_up(tile + 2 * step);
+        const uint32_t at = lds + stage * kRowStage, result = lds + 2 * kRowStage;
         f32x16_t acc[2] = {f32x16_zero(), f32x16_zero()};
 #pragma unroll
         for (int st = 0; st < kRank / 16; ++st)
@@ -1032,19 +1104,35 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restri
                 const bf16x8_t x = *(lds_frag_ptr)(size_t)(at + (st >> 2) * kPlane + r * 128 + (((2 * (st & 3) + half) ^ swizzle(r)) << 4));
                 acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[st], x, acc[i], 0, 0, 0);
             }
-        uint16_t* to = keys + ((int64_t)h * key_rows + (int64_t)tile * kKeys + (lane & 31)) * (2 * kHead) + wave * 32 + 4 * half;
+        reads_ahead<8, 2 * kRank / 16 - 8, 1, 8>();
+        // row r's piece c of 16 bytes lies at c ^ r % 16
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<uint2*>(to + i * 32 * 2 * kHead + 2 * e) =
-                    make_uint2(pack_bf16x2(acc[i][e], acc[i][e + 1]), pack_bf16x2(acc[i][e + 2], acc[i][e + 3]));
+            for (int e = 0; e < 16; e += 4) {
+                const int r = 32 * i + (lane & 31), c = 4 * wave + (e >> 2);
+                *(lds_u2_ptr)(size_t)(result + r * (4 * kHead) + ((c ^ (r & 15)) << 4) + 8 * half) =
+                    u32x2_t{pack_bf16x2(acc[i][e], acc[i][e + 1]), pack_bf16x2(acc[i][e + 2], acc[i][e + 3])};
+            }
+        lds_barrier();
+        uint16_t* to = keys + ((int64_t)h * key_rows + (int64_t)tile * kKeys) * (2 * kHead);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 16 * i + (tid >> 4), c = tid & 15;
+            *reinterpret_cast<u32x4_t*>(to + r * (2 * kHead) + c * 8) = *(lds_u4_ptr)(size_t)(result + r * (4 * kHead) + ((c ^ (r & 15)) << 4));
+        }
         if (tile % s.H == h) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int r = 32 * i + (tid >> 3), c = tid & 7;
-                *reinterpret_cast<u32x4_t*>(shared + ((int64_t)tile * kKeys + r) * kRope + c * 8) =
-                    *(lds_u4_ptr)(size_t)(at + kRank / 64 * kPlane + r * 128 + ((c ^ swizzle(r)) << 4));
+                const int r = 32 * i + (tid >> 3), c = tid & 7, p = here.key0 + r;
+                u32x4_t v = {0, 0, 0, 0};
+                if (p < here.end) {
+                    const int32_t page = batch_page(b, here.seq, p);
+                    v = page < 0 ? u32x4_t{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u}
+                                 : *reinterpret_cast<const u32x4_t*>(pool + (((int64_t)page << b.page_log) + (p & ((1 << b.page_log) - 1))) * kWidth +
+                                                                     kRank + c * 8);
+                }
+                *reinterpret_cast<u32x4_t*>(shared + ((int64_t)tile * kKeys + r) * kRope + c * 8) = v;
             }
         }
     }
@@ -1356,17 +1444,17 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
 }
 
 // 16 (token, head) rows a workgroup, 16 threads each: joins the parts of those that have several.
-__global__ __launch_bounds__(256) void chunk_finish_kernel(Batch b, Shape s, const Plan* plan, const Item* __restrict__ items,
-                                                           const int32_t* __restrict__ seq_item, const int32_t* __restrict__ tok_seq,
+__global__ __launch_bounds__(256) void chunk_finish_kernel(int64_t n_rows, Shape s, const Plan* plan, const Item* __restrict__ items,
+                                                           const int32_t* __restrict__ seq_item, const Token* __restrict__ tokens,
                                                            const float* __restrict__ sums, const float2* __restrict__ stats,
                                                            uint16_t* __restrict__ out) {
     const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), t = r / s.H;
     const int h = (int)(r - t * s.H), col = (threadIdx.x & 15) * 4;
-    if (t >= b.n_rows) return;
-    const int i = tok_seq[t];
-    if (i < 0) return;
-    int in = 0;
-    const Parts p = row_parts(b, s, plan, items, seq_item, i, t - b.starts[i], h, in);
+    if (t >= n_rows) return;
+    const Token token = tokens[t];
+    if (token.seq == kNoSeq) return;
+    int in;
+    const Parts p = row_parts(s, plan, items, seq_item, token.seq, token.index, h, in);
     if (p.n == 1) return;  // written as a whole
     float top = kLowest, l = 0.0f;
     f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1397,18 +1485,19 @@ int launch_chunk(const uint16_t* q, const uint16_t* w, const uint16_t* pool, con
     const ChunkLayout l = chunk_layout(b.n_rows, b.n_seq, s.H, (int64_t)b.width << b.page_log, s.groups);
     Plan* plan = (Plan*)(ws + l.plan);
     Item* items = (Item*)(ws + l.items);
-    int32_t *seq_item = (int32_t*)(ws + l.seq_item), *tok_seq = (int32_t*)(ws + l.tok_seq), *seq_keys = (int32_t*)(ws + l.seq_keys);
+    int32_t *seq_item = (int32_t*)(ws + l.seq_item), *seq_keys = (int32_t*)(ws + l.seq_keys);
+    Token* tokens = (Token*)(ws + l.tokens);
     float2 *turns = (float2*)(ws + l.turns), *stats = (float2*)(ws + l.stats);
     uint16_t *specials = (uint16_t*)(ws + l.specials), *keys = (uint16_t*)(ws + l.keys), *shared = (uint16_t*)(ws + l.shared);
     float* sums = (float*)(ws + l.sums);
     hipLaunchKernelGGL(chunk_prepare_kernel, dim3((unsigned)((b.n_rows + 7) / 8 + 1)), dim3(256), 0, stream, rates, b, s, l.max_items, plan, items,
-                       seq_item, seq_keys, tok_seq, specials, turns);
+                       seq_item, seq_keys, tokens, specials, turns);
     hipLaunchKernelGGL(expand_kernel, dim3((unsigned)(8 * s.H * ((2 * num_cus + 8 * s.H - 1) / (8 * s.H)))), dim3(256), 0, stream, w, pool, b, s, seq_keys, specials,
                        l.key_rows, keys, shared);
     hipLaunchKernelGGL(chunk_attend_kernel, dim3((unsigned)s.groups), dim3(256), 0, stream, q, turns, keys, shared, s, plan, items,
                        l.key_rows, sums, stats, out);
-    hipLaunchKernelGGL(chunk_finish_kernel, dim3((unsigned)((b.n_rows * s.H + 15) / 16)), dim3(256), 0, stream, b, s, plan, items, seq_item,
-                       tok_seq, sums, stats, out);
+    hipLaunchKernelGGL(chunk_finish_kernel, dim3((unsigned)((b.n_rows * s.H + 15) / 16)), dim3(256), 0, stream, b.n_rows, s, plan, items,
+                       seq_item, tokens, sums, stats, out);
     return (int)hipGetLastError();
 }
 
