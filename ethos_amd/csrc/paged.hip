@@ -639,6 +639,16 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
             }
         };
 
+        // zeros for the latents of these rows, by all waves, once every wave has its scores
+        auto clear_odd = [&](uint64_t odd, uint32_t at) {
+            lds_barrier();
+            for (int e = tid; e < kKeys * 32; e += W * 64) {
+                const int r = e & 63, c = e >> 6;
+                if (odd >> r & 1) *(lds_u4_ptr)(size_t)(at + (c >> 3) * kPlane + r * 128 + (c & 7) * 16) = u32x4_t{0, 0, 0, 0};
+            }
+            lds_barrier();
+        };
+        const bool active = wr * 16 < it.rows;  // (a wave without rows of its own copies only)
         load_pages(k_begin);
         Frag fq[kWidth / 32];
         {
@@ -685,6 +695,8 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
                 odd = ballot(bad);
             }
             f32x4_t x[KB];
+            if (odd != 0 && !active) clear_odd(odd, at);
+            if (!active) continue;
 #pragma unroll
             for (int i = 0; i < KB; ++i) x[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -710,12 +722,7 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
                         const int key = 16 * i + 4 * g + e;
                         if ((odd >> (wave_key + key) & 1) && key0 + key <= my_pos) l = NAN;
                     }
-                lds_barrier();
-                for (int e = tid; e < kKeys * 32; e += W * 64) {
-                    const int r = e & 63, c = e >> 6;
-                    if (odd >> r & 1) *(lds_u4_ptr)(size_t)(at + (c >> 3) * kPlane + r * 128 + (c & 7) * 16) = u32x4_t{0, 0, 0, 0};
-                }
-                lds_barrier();
+                clear_odd(odd, at);
             }
             float top = x[0][0];
 #pragma unroll
