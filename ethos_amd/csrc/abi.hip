@@ -1264,7 +1264,7 @@ int verify_sizes(int64_t n_seq, int32_t n_drafts, int64_t vocab, const char* wha
 
 size_t ethos_verify_workspace_bytes(int64_t n_seq, int32_t n_drafts, int64_t vocab) {
     if (n_seq == 0 || verify_sizes(n_seq, n_drafts, vocab, "ethos_verify_workspace_bytes") != 0) return 256;
-    return ethos::verify_workspace_bytes(n_seq, n_drafts, vocab);
+    return ethos::verify_workspace_bytes(n_seq, n_drafts, vocab, num_cus());
 }
 
 int ethos_verify(const void* logits, const int64_t* drafts, const void* probs, int32_t probs_dtype, const int32_t* counts,
@@ -1279,12 +1279,12 @@ int ethos_verify(const void* logits, const int64_t* drafts, const void* probs, i
     if (n_seq == 0) return 0;
     if (!logits || (n_drafts > 0 && (!drafts || !u_accept)) || !u_sample || !workspace || !accepted || !tokens)
         return fail(ETHOS_ENULL, "ethos_verify: null pointer");
-    const size_t need = ethos::verify_workspace_bytes(n_seq, n_drafts, vocab);
+    const size_t need = ethos::verify_workspace_bytes(n_seq, n_drafts, vocab, num_cus());
     if (workspace_bytes < need) return fail(ETHOS_EWORKSPACE, "ethos_verify: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     if (!aligned16(workspace) || !aligned_to(logits, dtype) || !aligned_to(probs, probs_dtype))
         return fail(ETHOS_EALIGN, "ethos_verify: logits, probs or workspace misaligned");
     return hip_status(ethos::launch_verify(logits, drafts, probs, probs_dtype, counts, u_accept, u_sample, n_seq, n_drafts, vocab, temperature,
-                                           dtype, workspace, accepted, tokens, (hipStream_t)stream),
+                                           dtype, workspace, accepted, tokens, num_cus(), (hipStream_t)stream),
                       "ethos_verify");
 }
 

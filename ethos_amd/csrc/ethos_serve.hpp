@@ -78,9 +78,9 @@ size_t paged_attention_workspace_bytes(int64_t n_rows, int n_seq, int H, int ran
 int launch_paged_attention(const void* q, const void* w, const void* pool, const Batch& b, const float* rates, int H, int rank, int rope,
                            int nope, int v_dim, int dtype, float scale, void* ws, void* out, int num_cus, hipStream_t stream);
 
-size_t verify_workspace_bytes(int64_t n_seq, int n_drafts, int64_t vocab);
+size_t verify_workspace_bytes(int64_t n_seq, int n_drafts, int64_t vocab, int num_cus);
 int launch_verify(const void* logits, const int64_t* drafts, const void* probs, int probs_dtype, const int32_t* counts,
                   const float* u_accept, const float* u_sample, int64_t n_seq, int n_drafts, int64_t vocab, double temperature, int dtype,
-                  void* ws, int32_t* accepted, int64_t* tokens, hipStream_t stream);
+                  void* ws, int32_t* accepted, int64_t* tokens, int num_cus, hipStream_t stream);
 
 }  // namespace ethos

@@ -831,44 +831,53 @@ def clip_grads(src: list, dst: list, sizes: list, codes: list, device: torch.dev
 # ----------------------------------------------------------- operators of serving from a cache
 def _batch(pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor, rates: torch.Tensor, rope: int):
     """Checks a batch over a cache: (table's row distance, its width, sequences)."""
-    _need_here(pool, "pool", FLOATS, 3)
-    _need_here(lens, "lens", (torch.int32,), 1)
-    _need_here(starts, "starts", (torch.int32,), 1)
-    _need_here(rates, "rates", (torch.float32,), 1)
-    if not isinstance(table, torch.Tensor) or table.get_device() != pool.get_device() or table.dtype != torch.int32 or table.dim() != 2:
+    device = _current_device()
+    if not (_dense_at(device, pool) and pool.dtype in FLOATS and pool.dim() == 3 and _dense_at(device, lens, torch.int32) and lens.dim() == 1
+            and _dense_at(device, starts, torch.int32) and starts.dim() == 1 and _dense_at(device, rates, torch.float32) and rates.dim() == 1):
+        _need_here(pool, "pool", FLOATS, 3)
+        _need_here(lens, "lens", (torch.int32,), 1)
+        _need_here(starts, "starts", (torch.int32,), 1)
+        _need_here(rates, "rates", (torch.float32,), 1)
+    if not isinstance(table, torch.Tensor) or table.get_device() != device or table.dtype != torch.int32 or table.dim() != 2:
         raise RuntimeError(f"table must be an int32 tensor [sequences, pages] on {pool.device}")
     n, width = table.shape
-    if width > 1 and table.stride(1) != 1 or n > 1 and table.stride(0) < width:
-        raise RuntimeError(f"table must have contiguous rows, got strides {table.stride()}")
-    if lens.numel() != n or starts.numel() != n + 1:
+    ld = width
+    if not table.is_contiguous():
+        ld = table.stride(0) if n > 1 else width
+        if width > 1 and table.stride(1) != 1 or ld < width:
+            raise RuntimeError(f"table must have contiguous rows, got strides {table.stride()}")
+    if lens.shape[0] != n or starts.shape[0] != n + 1:
         raise RuntimeError(f"{n} rows of table need as many lens and one more of starts, got {lens.numel()} and {starts.numel()}")
-    if rope % 2 or rates.numel() != rope // 2:
+    if rope % 2 or rates.shape[0] != rope // 2:
         raise RuntimeError(f"rates must have {rope // 2} values for a rotary width of {rope}, got {rates.numel()}")
-    return (table.stride(0) if n > 1 else width), width, n
+    return ld, width, n
 
 
 def latent_append(rows: torch.Tensor, gain: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
                   starts: torch.Tensor, rates: torch.Tensor, eps: float) -> None:
     """Writes the cache's rows of the new tokens' rows [n, rank + rope] (evenly spaced) into the pool."""
-    rank = gain.numel()
-    _need_here(gain, "gain", FLOATS, 1)
-    ld, width, n_seq = _batch(pool, table, lens, starts, rates, pool.shape[-1] - rank)
-    if not isinstance(rows, torch.Tensor) or rows.get_device() != pool.get_device() or rows.dtype != pool.dtype or gain.dtype != pool.dtype:
-        raise RuntimeError(f"rows and gain must be {pool.dtype} on {pool.device}")
-    if rows.dim() != 2 or rows.shape[1] != pool.shape[2] or rows.stride(1) != 1:
-        raise RuntimeError(f"rows must be [n, {pool.shape[2]}] with contiguous rows, got {tuple(rows.shape)} of strides {rows.stride()}")
-    rc = load().ethos_latent_append(rows.data_ptr(), rows.stride(0) if rows.shape[0] > 1 else rows.shape[1], gain.data_ptr(), rates.data_ptr(),
-                                    table.data_ptr(), ld, width, lens.data_ptr(), starts.data_ptr(), n_seq, rows.shape[0], rank,
-                                    pool.shape[2] - rank, pool.shape[0], pool.shape[1], float(eps), dtype_code(pool.dtype), pool.data_ptr(),
-                                    _stream())
+    rank, dtype = gain.numel(), pool.dtype
+    pages, page, wide = pool.shape
+    ld, width, n_seq = _batch(pool, table, lens, starts, rates, wide - rank)
+    device = pool.get_device()
+    if not _dense_at(device, gain, dtype) or not isinstance(rows, torch.Tensor) or rows.get_device() != device or rows.dtype != dtype:
+        raise RuntimeError(f"rows and gain must be {dtype} on {pool.device}, gain contiguous")
+    if rows.dim() != 2 or rows.shape[1] != wide or rows.stride(1) != 1 or gain.dim() != 1:
+        raise RuntimeError(f"rows must be [n, {wide}] with contiguous rows, got {tuple(rows.shape)} of strides {rows.stride()}")
+    n = rows.shape[0]
+    rc = load().ethos_latent_append(rows.data_ptr(), rows.stride(0) if n > 1 else wide, gain.data_ptr(), rates.data_ptr(), table.data_ptr(), ld,
+                                    width, lens.data_ptr(), starts.data_ptr(), n_seq, n, rank, wide - rank, pages, page, eps,
+                                    int(dtype == torch.bfloat16), pool.data_ptr(), _stream())
     check(rc, "ethos_latent_append")
 
 
 def paged_attention(q: torch.Tensor, w: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, starts: torch.Tensor,
                     rates: torch.Tensor, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [n, heads, nope + rope] over the cache -> [n, heads v_dim]."""
-    _need_here(q, "q", FLOATS, 3)
-    _need_here(w, "weight", FLOATS, 2)
+    device = _current_device()
+    if not (_dense_at(device, q) and q.dtype in FLOATS and q.dim() == 3 and _dense_at(device, w) and w.dtype in FLOATS and w.dim() == 2):
+        _need_here(q, "q", FLOATS, 3)
+        _need_here(w, "weight", FLOATS, 2)
     n, H, qw = q.shape
     rank = w.shape[1]
     rope = pool.shape[-1] - rank
@@ -898,12 +907,14 @@ def paged_attention(q: torch.Tensor, w: torch.Tensor, pool: torch.Tensor, table:
 def copy_pages(pool: torch.Tensor, src: list, dst: list) -> None:
     """Copies pages src[i] to dst[i] in every block of pool [blocks, pages, ...]."""
     a, b = array.array("i", src), array.array("i", dst)
-    size = pool.element_size()
-    pages, page_bytes = pool.shape[1], pool[0, 0].numel() * size if pool.numel() else 0
-    if page_bytes == 0 or not src:
+    if not src or pool.numel() == 0:
         return
+    pages = pool.shape[1]
+    page_bytes = pool.numel() // (pool.shape[0] * pages) * pool.element_size()
     rc = load().ethos_copy_pages(pool.data_ptr(), pool.shape[0], pages * page_bytes, pages, page_bytes, a.buffer_info()[0], b.buffer_info()[0],
                                  len(a), _stream())
+    if rc == -2:
+        raise IndexError(load().ethos_last_error().decode(errors="replace"))
     check(rc, "ethos_copy_pages")
 
 

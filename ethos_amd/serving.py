@@ -20,22 +20,35 @@ from . import hip, training
 __all__ = ["copy_pages", "latent_append", "paged_attention", "verify_drafts"]
 
 
+_requires_grad = operator.attrgetter("requires_grad")
+
+
 def _check(what: str, *ts) -> None:
     """Refuses what the kernels would hide from autograd, and other devices than the current one."""
     if training._is_followed():
         training._refuse_followed(what, *ts)
-    grad = torch.is_grad_enabled()
-    for t in ts:
-        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == hip._current_device()):
+    try:
+        devices = set(map(torch.Tensor.get_device, ts))
+    except TypeError:
+        devices = {-1}
+    if -1 in devices or devices != {hip._current_device()}:
+        for t in ts:
             training._device_check(f"{what}: an input", t)
-        if grad and t.requires_grad:
-            raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
+    if torch.is_grad_enabled() and any(map(_requires_grad, ts)):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
 
 
 def _written(t: torch.Tensor) -> None:
     """t was written by address."""
     if not t.is_inference():
         torch.autograd.graph.increment_version(t)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t [n, d], or a copy of it, as rows that the kernels can read: evenly spaced, 16-byte aligned."""
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.stride(0) * t.element_size() % 16 == 0 and t.stride(0) >= t.shape[1] or t.shape[0] < 2):
+        return t
+    return training._dense(t)
 
 
 def latent_append(rows: torch.Tensor, gain: torch.Tensor, pool: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
@@ -50,14 +63,11 @@ def latent_append(rows: torch.Tensor, gain: torch.Tensor, pool: torch.Tensor, ta
     (float32 [rope / 2], Rotary.rates), computed in float32 and rounded once.  Rows of no sequence, positions
     without a page and pages outside the pool are left out.  The sequences' new tokens may not share places."""
     _check("latent_append", rows, gain, pool, table, lens, starts, rates)
-    if rows.dim() != 2 or gain.dim() != 1 or pool.dim() != 3:
-        raise RuntimeError(f"latent_append: rows, gain and pool must have 2, 1 and 3 dims, got {tuple(rows.shape)}, {tuple(gain.shape)} and "
-                           f"{tuple(pool.shape)}")
-    if rows.shape[1] != pool.shape[2] or gain.numel() > rows.shape[1]:
+    if pool.dim() != 3 or rows.dim() != 2 or gain.dim() != 1 or rows.shape[1] != pool.shape[2] or gain.shape[0] > pool.shape[2]:
         raise RuntimeError(f"latent_append: inconsistent shapes {tuple(rows.shape)}, {tuple(gain.shape)} and {tuple(pool.shape)}")
-    if rows.dtype not in hip.FLOATS or rows.dtype != pool.dtype or gain.dtype != pool.dtype:
+    if pool.dtype not in hip.FLOATS or rows.dtype != pool.dtype or gain.dtype != pool.dtype:
         raise TypeError(f"rows, gain and pool must all be bfloat16 or all float32, got {rows.dtype}, {gain.dtype} and {pool.dtype}")
-    hip.latent_append(training._rows(rows), training._dense(gain), pool, table, lens, starts, rates, eps)
+    hip.latent_append(_rows(rows), training._dense(gain), pool, table, lens, starts, rates, eps)
     _written(pool)
 
 
@@ -82,15 +92,12 @@ def paged_attention(q: torch.Tensor, weight: torch.Tensor, pool: torch.Tensor, t
     return o
 
 
-def _page_list(name: str, v, n_pages: int) -> list:
+def _page_list(name: str, v) -> list:
     if isinstance(v, torch.Tensor):
         if v.is_cuda:
             raise TypeError(f"copy_pages: {name} must be on the host (a list, or a CPU tensor)")
-        v = v.tolist()
-    v = [operator.index(x) for x in v]
-    if v and not (0 <= min(v) and max(v) < n_pages):
-        raise IndexError(f"copy_pages: {name} holds pages outside the pool's {n_pages}")
-    return v
+        return v.tolist()
+    return v if isinstance(v, list) else list(v)
 
 
 def copy_pages(pool: torch.Tensor, src, dst) -> None:
@@ -101,7 +108,7 @@ def copy_pages(pool: torch.Tensor, src, dst) -> None:
     if pool.dim() < 3 or not pool.is_contiguous() or pool.element_size() not in (2, 4):
         raise RuntimeError(f"copy_pages: pool must be contiguous [blocks, pages, ...] of 2 or 4 bytes a value, got {tuple(pool.shape)} "
                            f"{pool.dtype}")
-    src, dst = _page_list("src", src, pool.shape[1]), _page_list("dst", dst, pool.shape[1])
+    src, dst = _page_list("src", src), _page_list("dst", dst)
     if len(src) != len(dst):
         raise ValueError(f"copy_pages: {len(src)} pages to copy but {len(dst)} places")
     to = set(dst)

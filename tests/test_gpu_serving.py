@@ -529,7 +529,7 @@ def _verify_case(b, m, V, dt, probs, seed, spread=2.5):
 
 @pytest.mark.parametrize("probs", ["fp32", "bf16", "none"])
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
-@pytest.mark.parametrize("b,m,V", [(1, 0, 1), (3, 0, 777), (2, 1, 2), (5, 3, 100), (7, 4, 8191), (4, 2, 8193), (2, 9, 20001), (1, 255, 33)])
+@pytest.mark.parametrize("b,m,V", [(1, 0, 1), (3, 0, 777), (2, 1, 2), (5, 3, 100), (7, 4, 8191), (4, 2, 8193), (2, 9, 20001), (1, 255, 33), (200, 2, 6000), (1, 1, 2200000)])
 def test_verify_against_float64(b, m, V, dt, probs):
     for temperature in (1.0, 0.6, 0.0):
         logits, drafts, ua, us, p = _verify_case(b, m, V, dt, probs, seed=b * 100 + V)
@@ -672,7 +672,7 @@ def test_refusals():
     pool = torch.zeros(2, 5, 4, 8, device="cuda")
     for src, dst, error in (([0], [5], IndexError), ([-1], [2], IndexError), ([0, 1], [2, 2], ValueError), ([0, 1], [1, 2], ValueError),
                             ([0], [0], ValueError), ([0, 1], [2], ValueError), ([0.5], [1], TypeError),
-                            (torch.tensor([0], device="cuda"), [1], TypeError)):
+                            (torch.tensor([0], device="cuda"), [1], TypeError), ([2 ** 40], [1], OverflowError), ([0, 5], [1, 2], IndexError)):
         with pytest.raises(error):
             ethos_amd.copy_pages(pool, src, dst)
     for bad in (pool.transpose(0, 1), pool[0, 0], pool.double(), pool.cpu()):
