@@ -14,13 +14,14 @@ from .layer import (  # noqa: F401
     ProductKeyRouter,
     SimplifiedHypernetMoE,
 )
-from .serving import copy_pages, latent_append, paged_attention, verify_drafts  # noqa: F401
+from .serving import LatentCache, copy_pages, latent_append, paged_attention, verify_drafts  # noqa: F401
 from .training import balance_loss, clip_grads, embedding, linear_cross_entropy  # noqa: F401
 
 __all__ = [
     "EthosExpertLayer",
     "ExpertGenerationNetwork",
     "FusedLowRankMoE_Reordered",
+    "LatentCache",
     "ProductKeyRouter",
     "SimplifiedHypernetMoE",
     "balance_loss",

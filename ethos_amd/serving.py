@@ -4,6 +4,9 @@
   paged_attention  latent attention of the new tokens over the cache
   copy_pages       pages of the cache copied, in every block's part at once
   verify_drafts    drafted tokens accepted or not by the model's probabilities, the token after them
+  LatentCache      the pages of a cache, and which sequence has which: extend, truncate, fork, free, compact
+
+CompressedMoEModel.extend and .speculate run them in the model's blocks.
 
 The reference has no cache and decodes nothing; its attention forms every token's keys and values anew
 (model.py:104-160).  Inputs are HIP tensors on the current device, bf16 or float32; there is no CPU path.
@@ -12,12 +15,14 @@ tensors that ask for one, forward-mode derivatives and torch.jit.trace are refus
 from __future__ import annotations
 
 import operator
+from array import array
+from typing import NamedTuple
 
 import torch
 
 from . import hip, training
 
-__all__ = ["copy_pages", "latent_append", "paged_attention", "verify_drafts"]
+__all__ = ["Batch", "LatentCache", "copy_pages", "latent_append", "paged_attention", "verify_drafts"]
 
 
 _requires_grad = operator.attrgetter("requires_grad")
@@ -138,3 +143,168 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u_accept: torch.Te
             raise TypeError(f"{name} must be {' or '.join(str(k) for k in kinds)}, got {t.dtype}")
     dense = [None if t is None else t.contiguous() for t in (logits, drafts, draft_probs, counts, u_accept, u_sample)]
     return hip.verify(*dense, temperature)
+
+
+# -------------------------------------------------------------------------- the cache
+class Batch(NamedTuple):
+    """New tokens of several sequences, as latent_append and paged_attention take them (int32, on the device)."""
+
+    table: torch.Tensor   # [sequences, pages]
+    lens: torch.Tensor    # [sequences], the new tokens included
+    starts: torch.Tensor  # [sequences + 1]: the rows of each one's new tokens
+    counts: list          # how many each has, on the host
+
+
+class _Sequence:
+    __slots__ = ("length", "pages")
+
+    def __init__(self, length: int, pages: array):
+        self.length, self.pages = length, pages
+
+
+class LatentCache:
+    """A cache of latents for `blocks` attention blocks in `pages` pages of `page` tokens (a power of two), and the
+    sequences in it.  pool [blocks, pages, page, rank + rope] holds, per token and block, the normalised latent and the rotated
+    key: in bf16 640 bytes for rank 256 and rope 64.  A page number stands for the same page of every block.
+
+    Which page is whose is known on the host: no call waits for the device.  `extend` makes room for new tokens and
+    gives the batch that the operators take; a fork shares its pages, and a shared page is copied when one of its
+    sequences first writes in it.  The device's work (page copies, the batch's tensors) is enqueued on the current stream:
+    use a cache on one stream, or let streams wait for each other."""
+
+    def __init__(self, blocks: int, rank: int, rope: int, pages: int, page: int = 64, dtype: torch.dtype = torch.bfloat16, device=None):
+        if blocks <= 0 or pages <= 0 or rank <= 0 or rope < 0:
+            raise ValueError(f"LatentCache: blocks, pages and rank must be positive, got {blocks}, {pages} and {rank}")
+        if page <= 0 or page & (page - 1) or page > 65536:
+            raise ValueError(f"LatentCache: page must be a power of two up to 65536, got {page}")
+        if dtype not in hip.FLOATS:
+            raise TypeError(f"LatentCache: dtype must be bfloat16 or float32, got {dtype}")
+        self.page, self.rank, self.rope = page, rank, rope
+        # (never-written memory is never read, but a NaN in it would be by a caller's own sums over pages)
+        self.pool = torch.zeros((blocks, pages, page, rank + rope), dtype=dtype, device=device or "cuda")
+        self._users = [0] * pages                       # sequences that have the page
+        self._free = array("i", range(pages - 1, -1, -1))  # the lowest is given out first
+        self._sequences: dict[int, _Sequence] = {}
+        self._next = 0
+
+    @property
+    def pages_free(self) -> int:
+        return len(self._free)
+
+    def _of(self, seq: int) -> _Sequence:
+        try:
+            return self._sequences[seq]
+        except KeyError:
+            raise KeyError(f"the cache has no sequence {seq}") from None
+
+    def new(self) -> int:
+        """An empty sequence's number."""
+        seq, self._next = self._next, self._next + 1
+        self._sequences[seq] = _Sequence(0, array("i"))
+        return seq
+
+    def length(self, seq: int) -> int:
+        return self._of(seq).length
+
+    def pages(self, seq: int) -> list:
+        """The page numbers of a sequence, in order."""
+        return self._of(seq).pages.tolist()
+
+    def fork(self, seq: int) -> int:
+        """A new sequence of the same tokens, on the same pages."""
+        s = self._of(seq)
+        new = self.new()
+        self._sequences[new] = _Sequence(s.length, array("i", s.pages))
+        for p in s.pages:
+            self._users[p] += 1
+        return new
+
+    def _drop(self, pages) -> None:
+        for p in pages:
+            self._users[p] -= 1
+            if self._users[p] == 0:
+                self._free.append(p)
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Forgets a sequence's tokens from `length` on."""
+        s = self._of(seq)
+        if not 0 <= length <= s.length:
+            raise ValueError(f"sequence {seq} has {s.length} tokens, it cannot be cut to {length}")
+        keep = -(-length // self.page)
+        self._drop(reversed(s.pages[keep:]))
+        del s.pages[keep:]
+        s.length = length
+
+    def free(self, seq: int) -> None:
+        """Forgets a sequence."""
+        self.truncate(seq, 0)
+        del self._sequences[seq]
+
+    def extend(self, seqs, counts) -> Batch:
+        """Room for counts[i] new tokens of sequence seqs[i]: their batch, in that order.  With too few free pages it raises
+        RuntimeError and changes nothing."""
+        seqs, counts = list(seqs), [operator.index(c) for c in counts]
+        if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or any(c < 0 for c in counts):
+            raise ValueError("extend: each sequence once, with the number of its new tokens")
+        own = [self._of(q) for q in seqs]
+        # shared pages that new tokens go to; of several batch sequences that share one, each but a last sole user copies it
+        copies, users = [], {}
+        need = 0
+        for i, (s, c) in enumerate(zip(own, counts)):
+            need += -(-(s.length + c) // self.page) - len(s.pages)
+            if c and s.length % self.page:
+                p = s.pages[-1]
+                left = users.get(p, self._users[p])
+                if left > 1:
+                    copies.append(i)
+                    users[p] = left - 1
+        if need + len(copies) > len(self._free):
+            raise RuntimeError(f"the cache has {len(self._free)} free pages, {need + len(copies)} are needed")
+        src, dst = [], []
+        for i in copies:
+            p = own[i].pages[-1]
+            src.append(p)
+            dst.append(self._free.pop())
+            self._users[p] -= 1
+            self._users[dst[-1]] = 1
+            own[i].pages[-1] = dst[-1]
+        if src:
+            copy_pages(self.pool, src, dst)
+        for s, c in zip(own, counts):
+            s.length += c
+            while len(s.pages) * self.page < s.length:
+                p = self._free.pop()
+                self._users[p] = 1
+                s.pages.append(p)
+        return self._batch(own, counts)
+
+    def _batch(self, own, counts) -> Batch:
+        """The batch's arrays, in one copy to the device."""
+        width, n = max([len(s.pages) for s in own], default=0), len(own)
+        flat = array("i", [s.length for s in own])
+        at = 0
+        flat.append(0)
+        for c in counts:
+            at += c
+            flat.append(at)
+        for s in own:
+            flat.extend(s.pages)
+            flat.extend(array("i", [-1]) * (width - len(s.pages)))
+        dev = torch.frombuffer(flat, dtype=torch.int32).to(self.pool.device)
+        return Batch(dev[2 * n + 1:].view(n, width), dev[:n], dev[n:2 * n + 1], counts)
+
+    def compact(self) -> int:
+        """Moves pages so that those in use are the first of the pool (which a caller may then copy into a smaller one);
+        their number.  Batches given out before are no longer valid."""
+        used = len(self._users) - len(self._free)
+        holes = [p for p in range(used) if self._users[p] == 0]
+        moved = [p for p in range(used, len(self._users)) if self._users[p] > 0]
+        if moved:
+            copy_pages(self.pool, moved, holes)
+            to = dict(zip(moved, holes))
+            for p, q in to.items():
+                self._users[q], self._users[p] = self._users[p], 0
+            for s in self._sequences.values():
+                s.pages = array("i", [to.get(p, p) for p in s.pages])
+        self._free = array("i", range(len(self._users) - 1, used - 1, -1))
+        return used

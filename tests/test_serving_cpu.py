@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import ethos_amd
-from ethos_amd import _lib
+from ethos_amd import _lib, serving
 
 BIG = 1 << 60
 
@@ -101,3 +101,151 @@ def test_operators_have_no_cpu_path():
             call()
     with pytest.raises(TypeError):
         ethos_amd.copy_pages([1], [0], [1])
+
+
+# ------------------------------------------------------------------------------- the cache's books
+def _book(monkeypatch, pages=12, page=4):
+    """A cache on the host, with the page copies done there."""
+    def copy(pool, src, dst):
+        assert len(set(dst)) == len(dst) and not set(dst) & set(src)
+        pool[:, dst] = pool[:, src]
+
+    monkeypatch.setattr(serving, "copy_pages", copy)
+    return serving.LatentCache(2, 8, 8, pages, page, torch.float32, "cpu")
+
+
+def _write(c, batch, values):
+    """Writes values[i] (a number a new token) of sequence i of the batch into the pool."""
+    for i, vs in enumerate(values):
+        first = int(batch.lens[i]) - len(vs)
+        assert int(batch.starts[i + 1] - batch.starts[i]) == len(vs)
+        for j, v in enumerate(vs):
+            p = first + j
+            c.pool[:, int(batch.table[i, p // c.page]), p % c.page] = v
+
+
+def _read(c, seq):
+    t = c.pages(seq)
+    return [float(c.pool[0, t[p // c.page], p % c.page, 0]) for p in range(c.length(seq))]
+
+
+def _consistent(c):
+    users = [0] * len(c._users)
+    for s in c._sequences.values():
+        assert len(s.pages) == -(-s.length // c.page)
+        for p in s.pages:
+            users[p] += 1
+    assert users == c._users
+    assert sorted(c._free) == [p for p, n in enumerate(users) if n == 0]
+
+
+def test_cache_keeps_every_sequence_its_tokens(monkeypatch):
+    c = _book(monkeypatch)
+    a, b = c.new(), c.new()
+    _write(c, c.extend([a, b], [6, 3]), [[1, 2, 3, 4, 5, 6], [11, 12, 13]])
+    assert c.length(a) == 6 and c.pages_free == 9
+    f = c.fork(a)
+    g = c.fork(a)
+    assert c.pages(f) == c.pages(a) and c.pages_free == 9
+    # all three write in the page that they share: two of them get a copy of it
+    _write(c, c.extend([a, f, g], [1, 2, 3]), [[7], [70, 80], [700, 800, 900]])
+    assert _read(c, a) == [1, 2, 3, 4, 5, 6, 7] and _read(c, f) == [1, 2, 3, 4, 5, 6, 70, 80]
+    assert _read(c, g) == [1, 2, 3, 4, 5, 6, 700, 800, 900] and _read(c, b) == [11, 12, 13]
+    _consistent(c)
+    c.truncate(g, 4)
+    c.truncate(f, 3)  # into a page that a and g have too
+    _write(c, c.extend([f, b], [1, 0]), [[33], []])
+    assert _read(c, f) == [1, 2, 3, 33] and _read(c, g) == [1, 2, 3, 4] and _read(c, a) == [1, 2, 3, 4, 5, 6, 7]
+    _consistent(c)
+    c.free(a)
+    c.free(b)
+    _consistent(c)
+    used = c.compact()
+    assert used == 2 and sorted(c.pages(f) + c.pages(g)) == [0, 1] and _read(c, f) == [1, 2, 3, 33] and _read(c, g) == [1, 2, 3, 4]
+    _consistent(c)
+    assert c.pages_free == 10 and c.compact() == 2
+    with pytest.raises(KeyError):
+        c.length(a)
+
+
+def test_cache_compacts_shared_pages(monkeypatch):
+    c = _book(monkeypatch, pages=9, page=2)
+    a, b = c.new(), c.new()
+    for k in range(4):
+        _write(c, c.extend([a], [2]), [[k, k + 0.5]])
+        _write(c, c.extend([b], [2]), [[10 + k, 10 + k + 0.5]])
+    f = c.fork(b)
+    c.free(a)
+    assert c.compact() == 4
+    assert sorted(c.pages(b)) == [0, 1, 2, 3] and c.pages(f) == c.pages(b)
+    assert _read(c, b) == _read(c, f) == [10, 10.5, 11, 11.5, 12, 12.5, 13, 13.5]
+    _consistent(c)
+
+
+def test_cache_refuses_and_changes_nothing(monkeypatch):
+    c = _book(monkeypatch, pages=3, page=4)
+    a, b = c.new(), c.new()
+    c.extend([a], [6])
+    f = c.fork(a)
+    before = (c.pages(a), c.pages(f), c.pages_free, c.length(a))
+    for seqs, counts, error in (([a, b], [3, 1], RuntimeError), ([a, f], [3, 1], RuntimeError), ([b], [5], RuntimeError), ([a], [-1], ValueError),
+                                ([a, a], [1, 1], ValueError), ([a], [1, 2], ValueError), ([99], [1], KeyError), ([a], [1.5], TypeError)):
+        with pytest.raises(error):
+            c.extend(seqs, counts)
+        assert (c.pages(a), c.pages(f), c.pages_free, c.length(a)) == before, (seqs, counts)
+    for length in (-1, 7):
+        with pytest.raises(ValueError):
+            c.truncate(a, length)
+    for bad in (dict(blocks=0), dict(pages=0), dict(page=3), dict(page=0), dict(page=1 << 17), dict(rank=0), dict(rope=-2)):
+        with pytest.raises(ValueError):
+            serving.LatentCache(**{**dict(blocks=1, rank=8, rope=8, pages=2, page=4, device="cpu"), **bad})
+    with pytest.raises(TypeError):
+        serving.LatentCache(1, 8, 8, 2, 4, torch.float16, "cpu")
+    e = c.extend([], [])
+    assert e.table.shape[0] == 0 and e.starts.tolist() == [0]
+    c.extend([b], [0])
+    assert c.length(b) == 0
+
+
+def test_cache_against_a_plain_one(monkeypatch):
+    """Random steps, with lists of numbers beside the cache."""
+    import random
+
+    rng = random.Random(5)
+    c = _book(monkeypatch, pages=40, page=4)
+    plain = {}
+    for step in range(400):
+        do = rng.choice(["new", "extend", "extend", "extend", "fork", "truncate", "free", "compact"])
+        live = list(plain)
+        if do == "new" or not live:
+            plain[c.new()] = []
+        elif do == "extend":
+            seqs = rng.sample(live, min(len(live), rng.randint(1, 4)))
+            values = [[rng.randint(1, 999) for _ in range(rng.randint(0, 9))] for _ in seqs]
+            try:
+                batch = c.extend(seqs, [len(v) for v in values])
+            except RuntimeError:
+                c.free(live[0])
+                del plain[live[0]]
+                continue
+            _write(c, batch, values)
+            for q, v in zip(seqs, values):
+                plain[q] += v
+        elif do == "fork":
+            q = rng.choice(live)
+            plain[c.fork(q)] = list(plain[q])
+        elif do == "truncate":
+            q = rng.choice(live)
+            n = rng.randint(0, len(plain[q]))
+            c.truncate(q, n)
+            del plain[q][n:]
+        elif do == "free":
+            q = rng.choice(live)
+            c.free(q)
+            del plain[q]
+        else:
+            used = c.compact()
+            assert all(p < used for q in plain for p in c.pages(q))
+        _consistent(c)
+        for q, v in plain.items():
+            assert _read(c, q) == v
