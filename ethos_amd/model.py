@@ -33,7 +33,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import hip, training
+from . import hip, serving, training
 from .layer import EthosExpertLayer
 
 # the reference's configs/default.yaml, with the benchmarked expert-layer shape (d_query
@@ -170,6 +170,16 @@ class MLAttention(nn.Module):
             o = F.scaled_dot_product_attention(qh, kh, vh, attn_mask=attention_mask.to(x.dtype), scale=self.scale)
         return self.o_proj(o.transpose(1, 2)[..., : self.vdim].reshape(b, n, H * self.vdim))
 
+    def extend(self, x: torch.Tensor, pool: torch.Tensor, batch: serving.Batch) -> torch.Tensor:
+        """The attention of new tokens x [n, d] of a batch over their sequences' tokens in a cache [pages, page,
+        kv_rank + rope], which they are added to (ethos_amd.serving).  No gradients."""
+        a = F.linear(x, _stacked(self, (self.q_a_proj, self.kv_a_proj_with_mqa)))
+        rates = self.rotary.rates(x.device)
+        serving.latent_append(a[:, self.q_rank:], self.kv_a_layernorm.weight, pool, batch.table, batch.lens, batch.starts, rates,
+                              eps=self.kv_a_layernorm.eps)
+        q = self.q_b_proj(self.q_a_layernorm(a[:, : self.q_rank])).view(-1, self.n_heads, self.qk_width)
+        return self.o_proj(serving.paged_attention(q, self.kv_b_proj.weight, pool, batch.table, batch.lens, batch.starts, rates, self.scale))
+
 
 class FFN(nn.Module):
     """SwiGLU feed-forward of the dense blocks, w2(silu(w1 x) * (w3 x)) (model.py:257-265),
@@ -209,6 +219,13 @@ class TransformerBlock(nn.Module):
         return h + (self.mlp(y, routing) if routing is not None and isinstance(self.mlp, EthosExpertLayer) else self.mlp(y))
 
 
+    def extend(self, x, pool, batch):
+        """The block on new tokens x [n, d] of a batch over a cache (MLAttention.extend)."""
+        h = x + self.self_attn.extend(self.input_layernorm(x), pool, batch)
+        y = self.post_attention_layernorm(h)
+        return h + (self.mlp.forward_flat(y) if isinstance(self.mlp, EthosExpertLayer) else self.mlp(y))
+
+
 class LossParts(NamedTuple):
     """What CompressedMoEModel.loss returns."""
 
@@ -238,6 +255,73 @@ class CompressedMoEModel(nn.Module):
         for block in self.layers:
             h = block(h, None, pos)  # None: causal attention
         return self.output(self.norm(h))
+
+    def cache(self, pages: int, page: int = 64) -> serving.LatentCache:
+        """A cache for this model's sequences: pages of `page` tokens, in the model's dtype on its device."""
+        c, w = self.config, self.tok_embeddings.weight
+        return serving.LatentCache(len(self.layers), c.kv_lora_rank, c.qk_rope_head_dim, pages, page, w.dtype, w.device)
+
+    @torch.no_grad()
+    def extend(self, input_ids: torch.Tensor, cache: serving.LatentCache, seqs, counts=None, last_only: bool = False) -> torch.Tensor:
+        """Logits of the next tokens of sequences in a cache, which they are added to: a prompt or a chunk of one, a token, a
+        few, or any mixture.  input_ids [n] int64, counts[i] tokens of sequence seqs[i] after each other, or [batch, m],
+        m of each.  Returns [n, vocab] (or [batch, m, vocab]); with `last_only` those of each sequence's last token
+        [batch, vocab] alone.  The model must be in eval mode.  An id outside the vocabulary has NaN for its logits and
+        counts as the nearest one inside for what follows it.
+        (`forward` computes the same function of whole sequences, with other rounding points.)"""
+        if self.training:
+            raise RuntimeError("extend needs the model in eval mode")
+        if input_ids.dtype not in (torch.int64, torch.int32) or input_ids.dim() not in (1, 2) or (counts is None) != (input_ids.dim() == 2):
+            raise RuntimeError("extend takes ids [n] with counts, or [batch, m] without")
+        seqs = list(seqs)
+        counts = [input_ids.shape[1]] * input_ids.shape[0] if counts is None else list(counts)
+        if len(counts) != len(seqs) or sum(counts) != input_ids.numel():
+            raise RuntimeError(f"extend: {input_ids.numel()} ids for {len(seqs)} sequences with counts {counts}")
+        if last_only and not all(c > 0 for c in counts):
+            raise RuntimeError("extend: last_only needs a token of every sequence")
+        c, pool, w = self.config, cache.pool, self.tok_embeddings.weight
+        if (pool.shape[0], cache.rank, cache.rope, pool.dtype, pool.device) != (len(self.layers), c.kv_lora_rank, c.qk_rope_head_dim,
+                                                                               w.dtype, w.device):
+            raise RuntimeError("extend: the cache is not one of this model's (blocks, rank, rope, dtype or device)")
+        training._device_check("input_ids", input_ids)
+        batch = cache.extend(seqs, counts)
+        try:
+            ids = input_ids.reshape(-1)
+            inside = ids.clamp(0, c.vocab_size - 1)  # (a NaN would go through the blocks, and their routers order numbers)
+            h = training.embedding(inside, w)
+            if h.shape[0] > 0:
+                for block, pages in zip(self.layers, pool):
+                    h = block.extend(h, pages, batch)
+            h = h.masked_fill((ids != inside)[:, None], math.nan)
+            if last_only:
+                h = h[batch.starts[1:].long() - 1]
+            logits = self.output(self.norm(h))
+            return logits if last_only or input_ids.dim() == 1 else logits.view(*input_ids.shape, c.vocab_size)
+        except BaseException:
+            for s, n in zip(seqs, counts):
+                cache.truncate(s, cache.length(s) - n)
+            raise
+
+    @torch.no_grad()
+    def speculate(self, cache: serving.LatentCache, seqs, last: torch.Tensor, drafts: torch.Tensor, u_accept: torch.Tensor,
+                  u_sample: torch.Tensor, draft_probs: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+                  temperature: float = 1.0):
+        """One step of decoding with drafted tokens: (accepted, tokens), lists of how many of each sequence's drafts stand
+        and the token behind them.  last [b] int64: each sequence's last token, not yet in the cache; drafts [b, m] (m = 0:
+        plain sampling); the rest as serving.verify_drafts takes it.  The cache keeps `last` and the drafts that stand; the
+        token is the next call's `last`.  Waits for the device."""
+        seqs = list(seqs)
+        logits = self.extend(torch.cat((last.view(-1, 1), drafts), 1), cache, seqs)
+        try:
+            accepted, tokens = serving.verify_drafts(logits, drafts, u_accept, u_sample, draft_probs, counts, temperature)
+            accepted, tokens = accepted.tolist(), tokens.tolist()
+        except BaseException:
+            for s in seqs:
+                cache.truncate(s, cache.length(s) - drafts.shape[1] - 1)
+            raise
+        for s, a in zip(seqs, accepted):
+            cache.truncate(s, cache.length(s) - (drafts.shape[1] - a))
+        return accepted, tokens
 
     def loss(self, input_ids: torch.Tensor, labels: torch.Tensor, balance_weight: float = 0.0, ignore_index: int = -100) -> LossParts:
         """The training loss of token ids [batch, seq]: labels int64 [batch, seq], the token that each

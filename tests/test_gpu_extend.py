@@ -1,0 +1,220 @@
+"""The language model over a cache (CompressedMoEModel.extend and .speculate, LatentCache): append, attention, page copies
+and verification together, against the model's own forward over whole sequences.
+
+Tolerances.  float32: the same function with other rounding points (products of up to 128 terms, three blocks): each rounding is
+2^-24 of a value, some hundred of them in series stay under 1e-5 of the logits' norm, 1e-4 is allowed (as for the model itself
+against its fixture).  Routing is a choice among scores that far apart.  bf16: about 14 roundings in series in each of three
+blocks, each 2^-9 / sqrt(3) of its value in the mean square: sqrt(42) of them is 0.7 %; 3 % is allowed, four times that; the
+experts' outputs there are 1e-5 of the stream, so that another choice of theirs does not show."""
+import pytest
+import torch
+
+from ethos_amd import workloads
+from ethos_amd.model import CompressedMoEModel, init_random_, lm_config
+from ethos_amd.serving import LatentCache
+
+pytestmark = pytest.mark.gpu
+
+
+def _nerr(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm())
+
+
+_models = {}
+
+
+def _model(kind):
+    if kind not in _models:
+        if kind == "fp32":
+            cfg, sd, _ = workloads.make_lm_inputs(seed=3)
+            m = CompressedMoEModel(cfg)
+            m.load_state_dict(sd)
+            _models[kind] = m.cuda().eval()
+        else:
+            cfg = lm_config(**{**workloads.LM_TINY, "kv_lora_rank": 256, "qk_rope_head_dim": 64, "qk_nope_head_dim": 64, "v_head_dim": 64})
+            _models[kind] = init_random_(CompressedMoEModel(cfg), seed=4).to(torch.bfloat16).cuda().eval()
+    return _models[kind]
+
+
+def _ids(b, n, seed=0):
+    return torch.randint(0, 500, (b, n), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+def _forward(m, ids):
+    with torch.no_grad():
+        return m(ids)
+
+
+BOUND = {"fp32": 1e-4, "bf16": 3e-2}
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+@pytest.mark.parametrize("page", [1, 4, 64])
+@pytest.mark.parametrize("steps", [[37], [1] * 20, [13, 1, 9, 1, 1, 8, 4], [30, 0, 3]])
+def test_chunks_give_the_logits_of_the_whole(kind, page, steps):
+    m, n = _model(kind), sum(steps)
+    ids = _ids(3, n)
+    ref = _forward(m, ids)
+    cache = m.cache(pages=3 * -(-n // page), page=page)
+    seqs = [cache.new() for _ in range(3)]
+    out, at = [], 0
+    for k in steps:
+        out.append(m.extend(ids[:, at: at + k], cache, seqs))
+        at += k
+    out = torch.cat(out, 1)
+    assert out.shape == ref.shape and out.dtype == ref.dtype
+    assert all(cache.length(s) == n for s in seqs)
+    e = _nerr(out, ref)
+    print(f"{kind}, page {page}, steps {steps}: {e:.2e}", flush=True)
+    assert e < BOUND[kind]
+
+
+def test_long_chunks_bf16():
+    """Chunks of hundreds of tokens (keys and values formed first) beside single ones."""
+    m = _model("bf16")
+    ids = _ids(2, 700, seed=8)
+    ref = _forward(m, ids)
+    cache = m.cache(pages=30)
+    a, b = cache.new(), cache.new()
+    o1 = m.extend(torch.cat((ids[0, :500], ids[1, :3])), cache, [a, b], [500, 3])
+    o2 = m.extend(torch.cat((ids[1, 3:650], ids[0, 500:501])), cache, [b, a], [647, 1])
+    o3 = m.extend(torch.cat((ids[0, 501:], ids[1, 650:])), cache, [a, b], [199, 50])
+    out = torch.stack((torch.cat((o1[:500], o2[647:], o3[:199])), torch.cat((o1[500:], o2[:647], o3[199:]))))
+    assert _nerr(out, ref) < BOUND["bf16"]
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_ragged_batches_forks_truncation_and_compaction(kind):
+    m = _model(kind)
+    ids = _ids(4, 60, seed=1)
+    cache = m.cache(pages=80, page=8)
+    pad = cache.new()
+    m.extend(_ids(1, 60, seed=99), cache, [pad])
+    a, b, c = cache.new(), cache.new(), cache.new()
+    # prompts of different lengths in one call
+    flat = torch.cat((ids[0, :21], ids[1, :40], ids[2, :1]))
+    out = m.extend(flat, cache, [a, b, c], [21, 40, 1])
+    last = m.extend(torch.cat((ids[0, 21:23], ids[1, 40:41])), cache, [a, b], [2, 1], last_only=True)
+    ref = [_forward(m, ids[i: i + 1])[0] for i in range(3)]
+    assert _nerr(out, torch.cat((ref[0][:21], ref[1][:40], ref[2][:1]))) < BOUND[kind]
+    assert last.shape == (2, 500) and _nerr(last, torch.stack((ref[0][22], ref[1][40]))) < BOUND[kind]
+    # a fork goes its own way from a page that it shares
+    f = cache.fork(a)
+    other = torch.cat((ids[0, :23], ids[3, :20]))[None]
+    both = m.extend(torch.stack((ids[0, 23:43], ids[3, :20])), cache, [a, f])
+    assert _nerr(both[0], ref[0][23:43]) < BOUND[kind]
+    assert _nerr(both[1], _forward(m, other)[0, 23:]) < BOUND[kind]
+    # back to the fork's point, then on with the first one's tokens; pages move in between
+    cache.truncate(f, 23)
+    cache.free(pad)
+    before = cache.pages_free
+    used = cache.compact()
+    assert cache.pages_free == before and all(p < used for s in (a, b, c, f) for p in cache.pages(s))
+    out = m.extend(torch.cat((ids[0, 23:30], ids[1, 41:60], ids[2, 1:9], ids[0, 43:60])), cache, [f, b, c, a], [7, 19, 8, 17])
+    assert _nerr(out, torch.cat((ref[0][23:30], ref[1][41:60], ref[2][1:9], ref[0][43:60]))) < BOUND[kind]
+
+
+def test_speculation_gives_the_greedy_tokens_fp32():
+    """At temperature 0 the tokens are the greedy ones, whatever the drafts: right ones, wrong ones, none, padding."""
+    m, b, total = _model("fp32"), 3, 24
+    prompt = _ids(b, 9, seed=2)
+    ids = prompt
+    for _ in range(total):
+        ids = torch.cat((ids, _forward(m, ids)[:, -1].argmax(-1, keepdim=True)), 1)
+    want = [r.tolist()[9:] for r in ids.cpu()]
+    cache = m.cache(pages=40, page=4)
+    seqs = [cache.new() for _ in range(b)]
+    first = m.extend(prompt, cache, seqs, last_only=True)
+    got = [[t] for t in first.argmax(-1).tolist()]
+    gen, calls = torch.Generator().manual_seed(11), 0
+    while min(len(g) for g in got) < total - 4:
+        drafts, counts = [], []
+        for i in range(b):
+            d = (want[i] + [7] * 8)[len(got[i]): len(got[i]) + 4]
+            n = (calls + i) % 5
+            if (calls + i) % 3 == 0 and n > 1:
+                d[1] = (d[1] + 1) % 500
+            drafts.append(d[:n] + [-1] * (4 - n))
+            counts.append(n)
+        last = torch.tensor([g[-1] for g in got]).cuda()
+        acc, tok = m.speculate(cache, seqs, last, torch.tensor(drafts).cuda(), torch.rand((b, 4), generator=gen).cuda(),
+                               torch.rand((b,), generator=gen).cuda(), counts=torch.tensor(counts, dtype=torch.int32).cuda(), temperature=0.0)
+        for i in range(b):
+            assert 0 <= acc[i] <= counts[i]
+            got[i] += drafts[i][: acc[i]] + [tok[i]]
+            assert cache.length(seqs[i]) == 9 + len(got[i]) - 1
+        calls += 1
+    for i in range(b):
+        n = min(len(got[i]), total)
+        assert got[i][:n] == want[i][:n]
+    assert calls < total  # some drafts stood
+
+
+def test_sampling_without_drafts():
+    m = _model("fp32")
+    cache = m.cache(pages=20, page=4)
+    s = cache.new()
+    prompt = _ids(1, 6, seed=6)
+    m.extend(prompt[:, :5], cache, [s])
+    p = torch.softmax(_forward(m, prompt)[0, -1].double() / 0.7, -1).cumsum(0)
+    for u in (0.0, 0.25, 0.5, 0.999):
+        acc, tok = m.speculate(cache, [s], prompt[:, 5], torch.empty((1, 0), dtype=torch.int64, device="cuda"),
+                               torch.empty((1, 0), device="cuda"), torch.tensor([u]).cuda(), temperature=0.7)
+        assert acc == [0] and cache.length(s) == 6
+        low = 0.0 if tok[0] == 0 else float(p[tok[0] - 1])
+        assert low - 1e-4 <= u <= float(p[tok[0]]) + 1e-4
+        cache.truncate(s, 5)
+
+
+def test_ids_outside_the_vocabulary():
+    m = _model("fp32")
+    ids = _ids(2, 10, seed=7)
+    bad = ids.clone()
+    bad[0, 4], bad[0, 9], ids[0, 4], ids[0, 9] = -1, 1 << 40, 0, 499
+    cache = m.cache(pages=10)
+    out = m.extend(bad, cache, [cache.new(), cache.new()])
+    ref = _forward(m, ids)
+    assert bool(out[0, [4, 9]].isnan().all()) and not bool(out[1].isnan().any())
+    keep = [0, 1, 2, 3, 5, 6, 7, 8]
+    assert _nerr(out[0, keep], ref[0, keep]) < 1e-4 and _nerr(out[1], ref[1]) < 1e-4
+
+
+def test_refusals_leave_the_cache_as_it_was():
+    m = _model("fp32")
+    cache = m.cache(pages=4, page=4)
+    s, t = cache.new(), cache.new()
+    m.extend(_ids(1, 6), cache, [s])
+    ids = _ids(1, 4)
+
+    def state():
+        return cache.length(s), cache.length(t), cache.pages(s), cache.pages_free
+
+    before = state()
+    wrong = LatentCache(2, 32, 16, 4, 4, torch.float32)
+    u = torch.zeros((1, 1), device="cuda")
+    for call, error in (
+            (lambda: m.extend(_ids(1, 20), cache, [t]), RuntimeError),                      # too few pages
+            (lambda: m.extend(ids, cache, [s, t]), RuntimeError),                           # one row, two sequences
+            (lambda: m.extend(ids[0], cache, [s]), RuntimeError),                           # [n] without counts
+            (lambda: m.extend(ids, cache, [s], [4]), RuntimeError),                         # [batch, m] with counts
+            (lambda: m.extend(ids[0], cache, [s], [3]), RuntimeError),
+            (lambda: m.extend(ids[0], cache, [s, t], [4, 0], last_only=True), RuntimeError),
+            (lambda: m.extend(ids.float(), cache, [s]), RuntimeError),
+            (lambda: m.extend(ids.cpu(), cache, [s]), RuntimeError),
+            (lambda: m.extend(ids, cache, [77]), KeyError),
+            (lambda: m.extend(torch.cat((ids, ids)), cache, [s, s]), ValueError),
+            (lambda: m.extend(ids, wrong, [wrong.new()]), RuntimeError),
+            (lambda: m.speculate(cache, [s], ids[0, :1], ids[:, :1], u.double(), u[0]), TypeError),
+            (lambda: m.speculate(cache, [s], ids[0, :1], ids[:, :1], u, u[0], temperature=-1.0), Exception)):
+        with pytest.raises(error):
+            call()
+        assert state() == before
+    m.train()
+    try:
+        with pytest.raises(RuntimeError):
+            m.extend(ids, cache, [s])
+    finally:
+        m.eval()
+    assert state() == before
+    assert m.extend(ids[:, :0], cache, [s]).shape == (1, 0, 500)
+    assert m.extend(torch.empty((0,), dtype=torch.int64, device="cuda"), cache, [], []).shape == (0, 500)
