@@ -418,7 +418,14 @@ int launch_any(const T* q, const T* w, const T* pool, const Batch& b, const floa
 // rows' reads of one piece, and the transposing reads' 4 rows by 4 pieces, touch every bank once.  Rows go from
 // memory straight into LDS, eight rows of a page (which has at least eight) and a plane at a time; rows behind the last key
 // come from rows of zeros, rows without a page from rows of NaN, so that the loop has no bounds to check.
+//
+// The products' operands are bf16.  A value that is rounded for one goes in as two, its bf16 value and the bf16 value of
+// what that leaves (2^-16 of it): the exponentials, the joined sums before W_v, and 128 of a query's 320 columns.  With
+// all rounded once the outputs' error against 64 bits is 1.9 times that of their own rounding, so it is 1.35 times
+// (0.0022 of their norm; of this the queries' other columns are two thirds).  64 sequences of one token: 48.5 -> 49.8 us;
+// 16 of five: 40.5 -> 44.4; all columns of a query in two: 54.0 and 48.7, for 1.1 times.
 constexpr int kRank = 256, kRope = 64, kWidth = kRank + kRope;
+constexpr int kRest = 128, kQuery = kWidth + kRest;  // a row's query, and what bf16 leaves of its last kRest columns
 constexpr int kBlockLog = 3, kBlock = 1 << kBlockLog;  // rows of a copy
 constexpr int kPlane = kKeys * 128, kStage = kWidth / 64 * kPlane;
 
@@ -437,6 +444,12 @@ union Frag {
     s16x4_t h[2];
 };
 
+// Two values as bf16, and what that leaves of them, as bf16 too: 16 bits of precision in two products.
+__device__ __forceinline__ void split_bf16x2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    hi = pack_bf16x2(a, b);
+    lo = pack_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+}
+
 __device__ __forceinline__ int swizzle(int row) { return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1); }
 
 // 16 bytes a lane into LDS at lds + 16 times the lane (lds: wave-uniform), from an address or from base + off.
@@ -453,13 +466,13 @@ __device__ __forceinline__ void copies_barrier() { asm volatile("s_waitcnt vmcnt
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // The order of a stretch of code between branches: N LDS reads, then M times a matrix product and R reads, then the
-// last products (left to itself the compiler reads one fragment ahead, and every product waits for LDS).
-template <int N, int M, int R, int L>
+// last products (left to itself the compiler reads one fragment ahead, and every product waits for LDS).  P products at a time.
+template <int N, int M, int R, int L, int P = 1>
 __device__ __forceinline__ void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x100, N, 0);
 #pragma unroll
     for (int i = 0; i < M; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, P, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
     }
     __builtin_amdgcn_sched_group_barrier(0x8, L, 0);
@@ -541,13 +554,17 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
     }
     if (s.nope == 0) __syncthreads();
     if (t0 + (lane & 31) < b.n_rows) {
-        uint16_t* to = queries + (my_t * s.H + h) * kWidth + wave * 64 + 4 * half;
+        uint16_t* to = queries + (my_t * s.H + h) * kQuery + wave * 64 + 4 * half;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<uint2*>(to + 32 * i + 2 * e) =
-                    make_uint2(pack_bf16x2(acc[i][e], acc[i][e + 1]), pack_bf16x2(acc[i][e + 2], acc[i][e + 3]));
+            for (int e = 0; e < 16; e += 4) {
+                uint2 hi, lo;
+                split_bf16x2(acc[i][e], acc[i][e + 1], hi.x, lo.x);
+                split_bf16x2(acc[i][e + 2], acc[i][e + 3], hi.y, lo.y);
+                *reinterpret_cast<uint2*>(to + 32 * i + 2 * e) = hi;
+                if (wave * 64 >= kWidth - kRest) *reinterpret_cast<uint2*>(to + kRest + 32 * i + 2 * e) = lo;
+            }
     }
     for (int e = tid; e < 32 * (kRope / 2); e += 256) {
         const int64_t t = t0 + (e >> 5);
@@ -557,9 +574,13 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
         rotary_angle(pos[e >> 5], rates[p], c, sn);
         const uint16_t* r = q + (t * s.H + h) * qw + s.nope;
         const float u = bf16_bits_to_f32(r[p]), v = bf16_bits_to_f32(r[32 + p]);
-        uint16_t* to = queries + (t * s.H + h) * kWidth + kRank;
-        to[p] = f32_to_bf16_bits(u * c - v * sn);
-        to[32 + p] = f32_to_bf16_bits(v * c + u * sn);
+        uint16_t* to = queries + (t * s.H + h) * kQuery + kRank;
+        uint32_t hi, lo;
+        split_bf16x2(u * c - v * sn, v * c + u * sn, hi, lo);
+        to[p] = (uint16_t)hi;
+        to[32 + p] = (uint16_t)(hi >> 16);
+        to[kRest + p] = (uint16_t)lo;
+        to[kRest + 32 + p] = (uint16_t)(lo >> 16);
     }
 }
 
@@ -650,14 +671,14 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
         };
         const bool active = wr * 16 < it.rows;  // (a wave without rows of its own copies only)
         load_pages(k_begin);
-        Frag fq[kWidth / 32];
+        Frag fq[kQuery / 32];
         {
-            const uint16_t* qp = queries + ((int64_t)it.tok0 * s.H + it.row0 + my_row) * kWidth + 8 * g;
+            const uint16_t* qp = queries + ((int64_t)it.tok0 * s.H + it.row0 + my_row) * kQuery + 8 * g;
 #pragma unroll
-            for (int i = 0; i < kWidth / 32; ++i) fq[i].u = *reinterpret_cast<const u32x4_t*>(qp + 32 * i);
+            for (int i = 0; i < kQuery / 32; ++i) fq[i].u = *reinterpret_cast<const u32x4_t*>(qp + 32 * i);
             // (here, not in the loop, is where they are waited for)
 #pragma unroll
-            for (int i = 0; i < kWidth / 32; ++i) asm volatile("" : "+v"(fq[i].u));
+            for (int i = 0; i < kQuery / 32; ++i) asm volatile("" : "+v"(fq[i].u));
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
@@ -705,8 +726,9 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
                 for (int i = 0; i < KB; ++i) {
                     const bf16x8_t a = *(lds_frag_ptr)(size_t)(at + k_at[st & 1] + (st >> 1) * kPlane + i * 16 * 128);
                     x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, fq[st].f, x[i], 0, 0, 0);
+                    if (st >= (kWidth - kRest) / 32) x[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, fq[st + kRest / 32].f, x[i], 0, 0, 0);
                 }
-            reads_ahead<8, KB * kWidth / 32 - 8, 1, 8>();
+            reads_ahead<8, KB * kWidth / 32 - 8, 1, 8 + KB * kRest / 32>();
             if (key0 + 16 * KB - 1 > wave_pos) {
 #pragma unroll
                 for (int i = 0; i < KB; ++i)
@@ -739,27 +761,33 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[i] *= r;
             }
-            Frag p[KB / 2];
+            Frag p[KB / 2], rest[KB / 2];
 #pragma unroll
             for (int i = 0; i < KB; ++i) {
                 float e[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], s.scale2, -shift));
                 l += (e[0] + e[1]) + (e[2] + e[3]);
-                p[i / 2].w[(i & 1) * 2] = pack_bf16x2(e[0], e[1]);
-                p[i / 2].w[(i & 1) * 2 + 1] = pack_bf16x2(e[2], e[3]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) split_bf16x2(e[2 * j], e[2 * j + 1], p[i / 2].w[(i & 1) * 2 + j], rest[i / 2].w[(i & 1) * 2 + j]);
             }
 #pragma unroll
             for (int i = 0; i < KB / 2; ++i)
 #pragma unroll
-                for (int d = 0; d < 16; ++d) {
-                    const uint32_t c = at + (d >> 2) * kPlane + i * 32 * 128 + c_at[d & 3];
-                    Frag a;
-                    a.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)c);
-                    a.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(c + 16 * 128));
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.f, p[i].f, o[d], 0, 0, 0);
+                for (int d = 0; d < 16; d += 2) {
+                    Frag a[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t c = at + (d >> 2) * kPlane + i * 32 * 128 + c_at[(d + j) & 3];
+                        a[j].h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)c);
+                        a[j].h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(size_t)(c + 16 * 128));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j].f, p[i].f, o[d + j], 0, 0, 0);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) o[d + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[j].f, rest[i].f, o[d + j], 0, 0, 0);
                 }
-            reads_ahead<12, 16 * KB / 2 - 6, 2, 6>();
+            reads_ahead<12, 8 * KB / 2 - 3, 4, 12, 4>();
         }
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
@@ -809,7 +837,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
                                                      const Token* __restrict__ tokens, const float* __restrict__ sums,
                                                      const float2* __restrict__ stats, uint16_t* __restrict__ out) {
     constexpr int G = 16 / TOK;  // groups of 16 threads that share a token
-    __shared__ __align__(16) uint16_t os[TOK][kRank + 8];
+    __shared__ __align__(16) uint16_t os[2][TOK][kRank + 8];
     __shared__ __align__(16) float part[G > 1 ? 16 : 1][kRank];
     __shared__ float tops[16], ls[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -876,14 +904,20 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
             float x = 0.0f;
 #pragma unroll
             for (int g = 0; g < G; ++g) x += part[mine + g][at] * f[g];
-            os[tok][at] = f32_to_bf16_bits(x * inv);
+            const uint16_t hi = f32_to_bf16_bits(x * inv);
+            os[0][tok][at] = hi;
+            os[1][tok][at] = f32_to_bf16_bits(x * inv - bf16_bits_to_f32(hi));
         }
     } else {
         const float inv = p.bad ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint2*>(&os[tok][c * 64 + col]) =
-                make_uint2(pack_bf16x2(v[4 * c] * inv, v[4 * c + 1] * inv), pack_bf16x2(v[4 * c + 2] * inv, v[4 * c + 3] * inv));
+        for (int c = 0; c < 4; ++c) {
+            uint2 hi, lo;
+            split_bf16x2(v[4 * c] * inv, v[4 * c + 1] * inv, hi.x, lo.x);
+            split_bf16x2(v[4 * c + 2] * inv, v[4 * c + 3] * inv, hi.y, lo.y);
+            *reinterpret_cast<uint2*>(&os[0][tok][c * 64 + col]) = hi;
+            *reinterpret_cast<uint2*>(&os[1][tok][c * 64 + col]) = lo;
+        }
     }
     __syncthreads();
     const int tc = (lane & 15) < TOK ? lane & 15 : TOK - 1;
@@ -894,8 +928,11 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
 #pragma unroll
         for (int st = 0; st < kRank / 32; ++st) {
             const bf16x8_t a = vb == wave ? first[st] : *reinterpret_cast<const bf16x8_t*>(wv + (int64_t)vb * 16 * kRank + 32 * st);
-            const bf16x8_t x = *reinterpret_cast<const bf16x8_t*>(&os[tc][32 * st + 8 * (lane >> 4)]);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, x, acc, 0, 0, 0);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const bf16x8_t x = *reinterpret_cast<const bf16x8_t*>(&os[half][tc][32 * st + 8 * (lane >> 4)]);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, x, acc, 0, 0, 0);
+            }
         }
         if (live)
             *reinterpret_cast<uint2*>(out + (to * s.H + h) * s.v_dim + vb * 16 + 4 * (lane >> 4)) =
@@ -919,7 +956,7 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
                 uint16_t* out, int num_cus, hipStream_t stream) {
     s.rows = fast_rows(b.n_rows, b.n_seq, s.H);
     s.groups = fast_groups(s.rows, num_cus);
-    const Layout l = layout(b.n_rows, b.n_seq, s.H, kWidth, s.rows, s.groups, 2, kRank);
+    const Layout l = layout(b.n_rows, b.n_seq, s.H, kQuery, s.rows, s.groups, 2, kRank);
     Plan* plan = (Plan*)(ws + l.plan);
     Item* items = (Item*)(ws + l.items);
     int32_t* seq_item = (int32_t*)(ws + l.seq_item);
@@ -1516,7 +1553,7 @@ size_t paged_attention_workspace_bytes(int64_t n_rows, int n_seq, int H, int ran
     const int64_t capacity = (int64_t)width << page_log;
     if (is_fast(rank, rope, nope, v_dim, page_log, dtype) && is_chunk(n_rows, n_seq, H, nope, v_dim, capacity))
         return chunk_layout(n_rows, n_seq, H, capacity, chunk_groups(num_cus)).bytes;
-    if (is_fast(rank, rope, nope, v_dim, page_log, dtype)) return layout(n_rows, n_seq, H, kWidth, rows, fast_groups(rows, num_cus), 2, kRank).bytes;
+    if (is_fast(rank, rope, nope, v_dim, page_log, dtype)) return layout(n_rows, n_seq, H, kQuery, rows, fast_groups(rows, num_cus), 2, kRank).bytes;
     return layout(n_rows, n_seq, H, rank + rope, kAnyRows, any_groups(num_cus), 4, rank).bytes;
 }
 
