@@ -441,6 +441,7 @@ union Frag {
     u32x4_t u;
     uint32_t w[4];
     bf16x8_t f;
+    _Float16 x __attribute__((ext_vector_type(8)));
     s16x4_t h[2];
 };
 
@@ -586,7 +587,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
 
 // WR KW waves: WR share a tile of 16 WR rows, 16 each, KW the 64 keys of a step.  S stages of LDS.
 template <int WR, int KW, int S>
-__global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
+__global__ __launch_bounds__(WR * KW * 64, WR * KW > 2 ? 2 : 1) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
                                                                  const Item* __restrict__ items, const uint16_t* __restrict__ queries,
                                                                  const uint16_t* __restrict__ specials, float* __restrict__ sums,
                                                                  float2* __restrict__ stats) {
@@ -994,6 +995,13 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
 // each sequence's rows filled up with zeros to a multiple of 64; the keys' rotated parts, which the heads share, likewise.
 // The attention is then that of any causal head: 128 tokens of a head a workgroup, 32 a wave, keys in steps of 64,
 // and heads as the outer dimension of the even shares, so that an XCD's workgroups read the same two heads' keys from its L2.
+//
+// Queries, keys, values and exponentials are fp16 there, of 11 bits instead of bf16's 8: the outputs' error against 64 bits
+// is that of their own rounding (with bf16 up to twice that; 120.2 -> 121.7 us for 2,048 tokens, 7,001 keys, 16 heads).  For
+// their range queries and keys are 2^-4 of themselves, values 2^-2, and a row's exponentials 2^6 at its maximum: a query or
+// key of 2^20 or a value of 2^18 and more counts as infinite; fp16's steps near zero are 2^-20 of a key, 2^-22 of a value
+// and 2^-30 of a weight, below bf16's where a key is 2^-11 or more and a value 2^-13.
+constexpr float kKeyScale = 0x1p-4f, kValueScale = 0x1p-2f, kQueryScale = 0x1p-4f, kTop = 6.0f;
 constexpr int kHead = 64;         // columns of a head's keys (before the rotated ones) and of its values
 constexpr int kChunkTok = 128;    // tokens of a tile
 constexpr int kChunkRows = 128;   // new tokens a sequence, on the average, from which this is the shorter way
@@ -1054,6 +1062,15 @@ __global__ __launch_bounds__(256) void chunk_prepare_kernel(const float* __restr
     float2 c;
     rotary_angle((int64_t)b.lens[i] - b.starts[i + 1] + t, rates[p], c.x, c.y);
     turns[t * 32 + p] = c;
+}
+
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef const __attribute__((address_space(3))) f16x8_t* lds_half_ptr;
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) { return __builtin_bit_cast(uint32_t, f16x2_t{(_Float16)a, (_Float16)b}); }
+// Two bf16 values, times a scale, as fp16.
+__device__ __forceinline__ uint32_t f16_of_bf16x2(uint32_t v, float scale) {
+    return pack_f16x2(__uint_as_float(v << 16) * scale, __uint_as_float(v & 0xffff0000u) * scale);
 }
 
 constexpr int kRowStage = kRank / 64 * kPlane;  // the latents of 64 rows
@@ -1150,13 +1167,14 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restri
             }
         reads_ahead<8, 2 * kRank / 16 - 8, 1, 8>();
         // row r's piece c of 16 bytes lies at c ^ r % 16
+        const float scale = wave < 2 ? kKeyScale : kValueScale;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int r = 32 * i + (lane & 31), c = 4 * wave + (e >> 2);
                 *(lds_u2_ptr)(size_t)(result + r * (4 * kHead) + ((c ^ (r & 15)) << 4) + 8 * half) =
-                    u32x2_t{pack_bf16x2(acc[i][e], acc[i][e + 1]), pack_bf16x2(acc[i][e + 2], acc[i][e + 3])};
+                    u32x2_t{pack_f16x2(acc[i][e] * scale, acc[i][e + 1] * scale), pack_f16x2(acc[i][e + 2] * scale, acc[i][e + 3] * scale)};
             }
         lds_barrier();
         uint16_t* to = keys + ((int64_t)h * key_rows + (int64_t)tile * kKeys) * (2 * kHead);
@@ -1176,6 +1194,8 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restri
                                  : *reinterpret_cast<const u32x4_t*>(pool + (((int64_t)page << b.page_log) + (p & ((1 << b.page_log) - 1))) * kWidth +
                                                                      kRank + c * 8);
                 }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = f16_of_bf16x2(v[j], kKeyScale);
                 *reinterpret_cast<u32x4_t*>(shared + ((int64_t)tile * kKeys + r) * kRope + c * 8) = v;
             }
         }
@@ -1185,7 +1205,7 @@ __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restri
 // A step's LDS: two planes of 64 rows for the keys and their rotated parts, one for the values.  A step takes the next
 // one's keys and its own values, so each have a ring of three steps of their own: both are copied two steps ahead.
 constexpr int kKeyStage = 2 * kPlane, kValueStage = kPlane, kValues = 3 * kKeyStage;  // (the values' ring behind the keys')
-// How far a row's maximum may grow before its sums are rescaled: exponentials stay below 2^8, of the same precision.
+// How far a row's maximum may grow before its sums are rescaled: exponentials stay below 2^14.
 constexpr float kSlack = 8.0f;
 
 constexpr int kAhead = 2;  // steps of a product that the keys' fragments are read ahead
@@ -1290,9 +1310,13 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
                     const uint32_t u = fq[4 + i].w[j], v = fq[6 + i].w[j];
                     const float u0 = __uint_as_float(u << 16), u1 = __uint_as_float(u & 0xffff0000u);
                     const float v0 = __uint_as_float(v << 16), v1 = __uint_as_float(v & 0xffff0000u);
-                    fq[4 + i].w[j] = pack_bf16x2(u0 * c.x - v0 * c.y, u1 * c.z - v1 * c.w);
-                    fq[6 + i].w[j] = pack_bf16x2(v0 * c.x + u0 * c.y, v1 * c.z + u1 * c.w);
+                    fq[4 + i].w[j] = pack_f16x2((u0 * c.x - v0 * c.y) * kQueryScale, (u1 * c.z - v1 * c.w) * kQueryScale);
+                    fq[6 + i].w[j] = pack_f16x2((v0 * c.x + u0 * c.y) * kQueryScale, (v1 * c.z + u1 * c.w) * kQueryScale);
                 }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) fq[i].w[j] = f16_of_bf16x2(fq[i].w[j], kQueryScale);
 #pragma unroll
             for (int i = 0; i < 8; ++i) asm volatile("" : "+v"(fq[i].u));
         }
@@ -1307,7 +1331,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
             }
         };
         auto read_keys = [&](const uint32_t (&base)[4], int st, int i) {
-            return *(lds_frag_ptr)(size_t)(base[st & 3] + (st >> 2) * kPlane + i * 32 * 128);
+            return *(lds_half_ptr)(size_t)(base[st & 3] + (st >> 2) * kPlane + i * 32 * 128);
         };
         // What the wave's tokens do not see of step j.
         auto mask = [&](f32x16_t (&z)[2], int j) {
@@ -1325,7 +1349,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
             for (int c = 0; c < 8; ++c) {
                 const u32x4_t v = *(lds_u4_ptr)(size_t)(at + lane * 128 + (((c + (lane >> 1)) & 7) << 4));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+                for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7c00u) == 0x7c00u || (v[i] & 0x7c000000u) == 0x7c000000u;
             }
             const uint64_t odd = ballot(bad);
             if (odd == 0) return;
@@ -1336,7 +1360,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
             lds_barrier();
         };
         auto new_top = [&](float top) {
-            top = halves_max(top) * s.scale2;
+            top = halves_max(top) * s.scale2 - kTop;
             if (ballot(top > shift + kSlack) != 0) {  // some token's maximum has grown
                 const float was = shift;
                 shift = fmaxf(shift, top);
@@ -1368,7 +1392,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
                 }
             if ((k_begin + j) * kKeys + kKeys - 1 > first_pos) clean(j, lds + kValues + stage * kValueStage);
             Frag p[4], fv[4][2];
-            bf16x8_t fk[8][2];
+            f16x8_t fk[8][2];
             if constexpr (more) {
                 key_bases(lds + next * kKeyStage, kb);
 #pragma unroll
@@ -1384,7 +1408,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if (st + kAhead < 8) fk[st + kAhead][i] = read_keys(kb, st + kAhead, i);
-                        y[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk[st][i], fq[st].f, y[i], 0, 0, 0);
+                        y[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fk[st][i], fq[st].x, y[i], 0, 0, 0);
                     }
                 }
                 if (st >= 4) {
@@ -1400,10 +1424,10 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
                 for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[st >> 2][4 * (st & 3) + i], s.scale2, -shift));
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const uint32_t w = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+                    const uint32_t w = pack_f16x2(e[2 * i], e[2 * i + 1]);
                     p[st >> 1].w[2 * (st & 1) + i] = w;
                     // the sum of what the values are weighted with, rounded as they are
-                    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, w), __builtin_bit_cast(bf16x2_v, 0x3f803f80u), l, false);
+                    l = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, w), f16x2_t{1, 1}, l, false);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -1415,7 +1439,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
             for (int i = 0; i < 4; ++i) {
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv[i][d].f, p[i].f, o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fv[i][d].x, p[i].x, o[d], 0, 0, 0);
                     if constexpr (more) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) top = fmaxf(top, y[i >> 1][8 * (i & 1) + 4 * d + e]);
@@ -1436,7 +1460,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
 #pragma unroll
             for (int st = 0; st < 8; ++st)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) x[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(read_keys(kb, st, i), fq[st].f, x[i], 0, 0, 0);
+                for (int i = 0; i < 2; ++i) x[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read_keys(kb, st, i), fq[st].x, x[i], 0, 0, 0);
             if (k_begin * kKeys + kKeys - 1 > first_pos) mask(x, 0);
             float top = x[0][0];
 #pragma unroll
@@ -1464,7 +1488,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
         lds_barrier();
         if (my < it.rows) {
             if (t == begin && to == finish) {  // the tile's whole work
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const float inv = l == 0.0f ? 0.0f : 1.0f / (l * kValueScale);
                 uint16_t* z = out + (row * s.H + h) * kHead + 4 * half;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -1511,7 +1535,7 @@ __global__ __launch_bounds__(256) void chunk_finish_kernel(int64_t n_rows, Shape
         l = l * f + ml.y * f2;
         v = v * f + x * f2;
     }
-    const float inv = p.bad ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = p.bad ? NAN : l == 0.0f ? 0.0f : 1.0f / (l * kValueScale);
     *reinterpret_cast<uint2*>(out + r * kHead + col) = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
 }
 
@@ -1526,6 +1550,7 @@ int launch_chunk(const uint16_t* q, const uint16_t* w, const uint16_t* pool, con
     s.rows = kChunkTok;
     s.groups = chunk_groups(num_cus);
     s.planes = s.H;
+    s.scale2 /= kKeyScale * kQueryScale;
     const ChunkLayout l = chunk_layout(b.n_rows, b.n_seq, s.H, (int64_t)b.width << b.page_log, s.groups);
     Plan* plan = (Plan*)(ws + l.plan);
     Item* items = (Item*)(ws + l.items);

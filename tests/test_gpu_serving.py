@@ -321,6 +321,32 @@ def test_many_new_tokens_against_float64(lens, new, H, page):
     assert torch.equal(_attend(c), got)
 
 
+@pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("of_rows,of_weight,of_query", [(64.0, 16.0, 1.0), (2.0 ** -6, 2.0 ** -3, 1.0), (1.0, 1.0, 2.0 ** 10), (1.0, 1.0, 2.0 ** -8),
+                                                        (2.0 ** -4, 2.0 ** 10, 2.0 ** -4)])
+def test_attention_of_other_magnitudes(new, of_rows, of_weight, of_query):
+    """Rows, weights and queries times powers of two, with scores as before: the same relative bounds."""
+    c = _case([400, 170], [new, new], 4, 256, 64, 64, 64, 16, "bf16", seed=new)
+    c["w"] = c["w"] * of_weight
+    rank = c["w"].shape[1]
+    c["pool"][..., :rank] *= of_rows
+    c["pool"][..., rank:] *= of_rows * of_weight
+    c["q"] = c["q"] * of_query
+    c["scale"] /= of_rows * of_weight * of_query
+    _near(_attend(c), c, f"{new} new")
+
+
+def test_keys_and_values_out_of_range_count_as_infinite():
+    """Many new tokens: a finite row whose values do not fit has no result where it is seen, and does not show elsewhere."""
+    c = _case([300, 200], [200, 150], 4, 256, 64, 64, 64, 16, "bf16", seed=3)
+    good = _attend(c)
+    at = _slots(c["table"], 0, torch.tensor([250], device="cuda"), 16)
+    c["pool"].view(-1, 320)[at] = 1e36
+    got = _attend(c)
+    assert torch.equal(got[:150], good[:150]) and torch.equal(got[200:], good[200:])
+    assert bool(got[150:200].isnan().all())
+
+
 @pytest.mark.parametrize("dt,rank", [("bf16", 256), ("bf16", 64), ("fp32", 64)])
 def test_attention_of_batches_that_do_not_fit(dt, rank):
     c = _case([70, 33, 100, 20], [3, 2, 4, 2], 4, rank, 64, 64, 64, 16, dt, seed=4)
