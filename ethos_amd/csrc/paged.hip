@@ -196,125 +196,235 @@ __device__ __forceinline__ int find_item(const Item* items, int n_items, int64_t
 }
 
 // ------------------------------------------------------------------------- any widths, both types
-constexpr int kAnyRows = 8, kAnyKeys = 16, kAnyRank = 512, kAnyRope = 128, kAnyWidth = kAnyRank + kAnyRope;
+// In float32 throughout, on 16 x 16 x 4 matrix products: tiles of 16 rows, a wave 16 keys of a step's 64.  A product's
+// columns and keys may come in any order, so each lane takes four neighbouring columns at a time: of one of 16 keys for
+// the scores, of 64 columns of one of four keys for the sums.  S^T = K Q^T leaves keys 4 g + e of a row in lane (row, g),
+// which is where O^T = C^T P^T takes them with key 4 g + e in place g of its product e: nothing goes through LDS but the
+// queries, and the waves run by themselves up to the end of a share, where their sums are joined.
+constexpr int kAnyRows = 16, kAnyKeys = 16, kAnyRank = 512, kAnyRope = 128, kAnyWidth = kAnyRank + kAnyRope;
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-// Block 0 the plan; each other block a token's rows.
+__device__ __forceinline__ f32x4_t load4(const float* p) { return *reinterpret_cast<const f32x4_t*>(p); }
+__device__ __forceinline__ f32x4_t load4(const uint16_t* p) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    return f32x4_t{__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u)};
+}
+
+// Block 0 the plan and a row of zeros; each other block 16 tokens of a head, [c][token] = W_k,h^T q^T, a wave every
+// fourth 64 columns.
 template <typename T>
-__global__ __launch_bounds__(1024) void any_prepare_kernel(const T* __restrict__ q, const T* __restrict__ w, const float* __restrict__ rates,
-                                                           Batch b, Shape s, int64_t max_items, Plan* plan, Item* items, int32_t* seq_item,
-                                                           Token* tokens, float* __restrict__ queries) {
+__global__ __launch_bounds__(256) void any_prepare_kernel(const T* __restrict__ q, const T* __restrict__ w, const float* __restrict__ rates,
+                                                          Batch b, Shape s, int64_t max_items, Plan* plan, Item* items, int32_t* seq_item,
+                                                          Token* tokens, T* __restrict__ zeros, float* __restrict__ queries) {
+    __shared__ float qs[16][64 + 4];
+    __shared__ int64_t pos[16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, width = s.rank + s.rope;
     if (blockIdx.x == 0) {
-        make_plan<1024>(b, s, max_items, plan, items, seq_item, nullptr, threadIdx.x);
+        for (int e = tid; e < width; e += 256) zeros[e] = 0;
+        make_plan<256>(b, s, max_items, plan, items, seq_item, nullptr, tid);
         return;
     }
-    const int64_t t = blockIdx.x - 1;
-    const int i = batch_seq(b, t), width = s.rank + s.rope, qw = s.nope + s.rope;
-    if (threadIdx.x == 0) tokens[t] = token_of(b, t, i);
-    if (i < 0) return;
-    const int64_t pos = (int64_t)b.lens[i] - b.starts[i + 1] + t;
-    const T* qt = q + t * s.H * qw;
-    float* out = queries + t * s.H * width;
-    for (int e = threadIdx.x; e < s.H * width; e += 1024) {
-        const int h = e / width, c = e - h * width;
-        const T* qh = qt + h * qw;
-        float v = 0.0f;
-        if (c < s.rank) {
-            const T* wh = w + (int64_t)h * (s.nope + s.v_dim) * s.rank + c;
-            for (int j = 0; j < s.nope; ++j) v = __builtin_fmaf(Elem<T>::to_f32(qh[j]), Elem<T>::to_f32(wh[(int64_t)j * s.rank]), v);
-        } else {
-            const int half = s.rope / 2, p = (c - s.rank) % half;
-            float cs, sn;
-            rotary_angle(pos, rates[p], cs, sn);
-            const float u = Elem<T>::to_f32(qh[s.nope + p]), x = Elem<T>::to_f32(qh[s.nope + half + p]);
-            v = c - s.rank < half ? u * cs - x * sn : x * cs + u * sn;
+    const int h = (blockIdx.x - 1) % s.H, qw = s.nope + s.rope;
+    const int64_t t0 = (int64_t)((blockIdx.x - 1) / s.H) * 16;
+    if (tid < 16 && t0 + tid < b.n_rows) {
+        const int64_t t = t0 + tid;
+        const int i = batch_seq(b, t);
+        if (h == 0) tokens[t] = token_of(b, t, i);
+        pos[tid] = i >= 0 ? (int64_t)b.lens[i] - b.starts[i + 1] + t : 0;
+    }
+    constexpr int NB = kAnyRank / 64 / 4;
+    f32x4_t acc[NB][4] = {};
+    const T* wh = w + (int64_t)h * (s.nope + s.v_dim) * s.rank;
+    for (int j0 = 0; j0 < s.nope; j0 += 64) {
+        __syncthreads();
+        for (int e = tid; e < 16 * 64; e += 256) {
+            const int64_t t = t0 + (e >> 6);
+            const int j = j0 + (e & 63);
+            qs[e >> 6][e & 63] = t < b.n_rows && j < s.nope ? Elem<T>::to_f32(q[(t * s.H + h) * qw + j]) : 0.0f;
         }
-        out[e] = v;
+        __syncthreads();
+        const int n = s.nope - j0 < 64 ? s.nope - j0 : 64;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int c = 64 * (wave + 4 * i), at = c + 4 * (lane & 15);
+            if (c >= s.rank) break;
+            for (int j = 0; j < n; j += 16) {
+                f32x4_t a[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int r = j + 4 * k + g;
+                    a[k] = load4(wh + (int64_t)(j0 + (r < n ? r : 0)) * s.rank + (at < s.rank ? at : 0));
+                    if (r >= n) a[k] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        acc[i][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[k][d], qs[lane & 15][j + 4 * k + g], acc[i][d], 0, 0, 0);
+            }
+        }
+    }
+    if (s.nope == 0) __syncthreads();
+    const int64_t my_t = t0 + (lane & 15);
+    if (my_t < b.n_rows)
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int c = 64 * (wave + 4 * i) + 16 * g + 4 * e;
+                if (c < s.rank)
+                    *reinterpret_cast<f32x4_t*>(queries + (my_t * s.H + h) * width + c) = f32x4_t{acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
+            }
+    const int half = s.rope / 2;
+    for (int e = tid; e < 16 * half; e += 256) {
+        const int64_t t = t0 + e / half;
+        const int p = e % half;
+        if (t >= b.n_rows) break;
+        float c, sn;
+        rotary_angle(pos[e / half], rates[p], c, sn);
+        const T* r = q + (t * s.H + h) * qw + s.nope;
+        const float u = Elem<T>::to_f32(r[p]), v = Elem<T>::to_f32(r[half + p]);
+        float* to = queries + (t * s.H + h) * width + s.rank;
+        to[p] = u * c - v * sn;
+        to[half + p] = v * c + u * sn;
     }
 }
 
-// Tiles of 8 rows, 16 keys at a time in LDS; 32 threads score a row's 16 keys, two a key; then a thread sums two
-// columns of the latent for all rows.  Keys that a row does not see are left out of its sums, whatever they hold.
-template <typename T>
-__global__ __launch_bounds__(256) void any_attend_kernel(const T* __restrict__ pool, Batch b, Shape s, const Plan* plan,
-                                                         const Item* __restrict__ items, const float* __restrict__ queries,
-                                                         float* __restrict__ sums, float2* __restrict__ stats) {
-    __shared__ __align__(16) float qs[kAnyRows][kAnyWidth];
-    __shared__ __align__(16) float ks[kAnyKeys][kAnyWidth + 4];
-    __shared__ float ps[kAnyRows][kAnyKeys], turn[kAnyRows];
-    const int tid = threadIdx.x, width = s.rank + s.rope;
-    const int row = tid >> 5, key = (tid >> 1) & 15, part = tid & 1;
+// RB: the rank in blocks of 64 columns, rounded up.
+template <typename T, int RB>
+__global__ __launch_bounds__(256, RB > 4 ? 1 : 2) void any_attend_kernel(const T* __restrict__ pool, Batch b, Shape s, const Plan* plan,
+                                                                         const Item* __restrict__ items, const T* __restrict__ zeros,
+                                                                         const float* __restrict__ queries, float* __restrict__ sums,
+                                                                         float2* __restrict__ stats) {
+    __shared__ __align__(16) float qs[kAnyRows * (kAnyWidth + 4)];
+    __shared__ __align__(16) float part[4][kAnyRows][64 + 4];
+    __shared__ float tops[4][kAnyRows], ls[4][kAnyRows];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+    const int width = s.rank + s.rope, blocks = (width + 63) / 64 * 4, pitch = blocks * 16 + 4;
     const int64_t quota = plan->quota, last = plan->tiles;
     int64_t t = blockIdx.x * quota;
     const int64_t stop = t + quota < last ? t + quota : last;
     if (t >= stop) return;
-    int item = find_item(items, plan->n_items, t, tid & 63);
+    int item = find_item(items, plan->n_items, t, lane);
     for (; t < stop; ++item) {
         const Item it = items[item];
         const int64_t begin = item > 0 ? items[item - 1].end : 0;
         const int64_t to = it.end < stop ? it.end : stop;
         if (to <= t) continue;
-        for (int e = tid; e < kAnyRows * width; e += 256) {
-            const int r = e / width, c = e - r * width;
-            qs[r][c] = r < it.rows ? queries[((int64_t)it.tok0 * s.H + it.row0 + r) * width + c] : 0.0f;
+        for (int e = tid; e < kAnyRows * blocks * 16; e += 256) {
+            const int r = e / (blocks * 16), c = e - r * (blocks * 16);
+            qs[r * pitch + c] = r < it.rows && c < width ? queries[((int64_t)it.tok0 * s.H + it.row0 + r) * width + c] : 0.0f;
         }
-        const int64_t my_pos = (int64_t)it.pos0 + (it.row0 + (row < it.rows ? row : it.rows - 1)) / s.H;
-        const int64_t end = (int64_t)it.pos0 + (it.row0 + it.rows - 1) / s.H + 1;  // keys that some row sees
-        float acc[kAnyRows][2] = {}, m = kLowest, l = 0.0f;
-        for (int64_t k0 = (t - begin) * kKeys; k0 < (to - begin) * kKeys; k0 += kAnyKeys) {
-            if (k0 >= end) break;
-            __syncthreads();
-            for (int e = tid; e < kAnyKeys * width; e += 256) {
-                const int r = e / width, c = e - r * width;
-                float v = 0.0f;
-                if (k0 + r < end) {
-                    const int32_t page = batch_page(b, it.seq, k0 + r);
-                    const int64_t in = (k0 + r) & (((int64_t)1 << b.page_log) - 1);
-                    v = page < 0 ? NAN : Elem<T>::to_f32(pool[(((int64_t)page << b.page_log) + in) * width + c]);
-                }
-                ks[r][c] = v;
-            }
-            __syncthreads();
-            float x = 0.0f;
-            for (int c = part * 4; c < width; c += 8) {
-                const float4 u = *reinterpret_cast<const float4*>(&qs[row][c]), v = *reinterpret_cast<const float4*>(&ks[key][c]);
-                x = __builtin_fmaf(u.x, v.x, x);
-                x = __builtin_fmaf(u.y, v.y, x);
-                x = __builtin_fmaf(u.z, v.z, x);
-                x = __builtin_fmaf(u.w, v.w, x);
-            }
-            x += __shfl_xor(x, 1, 64);
-            x = k0 + key > my_pos ? -INFINITY : x * s.scale2;
-            float top = x;
-            for (int d = 2; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-            const float next = fmaxf(m, top), r = exp2f(m - next), p = exp2f(x - next);
-            float sum = p;
-            for (int d = 2; d < 32; d <<= 1) sum += __shfl_xor(sum, d, 64);
-            l = l * r + sum;
-            m = next;
-            if (part == 0) ps[row][key] = p;
-            if (key == 0 && part == 0) turn[row] = r;
-            __syncthreads();
-#pragma unroll
-            for (int r8 = 0; r8 < kAnyRows; ++r8) {
-                const int64_t seen = (int64_t)it.pos0 + (it.row0 + (r8 < it.rows ? r8 : it.rows - 1)) / s.H - k0;
-                const float f = turn[r8];
-#pragma unroll
-                for (int d = 0; d < 2; ++d) acc[r8][d] *= f;
-                for (int k = 0; k < kAnyKeys && k <= seen; ++k) {
-                    const float pk = ps[r8][k];
-#pragma unroll
-                    for (int d = 0; d < 2; ++d)
-                        if (tid + 256 * d < s.rank) acc[r8][d] = __builtin_fmaf(pk, ks[k][tid + 256 * d], acc[r8][d]);
-                }
-            }
-        }
-        const int64_t slot = (int64_t)blockIdx.x + item;
-        for (int r = 0; r < it.rows; ++r)
-            for (int d = 0; d < 2; ++d)
-                if (tid + 256 * d < s.rank) sums[(slot * kAnyRows + r) * s.rank + tid + 256 * d] = acc[r][d];
-        if (key == 0 && part == 0 && row < it.rows) stats[slot * kAnyRows + row] = make_float2(m, l);
-        t = to;
+        const int first_pos = it.pos0 + it.row0 / s.H, my_pos = it.pos0 + (it.row0 + (m < it.rows ? m : it.rows - 1)) / s.H;
+        const int end = it.pos0 + (it.row0 + it.rows - 1) / s.H + 1;  // keys that some row sees
+        const float* my_q = qs + m * pitch + 4 * g;
         __syncthreads();
+        f32x4_t o[RB][4] = {};
+        float shift = kLowest, l = 0.0f;
+        int32_t page = 0;  // of the lane's key, looked up a step before
+        auto look_up = [&](int64_t k) {
+            const int64_t key = k * kKeys + wave * kAnyKeys + m;
+            page = key < end ? batch_page(b, it.seq, key) : -1;
+        };
+        look_up(t - begin);
+        for (int64_t k = t - begin; k < to - begin; ++k) {
+            const int key0 = (int)(k * kKeys) + wave * kAnyKeys;  // the wave's first key
+            const bool lost = page < 0 && key0 + m < end;          // a key without a page
+            const T* row = page < 0 ? zeros : pool + (((int64_t)page << b.page_log) + ((key0 + m) & ((1 << b.page_log) - 1))) * width;
+            look_up(k + 1);
+            if (key0 >= end) continue;
+            f32x4_t x = {0.0f, 0.0f, 0.0f, 0.0f}, y = x;
+            for (int j = 0; j < blocks; j += 4) {  // 64 columns at a time
+                f32x4_t a[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int c = 16 * (j + i) + 4 * g;
+                    a[i] = load4(c < width ? row + c : zeros);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4_t u = *reinterpret_cast<const f32x4_t*>(my_q + 16 * (j + i));
+                    x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][0], u[0], x, 0, 0, 0);
+                    y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][1], u[1], y, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][2], u[2], x, 0, 0, 0);
+                    y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i][3], u[3], y, 0, 0, 0);
+                }
+            }
+            x += y;
+            // keys without a page, and rows that only some of the tile see and whose latents are not finite: no result for a
+            // row that sees one of them, zeros for the others
+            bool bad = lost;
+            if (key0 + kAnyKeys - 1 > first_pos)
+                for (int c = 4 * g; c < s.rank; c += 16) {
+                    const f32x4_t v = load4(row + c);
+                    bad |= !(isfinite(v[0]) && isfinite(v[1]) && isfinite(v[2]) && isfinite(v[3]));
+                }
+            uint64_t odd = ballot(bad);
+            odd = (odd | odd >> 16 | odd >> 32 | odd >> 48) & 0xffff;
+            float top = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int key = 4 * g + e;
+                if ((odd >> key & 1) && key0 + key <= my_pos) l = NAN;
+                x[e] = key0 + key > my_pos ? -INFINITY : x[e];
+                top = fmaxf(top, x[e]);
+            }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64)) * s.scale2;
+            if (ballot(top > shift) != 0) {  // some row has a new maximum
+                const float before = shift;
+                shift = fmaxf(shift, top);
+                const float r = exp2f(before - shift);
+                l *= r;
+#pragma unroll
+                for (int i = 0; i < RB; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[i][c] *= r;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = exp2f(__builtin_fmaf(x[e], s.scale2, -shift));
+                l += p;
+                const uint64_t at = (uint64_t)(uintptr_t)row;
+                const uint32_t lo = __shfl((int)(uint32_t)at, 4 * g + e, 64), hi = __shfl((int)(uint32_t)(at >> 32), 4 * g + e, 64);
+                const T* from = odd >> (4 * g + e) & 1 ? zeros : (const T*)(uintptr_t)((uint64_t)hi << 32 | lo);
+#pragma unroll
+                for (int i = 0; i < RB; ++i) {
+                    const int c = 64 * i + 4 * m;
+                    const f32x4_t a = load4(from + (c < s.rank ? c : 0));  // (what lies beyond is not stored)
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) o[i][d] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[d], p, o[i][d], 0, 0, 0);
+                }
+            }
+        }
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (g == 0) tops[wave][m] = shift, ls[wave][m] = l;
+        __syncthreads();
+        float all = tops[0][m], sum = 0.0f;
+#pragma unroll
+        for (int i = 1; i < 4; ++i) all = fmaxf(all, tops[i][m]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += ls[i][m] * exp2f(tops[i][m] - all);
+        const float f = exp2f(shift - all);
+        const int64_t slot = ((int64_t)blockIdx.x + item) * kAnyRows;
+        if (wave == 0 && g == 0 && m < it.rows) stats[slot + m] = make_float2(all, sum);
+        const int r = tid >> 4, c = (tid & 15) * 4;
+#pragma unroll
+        for (int i = 0; i < RB; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<f32x4_t*>(&part[wave][m][16 * g + 4 * e]) = f32x4_t{o[i][0][e], o[i][1][e], o[i][2][e], o[i][3][e]} * f;
+            __syncthreads();
+            if (r < it.rows && 64 * i + c < s.rank) {
+                f32x4_t v = *reinterpret_cast<const f32x4_t*>(&part[0][r][c]);
+#pragma unroll
+                for (int k = 1; k < 4; ++k) v += *reinterpret_cast<const f32x4_t*>(&part[k][r][c]);
+                *reinterpret_cast<f32x4_t*>(sums + (slot + r) * s.rank + 64 * i + c) = v;
+            }
+            __syncthreads();
+        }
+        t = to;
     }
 }
 
@@ -345,43 +455,77 @@ __device__ __forceinline__ Parts row_parts(const Shape& s, const Plan* plan, con
     return p;
 }
 
-// One workgroup a token: joins each row's parts, in order, and multiplies with W_v,h.
+// A workgroup a (token, head): joins its row's parts, four columns a thread and as many parts side by side as there are
+// threads for, and multiplies with W_v,h, 16 threads a column.
 template <typename T>
 __global__ __launch_bounds__(256) void any_finish_kernel(const T* __restrict__ w, Shape s, const Plan* plan,
                                                          const Item* __restrict__ items, const int32_t* __restrict__ seq_item,
                                                          const Token* __restrict__ tokens, const float* __restrict__ sums,
                                                          const float2* __restrict__ stats, T* __restrict__ out) {
-    __shared__ float o[kAnyRank];
-    const int64_t t = blockIdx.x;
+    __shared__ __align__(16) float part[1024], o[kAnyRank];
+    __shared__ float tops[256], ls[256];
+    const int64_t t = blockIdx.x / s.H;
+    const int h = (int)(blockIdx.x - t * s.H), tid = threadIdx.x;
     const Token token = tokens[t];
-    const int tid = threadIdx.x;
     if (token.seq == kNoSeq) return;  // behind the last sequence
-    for (int h = 0; h < s.H; ++h) {
-        int in = 0;
-        const Parts p = row_parts(s, plan, items, seq_item, token.seq, (int64_t)token.index * s.H + h, 0, in);
+    const int cols = s.rank / 4, groups = 256 / cols, grp = tid / cols, col = (tid - grp * cols) * 4;
+    int in = 0;
+    const Parts p = row_parts(s, plan, items, seq_item, token.seq, (int64_t)token.index * s.H + h, 0, in);
+    if (grp < groups) {
         float top = kLowest, l = 0.0f;
-        for (int k = 0; k < p.n; ++k) top = fmaxf(top, stats[(p.slot + k) * s.rows + in].x);
-        for (int k = 0; k < p.n; ++k) {
-            const float2 ml = stats[(p.slot + k) * s.rows + in];
-            l += ml.y * exp2f(ml.x - top);
+        f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = grp; k < p.n; k += 4 * groups) {  // four parts' loads on their way at a time
+            float2 ml[4];
+            f32x4_t x[4];
+            float next = top;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t at = (p.slot + (k + j * groups < p.n ? k + j * groups : k)) * s.rows + in;
+                ml[j] = stats[at];
+                x[j] = load4(sums + at * s.rank + col);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) next = fmaxf(next, ml[j].x);
+            const float r = exp2f(top - next);
+            top = next;
+            l *= r;
+            v *= r;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (k + j * groups >= p.n) break;
+                const float f = exp2f(ml[j].x - top);
+                l = __builtin_fmaf(ml[j].y, f, l);
+                v += x[j] * f;
+            }
+        }
+        *reinterpret_cast<f32x4_t*>(part + grp * s.rank + col) = v;
+        if (col == 0) tops[grp] = top, ls[grp] = l;
+    }
+    __syncthreads();
+    if (tid < cols) {
+        float all = tops[0], l = 0.0f;
+        for (int k = 1; k < groups; ++k) all = fmaxf(all, tops[k]);
+        f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < groups; ++k) {
+            const float f = exp2f(tops[k] - all);
+            l += ls[k] * f;
+            v += *reinterpret_cast<const f32x4_t*>(part + k * s.rank + tid * 4) * f;
         }
         const float inv = p.bad ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
-        __syncthreads();
-        for (int c = tid; c < s.rank; c += 256) {
-            float v = 0.0f;
-            for (int k = 0; k < p.n; ++k)
-                v += sums[((p.slot + k) * s.rows + in) * s.rank + c] * exp2f(stats[(p.slot + k) * s.rows + in].x - top);
-            o[c] = v * inv;
+        *reinterpret_cast<f32x4_t*>(o + tid * 4) = v * inv;
+    }
+    __syncthreads();
+    for (int j = tid >> 4; j < s.v_dim; j += 16) {
+        const T* wr = w + ((int64_t)h * (s.nope + s.v_dim) + s.nope + j) * s.rank;
+        float v = 0.0f;
+        for (int c = (tid & 15) * 4; c < s.rank; c += 64) {
+            const f32x4_t a = load4(wr + c), x = *reinterpret_cast<const f32x4_t*>(o + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v = __builtin_fmaf(a[i], x[i], v);
         }
-        __syncthreads();
-        for (int j = tid >> 2; j < s.v_dim; j += 64) {
-            const T* wr = w + ((int64_t)h * (s.nope + s.v_dim) + s.nope + j) * s.rank;
-            float v = 0.0f;
-            for (int c = tid & 3; c < s.rank; c += 4) v = __builtin_fmaf(o[c], Elem<T>::to_f32(wr[c]), v);
-            v += __shfl_xor(v, 1, 64);
-            v += __shfl_xor(v, 2, 64);
-            if ((tid & 3) == 0) out[(t * s.H + h) * s.v_dim + j] = Elem<T>::from_f32(v);
-        }
+#pragma unroll
+        for (int k = 1; k < 16; k <<= 1) v += __shfl_xor(v, k, 64);
+        if ((tid & 15) == 0) out[(t * s.H + h) * s.v_dim + j] = Elem<T>::from_f32(v);
     }
 }
 
@@ -397,12 +541,19 @@ int launch_any(const T* q, const T* w, const T* pool, const Batch& b, const floa
     Item* items = (Item*)(ws + l.items);
     int32_t* seq_item = (int32_t*)(ws + l.seq_item);
     Token* tokens = (Token*)(ws + l.tokens);
+    T* zeros = (T*)(ws + l.specials);
     float *queries = (float*)(ws + l.queries), *sums = (float*)(ws + l.sums);
     float2* stats = (float2*)(ws + l.stats);
-    hipLaunchKernelGGL((any_prepare_kernel<T>), dim3((unsigned)(b.n_rows + 1)), dim3(1024), 0, stream, q, w, rates, b, s, l.max_items, plan,
-                       items, seq_item, tokens, queries);
-    hipLaunchKernelGGL((any_attend_kernel<T>), dim3((unsigned)s.groups), dim3(256), 0, stream, pool, b, s, plan, items, queries, sums, stats);
-    hipLaunchKernelGGL((any_finish_kernel<T>), dim3((unsigned)b.n_rows), dim3(256), 0, stream, w, s, plan, items, seq_item, tokens, sums,
+    hipLaunchKernelGGL((any_prepare_kernel<T>), dim3((unsigned)((b.n_rows + 15) / 16 * s.H + 1)), dim3(256), 0, stream, q, w, rates, b, s,
+                       l.max_items, plan, items, seq_item, tokens, zeros, queries);
+    auto attend = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)s.groups), dim3(256), 0, stream, pool, b, s, plan, items, zeros, queries, sums, stats);
+    };
+    if (s.rank <= 64) attend(any_attend_kernel<T, 1>);
+    else if (s.rank <= 128) attend(any_attend_kernel<T, 2>);
+    else if (s.rank <= 256) attend(any_attend_kernel<T, 4>);
+    else attend(any_attend_kernel<T, 8>);
+    hipLaunchKernelGGL((any_finish_kernel<T>), dim3((unsigned)(b.n_rows * s.H)), dim3(256), 0, stream, w, s, plan, items, seq_item, tokens, sums,
                        stats, out);
     return (int)hipGetLastError();
 }
@@ -435,7 +586,6 @@ typedef __attribute__((address_space(3))) s16x4_t* lds_tr_ptr;
 typedef __attribute__((address_space(3))) u32x4_t* lds_u4_ptr;
 typedef __attribute__((address_space(3))) u32x2_t* lds_u2_ptr;
 typedef __attribute__((address_space(3))) float* lds_f_ptr;
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 union Frag {
     u32x4_t u;
