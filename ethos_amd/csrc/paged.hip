@@ -669,7 +669,36 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
             pos[tid] = i >= 0 ? (int64_t)c.lens[i] - c.starts[i + 1] + t : 0;
         }
     };
-    if (s.nope == 0) find_positions();
+    // the queries' last parts: four of the 32 tokens by 32 angles a thread, read first and turned while the weight is on
+    // its way
+    float2 ends[4];
+    const int p = tid & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t t = t0 + (tid >> 5) + 8 * i;
+        const uint16_t* r = q + ((t < b.n_rows ? t : b.n_rows - 1) * s.H + h) * qw + s.nope;
+        ends[i] = make_float2(bf16_bits_to_f32(r[p]), bf16_bits_to_f32(r[32 + p]));
+    }
+    const float rate = rates[p];
+    auto turn_ends = [&]() {
+        find_positions();
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int at = (tid >> 5) + 8 * i;
+            if (t0 + at >= b.n_rows) break;
+            float c, sn;
+            rotary_angle(pos[at], rate, c, sn);
+            uint16_t* to = queries + ((t0 + at) * s.H + h) * kQuery + kRank;
+            uint32_t hi, lo;
+            split_bf16x2(ends[i].x * c - ends[i].y * sn, ends[i].y * c + ends[i].x * sn, hi, lo);
+            to[p] = (uint16_t)hi;
+            to[32 + p] = (uint16_t)(hi >> 16);
+            to[kRest + p] = (uint16_t)lo;
+            to[kRest + 32 + p] = (uint16_t)(lo >> 16);
+        }
+    };
+    if (s.nope == 0) turn_ends();
     for (int j0 = 0; j0 < s.nope; j0 += 64) {
         const int rows = s.nope - j0 < 64 ? s.nope - j0 : 64;
         const uint16_t* wh = w + ((int64_t)h * (s.nope + s.v_dim) + j0) * kRank;
@@ -679,7 +708,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
             const int r = (tid >> 5) + 8 * i;
             part[i] = *reinterpret_cast<const u32x4_t*>(wh + (int64_t)(r < rows ? r : rows - 1) * kRank + (tid & 31) * 8);
         }
-        if (j0 == 0) find_positions();  // (while the weight is on its way)
+        if (j0 == 0) turn_ends();
         else __syncthreads();
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -703,7 +732,6 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
             }
         }
     }
-    if (s.nope == 0) __syncthreads();
     if (t0 + (lane & 31) < b.n_rows) {
         uint16_t* to = queries + (my_t * s.H + h) * kQuery + wave * 64 + 4 * half;
 #pragma unroll
@@ -716,22 +744,6 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
                 *reinterpret_cast<uint2*>(to + 32 * i + 2 * e) = hi;
                 if (wave * 64 >= kWidth - kRest) *reinterpret_cast<uint2*>(to + kRest + 32 * i + 2 * e) = lo;
             }
-    }
-    for (int e = tid; e < 32 * (kRope / 2); e += 256) {
-        const int64_t t = t0 + (e >> 5);
-        const int p = e & 31;
-        if (t >= b.n_rows) break;
-        float c, sn;
-        rotary_angle(pos[e >> 5], rates[p], c, sn);
-        const uint16_t* r = q + (t * s.H + h) * qw + s.nope;
-        const float u = bf16_bits_to_f32(r[p]), v = bf16_bits_to_f32(r[32 + p]);
-        uint16_t* to = queries + (t * s.H + h) * kQuery + kRank;
-        uint32_t hi, lo;
-        split_bf16x2(u * c - v * sn, v * c + u * sn, hi, lo);
-        to[p] = (uint16_t)hi;
-        to[32 + p] = (uint16_t)(hi >> 16);
-        to[kRest + p] = (uint16_t)lo;
-        to[kRest + 32 + p] = (uint16_t)(lo >> 16);
     }
 }
 
@@ -1125,16 +1137,17 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
     else if (s.rows == 32) attend(attend_kernel<2, 2, 2>, 256);
     else if (s.rows == 64) attend(attend_kernel<4, 2, 3>, 512);
     else attend(attend_kernel<8, 1, 3>, 512);
-    // (few tokens have many parts each: more threads a token)
-    if (b.n_rows <= 8)
-        hipLaunchKernelGGL((finish_kernel<1>), dim3((unsigned)(b.n_rows * s.H)), dim3(256), 0, stream, w, b.n_rows, s, plan, items, seq_item,
-                           tokens, sums, stats, out);
-    else if (b.n_rows <= 256)
-        hipLaunchKernelGGL((finish_kernel<4>), dim3((unsigned)((b.n_rows + 3) / 4 * s.H)), dim3(256), 0, stream, w, b.n_rows, s, plan, items,
-                           seq_item, tokens, sums, stats, out);
-    else
-        hipLaunchKernelGGL((finish_kernel<16>), dim3((unsigned)((b.n_rows + 15) / 16 * s.H)), dim3(256), 0, stream, w, b.n_rows, s, plan, items,
-                           seq_item, tokens, sums, stats, out);
+    // The more parts a row may have, the more threads join them.  us, with a token in 256 | 64 | 16 threads: one token of 65,536
+    // keys (256 parts) 29.4 | 44.6 | -, 16 sequences of 8,192 (32) 32.4 | 34.6 | 43.0, 16 of 4,096 and 5 tokens (16) - | 43.6 | 48.2,
+    // 64 of 4,096 (8) 47.6 | 45.3 | 46.8, 128 of 2,048 (4) 46.1 | 46.2 | 45.4, 256 of 2,048 (2) 79.7 | 80.0 | 76.8.
+    const int64_t tiles_of_rows = b.n_rows * s.H / s.rows, parts = s.groups / (tiles_of_rows > b.n_seq ? tiles_of_rows : b.n_seq);
+    auto finish = [&](auto kernel, int tokens_each) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((b.n_rows + tokens_each - 1) / tokens_each * s.H)), dim3(256), 0, stream, w, b.n_rows, s, plan,
+                           items, seq_item, tokens, sums, stats, out);
+    };
+    if (parts >= 32) finish(finish_kernel<1>, 1);
+    else if (parts >= 8) finish(finish_kernel<4>, 4);
+    else finish(finish_kernel<16>, 16);
     return (int)hipGetLastError();
 }
 
