@@ -749,7 +749,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
 
 // WR KW waves: WR share a tile of 16 WR rows, 16 each, KW the 64 keys of a step.  S stages of LDS.
 template <int WR, int KW, int S>
-__global__ __launch_bounds__(WR * KW * 64, WR * KW > 2 ? 2 : 1) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
+__global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
                                                                  const Item* __restrict__ items, const uint16_t* __restrict__ queries,
                                                                  const uint16_t* __restrict__ specials, float* __restrict__ sums,
                                                                  float2* __restrict__ stats) {
@@ -1107,12 +1107,14 @@ bool is_fast(int rank, int rope, int nope, int v_dim, int page_log, int dtype) {
     return dtype == kBF16 && rank == kRank && rope == kRope && nope % 16 == 0 && v_dim % 16 == 0 && page_log >= kBlockLog;
 }
 
-// Rows of a tile: as many as a sequence's new tokens have on the average, 16 to 128.  Workgroups of up to 32 leave room for
-// a second one on their CU.
+// Rows of a tile: as many as a sequence's new tokens have on the average, 32 to 128.  us, 64 sequences of up to 8,192 keys and 16
+// heads: two tokens 59.1 (tiles of 16: 75.1), four 74.4 in tiles of 64, 81.9 of 128, 83.3 of 32; 16 sequences, two tokens 37.5
+// in tiles of 32, 40.7 of 64.  (One token in tiles of 16: 50.0 and 30.2, of 32: 50.6 and 29.1; there are none of 16.)
 int fast_rows(int64_t n_rows, int n_seq, int H) {
     const int64_t each = n_rows * H / n_seq;
-    return each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
+    return each <= 32 ? 32 : each <= 64 ? 64 : 128;
 }
+// Workgroups of 32 rows leave room for a second one on their CU (64 sequences of one token: 55.4 us with one, 50.0 with two).
 int fast_groups(int rows, int num_cus) { return rows <= 32 ? 2 * num_cus : num_cus; }
 
 int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, const Batch& b, const float* rates, Shape s, unsigned char* ws,
@@ -1133,8 +1135,7 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
     auto attend = [&](auto kernel, int threads) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)s.groups), dim3(threads), 0, stream, pool, b, s, plan, items, queries, specials, sums, stats);
     };
-    if (s.rows == 16) attend(attend_kernel<1, 2, 2>, 128);
-    else if (s.rows == 32) attend(attend_kernel<2, 2, 2>, 256);
+    if (s.rows == 32) attend(attend_kernel<2, 2, 2>, 256);
     else if (s.rows == 64) attend(attend_kernel<4, 2, 3>, 512);
     else attend(attend_kernel<8, 1, 3>, 512);
     // The more parts a row may have, the more threads join them.  us, with a token in 256 | 64 | 16 threads: one token of 65,536
