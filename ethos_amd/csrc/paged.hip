@@ -6,10 +6,13 @@
 // the keys, which all heads then take over the same rows: one read of the cache serves every head.  A
 // sequence's rows are its (token, head) pairs, token by token, so that a tile of rows sees nearly the same keys.
 //
-// Three launches.  paged_prepare: queries [W_k,h^T q | rotated rest] per row, and the plan: tiles of rows,
+// Three launches.  The first: queries [W_k,h^T q | rotated rest] per row, and the plan: tiles of rows,
 // each with its tiles of kKeys keys, as one line of work that is cut into even shares, whatever the lengths
 // of the sequences are.  The second goes over the keys with a running maximum and sum; where a share ends
-// inside a tile of rows, each side leaves its sums.  The third joins them and multiplies with W_v,h.
+// inside a tile of rows, each side leaves its sums.  The third joins them, in order, and multiplies with W_v,h.
+//
+// Three forms: any widths in float32 arithmetic (any_*), bf16 of the model's widths, and the same with many new tokens a
+// sequence, where keys and values are formed first (expand and chunk_*).
 //
 // Without bounds of the host on lengths, tables or starts: what they hold is checked where it is used.  A page
 // outside the cache reads as a row of NaN, a length beyond the table makes its sequence's outputs NaN.
@@ -172,9 +175,11 @@ __device__ void make_plan(const Batch& b, const Shape& s, int64_t max_items, Pla
     }
     if (tid == 0) {
         if (seq_keys) seq_keys[b.n_seq] = (int32_t)key_tiles;
-        // (few tiles a workgroup, two workgroups a CU: one on each, whose parts are then half as many to join)
+        // Few tiles a workgroup, two workgroups a CU: one on each, whose parts are then half as many to join.  us with two | one,
+        // up to four tiles a workgroup of two: one sequence of 65,536 keys 35.2 | 28.2, 8 of 8,192 27.1 | 24.8, 16 of 8,192
+        // 32.8 | 30.5; beyond: 8 of 20,000 35.7 | 36.1.
         tiles *= s.planes;
-        const int64_t groups = s.rows <= 32 && tiles < 4 * (int64_t)s.groups ? (s.groups + 1) / 2 : s.groups;
+        const int64_t groups = s.rows <= 32 && tiles <= 4 * (int64_t)s.groups ? (s.groups + 1) / 2 : s.groups;
         plan->tiles = tiles;
         plan->quota = tiles > groups ? (tiles + groups - 1) / groups : 1;
         plan->n_items = (int32_t)base;
@@ -201,6 +206,10 @@ __device__ __forceinline__ int find_item(const Item* items, int n_items, int64_t
 // the scores, of 64 columns of one of four keys for the sums.  S^T = K Q^T leaves keys 4 g + e of a row in lane (row, g),
 // which is where O^T = C^T P^T takes them with key 4 g + e in place g of its product e: nothing goes through LDS but the
 // queries, and the waves run by themselves up to the end of a share, where their sums are joined.
+//
+// 512 float32 tokens over 2,048 keys, rank 256, rope 64, 16 heads: 309 us in all, 54 TFLOP/s of 129 that a large float32
+// product reaches (vector instructions over keys in LDS: 5,158).  16 sequences of one token and up to 4,096 keys: 66 us (758).  Five
+// sequences of 33 tokens, rank 32: 19 us, of which 8, 6 and 5 are the three kernels' times: launches and dependent loads.
 constexpr int kAnyRows = 16, kAnyKeys = 16, kAnyRank = 512, kAnyRope = 128, kAnyWidth = kAnyRank + kAnyRope;
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
@@ -632,7 +641,8 @@ __device__ __forceinline__ void reads_ahead() {
 constexpr int kSeqsNear = 1024;
 
 // Block 0: the plan and the two special rows.  The others: 32 tokens of a head; [c][token] = W_k,h^T q^T, the weight
-// (k as the row) through LDS in the layout of the loss's R tiles.
+// (k as the row) through LDS in the layout of the loss's R tiles.  64 sequences of a token, 16 heads: 7 to 8 us for 1.3 MB,
+// which is the launch and three loads that wait for each other; the plan takes as long beside it.
 __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ w,
                                                       const float* __restrict__ rates, Batch b, Shape s, int64_t max_items, Plan* plan,
                                                       Item* items, int32_t* seq_item, Token* tokens, uint16_t* __restrict__ specials,
@@ -747,7 +757,10 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
     }
 }
 
-// WR KW waves: WR share a tile of 16 WR rows, 16 each, KW the 64 keys of a step.  S stages of LDS.
+// WR KW waves: WR share a tile of 16 WR rows, 16 each, KW the 64 keys of a step.  S stages of LDS.  64 sequences of one token and up
+// to 8,192 keys: 186 MB in 34 us, 5.5 TB/s (256 of 2,048: 335 MB in 63), where a large copy moves 4.95: bound by memory.  16 of
+// five tokens and up to 4,096: 23 MB of cache in 26 us, three steps a workgroup between reading its queries and writing 80 rows of
+// sums (16 MB): bound by those.
 template <int WR, int KW, int S>
 __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
                                                                  const Item* __restrict__ items, const uint16_t* __restrict__ queries,
@@ -993,7 +1006,8 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
 }
 
 // TOK tokens of a head: 256 / TOK threads a token join its parts, 16 columns a thread and 16 / TOK parts side by side,
-// then [v][token] = W_v,h o^T by 16 x 16 x 32 MFMAs, a wave for every 16 of v_dim.
+// then [v][token] = W_v,h o^T by 16 x 16 x 32 MFMAs, a wave for every 16 of v_dim.  64 tokens of 16 heads and up to 16 parts: 7 us
+// for 20 MB of sums; one token's 256 parts: 10 us.  Bound by the chain token, tile, parts, sums: each read waits for the last.
 template <int TOK>
 __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict__ w, int64_t n_rows, Shape s, const Plan* plan,
                                                      const Item* __restrict__ items, const int32_t* __restrict__ seq_item,
@@ -1161,14 +1175,17 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
 // and heads as the outer dimension of the even shares, so that an XCD's workgroups read the same two heads' keys from its L2.
 //
 // Queries, keys, values and exponentials are fp16 there, of 11 bits instead of bf16's 8: the outputs' error against 64 bits
-// is that of their own rounding (with bf16 up to twice that; 120.2 -> 121.7 us for 2,048 tokens, 7,001 keys, 16 heads).  For
+// is that of their own rounding (with bf16 up to twice that; 120.9 -> 124.6 us for 2,048 tokens, 7,001 keys, 16 heads).  For
 // their range queries and keys are 2^-4 of themselves, values 2^-2, and a row's exponentials 2^6 at its maximum: a query or
 // key of 2^20 or a value of 2^18 and more counts as infinite; fp16's steps near zero are 2^-20 of a key, 2^-22 of a value
 // and 2^-30 of a weight, below bf16's where a key is 2^-11 or more and a value 2^-13.
 constexpr float kKeyScale = 0x1p-4f, kValueScale = 0x1p-2f, kQueryScale = 0x1p-4f, kTop = 6.0f;
 constexpr int kHead = 64;         // columns of a head's keys (before the rotated ones) and of its values
 constexpr int kChunkTok = 128;    // tokens of a tile
-constexpr int kChunkRows = 128;   // new tokens a sequence, on the average, from which this is the shorter way
+// New tokens a sequence, on the average, from which this is the shorter way.  us, the weight with the queries | with the keys and
+// values: 8 sequences of 4,096 keys, 64 tokens 92.5 | 115.0, 96 128.2 | 113.0, 128 158.0 | 115.6; one of 4,096, 64 tokens
+// 43.5 | 48.5, 128 57.4 | 53.5, 256 73.4 | 50.2; one of 16,384, 128 tokens 96.4 | 81.8.
+constexpr int kChunkRows = 96;
 constexpr size_t kChunkBytes = (size_t)1 << 30;  // of keys and values, at most
 
 struct ChunkLayout {
@@ -1242,7 +1259,8 @@ constexpr int kRowStage = kRank / 64 * kPlane;  // the latents of 64 rows
 // Keys and values of a head for some tiles of 64 cached rows: [column][row] = W_h c^T, a wave 32 of the
 // head's 128 columns, the weight's fragments in registers, the rows from LDS in the planes of above, the next tile's on
 // their way.  The result goes through LDS, so that its rows are stored 16 bytes a lane, one after the other (8 bytes a lane
-// at 32 rows: 21 us for 7,001 rows and 16 heads).  The rotated keys are copied by one head's workgroup of each tile.
+// at 32 rows take 2.5 us more).  The rotated keys are copied by one head's workgroup of each tile.  7,001 rows and 16 heads:
+// 19 us for 29 MB written and 7.3 GFLOP; bound by the barriers of its 2.7 tiles a workgroup.
 __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restrict__ w, const uint16_t* __restrict__ pool, Batch b, Shape s,
                                                         const int32_t* __restrict__ seq_keys, const uint16_t* __restrict__ specials,
                                                         int64_t key_rows, uint16_t* __restrict__ keys, uint16_t* __restrict__ shared) {
@@ -1386,6 +1404,10 @@ __device__ __forceinline__ void copy16_at(const void* base, uint32_t off, uint32
     asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(ring), "v"(off), "s"(base), "n"(AT) : "memory", "scc");
 }
 
+// A tile's steps for a share of its keys, two workgroups a CU; a wave 32 tokens of its own, S^T = K Q^T and O^T = V^T P^T in
+// 32 x 32 x 16 products, as in attend_kernel.  2,048 tokens over 7,001 keys, 16 heads: 75 GFLOP in 98 us, 770 TFLOP/s,
+// where a large bf16 product reaches 1,084.  Bound by a step's matrix and vector instructions, which overlap in part: 32 exponentials,
+// their sum, rounding and maximum a lane beside 24 products.
 __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __restrict__ q, const float2* __restrict__ turns,
                                                               const uint16_t* __restrict__ keys, const uint16_t* __restrict__ shared, Shape s,
                                                               const Plan* plan, const Item* __restrict__ items, int64_t key_rows,
@@ -1675,7 +1697,8 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
     }
 }
 
-// 16 (token, head) rows a workgroup, 16 threads each: joins the parts of those that have several.
+// 16 (token, head) rows a workgroup, 16 threads each: joins the parts of those that have several (8 us for 32,768 rows: 34 MB
+// of sums).
 __global__ __launch_bounds__(256) void chunk_finish_kernel(int64_t n_rows, Shape s, const Plan* plan, const Item* __restrict__ items,
                                                            const int32_t* __restrict__ seq_item, const Token* __restrict__ tokens,
                                                            const float* __restrict__ sums, const float2* __restrict__ stats,
