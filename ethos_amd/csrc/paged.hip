@@ -758,8 +758,8 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
 }
 
 // WR KW waves: WR share a tile of 16 WR rows, 16 each, KW the 64 keys of a step.  S stages of LDS.  64 sequences of one token and up
-// to 8,192 keys: 186 MB in 34 us, 5.5 TB/s (256 of 2,048: 335 MB in 63), where a large copy moves 4.95: bound by memory.  16 of
-// five tokens and up to 4,096: 23 MB of cache in 26 us, three steps a workgroup between reading its queries and writing 80 rows of
+// to 8,192 keys: 186 MB in 35 us, 5.3 TB/s (256 of 2,048: 335 MB in 63), where a large copy moves 4.95: bound by memory.  16 of
+// five tokens and up to 4,096: 23 MB of cache in 27 us, three steps a workgroup between reading its queries and writing 80 rows of
 // sums (16 MB): bound by those.
 template <int WR, int KW, int S>
 __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
@@ -1260,7 +1260,7 @@ constexpr int kRowStage = kRank / 64 * kPlane;  // the latents of 64 rows
 // head's 128 columns, the weight's fragments in registers, the rows from LDS in the planes of above, the next tile's on
 // their way.  The result goes through LDS, so that its rows are stored 16 bytes a lane, one after the other (8 bytes a lane
 // at 32 rows take 2.5 us more).  The rotated keys are copied by one head's workgroup of each tile.  7,001 rows and 16 heads:
-// 19 us for 29 MB written and 7.3 GFLOP; bound by the barriers of its 2.7 tiles a workgroup.
+// 20 us for 29 MB written and 7.3 GFLOP; bound by the barriers of its 2.7 tiles a workgroup.
 __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restrict__ w, const uint16_t* __restrict__ pool, Batch b, Shape s,
                                                         const int32_t* __restrict__ seq_keys, const uint16_t* __restrict__ specials,
                                                         int64_t key_rows, uint16_t* __restrict__ keys, uint16_t* __restrict__ shared) {
@@ -1405,8 +1405,8 @@ __device__ __forceinline__ void copy16_at(const void* base, uint32_t off, uint32
 }
 
 // A tile's steps for a share of its keys, two workgroups a CU; a wave 32 tokens of its own, S^T = K Q^T and O^T = V^T P^T in
-// 32 x 32 x 16 products, as in attend_kernel.  2,048 tokens over 7,001 keys, 16 heads: 75 GFLOP in 98 us, 770 TFLOP/s,
-// where a large bf16 product reaches 1,084.  Bound by a step's matrix and vector instructions, which overlap in part: 32 exponentials,
+// 32 x 32 x 16 products, as in attend_kernel.  2,048 tokens over 7,001 keys, 16 heads: 75 GFLOP in 96 to 100 us, 770 TFLOP/s,
+// where a large bf16 product reaches 1,127.  Bound by a step's matrix and vector instructions, which overlap in part: 32 exponentials,
 // their sum, rounding and maximum a lane beside 24 products.
 __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __restrict__ q, const float2* __restrict__ turns,
                                                               const uint16_t* __restrict__ keys, const uint16_t* __restrict__ shared, Shape s,
