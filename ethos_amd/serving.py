@@ -172,7 +172,7 @@ class LatentCache:
     Which page is whose is known on the host: no call waits for the device.  `extend` makes room for new tokens and
     gives the batch that the operators take; a fork shares its pages, and a shared page is copied when one of its
     sequences first writes in it.  The device's work (page copies, the batch's tensors) is enqueued on the current stream:
-    use a cache on one stream, or let streams wait for each other."""
+    use a cache on one stream, or let streams wait for each other.  Its calls are not for graph capture."""
 
     def __init__(self, blocks: int, rank: int, rope: int, pages: int, page: int = 64, dtype: torch.dtype = torch.bfloat16, device=None):
         if blocks <= 0 or pages <= 0 or rank <= 0 or rope < 0:
@@ -229,9 +229,12 @@ class LatentCache:
 
     def truncate(self, seq: int, length: int) -> None:
         """Forgets a sequence's tokens from `length` on."""
-        s = self._of(seq)
+        s, length = self._of(seq), operator.index(length)
         if not 0 <= length <= s.length:
             raise ValueError(f"sequence {seq} has {s.length} tokens, it cannot be cut to {length}")
+        self._cut(s, length)
+
+    def _cut(self, s: _Sequence, length: int) -> None:
         keep = -(-length // self.page)
         self._drop(reversed(s.pages[keep:]))
         del s.pages[keep:]
@@ -262,23 +265,26 @@ class LatentCache:
                     users[p] = left - 1
         if need + len(copies) > len(self._free):
             raise RuntimeError(f"the cache has {len(self._free)} free pages, {need + len(copies)} are needed")
-        src, dst = [], []
-        for i in copies:
-            p = own[i].pages[-1]
-            src.append(p)
-            dst.append(self._free.pop())
-            self._users[p] -= 1
-            self._users[dst[-1]] = 1
-            own[i].pages[-1] = dst[-1]
-        if src:
+        if copies:  # (the books behind the copies: a refused copy changes nothing)
+            src, dst = [own[i].pages[-1] for i in copies], self._free[-len(copies):].tolist()
             copy_pages(self.pool, src, dst)
+            del self._free[-len(copies):]
+            for i, p, q in zip(copies, src, dst):
+                self._users[p] -= 1
+                self._users[q] = 1
+                own[i].pages[-1] = q
         for s, c in zip(own, counts):
             s.length += c
             while len(s.pages) * self.page < s.length:
                 p = self._free.pop()
                 self._users[p] = 1
                 s.pages.append(p)
-        return self._batch(own, counts)
+        try:
+            return self._batch(own, counts)
+        except BaseException:
+            for s, c in zip(own, counts):
+                self._cut(s, s.length - c)
+            raise
 
     def _batch(self, own, counts) -> Batch:
         """The batch's arrays, in one copy to the device."""
@@ -292,7 +298,10 @@ class LatentCache:
         for s in own:
             flat.extend(s.pages)
             flat.extend(array("i", [-1]) * (width - len(s.pages)))
-        dev = torch.frombuffer(flat, dtype=torch.int32).to(self.pool.device)
+        host = torch.frombuffer(flat, dtype=torch.int32)
+        if self.pool.is_cuda:  # (from pinned memory: a copy from other memory waits for the stream)
+            host = torch.empty(host.shape, dtype=torch.int32, pin_memory=True).copy_(host)
+        dev = host.to(self.pool.device, non_blocking=True)
         return Batch(dev[2 * n + 1:].view(n, width), dev[:n], dev[n:2 * n + 1], counts)
 
     def compact(self) -> int:

@@ -166,6 +166,28 @@ def test_sampling_without_drafts():
         cache.truncate(s, 5)
 
 
+def test_a_step_does_not_wait_for_the_device():
+    """Extending (with a page to copy), truncating and the model's step return while earlier work still runs."""
+    m = _model("bf16")
+    cache = m.cache(pages=20, page=8)
+    s = cache.new()
+    ids = _ids(1, 20)
+    m.extend(ids, cache, [s])
+    f = cache.fork(s)
+    m.extend(ids[:, :1], cache, [s])  # (the copy's kernel has run once)
+    cache.truncate(s, 20)
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    torch.cuda._sleep(1 << 28)  # (a kernel of some hundred ms)
+    done.record()
+    f2 = cache.fork(f)
+    logits = m.extend(ids[:, :2].expand(2, 2).contiguous(), cache, [f, f2])
+    cache.truncate(f, 20)
+    assert not done.query()
+    torch.cuda.synchronize()
+    assert bool(logits.isfinite().all()) and torch.equal(logits[0], logits[1])
+
+
 def test_ids_outside_the_vocabulary():
     m = _model("fp32")
     ids = _ids(2, 10, seed=7)

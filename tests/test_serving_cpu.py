@@ -207,6 +207,35 @@ def test_cache_refuses_and_changes_nothing(monkeypatch):
     assert c.length(b) == 0
 
 
+def test_cache_is_as_it_was_after_a_failure(monkeypatch):
+    c = _book(monkeypatch, pages=8, page=4)
+    a = c.new()
+    _write(c, c.extend([a], [6]), [[1, 2, 3, 4, 5, 6]])
+    f = c.fork(a)
+
+    def refuse(*args):
+        raise RuntimeError("refused")
+
+    def state():
+        return c.pages(a), c.pages(f), c.length(a), c.length(f), c.pages_free, sorted(c._free)
+
+    before = state()
+    with monkeypatch.context() as m:
+        m.setattr(serving, "copy_pages", refuse)
+        with pytest.raises(RuntimeError, match="refused"):
+            c.extend([f, a], [1, 9])
+    assert state() == before
+    _consistent(c)
+    with monkeypatch.context() as m:
+        m.setattr(c, "_batch", refuse)
+        with pytest.raises(RuntimeError, match="refused"):
+            c.extend([a], [9])
+    assert (c.length(a), c.length(f)) == (6, 6) and _read(c, a) == _read(c, f) == [1, 2, 3, 4, 5, 6]
+    _consistent(c)
+    with pytest.raises(TypeError):
+        c.truncate(a, 2.0)
+
+
 def test_cache_against_a_plain_one(monkeypatch):
     """Random steps, with lists of numbers beside the cache."""
     import random
