@@ -882,14 +882,22 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
             // rows that some of the tile's rows do not see may hold anything: those whose latents are not finite
             uint64_t odd = 0;
             if (first_pos < end - 1 && k * kKeys + kKeys - 1 > first_pos) {
-                // (each wave by itself: a lane a row, its pieces in an order that spreads over the banks)
-                bool bad = false;
-                for (int c = 0; c < kRank / 8; ++c) {
-                    const u32x4_t v = *(lds_u4_ptr)(size_t)(at + (c >> 3) * kPlane + lane * 128 + (((c + (lane >> 1)) & 7) << 4));
+                // (each wave by itself, four of those rows at a time, 16 lanes a row)
+                const int seen = first_pos + 1 - k * kKeys, stop_row = end - k * kKeys < kKeys ? end - k * kKeys : kKeys;
+                for (int r0 = seen > 0 ? seen : 0; r0 < stop_row; r0 += 4) {
+                    const int r = r0 + g;
+                    bool bad = false;
+                    if (r < stop_row)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+                        for (int c = 0; c < kRank / 64; c += 2) {
+                            const u32x4_t v = *(lds_u4_ptr)(size_t)(at + (c + ((lane >> 3) & 1)) * kPlane + r * 128 + ((lane & 7) << 4));
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+                        }
+                    const uint64_t some = ballot(bad);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) odd |= (uint64_t)((some >> (16 * i) & 0xffff) != 0) << ((r0 + i) & 63);
                 }
-                odd = ballot(bad);
             }
             f32x4_t x[KB];
             if (odd != 0 && !active) clear_odd(odd, at);
