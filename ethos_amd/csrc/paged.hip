@@ -759,8 +759,8 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
 
 // WR KW waves: WR share a tile of 16 WR rows, 16 each, KW the 64 keys of a step.  S stages of LDS.  64 sequences of one token and up
 // to 8,192 keys: 186 MB in 35 us, 5.3 TB/s (256 of 2,048: 335 MB in 63), where a large copy moves 4.95: bound by memory.  16 of
-// five tokens and up to 4,096: 23 MB of cache in 27 us, three steps a workgroup between reading its queries and writing 80 rows of
-// sums (16 MB): bound by those.
+// five tokens and up to 4,096: 23 MB of cache in 24 us, three steps a workgroup, bound by LDS (a fragment serves 16 rows), between
+// reading its queries and writing 80 rows of sums (16 MB).
 template <int WR, int KW, int S>
 __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
                                                                  const Item* __restrict__ items, const uint16_t* __restrict__ queries,

@@ -11,7 +11,7 @@ import torch
 
 from ethos_amd import workloads
 from ethos_amd.model import CompressedMoEModel, init_random_, lm_config
-from ethos_amd.serving import LatentCache
+from ethos_amd.serving import Batch, LatentCache
 
 pytestmark = pytest.mark.gpu
 
@@ -186,6 +186,49 @@ def test_a_step_does_not_wait_for_the_device():
     assert not done.query()
     torch.cuda.synchronize()
     assert bool(logits.isfinite().all()) and torch.equal(logits[0], logits[1])
+
+
+@pytest.mark.parametrize("kind", ["fp32", "bf16"])
+def test_captured_steps_over_a_batch_of_ones_own(kind):
+    """The blocks' steps captured once, over a batch in fixed tensors, and replayed with eager work in between."""
+    m, b, width = _model(kind), 3, 12
+    ids = _ids(b, 40, seed=12)
+    caches = [m.cache(pages=50, page=8) for _ in range(2)]
+    seqs = [[c.new() for _ in range(b)] for c in caches]
+    for c, q in zip(caches, seqs):
+        m.extend(torch.cat((ids[0, :20], ids[1, :3], ids[2, :9])), c, q, [20, 3, 9])
+    at = [20, 3, 9]
+    table = torch.full((b, width), -1, dtype=torch.int32, device="cuda")
+    lens, starts = torch.zeros(b, dtype=torch.int32, device="cuda"), torch.arange(b + 1, dtype=torch.int32, device="cuda")
+    batch = Batch(table, lens, starts, [1] * b)
+    x = torch.zeros(b, m.config.d_model, dtype=m.tok_embeddings.weight.dtype, device="cuda")
+
+    def blocks():
+        h = x
+        for block, pool in zip(m.layers, caches[0].pool):
+            h = block.extend(h, pool, batch)
+        return m.output(m.norm(h))
+
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            blocks()  # (lengths of zero: nothing is written or seen)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = blocks()
+    for step in range(8):
+        token = torch.stack([ids[i, at[i] + step] for i in range(b)])
+        now = caches[0].extend(seqs[0], [1] * b)
+        table.fill_(-1)
+        table[:, : now.table.shape[1]] = now.table
+        lens.copy_(now.lens)
+        x.copy_(m.tok_embeddings.weight[token])
+        graph.replay()
+        want = m.extend(token[:, None], caches[1], seqs[1])[:, 0]
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), step
 
 
 def test_ids_outside_the_vocabulary():
