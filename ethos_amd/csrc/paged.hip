@@ -1773,7 +1773,8 @@ size_t paged_attention_workspace_bytes(int64_t n_rows, int n_seq, int H, int ran
     const int64_t capacity = (int64_t)width << page_log;
     if (is_fast(rank, rope, nope, v_dim, page_log, dtype) && is_chunk(n_rows, n_seq, H, nope, v_dim, capacity))
         return chunk_layout(n_rows, n_seq, H, capacity, chunk_groups(num_cus)).bytes;
-    if (is_fast(rank, rope, nope, v_dim, page_log, dtype)) return layout(n_rows, n_seq, H, kQuery, rows, fast_groups(rows, num_cus), 2, kRank).bytes;
+    if (is_fast(rank, rope, nope, v_dim, page_log, dtype))
+        return layout(n_rows, n_seq, H, kQuery, rows, fast_groups(rows, num_cus), 2, kRank).bytes;
     return layout(n_rows, n_seq, H, rank + rope, kAnyRows, any_groups(num_cus), 4, rank).bytes;
 }
 

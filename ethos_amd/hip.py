@@ -921,10 +921,14 @@ def copy_pages(pool: torch.Tensor, src: list, dst: list) -> None:
 def verify(logits: torch.Tensor, drafts: torch.Tensor, probs: torch.Tensor | None, counts: torch.Tensor | None, u_accept: torch.Tensor,
            u_sample: torch.Tensor, temperature: float):
     """(accepted int32 [b], tokens int64 [b]) of logits [b, m + 1, V]."""
-    _need_here(logits, "logits", FLOATS, 3)
-    _need_here(drafts, "drafts", (torch.int64,), 2)
-    _need_here(u_accept, "u_accept", (torch.float32,), 2)
-    _need_here(u_sample, "u_sample", (torch.float32,), 1)
+    device = _current_device()
+    if not (_dense_at(device, logits) and logits.dtype in FLOATS and logits.dim() == 3 and _dense_at(device, drafts, torch.int64)
+            and drafts.dim() == 2 and _dense_at(device, u_accept, torch.float32) and u_accept.dim() == 2
+            and _dense_at(device, u_sample, torch.float32) and u_sample.dim() == 1):
+        _need_here(logits, "logits", FLOATS, 3)
+        _need_here(drafts, "drafts", (torch.int64,), 2)
+        _need_here(u_accept, "u_accept", (torch.float32,), 2)
+        _need_here(u_sample, "u_sample", (torch.float32,), 1)
     b, rows, V = logits.shape
     m = rows - 1
     if probs is not None:

@@ -137,12 +137,11 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u_accept: torch.Te
     stand, or that is 0 everywhere): the lowest index whose weights up to it exceed u_sample of their sum.  Tokens and drafts
     together are then distributed as p's.  Without drafts (m = 0) it samples.  Words may be masked by logits of -inf.  A
     token is -1 where its row has a NaN, no finite logit, or one that is +inf (with a temperature).  All in float64."""
-    _check("verify_drafts", *(t for t in (logits, drafts, u_accept, u_sample, draft_probs, counts) if t is not None))
-    for name, t, kinds in (("logits", logits, hip.FLOATS), ("draft_probs", draft_probs, hip.FLOATS), ("drafts", drafts, (torch.int64,)),
-                           ("counts", counts, (torch.int32,)), ("u_accept", u_accept, (torch.float32,)),
-                           ("u_sample", u_sample, (torch.float32,))):
-        if t is not None and t.dtype not in kinds:
-            raise TypeError(f"{name} must be {' or '.join(str(k) for k in kinds)}, got {t.dtype}")
+    _check("verify_drafts", *[t for t in (logits, drafts, u_accept, u_sample, draft_probs, counts) if t is not None])
+    if (logits.dtype not in hip.FLOATS or drafts.dtype != torch.int64 or u_accept.dtype != torch.float32 or u_sample.dtype != torch.float32
+            or draft_probs is not None and draft_probs.dtype not in hip.FLOATS or counts is not None and counts.dtype != torch.int32):
+        raise TypeError(f"verify_drafts takes logits and draft_probs of {' or '.join(map(str, hip.FLOATS))}, int64 drafts, float32 u_accept and "
+                        f"u_sample and int32 counts, got {[t if t is None else t.dtype for t in (logits, draft_probs, drafts, u_accept, u_sample, counts)]}")
     dense = [None if t is None else t.contiguous() for t in (logits, drafts, draft_probs, counts, u_accept, u_sample)]
     return hip.verify(*dense, temperature)
 

@@ -622,8 +622,9 @@ int ethos_latent_append(const void* rows, int64_t ld, const void* gain, const fl
  *   w    [n_heads (nope + v_dim), rank] dtype T (kv_b_proj's weight): head h's keys are its first nope rows times the
  *        cached latent, then the cached key; its values the next v_dim rows times the latent
  *   out  [n_rows, n_heads, v_dim] dtype T: softmax(scale q k) v
- * The weight enters with the queries and behind the sums over latents: in bf16 these products, and the exponentials,
- * are rounded to bf16; scores, maxima and sums are float32.  A token that sees no position has a row of zeros; one that sees
+ * Scores, maxima and sums are float32, products of bf16 tensors of bf16 operands, or of float32 ones where widths are others
+ * than rank 256 and rope 64; with 96 new tokens or more a sequence on the average, and nope = v_dim = 64, of fp16 ones: a query
+ * or key of 2^20 and more, or a value of 2^18, then counts as infinite.  A token that sees no position has a row of zeros; one that sees
  * a position without a page, or a row with a value that is not finite, has NaN, as have all tokens of a sequence whose
  * length is negative, over 2^30 or beyond its table, or whose rows are not in the batch.
  *   workspace  >= ethos_paged_attention_workspace_bytes(...) bytes (scratch)
