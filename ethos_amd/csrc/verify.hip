@@ -163,22 +163,25 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args a) {
     }
 }
 
-// A row's maximum, sum and arg from its chunks, by a wave; NaN where the row has no distribution.
+// A row's maximum, sum and arg from its chunks, by W neighbouring lanes (lane: its place among them); NaN where the row has no
+// distribution.
+template <int W>
 __device__ __forceinline__ Chunk join_chunks(const Args& a, const double* table, int64_t row, int lane) {
     float m = -INFINITY;
     int32_t at = INT32_MAX;
     const Chunk* stats = a.stats + row * a.chunks;
-    for (int s = lane; s < a.chunks; s += 64) take_first(m, at, stats[s].max, stats[s].arg);
+    for (int s = lane; s < a.chunks; s += W) take_first(m, at, stats[s].max, stats[s].arg);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) take_first(m, at, __shfl_xor(m, d, 64), __shfl_xor(at, d, 64));
+    for (int d = 1; d < W; d <<= 1) take_first(m, at, __shfl_xor(m, d, 64), __shfl_xor(at, d, 64));
     const Exp x = exp_from(m, a.rate);
     double sum = 0.0;
-    for (int s = lane; s < a.chunks; s += 64) {
+    for (int s = lane; s < a.chunks; s += W) {
         const Chunk k = stats[s];
         // (a chunk without a finite value: its sum is 0, or NaN)
         sum += k.max == -INFINITY || a.rate == 0.0 ? k.sum : k.sum * exp_of(x, table, k.max);
     }
-    sum = wave_sum_f64(sum);
+#pragma unroll
+    for (int d = 1; d < W; d <<= 1) sum += __shfl_xor(sum, d, 64);
     return Chunk{m == -INFINITY ? NAN : sum, m, at};
 }
 
@@ -215,9 +218,17 @@ __device__ __forceinline__ int decide(const Args& a, int64_t i, int n, double* t
     exp_table(table, tid);
     if (tid == 0) first_bad = n;
     __syncthreads();
-    for (int j = wave; j <= n; j += 4) {
-        const Chunk k = join_chunks(a, table, row0 + j, lane);
-        if (lane == 0) rows[j] = k;
+    // rows of few chunks four a wave (16 sequences of 9 rows of 4 chunks, the kernel's time: 13.1 us with one a wave, 11.0 with four)
+    if (a.chunks <= 16) {
+        for (int j = tid >> 4; j <= n; j += 16) {
+            const Chunk k = join_chunks<16>(a, table, row0 + j, lane & 15);
+            if ((lane & 15) == 0) rows[j] = k;
+        }
+    } else {
+        for (int j = wave; j <= n; j += 4) {
+            const Chunk k = join_chunks<64>(a, table, row0 + j, lane);
+            if (lane == 0) rows[j] = k;
+        }
     }
     __syncthreads();
     if (tid < n) {
@@ -411,8 +422,8 @@ __global__ __launch_bounds__(256) void token_kernel(Args a) {
 
 // All three in one launch for few sequences: each workgroup decides by itself which row its part is of, and the
 // sequence's last one to come here finds the token.  (For many, a launch each: a workgroup that says that it is done waits
-// for the caches, some 0.2 us one after the other on an XCD.  64 sequences of 100,277 words: 85 us in one launch, and in three 5.8,
-// 11.7 and 7.3.)
+// for the caches, some 0.2 us one after the other on an XCD.  64 sequences of 100,277 words: 85 us in one launch, and in three 4.8,
+// 11.6 and 7.2.)
 template <typename T, typename Q>
 __global__ __launch_bounds__(256) void draw_kernel(Args a) {
     __shared__ double table[32], sums[kPartsMax], ss[4];
