@@ -1268,7 +1268,8 @@ constexpr int kRowStage = kRank / 64 * kPlane;  // the latents of 64 rows
 // head's 128 columns, the weight's fragments in registers, the rows from LDS in the planes of above, the next tile's on
 // their way.  The result goes through LDS, so that its rows are stored 16 bytes a lane, one after the other (8 bytes a lane
 // at 32 rows take 2.5 us more).  The rotated keys are copied by one head's workgroup of each tile.  7,001 rows and 16 heads:
-// 20 us for 29 MB written and 7.3 GFLOP; bound by the barriers of its 2.7 tiles a workgroup.
+// 20 us for 29 MB written and 7.3 GFLOP; bound by a chain of lookups, first copies and the weight, then four tiles a workgroup one
+// after the other (copies two tiles ahead change nothing).
 __global__ __launch_bounds__(256, 2) void expand_kernel(const uint16_t* __restrict__ w, const uint16_t* __restrict__ pool, Batch b, Shape s,
                                                         const int32_t* __restrict__ seq_keys, const uint16_t* __restrict__ specials,
                                                         int64_t key_rows, uint16_t* __restrict__ keys, uint16_t* __restrict__ shared) {
@@ -1756,8 +1757,8 @@ int launch_chunk(const uint16_t* q, const uint16_t* w, const uint16_t* pool, con
     float* sums = (float*)(ws + l.sums);
     hipLaunchKernelGGL(chunk_prepare_kernel, dim3((unsigned)((b.n_rows + 7) / 8 + 1)), dim3(256), 0, stream, rates, b, s, l.max_items, plan, items,
                        seq_item, seq_keys, tokens, specials, turns);
-    hipLaunchKernelGGL(expand_kernel, dim3((unsigned)(8 * s.H * ((2 * num_cus + 8 * s.H - 1) / (8 * s.H)))), dim3(256), 0, stream, w, pool, b, s, seq_keys, specials,
-                       l.key_rows, keys, shared);
+    const unsigned expand_groups = (unsigned)(8 * s.H * ((2 * num_cus + 8 * s.H - 1) / (8 * s.H)));  // eight tiles for all heads, times
+    hipLaunchKernelGGL(expand_kernel, dim3(expand_groups), dim3(256), 0, stream, w, pool, b, s, seq_keys, specials, l.key_rows, keys, shared);
     hipLaunchKernelGGL(chunk_attend_kernel, dim3((unsigned)s.groups), dim3(256), 0, stream, q, turns, keys, shared, s, plan, items,
                        l.key_rows, sums, stats, out);
     hipLaunchKernelGGL(chunk_finish_kernel, dim3((unsigned)((b.n_rows * s.H + 15) / 16)), dim3(256), 0, stream, b.n_rows, s, plan, items,
