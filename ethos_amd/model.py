@@ -21,6 +21,7 @@ How it is computed here:
     the attention (rotations, scores, softmax, values) is a HIP kernel that reads the
     projections' outputs as they are (bf16, head widths 64 + 64 and 64); under autograd, with a
     mask, or in other shapes they are torch operations and SDPA.
+New tokens over a cache of what came before (extend, speculate) go through the kernels of ethos_amd.serving.
 The expert layer is EthosExpertLayer (HIP kernels).  Inputs live on a HIP device.
 """
 from __future__ import annotations
