@@ -31,21 +31,21 @@ struct Chunk {
 // exponent and the series of 2^r to r^4, whose rest is 1.2e-12.  (The table of 32 doubles is LDS's 64 banks once: lanes
 // read it without conflicts.  With the series alone, to r^11 and over a range of 1, the rows' sums took 36 us where
 // they now take 28: the kernel is bound by its vector instructions, a dozen of float64 a value.)  Below 2^-1020: zero.  NaN stays.
+// The difference comes before the scale: it is 0 at the maximum, however far from zero that is, where
+// l rate - RN(max rate) would be the rounding of max rate, an exponent of any size for maxima of 1e16 and more.
 struct Exp {
-    double rate32, off;
-    float base;
+    double rate32, base;
 };
 __device__ __forceinline__ Exp exp_from(float base, double rate) {
     // (a maximum of -inf: no value has a weight)
-    const float b = base == -INFINITY ? 0.0f : base;
-    return Exp{rate * 32.0, -(double)b * (rate * 32.0), b};
+    return Exp{rate * 32.0, base == -INFINITY ? 0.0 : (double)base};
 }
 __device__ __forceinline__ void exp_table(double* table, int tid) {
     if (tid < 32) table[tid] = exp2((double)tid / 32.0);
 }
 __device__ __forceinline__ double exp_of(const Exp& x, const double* table, float l) {
     constexpr double kLn = 0.6931471805599453 / 32.0, kMagic = 6755399441055744.0;  // 1.5 2^52: its sum's low word is a rounded k
-    const double t = __builtin_fma((double)l, x.rate32, x.off), s = t + kMagic, r = t - (s - kMagic);
+    const double t = ((double)l - x.base) * x.rate32, s = t + kMagic, r = t - (s - kMagic);
     const int k = __double2loint(s);
     double e = __builtin_fma(r, kLn * kLn * kLn * kLn / 24.0, kLn * kLn * kLn / 6.0);
     e = __builtin_fma(e, r, kLn * kLn / 2.0);

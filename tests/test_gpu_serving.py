@@ -622,6 +622,48 @@ def test_verify_takes_the_first_of_equal_logits():
     assert got[0].tolist() == [1, 1, 0] and got[1].tolist() == [0, 20000, 29999]
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("mask", [-1e4, -1e9, -1e19, -1e20, -1e25, -1e30, "lowest"])
+@pytest.mark.parametrize("b,m", [(5, 2), (130, 2)])
+def test_verify_under_finite_masks(b, m, mask, dt):
+    """Whole chunks (of 2,048 words, and of 8,192 where there are many rows) at one large finite value, and rows with nothing else."""
+    V, T = 30001, DT[dt]
+    value = torch.finfo(T).min if mask == "lowest" else mask
+    logits, _, ua, us, _ = _verify_case(b, m, V, dt, "none", seed=11)
+    logits[:, :, 2048:4096] = value
+    logits[:, :, 8192:24576] = value
+    logits[3] = value
+    logits[4, :, 5000:] = value
+    p = torch.softmax(logits[:, :m].float(), -1)
+    drafts = torch.multinomial(p.view(-1, V), 1, generator=_gen(12)).view(b, m)
+    drafts[0, 1] = 3000  # one of no weight
+    for temperature in (1.0, 0.92, 1.03, 1.21, 0.7, 1e-6, 1e6, 0.0) if b == 5 else (1.0, 1.21, 0.0):
+        for probs in (p, None):
+            got = ethos_amd.verify_drafts(logits, drafts, ua, us, draft_probs=probs, temperature=temperature)
+            assert (got[0].tolist(), got[1].tolist()) == _verify_oracle(logits, drafts, ua, us, probs, None, temperature), temperature
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("top", [1e16, -1e16, 1e20, -1e20, 1e30, -1e30, "highest", "lowest"])
+def test_verify_of_rows_far_from_zero(top, dt):
+    """Rows whose largest logits, some of each row's, are alike and far from zero: those share the weight, whatever the temperature."""
+    b, m, V, T, g = 6, 3, 20001, DT[dt], _gen(13)
+    top = torch.finfo(T).max if top == "highest" else torch.finfo(T).min if top == "lowest" else top
+    high = torch.tensor(top, dtype=T, device="cuda")
+    low = high.double() - abs(high.double()) / 64
+    low = torch.tensor(max(float(low), float(torch.finfo(T).min)), dtype=T, device="cuda")
+    logits = torch.where(torch.rand(b, m + 1, V, generator=g, device="cuda") < 0.3, high, low)
+    drafts = logits[:, :m].float().argmax(-1)
+    # draft probabilities around the model's: the random numbers accept some and refuse others
+    count = (logits[:, :m] == logits[:, :m].amax(-1, keepdim=True)).sum(-1, keepdim=True)
+    p = (logits[:, :m] == logits[:, :m].amax(-1, keepdim=True)).float() / count * (0.5 + torch.rand(b, m, V, generator=g, device="cuda") * 2)
+    ua, us = torch.rand(b, m, generator=g, device="cuda"), torch.rand(b, generator=g, device="cuda")
+    for temperature in (1.0, 0.8, 0.7, 1.3, 0.0):
+        for probs in (p, None):
+            got = ethos_amd.verify_drafts(logits, drafts, ua, us, draft_probs=probs, temperature=temperature)
+            assert (got[0].tolist(), got[1].tolist()) == _verify_oracle(logits, drafts, ua, us, probs, None, temperature), temperature
+
+
 def test_verified_tokens_are_distributed_as_the_model_says():
     """100,000 sequences of one draft over 12 words: each word's frequency as first token within five standard deviations."""
     n, V, g = 100000, 12, _gen(3)
