@@ -437,22 +437,22 @@ __global__ __launch_bounds__(256, RB > 4 ? 1 : 2) void any_attend_kernel(const T
     }
 }
 
-// The parts of a row's sums: n of them, in slots one apart.  `row` of the sequence's in a plane; in: its place in a part.
+// The parts of a row's sums: n of them, in slots one apart.  `row`: of the token's sequence in a plane; in: its place in a part.
 struct Parts {
     int64_t slot;
     int n;
-    bool bad;  // no result
+    bool blind;  // its token sees no position: the result is zeros
 };
-__device__ __forceinline__ Parts row_parts(const Shape& s, const Plan* plan, const Item* items, const int32_t* seq_item, int seq, int64_t row,
-                                           int plane, int& in) {
-    Parts p = {0, 0, true};
+__device__ __forceinline__ Parts row_parts(const Shape& s, const Plan* plan, const Item* items, const int32_t* seq_item, const Token& token,
+                                           int64_t row, int plane, int& in) {
+    Parts p = {0, 0, false};
     in = 0;
-    if (seq < 0) return p;
-    const int32_t first = seq_item[seq];
+    if (token.seq < 0) return p;
+    const int32_t first = seq_item[token.seq];
     if (first < 0) return p;  // there was no room for it
-    p.bad = false;
     const int64_t item = first + row / s.rows;
     in = (int)(row % s.rows);
+    p.blind = items[item].pos0 + token.index < 0;
     int64_t begin = item > 0 ? items[item - 1].end : 0, end = items[item].end;
     if (end > begin) {
         const int64_t before = plane * (plan->tiles / s.planes);  // the work of the planes before
@@ -463,6 +463,9 @@ __device__ __forceinline__ Parts row_parts(const Shape& s, const Plan* plan, con
     }
     return p;
 }
+// What a row's sums are multiplied with.  No weight at all (nothing to join, or every score -inf) is no result, NaN, unless the
+// token sees nothing.
+__device__ __forceinline__ float inverse(float l, bool blind) { return l != 0.0f ? 1.0f / l : blind ? 0.0f : NAN; }
 
 // A workgroup a (token, head): joins its row's parts, four columns a thread and as many parts side by side as there are
 // threads for, and multiplies with W_v,h, 16 threads a column.
@@ -479,7 +482,7 @@ __global__ __launch_bounds__(256) void any_finish_kernel(const T* __restrict__ w
     if (token.seq == kNoSeq) return;  // behind the last sequence
     const int cols = s.rank / 4, groups = 256 / cols, grp = tid / cols, col = (tid - grp * cols) * 4;
     int in = 0;
-    const Parts p = row_parts(s, plan, items, seq_item, token.seq, (int64_t)token.index * s.H + h, 0, in);
+    const Parts p = row_parts(s, plan, items, seq_item, token, (int64_t)token.index * s.H + h, 0, in);
     if (grp < groups) {
         float top = kLowest, l = 0.0f;
         f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -520,7 +523,7 @@ __global__ __launch_bounds__(256) void any_finish_kernel(const T* __restrict__ w
             l += ls[k] * f;
             v += *reinterpret_cast<const f32x4_t*>(part + k * s.rank + tid * 4) * f;
         }
-        const float inv = p.bad ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = inverse(l, p.blind);
         *reinterpret_cast<f32x4_t*>(o + tid * 4) = v * inv;
     }
     __syncthreads();
@@ -1038,7 +1041,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
         first[st] = *reinterpret_cast<const bf16x8_t*>(wv + (int64_t)(wave * 16 < s.v_dim ? wave * 16 : 0) * kRank + 32 * st);
     const Token token = t < n_rows ? tokens[t] : Token{kNoSeq, 0};
     int in;
-    const Parts p = row_parts(s, plan, items, seq_item, token.seq, (int64_t)token.index * s.H + h, 0, in);
+    const Parts p = row_parts(s, plan, items, seq_item, token, (int64_t)token.index * s.H + h, 0, in);
     float top = kLowest, l = 0.0f, v[16] = {};
     for (int k = sub; k < p.n; k += 4 * G) {  // four parts' loads on their way at a time
         float2 ml[4];
@@ -1082,7 +1085,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
             f[g] = __builtin_amdgcn_exp2f(tops[mine + g] - all);
             sum += ls[mine + g] * f[g];
         }
-        const float inv = p.bad ? NAN : sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = inverse(sum, p.blind);
 #pragma unroll
         for (int c = 0; c < TOK; ++c) {
             const int at = c * 16 * G + (sub * 16 + (tid & 15));
@@ -1094,7 +1097,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
             os[1][tok][at] = f32_to_bf16_bits(x * inv - bf16_bits_to_f32(hi));
         }
     } else {
-        const float inv = p.bad ? NAN : l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = inverse(l, p.blind);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             uint2 hi, lo;
@@ -1683,7 +1686,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
         lds_barrier();
         if (my < it.rows) {
             if (t == begin && to == finish) {  // the tile's whole work
-                const float inv = l == 0.0f ? 0.0f : 1.0f / (l * kValueScale);
+                const float inv = inverse(l * kValueScale, my_pos < 0);
                 uint16_t* z = out + (row * s.H + h) * kHead + 4 * half;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -1718,7 +1721,7 @@ __global__ __launch_bounds__(256) void chunk_finish_kernel(int64_t n_rows, Shape
     const Token token = tokens[t];
     if (token.seq == kNoSeq) return;
     int in;
-    const Parts p = row_parts(s, plan, items, seq_item, token.seq, token.index, h, in);
+    const Parts p = row_parts(s, plan, items, seq_item, token, token.index, h, in);
     if (p.n == 1) return;  // written as a whole
     float top = kLowest, l = 0.0f;
     f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1731,7 +1734,7 @@ __global__ __launch_bounds__(256) void chunk_finish_kernel(int64_t n_rows, Shape
         l = l * f + ml.y * f2;
         v = v * f + x * f2;
     }
-    const float inv = p.bad ? NAN : l == 0.0f ? 0.0f : 1.0f / (l * kValueScale);
+    const float inv = inverse(l * kValueScale, p.blind);
     *reinterpret_cast<uint2*>(out + r * kHead + col) = make_uint2(pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
 }
 

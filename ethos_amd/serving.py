@@ -85,7 +85,8 @@ def paged_attention(q: torch.Tensor, weight: torch.Tensor, pool: torch.Tensor, t
     softmax(scale q k) v over them, with k = [weight's nope rows of the head times the latent | the cached key] and v its
     v_dim rows times the latent.  One token a sequence, a few or thousands: any mixture.  Rows of no sequence are left as
     they are (`out`, or uninitialised); a token that sees nothing has zeros; one that sees a position without a page,
-    or a latent that is not finite, NaN.  Scores and sums are float32; in bf16
+    a latent that is not finite or a key that is NaN, NaN.  An infinite key gives NaN, or no weight where the score is -inf; if all are,
+    NaN.  Scores and sums are float32; in bf16
     (rank 256, rope 64, pages of 8 tokens or more) products take bf16 operands, and where sequences have 96 new tokens or
     more on the average, and nope and v_dim are 64, fp16 ones: there a query or a key of 2^20 and more, or a value of 2^18,
     counts as infinite.  `out`: a contiguous tensor for the result, apart from the inputs."""

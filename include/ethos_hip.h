@@ -625,8 +625,10 @@ int ethos_latent_append(const void* rows, int64_t ld, const void* gain, const fl
  * Scores, maxima and sums are float32, products of bf16 tensors of bf16 operands, or of float32 ones where widths are others
  * than rank 256 and rope 64; with 96 new tokens or more a sequence on the average, and nope = v_dim = 64, of fp16 ones: a query
  * or key of 2^20 and more, or a value of 2^18, then counts as infinite.  A token that sees no position has a row of zeros; one that sees
- * a position without a page, or a row with a value that is not finite, has NaN, as have all tokens of a sequence whose
- * length is negative, over 2^30 or beyond its table, or whose rows are not in the batch.
+ * a position without a page, a latent that is not finite or a key that is NaN has NaN, as have all tokens of a sequence whose
+ * length is negative, over 2^30 or beyond its table, or whose rows are not in the batch.  An infinity in a cached key alone
+ * gives NaN, or no weight to its position where the score is -inf (scores times `scale` under -2^125 count as -inf); a token
+ * all of whose scores are -inf has NaN.
  *   workspace  >= ethos_paged_attention_workspace_bytes(...) bytes (scratch)
  * q, w, pool, workspace and out 16-byte aligned; scale positive.
  */

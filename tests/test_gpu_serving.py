@@ -439,6 +439,48 @@ def test_attention_under_large_scores(dt):
     assert not bool(((got.double() - want).abs() > bound)[sure].any())
 
 
+@pytest.mark.parametrize("dt,rank,new", [("bf16", 256, 3), ("bf16", 256, 150), ("bf16", 64, 3), ("fp32", 64, 40)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attention_over_infinite_rotary_keys(dt, rank, new, sign):
+    """An infinite value in a cached key alone: a score of +inf leaves no result, one of -inf no weight (or, of a query that goes into the
+    products as two values, no result); scores of -inf everywhere leave none.  (With rates of zero, so that a query keeps its signs.)"""
+    c = _case([400, 170], [new, new], 4, rank, 64, 64, 64, 16, dt, seed=21)
+    c["rates"] = torch.zeros_like(c["rates"])
+    c["q"][:, :2, 64 + 5] = c["q"][:, :2, 64 + 5].abs() * sign + 0.25 * sign  # heads 0 and 1 towards +inf, 2 and 3 to -inf
+    c["q"][:, 2:, 64 + 5] = c["q"][:, 2:, 64 + 5].abs() * -sign - 0.25 * sign
+    good = _attend(c)
+    _near(good, c)
+    flat = c["pool"].view(-1, rank + 64)
+    at = _slots(c["table"], 0, torch.tensor([200], device="cuda"), 16)
+    flat[at, rank + 5] = sign * math.inf
+    got = _attend(c)
+    assert torch.equal(got[new:], good[new:])
+    heads = got.view(-1, 4, 64)
+    assert bool(heads[:new, :2].isnan().all())
+    split = dt == "bf16" and rank == 256 and new < 96
+    # the same without that position
+    rest = dict(c, pool=c["pool"].clone(), lens=i32([399, 170]))
+    p = torch.arange(400, device="cuda")
+    rest["pool"].view(-1, rank + 64)[_slots(c["table"], 0, p[:399], 16)] = flat[_slots(c["table"], 0, p[p != 200], 16)]
+    want, bound, _ = _oracle(rest)
+    far = (heads.double() - want.view(heads.shape)).abs() > bound.view(heads.shape)
+    none = heads.isnan()
+    assert not bool((far & ~none)[:new, 2:].any()) and (split or not bool(none[:new, 2:].any()))
+    # one that the last token alone sees
+    keep = flat[_slots(c["table"], 0, p, 16), rank + 5].clone()
+    keep[200] = 0.5
+    flat[_slots(c["table"], 0, p, 16), rank + 5] = keep
+    good[:new] = _attend(c)[:new]
+    flat[_slots(c["table"], 0, p[399:], 16), rank + 5] = sign * math.inf
+    got = _attend(c)
+    assert torch.equal(got[:new - 1], good[:new - 1]) and torch.equal(got[new:], good[new:])
+    assert bool(got.view(-1, 4, 64)[new - 1, :2].isnan().all())
+    # every position
+    flat[_slots(c["table"], 0, p, 16), rank + 5] = sign * math.inf
+    got = _attend(c)
+    assert torch.equal(got[new:], good[new:]) and bool(got[:new].isnan().all())
+
+
 @pytest.mark.parametrize("new", [1, 6, 64])
 @pytest.mark.parametrize("middle", [1, 333])
 def test_attention_in_streams_and_graphs(new, middle):
