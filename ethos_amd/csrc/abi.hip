@@ -1233,7 +1233,9 @@ int ethos_paged_attention(const void* q, const void* w, const void* pool, const 
     g_err[0] = 0;
     if (const int rc = batch_sizes(n_rows, n_seq, table_ld, table_width, n_pages, page, rank, rope, dtype, "ethos_paged_attention")) return rc;
     if (const int rc = paged_sizes(n_rows, n_heads, nope, v_dim, "ethos_paged_attention")) return rc;
-    if (!(scale > 0.0f && scale <= 3.0e38f)) return fail(ETHOS_ESIZE, "ethos_paged_attention: scale must be positive, got %g", (double)scale);
+    // (the kernels' factor of a score, up to 2^8 log2 e times the scale, is a float32 number)
+    if (!(scale > 0.0f && scale <= 1.0e35f))
+        return fail(ETHOS_ESIZE, "ethos_paged_attention: scale must be positive and at most 1e35, got %g", (double)scale);
     if (n_rows == 0 || n_seq == 0) return 0;
     if (!q || !w || !pool || (table_width > 0 && !table) || !lens || !starts || (rope > 0 && !rates) || !workspace || !out)
         return fail(ETHOS_ENULL, "ethos_paged_attention: null pointer");

@@ -82,7 +82,7 @@ def paged_attention(q: torch.Tensor, weight: torch.Tensor, pool: torch.Tensor, t
 
     q [n, heads, nope + rope], the rotary part not yet rotated; weight [heads (nope + v_dim), rank], kv_b_proj's;
     pool, table, lens, starts and rates as latent_append takes them.  A token sees its sequence's positions up to its own:
-    softmax(scale q k) v over them, with k = [weight's nope rows of the head times the latent | the cached key] and v its
+    softmax(scale q k) v (scale positive, at most 1e35) over them, with k = [weight's nope rows of the head times the latent | the cached key] and v its
     v_dim rows times the latent.  One token a sequence, a few or thousands: any mixture.  Rows of no sequence are left as
     they are (`out`, or uninitialised); a token that sees nothing has zeros; one that sees a position without a page,
     a latent that is not finite or a key that is NaN, NaN.  An infinite key gives NaN, or no weight where the score is -inf; if all are,

@@ -481,6 +481,19 @@ def test_attention_over_infinite_rotary_keys(dt, rank, new, sign):
     assert torch.equal(got[new:], good[new:]) and bool(got[:new].isnan().all())
 
 
+@pytest.mark.parametrize("dt,rank,new", [("bf16", 256, 3), ("bf16", 256, 150), ("fp32", 64, 3)])
+def test_attention_under_the_largest_and_smallest_scales(dt, rank, new):
+    """Scores of zero at 1e35, and a scale that leaves no differences: the mean of the values that a token sees."""
+    for scale in (1e35, 1e-38):
+        c = _case([200, 170], [new, new], 4, rank, 64, 64, 64, 16, dt, seed=22)
+        if scale > 1:
+            c["q"] = torch.zeros_like(c["q"])
+        c["scale"] = scale
+        _near(_attend(c), c, str(scale))
+    with pytest.raises(RuntimeError, match="1e35"):
+        _attend(dict(c, scale=2e35))
+
+
 @pytest.mark.parametrize("new", [1, 6, 64])
 @pytest.mark.parametrize("middle", [1, 333])
 def test_attention_in_streams_and_graphs(new, middle):

@@ -57,6 +57,13 @@ def test_paged_attention_argument_errors_are_codes():
     assert L.ethos_paged_attention_workspace_bytes(-3, 2, 16, 256, 64, 64, 64, 4, 64, 1) == 256
 
 
+def test_paged_attention_refuses_scales_beyond_its_arithmetic():
+    L = _lib.load()
+    for scale, code in ((3e38, -2), (1e36, -2), (1.01e35, -2), (1e35, -5), (1e-38, -5)):  # (-5: past the scale, to the workspace)
+        assert L.ethos_paged_attention(16, 16, 16, 16, 4, 4, 16, 16, 16, 3, 2, 16, 256, 64, 64, 64, 9, 64, 1, scale, 16, 0, 16, None) == code, scale
+    assert b"1e35" not in L.ethos_last_error()
+
+
 def test_copy_pages_argument_errors_are_codes():
     L = _lib.load()
     arr = lambda *v: (ctypes.c_int32 * len(v))(*v)  # noqa: E731
