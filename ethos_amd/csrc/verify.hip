@@ -18,6 +18,7 @@ constexpr int kPiece = 8;               // values of a thread that follow each o
 constexpr int kSpan = 256 * kPiece;     // of a workgroup
 constexpr int kDraftsMax = 255;
 constexpr int kPartsMax = 1024;
+constexpr int64_t kLaunchGroups = (int64_t)1 << 23;  // workgroups of a launch, whose threads have to stay below 2^32
 
 // Of a chunk of a row: its maximum, where that is first, and the sum of exp2((l - max) rate); NaN if any value is
 // NaN, or +inf (unless greedy).
@@ -87,7 +88,8 @@ struct Args {
     const float *u_accept, *u_sample;
     int m;  // drafts of a sequence, at most
     int64_t vocab;
-    double rate;  // log2 e / temperature; 0: greedy
+    int64_t first;  // the row or sequence that a launch begins with
+    double rate;    // log2 e / temperature; 0: greedy
     int chunks;   // of a row, for its sums
     int parts;    // of the row that a token is drawn from
     int part_pieces;
@@ -105,7 +107,7 @@ __device__ __forceinline__ int draft_count(const Args& a, int64_t i) {
     return n < 0 ? 0 : n > a.m ? a.m : n;
 }
 
-// Chunk blockIdx.x % chunks of row blockIdx.x / chunks.  320 rows of 100,277 bf16 words: 64 MB in 28.5 us, 2.3 TB/s, bound by the
+// Chunk blockIdx.x % chunks of a launch's row blockIdx.x / chunks.  320 rows of 100,277 bf16 words: 64 MB in 28.5 us, 2.3 TB/s, bound by the
 // exponentials' instructions.
 template <typename T, int PC, bool GREEDY>
 __global__ __launch_bounds__(256) void chunk_kernel(Args a) {
@@ -114,7 +116,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(Args a) {
     __shared__ int32_t ats[4];
     __shared__ double ss[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row = blockIdx.x / a.chunks;
+    const int64_t row = a.first + blockIdx.x / a.chunks;
     const int s = blockIdx.x % a.chunks;
     const int64_t i = row / (a.m + 1);
     const int j = (int)(row - i * (a.m + 1));
@@ -249,7 +251,7 @@ __device__ __forceinline__ int decide(const Args& a, int64_t i, int n, double* t
 template <typename T, typename Q>
 __global__ __launch_bounds__(256) void decide_kernel(Args a) {
     __shared__ double table[32];
-    const int64_t i = blockIdx.x;
+    const int64_t i = a.first + blockIdx.x;
     Chunk k;
     const int took = decide<T, Q>(a, i, draft_count(a, i), table, k);
     if (threadIdx.x == 0) {
@@ -390,13 +392,13 @@ __device__ __forceinline__ int64_t find_token(const Args& a, const double* table
     return (int64_t)chosen * PC * kSpan + (low != INT32_MAX ? low : high);
 }
 
-// Part blockIdx.x % parts of sequence blockIdx.x / parts: the part's sum of weights.  64 rows of 100,277 words, bf16 logits and
+// Part blockIdx.x % parts of a launch's sequence blockIdx.x / parts: the part's sum of weights.  64 rows of 100,277 words, bf16 logits and
 // float32 probabilities: 38 MB in 11.5 us, 3.3 TB/s, by loads and exponentials in turn.
 template <typename T, typename Q, int PC>
 __global__ __launch_bounds__(256) void part_kernel(Args a) {
     __shared__ double table[32], ss[4];
     const int tid = threadIdx.x;
-    const int64_t i = blockIdx.x / a.parts;
+    const int64_t i = a.first + blockIdx.x / a.parts;
     const int s = blockIdx.x % a.parts;
     const Chunk k = a.rows[i];
     if (k.sum != k.sum) return;
@@ -406,12 +408,12 @@ __global__ __launch_bounds__(256) void part_kernel(Args a) {
     if (tid == 0) a.weights[i * a.parts + s] = sum;
 }
 
-// The token of sequence blockIdx.x from its parts' sums.
+// The token of a launch's sequence blockIdx.x from its parts' sums.
 template <typename T, typename Q, int PC>
 __global__ __launch_bounds__(256) void token_kernel(Args a) {
     __shared__ double table[32], sums[kPartsMax], ss[4];
     const int tid = threadIdx.x;
-    const int64_t i = blockIdx.x;
+    const int64_t i = a.first + blockIdx.x;
     const Chunk k = a.rows[i];
     if (k.sum != k.sum) return;
     for (int c = tid; c < a.parts; c += 256) sums[c] = a.weights[i * a.parts + c];
@@ -459,28 +461,36 @@ int part_pieces(int64_t vocab) { return vocab <= (int64_t)kPartsMax * kSpan ? 1 
 int pieces_in(int64_t vocab, int pieces) { return (int)((vocab + (int64_t)pieces * kSpan - 1) / ((int64_t)pieces * kSpan)); }
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// `each` workgroups for each of n rows or sequences, in as many launches as that takes.
+template <typename K>
+void launch(K kernel, Args a, int64_t n, int each, hipStream_t stream) {
+    const int64_t most = kLaunchGroups / each;
+    for (a.first = 0; a.first < n; a.first += most) {
+        const int64_t here = n - a.first < most ? n - a.first : most;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(here * each)), dim3(256), 0, stream, a);
+    }
+}
+
 template <typename T, typename Q>
 void launch_draw(const Args& a, int64_t n_seq, hipStream_t stream) {
-    const dim3 each((unsigned)n_seq), parts((unsigned)(n_seq * a.parts));
-    auto launch = [&](auto kernel, dim3 grid) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a); };
-    if (a.rate != 0.0 && a.part_pieces == 1 && n_seq * a.parts <= a.own_parts) return launch(draw_kernel<T, Q>, parts);
-    launch(decide_kernel<T, Q>, each);
+    if (a.rate != 0.0 && a.part_pieces == 1 && n_seq * a.parts <= a.own_parts) return launch(draw_kernel<T, Q>, a, n_seq, a.parts, stream);
+    launch(decide_kernel<T, Q>, a, n_seq, 1, stream);
     if (a.rate == 0.0) return;
     if (a.part_pieces == 1) {
-        launch(part_kernel<T, Q, 1>, parts);
-        launch(token_kernel<T, Q, 1>, each);
+        launch(part_kernel<T, Q, 1>, a, n_seq, a.parts, stream);
+        launch(token_kernel<T, Q, 1>, a, n_seq, 1, stream);
     } else {
-        launch(part_kernel<T, Q, 16>, parts);
-        launch(token_kernel<T, Q, 16>, each);
+        launch(part_kernel<T, Q, 16>, a, n_seq, a.parts, stream);
+        launch(token_kernel<T, Q, 16>, a, n_seq, 1, stream);
     }
 }
 
 template <typename T>
 void launch_all(const Args& a, int64_t n_seq, int probs_dtype, int pieces, hipStream_t stream) {
-    const dim3 grid((unsigned)(n_seq * (a.m + 1) * a.chunks));
-    if (a.rate == 0.0) hipLaunchKernelGGL((chunk_kernel<T, 4, true>), grid, dim3(256), 0, stream, a);
-    else if (pieces == 4) hipLaunchKernelGGL((chunk_kernel<T, 4, false>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((chunk_kernel<T, 1, false>), grid, dim3(256), 0, stream, a);
+    const int64_t rows = n_seq * (a.m + 1);
+    if (a.rate == 0.0) launch(chunk_kernel<T, 4, true>, a, rows, a.chunks, stream);
+    else if (pieces == 4) launch(chunk_kernel<T, 4, false>, a, rows, a.chunks, stream);
+    else launch(chunk_kernel<T, 1, false>, a, rows, a.chunks, stream);
     if (probs_dtype == kBF16) launch_draw<T, uint16_t>(a, n_seq, stream);
     else launch_draw<T, float>(a, n_seq, stream);
 }

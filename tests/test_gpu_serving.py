@@ -733,6 +733,37 @@ def test_verified_tokens_are_distributed_as_the_model_says():
     assert bool(((freq - p).abs() <= 5 * (p * (1 - p) / n).sqrt()).all())
 
 
+def test_verify_of_more_sequences_than_a_launch_has_threads_for():
+    """2^24 sequences and some, a draft for each but a few: over every launch's border, against float64."""
+    n, V, g = (1 << 24) + 5, 8, _gen(8)
+    for m in (0, 1):
+        b = n if m == 0 else n // 2 + 1
+        logits = (torch.randn(b, m + 1, V, generator=g, device="cuda") * 2).to(torch.bfloat16)
+        drafts = torch.randint(0, V, (b, m), generator=g, device="cuda")
+        ua, us = torch.rand(b, m, generator=g, device="cuda"), torch.rand(b, generator=g, device="cuda")
+        accepted, tokens = ethos_amd.verify_drafts(logits, drafts, ua, us)
+        z = logits.double()
+        e = (z - z.amax(-1, keepdim=True)).exp()
+        p = e / e.sum(-1, keepdim=True)
+        del z, e
+        took = torch.zeros(b, dtype=torch.int64, device="cuda")
+        if m:
+            took = (ua[:, 0].double() < p[:, 0].gather(1, drafts)[:, 0]).long()
+        left = p.gather(1, took[:, None, None].expand(b, 1, V))[:, 0]
+        if m:
+            left.scatter_(1, drafts, torch.where(took[:, None] > 0, left.gather(1, drafts), 0.0))
+        up = left.cumsum(1)
+        del p, left
+        above = us.double()[:, None] * up[:, -1:]
+        want = (up <= above).sum(1)
+        # (where a sum is within float64's rounding of the random number's place, either word is right)
+        sure = ~((up - above).abs() < 1e-12).any(1)
+        assert torch.equal(accepted.long(), took) and torch.equal(tokens[sure], want[sure]) and int((~sure).sum()) < 100
+        if m == 0:
+            greedy = ethos_amd.verify_drafts(logits, drafts, ua, us, temperature=0.0)[1]
+            assert torch.equal(greedy, (logits[:, 0] == logits[:, 0].amax(-1, keepdim=True)).int().argmax(-1))
+
+
 def test_verify_in_graphs_and_streams():
     cases = [_verify_case(9, 4, 30011, "bf16", "fp32", seed=s) for s in (4, 5)]
     want = [ethos_amd.verify_drafts(lo, d, ua, us, draft_probs=p) for lo, d, ua, us, p in cases]
