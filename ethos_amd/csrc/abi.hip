@@ -1209,10 +1209,15 @@ int ethos_copy_pages(void* pool, int64_t n_blocks, int64_t block_bytes, int64_t 
 
 namespace {
 
+constexpr int64_t kPagedRowsMax = ((int64_t)1 << 27) - 2048;
+
 int paged_sizes(int64_t n_rows, int32_t n_heads, int32_t nope, int32_t v_dim, const char* what) {
     if (n_heads <= 0 || n_heads > 1024 || nope < 0 || v_dim <= 0 || nope > 4096 || v_dim > 4096)
         return fail(ETHOS_ESIZE, "%s: bad sizes n_heads=%d nope=%d v_dim=%d", what, n_heads, nope, v_dim);
-    if (n_rows * n_heads > INT32_MAX / 4) return fail(ETHOS_ESIZE, "%s: too many rows", what);
+    // (each form's launches of up to n_rows n_heads / 8 workgroups and one have fewer than 2^32 threads; workspaces reach the card's
+    // memory before, but for small ranks)
+    if (n_rows * n_heads > kPagedRowsMax)
+        return fail(ETHOS_ESIZE, "%s: at most %lld rows of all heads, got %lld", what, (long long)kPagedRowsMax, (long long)(n_rows * n_heads));
     return 0;
 }
 

@@ -467,17 +467,17 @@ __device__ __forceinline__ Parts row_parts(const Shape& s, const Plan* plan, con
 // token sees nothing.
 __device__ __forceinline__ float inverse(float l, bool blind) { return l != 0.0f ? 1.0f / l : blind ? 0.0f : NAN; }
 
-// A workgroup a (token, head): joins its row's parts, four columns a thread and as many parts side by side as there are
+// A workgroup a (token, head), from row t0 of the batch on: joins its row's parts, four columns a thread and as many parts side by side as there are
 // threads for, and multiplies with W_v,h, 16 threads a column.
 template <typename T>
-__global__ __launch_bounds__(256) void any_finish_kernel(const T* __restrict__ w, Shape s, const Plan* plan,
+__global__ __launch_bounds__(256) void any_finish_kernel(const T* __restrict__ w, int64_t t0, Shape s, const Plan* plan,
                                                          const Item* __restrict__ items, const int32_t* __restrict__ seq_item,
                                                          const Token* __restrict__ tokens, const float* __restrict__ sums,
                                                          const float2* __restrict__ stats, T* __restrict__ out) {
     __shared__ __align__(16) float part[1024], o[kAnyRank];
     __shared__ float tops[256], ls[256];
-    const int64_t t = blockIdx.x / s.H;
-    const int h = (int)(blockIdx.x - t * s.H), tid = threadIdx.x;
+    const int64_t t = t0 + blockIdx.x / s.H;
+    const int h = blockIdx.x % s.H, tid = threadIdx.x;
     const Token token = tokens[t];
     if (token.seq == kNoSeq) return;  // behind the last sequence
     const int cols = s.rank / 4, groups = 256 / cols, grp = tid / cols, col = (tid - grp * cols) * 4;
@@ -565,8 +565,11 @@ int launch_any(const T* q, const T* w, const T* pool, const Batch& b, const floa
     else if (s.rank <= 128) attend(any_attend_kernel<T, 2>);
     else if (s.rank <= 256) attend(any_attend_kernel<T, 4>);
     else attend(any_attend_kernel<T, 8>);
-    hipLaunchKernelGGL((any_finish_kernel<T>), dim3((unsigned)(b.n_rows * s.H)), dim3(256), 0, stream, w, s, plan, items, seq_item, tokens, sums,
-                       stats, out);
+    // (a launch's threads have to stay below 2^32; the other kernels' do with as many rows as a call may have)
+    const int64_t most = ((int64_t)1 << 23) / s.H;
+    for (int64_t t0 = 0; t0 < b.n_rows; t0 += most)
+        hipLaunchKernelGGL((any_finish_kernel<T>), dim3((unsigned)((b.n_rows - t0 < most ? b.n_rows - t0 : most) * s.H)), dim3(256), 0, stream, w,
+                           t0, s, plan, items, seq_item, tokens, sums, stats, out);
     return (int)hipGetLastError();
 }
 

@@ -630,7 +630,7 @@ int ethos_latent_append(const void* rows, int64_t ld, const void* gain, const fl
  * gives NaN, or no weight to its position where the score is -inf (scores times `scale` under -2^125 count as -inf); a token
  * all of whose scores are -inf has NaN.
  *   workspace  >= ethos_paged_attention_workspace_bytes(...) bytes (scratch)
- * q, w, pool, workspace and out 16-byte aligned; scale positive, at most 1e35.
+ * q, w, pool, workspace and out 16-byte aligned; scale positive, at most 1e35; n_rows n_heads <= 2^27 - 2048.
  */
 size_t ethos_paged_attention_workspace_bytes(int64_t n_rows, int32_t n_seq, int32_t n_heads, int32_t rank, int32_t rope, int32_t nope,
                                              int32_t v_dim, int32_t table_width, int32_t page, int32_t dtype);

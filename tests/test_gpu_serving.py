@@ -532,6 +532,30 @@ def test_attention_in_streams_and_graphs(new, middle):
         assert torch.equal(out if k % 3 else out2, w) and torch.equal(eager, w), k
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_attention_of_more_rows_than_a_launch_has_threads_for(dt):
+    """16,385 tokens of 1,024 heads: 2^24 rows and some."""
+    n, H, g, T = 16385, 1024, _gen(23), DT[dt]
+    pool = torch.randn(2, 4, 8, generator=g, device="cuda").to(T)
+    w = torch.randn(H * 2, 8, generator=g, device="cuda").to(T) / 3
+    q = torch.randn(n, H, 1, generator=g, device="cuda").to(T)
+    lens = torch.randint(1, 9, (n,), generator=g, device="cuda").to(torch.int32)
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda").repeat(n, 1)
+    got = ethos_amd.paged_attention(q, w, pool, table, lens, torch.arange(n + 1, dtype=torch.int32, device="cuda"), _rates(0), 0.7)
+    rows = pool.view(8, 8).double()
+    k, v = rows @ w.double().view(H, 2, 8)[:, 0].T, rows @ w.double().view(H, 2, 8)[:, 1].T  # [8, H]
+    size = rows.abs() @ w.double().abs().view(H, 2, 8)[:, 0].T
+    for t0 in range(0, n, 4096):
+        a = q[t0:t0 + 4096, :, 0].double()
+        seen = torch.arange(8, device="cuda")[None, :, None] < lens[t0:t0 + 4096, None, None]
+        s = (a[:, None, :] * k * 0.7).masked_fill(~seen, -math.inf)  # [., 8, H]
+        want = (torch.softmax(s, 1) * v).sum(1)
+        # float32 throughout: a score's terms are each off by some roundings, so is each weighted value's sum
+        e = (a.abs()[:, None, :] * size * 0.7).amax(1) * 32 * U
+        bound = (2 * e + 64 * U) * (rows.abs() @ w.double().abs().view(H, 2, 8)[:, 1].T).amax(0) + half_step(T) * want.abs() * 1.01
+        _within(got[t0:t0 + 4096], want, bound, f"rows from {t0}")
+
+
 # ------------------------------------------------------------------------------- pages
 @pytest.mark.parametrize("dt", ["bf16", "fp32"])
 @pytest.mark.parametrize("blocks,pages,page,width,pairs", [(1, 2, 1, 1, 1), (3, 40, 16, 320, 20), (2, 2000, 2, 24, 1000), (12, 9, 64, 320, 4),

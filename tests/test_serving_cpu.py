@@ -57,6 +57,12 @@ def test_paged_attention_argument_errors_are_codes():
     assert L.ethos_paged_attention_workspace_bytes(-3, 2, 16, 256, 64, 64, 64, 4, 64, 1) == 256
 
 
+def test_paged_attention_refuses_more_rows_than_its_launches_take():
+    L = _lib.load()
+    for n, H, code in (((1 << 27) - 2047, 1, -2), ((1 << 23), 16, -2), ((1 << 27) - 2048, 1, -5), ((1 << 23) - 128, 16, -5), ((1 << 17) - 2, 1024, -5)):
+        assert L.ethos_paged_attention(16, 16, 16, 16, 4, 4, 16, 16, 16, n, 2, H, 256, 64, 64, 64, 9, 64, 1, 0.1, 16, 0, 16, None) == code, (n, H)
+
+
 def test_paged_attention_refuses_scales_beyond_its_arithmetic():
     L = _lib.load()
     for scale, code in ((3e38, -2), (1e36, -2), (1.01e35, -2), (1e35, -5), (1e-38, -5)):  # (-5: past the scale, to the workspace)
