@@ -9,18 +9,18 @@
 namespace ethos {
 namespace {
 
-// One wave a row: the latent times 1 / sqrt(mean of its squares + eps) and the gain, the key's halves
+// One wave a row, from row0 of the batch on: the latent times 1 / sqrt(mean of its squares + eps) and the gain, the key's halves
 // [a, b] -> [a cos - b sin, b cos + a sin]; both in float32, rounded once.  One pass: a piece of
 // 16 bytes of the latent a lane in registers, and half a wave's lanes a pair of the key each.  8,192 rows of 640 bytes: 7.2 us,
 // 1.5 TB/s; 64 rows 3.6: bound by the search for a row's sequence, its page and the angle, one after the other, not by memory.
 template <typename T, int CH>
 __global__ __launch_bounds__(256) void append_kernel(const T* __restrict__ rows, int64_t ld, const T* __restrict__ gain,
-                                                     const float* __restrict__ rates, Batch b, int rank, int rope, float eps,
-                                                     T* __restrict__ pool) {
+                                                     const float* __restrict__ rates, Batch b, int64_t row0, int rank, int rope,
+                                                     float eps, T* __restrict__ pool) {
     constexpr int N = Vec16<T>::kN;
     typedef typename Vec16<T>::raw Raw;
     const int lane = threadIdx.x & 63;
-    const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t r = row0 + (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (r >= b.n_rows) return;
     const T* x = rows + r * ld;
     Raw xr[CH], gr[CH];
@@ -88,13 +88,17 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(unsigned char* pool, in
 
 int launch_latent_append(const void* rows, int64_t ld, const void* gain, const float* rates, const Batch& b, int rank, int rope, float eps,
                          int dtype, void* pool, hipStream_t stream) {
-    const dim3 grid((unsigned)((b.n_rows + 3) / 4));
-    if (dtype == kBF16)
-        hipLaunchKernelGGL((append_kernel<uint16_t, 1>), grid, dim3(256), 0, stream, (const uint16_t*)rows, ld, (const uint16_t*)gain, rates,
-                           b, rank, rope, eps, (uint16_t*)pool);
-    else
-        hipLaunchKernelGGL((append_kernel<float, 2>), grid, dim3(256), 0, stream, (const float*)rows, ld, (const float*)gain, rates, b, rank,
-                           rope, eps, (float*)pool);
+    constexpr int64_t kLaunchRows = (int64_t)1 << 25;  // (a launch's threads have to stay below 2^32)
+    for (int64_t row0 = 0; row0 < b.n_rows; row0 += kLaunchRows) {
+        const int64_t n = b.n_rows - row0 < kLaunchRows ? b.n_rows - row0 : kLaunchRows;
+        const dim3 grid((unsigned)((n + 3) / 4));
+        if (dtype == kBF16)
+            hipLaunchKernelGGL((append_kernel<uint16_t, 1>), grid, dim3(256), 0, stream, (const uint16_t*)rows, ld, (const uint16_t*)gain,
+                               rates, b, row0, rank, rope, eps, (uint16_t*)pool);
+        else
+            hipLaunchKernelGGL((append_kernel<float, 2>), grid, dim3(256), 0, stream, (const float*)rows, ld, (const float*)gain, rates, b,
+                               row0, rank, rope, eps, (float*)pool);
+    }
     return (int)hipGetLastError();
 }
 

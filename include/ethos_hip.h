@@ -604,7 +604,7 @@ int ethos_clip_grads(const void* const* in, void* const* out, const int64_t* siz
  *           tokens, the last ones of its lens[i]; rows of no sequence (behind the last one) are left as they are
  * What table, lens and starts hold cannot make a kernel leave the arrays: a page outside [0, n_pages), or a position
  * without one, is neither written nor read.
- * Limits: page a power of two up to 65536; rank <= 512 and rope <= 128, multiples of 8 (bf16) or 4; n_seq <= 2^20.
+ * Limits: page a power of two up to 65536; rank <= 512 and rope <= 128, multiples of 8 (bf16) or 4; n_seq <= 2^20; n_rows < 2^29.
  *
  * ethos_latent_append writes the new tokens' rows (model.py:104-125 before the heads' projections): of the
  * batch's rows [latent | key] (ld apart), y = RN_T(gain x / sqrt(mean(x^2) + eps)) of the latent and, of the key's halves

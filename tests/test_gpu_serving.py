@@ -123,6 +123,24 @@ def test_append_leaves_out_what_has_no_place():
     assert float(pool.abs().sum()) == 0.0
 
 
+def test_append_of_more_rows_than_a_launch_has_threads_for():
+    """2^26 rows and some, of two sequences."""
+    n, page, first, g = (1 << 26) + 7, 65536, (1 << 25) + 12345, _gen(24)
+    rows = (torch.randn(n, 8, generator=g, device="cuda") * 2).to(torch.bfloat16)
+    gain = (1 + 0.2 * torch.randn(8, generator=g, device="cuda")).to(torch.bfloat16)
+    width = -(-(n - first) // page) + 1
+    table = torch.randperm(2 * width, generator=g, device="cuda").to(torch.int32).view(2, width)
+    pool = torch.full((2 * width, page, 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    ethos_amd.latent_append(rows, gain, pool, table, i32([first, n - first]), i32([0, first, n]), _rates(0), eps=1e-6)
+    for i, (a, z) in enumerate(((0, first), (first, n))):
+        whole = pool[table[i].long()].view(-1, 8)  # the sequence's rows in order
+        for r0 in range(a, z, 1 << 24):
+            x = rows[r0:min(z, r0 + (1 << 24))].double()
+            want = x * torch.rsqrt(x.square().mean(1, keepdim=True) + 1e-6) * gain.double()
+            _within(whole[r0 - a:r0 - a + len(x)], want, want.abs() * (24 * U + half_step(torch.bfloat16) * 1.01), f"rows from {r0}")
+        assert bool((whole[z - a:] == 7.0).all())
+
+
 # ------------------------------------------------------------------------------- attention
 def _case(lens, new, H, rank, rope, nope, v, page, dt, seed=0, extra=3, size=1.5):
     g, T = _gen(seed), DT[dt]
