@@ -183,7 +183,7 @@ class LatentCache:
             raise TypeError(f"LatentCache: dtype must be bfloat16 or float32, got {dtype}")
         self.page, self.rank, self.rope = page, rank, rope
         # (never-written memory is never read, but a NaN in it would be by a caller's own sums over pages)
-        self.pool = torch.zeros((blocks, pages, page, rank + rope), dtype=dtype, device=device or "cuda")
+        self.pool = torch.zeros((blocks, pages, page, rank + rope), dtype=dtype, device="cuda" if device is None else device)
         self._users = [0] * pages                       # sequences that have the page
         self._free = array("i", range(pages - 1, -1, -1))  # the lowest is given out first
         self._sequences: dict[int, _Sequence] = {}

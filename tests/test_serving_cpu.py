@@ -152,6 +152,20 @@ def _consistent(c):
     assert sorted(c._free) == [p for p, n in enumerate(users) if n == 0]
 
 
+def test_cache_is_made_on_the_device_it_is_given(monkeypatch):
+    """A device's number too, zero among them."""
+    asked = []
+
+    def zeros(shape, dtype, device):
+        asked.append(device)
+        return torch.empty(shape, dtype=dtype)
+
+    monkeypatch.setattr(serving.torch, "zeros", zeros)
+    for device in (None, 0, 1, "cpu", torch.device("cuda", 0)):
+        serving.LatentCache(1, 8, 8, 2, 4, torch.float32, device)
+    assert asked == ["cuda", 0, 1, "cpu", torch.device("cuda", 0)]
+
+
 def test_cache_keeps_every_sequence_its_tokens(monkeypatch):
     c = _book(monkeypatch)
     a, b = c.new(), c.new()
