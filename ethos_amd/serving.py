@@ -100,12 +100,23 @@ def paged_attention(q: torch.Tensor, weight: torch.Tensor, pool: torch.Tensor, t
     return o
 
 
-def _page_list(name: str, v) -> list:
+def _page_list(name: str, v) -> array:
     if isinstance(v, torch.Tensor):
         if v.is_cuda:
             raise TypeError(f"copy_pages: {name} must be on the host (a list, or a CPU tensor)")
-        return v.tolist()
-    return v if isinstance(v, list) else list(v)
+        v = v.tolist()
+    return array("i", v if isinstance(v, list) else list(v))
+
+
+def _page_pairs(src, dst) -> tuple[array, array]:
+    """Which pages are copied where, checked (as plain numbers: tensors of one value would be told apart by what they are)."""
+    src, dst = _page_list("src", src), _page_list("dst", dst)
+    if len(src) != len(dst):
+        raise ValueError(f"copy_pages: {len(src)} pages to copy but {len(dst)} places")
+    to = set(dst)
+    if len(to) != len(dst) or not to.isdisjoint(src):
+        raise ValueError("copy_pages: a page is written twice, or both read and written")
+    return src, dst
 
 
 def copy_pages(pool: torch.Tensor, src, dst) -> None:
@@ -116,13 +127,7 @@ def copy_pages(pool: torch.Tensor, src, dst) -> None:
     if pool.dim() < 3 or not pool.is_contiguous() or pool.element_size() not in (2, 4):
         raise RuntimeError(f"copy_pages: pool must be contiguous [blocks, pages, ...] of 2 or 4 bytes a value, got {tuple(pool.shape)} "
                            f"{pool.dtype}")
-    src, dst = _page_list("src", src), _page_list("dst", dst)
-    if len(src) != len(dst):
-        raise ValueError(f"copy_pages: {len(src)} pages to copy but {len(dst)} places")
-    to = set(dst)
-    if len(to) != len(dst) or not to.isdisjoint(src):
-        raise ValueError("copy_pages: a page is written twice, or both read and written")
-    hip.copy_pages(pool, src, dst)
+    hip.copy_pages(pool, *_page_pairs(src, dst))
     _written(pool)
 
 

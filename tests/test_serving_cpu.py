@@ -84,6 +84,22 @@ def test_copy_pages_argument_errors_are_codes():
     assert L.ethos_copy_pages(16, 2, 4096, 4, 1024, None, None, 1, None) == -3
 
 
+def test_copy_pages_tells_the_same_page_by_its_number(monkeypatch):
+    """Whatever kind of number it comes as."""
+    numpy = pytest.importorskip("numpy")
+    pairs = []
+    monkeypatch.setattr(serving, "_check", lambda *a: None)
+    monkeypatch.setattr(serving.hip, "copy_pages", lambda pool, src, dst: pairs.append((list(src), list(dst))))
+    pool = torch.zeros(1, 9, 2)
+    t = torch.tensor
+    for src, dst in (([0, 1], [t(5), t(5)]), ([t(3)], [t(3)]), ([0, 1], [numpy.int64(5), t(5)]), ([3], [t(3)]), (t([1, 2]), [t(4), t(1)])):
+        with pytest.raises(ValueError, match="twice"):
+            ethos_amd.copy_pages(pool, src, dst)
+    ethos_amd.copy_pages(pool, [t(0), numpy.int32(1)], (p for p in (t(5), 6)))
+    ethos_amd.copy_pages(pool, numpy.array([2]), t([3], dtype=torch.int32))
+    assert pairs == [([0, 1], [5, 6]), ([2], [3])]
+
+
 def test_verify_argument_errors_are_codes():
     L = _lib.load()
 
