@@ -907,9 +907,11 @@ def paged_attention(q: torch.Tensor, w: torch.Tensor, pool: torch.Tensor, table:
 def copy_pages(pool: torch.Tensor, src: list, dst: list) -> None:
     """Copies pages src[i] to dst[i] in every block of pool [blocks, pages, ...]."""
     a, b = array.array("i", src), array.array("i", dst)
-    if not src or pool.numel() == 0:
-        return
     pages = pool.shape[1]
+    if not src or pool.numel() == 0:
+        if not all(0 <= p < pages for p in a + b):
+            raise IndexError(f"copy_pages: a page is outside the {pages} pages")
+        return
     page_bytes = pool.numel() // (pool.shape[0] * pages) * pool.element_size()
     rc = load().ethos_copy_pages(pool.data_ptr(), pool.shape[0], pages * page_bytes, pages, page_bytes, a.buffer_info()[0], b.buffer_info()[0],
                                  len(a), _stream())

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import ethos_amd
-from ethos_amd import _lib, serving
+from ethos_amd import _lib, hip, serving
 
 BIG = 1 << 60
 
@@ -98,6 +98,17 @@ def test_copy_pages_tells_the_same_page_by_its_number(monkeypatch):
     ethos_amd.copy_pages(pool, [t(0), numpy.int32(1)], (p for p in (t(5), 6)))
     ethos_amd.copy_pages(pool, numpy.array([2]), t([3], dtype=torch.int32))
     assert pairs == [([0, 1], [5, 6]), ([2], [3])]
+
+
+def test_copy_pages_of_an_empty_pool_checks_the_pages():
+    for shape in ((0, 5, 4, 8), (2, 5, 0, 8), (2, 5, 4, 0)):
+        hip.copy_pages(torch.zeros(shape), [0, 3], [1, 4])
+        hip.copy_pages(torch.zeros(shape), [], [])
+        for src, dst in (([5], [1]), ([1], [5]), ([-1], [2]), ([2], [-1])):
+            with pytest.raises(IndexError):
+                hip.copy_pages(torch.zeros(shape), src, dst)
+    with pytest.raises(IndexError):
+        hip.copy_pages(torch.zeros(2, 0, 4, 8), [0], [1])
 
 
 def test_verify_argument_errors_are_codes():
