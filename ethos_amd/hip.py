@@ -908,6 +908,8 @@ def copy_pages(pool: torch.Tensor, src: list, dst: list) -> None:
     """Copies pages src[i] to dst[i] in every block of pool [blocks, pages, ...]."""
     a, b = array.array("i", src), array.array("i", dst)
     pages = pool.shape[1]
+    if pool.shape[0] > 65535:
+        raise RuntimeError(f"copy_pages: a pool may have 65,535 blocks, got {pool.shape[0]}")
     if not src or pool.numel() == 0:
         if not all(0 <= p < pages for p in a + b):
             raise IndexError(f"copy_pages: a page is outside the {pages} pages")

@@ -120,8 +120,8 @@ def _page_pairs(src, dst) -> tuple[array, array]:
 
 
 def copy_pages(pool: torch.Tensor, src, dst) -> None:
-    """Copies page src[i] to page dst[i], for every i, in all blocks of pool [blocks, pages, ...] (contiguous, any dtype of
-    two or four bytes).  src and dst: sequences of whole numbers on the host, read during the call; no page may be written
+    """Copies page src[i] to page dst[i], for every i, in all blocks (65,535 at most) of pool [blocks, pages, ...] (contiguous,
+    any dtype of two or four bytes).  src and dst: sequences of whole numbers on the host, read during the call; no page may be written
     twice or both read and written."""
     _check("copy_pages", pool)
     if pool.dim() < 3 or not pool.is_contiguous() or pool.element_size() not in (2, 4):

@@ -642,7 +642,7 @@ int ethos_paged_attention(const void* q, const void* w, const void* pool, const 
 /*
  * Copies pages: of each of n_blocks arrays of n_pages pages, block_bytes apart, page src[i] to page dst[i].
  * src and dst: host arrays, read during the call only; every page inside the pool, no page twice in dst, none of dst
- * in src.  pool, page_bytes and block_bytes even; fastest as multiples of 16.
+ * in src.  pool, page_bytes and block_bytes even; fastest as multiples of 16.  n_blocks <= 65535.
  */
 int ethos_copy_pages(void* pool, int64_t n_blocks, int64_t block_bytes, int64_t n_pages, int64_t page_bytes, const int32_t* src,
                      const int32_t* dst, int32_t n_pairs, void* stream);

@@ -111,6 +111,12 @@ def test_copy_pages_of_an_empty_pool_checks_the_pages():
         hip.copy_pages(torch.zeros(2, 0, 4, 8), [0], [1])
 
 
+def test_copy_pages_names_too_many_blocks():
+    """Not as pages outside the pool."""
+    with pytest.raises(RuntimeError, match="65,535 blocks"):
+        hip.copy_pages(torch.zeros(65536, 2, 1), [0], [1])
+
+
 def test_verify_argument_errors_are_codes():
     L = _lib.load()
 
