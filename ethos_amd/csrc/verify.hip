@@ -277,7 +277,7 @@ __device__ __forceinline__ Draw<T, Q> draw_of(const Args& a, int64_t i, int n, i
                       !a.probs && took < n ? a.drafts[i * a.m + took] : -1, exp_from(k.max, a.rate), 1.0 / k.sum};
 }
 
-// The weights at 8 places of the row; p alone where there is no q.
+// The weights at 8 places of the row; p alone where there is no q, NaN among them where q has one.
 template <typename T, typename Q>
 __device__ __forceinline__ void weights8(const Args& a, const double* table, const Draw<T, Q>& d, int64_t e, double* w) {
     float f[kPiece], g[kPiece] = {};
@@ -286,8 +286,12 @@ __device__ __forceinline__ void weights8(const Args& a, const double* table, con
 #pragma unroll
     for (int v = 0; v < kPiece; ++v) {
         const double p = exp_of(d.x, table, f[v]) * d.inv;
-        w[v] = fmax(e + v == d.one ? p - 1.0 : p - (double)g[v], 0.0);
+        w[v] = fmax(e + v == d.one ? p - 1.0 : p - (double)g[v], 0.0);  // (0 of a NaN)
     }
+    bool none = false;
+#pragma unroll
+    for (int v = 0; v < kPiece; ++v) none |= g[v] != g[v];
+    if (none) w[0] = NAN;
 }
 
 // A part's sum of weights, by a workgroup; ss: 4 values.
@@ -303,7 +307,7 @@ __device__ __forceinline__ double part_sum(const Args& a, const double* table, c
     return block_sum_f64(sum, ss, tid);
 }
 
-// The token, from the parts' sums in LDS, by a workgroup.
+// The token, from the parts' sums in LDS, by a workgroup; -1 without a distribution.
 template <int PC, typename T, typename Q>
 __device__ __forceinline__ int64_t find_token(const Args& a, const double* table, Draw<T, Q> d, float u, double* sums, double* ss, int tid) {
     __shared__ int low, high, chosen;
@@ -346,6 +350,7 @@ __device__ __forceinline__ int64_t find_token(const Args& a, const double* table
         __syncthreads();
     };
     find_part();
+    if (rest != rest) return -1;
     if (rest == 0.0) {  // q covers p: drawn from p itself
         d.q = nullptr;
         d.one = -1;

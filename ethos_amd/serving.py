@@ -142,7 +142,8 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u_accept: torch.Te
     before it do and u_accept q_j(x_j) < p_j(x_j).  The token is drawn from max(p_a - q_a, 0) behind the a-th (from p_a if all
     stand, or that is 0 everywhere): the lowest index whose weights up to it exceed u_sample of their sum.  Tokens and drafts
     together are then distributed as p's.  Without drafts (m = 0) it samples.  Words may be masked by logits of -inf.  A
-    token is -1 where its row has a NaN, no finite logit, or one that is +inf (with a temperature).  All in float64."""
+    token is -1 where its row of logits has a NaN, no finite one, or one that is +inf (with a temperature), and where the row of
+    draft_probs that is subtracted (with a temperature) has a NaN.  All in float64."""
     _check("verify_drafts", *[t for t in (logits, drafts, u_accept, u_sample, draft_probs, counts) if t is not None])
     if (logits.dtype not in hip.FLOATS or drafts.dtype != torch.int64 or u_accept.dtype != torch.float32 or u_sample.dtype != torch.float32
             or draft_probs is not None and draft_probs.dtype not in hip.FLOATS or counts is not None and counts.dtype != torch.int32):

@@ -659,8 +659,8 @@ int ethos_copy_pages(void* pool, int64_t n_blocks, int64_t block_bytes, int64_t 
  *   accepted  [n_seq] int32: a, the number of accepted drafts
  *   tokens    [n_seq] int64: the token behind them, the lowest index whose sum of weights up to it exceeds
  *             u_sample times their sum; the weights are p_a where all were accepted, else max(p_a - probs_a, 0)
- *             (where that is 0 everywhere, p_a).  -1 where p_a is no distribution: a NaN, no finite logit, or
- *             (not greedy) one that is +inf.
+ *             (where that is 0 everywhere, p_a).  -1 where p_a is no distribution (a NaN, no finite logit, or,
+ *             not greedy, one that is +inf) and where a probs_a that is subtracted (not greedy) has a NaN.
  * Exponentials and sums are float64.
  *   workspace  >= ethos_verify_workspace_bytes(...) bytes, 16-byte aligned (scratch)
  * Limits: n_drafts <= 255, vocab <= 2^24; temperature 0, or from 1e-6 to 1e6.

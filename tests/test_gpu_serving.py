@@ -709,6 +709,30 @@ def test_verify_of_odd_inputs():
     assert ethos_amd.verify_drafts(logits[:0], drafts[:0], ua[:0], us[:0])[0].shape == (0,)
 
 
+def test_verify_of_draft_probabilities_that_are_nan():
+    """NaN in the row that the token is drawn with: no token.  In other rows it does not show."""
+    V = 5000
+    logits, _, ua, us, p = _verify_case(6, 2, V, "fp32", "fp32", seed=6)
+    drafts = logits[:, :2].argmax(-1)
+    ua.zero_()          # a draft of any weight stands
+    ua[:4, 1] = 3e38    # ... but the second of these is refused
+    good = ethos_amd.verify_drafts(logits, drafts, ua, us, draft_probs=p)
+    assert good[0].tolist() == [1, 1, 1, 1, 2, 2] and bool((good[1] >= 0).all())
+    p = p.clone()
+    p[0, 1, 4999] = math.nan               # the refused draft's row
+    p[1, 1, int(drafts[1, 1])] = math.nan  # ... at the draft itself
+    p[2, 0, (int(drafts[2, 0]) + 1) % V] = math.nan  # the row of one that stands
+    p[4, 1, (int(drafts[4, 1]) + 1) % V] = math.nan
+    p[5, 0, int(drafts[5, 0])] = math.nan  # a draft of no known probability does not stand
+    for many in (1, 90):  # (in one launch, in several)
+        got = ethos_amd.verify_drafts(*[t.repeat(many, *[1] * (t.dim() - 1)) for t in (logits, drafts, ua, us)],
+                                      draft_probs=p.repeat(many, 1, 1))
+        assert got[0].tolist() == [1, 1, 1, 1, 2, 0] * many
+        want = good[1].clone()
+        want[[0, 1, 5]] = -1
+        assert torch.equal(got[1], want.repeat(many))
+
+
 def test_verify_takes_the_first_of_equal_logits():
     logits = torch.zeros(3, 2, 30000, device="cuda")
     logits[1, :, 20000:] = 1.0
