@@ -178,7 +178,8 @@ class LatentCache:
     Which page is whose is known on the host: no call waits for the device.  `extend` makes room for new tokens and
     gives the batch that the operators take; a fork shares its pages, and a shared page is copied when one of its
     sequences first writes in it.  The device's work (page copies, the batch's tensors) is enqueued on the current stream:
-    use a cache on one stream, or let streams wait for each other.  Its calls are not for graph capture."""
+    use a cache on one stream, or let streams wait for each other.  `extend` and `compact` refuse to be captured into a graph,
+    whose replays would read the batch from host memory long used again, and move pages that the books have moved already."""
 
     def __init__(self, blocks: int, rank: int, rope: int, pages: int, page: int = 64, dtype: torch.dtype = torch.bfloat16, device=None):
         if blocks <= 0 or pages <= 0 or rank <= 0 or rope < 0:
@@ -194,6 +195,10 @@ class LatentCache:
         self._free = array("i", range(pages - 1, -1, -1))  # the lowest is given out first
         self._sequences: dict[int, _Sequence] = {}
         self._next = 0
+
+    def _refuse_capture(self, what: str) -> None:
+        if self.pool.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"LatentCache.{what} cannot be captured into a graph")
 
     @property
     def pages_free(self) -> int:
@@ -254,6 +259,7 @@ class LatentCache:
     def extend(self, seqs, counts) -> Batch:
         """Room for counts[i] new tokens of sequence seqs[i]: their batch, in that order.  With too few free pages it raises
         RuntimeError and changes nothing."""
+        self._refuse_capture("extend")
         seqs, counts = list(seqs), [operator.index(c) for c in counts]
         if len(seqs) != len(counts) or len(set(seqs)) != len(seqs) or any(c < 0 for c in counts):
             raise ValueError("extend: each sequence once, with the number of its new tokens")
@@ -313,6 +319,7 @@ class LatentCache:
     def compact(self) -> int:
         """Moves pages so that those in use are the first of the pool (which a caller may then copy into a smaller one);
         their number.  Batches given out before are no longer valid."""
+        self._refuse_capture("compact")
         used = len(self._users) - len(self._free)
         holes = [p for p in range(used) if self._users[p] == 0]
         moved = [p for p in range(used, len(self._users)) if self._users[p] > 0]

@@ -231,6 +231,29 @@ def test_captured_steps_over_a_batch_of_ones_own(kind):
         assert torch.equal(out, want), step
 
 
+def test_cache_refuses_to_be_captured():
+    """A captured batch would be copied from host memory that is used again before the replays."""
+    c = LatentCache(2, 16, 8, 9, 4, torch.float32)
+    s, t = c.new(), c.new()
+    c.extend([s], [3])
+    c.extend([t], [5])
+    c.free(s)  # (so that a page could move)
+
+    def state():
+        return c.length(t), c.pages(t), c.pages_free
+
+    before, x = state(), torch.zeros(4, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        for call in (lambda: c.extend([t], [1]), lambda: c.compact()):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+    assert state() == before
+    graph.replay()
+    assert c.extend([t], [1]).lens.tolist() == [6] and c.compact() == 2 and float(x.sum()) == 4.0
+
+
 def test_ids_outside_the_vocabulary():
     m = _model("fp32")
     ids = _ids(2, 10, seed=7)
