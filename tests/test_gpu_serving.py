@@ -339,6 +339,19 @@ def test_many_new_tokens_against_float64(lens, new, H, page):
     assert torch.equal(_attend(c), got)
 
 
+@pytest.mark.parametrize("dt,rank", [("bf16", 256), ("fp32", 64)])
+@pytest.mark.parametrize("singles,drafts,idle", [(3, 1, 0), (8, 0, 2), (20, 4, 0), (60, 0, 5), (1, 0, 30)])
+def test_chunks_beside_single_tokens_against_float64(singles, drafts, idle, dt, rank):
+    """A chunk of a prompt, a shorter one, single tokens, a few drafted ones and sequences without new tokens in one batch: with 96 and
+    more new tokens a sequence on the average, and with fewer."""
+    new = [1] * singles + [700] + [5] * drafts + [0] * idle + [300]
+    lens = [1 + (i * 613) % 1500 for i in range(singles)] + [1200] + [5 + 77 * i for i in range(drafts)] + [200] * idle + [300]
+    c = _case(lens, new, 4, rank, 64, 64, 64, 32, dt, seed=singles)
+    got = _attend(c)
+    _near(got, c, f"{singles} {drafts} {idle}")
+    assert torch.equal(_attend(c), got)
+
+
 @pytest.mark.parametrize("new", [1, 150])
 @pytest.mark.parametrize("of_rows,of_weight,of_query", [(64.0, 16.0, 1.0), (2.0 ** -6, 2.0 ** -3, 1.0), (1.0, 1.0, 2.0 ** 10), (1.0, 1.0, 2.0 ** -8),
                                                         (2.0 ** -4, 2.0 ** 10, 2.0 ** -4)])
