@@ -458,9 +458,10 @@ __global__ __launch_bounds__(256) void draw_kernel(Args a) {
     if (tid == 0) a.tokens[i] = token;
 }
 
-// Chunks of 8,192 values, which spare sums and maxima of a workgroup; of 2,048 where there are few.  us of a call with 8,192 |
-// 2,048, rows of 100,277: 320 rows 50 | 54, 160 36.5 | 37.0, 80 28.1 | 27.7, 40 24.1 | 22.8, and one row's sums 6.2 | 4.
-int chunk_pieces(int64_t rows, int64_t vocab, int num_cus) { return rows * ((vocab + 4 * kSpan - 1) / (4 * kSpan)) >= 6 * num_cus ? 4 : 1; }
+// Chunks of 8,192 values, which spare sums and maxima of a workgroup and joins of chunks; of 2,048 where there are fewer than
+// CUs.  us with 8,192 | 2,048, rows of 100,277, a call: 320 rows 55.7 | 62.3, 160 37.0 | 39.1, 80 27.4 | 28.5; its kernels' sum:
+// 40 rows 26.2 | 26.5, 20 20.7 | 20.8, 5 17.4 | 17.0, one 15.9 | 13.9.
+int chunk_pieces(int64_t rows, int64_t vocab, int num_cus) { return rows * ((vocab + 4 * kSpan - 1) / (4 * kSpan)) >= num_cus ? 4 : 1; }
 // Parts of 2,048 values, of 32,768 where they would be too many to list.
 int part_pieces(int64_t vocab) { return vocab <= (int64_t)kPartsMax * kSpan ? 1 : 16; }
 int pieces_in(int64_t vocab, int pieces) { return (int)((vocab + (int64_t)pieces * kSpan - 1) / ((int64_t)pieces * kSpan)); }
@@ -527,8 +528,8 @@ int launch_verify(const void* logits, const int64_t* drafts, const void* probs, 
     a.chunks = pieces_in(vocab, pieces);
     a.part_pieces = part_pieces(vocab);
     a.parts = pieces_in(vocab, a.part_pieces);
-    // us with the decision by itself | in every part's workgroup, four drafts of rows of 100,277: 1 sequence (49 parts) 26.4 | 20.5,
-    // 8 26.3 | 24.1, 16 28.1 | 34.1, 64 50 | 124.
+    // us with the decision by itself | in every part's workgroup, four drafts of rows of 100,277: 1 sequence (49 parts) 24.8 | 20.8,
+    // 4 24.3 | 20.5, 8 24.4 | 25.0, 16 28.5 | 37.8, 64 54 | 125.
     a.own_parts = 2 * num_cus;
     unsigned char* w = (unsigned char*)ws;
     a.stats = (Chunk*)w;
