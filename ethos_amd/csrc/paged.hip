@@ -207,9 +207,10 @@ __device__ __forceinline__ int find_item(const Item* items, int n_items, int64_t
 // which is where O^T = C^T P^T takes them with key 4 g + e in place g of its product e: nothing goes through LDS but the
 // queries, and the waves run by themselves up to the end of a share, where their sums are joined.
 //
-// 512 float32 tokens over 2,048 keys, rank 256, rope 64, 16 heads: 309 us in all, 54 TFLOP/s of 129 that a large float32
-// product reaches (vector instructions over keys in LDS: 5,158).  16 sequences of one token and up to 4,096 keys: 66 us (758).  Five
-// sequences of 33 tokens, rank 32: 19 us, of which 8, 6 and 5 are the three kernels' times: launches and dependent loads.
+// 512 float32 tokens over 2,048 keys, rank 256, rope 64, 16 heads: 301 us in all, 55 TFLOP/s of 132 that a large float32
+// product reaches; what holds it there has not been measured apart (vector instructions over keys in LDS took 5,158).  16 sequences of
+// one token and up to 4,096 keys: 65 us (758).  Five sequences of 33 tokens, rank 32: 19 us, the three kernels' times 5, 8 and 6:
+// launches and dependent loads.
 constexpr int kAnyRows = 16, kAnyKeys = 16, kAnyRank = 512, kAnyRope = 128, kAnyWidth = kAnyRank + kAnyRope;
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
@@ -586,10 +587,11 @@ int launch_any(const T* q, const T* w, const T* pool, const Batch& b, const floa
 // come from rows of zeros, rows without a page from rows of NaN, so that the loop has no bounds to check.
 //
 // The products' operands are bf16.  A value that is rounded for one goes in as two, its bf16 value and the bf16 value of
-// what that leaves (2^-16 of it): the exponentials, the joined sums before W_v, and 128 of a query's 320 columns.  With
-// all rounded once the outputs' error against 64 bits is 1.9 times that of their own rounding, so it is 1.35 times
-// (0.0022 of their norm; of this the queries' other columns are two thirds).  64 sequences of one token: 48.5 -> 49.8 us;
-// 16 of five: 40.5 -> 44.4; all columns of a query in two: 54.0 and 48.7, for 1.1 times.
+// what that leaves (2^-16 of it): the exponentials, the joined sums before W_v, and 128 of a query's 320 columns (columns weigh
+// alike, so any would do: it is the last 64 of the latent's, which one wave forms, and the rotated 64).  With all rounded once the
+// outputs' error against 64 bits is 1.9 times that of their own rounding, so it is 1.35 times (0.0022 of their norm; of this the
+// queries' other columns are two thirds).  64 sequences of one token: 48.5 -> 49.8 us; 16 of five: 40.5 -> 44.4; all columns of a
+// query in two: 54.0 and 48.7, for 1.1 times.
 constexpr int kRank = 256, kRope = 64, kWidth = kRank + kRope;
 constexpr int kRest = 128, kQuery = kWidth + kRest;  // a row's query, and what bf16 leaves of its last kRest columns
 constexpr int kBlockLog = 3, kBlock = 1 << kBlockLog;  // rows of a copy
@@ -764,9 +766,10 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
 }
 
 // WR KW waves: WR share a tile of 16 WR rows, 16 each, KW the 64 keys of a step.  S stages of LDS.  64 sequences of one token and up
-// to 8,192 keys: 186 MB in 35 us, 5.3 TB/s (256 of 2,048: 335 MB in 63), where a large copy moves 4.95: bound by memory.  16 of
-// five tokens and up to 4,096: 23 MB of cache in 24 us, three steps a workgroup, bound by LDS (a fragment serves 16 rows), between
-// reading its queries and writing 80 rows of sums (16 MB).
+// to 8,192 keys: 186 MB in 36.5 us, 5.1 TB/s (256 of 2,048: 335 MB in 62, 5.4), where plain streaming reads reach 5.6, with eight
+// loads of a thread in flight 6.3, and a large copy moves 4.95: near memory's rate.  16 of five tokens and up to 4,096: 23 MB of
+// cache in 24.6 us, three steps a workgroup.  LDS reads (a fragment serves 16 rows) account for some 4 us of that and the products
+// for 5 at most; reading the queries and writing 16 MB of sums lie around the steps; the rest has not been told apart.
 template <int WR, int KW, int S>
 __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
                                                                  const Item* __restrict__ items, const uint16_t* __restrict__ queries,
@@ -1192,15 +1195,20 @@ int launch_fast(const uint16_t* q, const uint16_t* w, const uint16_t* pool, cons
 // is that of their own rounding (with bf16 up to twice that; 120.9 -> 124.6 us for 2,048 tokens, 7,001 keys, 16 heads).  For
 // their range queries and keys are 2^-4 of themselves, values 2^-2, and a row's exponentials 2^6 at its maximum: a query or
 // key of 2^20 or a value of 2^18 and more counts as infinite; fp16's steps near zero are 2^-20 of a key, 2^-22 of a value
-// and 2^-30 of a weight, below bf16's where a key is 2^-11 or more and a value 2^-13.
+// and 2^-30 of a weight, as fine as bf16's where a key is 2^-13 or more and a value 2^-15.
 constexpr float kKeyScale = 0x1p-4f, kValueScale = 0x1p-2f, kQueryScale = 0x1p-4f, kTop = 6.0f;
 constexpr int kHead = 64;         // columns of a head's keys (before the rotated ones) and of its values
 constexpr int kChunkTok = 128;    // tokens of a tile
-// New tokens a sequence, on the average, from which this is the shorter way.  us, the weight with the queries | with the keys and
+// New tokens a sequence, on the average, from which this is the shorter way.  It is measured on sequences that are alike; a batch
+// of others takes one form all the same, and is right in either, but slower than two calls: a chunk of 2,048 tokens over 7,001 keys
+// (129 us by itself) beside 63 single tokens of up to 8,192 keys (53) 489, beside four of 50,000 (41), whose keys are all formed
+// for one token each, 802.  us, the weight with the queries | with the keys and
 // values: 8 sequences of 4,096 keys, 64 tokens 92.5 | 115.0, 96 128.2 | 113.0, 128 158.0 | 115.6; one of 4,096, 64 tokens
 // 43.5 | 48.5, 128 57.4 | 53.5, 256 73.4 | 50.2; one of 16,384, 128 tokens 96.4 | 81.8.
 constexpr int kChunkRows = 96;
-constexpr size_t kChunkBytes = (size_t)1 << 30;  // of keys and values, at most
+// Keys and values that a call may form, by what its table could hold: a limit on the workspace, not where the other form would be
+// shorter.  Four sequences of 512 tokens over 65,000 keys: 1,549 us; over 66,000, beyond it: 3,562.
+constexpr size_t kChunkBytes = (size_t)1 << 30;
 
 struct ChunkLayout {
     size_t plan, items, seq_item, tokens, seq_keys, specials, turns, keys, shared, sums, stats, bytes;
@@ -1420,8 +1428,8 @@ __device__ __forceinline__ void copy16_at(const void* base, uint32_t off, uint32
 }
 
 // A tile's steps for a share of its keys, two workgroups a CU; a wave 32 tokens of its own, S^T = K Q^T and O^T = V^T P^T in
-// 32 x 32 x 16 products, as in attend_kernel.  2,048 tokens over 7,001 keys, 16 heads: 75 GFLOP in 96 to 100 us, 770 TFLOP/s,
-// where a large bf16 product reaches 1,127.  Bound by a step's matrix and vector instructions, which overlap in part: 32 exponentials,
+// 32 x 32 x 16 products, as in attend_kernel.  2,048 tokens over 7,001 keys, 16 heads: 75 GFLOP in 98 us (96.2 at the least),
+// 760 TFLOP/s, where large bf16 products reach 1,127 to 1,405 by the card.  Bound by a step's matrix and vector instructions, which overlap in part: 32 exponentials,
 // their sum, rounding and maximum a lane beside 24 products.
 __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __restrict__ q, const float2* __restrict__ turns,
                                                               const uint16_t* __restrict__ keys, const uint16_t* __restrict__ shared, Shape s,
@@ -1712,7 +1720,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
     }
 }
 
-// 16 (token, head) rows a workgroup, 16 threads each: joins the parts of those that have several (8 us for 32,768 rows: 34 MB
+// 16 (token, head) rows a workgroup, 16 threads each: joins the parts of those that have several (9 us for 32,768 rows: 34 MB
 // of sums).
 __global__ __launch_bounds__(256) void chunk_finish_kernel(int64_t n_rows, Shape s, const Plan* plan, const Item* __restrict__ items,
                                                            const int32_t* __restrict__ seq_item, const Token* __restrict__ tokens,

@@ -31,7 +31,8 @@ struct Chunk {
 // exp2((l - max) rate) for l <= max, in float64: 2^(k / 32 + r), |r| <= 1/64, as a table's 2^(k % 32 / 32), an
 // exponent and the series of 2^r to r^4, whose rest is 1.2e-12.  (The table of 32 doubles is LDS's 64 banks once: lanes
 // read it without conflicts.  With the series alone, to r^11 and over a range of 1, the rows' sums took 36 us where
-// they now take 28: the kernel is bound by its vector instructions, a dozen of float64 a value.)  Below 2^-1020: zero.  NaN stays.
+// the table took 28, and 30 with the difference first: the kernel is bound by its vector instructions, a dozen of float64 a value.)
+// Below 2^-1020: zero.  NaN stays.
 // The difference comes before the scale: it is 0 at the maximum, however far from zero that is, where
 // l rate - RN(max rate) would be the rounding of max rate, an exponent of any size for maxima of 1e16 and more.
 struct Exp {
@@ -107,8 +108,9 @@ __device__ __forceinline__ int draft_count(const Args& a, int64_t i) {
     return n < 0 ? 0 : n > a.m ? a.m : n;
 }
 
-// Chunk blockIdx.x % chunks of a launch's row blockIdx.x / chunks.  320 rows of 100,277 bf16 words: 64 MB in 28.5 us, 2.3 TB/s, bound by the
-// exponentials' instructions.
+// Chunk blockIdx.x % chunks of a launch's row blockIdx.x / chunks.  320 rows of 100,277 bf16 words: 64 MB in 34 us, 1.9 TB/s (269 of
+// them, the others behind their sequences' drafts: 30), bound by the exponentials' instructions; the largest logits of those 269
+// (temperature 0) 16.5.
 template <typename T, int PC, bool GREEDY>
 __global__ __launch_bounds__(256) void chunk_kernel(Args a) {
     __shared__ double table[32];
@@ -398,7 +400,7 @@ __device__ __forceinline__ int64_t find_token(const Args& a, const double* table
 }
 
 // Part blockIdx.x % parts of a launch's sequence blockIdx.x / parts: the part's sum of weights.  64 rows of 100,277 words, bf16 logits and
-// float32 probabilities: 38 MB in 11.5 us, 3.3 TB/s, by loads and exponentials in turn.
+// float32 probabilities: 38 MB in 12 us, 3.2 TB/s, by loads and exponentials in turn.
 template <typename T, typename Q, int PC>
 __global__ __launch_bounds__(256) void part_kernel(Args a) {
     __shared__ double table[32], ss[4];
@@ -429,8 +431,8 @@ __global__ __launch_bounds__(256) void token_kernel(Args a) {
 
 // All three in one launch for few sequences: each workgroup decides by itself which row its part is of, and the
 // sequence's last one to come here finds the token.  (For many, a launch each: a workgroup that says that it is done waits
-// for the caches, some 0.2 us one after the other on an XCD.  64 sequences of 100,277 words: 85 us in one launch, and in three 4.8,
-// 11.6 and 7.2.)
+// for the caches, some 0.2 us one after the other on an XCD.  64 sequences of 100,277 words: 85 us in one launch, and in three 4.7,
+// 12 and 7.3.)
 template <typename T, typename Q>
 __global__ __launch_bounds__(256) void draw_kernel(Args a) {
     __shared__ double table[32], sums[kPartsMax], ss[4];

@@ -82,14 +82,16 @@ def paged_attention(q: torch.Tensor, weight: torch.Tensor, pool: torch.Tensor, t
 
     q [n, heads, nope + rope], the rotary part not yet rotated; weight [heads (nope + v_dim), rank], kv_b_proj's;
     pool, table, lens, starts and rates as latent_append takes them.  A token sees its sequence's positions up to its own:
-    softmax(scale q k) v (scale positive, at most 1e35) over them, with k = [weight's nope rows of the head times the latent | the cached key] and v its
-    v_dim rows times the latent.  One token a sequence, a few or thousands: any mixture.  Rows of no sequence are left as
-    they are (`out`, or uninitialised); a token that sees nothing has zeros; one that sees a position without a page,
-    a latent that is not finite or a key that is NaN, NaN.  An infinite key gives NaN, or no weight where the score is -inf; if all are,
-    NaN.  Scores and sums are float32; in bf16
-    (rank 256, rope 64, pages of 8 tokens or more) products take bf16 operands, and where sequences have 96 new tokens or
-    more on the average, and nope and v_dim are 64, fp16 ones: there a query or a key of 2^20 and more, or a value of 2^18,
-    counts as infinite.  `out`: a contiguous tensor for the result, apart from the inputs."""
+    softmax(scale q k) v over them (scale positive, at most 1e35), with k = [weight's nope rows of the head times the latent | the
+    cached key] and v its v_dim rows times the latent.  One token a sequence, a few or thousands: any mixture, though a batch
+    takes one form, and long chunks beside single tokens are faster in two calls.  Rows of no sequence are left as they are
+    (`out`, or uninitialised); a token that sees nothing has zeros; one that sees a position without a page, a latent that is not
+    finite or a key that is NaN, NaN.  An infinite key gives NaN, or no weight where the score is -inf; if all are, NaN.
+
+    Scores and sums are float32; in bf16 (rank 256, rope 64, pages of 8 tokens or more) products take bf16 operands, and where
+    sequences have 96 new tokens or more on the average, and nope and v_dim are 64, fp16 ones: there a query or a key of 2^20 and
+    more, or a value of 2^18, counts as infinite, and steps are no finer than 2^-20 of a query or key and 2^-22 of a value, fewer
+    bits than bf16's below 2^-13 and 2^-15.  `out`: a contiguous tensor for the result, apart from the inputs."""
     _check("paged_attention", q, weight, pool, table, lens, starts, rates, *(() if out is None else (out,)))
     if q.dim() != 3 or weight.dim() != 2 or pool.dim() != 3:
         raise RuntimeError(f"paged_attention: q, weight and pool must have 3, 2 and 3 dims, got {tuple(q.shape)}, {tuple(weight.shape)} and "

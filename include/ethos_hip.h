@@ -624,11 +624,12 @@ int ethos_latent_append(const void* rows, int64_t ld, const void* gain, const fl
  *   out  [n_rows, n_heads, v_dim] dtype T: softmax(scale q k) v
  * Scores, maxima and sums are float32, products of bf16 tensors of bf16 operands, or of float32 ones where widths are others
  * than rank 256 and rope 64; with 96 new tokens or more a sequence on the average, and nope = v_dim = 64, of fp16 ones: a query
- * or key of 2^20 and more, or a value of 2^18, then counts as infinite.  A token that sees no position has a row of zeros; one that sees
- * a position without a page, a latent that is not finite or a key that is NaN has NaN, as have all tokens of a sequence whose
- * length is negative, over 2^30 or beyond its table, or whose rows are not in the batch.  An infinity in a cached key alone
- * gives NaN, or no weight to its position where the score is -inf (scores times `scale` under -2^125 count as -inf); a token
- * all of whose scores are -inf has NaN.
+ * or key of 2^20 and more, or a value of 2^18, then counts as infinite, and steps are no finer than 2^-20 of a query or key
+ * and 2^-22 of a value, fewer bits than bf16's below 2^-13 and 2^-15.
+ * A token that sees no position has a row of zeros; one that sees a position without a page, a latent that is not finite or a
+ * key that is NaN has NaN, as have all tokens of a sequence whose length is negative, over 2^30 or beyond its table, or whose
+ * rows are not in the batch.  An infinity in a cached key alone gives NaN, or no weight to its position where the score is -inf
+ * (scores times `scale` under -2^125 count as -inf); a token all of whose scores are -inf has NaN.
  *   workspace  >= ethos_paged_attention_workspace_bytes(...) bytes (scratch)
  * q, w, pool, workspace and out 16-byte aligned; scale positive, at most 1e35; n_rows n_heads <= 2^27 - 2048.
  */
