@@ -29,6 +29,8 @@ namespace {
 constexpr int kKeys = 64;          // keys of a tile of work
 constexpr float kLog2E = 1.44269504f;
 constexpr float kLowest = -0x1p126f;  // a running maximum's start: finite, so that masked scores weigh nothing
+// Running maxima are of scores as they are, which a weight's exponent takes off before the scale: s scale2 - RN(max scale2) is
+// the rounding of max scale2 at the maximum, 2^6 for scores of 2^29 and more than any exponent soon after.
 constexpr int32_t kLongest = 1 << 30;  // a sequence's length, at most
 
 // A tile of rows: `rows` of sequence seq from its row `row0` (token row0 / H, head row0 % H) on; the first new
@@ -380,11 +382,11 @@ __global__ __launch_bounds__(256, RB > 4 ? 1 : 2) void any_attend_kernel(const T
                 top = fmaxf(top, x[e]);
             }
             top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64)) * s.scale2;
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
             if (ballot(top > shift) != 0) {  // some row has a new maximum
                 const float before = shift;
                 shift = fmaxf(shift, top);
-                const float r = exp2f(before - shift);
+                const float r = exp2f((before - shift) * s.scale2);
                 l *= r;
 #pragma unroll
                 for (int i = 0; i < RB; ++i)
@@ -393,7 +395,7 @@ __global__ __launch_bounds__(256, RB > 4 ? 1 : 2) void any_attend_kernel(const T
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p = exp2f(__builtin_fmaf(x[e], s.scale2, -shift));
+                const float p = exp2f((x[e] - shift) * s.scale2);
                 l += p;
                 const uint64_t at = (uint64_t)(uintptr_t)row;
                 const uint32_t lo = __shfl((int)(uint32_t)at, 4 * g + e, 64), hi = __shfl((int)(uint32_t)(at >> 32), 4 * g + e, 64);
@@ -415,8 +417,8 @@ __global__ __launch_bounds__(256, RB > 4 ? 1 : 2) void any_attend_kernel(const T
 #pragma unroll
         for (int i = 1; i < 4; ++i) all = fmaxf(all, tops[i][m]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += ls[i][m] * exp2f(tops[i][m] - all);
-        const float f = exp2f(shift - all);
+        for (int i = 0; i < 4; ++i) sum += ls[i][m] * exp2f((tops[i][m] - all) * s.scale2);
+        const float f = exp2f((shift - all) * s.scale2);
         const int64_t slot = ((int64_t)blockIdx.x + item) * kAnyRows;
         if (wave == 0 && g == 0 && m < it.rows) stats[slot + m] = make_float2(all, sum);
         const int r = tid >> 4, c = (tid & 15) * 4;
@@ -499,14 +501,14 @@ __global__ __launch_bounds__(256) void any_finish_kernel(const T* __restrict__ w
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) next = fmaxf(next, ml[j].x);
-            const float r = exp2f(top - next);
+            const float r = exp2f((top - next) * s.scale2);
             top = next;
             l *= r;
             v *= r;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (k + j * groups >= p.n) break;
-                const float f = exp2f(ml[j].x - top);
+                const float f = exp2f((ml[j].x - top) * s.scale2);
                 l = __builtin_fmaf(ml[j].y, f, l);
                 v += x[j] * f;
             }
@@ -520,7 +522,7 @@ __global__ __launch_bounds__(256) void any_finish_kernel(const T* __restrict__ w
         for (int k = 1; k < groups; ++k) all = fmaxf(all, tops[k]);
         f32x4_t v = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int k = 0; k < groups; ++k) {
-            const float f = exp2f(tops[k] - all);
+            const float f = exp2f((tops[k] - all) * s.scale2);
             l += ls[k] * f;
             v += *reinterpret_cast<const f32x4_t*>(part + k * s.rank + tid * 4) * f;
         }
@@ -876,7 +878,7 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
         f32x4_t o[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        float shift = kLowest, l = 0.0f;  // the running maximum of the scores times scale2, and the lane's part of the sum
+        float shift = kLowest, l = 0.0f;  // the running maximum of the scores, and the lane's part of the sum
         int stage = 0;
         for (int k = k_begin; k < k_end; ++k) {
             if (S == 3 && k + 1 < k_end) copies_barrier<(S - 2) * NC>();
@@ -945,11 +947,11 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top = fmaxf(top, x[i][e]);
             top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64)) * s.scale2;
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
             if (ballot(top > shift) != 0) {  // some row has a new maximum
                 const float before = shift;
                 shift = fmaxf(shift, top);
-                const float r = __builtin_amdgcn_exp2f(before - shift);
+                const float r = __builtin_amdgcn_exp2f((before - shift) * s.scale2);
                 l *= r;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[i] *= r;
@@ -959,7 +961,7 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
             for (int i = 0; i < KB; ++i) {
                 float e[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], s.scale2, -shift));
+                for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f((x[i][j] - shift) * s.scale2);
                 l += (e[0] + e[1]) + (e[2] + e[3]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) split_bf16x2(e[2 * j], e[2 * j + 1], p[i / 2].w[(i & 1) * 2 + j], rest[i / 2].w[(i & 1) * 2 + j]);
@@ -1001,7 +1003,7 @@ __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t*
             if (wk == 0) {
                 const float other = *(lds_f_ptr)(size_t)(mine + 64 * 256), l2 = *(lds_f_ptr)(size_t)(mine + 65 * 256);
                 const float both = fmaxf(shift, other);
-                const float f = __builtin_amdgcn_exp2f(shift - both), f2 = __builtin_amdgcn_exp2f(other - both);
+                const float f = __builtin_amdgcn_exp2f((shift - both) * s.scale2), f2 = __builtin_amdgcn_exp2f((other - both) * s.scale2);
                 shift = both;
                 l = l * f + l2 * f2;
 #pragma unroll
@@ -1062,7 +1064,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) next = fmaxf(next, ml[j].x);
-        const float r = __builtin_amdgcn_exp2f(top - next);
+        const float r = __builtin_amdgcn_exp2f((top - next) * s.scale2);
         top = next;
         l *= r;
 #pragma unroll
@@ -1070,7 +1072,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (k + j * G >= p.n) break;
-            const float f = __builtin_amdgcn_exp2f(ml[j].x - top);
+            const float f = __builtin_amdgcn_exp2f((ml[j].x - top) * s.scale2);
             l = __builtin_fmaf(ml[j].y, f, l);
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = __builtin_fmaf(x[j][e >> 2][e & 3], f, v[e]);
@@ -1088,7 +1090,7 @@ __global__ __launch_bounds__(256) void finish_kernel(const uint16_t* __restrict_
         for (int g = 1; g < G; ++g) all = fmaxf(all, tops[mine + g]);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            f[g] = __builtin_amdgcn_exp2f(tops[mine + g] - all);
+            f[g] = __builtin_amdgcn_exp2f((tops[mine + g] - all) * s.scale2);
             sum += ls[mine + g] * f[g];
         }
         const float inv = inverse(sum, p.blind);
@@ -1569,11 +1571,11 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
             lds_barrier();
         };
         auto new_top = [&](float top) {
-            top = halves_max(top) * s.scale2 - kTop;
-            if (ballot(top > shift + kSlack) != 0) {  // some token's maximum has grown
+            top = halves_max(top);
+            if (ballot((top - shift) * s.scale2 > kSlack) != 0) {  // some token's maximum has grown
                 const float was = shift;
                 shift = fmaxf(shift, top);
-                const float r = __builtin_amdgcn_exp2f(was - shift);
+                const float r = __builtin_amdgcn_exp2f((was - shift) * s.scale2);
                 l *= r;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -1630,7 +1632,7 @@ __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __
                 if (st == 0) __builtin_amdgcn_s_setprio(1);  // (before a wave that is at its second part: 93.6 us against 96.5)
                 float e[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[st >> 2][4 * (st & 3) + i], s.scale2, -shift));
+                for (int i = 0; i < 4; ++i) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[st >> 2][4 * (st & 3) + i] - shift, s.scale2, kTop));
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const uint32_t w = pack_f16x2(e[2 * i], e[2 * i + 1]);
@@ -1740,7 +1742,8 @@ __global__ __launch_bounds__(256) void chunk_finish_kernel(int64_t n_rows, Shape
         const int64_t at = (p.slot + k) * kChunkTok + in;
         const float2 ml = stats[at];
         const f32x4_t x = *reinterpret_cast<const f32x4_t*>(sums + at * kHead + col);
-        const float next = fmaxf(top, ml.x), f = __builtin_amdgcn_exp2f(top - next), f2 = __builtin_amdgcn_exp2f(ml.x - next);
+        const float next = fmaxf(top, ml.x);
+        const float f = __builtin_amdgcn_exp2f((top - next) * s.scale2), f2 = __builtin_amdgcn_exp2f((ml.x - next) * s.scale2);
         top = next;
         l = l * f + ml.y * f2;
         v = v * f + x * f2;

@@ -629,7 +629,7 @@ int ethos_latent_append(const void* rows, int64_t ld, const void* gain, const fl
  * A token that sees no position has a row of zeros; one that sees a position without a page, a latent that is not finite or a
  * key that is NaN has NaN, as have all tokens of a sequence whose length is negative, over 2^30 or beyond its table, or whose
  * rows are not in the batch.  An infinity in a cached key alone gives NaN, or no weight to its position where the score is -inf
- * (scores times `scale` under -2^125 count as -inf); a token all of whose scores are -inf has NaN.
+ * (scores under -2^126, before `scale`, count as -inf); a token all of whose scores are -inf has NaN.
  *   workspace  >= ethos_paged_attention_workspace_bytes(...) bytes (scratch)
  * q, w, pool, workspace and out 16-byte aligned; scale positive, at most 1e35; n_rows n_heads <= 2^27 - 2048.
  */

@@ -512,6 +512,41 @@ def test_attention_over_infinite_rotary_keys(dt, rank, new, sign):
     assert torch.equal(got[new:], good[new:]) and bool(got[:new].isnan().all())
 
 
+@pytest.mark.parametrize("dt,rank,new", [("bf16", 256, 2), ("bf16", 256, 130), ("bf16", 64, 2), ("fp32", 64, 40)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attention_under_scores_far_from_zero(dt, rank, new, sign):
+    """Scores of up to 2^20 to 2^100 (2^36 with many new tokens, whose keys have a range) at one position, at half of that or less,
+    or twice as far below zero, at the others: the value at that position.  In the rotary columns alone, which rates of zero leave."""
+    lens, at = [333, 170], [210, 5]
+    for exponent in (10, 20, 24, 26, 27, 28, 29, 30, 31, 32, 33, 36, 50, 100)[:12 if new > 96 else None]:
+        c = _case(lens, [new, new], 4, rank, 64, 64, 64, 16, dt, seed=exponent)
+        c["rates"] = torch.zeros_like(c["rates"])
+        g = _gen(exponent)
+        # a query of `size` times a number in (1, 1.9) a row, along a key of as much, 64 columns: no power of two anywhere
+        size = math.sqrt(2.0 ** exponent / 64 / c["scale"])
+        u = 1.0 + 0.2 * torch.rand(64, generator=g, device="cuda")
+        far = 1.0 + 0.9 * torch.rand(2 * new, 4, 1, generator=g, device="cuda")
+        c["q"] = torch.cat((torch.zeros(2 * new, 4, 64, device="cuda"), far * size * u), -1).to(DT[dt])
+        flat = c["pool"].view(-1, rank + 64)
+        want = []
+        for i in range(2):
+            slots = _slots(c["table"], i, torch.arange(lens[i], device="cuda"), 16)
+            part = torch.rand(lens[i], 1, generator=g, device="cuda") * 0.5 if sign > 0 else -2.0 - torch.rand(lens[i], 1, generator=g, device="cuda")
+            part[at[i]] = sign
+            flat[slots, rank:] = (part * size * u).to(DT[dt])
+            row = flat[slots[at[i]], :rank].double()
+            w = c["w"].double().view(4, 128, rank)[:, 64:]
+            for pos in range(lens[i] - new, lens[i]):
+                want.append(((w @ row).reshape(-1), (w.abs() @ row.abs()).reshape(-1)) if pos >= at[i] else None)
+        got = _attend(c)
+        assert bool(got.isfinite().all()), exponent
+        for k, x in enumerate(want):
+            if x is not None:
+                # the row's rounding as an operand and the result's, and those of its parts' join
+                _within(got[k], x[0], x[1] * (2 * (half_step(DT[dt]) if dt == "bf16" else 0.0) + (rank + 64) * U) + half_step(DT[dt]) * x[0].abs() * 1.01,
+                        f"2^{exponent}, row {k}")
+
+
 @pytest.mark.parametrize("dt,rank,new", [("bf16", 256, 3), ("bf16", 256, 150), ("fp32", 64, 3)])
 def test_attention_under_the_largest_and_smallest_scales(dt, rank, new):
     """Scores of zero at 1e35, and a scale that leaves no differences: the mean of the values that a token sees."""
