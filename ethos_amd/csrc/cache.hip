@@ -11,8 +11,8 @@ namespace {
 
 // One wave a row, from row0 of the batch on: the latent times 1 / sqrt(mean of its squares + eps) and the gain, the key's halves
 // [a, b] -> [a cos - b sin, b cos + a sin]; both in float32, rounded once.  One pass: a piece of
-// 16 bytes of the latent a lane in registers, and half a wave's lanes a pair of the key each.  8,192 rows of 640 bytes: 7.4 us,
-// 1.4 TB/s; 64 rows 4.3: bound by the search for a row's sequence, its page and the angle, one after the other, not by memory.
+// 16 bytes of the latent a lane in registers, and half a wave's lanes a pair of the key each.  8,192 rows of 640 bytes: 7.4 to 7.9
+// us, 1.4 TB/s; 64 rows 4.3: bound by the search for a row's sequence, its page and the angle, one after the other, not by memory.
 template <typename T, int CH>
 __global__ __launch_bounds__(256) void append_kernel(const T* __restrict__ rows, int64_t ld, const T* __restrict__ gain,
                                                      const float* __restrict__ rates, Batch b, int64_t row0, int rank, int rope,
@@ -72,7 +72,7 @@ struct PagePairs {
 };
 
 // Block y of the grid copies block y of the pool; the pieces of its pages go round the workgroups.  64 pages of 40 KB in 12
-// blocks: 63 MB read and written in 10.8 us, 5.8 TB/s; 300 in 6: 147 MB in 24.0, 6.1 TB/s (from caches that hold a part).
+// blocks: 63 MB read and written in 10.6 us, 5.9 TB/s; 300 in 6: 147 MB in 24.1, 6.1 TB/s (from caches that hold a part).
 template <typename V>
 __global__ __launch_bounds__(256) void copy_pages_kernel(unsigned char* pool, int64_t block_bytes, int64_t page_bytes, int n_pairs,
                                                          int parts, PagePairs pairs) {

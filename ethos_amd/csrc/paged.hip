@@ -768,9 +768,9 @@ __global__ __launch_bounds__(256) void prepare_kernel(const uint16_t* __restrict
 }
 
 // WR KW waves: WR share a tile of 16 WR rows, 16 each, KW the 64 keys of a step.  S stages of LDS.  64 sequences of one token and up
-// to 8,192 keys: 186 MB in 36.5 us, 5.1 TB/s (256 of 2,048: 335 MB in 62, 5.4), where plain streaming reads reach 5.6, with eight
+// to 8,192 keys: 186 MB in 36.3 us, 5.1 TB/s (256 of 2,048: 335 MB in 62, 5.4), where plain streaming reads reach 5.6, with eight
 // loads of a thread in flight 6.3, and a large copy moves 4.95: near memory's rate.  16 of five tokens and up to 4,096: 23 MB of
-// cache in 24.6 us, three steps a workgroup.  LDS reads (a fragment serves 16 rows) account for some 4 us of that and the products
+// cache in 24.9 us, three steps a workgroup.  LDS reads (a fragment serves 16 rows) account for some 4 us of that and the products
 // for 5 at most; reading the queries and writing 16 MB of sums lie around the steps; the rest has not been told apart.
 template <int WR, int KW, int S>
 __global__ __launch_bounds__(WR * KW * 64, 2) void attend_kernel(const uint16_t* __restrict__ pool, Batch b, Shape s, const Plan* plan,
@@ -1430,8 +1430,8 @@ __device__ __forceinline__ void copy16_at(const void* base, uint32_t off, uint32
 }
 
 // A tile's steps for a share of its keys, two workgroups a CU; a wave 32 tokens of its own, S^T = K Q^T and O^T = V^T P^T in
-// 32 x 32 x 16 products, as in attend_kernel.  2,048 tokens over 7,001 keys, 16 heads: 75 GFLOP in 98 us (96.2 at the least),
-// 760 TFLOP/s, where large bf16 products reach 1,127 to 1,405 by the card.  Bound by a step's matrix and vector instructions, which overlap in part: 32 exponentials,
+// 32 x 32 x 16 products, as in attend_kernel.  2,048 tokens over 7,001 keys, 16 heads: 75 GFLOP in 99 to 104 us by the
+// card (97 at the least), 720 to 760 TFLOP/s, where large bf16 products reach 1,127 to 1,405.  Bound by a step's matrix and vector instructions, which overlap in part: 32 exponentials,
 // their sum, rounding and maximum a lane beside 24 products.
 __global__ __launch_bounds__(256, 2) void chunk_attend_kernel(const uint16_t* __restrict__ q, const float2* __restrict__ turns,
                                                               const uint16_t* __restrict__ keys, const uint16_t* __restrict__ shared, Shape s,
