@@ -266,9 +266,9 @@ class CompressedMoEModel(nn.Module):
     def extend(self, input_ids: torch.Tensor, cache: serving.LatentCache, seqs, counts=None, last_only: bool = False) -> torch.Tensor:
         """Logits of the next tokens of sequences in a cache, which they are added to: a prompt or a chunk of one, a token, a
         few, or any mixture (long chunks and single tokens are faster in a call each).  input_ids [n] int64, counts[i] tokens of
-        sequence seqs[i] after each other, or [batch, m], m of each.  Returns [n, vocab] (or [batch, m, vocab]); with `last_only` those of each sequence's last token
-        [batch, vocab] alone.  The model must be in eval mode.  An id outside the vocabulary has NaN for its logits and
-        counts as the nearest one inside for what follows it.
+        sequence seqs[i] after each other, or [batch, m], m of each.  Returns [n, vocab] (or [batch, m, vocab]); with
+        `last_only` those of each sequence's last token [batch, vocab] alone.  The model must be in eval mode.  An id outside the
+        vocabulary has NaN for its logits and counts as the nearest one inside for what follows it.
         (`forward` computes the same function of whole sequences, with other rounding points.  A graph cannot capture it.)"""
         if self.training:
             raise RuntimeError("extend needs the model in eval mode")
